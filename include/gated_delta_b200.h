@@ -254,6 +254,44 @@ int gd_conv_bwd(const void* x, const void* w, const void* dq, const void* dk, co
                 int dtype, int wdtype, int B, int T, int C, int KD, int DK, int REP, int DV, void* workspace,
                 size_t workspace_bytes, void* stream);
 
+/* ---- the residual addition with its RMS norm (the step that opens every layer of the decoder) ----
+ * s = (x + res) rounded to `dtype`, y = s rsqrt(mean(s^2) + eps) w' in `dtype` (fp32 math on the rounded s, one
+ * rounding), w' = w, or 1 + w when zero_centered; over `rows` rows of width D. res NULL: s is x itself and the s pointer
+ * is not used. x, res, s, y: [rows, D] in `dtype`; w: [D] in `dtype` or GD_FLOAT32. A row takes at most 2,048 chunks of
+ * 16 bytes: D <= 16,384 at 16 bits, 8,192 at fp32 (two chunks less where D is not a multiple of the chunk). Every
+ * pointer 16-byte aligned. No allocation, asynchronous on `stream`. */
+int gd_rnorm_fwd(const void* x, const void* res, const void* w, void* s, void* y, int dtype, int wdtype,
+                 int zero_centered, long long rows, int D, float eps, void* stream);
+
+/* The same with y in 8 bits: q [rows, D] e4m3 and scale [rows, ceil(D / group)] fp32, y = q scale. Each `group`
+ * channels (a multiple of 8; 0: the whole row) share scale = max |y| / 448, or 1 where they are all zero. */
+int gd_rnorm_fp8(const void* x, const void* res, const void* w, void* s, void* q, float* scale, int dtype, int wdtype,
+                 int zero_centered, long long rows, int D, int group, float eps, void* stream);
+
+/* Bytes of workspace gd_rnorm_bwd needs when it forms dw (0 for invalid sizes). */
+size_t gd_rnorm_workspace_bytes(long long rows, int D);
+
+/* dx [rows, D] in `dtype`, the gradient of x and of res, from s (x without a residual), dy and ds (either NULL = a zero
+ * cotangent): h = dy w', dx = ds + r (h - xh mean(h xh)), xh = s r. dw [D] = the sum over rows of dy xh in `wdtype`,
+ * when not NULL (then `workspace` holds gd_rnorm_workspace_bytes(rows, D)); the sum is taken in a fixed order (no
+ * atomics: the same bits every run). */
+int gd_rnorm_bwd(const void* s, const void* w, const void* dy, const void* ds, void* dx, void* dw, int dtype, int wdtype,
+                 int zero_centered, long long rows, int D, float eps, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* ---- rotary positions ----
+ * q [B, T, H, D] and k [B, T, HK, D] (HK = 0: none) in `dtype`, read through their batch, token and head strides (in
+ * elements; a head's channels adjacent), written contiguously to oq and ok: channels [0, R) turned in pairs, (i, i + R/2)
+ * or (2 i, 2 i + 1) when interleaved, by the angles whose cos and sin table [table_rows, R/2, 2] (fp32) holds for the
+ * token's position, the others copied. inverse: by the opposite angles (the backward). positions: int32 or int64
+ * (positions64), of token (b, t) at b pos_stride_b + t; NULL: t. A position outside the table is clamped to it. Pointers
+ * aligned to their element (the table to 8 bytes); 16-byte accesses where widths, strides and addresses allow. No
+ * allocation, asynchronous on `stream`. */
+int gd_rotary(const void* q, const void* k, void* oq, void* ok, const float* table, const void* positions,
+              int positions64, long long pos_stride_b, long long table_rows, int dtype, int B, int T, int H, int HK,
+              int D, int R, long long q_stride_b, long long q_stride_t, long long q_stride_h, long long k_stride_b,
+              long long k_stride_t, long long k_stride_h, int interleaved, int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

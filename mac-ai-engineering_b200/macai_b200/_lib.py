@@ -30,11 +30,13 @@ EXPORTS = ("gd_status_string", "gd_workspace_bytes", "gd_prep", "gd_fwd_state", 
            "gd_forward", "gd_backward", "gd_read_error", "gd_forward_noalloc", "gd_gates_fwd",
            "gd_gates_workspace_bytes", "gd_gates_bwd", "gd_gnorm_fwd", "gd_gnorm_workspace_bytes", "gd_gnorm_bwd",
            "gd_conv_fwd", "gd_conv_workspace_bytes", "gd_conv_bwd", "gd_workspace_bytes_packed", "gd_forward_packed",
-           "gd_backward_packed")
+           "gd_backward_packed", "gd_rnorm_fwd", "gd_rnorm_fp8", "gd_rnorm_workspace_bytes", "gd_rnorm_bwd",
+           "gd_rotary")
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
 _DIMS = [_I] * 7 + [_I]          # dtype?, B, T, H, HK, DK, DV, flags (see each signature)
 _SIGS = {
     "gd_status_string": ([_I], ctypes.c_char_p),
@@ -59,6 +61,11 @@ _SIGS = {
     "gd_workspace_bytes_packed": ([_I] * 7, _SZ),
     "gd_forward_packed": ([_P] * 9 + [_I] * 8 + [_P, _SZ, _P], _I),
     "gd_backward_packed": ([_P] * 15 + [_I] * 8 + [_P, _SZ, _P], _I),
+    "gd_rnorm_fwd": ([_P] * 5 + [_I, _I, _I, _LL, _I, ctypes.c_float, _P], _I),
+    "gd_rnorm_fp8": ([_P] * 6 + [_I, _I, _I, _LL, _I, _I, ctypes.c_float, _P], _I),
+    "gd_rnorm_workspace_bytes": ([_LL, _I], _SZ),
+    "gd_rnorm_bwd": ([_P] * 6 + [_I, _I, _I, _LL, _I, ctypes.c_float, _P, _SZ, _P], _I),
+    "gd_rotary": ([_P] * 6 + [_I, _LL, _LL] + [_I] * 7 + [_LL] * 6 + [_I, _I, _P], _I),
 }
 
 _lib = None
