@@ -258,7 +258,7 @@ int gd_conv_bwd(const void* x, const void* w, const void* dq, const void* dk, co
  * s = (x + res) rounded to `dtype`, y = s rsqrt(mean(s^2) + eps) w' in `dtype` (fp32 math on the rounded s, one
  * rounding), w' = w, or 1 + w when zero_centered; over `rows` rows of width D. res NULL: s is x itself and the s pointer
  * is not used. x, res, s, y: [rows, D] in `dtype`; w: [D] in `dtype` or GD_FLOAT32. A row takes at most 2,048 chunks of
- * 16 bytes: D <= 16,384 at 16 bits, 8,192 at fp32 (two chunks less where D is not a multiple of the chunk). Every
+ * 16 bytes: D <= 16,384 at 16 bits, 8,192 at fp32 (16,375 and 8,187 where D is not a multiple of the chunk). Every
  * pointer 16-byte aligned. No allocation, asynchronous on `stream`. */
 int gd_rnorm_fwd(const void* x, const void* res, const void* w, void* s, void* y, int dtype, int wdtype,
                  int zero_centered, long long rows, int D, float eps, void* stream);

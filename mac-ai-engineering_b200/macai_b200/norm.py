@@ -24,8 +24,8 @@ MAX_CHUNKS = 2048  # 16-byte chunks of a row (a width that fills no whole number
 
 def supported(x, residual, weight) -> bool:
     """The cases the kernels take: x [..., D] (and the residual, of its shape and dtype) in float32, float16 or
-    bfloat16; weight [D] in x's dtype or float32; CUDA tensors; D up to 16,384 at 16 bits (16,368 where it is not a
-    multiple of 8) and 8,192 at float32 (8,184 where it is not a multiple of 4)."""
+    bfloat16; weight [D] in x's dtype or float32; CUDA tensors; D up to 16,384 at 16 bits (16,375 where it is not a
+    multiple of 8) and 8,192 at float32 (8,187 where it is not a multiple of 4)."""
     ts = (x, weight) if residual is None else (x, residual, weight)
     if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in ts) or x.dim() == 0 or x.dtype not in _DTYPES:
         return False

@@ -13,7 +13,7 @@ def test_rnorm_refusals():
     f = lambda x=ONE, w=ONE, s=ONE, y=ONE, dt=BF, wt=BF, rows=10, D=128: lib.gd_rnorm_fwd(  # noqa: E731
         x, ONE, w, s, y, dt, wt, 0, rows, D, 1e-6, NUL)
     assert f(dt=7) == _lib.GD_ERR_ARG and f(wt=F16) == _lib.GD_ERR_ARG
-    for D in (0, -1, 16385, 16369):
+    for D in (0, -1, 16385, 16377):
         assert f(D=D) == _lib.GD_ERR_SHAPE
     assert f(dt=F32, wt=F32, D=8196) == _lib.GD_ERR_SHAPE and f(rows=-1) == _lib.GD_ERR_SHAPE
     assert f(x=NUL) == _lib.GD_ERR_ARG and f(s=NUL) == _lib.GD_ERR_ARG and f(w=NUL) == _lib.GD_ERR_ARG
