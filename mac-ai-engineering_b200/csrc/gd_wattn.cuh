@@ -1,0 +1,287 @@
+// Shared parts of the softmax-attention kernels (causal, sliding window, first tokens that stay visible): the tile ranges,
+// packed rows, the swizzled tiles that TMA writes and tcgen05 reads, TMEM operands.
+//
+// A tile is 128 rows (tokens of one head) by NS slabs of 64 channels; a slab is 128 rows of 128 bytes in the 128-byte
+// swizzle (TMA box 64 x 1 x 128 x 1), 16 KB. The same bytes are a K-major operand (rows = M or N, channels = K) and an
+// MN-major one (rows = K, channels = M or N): only the descriptor differs. Channels past D and tokens past T read as
+// zeros (TMA's fill), so head widths up to NS * 64 and ragged lengths need no copies.
+#pragma once
+
+#include "gd_common.cuh"
+
+namespace gd {
+namespace wattn {
+
+constexpr int kTile = 128;
+constexpr int kSlabBytes = kTile * 128;
+constexpr int kNoWindow = 0x3fffffff;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Problem {
+  int B, Tq, Tk, H, HK;    // packed rows: B = 1, Tq = Tk = all rows
+  int D;
+  int window, sinks;       // key j is visible to position p: j <= p and (j > p - window or j < sinks)
+  float scale, scale_log2;  // scale, and scale * log2(e)
+  const int* cu;           // packed rows' boundaries [N + 1], or NULL
+  int N;
+};
+
+// One row of the batch or one packed sequence: the rows it covers, and its queries' first position.
+struct Seq {
+  int b, q0, Tq, k0, Tk;
+  __device__ __forceinline__ int offset() const { return Tk - Tq; }  // query i stands at position i + offset
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+
+// The packed sequence that owns work item `item`, when a sequence of n rows has count(n) items; returns its index within
+// the sequence, or -1 past the last. One whole warp; boundaries are clamped into [0, rows], so no input leaves the arrays.
+template <typename Count>
+__device__ __forceinline__ int find_item(const int* cu, int N, int rows, int item, Count count, Seq& s) {
+  constexpr int kPer = 8;
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int base = 0; base < N; base += 32 * kPer) {
+    int first[kPer], len[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int n = base + lane * kPer + i;
+      first[i] = n < N ? clampi(__ldg(cu + n), 0, rows) : 0;
+      len[i] = n < N ? clampi(__ldg(cu + n + 1), first[i], rows) - first[i] : 0;
+      sum += count(len[i]);
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    if (item < before + total) {
+      int at = before + incl - sum, found = -1, f0 = 0, fl = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int c = count(len[i]);
+        if (found < 0 && item >= at && item < at + c) {
+          found = item - at;
+          f0 = first[i];
+          fl = len[i];
+        }
+        at += c;
+      }
+      const unsigned who = __ballot_sync(0xffffffffu, found >= 0);
+      const int src = __ffs(who) - 1;
+      s.b = 0;
+      s.q0 = s.k0 = __shfl_sync(0xffffffffu, f0, src);
+      s.Tq = s.Tk = __shfl_sync(0xffffffffu, fl, src);
+      return __shfl_sync(0xffffffffu, found, src);
+    }
+    before += total;
+  }
+  return -1;
+}
+
+// The key tiles that queries [i0, i1] (positions p0 .. p1) of a sequence see: the first `head` tiles, then tiles
+// lo .. lo + n - head - 1.
+struct KeyRange {
+  int n, head, lo;
+  __device__ __forceinline__ KeyRange(int p0, int p1, int window, int sinks) {
+    n = head = lo = 0;
+    if (p1 < 0) return;  // no position reached: no key visible
+    const int hi = p1 / kTile;
+    const int from = p0 - window + 1;
+    lo = from > 0 ? from / kTile : 0;
+    head = (sinks + kTile - 1) / kTile;
+    if (head > lo) head = lo;
+    n = head + hi - lo + 1;
+  }
+  __device__ __forceinline__ int key(int j) const { return (j < head ? j : lo + j - head) * kTile; }  // tile j's first key
+};
+
+// mbar_wait by a whole warp, with one answer for all its lanes (the aligned tcgen05 instructions that follow need that).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, ErrorWord* err, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, where));
+}
+
+// Does every query at positions p0 .. p1 see all keys c .. c + 127?
+__device__ __forceinline__ bool all_visible(int c, int p0, int p1, int window, int sinks) {
+  return c + kTile - 1 <= p0 && (c > p1 - window || c + kTile <= sinks);
+}
+
+// ---- host: [B, T, heads, D] rows read through strides (in elements) as boxes of 64 channels x `box_t` tokens of a head
+inline bool tile_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int B, int T, int heads, int D,
+                     long long sb, long long st, long long sh, int box_t) {
+  EncodeTiled enc = encode_tiled();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T, (cuuint64_t)B};
+  // a dimension of one entry has no stride of its own: any multiple of 16 bytes
+  const cuuint64_t strides[3] = {(cuuint64_t)(heads > 1 ? sh : D) * 2, (cuuint64_t)(T > 1 ? st : D) * 2,
+                                 (cuuint64_t)(B > 1 ? sb : D) * 2};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)box_t, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(m, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// all NS slabs of the tile at token t of head h, row b
+template <int NS>
+__device__ __forceinline__ void load_tile(uint32_t smem, const CUtensorMap* m, int h, int t, int b, uint64_t* bar) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem + s * kSlabBytes),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(64 * s), "r"(h), "r"(t), "r"(b), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// ---- tcgen05 operands in the 128-byte swizzle (layout type 2)
+// K-major: 8-row groups 1024 bytes apart; 16 channels further = 32 bytes
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major: 64-channel groups one slab apart, 8-row groups 1024 bytes apart; 16 rows further = 2048 bytes
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kSlabBytes >> 4) << 16) | (64ull << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc(int M, int N, bool b_mn) {
+  return (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// D (+)= A B with A in TMEM (128 lanes, 16-bit pairs in 32-bit columns)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+// D[128 x 128] = X Y^T, both tiles of NS slabs, contracted over their channels
+template <typename T, int NS>
+__device__ __forceinline__ void mma_xyt(uint32_t d, uint32_t x, uint32_t y, bool acc = false) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      mma_bf16(d, desc_k(x + s * kSlabBytes) + 2 * k, desc_k(y + s * kSlabBytes) + 2 * k, idesc<T>(128, 128, false),
+               acc || s > 0 || k > 0);
+}
+// D[128 x NS 64] (+)= P Y: P in TMEM (128 rows, 128 contracted columns as 64 words), Y's rows contracted. `gap`: words
+// between P's two halves of 64 contracted columns (32: adjacent)
+template <typename T, int NS>
+__device__ __forceinline__ void mma_py(uint32_t d, uint32_t p, uint32_t y, bool acc, int gap = 32) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    mma_ts(d, p + (k & 3) * 8 + (k >> 2) * gap, desc_mn(y) + 128 * k, idesc<T>(128, NS * 64, true), acc || k > 0);
+}
+
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// 128 consecutive fp32 columns of the thread's own lane, one wait.
+__device__ __forceinline__ void tmem_ld128(uint32_t a, float (&v)[128]) {
+  uint32_t r[128];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      :
+        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]),
+        "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]),
+        "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]),
+        "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]),
+        "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(a), "r"(a + 32), "r"(a + 64), "r"(a + 96)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 64 of them.
+__device__ __forceinline__ void tmem_ld64(uint32_t a, float (&v)[64]) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      :
+        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(a), "r"(a + 32)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// registers -> 16 consecutive words of the thread's own lane (asynchronous: tmem_st_wait).
+__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// 32 of them.
+__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// The entry points' parts (host): strides of q, k, v in elements, (batch, token, head) each
+int forward(const void* q, const void* k, const void* v, const long long* strides, const Problem& pr, int dtype, void* o,
+            float* lse, ErrorWord* err, cudaStream_t stream);
+
+}  // namespace wattn
+}  // namespace gd
