@@ -136,6 +136,17 @@ __device__ __forceinline__ void load_tile(uint32_t smem, const CUtensorMap* m, i
         : "memory");
 }
 
+// half x (128 channels, two slabs) of a 256-channel tile
+__device__ __forceinline__ void load_half(uint32_t smem, const CUtensorMap* m, int x, int h, int t, int b, uint64_t* bar) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem + s * kSlabBytes),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(64 * (2 * x + s)), "r"(h), "r"(t), "r"(b), "r"(smem_u32(bar))
+        : "memory");
+}
+
 // ---- tcgen05 operands in the 128-byte swizzle (layout type 2)
 // K-major: 8-row groups 1024 bytes apart; 16 channels further = 32 bytes
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
@@ -282,6 +293,10 @@ __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
 // The entry points' parts (host): strides of q, k, v in elements, (batch, token, head) each
 int forward(const void* q, const void* k, const void* v, const long long* strides, const Problem& pr, int dtype, void* o,
             float* lse, ErrorWord* err, cudaStream_t stream);
+// (and of dO: strides[9 .. 11]); the first `heavy` key tiles are cut into `parts` CTAs with fp32 partial tiles at `part`
+int backward(const void* q, const void* k, const void* v, const void* o, const void* g, const long long* strides,
+             const Problem& pr, int dtype, const float* lse, float* delta, void* dq, void* dk, void* dv, int heavy,
+             int parts, float* part, ErrorWord* err, cudaStream_t stream);
 
 }  // namespace wattn
 }  // namespace gd

@@ -1,0 +1,825 @@
+// Backward of the causal softmax attention with a sliding window and first tokens that stay visible. With P = softmax,
+// L the forward's log2-sum and delta = rowsum(dO O):
+//   P = exp2(scale log2(e) S - L),  dP = dO V^T,  dS = P (dP - delta)
+//   dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q       (dK, dV summed over the query heads of a key head)
+// Three kernels, none of which waits on another CTA and none with atomics on results (the same bits every run):
+//   delta_kernel  delta, and for float16 the largest |dO| (the scale below)
+//   dq_kernel     one CTA per 128 queries of a head, over the key tiles they see
+//   dkv_kernel    one CTA per 128 keys of a key head, over the group's query heads and the query tiles that see them
+// S and dP are formed twice (7 products of 128 x 128 x D a tile pair instead of 5): with the queries on the rows in the
+// first kernel and the keys on the rows in the second, so that every accumulator stays in TMEM for the whole loop and
+// dS, P are the A operands of the products that follow straight from TMEM; nothing is exchanged between CTAs.
+//
+// P and dS are rounded to the inputs' 16-bit type (the operand type of the matrix instruction); exponentials, sums and
+// accumulators are fp32. float16: dS is scaled by a power of two that brings the largest |dO| into [1, 2) before its
+// rounding, and dQ, dK are scaled back: gradients of any size keep float16's 11 bits.
+#include "gd_wattn.cuh"
+
+namespace gd {
+namespace wattn {
+namespace {
+
+constexpr int kWarpsEw = 8;                      // two threads a row, 64 columns each
+constexpr int kThreads = 32 * (kWarpsEw + 2);    // + loads, + products
+
+// the error word's first spare field holds the bits of the largest |dO| (float16)
+__device__ __forceinline__ float ds_scale(const ErrorWord* err) {
+  const float a = __int_as_float(*reinterpret_cast<const volatile int*>(&err->pad[0]));
+  if (!(a > 0.f) || a > 3e38f) return 1.f;
+  const int e = 127 - ((__float_as_int(a) >> 23) & 0xff);  // a 2^e in [1, 2); subnormal a: e = 127
+  return __int_as_float((127 + (e > 100 ? 100 : e)) << 23);
+}
+
+// ---- delta: 16 lanes a row of [B, Tq, H]
+template <typename T>
+__global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, const T* __restrict__ g, long long gb,
+                                                    long long gt, long long gh, float* __restrict__ delta, int B, int Tq,
+                                                    int H, int D, ErrorWord* err) {
+  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4, rows = (long long)B * Tq * H;
+  const int sub = threadIdx.x & 15;
+  float s = 0.f, top = 0.f;
+  int h = 0, t = 0;
+  long long b = 0;
+  if (row < rows) {
+    h = (int)(row % H);
+    const long long bt = row / H;
+    b = bt / Tq;
+    t = (int)(bt - b * Tq);
+    const T* po = o + row * D;
+    const T* pg = g + b * gb + t * gt + h * gh;
+    for (int c = sub * 8; c < D; c += 128) {
+      const uint4 a = *reinterpret_cast<const uint4*>(po + c), d = *reinterpret_cast<const uint4*>(pg + c);
+      const uint32_t ua[4] = {a.x, a.y, a.z, a.w}, ud[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 x, y;
+        if constexpr (std::is_same<T, __half>::value) {
+          x = __half22float2(*reinterpret_cast<const __half2*>(ua + i));
+          y = __half22float2(*reinterpret_cast<const __half2*>(ud + i));
+          top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+        } else {
+          x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(ua + i));
+          y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(ud + i));
+        }
+        s = fmaf(x.x, y.x, s);
+        s = fmaf(x.y, y.y, s);
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 8; w >= 1; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+  if (row < rows && sub == 0) delta[(b * H + h) * Tq + t] = s;
+  if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&err->pad[0], __float_as_int(top));  // a maximum: any order
+  }
+}
+
+// 32 fp32 columns of the accumulator times f -> row `out` (16-bit), channels c .. c + 31 below D
+template <typename T>
+__device__ __forceinline__ void store32(T* out, int c, int D, const float (&v)[32], float f) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    if (c + k >= D) break;
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = pack16<T>(v[k + 2 * e] * f, v[k + 2 * e + 1] * f);
+    *reinterpret_cast<uint4*>(out + c + k) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// dS of 64 columns: p (dp - delta) f, packed
+template <typename T>
+__device__ __forceinline__ uint32_t ds2(float p0, float p1, float d0, float d1, float e0, float e1, float f) {
+  if constexpr (std::is_same<T, __half>::value) return pack16<T>(p0 * ((d0 - e0) * f), p1 * ((d1 - e1) * f));
+  else return pack16<T>(p0 * (d0 - e0), p1 * (d1 - e1));
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// dQ. TMEM: S | dP | dQ | dS (NS = 4: dS over dP). The products of the next key tile run under the elementwise work of
+// this one as soon as its S and dP are in registers. Shared memory: Q, dO, a ring of key tiles (used twice: S, dQ) and
+// one of value tiles; NS = 4: one ring of half tiles (128 channels) in the order of their use, keys loaded twice.
+template <int NS>
+struct DqCfg {
+  static constexpr bool kHalves = NS == 4;
+  static constexpr int kUnit = (kHalves ? 2 : NS) * kSlabBytes;
+  static constexpr int kKs = kHalves ? 3 : NS == 1 ? 4 : 3, kVs = kHalves ? 0 : NS == 1 ? 4 : 2;
+  static constexpr int kDp = 128, kDq = 256, kDs = kHalves ? 128 : 256 + NS * 64;
+  static constexpr int kBarriers = 1 + 2 * (kKs + kVs) + 7;
+  static constexpr size_t kSmem = 1024 + 2 * NS * kSlabBytes + (size_t)kUnit * (kKs + kVs) + 8 * kBarriers + 64;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+template <typename T, int NS>
+__global__ void __launch_bounds__(kThreads, 1)
+    dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+              const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo, const Problem pr,
+              const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dq, ErrorWord* err) {
+  using C = DqCfg<NS>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + 2 * NS * kSlabBytes + C::kUnit * (C::kKs + C::kVs));
+  uint64_t* in_full = bars;  // Q and dO
+  uint64_t* full = bars + 1;  // key ring, then value ring
+  uint64_t* empty = full + C::kKs + C::kVs;
+  uint64_t* s_full = empty + C::kKs + C::kVs;
+  uint64_t* dp_full = s_full + 1;
+  uint64_t* s_read = s_full + 2;
+  uint64_t* dp_read = s_full + 3;
+  uint64_t* ds_full = s_full + 4;
+  uint64_t* dq_done = s_full + 5;
+  uint64_t* fin = s_full + 6;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
+  int* info = reinterpret_cast<int*>(tslot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(in_full, 1);
+    for (int i = 0; i < C::kKs + C::kVs; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(s_read, kWarpsEw);
+    mbar_init(dp_read, kWarpsEw);
+    mbar_init(ds_full, kWarpsEw);
+    mbar_init(dq_done, 1);
+    mbar_init(fin, 1);
+    fence_mbar_init();
+  }
+  if (warp == kWarpsEw + 1) {
+    tmem_alloc(tslot, 512);
+    tmem_relinquish();
+  }
+  const int item = gridDim.x - 1 - blockIdx.x, h = blockIdx.y;  // later tiles see more keys: first
+  Seq sq;
+  int tile = item;
+  if (pr.cu != nullptr && warp == 0) {
+    tile = find_item(pr.cu, pr.N, pr.Tq, item, [](int n) { return (n + kTile - 1) / kTile; }, sq);
+    if (lane == 0) {
+      info[0] = tile;
+      info[1] = sq.q0;
+      info[2] = sq.Tq;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (pr.cu != nullptr) {
+    tile = info[0];
+    sq.b = 0;
+    sq.q0 = sq.k0 = info[1];
+    sq.Tq = sq.Tk = info[2];
+  } else {
+    sq = {(int)blockIdx.z, 0, pr.Tq, 0, pr.Tk};
+  }
+  const uint32_t tm = *tslot;
+  const int i0 = tile * kTile;
+  const int i1 = i0 + kTile - 1 < sq.Tq - 1 ? i0 + kTile - 1 : sq.Tq - 1;
+  const int p0 = i0 + sq.offset(), p1 = i1 + sq.offset();
+  const KeyRange kr(tile < 0 ? -1 : p0, tile < 0 ? -1 : p1, pr.window, pr.sinks);
+  const uint32_t s_q = smem_u32(base), s_o = s_q + NS * kSlabBytes, s_k = s_o + NS * kSlabBytes,
+                 s_v = s_k + C::kKs * C::kUnit;
+
+  if (warp == kWarpsEw) {
+    if (lane == 0 && kr.n > 0) {
+      const int hk = h / (pr.H / pr.HK);
+      mbar_arrive_expect_tx(in_full, 2 * NS * kSlabBytes);
+      load_tile<NS>(s_q, &mq, h, sq.q0 + i0, sq.b, in_full);
+      load_tile<NS>(s_o, &mo, h, sq.q0 + i0, sq.b, in_full);
+      bool ok = true;
+      int nk = 0, nv = 0;  // units loaded into each ring
+      if constexpr (!C::kHalves) {
+        for (int j = 0; ok && j < kr.n; ++j) {
+          const int t = sq.k0 + kr.key(j);
+          const int a = nk % C::kKs, b = nv % C::kVs;
+          if (nk >= C::kKs && !(ok = mbar_wait(empty + a, (nk / C::kKs - 1) & 1, err, 80))) break;
+          mbar_arrive_expect_tx(full + a, C::kUnit);
+          load_tile<NS>(s_k + a * C::kUnit, &mk, hk, t, sq.b, full + a);
+          ++nk;
+          if (nv >= C::kVs && !(ok = mbar_wait(empty + C::kKs + b, (nv / C::kVs - 1) & 1, err, 81))) break;
+          mbar_arrive_expect_tx(full + C::kKs + b, C::kUnit);
+          load_tile<NS>(s_v + b * C::kUnit, &mv, hk, t, sq.b, full + C::kKs + b);
+          ++nv;
+        }
+      } else {
+        auto halves = [&](const CUtensorMap* m, int j) {  // the two halves of tile j
+#pragma unroll 1
+          for (int x = 0; ok && x < 2; ++x) {
+            const int a = nk % C::kKs;
+            if (nk >= C::kKs && !(ok = mbar_wait(empty + a, (nk / C::kKs - 1) & 1, err, 82))) return;
+            mbar_arrive_expect_tx(full + a, C::kUnit);
+            load_half(s_k + a * C::kUnit, m, x, hk, sq.k0 + kr.key(j), sq.b, full + a);
+            ++nk;
+          }
+        };
+        halves(&mk, 0);
+        if (ok) halves(&mv, 0);
+        for (int j = 0; ok && j < kr.n; ++j) {
+          if (j + 1 < kr.n) halves(&mk, j + 1);
+          if (ok) halves(&mk, j);
+          if (ok && j + 1 < kr.n) halves(&mv, j + 1);
+        }
+      }
+      mbar_wait(in_full, 0, err, 83);  // the copies in flight land before the CTA ends
+      for (int l = nk > C::kKs ? nk - C::kKs : 0; l < nk; ++l) mbar_wait(full + l % C::kKs, (l / C::kKs) & 1, err, 83);
+      if constexpr (C::kVs > 0)
+        for (int l = nv > C::kVs ? nv - C::kVs : 0; l < nv; ++l)
+          mbar_wait(full + C::kKs + l % C::kVs, (l / C::kVs) & 1, err, 83);
+    }
+  } else if (warp == kWarpsEw + 1) {
+    if (lane == 0 && kr.n > 0) {
+      bool ok = mbar_wait(in_full, 0, err, 84);
+      if constexpr (!C::kHalves) {
+        auto first = [&](int j) {  // S and dP of tile j
+          const int a = j % C::kKs, b = C::kKs + j % C::kVs;
+          if (!mbar_wait(full + a, (j / C::kKs) & 1, err, 85)) return false;
+          if (j > 0 && !mbar_wait(s_read, (j - 1) & 1, err, 86)) return false;
+          tc_fence_after();
+          mma_xyt<T, NS>(tm, s_q, s_k + a * C::kUnit);
+          mma_commit(s_full);
+          if (!mbar_wait(full + b, (j / C::kVs) & 1, err, 87)) return false;
+          if (j > 0 && !mbar_wait(dp_read, (j - 1) & 1, err, 88)) return false;
+          tc_fence_after();
+          mma_xyt<T, NS>(tm + C::kDp, s_o, s_v + (j % C::kVs) * C::kUnit);
+          mma_commit(dp_full);
+          mma_commit(empty + b);
+          return true;
+        };
+        ok = ok && first(0);
+        for (int j = 0; ok && j < kr.n; ++j) {
+          if (j + 1 < kr.n) ok = first(j + 1);
+          if (!(ok = ok && mbar_wait(ds_full, j & 1, err, 89))) break;
+          tc_fence_after();
+          mma_py<T, NS>(tm + C::kDq, tm + C::kDs, s_k + (j % C::kKs) * C::kUnit, j > 0);
+          mma_commit(empty + j % C::kKs);
+          mma_commit(dq_done);
+        }
+      } else {
+        int n = 0;  // units used
+        auto pair = [&](uint32_t d, uint32_t x) {  // D = X Y^T over the ring's next two halves
+          for (int y = 0; y < 2; ++y, ++n) {
+            const int a = n % C::kKs;
+            if (!mbar_wait(full + a, (n / C::kKs) & 1, err, 85)) return false;
+            tc_fence_after();
+            mma_xyt<T, 2>(d, x + y * 2 * kSlabBytes, s_k + a * C::kUnit, y > 0);
+            mma_commit(empty + a);
+          }
+          return true;
+        };
+        ok = ok && pair(tm, s_q);
+        if (ok) mma_commit(s_full);
+        ok = ok && pair(tm + C::kDp, s_o);
+        if (ok) mma_commit(dp_full);
+        for (int j = 0; ok && j < kr.n; ++j) {
+          if (j + 1 < kr.n) {
+            ok = mbar_wait(s_read, j & 1, err, 86) && pair(tm, s_q);
+            if (ok) mma_commit(s_full);
+          }
+          if (!(ok = ok && mbar_wait(ds_full, j & 1, err, 89))) break;
+          tc_fence_after();
+          for (int y = 0; ok && y < 2; ++y, ++n) {
+            const int a = n % C::kKs;
+            if (!(ok = mbar_wait(full + a, (n / C::kKs) & 1, err, 85))) break;
+            tc_fence_after();
+            mma_py<T, 2>(tm + C::kDq + y * 128, tm + C::kDs, s_k + a * C::kUnit, j > 0);
+            mma_commit(empty + a);
+          }
+          if (!ok) break;
+          mma_commit(dq_done);
+          if (j + 1 < kr.n) {  // dP over dS, once its products have read it
+            ok = mbar_wait(dq_done, j & 1, err, 88);
+            tc_fence_after();
+            ok = ok && pair(tm + C::kDp, s_o);
+            if (ok) mma_commit(dp_full);
+          }
+        }
+      }
+      mma_commit(fin);
+      mbar_wait(fin, 0, err, 90);
+    }
+  } else if (tile >= 0) {
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int i = i0 + row, p = p0 + row;
+    const bool live = i < sq.Tq;
+    const long long at = ((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i;
+    const float L = live ? lse[at] : INFINITY, de = live ? delta[at] : 0.f;
+    float f = 1.f;
+    if constexpr (std::is_same<T, __half>::value) f = ds_scale(err);
+    bool ok = true;
+    for (int j = 0; j < kr.n; ++j) {
+      const int c0 = kr.key(j) + half * 64;
+      const bool whole = all_visible(kr.key(j), p0, p1, pr.window, pr.sinks);
+      const int last = p - c0, from = p - pr.window + 1 - c0, sink = pr.sinks - c0;
+      float s[64], d[64];
+      if (!(ok = warp_wait(s_full, j & 1, err, 91))) break;
+      tc_fence_after();
+      tmem_ld64(tm + lanes + half * 64, s);
+      tc_fence_before();
+      mbar_arrive_warp(s_read);
+#pragma unroll
+      for (int c = 0; c < 64; ++c) s[c] = ex2(fmaf(s[c], pr.scale_log2, -L));
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c > last || (c < from && c >= sink)) s[c] = 0.f;
+      }
+      if (!(ok = warp_wait(dp_full, j & 1, err, 92))) break;
+      tc_fence_after();
+      tmem_ld64(tm + lanes + C::kDp + half * 64, d);
+      tc_fence_before();
+      mbar_arrive_warp(dp_read);
+      if (!whole) {  // nothing of a masked key reaches dS, infinities and NaN included
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c > last || (c < from && c >= sink)) d[c] = de;
+      }
+      uint32_t u[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) u[c / 2] = ds2<T>(s[c], s[c + 1], d[c], d[c + 1], de, de, f);
+      // dS's columns: free once the last dQ product has read them. NS = 4: over dP, where both halves of a row's dP
+      // must be in registers first
+      if (C::kHalves) {
+        if (!(ok = warp_wait(dp_read, j & 1, err, 93))) break;
+      } else if (j > 0) {
+        if (!(ok = warp_wait(dq_done, (j - 1) & 1, err, 93))) break;
+      }
+      tc_fence_after();
+      tmem_st32(tm + lanes + C::kDs + half * 32, u);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive_warp(ds_full);
+    }
+    if (ok && kr.n > 0) {
+      ok = warp_wait(dq_done, (kr.n - 1) & 1, err, 94);
+      tc_fence_after();
+    }
+    T* out = dq + (((long long)sq.b * pr.Tq + sq.q0 + i) * pr.H + h) * pr.D;
+    const float g = ok ? pr.scale / f : NAN;
+#pragma unroll 1
+    for (int c = half * NS * 32; c < (half + 1) * NS * 32; c += 32) {
+      float v[32];
+      if (kr.n > 0) {
+        tmem_ld32(tm + lanes + C::kDq + c, v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = 0.f;
+      }
+      if (live) store32(out, c, pr.D, v, g);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpsEw + 1) {
+    tc_fence_after();
+    tmem_dealloc(tm, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// dK, dV. S^T = K Q^T and dP^T = V dO^T with the keys on the rows. TMEM: S^T | dP^T | dV | dK, P^T over S^T and dS^T over
+// dP^T (each thread's 64 columns over its own). Order of the products, so that each runs under elementwise work:
+// dV(i), S(i + 1) under dS(i); dK(i), dP(i + 1) under P(i + 1). NS = 4: a CTA accumulates one half of the channels
+// (S^T and dP^T over all of them), Q and dO pass through a ring of half tiles in the order of their use.
+// parts > 1 (the first `heavy` key tiles): the tile's list of (query head, query tile) is cut into `parts` pieces, a CTA
+// each, whose sums go to fp32 partial tiles that sum_parts adds in order.
+template <int NS>
+struct DkvCfg {
+  static constexpr bool kHalves = NS == 4;
+  static constexpr int kAcc = NS == 1 ? 64 : 128;  // channels a CTA accumulates
+  static constexpr int kUnit = (kHalves ? 2 : NS) * kSlabBytes;
+  static constexpr int kQs = kHalves ? 3 : 2, kOs = kHalves ? 0 : 2;
+  static constexpr int kDp = 128, kDv = 256, kDk = 256 + kAcc;
+  static constexpr int kStats = kHalves ? 1 : 2;   // buffers of L and delta of a query tile
+  static constexpr int kBarriers = 1 + 2 * (kQs + kOs) + 8;
+  static constexpr size_t kSmem =
+      1024 + 2 * NS * kSlabBytes + (size_t)kUnit * (kQs + kOs) + 8 * kBarriers + 64 + kStats * 2 * 4 * kTile;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+struct Split {
+  int heavy, parts;
+  float* part;  // [b, key head, heavy tile, part][dK, dV][128][D]
+};
+
+template <typename T, int NS>
+__global__ void __launch_bounds__(kThreads, 1)
+    dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+               const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo, const Problem pr,
+               const Split sp, const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
+               T* __restrict__ dv, ErrorWord* err) {
+  using C = DkvCfg<NS>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* stats = reinterpret_cast<float*>(base + 2 * NS * kSlabBytes + C::kUnit * (C::kQs + C::kOs));  // [kStats][L, delta][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stats + C::kStats * 2 * kTile);
+  uint64_t* in_full = bars;   // K and V
+  uint64_t* full = bars + 1;  // Q ring, then dO ring
+  uint64_t* empty = full + C::kQs + C::kOs;
+  uint64_t* s_full = empty + C::kQs + C::kOs;
+  uint64_t* dp_full = s_full + 1;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* ds_full = s_full + 3;
+  uint64_t* dv_done = s_full + 4;
+  uint64_t* dk_done = s_full + 5;
+  uint64_t* st_full = s_full + 6;
+  uint64_t* fin = s_full + 7;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
+  int* info = reinterpret_cast<int*>(tslot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(in_full, 1);
+    for (int i = 0; i < C::kQs + C::kOs; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_full, kWarpsEw);
+    mbar_init(ds_full, kWarpsEw);
+    mbar_init(dv_done, 1);
+    mbar_init(dk_done, 1);
+    mbar_init(st_full, kWarpsEw);
+    mbar_init(fin, 1);
+    fence_mbar_init();
+  }
+  if (warp == kWarpsEw + 1) {
+    tmem_alloc(tslot, 512);
+    tmem_relinquish();
+  }
+  const int xh = C::kHalves ? (int)(blockIdx.y & 1) : 0;  // which half of the channels is accumulated
+  const int hk = C::kHalves ? (int)(blockIdx.y >> 1) : (int)blockIdx.y;
+  const int G = pr.H / pr.HK;
+  Seq sq;
+  // the first key tiles are seen by most queries: they start first, cut into parts where that pays
+  int tile = blockIdx.x, part = 0, parts = 1;
+  if (tile < sp.heavy * sp.parts) {
+    parts = sp.parts;
+    part = tile % parts;
+    tile /= parts;
+  } else {
+    tile -= sp.heavy * (sp.parts - 1);
+  }
+  if (pr.cu != nullptr && warp == 0) {
+    tile = find_item(pr.cu, pr.N, pr.Tk, blockIdx.x, [](int n) { return (n + kTile - 1) / kTile; }, sq);
+    if (lane == 0) {
+      info[0] = tile;
+      info[1] = sq.q0;
+      info[2] = sq.Tq;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (pr.cu != nullptr) {
+    tile = info[0];
+    sq.b = 0;
+    sq.q0 = sq.k0 = info[1];
+    sq.Tq = sq.Tk = info[2];
+  } else {
+    sq = {(int)blockIdx.z, 0, pr.Tq, 0, pr.Tk};
+  }
+  const uint32_t tm = *tslot;
+  const int c0 = tile * kTile, off = sq.offset();
+  // the query tiles that see some of these keys
+  int lo = 0, nq = 0;
+  if (tile >= 0) {
+    const int from = c0 - off > 0 ? c0 - off : 0;
+    int last = sq.Tq - 1;
+    if (c0 >= pr.sinks && pr.window < kNoWindow) {
+      const long long w = (long long)c0 + kTile - 1 + pr.window - 1 - off;
+      if (w < last) last = (int)w;
+    }
+    lo = from / kTile;
+    if (last >= from) nq = last / kTile - lo + 1;
+  }
+  const int all = nq * G;
+  const int it0 = (int)((long long)all * part / parts), n = (int)((long long)all * (part + 1) / parts) - it0;
+  const uint32_t s_k = smem_u32(base), s_v = s_k + NS * kSlabBytes, s_q = s_v + NS * kSlabBytes,
+                 s_o = s_q + C::kQs * C::kUnit;
+
+  if (warp == kWarpsEw) {
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(in_full, 2 * NS * kSlabBytes);
+      load_tile<NS>(s_k, &mk, hk, sq.k0 + c0, sq.b, in_full);
+      load_tile<NS>(s_v, &mv, hk, sq.k0 + c0, sq.b, in_full);
+      bool ok = true;
+      int a_n = 0, b_n = 0;
+      if constexpr (!C::kHalves) {
+        for (int i = 0; ok && i < n; ++i) {
+          const int h = hk * G + (it0 + i) / nq, t = sq.q0 + (lo + (it0 + i) % nq) * kTile;
+          const int a = i % C::kQs, b = C::kQs + i % C::kOs;
+          if (i >= C::kQs && !(ok = mbar_wait(empty + a, (i / C::kQs - 1) & 1, err, 100))) break;
+          mbar_arrive_expect_tx(full + a, C::kUnit);
+          load_tile<NS>(s_q + a * C::kUnit, &mq, h, t, sq.b, full + a);
+          ++a_n;
+          if (i >= C::kOs && !(ok = mbar_wait(empty + b, (i / C::kOs - 1) & 1, err, 101))) break;
+          mbar_arrive_expect_tx(full + b, C::kUnit);
+          load_tile<NS>(s_o + (i % C::kOs) * C::kUnit, &mo, h, t, sq.b, full + b);
+          ++b_n;
+        }
+      } else {
+        auto unit = [&](const CUtensorMap* m, int x, int i) {
+          const int h = hk * G + (it0 + i) / nq, t = sq.q0 + (lo + (it0 + i) % nq) * kTile;
+          const int a = a_n % C::kQs;
+          if (a_n >= C::kQs && !(ok = ok && mbar_wait(empty + a, (a_n / C::kQs - 1) & 1, err, 102))) return;
+          mbar_arrive_expect_tx(full + a, C::kUnit);
+          load_half(s_q + a * C::kUnit, m, x, h, t, sq.b, full + a);
+          ++a_n;
+        };
+        unit(&mq, 0, 0);
+        unit(&mq, 1, 0);
+        unit(&mo, 0, 0);
+        if (ok) unit(&mo, 1, 0);
+        for (int i = 0; ok && i < n; ++i) {
+          unit(&mo, xh, i);
+          if (ok && i + 1 < n) unit(&mq, 0, i + 1);
+          if (ok && i + 1 < n) unit(&mq, 1, i + 1);
+          if (ok) unit(&mq, xh, i);
+          if (ok && i + 1 < n) unit(&mo, 0, i + 1);
+          if (ok && i + 1 < n) unit(&mo, 1, i + 1);
+        }
+      }
+      mbar_wait(in_full, 0, err, 103);  // the copies in flight land before the CTA ends
+      for (int l = a_n > C::kQs ? a_n - C::kQs : 0; l < a_n; ++l) mbar_wait(full + l % C::kQs, (l / C::kQs) & 1, err, 103);
+      if constexpr (C::kOs > 0)
+        for (int l = b_n > C::kOs ? b_n - C::kOs : 0; l < b_n; ++l)
+          mbar_wait(full + C::kQs + l % C::kOs, (l / C::kOs) & 1, err, 103);
+    }
+  } else if (warp == kWarpsEw + 1) {
+    if (lane == 0 && n > 0) {
+      bool ok = mbar_wait(in_full, 0, err, 104);
+      if constexpr (!C::kHalves) {
+        auto scores = [&](int i) {
+          const int a = i % C::kQs;
+          if (!mbar_wait(full + a, (i / C::kQs) & 1, err, 105)) return false;
+          if (i > 0 && !mbar_wait(dv_done, (i - 1) & 1, err, 106)) return false;  // P^T of the columns is read
+          tc_fence_after();
+          mma_xyt<T, NS>(tm, s_k, s_q + a * C::kUnit);
+          mma_commit(s_full);
+          return true;
+        };
+        auto dps = [&](int i) {
+          const int b = i % C::kOs;
+          if (!mbar_wait(full + C::kQs + b, (i / C::kOs) & 1, err, 107)) return false;
+          if (i > 0 && !mbar_wait(dk_done, (i - 1) & 1, err, 108)) return false;  // dS^T of the columns is read
+          tc_fence_after();
+          mma_xyt<T, NS>(tm + C::kDp, s_v, s_o + b * C::kUnit);
+          mma_commit(dp_full);
+          return true;
+        };
+        ok = ok && scores(0) && dps(0);
+        for (int i = 0; ok && i < n; ++i) {
+          if (!(ok = mbar_wait(p_full, i & 1, err, 109))) break;
+          tc_fence_after();
+          mma_py<T, NS>(tm + C::kDv, tm, s_o + (i % C::kOs) * C::kUnit, i > 0, 64);
+          mma_commit(dv_done);
+          mma_commit(empty + C::kQs + i % C::kOs);
+          if (i + 1 < n) ok = scores(i + 1);
+          if (!(ok = ok && mbar_wait(ds_full, i & 1, err, 110))) break;
+          tc_fence_after();
+          mma_py<T, NS>(tm + C::kDk, tm + C::kDp, s_q + (i % C::kQs) * C::kUnit, i > 0, 64);
+          mma_commit(dk_done);
+          mma_commit(empty + i % C::kQs);
+          if (i + 1 < n) ok = dps(i + 1);
+        }
+      } else {
+        int u = 0;  // units used
+        auto next = [&]() { return mbar_wait(full + u % C::kQs, (u / C::kQs) & 1, err, 105); };
+        auto pair = [&](uint32_t d, uint32_t x) {
+          for (int y = 0; y < 2; ++y, ++u) {
+            if (!next()) return false;
+            tc_fence_after();
+            mma_xyt<T, 2>(d, x + y * 2 * kSlabBytes, s_q + u % C::kQs * C::kUnit, y > 0);
+            mma_commit(empty + u % C::kQs);
+          }
+          return true;
+        };
+        ok = ok && pair(tm, s_k);
+        if (ok) mma_commit(s_full);
+        ok = ok && pair(tm + C::kDp, s_v);
+        if (ok) mma_commit(dp_full);
+        for (int i = 0; ok && i < n; ++i) {
+          if (!(ok = mbar_wait(p_full, i & 1, err, 109) && next())) break;
+          tc_fence_after();
+          mma_py<T, 2>(tm + C::kDv, tm, s_q + u % C::kQs * C::kUnit, i > 0, 64);
+          mma_commit(empty + u % C::kQs);
+          mma_commit(dv_done);
+          ++u;
+          if (i + 1 < n) {
+            ok = mbar_wait(dv_done, i & 1, err, 106);
+            tc_fence_after();
+            ok = ok && pair(tm, s_k);
+            if (ok) mma_commit(s_full);
+          }
+          if (!(ok = ok && mbar_wait(ds_full, i & 1, err, 110) && next())) break;
+          tc_fence_after();
+          mma_py<T, 2>(tm + C::kDk, tm + C::kDp, s_q + u % C::kQs * C::kUnit, i > 0, 64);
+          mma_commit(empty + u % C::kQs);
+          mma_commit(dk_done);
+          ++u;
+          if (i + 1 < n) {
+            ok = mbar_wait(dk_done, i & 1, err, 108);
+            tc_fence_after();
+            ok = ok && pair(tm + C::kDp, s_v);
+            if (ok) mma_commit(dp_full);
+          }
+        }
+      }
+      mma_commit(fin);
+      mbar_wait(fin, 0, err, 111);
+    }
+  } else if (tile >= 0) {
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int key = c0 + row;
+    float f = 1.f;
+    if constexpr (std::is_same<T, __half>::value) f = ds_scale(err);
+    bool ok = true;
+    // L and delta of the queries of iteration i: thread t < 128 loads L of query t, the others delta
+    auto stat = [&](int i) -> float {
+      const int h = hk * G + (it0 + i) / nq, t = (lo + (it0 + i) % nq) * kTile + (threadIdx.x & 127);
+      const bool live = t < sq.Tq;
+      const long long at = ((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + t;
+      return threadIdx.x < 128 ? (live ? lse[at] : INFINITY) : (live ? delta[at] : 0.f);
+    };
+    float ahead = n > 0 ? stat(0) : 0.f;
+    for (int i = 0; i < n; ++i) {
+      // two buffers: all warps have passed iteration i - 1's barrier, so they are done with iteration i - 2's values; one
+      // buffer: they are done with iteration i - 1's when they have handed on its dS
+      float* st = stats + (i % C::kStats) * 256;
+      if (C::kStats == 1 && i > 0 && !(ok = warp_wait(ds_full, (i - 1) & 1, err, 115))) break;
+      st[threadIdx.x] = ahead;
+      mbar_arrive_warp(st_full);
+      if (i + 1 < n) ahead = stat(i + 1);
+      if (!(ok = warp_wait(st_full, i & 1, err, 116))) break;
+      const float4* L4 = reinterpret_cast<const float4*>(st + half * 64);
+      const float4* D4 = reinterpret_cast<const float4*>(st + 128 + half * 64);
+      const int i0 = (lo + (it0 + i) % nq) * kTile, q0 = i0 + off;  // the tile's first query and its position
+      const bool whole = i0 + kTile <= sq.Tq && all_visible(c0, q0, q0 + kTile - 1, pr.window, pr.sinks);
+      // query column c (position q0 + 64 half + c) sees the key: key <= position, key > position - window or key < sinks
+      const int from = key - q0 - half * 64;
+      const long long to = key < pr.sinks ? (1ll << 40) : (long long)key + pr.window - q0 - half * 64;
+      int end = sq.Tq - i0 - half * 64;
+      if (to < end) end = (int)to;
+      if (!(ok = warp_wait(s_full, i & 1, err, 112))) break;
+      tc_fence_after();
+      float s[64], d[64];
+      tmem_ld64(tm + lanes + half * 64, s);
+      uint32_t u[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 L = L4[c / 4];
+        s[c] = ex2(fmaf(s[c], pr.scale_log2, -L.x));
+        s[c + 1] = ex2(fmaf(s[c + 1], pr.scale_log2, -L.y));
+        s[c + 2] = ex2(fmaf(s[c + 2], pr.scale_log2, -L.z));
+        s[c + 3] = ex2(fmaf(s[c + 3], pr.scale_log2, -L.w));
+      }
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c < from || c >= end) s[c] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) u[c / 2] = pack16<T>(s[c], s[c + 1]);
+      tmem_st32(tm + lanes + half * 64, u);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive_warp(p_full);
+      if (!(ok = warp_wait(dp_full, i & 1, err, 113))) break;
+      tc_fence_after();
+      tmem_ld64(tm + lanes + C::kDp + half * 64, d);
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 e = D4[c / 4];
+        if (!whole) {  // nothing of a masked pair reaches dS, infinities and NaN included
+          if (c < from || c >= end) d[c] = e.x;
+          if (c + 1 < from || c + 1 >= end) d[c + 1] = e.y;
+          if (c + 2 < from || c + 2 >= end) d[c + 2] = e.z;
+          if (c + 3 < from || c + 3 >= end) d[c + 3] = e.w;
+        }
+        u[c / 2] = ds2<T>(s[c], s[c + 1], d[c], d[c + 1], e.x, e.y, f);
+        u[c / 2 + 1] = ds2<T>(s[c + 2], s[c + 3], d[c + 2], d[c + 3], e.z, e.w, f);
+      }
+      tmem_st32(tm + lanes + C::kDp + half * 64, u);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive_warp(ds_full);
+    }
+    if (ok && n > 0) {
+      ok = warp_wait(dv_done, (n - 1) & 1, err, 114) && warp_wait(dk_done, (n - 1) & 1, err, 114);
+      tc_fence_after();
+    }
+    // threads 0 .. 127 write dK, the others dV; key row each
+    const bool is_k = half == 0;
+    const float g = !ok ? NAN : is_k ? pr.scale / f : 1.f;
+    const uint32_t acc = tm + lanes + (is_k ? C::kDk : C::kDv);
+    const int ch = xh * 128;  // the first channel accumulated
+#pragma unroll 1
+    for (int c = 0; c < C::kAcc; c += 32) {
+      float v[32];
+      if (n > 0) {
+        tmem_ld32(acc + c, v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = 0.f;
+      }
+      if (key >= sq.Tk) continue;
+      if (parts > 1) {
+        float* out = sp.part + (((((long long)sq.b * pr.HK + hk) * sp.heavy + tile) * parts + part) * 2 + (is_k ? 0 : 1)) *
+                                   kTile * pr.D + (long long)row * pr.D;
+#pragma unroll
+        for (int k = 0; k < 32; k += 4)
+          if (ch + c + k < pr.D)
+            *reinterpret_cast<float4*>(out + ch + c + k) = make_float4(v[k] * g, v[k + 1] * g, v[k + 2] * g, v[k + 3] * g);
+      } else {
+        store32((is_k ? dk : dv) + (((long long)sq.b * pr.Tk + sq.k0 + key) * pr.HK + hk) * pr.D, ch + c, pr.D, v, g);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpsEw + 1) {
+    tc_fence_after();
+    tmem_dealloc(tm, 512);
+  }
+}
+
+// dK and dV of the heavy tiles: their parts in order; a thread 4 channels of a row
+template <typename T>
+__global__ void __launch_bounds__(256) sum_parts(const float* __restrict__ part, T* __restrict__ dk, T* __restrict__ dv,
+                                                 int Tk, int HK, int D, int heavy, int parts) {
+  const int per = kTile * D / 4, i = blockIdx.x * 256 + threadIdx.x;
+  const int tile = blockIdx.y >> 1, which = blockIdx.y & 1;
+  const int b = blockIdx.z / HK, hk = blockIdx.z % HK;
+  if (i >= per) return;
+  const int row = i / (D / 4), c = i % (D / 4) * 4, key = tile * kTile + row;
+  if (key >= Tk) return;
+  const float* p = part + ((((long long)b * HK + hk) * heavy + tile) * parts * 2 + which) * kTile * D + (long long)row * D + c;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int x = 0; x < parts; ++x) {
+    const float4 v = *reinterpret_cast<const float4*>(p + (long long)x * 2 * kTile * D);
+    t.x += v.x;
+    t.y += v.y;
+    t.z += v.z;
+    t.w += v.w;
+  }
+  T* out = (which ? dv : dk) + (((long long)b * Tk + key) * HK + hk) * D + c;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(t.x, t.y), pack16<T>(t.z, t.w));
+}
+
+template <typename T, int NS>
+int launch(const void* q, const void* k, const void* v, const void* o, const void* g, const long long* st,
+           const Problem& pr, const float* lse, float* delta, void* dq, void* dk, void* dv, Split sp, ErrorWord* err,
+           cudaStream_t stream) {
+  CUtensorMap mq, mk, mv, mo;
+  const CUtensorMapDataType dt = map_dtype<T>();
+  if (!tile_map(&mq, q, dt, pr.B, pr.Tq, pr.H, pr.D, st[0], st[1], st[2], kTile) ||
+      !tile_map(&mk, k, dt, pr.B, pr.Tk, pr.HK, pr.D, st[3], st[4], st[5], kTile) ||
+      !tile_map(&mv, v, dt, pr.B, pr.Tk, pr.HK, pr.D, st[6], st[7], st[8], kTile) ||
+      !tile_map(&mo, g, dt, pr.B, pr.Tq, pr.H, pr.D, st[9], st[10], st[11], kTile))
+    return GD_ERR_LAUNCH;
+  const long long rows = (long long)pr.B * pr.Tq * pr.H;
+  delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(static_cast<const T*>(o), static_cast<const T*>(g),
+                                                                   st[9], st[10], st[11], delta, pr.B, pr.Tq, pr.H, pr.D,
+                                                                   err);
+  static bool done_q[kMaxDevices], done_kv[kMaxDevices];
+  auto kq = dq_kernel<T, NS>;
+  auto kkv = dkv_kernel<T, NS>;
+  if (set_smem_once(kq, DqCfg<NS>::kSmem, done_q) != cudaSuccess || set_smem_once(kkv, DkvCfg<NS>::kSmem, done_kv) != cudaSuccess)
+    return (cudaGetLastError(), GD_ERR_LAUNCH);
+  const long long qt = pr.cu ? (long long)pr.Tq / kTile + pr.N : (pr.Tq + kTile - 1) / kTile;
+  const long long kt = (pr.cu ? (long long)pr.Tk / kTile + pr.N : (pr.Tk + kTile - 1) / kTile) + (long long)sp.heavy * (sp.parts - 1);
+  kq<<<dim3((unsigned)qt, (unsigned)pr.H, (unsigned)pr.B), kThreads, DqCfg<NS>::kSmem, stream>>>(
+      mq, mk, mv, mo, pr, lse, delta, static_cast<T*>(dq), err);
+  kkv<<<dim3((unsigned)kt, (unsigned)(pr.HK * (NS == 4 ? 2 : 1)), (unsigned)pr.B), kThreads, DkvCfg<NS>::kSmem, stream>>>(
+      mq, mk, mv, mo, pr, sp, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), err);
+  if (sp.parts > 1)
+    sum_parts<T><<<dim3((unsigned)((kTile * pr.D / 4 + 255) / 256), (unsigned)(2 * sp.heavy), (unsigned)(pr.B * pr.HK)), 256,
+                   0, stream>>>(sp.part, static_cast<T*>(dk), static_cast<T*>(dv), pr.Tk, pr.HK, pr.D, sp.heavy, sp.parts);
+  return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
+}
+
+}  // namespace
+
+int backward(const void* q, const void* k, const void* v, const void* o, const void* g, const long long* strides,
+             const Problem& pr, int dtype, const float* lse, float* delta, void* dq, void* dk, void* dv, int heavy,
+             int parts, float* part, ErrorWord* err, cudaStream_t stream) {
+  const Split sp = {heavy, parts, part};
+  auto run = [&](auto t, auto ns) {
+    return launch<decltype(t), decltype(ns)::value>(q, k, v, o, g, strides, pr, lse, delta, dq, dk, dv, sp, err, stream);
+  };
+  auto by_width = [&](auto t) {
+    return pr.D <= 64    ? run(t, std::integral_constant<int, 1>{})
+           : pr.D <= 128 ? run(t, std::integral_constant<int, 2>{})
+                         : run(t, std::integral_constant<int, 4>{});
+  };
+  return dtype == GD_FLOAT16 ? by_width(__half{}) : by_width(__nv_bfloat16{});
+}
+
+}  // namespace wattn
+}  // namespace gd
