@@ -181,16 +181,55 @@ __device__ __forceinline__ void mma_xyt(uint32_t d, uint32_t x, uint32_t y, bool
       mma_bf16(d, desc_k(x + s * kSlabBytes) + 2 * k, desc_k(y + s * kSlabBytes) + 2 * k, idesc<T>(128, 128, false),
                acc || s > 0 || k > 0);
 }
-// D[128 x NS 64] (+)= P Y: P in TMEM (128 rows, 128 contracted columns as 64 words), Y's rows contracted. `gap`: words
-// between P's two halves of 64 contracted columns (32: adjacent)
+// D[128 x NS 64] (+)= P Y: P in TMEM (128 rows, 128 contracted columns as 64 words), Y's rows contracted. P stands in
+// pieces of 32 contracted columns (16 words), `gap` words apart.
 template <typename T, int NS>
-__device__ __forceinline__ void mma_py(uint32_t d, uint32_t p, uint32_t y, bool acc, int gap = 32) {
+__device__ __forceinline__ void mma_py(uint32_t d, uint32_t p, uint32_t y, bool acc, int gap) {
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    mma_ts(d, p + (k & 3) * 8 + (k >> 2) * gap, desc_mn(y) + 128 * k, idesc<T>(128, NS * 64, true), acc || k > 0);
+    mma_ts(d, p + (k & 1) * 8 + (k >> 1) * gap, desc_mn(y) + 128 * k, idesc<T>(128, NS * 64, true), acc || k > 0);
 }
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// two fp32 values at once (the packed instructions take an issue slot for two operations)
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unf2(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// bits [from, end) of 32 (any ints)
+__device__ __forceinline__ uint32_t bits(int from, int end) {
+  const uint32_t lo = from <= 0 ? 0xffffffffu : from >= 32 ? 0u : 0xffffffffu << from;
+  const uint32_t hi = end >= 32 ? 0xffffffffu : end <= 0 ? 0u : 0xffffffffu >> (32 - end);
+  return lo & hi;
+}
+// the visible ones of keys c .. c + 31 to position p: key <= p, and key > p - window or key < sinks
+__device__ __forceinline__ uint32_t visible_keys(int c, int p, int window, int sinks) {
+  return (bits(p - window + 1 - c, p + 1 - c) | bits(0, sinks - c)) & bits(0, p + 1 - c);
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -208,44 +247,7 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   }
 }
 
-// 128 consecutive fp32 columns of the thread's own lane, one wait.
-__device__ __forceinline__ void tmem_ld128(uint32_t a, float (&v)[128]) {
-  uint32_t r[128];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      :
-        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]),
-        "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]),
-        "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]),
-        "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]),
-        "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
-      : "r"(a), "r"(a + 32), "r"(a + 64), "r"(a + 96)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// 64 of them.
+// 64 consecutive fp32 columns of the thread's own lane, one wait.
 __device__ __forceinline__ void tmem_ld64(uint32_t a, float (&v)[64]) {
   uint32_t r[64];
   asm volatile(

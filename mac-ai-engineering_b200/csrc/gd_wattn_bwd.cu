@@ -19,7 +19,7 @@ namespace gd {
 namespace wattn {
 namespace {
 
-constexpr int kWarpsEw = 8;                      // two threads a row, 64 columns each
+constexpr int kWarpsEw = 16;                     // elementwise work: four threads a row, 32 columns each
 constexpr int kThreads = 32 * (kWarpsEw + 2);    // + loads, + products
 
 // the error word's first spare field holds the bits of the largest |dO| (float16)
@@ -76,11 +76,11 @@ __global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, con
   }
 }
 
-// 32 fp32 columns of the accumulator times f -> row `out` (16-bit), channels c .. c + 31 below D
+// 16 fp32 columns of the accumulator times f -> row `out` (16-bit), channels c .. c + 15 below D
 template <typename T>
-__device__ __forceinline__ void store32(T* out, int c, int D, const float (&v)[32], float f) {
+__device__ __forceinline__ void store16(T* out, int c, int D, const float (&v)[16], float f) {
 #pragma unroll
-  for (int k = 0; k < 32; k += 8) {
+  for (int k = 0; k < 16; k += 8) {
     if (c + k >= D) break;
     uint32_t u[4];
 #pragma unroll
@@ -89,11 +89,15 @@ __device__ __forceinline__ void store32(T* out, int c, int D, const float (&v)[3
   }
 }
 
-// dS of 64 columns: p (dp - delta) f, packed
+// dS of two columns: p (dp - delta) f, packed
 template <typename T>
-__device__ __forceinline__ uint32_t ds2(float p0, float p1, float d0, float d1, float e0, float e1, float f) {
-  if constexpr (std::is_same<T, __half>::value) return pack16<T>(p0 * ((d0 - e0) * f), p1 * ((d1 - e1) * f));
-  else return pack16<T>(p0 * (d0 - e0), p1 * (d1 - e1));
+__device__ __forceinline__ uint32_t ds2(F2 p, F2 d, F2 minus_delta, float f) {
+  F2 x = add2(d, minus_delta);
+  if constexpr (std::is_same<T, __half>::value) x = mul2(x, f2(f, f));
+  x = mul2(p, x);
+  float a, b;
+  unf2(x, a, b);
+  return pack16<T>(a, b);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -253,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j + 1 < kr.n) ok = first(j + 1);
           if (!(ok = ok && mbar_wait(ds_full, j & 1, err, 89))) break;
           tc_fence_after();
-          mma_py<T, NS>(tm + C::kDq, tm + C::kDs, s_k + (j % C::kKs) * C::kUnit, j > 0);
+          mma_py<T, NS>(tm + C::kDq, tm + C::kDs, s_k + (j % C::kKs) * C::kUnit, j > 0, 16);
           mma_commit(empty + j % C::kKs);
           mma_commit(dq_done);
         }
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int a = n % C::kKs;
             if (!(ok = mbar_wait(full + a, (n / C::kKs) & 1, err, 85))) break;
             tc_fence_after();
-            mma_py<T, 2>(tm + C::kDq + y * 128, tm + C::kDs, s_k + a * C::kUnit, j > 0);
+            mma_py<T, 2>(tm + C::kDq + y * 128, tm + C::kDs, s_k + a * C::kUnit, j > 0, 16);
             mma_commit(empty + a);
           }
           if (!ok) break;
@@ -301,54 +305,57 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(fin, 0, err, 90);
     }
   } else if (tile >= 0) {
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const int row = (warp & 3) * 32 + lane, part = warp >> 2;  // TMEM lane, which 32 columns
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int i = i0 + row, p = p0 + row;
     const bool live = i < sq.Tq;
     const long long at = ((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i;
     const float L = live ? lse[at] : INFINITY, de = live ? delta[at] : 0.f;
+    const F2 sc = f2(pr.scale_log2, pr.scale_log2), mL = f2(-L, -L), mde = f2(-de, -de);
     float f = 1.f;
     if constexpr (std::is_same<T, __half>::value) f = ds_scale(err);
     bool ok = true;
     for (int j = 0; j < kr.n; ++j) {
-      const int c0 = kr.key(j) + half * 64;
+      const int c0 = kr.key(j) + part * 32;
       const bool whole = all_visible(kr.key(j), p0, p1, pr.window, pr.sinks);
-      const int last = p - c0, from = p - pr.window + 1 - c0, sink = pr.sinks - c0;
-      float s[64], d[64];
+      const uint32_t vis = whole ? 0xffffffffu : visible_keys(c0, p, pr.window, pr.sinks);
+      float s[32], d[32];
       if (!(ok = warp_wait(s_full, j & 1, err, 91))) break;
       tc_fence_after();
-      tmem_ld64(tm + lanes + half * 64, s);
+      tmem_ld32(tm + lanes + part * 32, s);
       tc_fence_before();
       mbar_arrive_warp(s_read);
 #pragma unroll
-      for (int c = 0; c < 64; ++c) s[c] = ex2(fmaf(s[c], pr.scale_log2, -L));
-      if (!whole) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c > last || (c < from && c >= sink)) s[c] = 0.f;
+      for (int c = 0; c < 32; c += 2) {
+        float a, b;
+        unf2(fma2(f2(s[c], s[c + 1]), sc, mL), a, b);
+        s[c] = ex2(a);
+        s[c + 1] = ex2(b);
       }
       if (!(ok = warp_wait(dp_full, j & 1, err, 92))) break;
       tc_fence_after();
-      tmem_ld64(tm + lanes + C::kDp + half * 64, d);
+      tmem_ld32(tm + lanes + C::kDp + part * 32, d);
       tc_fence_before();
       mbar_arrive_warp(dp_read);
       if (!whole) {  // nothing of a masked key reaches dS, infinities and NaN included
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c > last || (c < from && c >= sink)) d[c] = de;
+        for (int c = 0; c < 32; ++c) {
+          s[c] = (vis >> c) & 1 ? s[c] : 0.f;
+          d[c] = (vis >> c) & 1 ? d[c] : de;
+        }
       }
-      uint32_t u[32];
+      uint32_t u[16];
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) u[c / 2] = ds2<T>(s[c], s[c + 1], d[c], d[c + 1], de, de, f);
-      // dS's columns: free once the last dQ product has read them. NS = 4: over dP, where both halves of a row's dP
-      // must be in registers first
+      for (int c = 0; c < 32; c += 2) u[c / 2] = ds2<T>(f2(s[c], s[c + 1]), f2(d[c], d[c + 1]), mde, f);
+      // dS's columns: free once the last dQ product has read them. NS = 4: over dP, where all of a row's dP must be in
+      // registers first
       if (C::kHalves) {
         if (!(ok = warp_wait(dp_read, j & 1, err, 93))) break;
       } else if (j > 0) {
         if (!(ok = warp_wait(dq_done, (j - 1) & 1, err, 93))) break;
       }
       tc_fence_after();
-      tmem_st32(tm + lanes + C::kDs + half * 32, u);
+      tmem_st16(tm + lanes + C::kDs + part * 16, u);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive_warp(ds_full);
@@ -360,15 +367,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     T* out = dq + (((long long)sq.b * pr.Tq + sq.q0 + i) * pr.H + h) * pr.D;
     const float g = ok ? pr.scale / f : NAN;
 #pragma unroll 1
-    for (int c = half * NS * 32; c < (half + 1) * NS * 32; c += 32) {
-      float v[32];
+    for (int c = part * NS * 16; c < (part + 1) * NS * 16; c += 16) {
+      float v[16];
       if (kr.n > 0) {
-        tmem_ld32(tm + lanes + C::kDq + c, v);
+        tmem_ld16(tm + lanes + C::kDq + c, v);
       } else {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = 0.f;
+        for (int k = 0; k < 16; ++k) v[k] = 0.f;
       }
-      if (live) store32(out, c, pr.D, v, g);
+      if (live) store16(out, c, pr.D, v, g);
     }
   }
   tc_fence_before();
@@ -381,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------------------------------------------------------
 // dK, dV. S^T = K Q^T and dP^T = V dO^T with the keys on the rows. TMEM: S^T | dP^T | dV | dK, P^T over S^T and dS^T over
-// dP^T (each thread's 64 columns over its own). Order of the products, so that each runs under elementwise work:
+// dP^T (each thread's 32 columns over its own). Order of the products, so that each runs under elementwise work:
 // dV(i), S(i + 1) under dS(i); dK(i), dP(i + 1) under P(i + 1). NS = 4: a CTA accumulates one half of the channels
 // (S^T and dP^T over all of them), Q and dO pass through a ring of half tiles in the order of their use.
 // parts > 1 (the first `heavy` key tiles): the tile's list of (query head, query tile) is cut into `parts` pieces, a CTA
@@ -576,13 +583,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; ok && i < n; ++i) {
           if (!(ok = mbar_wait(p_full, i & 1, err, 109))) break;
           tc_fence_after();
-          mma_py<T, NS>(tm + C::kDv, tm, s_o + (i % C::kOs) * C::kUnit, i > 0, 64);
+          mma_py<T, NS>(tm + C::kDv, tm, s_o + (i % C::kOs) * C::kUnit, i > 0, 32);
           mma_commit(dv_done);
           mma_commit(empty + C::kQs + i % C::kOs);
           if (i + 1 < n) ok = scores(i + 1);
           if (!(ok = ok && mbar_wait(ds_full, i & 1, err, 110))) break;
           tc_fence_after();
-          mma_py<T, NS>(tm + C::kDk, tm + C::kDp, s_q + (i % C::kQs) * C::kUnit, i > 0, 64);
+          mma_py<T, NS>(tm + C::kDk, tm + C::kDp, s_q + (i % C::kQs) * C::kUnit, i > 0, 32);
           mma_commit(dk_done);
           mma_commit(empty + i % C::kQs);
           if (i + 1 < n) ok = dps(i + 1);
@@ -606,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; ok && i < n; ++i) {
           if (!(ok = mbar_wait(p_full, i & 1, err, 109) && next())) break;
           tc_fence_after();
-          mma_py<T, 2>(tm + C::kDv, tm, s_q + u % C::kQs * C::kUnit, i > 0, 64);
+          mma_py<T, 2>(tm + C::kDv, tm, s_q + u % C::kQs * C::kUnit, i > 0, 32);
           mma_commit(empty + u % C::kQs);
           mma_commit(dv_done);
           ++u;
@@ -618,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!(ok = ok && mbar_wait(ds_full, i & 1, err, 110) && next())) break;
           tc_fence_after();
-          mma_py<T, 2>(tm + C::kDk, tm + C::kDp, s_q + u % C::kQs * C::kUnit, i > 0, 64);
+          mma_py<T, 2>(tm + C::kDk, tm + C::kDp, s_q + u % C::kQs * C::kUnit, i > 0, 32);
           mma_commit(empty + u % C::kQs);
           mma_commit(dk_done);
           ++u;
@@ -634,78 +641,86 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(fin, 0, err, 111);
     }
   } else if (tile >= 0) {
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const int row = (warp & 3) * 32 + lane, quarter = warp >> 2;  // TMEM lane, which 32 columns
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int key = c0 + row;
+    const F2 sc = f2(pr.scale_log2, pr.scale_log2);
     float f = 1.f;
     if constexpr (std::is_same<T, __half>::value) f = ds_scale(err);
     bool ok = true;
-    // L and delta of the queries of iteration i: thread t < 128 loads L of query t, the others delta
-    auto stat = [&](int i) -> float {
-      const int h = hk * G + (it0 + i) / nq, t = (lo + (it0 + i) % nq) * kTile + (threadIdx.x & 127);
-      const bool live = t < sq.Tq;
-      const long long at = ((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + t;
-      return threadIdx.x < 128 ? (live ? lse[at] : INFINITY) : (live ? delta[at] : 0.f);
+    // -L and -delta of the queries of iteration i: thread t < 128 loads L of query t, threads 128 .. 255 delta
+    const float* stat_of = (threadIdx.x < 128 ? lse : delta) + (long long)sq.b * pr.H * pr.Tq + sq.q0;
+    auto stat = [&](int h, int qt) -> float {
+      const int t = qt * kTile + (threadIdx.x & 127);
+      return t < sq.Tq ? -__ldg(stat_of + (long long)h * pr.Tq + t) : threadIdx.x < 128 ? -INFINITY : 0.f;
     };
-    float ahead = n > 0 ? stat(0) : 0.f;
+    int h = hk * G + (n > 0 ? it0 / nq : 0), qt = lo + (n > 0 ? it0 % nq : 0);  // of the iteration
+    float ahead = n > 0 && threadIdx.x < 256 ? stat(h, qt) : 0.f;
     for (int i = 0; i < n; ++i) {
       // two buffers: all warps have passed iteration i - 1's barrier, so they are done with iteration i - 2's values; one
       // buffer: they are done with iteration i - 1's when they have handed on its dS
       float* st = stats + (i % C::kStats) * 256;
       if (C::kStats == 1 && i > 0 && !(ok = warp_wait(ds_full, (i - 1) & 1, err, 115))) break;
-      st[threadIdx.x] = ahead;
+      if (threadIdx.x < 256) st[threadIdx.x] = ahead;
       mbar_arrive_warp(st_full);
-      if (i + 1 < n) ahead = stat(i + 1);
+      const int i0 = qt * kTile, q0 = i0 + off;  // the tile's first query and its position
+      if (++qt == lo + nq) {
+        qt = lo;
+        ++h;
+      }
+      if (i + 1 < n && threadIdx.x < 256) ahead = stat(h, qt);
       if (!(ok = warp_wait(st_full, i & 1, err, 116))) break;
-      const float4* L4 = reinterpret_cast<const float4*>(st + half * 64);
-      const float4* D4 = reinterpret_cast<const float4*>(st + 128 + half * 64);
-      const int i0 = (lo + (it0 + i) % nq) * kTile, q0 = i0 + off;  // the tile's first query and its position
+      const ulonglong2* L4 = reinterpret_cast<const ulonglong2*>(st + quarter * 32);
+      const ulonglong2* D4 = reinterpret_cast<const ulonglong2*>(st + 128 + quarter * 32);
       const bool whole = i0 + kTile <= sq.Tq && all_visible(c0, q0, q0 + kTile - 1, pr.window, pr.sinks);
-      // query column c (position q0 + 64 half + c) sees the key: key <= position, key > position - window or key < sinks
-      const int from = key - q0 - half * 64;
-      const long long to = key < pr.sinks ? (1ll << 40) : (long long)key + pr.window - q0 - half * 64;
-      int end = sq.Tq - i0 - half * 64;
-      if (to < end) end = (int)to;
+      uint32_t vis = 0xffffffffu;
+      if (!whole) {
+        // query column c (position q0 + 32 quarter + c) sees the key: key <= position, key > position - window or key < sinks
+        const long long to = key < pr.sinks ? (1ll << 40) : (long long)key + pr.window - q0 - quarter * 32;
+        int end = sq.Tq - i0 - quarter * 32;
+        if (to < end) end = (int)to;
+        vis = bits(key - q0 - quarter * 32, end);
+      }
       if (!(ok = warp_wait(s_full, i & 1, err, 112))) break;
       tc_fence_after();
-      float s[64], d[64];
-      tmem_ld64(tm + lanes + half * 64, s);
-      uint32_t u[32];
+      float s[32], d[32];
+      tmem_ld32(tm + lanes + quarter * 32, s);
+      uint32_t u[16];
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 L = L4[c / 4];
-        s[c] = ex2(fmaf(s[c], pr.scale_log2, -L.x));
-        s[c + 1] = ex2(fmaf(s[c + 1], pr.scale_log2, -L.y));
-        s[c + 2] = ex2(fmaf(s[c + 2], pr.scale_log2, -L.z));
-        s[c + 3] = ex2(fmaf(s[c + 3], pr.scale_log2, -L.w));
+      for (int c = 0; c < 32; c += 4) {
+        const ulonglong2 L = L4[c / 4];
+        float a, b;
+        unf2(fma2(f2(s[c], s[c + 1]), sc, L.x), a, b);
+        s[c] = ex2(a);
+        s[c + 1] = ex2(b);
+        unf2(fma2(f2(s[c + 2], s[c + 3]), sc, L.y), a, b);
+        s[c + 2] = ex2(a);
+        s[c + 3] = ex2(b);
       }
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < from || c >= end) s[c] = 0.f;
+        for (int c = 0; c < 32; ++c) s[c] = (vis >> c) & 1 ? s[c] : 0.f;
       }
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) u[c / 2] = pack16<T>(s[c], s[c + 1]);
-      tmem_st32(tm + lanes + half * 64, u);
+      for (int c = 0; c < 32; c += 2) u[c / 2] = pack16<T>(s[c], s[c + 1]);
+      tmem_st16(tm + lanes + quarter * 32, u);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive_warp(p_full);
       if (!(ok = warp_wait(dp_full, i & 1, err, 113))) break;
       tc_fence_after();
-      tmem_ld64(tm + lanes + C::kDp + half * 64, d);
+      tmem_ld32(tm + lanes + C::kDp + quarter * 32, d);
+      if (!whole) {  // nothing of a masked pair reaches dS, infinities and NaN included
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 e = D4[c / 4];
-        if (!whole) {  // nothing of a masked pair reaches dS, infinities and NaN included
-          if (c < from || c >= end) d[c] = e.x;
-          if (c + 1 < from || c + 1 >= end) d[c + 1] = e.y;
-          if (c + 2 < from || c + 2 >= end) d[c + 2] = e.z;
-          if (c + 3 < from || c + 3 >= end) d[c + 3] = e.w;
-        }
-        u[c / 2] = ds2<T>(s[c], s[c + 1], d[c], d[c + 1], e.x, e.y, f);
-        u[c / 2 + 1] = ds2<T>(s[c + 2], s[c + 3], d[c + 2], d[c + 3], e.z, e.w, f);
+        for (int c = 0; c < 32; ++c) d[c] = (vis >> c) & 1 ? d[c] : 0.f;
       }
-      tmem_st32(tm + lanes + C::kDp + half * 64, u);
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const ulonglong2 e = D4[c / 4];
+        u[c / 2] = ds2<T>(f2(s[c], s[c + 1]), f2(d[c], d[c + 1]), e.x, f);
+        u[c / 2 + 1] = ds2<T>(f2(s[c + 2], s[c + 3]), f2(d[c + 2], d[c + 3]), e.y, f);
+      }
+      tmem_st16(tm + lanes + C::kDp + quarter * 32, u);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive_warp(ds_full);
@@ -714,30 +729,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = warp_wait(dv_done, (n - 1) & 1, err, 114) && warp_wait(dk_done, (n - 1) & 1, err, 114);
       tc_fence_after();
     }
-    // threads 0 .. 127 write dK, the others dV; key row each
-    const bool is_k = half == 0;
+    // quarters 0 and 1 write dK's channels, 2 and 3 dV's; key row each
+    const bool is_k = quarter < 2;
     const float g = !ok ? NAN : is_k ? pr.scale / f : 1.f;
     const uint32_t acc = tm + lanes + (is_k ? C::kDk : C::kDv);
     const int ch = xh * 128;  // the first channel accumulated
 #pragma unroll 1
-    for (int c = 0; c < C::kAcc; c += 32) {
-      float v[32];
+    for (int c = (quarter & 1) * (C::kAcc / 2); c < ((quarter & 1) + 1) * (C::kAcc / 2); c += 16) {
+      float v[16];
       if (n > 0) {
-        tmem_ld32(acc + c, v);
+        tmem_ld16(acc + c, v);
       } else {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = 0.f;
+        for (int k = 0; k < 16; ++k) v[k] = 0.f;
       }
       if (key >= sq.Tk) continue;
       if (parts > 1) {
         float* out = sp.part + (((((long long)sq.b * pr.HK + hk) * sp.heavy + tile) * parts + part) * 2 + (is_k ? 0 : 1)) *
                                    kTile * pr.D + (long long)row * pr.D;
 #pragma unroll
-        for (int k = 0; k < 32; k += 4)
+        for (int k = 0; k < 16; k += 4)
           if (ch + c + k < pr.D)
             *reinterpret_cast<float4*>(out + ch + c + k) = make_float4(v[k] * g, v[k + 1] * g, v[k + 2] * g, v[k + 3] * g);
       } else {
-        store32((is_k ? dk : dv) + (((long long)sq.b * pr.Tk + sq.k0 + key) * pr.HK + hk) * pr.D, ch + c, pr.D, v, g);
+        store16((is_k ? dk : dv) + (((long long)sq.b * pr.Tk + sq.k0 + key) * pr.HK + hk) * pr.D, ch + c, pr.D, v, g);
       }
     }
   }

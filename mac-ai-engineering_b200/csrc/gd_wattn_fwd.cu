@@ -3,8 +3,9 @@
 // in one pass over the keys with a running maximum and sum (fp32); O stays in TMEM between key tiles. A query without a
 // visible key gets zeros and L = +inf.
 //
-// One CTA takes 128 queries of a head. Roles: warps 0-3 softmax (a thread owns a query row, TMEM lane = row), warp 4
-// loads (TMA), warp 5 issues the products. Key tiles outside the window and past the first tokens are never loaded.
+// One CTA takes 128 queries of a head. Roles: warps 0-7 softmax (TMEM lane = query row; two threads a row, 64 key columns
+// each, which agree on the row's maximum through shared memory when it moves), warp 8 loads (TMA), warp 9 issues the
+// products. Key tiles outside the window and past the first tokens are never loaded.
 //   S (128 x 128 fp32) comes from tcgen05 into TMEM; the softmax writes P over it as 16-bit pairs, where it is the A
 //   operand of P V (no trip through shared memory). P is rounded to the inputs' 16-bit type (the operand type of the
 //   matrix instruction); its sum is taken before the rounding, in fp32.
@@ -18,7 +19,8 @@ namespace gd {
 namespace wattn {
 namespace {
 
-constexpr int kThreads = 192;
+constexpr int kWarpsSm = 8;                     // softmax: two threads a query row, 64 columns each
+constexpr int kThreads = 32 * (kWarpsSm + 2);   // + loads, + products
 constexpr float kMaxGrowth = 8.f;  // log2
 
 template <int NS>
@@ -29,7 +31,7 @@ struct Cfg {
   static constexpr int kCols = NS == 4 ? 512 : 256;        // TMEM columns
   static constexpr int kO = kBufs * 128;                   // O's first column
   static constexpr int kBarriers = 1 + 2 * kSlots + 2 * kBufs + 2;
-  static constexpr size_t kSmem = 1024 + (size_t)kTileBytes * (1 + kSlots) + 8 * kBarriers + 64;
+  static constexpr size_t kSmem = 1024 + (size_t)kTileBytes * (1 + kSlots) + 8 * kBarriers + 64 + 8 * kTile;
 };
 
 template <typename T, int NS>
@@ -50,6 +52,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   uint64_t* fin = o_done + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   int* info = reinterpret_cast<int*>(tslot + 1);  // the packed sequence and tile of this CTA
+  float* xchg = reinterpret_cast<float*>(bars + C::kBarriers) + 16;  // [2][128]: a row's two threads
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -60,13 +63,13 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     }
     for (int i = 0; i < C::kBufs; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
+      mbar_init(p_full + i, kWarpsSm);
     }
     mbar_init(o_done, 1);
     mbar_init(fin, 1);
     fence_mbar_init();
   }
-  if (warp == 5) {
+  if (warp == kWarpsSm + 1) {
     tmem_alloc(tslot, C::kCols);
     tmem_relinquish();
   }
@@ -102,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   const KeyRange kr(tile < 0 ? -1 : p0, tile < 0 ? -1 : p1, pr.window, pr.sinks);
   const uint32_t s_q = smem_u32(base), s_kv = s_q + C::kTileBytes;
 
-  if (warp == 4) {
+  if (warp == kWarpsSm) {
     if (lane == 0 && kr.n > 0) {
       const int hk = h / (pr.H / pr.HK);
       mbar_arrive_expect_tx(q_full, C::kTileBytes);
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       mbar_wait(q_full, 0, err, 61);
       for (int l = c > C::kSlots ? c - C::kSlots : 0; l < c; ++l) mbar_wait(full + l % C::kSlots, (l / C::kSlots) & 1, err, 61);
     }
-  } else if (warp == 5) {
+  } else if (warp == kWarpsSm + 1) {
     if (lane == 0 && kr.n > 0) {
       bool ok = mbar_wait(q_full, 0, err, 62);
       auto scores = [&](int j) {  // S of tile j
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
         ok = ok && mbar_wait(full + slot, (c / C::kSlots) & 1, err, 65) && mbar_wait(p_full + buf, (j / C::kBufs) & 1, err, 66);
         if (!ok) break;
         tc_fence_after();
-        mma_py<T, NS>(tm + C::kO, tm + buf * 128, s_kv + slot * C::kTileBytes, j > 0);
+        mma_py<T, NS>(tm + C::kO, tm + buf * 128, s_kv + slot * C::kTileBytes, j > 0, 32);
         mma_commit(empty + slot);
         mma_commit(o_done);
       }
@@ -147,88 +150,113 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       mbar_wait(fin, 0, err, 67);
     }
   } else if (tile >= 0) {
-    const int row = threadIdx.x;  // TMEM lane
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;  // TMEM lane, which 64 columns
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int pair = 1 + (warp & 3);  // named barrier of the two warps that share 32 rows
     const int p = p0 + row;
-    float m = -INFINITY, l = 0.f;  // running maximum (log2 units, of scaled scores) and sum
-    bool ok = true;
+    float m = -INFINITY;             // the maximum P refers to (log2 units, of scaled scores): the same in both threads
+    F2 l2 = f2(0.f, 0.f);            // this thread's part of the sum
+    bool ok = true;                  // (a failed wait leaves the loop's barriers in step: both warps go on without waiting)
     for (int j = 0; j < kr.n; ++j) {
       const int buf = j % C::kBufs;
-      if (!(ok = warp_wait(s_full + buf, (j / C::kBufs) & 1, err, 68))) break;
+      ok = ok && warp_wait(s_full + buf, (j / C::kBufs) & 1, err, 68);
       tc_fence_after();
-      const uint32_t ts = tm + lanes + buf * 128;
-      float s[128];
-      tmem_ld128(ts, s);
+      const uint32_t ts = tm + lanes + buf * 128 + half * 64;
+      float s[64];
+      tmem_ld64(ts, s);
       const int c0 = kr.key(j);
       if (!all_visible(c0, p0, p1, pr.window, pr.sinks)) {
-        // visible: key <= p, and key > p - window or key < sinks
-        const int last = p - c0, from = p - pr.window + 1 - c0, sink = pr.sinks - c0;
+        const uint32_t v0 = visible_keys(c0 + half * 64, p, pr.window, pr.sinks);
+        const uint32_t v1 = visible_keys(c0 + half * 64 + 32, p, pr.window, pr.sinks);
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i > last || (i < from && i >= sink)) s[i] = -INFINITY;
+        for (int i = 0; i < 32; ++i) {
+          s[i] = (v0 >> i) & 1 ? s[i] : -INFINITY;
+          s[32 + i] = (v1 >> i) & 1 ? s[32 + i] : -INFINITY;
+        }
       }
       float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * pr.scale_log2;
-      const bool grow = top > m + kMaxGrowth;  // also the first finite maximum
-      if (__any_sync(0xffffffffu, grow)) {
-        const float next = grow ? top : m;
-        const float f = m == -INFINITY ? 0.f : ex2(m - next);
-        l *= f;
-        if (j > 0) {  // O of the tiles so far, once their products are done
-          if (!(ok = warp_wait(o_done, (j - 1) & 1, err, 69))) break;
-          tc_fence_after();
-          const float g = grow ? f : 1.f;
-#pragma unroll 1
-          for (int c = 0; c < NS * 64; c += 32) {
-            float v[32];
-            uint32_t u[32];
-            tmem_ld32(tm + lanes + C::kO + c, v);
+      for (int i = 4; i < 60; i += 8) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(v[i] * g);
-            tmem_st32(tm + lanes + C::kO + c, u);
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + 2 * e], s[i + 2 * e + 1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[60 + e]);
+      float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * pr.scale_log2;
+      // does a row of the two warps outgrow its reference (or meet its first visible key)?
+      uint32_t any;
+      asm volatile(
+          "{\n\t.reg .pred a, b;\n\t"
+          "setp.ne.u32 a, %1, 0;\n\t"
+          "barrier.cta.red.or.pred b, %2, 64, a;\n\t"
+          "selp.u32 %0, 1, 0, b;\n\t}\n"
+          : "=r"(any)
+          : "r"((uint32_t)(top > m + kMaxGrowth)), "r"(pair)
+          : "memory");
+      if (any) {
+        xchg[half * 128 + row] = top;
+        asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair) : "memory");
+        top = fmaxf(top, xchg[(half ^ 1) * 128 + row]);
+        const bool grow = top > m + kMaxGrowth;
+        const float next = grow ? top : m;
+        const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2(m - next);
+        l2 = mul2(l2, f2(f, f));
+        if (j > 0) {  // O of the tiles so far, once their products are done; half of its columns each
+          ok = ok && warp_wait(o_done, (j - 1) & 1, err, 69);
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = half * NS * 32; c < (half + 1) * NS * 32; c += 16) {
+            float v[16];
+            uint32_t u[16];
+            tmem_ld16(tm + lanes + C::kO + c, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[i] * f);
+            tmem_st16(tm + lanes + C::kO + c, u);
           }
         }
         m = next;
       }
       const float ref = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const F2 sc = f2(pr.scale_log2, pr.scale_log2), rf = f2(-ref, -ref);
+      F2 acc = f2(0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < 128; c += 32) {
+      for (int c = 0; c < 64; c += 32) {
         uint32_t u[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          const float a = ex2(fmaf(s[c + i], pr.scale_log2, -ref)), b = ex2(fmaf(s[c + i + 1], pr.scale_log2, -ref));
-          sum[i & 2] += a;
-          sum[(i & 2) + 1] += b;
+          float a, b;
+          unf2(fma2(f2(s[c + i], s[c + i + 1]), sc, rf), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          acc = add2(acc, f2(a, b));
           u[i / 2] = pack16<T>(a, b);
         }
-        tmem_st16(ts + c / 2, u);
+        tmem_st16(ts + c, u);  // over this thread's own columns, a piece of 32 keys every 32 words
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l2 = add2(l2, acc);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive_warp(p_full + buf);
     }
-    if (ok && kr.n > 0) {
-      ok = warp_wait(o_done, (kr.n - 1) & 1, err, 70);
+    if (kr.n > 0) {
+      ok = ok && warp_wait(o_done, (kr.n - 1) & 1, err, 70);
       tc_fence_after();
     }
+    float l, lb;
+    unf2(l2, l, lb);
+    l += lb;
+    xchg[half * 128 + row] = l;  // (every row had its exchanges of the loop before the last barrier there)
+    asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair) : "memory");
+    l = xchg[row] + xchg[128 + row];
     const int i = i0 + row;
     const bool live = i < sq.Tq;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN scores stay NaN
-    if (live) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m + log2f(l);
+    const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;  // a wait that gave up leaves NaN
+    if (live && half == 0) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m + log2f(l);
     T* out = o + (((long long)sq.b * pr.Tq + sq.q0 + i) * pr.H + h) * pr.D;
 #pragma unroll 1
-    for (int c = 0; c < NS * 64 && c < pr.D; c += 32) {
+    for (int c = half * NS * 32; c < (half + 1) * NS * 32; c += 32) {
       float v[32];
-      if (kr.n > 0) {
-        tmem_ld32(tm + lanes + C::kO + c, v);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = 0.f;
-      }
+      if (kr.n > 0) tmem_ld32(tm + lanes + C::kO + c, v);
       if (!live) continue;
 #pragma unroll
       for (int k = 0; k < 32; k += 8) {
@@ -236,9 +264,8 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
         uint32_t u[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          // a wait that gave up leaves NaN; a row without a visible key zeros
-          const float a = !ok ? NAN : l == 0.f ? 0.f : v[k + 2 * e] * inv, b = !ok ? NAN : l == 0.f ? 0.f : v[k + 2 * e + 1] * inv;
-          u[e] = pack16<T>(a, b);
+          const bool none = l == 0.f && ok;  // a row without a visible key: zeros, whatever O's columns hold
+          u[e] = none ? 0u : pack16<T>(v[k + 2 * e] * inv, v[k + 2 * e + 1] * inv);
         }
         *reinterpret_cast<uint4*>(out + c + k) = make_uint4(u[0], u[1], u[2], u[3]);
       }
@@ -246,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == kWarpsSm + 1) {
     tc_fence_after();
     tmem_dealloc(tm, C::kCols);
   }
