@@ -292,6 +292,45 @@ int gd_rotary(const void* q, const void* k, void* oq, void* ok, const float* tab
               int D, int R, long long q_stride_b, long long q_stride_t, long long q_stride_h, long long k_stride_b,
               long long k_stride_t, long long k_stride_h, int interleaved, int inverse, void* stream);
 
+/* ---- causal softmax attention with a sliding window and first tokens that stay visible ----
+ * The mixer of the layers that alternate with the rule's. Query i of Tq stands at position p = i + Tk - Tq and sees key j
+ * when j <= p and (j > p - window or j < sinks); window 0: no window. o = softmax(scale q k^T) v over the visible keys,
+ * zeros for a query that sees none. q [B, Tq, H, D], k, v [B, Tk, HK, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), H a
+ * multiple of HK (each key head serves H / HK consecutive query heads), D a multiple of 8 up to 256, read through
+ * `strides` (host array, elements: batch, token and head stride of q, k, v, and for the backward of d_o; multiples of 8,
+ * channels adjacent); o, dq [B, Tq, H, D] and dk, dv [B, Tk, HK, D] contiguous; every pointer 16-byte aligned. lse
+ * [B, H, Tq] fp32: log2 of the sum of the exponentials, for the backward. cu_seqlens (device int32 [N + 1], or NULL):
+ * packed rows, B = 1 and Tq = Tk, each sequence on its own; boundaries outside [0, Tq] or falling are clamped.
+ * The workspace starts with an error word (gd_read_error). A wait that gives up leaves NaN in the rows it was for. */
+
+/* Bytes of workspace gd_wattn_fwd (for_backward 0) or gd_wattn_bwd need (0 for invalid sizes); packed: with cu_seqlens. */
+size_t gd_wattn_workspace_bytes(int B, int Tq, int Tk, int H, int HK, int D, int window, int sinks, int packed,
+                                int for_backward);
+
+/* o_low (for the backward; NULL otherwise): what o's rounding took away, in `dtype`, with o's shape. */
+int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, const int* cu_seqlens,
+                 int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D, const long long* strides, int window, int sinks, float scale,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* dq, dk, dv from the forward's inputs, o, o_low and lse, and d_o. dk and dv are summed over the query heads of a key head in a
+ * fixed order (no atomics: the same bits every run). */
+int gd_wattn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse,
+                 const void* d_o, void* dq, void* dk, void* dv, const int* cu_seqlens, int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D,
+                 const long long* strides, int window, int sinks, float scale, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* The single-token form over a cache: request b's new token stands at position p = lengths[b] (device int32; negative:
+ * idle, zeros, nothing stored). Stores its key and value rows k, v [B, HK, D] in their slot of k_cache, v_cache
+ * [B, S, HK, D] (strides: host array, elements, batch, slot and head stride of both) and writes o [B, H, D] = the
+ * attention of q [B, H, D] over the visible positions, the new one included. Position j stands in slot j while j < S, then
+ * in slot sinks + (j - sinks) mod (S - sinks), so the cache may roll; once p >= S the last S - sinks positions at most are
+ * visible besides the first tokens. The workspace (gd_wattn_step_workspace_bytes(), 0 for most sizes) need not be
+ * initialised. */
+size_t gd_wattn_step_workspace_bytes(int B, int S, int H, int HK, int D, int window, int sinks);
+int gd_wattn_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache, const int* lengths, void* o,
+                  int dtype, int B, int S, int H, int HK, int D, const long long* strides, int window, int sinks,
+                  float scale, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -96,28 +96,30 @@ extern "C" size_t gd_wattn_workspace_bytes(int B, int Tq, int Tk, int H, int HK,
   return delta_at() + delta_bytes(B, Tq, H) + part_bytes(c, B, HK, D);
 }
 
-extern "C" int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu_seqlens,
-                            int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D, const long long* strides,
+extern "C" int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse,
+                            const int* cu_seqlens, int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D, const long long* strides,
                             int window, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int st = check(q, k, v, strides, cu_seqlens, N, dtype, B, Tq, Tk, H, HK, D, window, sinks, scale)) return st;
   if (B == 0 || Tq == 0) return GD_OK;
   if (o == nullptr || lse == nullptr) return GD_ERR_ARG;
-  if (!aligned16(o) || !aligned16(workspace)) return GD_ERR_ALIGN;
+  if (!aligned16(o) || !aligned16(o_low) || !aligned16(workspace)) return GD_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < sizeof(ErrorWord)) return GD_ERR_WORKSPACE;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   if (cudaMemsetAsync(workspace, 0, sizeof(ErrorWord), cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const Problem p = problem(cu_seqlens, N, B, Tq, Tk, H, HK, D, window, sinks, scale);
   if (Tk == 0) {  // no keys at all: zeros
-    if (cudaMemsetAsync(o, 0, (size_t)B * Tq * H * D * 2, cs) != cudaSuccess ||
+    const size_t n = (size_t)B * Tq * H * D * 2;
+    if (cudaMemsetAsync(o, 0, n, cs) != cudaSuccess ||
+        (o_low != nullptr && cudaMemsetAsync(o_low, 0, n, cs) != cudaSuccess) ||
         cudaMemsetAsync(lse, 0x7f, (size_t)B * H * Tq * sizeof(float), cs) != cudaSuccess)  // 3.4e38: as good as +inf
       return (cudaGetLastError(), GD_ERR_LAUNCH);
     return GD_OK;
   }
-  return gd::wattn::forward(q, k, v, strides, p, dtype, o, lse, static_cast<ErrorWord*>(workspace), cs);
+  return gd::wattn::forward(q, k, v, strides, p, dtype, o, o_low, lse, static_cast<ErrorWord*>(workspace), cs);
 }
 
-extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o,
-                            void* dq, void* dk, void* dv, const int* cu_seqlens, int N, int dtype, int B, int Tq, int Tk,
+extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low,
+                            const float* lse, const void* d_o, void* dq, void* dk, void* dv, const int* cu_seqlens, int N, int dtype, int B, int Tq, int Tk,
                             int H, int HK, int D, const long long* strides, int window, int sinks, float scale,
                             void* workspace, size_t workspace_bytes, void* stream) {
   if (const int st = check(q, k, v, strides, cu_seqlens, N, dtype, B, Tq, Tk, H, HK, D, window, sinks, scale)) return st;
@@ -130,8 +132,8 @@ extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const v
       return (cudaGetLastError(), GD_ERR_LAUNCH);
     return GD_OK;
   }
-  if (o == nullptr || lse == nullptr || d_o == nullptr || dq == nullptr || dk == nullptr || dv == nullptr) return GD_ERR_ARG;
-  if (!aligned16(o) || !aligned16(d_o) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(workspace))
+  if (o == nullptr || o_low == nullptr || lse == nullptr || d_o == nullptr || dq == nullptr || dk == nullptr || dv == nullptr) return GD_ERR_ARG;
+  if (!aligned16(o) || !aligned16(o_low) || !aligned16(d_o) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(workspace))
     return GD_ERR_ALIGN;
   if (!strides_ok(strides + 9, B, Tq, H)) return GD_ERR_ALIGN;
   if (workspace == nullptr ||
@@ -141,7 +143,7 @@ extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const v
   const Problem p = problem(cu_seqlens, N, B, Tq, Tk, H, HK, D, window, sinks, scale);
   const Cut c = cu_seqlens != nullptr ? Cut{0, 1} : cut_of(B, Tq, Tk, H, HK, D, p.window, p.sinks);
   char* ws = static_cast<char*>(workspace);
-  return gd::wattn::backward(q, k, v, o, d_o, strides, p, dtype, lse, reinterpret_cast<float*>(ws + delta_at()), dq, dk, dv,
+  return gd::wattn::backward(q, k, v, o, o_low, d_o, strides, p, dtype, lse, reinterpret_cast<float*>(ws + delta_at()), dq, dk, dv,
                              c.heavy, c.parts, reinterpret_cast<float*>(ws + delta_at() + delta_bytes(B, Tq, H)),
                              static_cast<ErrorWord*>(workspace), cs);
 }

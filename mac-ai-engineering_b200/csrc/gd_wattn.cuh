@@ -292,11 +292,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
       : "memory");
 }
 
-// The entry points' parts (host): strides of q, k, v in elements, (batch, token, head) each
+template <typename T>
+__device__ __forceinline__ float2 unpack16(uint32_t u) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+
+// The entry points' parts (host): strides of q, k, v in elements, (batch, token, head) each; low: what o's rounding took
+// away (may be NULL in the forward)
 int forward(const void* q, const void* k, const void* v, const long long* strides, const Problem& pr, int dtype, void* o,
-            float* lse, ErrorWord* err, cudaStream_t stream);
+            void* low, float* lse, ErrorWord* err, cudaStream_t stream);
 // (and of dO: strides[9 .. 11]); the first `heavy` key tiles are cut into `parts` CTAs with fp32 partial tiles at `part`
-int backward(const void* q, const void* k, const void* v, const void* o, const void* g, const long long* strides,
+int backward(const void* q, const void* k, const void* v, const void* o, const void* low, const void* g, const long long* strides,
              const Problem& pr, int dtype, const float* lse, float* delta, void* dq, void* dk, void* dv, int heavy,
              int parts, float* part, ErrorWord* err, cudaStream_t stream);
 

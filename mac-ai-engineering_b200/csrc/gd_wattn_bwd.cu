@@ -30,45 +30,55 @@ __device__ __forceinline__ float ds_scale(const ErrorWord* err) {
   return __int_as_float((127 + (e > 100 ? 100 : e)) << 23);
 }
 
-// ---- delta: 16 lanes a row of [B, Tq, H]
+// ---- delta = rowsum(dO O), O as its 16-bit value and what its rounding took away (delta and dP nearly cancel in rows
+// that see few keys: O's rounding alone would cost dS half a bit there). 16 lanes a row of [B, Tq, H], kRowsEach rows in
+// flight. HBM-bound: three reads of [B, Tq, H, D].
+constexpr int kRowsEach = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, const T* __restrict__ g, long long gb,
-                                                    long long gt, long long gh, float* __restrict__ delta, int B, int Tq,
-                                                    int H, int D, ErrorWord* err) {
-  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4, rows = (long long)B * Tq * H;
+__global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, const T* __restrict__ low,
+                                                    const T* __restrict__ g, long long gb, long long gt, long long gh,
+                                                    float* __restrict__ delta, int B, int Tq, int H, int D, ErrorWord* err) {
   const int sub = threadIdx.x & 15;
-  float s = 0.f, top = 0.f;
-  int h = 0, t = 0;
-  long long b = 0;
-  if (row < rows) {
-    h = (int)(row % H);
-    const long long bt = row / H;
-    b = bt / Tq;
-    t = (int)(bt - b * Tq);
-    const T* po = o + row * D;
-    const T* pg = g + b * gb + t * gt + h * gh;
-    for (int c = sub * 8; c < D; c += 128) {
-      const uint4 a = *reinterpret_cast<const uint4*>(po + c), d = *reinterpret_cast<const uint4*>(pg + c);
-      const uint32_t ua[4] = {a.x, a.y, a.z, a.w}, ud[4] = {d.x, d.y, d.z, d.w};
+  const long long rows = (long long)B * Tq * H, row0 = (long long)blockIdx.x * (16 * kRowsEach) + (threadIdx.x >> 4);
+  float s[kRowsEach], top = 0.f;
+  long long to[kRowsEach];
+#pragma unroll
+  for (int r = 0; r < kRowsEach; ++r) s[r] = 0.f;
+  for (int c = sub * 8; c < D; c += 128) {
+    uint4 a[kRowsEach], l[kRowsEach], d[kRowsEach];
+#pragma unroll
+    for (int r = 0; r < kRowsEach; ++r) {
+      const long long row = row0 + r * 16;
+      a[r] = l[r] = d[r] = make_uint4(0, 0, 0, 0);
+      if (row < rows) {
+        const unsigned h = (unsigned)(row % H);
+        const long long bt = row / H, b = bt / Tq, t = bt - b * Tq;
+        to[r] = (b * H + h) * Tq + t;
+        a[r] = __ldg(reinterpret_cast<const uint4*>(o + row * D + c));
+        l[r] = __ldg(reinterpret_cast<const uint4*>(low + row * D + c));
+        d[r] = __ldg(reinterpret_cast<const uint4*>(g + b * gb + t * gt + h * gh + c));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRowsEach; ++r) {
+      const uint32_t ua[4] = {a[r].x, a[r].y, a[r].z, a[r].w}, ul[4] = {l[r].x, l[r].y, l[r].z, l[r].w},
+                     ud[4] = {d[r].x, d[r].y, d[r].z, d[r].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float2 x, y;
-        if constexpr (std::is_same<T, __half>::value) {
-          x = __half22float2(*reinterpret_cast<const __half2*>(ua + i));
-          y = __half22float2(*reinterpret_cast<const __half2*>(ud + i));
-          top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
-        } else {
-          x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(ua + i));
-          y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(ud + i));
-        }
-        s = fmaf(x.x, y.x, s);
-        s = fmaf(x.y, y.y, s);
+        const float2 x = unpack16<T>(ua[i]), z = unpack16<T>(ul[i]), y = unpack16<T>(ud[i]);
+        if constexpr (std::is_same<T, __half>::value) top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+        s[r] = fmaf(x.x + z.x, y.x, s[r]);
+        s[r] = fmaf(x.y + z.y, y.y, s[r]);
       }
     }
   }
 #pragma unroll
-  for (int w = 8; w >= 1; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-  if (row < rows && sub == 0) delta[(b * H + h) * Tq + t] = s;
+  for (int r = 0; r < kRowsEach; ++r) {
+#pragma unroll
+    for (int w = 8; w >= 1; w >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], w);
+    if (row0 + r * 16 < rows && sub == 0) delta[to[r]] = s[r];
+  }
   if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
     for (int w = 16; w >= 1; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
@@ -788,7 +798,7 @@ __global__ void __launch_bounds__(256) sum_parts(const float* __restrict__ part,
 }
 
 template <typename T, int NS>
-int launch(const void* q, const void* k, const void* v, const void* o, const void* g, const long long* st,
+int launch(const void* q, const void* k, const void* v, const void* o, const void* low, const void* g, const long long* st,
            const Problem& pr, const float* lse, float* delta, void* dq, void* dk, void* dv, Split sp, ErrorWord* err,
            cudaStream_t stream) {
   CUtensorMap mq, mk, mv, mo;
@@ -799,9 +809,9 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
       !tile_map(&mo, g, dt, pr.B, pr.Tq, pr.H, pr.D, st[9], st[10], st[11], kTile))
     return GD_ERR_LAUNCH;
   const long long rows = (long long)pr.B * pr.Tq * pr.H;
-  delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(static_cast<const T*>(o), static_cast<const T*>(g),
-                                                                   st[9], st[10], st[11], delta, pr.B, pr.Tq, pr.H, pr.D,
-                                                                   err);
+  delta_kernel<T><<<(unsigned)((rows + 16 * kRowsEach - 1) / (16 * kRowsEach)), 256, 0, stream>>>(
+      static_cast<const T*>(o), static_cast<const T*>(low), static_cast<const T*>(g), st[9], st[10], st[11], delta, pr.B,
+      pr.Tq, pr.H, pr.D, err);
   static bool done_q[kMaxDevices], done_kv[kMaxDevices];
   auto kq = dq_kernel<T, NS>;
   auto kkv = dkv_kernel<T, NS>;
@@ -821,12 +831,12 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
 
 }  // namespace
 
-int backward(const void* q, const void* k, const void* v, const void* o, const void* g, const long long* strides,
+int backward(const void* q, const void* k, const void* v, const void* o, const void* low, const void* g, const long long* strides,
              const Problem& pr, int dtype, const float* lse, float* delta, void* dq, void* dk, void* dv, int heavy,
              int parts, float* part, ErrorWord* err, cudaStream_t stream) {
   const Split sp = {heavy, parts, part};
   auto run = [&](auto t, auto ns) {
-    return launch<decltype(t), decltype(ns)::value>(q, k, v, o, g, strides, pr, lse, delta, dq, dk, dv, sp, err, stream);
+    return launch<decltype(t), decltype(ns)::value>(q, k, v, o, low, g, strides, pr, lse, delta, dq, dk, dv, sp, err, stream);
   };
   auto by_width = [&](auto t) {
     return pr.D <= 64    ? run(t, std::integral_constant<int, 1>{})

@@ -37,7 +37,8 @@ struct Cfg {
 template <typename T, int NS>
 __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-               const __grid_constant__ CUtensorMap mv, const Problem pr, T* __restrict__ o, float* __restrict__ lse,
+               const __grid_constant__ CUtensorMap mv, const Problem pr, T* __restrict__ o, T* __restrict__ o_low,
+               float* __restrict__ lse,
                ErrorWord* err) {
   using C = Cfg<NS>;
   extern __shared__ uint8_t smem_raw[];
@@ -252,7 +253,8 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     const bool live = i < sq.Tq;
     const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;  // a wait that gave up leaves NaN
     if (live && half == 0) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m + log2f(l);
-    T* out = o + (((long long)sq.b * pr.Tq + sq.q0 + i) * pr.H + h) * pr.D;
+    const long long at = (((long long)sq.b * pr.Tq + sq.q0 + i) * pr.H + h) * pr.D;
+    const bool none = l == 0.f && ok;  // a row without a visible key: zeros, whatever O's columns hold
 #pragma unroll 1
     for (int c = half * NS * 32; c < (half + 1) * NS * 32; c += 32) {
       float v[32];
@@ -261,13 +263,17 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
 #pragma unroll
       for (int k = 0; k < 32; k += 8) {
         if (c + k >= pr.D) break;
-        uint32_t u[4];
+        uint32_t u[4], w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool none = l == 0.f && ok;  // a row without a visible key: zeros, whatever O's columns hold
-          u[e] = none ? 0u : pack16<T>(v[k + 2 * e] * inv, v[k + 2 * e + 1] * inv);
+          const float a = none ? 0.f : v[k + 2 * e] * inv, b = none ? 0.f : v[k + 2 * e + 1] * inv;
+          u[e] = pack16<T>(a, b);
+          const float2 r = unpack16<T>(u[e]);
+          w[e] = pack16<T>(a - r.x, b - r.y);
         }
-        *reinterpret_cast<uint4*>(out + c + k) = make_uint4(u[0], u[1], u[2], u[3]);
+        *reinterpret_cast<uint4*>(o + at + c + k) = make_uint4(u[0], u[1], u[2], u[3]);
+        // what the rounding took away, for the backward's delta
+        if (o_low != nullptr) *reinterpret_cast<uint4*>(o_low + at + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   }
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
 }
 
 template <typename T, int NS>
-int launch(const void* q, const void* k, const void* v, const long long* st, const Problem& pr, void* o, float* lse,
+int launch(const void* q, const void* k, const void* v, const long long* st, const Problem& pr, void* o, void* low, float* lse,
            ErrorWord* err, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
   if (!tile_map(&mq, q, map_dtype<T>(), pr.B, pr.Tq, pr.H, pr.D, st[0], st[1], st[2], kTile) ||
@@ -292,21 +298,21 @@ int launch(const void* q, const void* k, const void* v, const long long* st, con
   if (set_smem_once(kern, Cfg<NS>::kSmem, done) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const long long tiles = pr.cu ? (long long)pr.Tq / kTile + pr.N : (pr.Tq + kTile - 1) / kTile;
   const dim3 grid((unsigned)tiles, (unsigned)pr.H, (unsigned)pr.B);
-  kern<<<grid, kThreads, Cfg<NS>::kSmem, stream>>>(mq, mk, mv, pr, static_cast<T*>(o), lse, err);
+  kern<<<grid, kThreads, Cfg<NS>::kSmem, stream>>>(mq, mk, mv, pr, static_cast<T*>(o), static_cast<T*>(low), lse, err);
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
 }
 
 }  // namespace
 
 int forward(const void* q, const void* k, const void* v, const long long* strides, const Problem& pr, int dtype, void* o,
-            float* lse, ErrorWord* err, cudaStream_t stream) {
+            void* low, float* lse, ErrorWord* err, cudaStream_t stream) {
   if (dtype == GD_FLOAT16)
-    return pr.D <= 64    ? launch<__half, 1>(q, k, v, strides, pr, o, lse, err, stream)
-           : pr.D <= 128 ? launch<__half, 2>(q, k, v, strides, pr, o, lse, err, stream)
-                         : launch<__half, 4>(q, k, v, strides, pr, o, lse, err, stream);
-  return pr.D <= 64    ? launch<__nv_bfloat16, 1>(q, k, v, strides, pr, o, lse, err, stream)
-         : pr.D <= 128 ? launch<__nv_bfloat16, 2>(q, k, v, strides, pr, o, lse, err, stream)
-                       : launch<__nv_bfloat16, 4>(q, k, v, strides, pr, o, lse, err, stream);
+    return pr.D <= 64    ? launch<__half, 1>(q, k, v, strides, pr, o, low, lse, err, stream)
+           : pr.D <= 128 ? launch<__half, 2>(q, k, v, strides, pr, o, low, lse, err, stream)
+                         : launch<__half, 4>(q, k, v, strides, pr, o, low, lse, err, stream);
+  return pr.D <= 64    ? launch<__nv_bfloat16, 1>(q, k, v, strides, pr, o, low, lse, err, stream)
+         : pr.D <= 128 ? launch<__nv_bfloat16, 2>(q, k, v, strides, pr, o, low, lse, err, stream)
+                       : launch<__nv_bfloat16, 4>(q, k, v, strides, pr, o, low, lse, err, stream);
 }
 
 }  // namespace wattn

@@ -1,0 +1,38 @@
+"""How the operators of the softmax-attention layer's steps reach the C ABI: on the tensor's device and its current
+stream, with as little host work as a call of a few microseconds can bear (a device guard only when another device is
+current)."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle without the Stream object around it
+
+
+def launch(name: str, index: int, *args) -> None:
+    """lib.<name>(*args, stream) with device `index` current; a failure status raises GatedDeltaError."""
+    fn = getattr(_lib.load(), name)
+    if index == torch.cuda.current_device():
+        st = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, _raw_stream(index))
+    if st:
+        _lib.check(st, name)
+
+
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous with a 16-byte aligned start (a copy only when the view is not)."""
+    if not t.is_contiguous():
+        return t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def recorded(*ts) -> bool:
+    """Whether autograd records a call with these inputs (None allowed)."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False

@@ -31,7 +31,8 @@ EXPORTS = ("gd_status_string", "gd_workspace_bytes", "gd_prep", "gd_fwd_state", 
            "gd_gates_workspace_bytes", "gd_gates_bwd", "gd_gnorm_fwd", "gd_gnorm_workspace_bytes", "gd_gnorm_bwd",
            "gd_conv_fwd", "gd_conv_workspace_bytes", "gd_conv_bwd", "gd_workspace_bytes_packed", "gd_forward_packed",
            "gd_backward_packed", "gd_rnorm_fwd", "gd_rnorm_fp8", "gd_rnorm_workspace_bytes", "gd_rnorm_bwd",
-           "gd_rotary", "gd_wattn_workspace_bytes", "gd_wattn_fwd", "gd_wattn_bwd")
+           "gd_rotary", "gd_wattn_workspace_bytes", "gd_wattn_fwd", "gd_wattn_bwd",
+           "gd_wattn_step_workspace_bytes", "gd_wattn_step")
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -66,8 +67,10 @@ _SIGS = {
     "gd_rnorm_workspace_bytes": ([_LL, _I], _SZ),
     "gd_rnorm_bwd": ([_P] * 6 + [_I, _I, _I, _LL, _I, ctypes.c_float, _P, _SZ, _P], _I),
     "gd_wattn_workspace_bytes": ([_I] * 10, _SZ),
-    "gd_wattn_fwd": ([_P] * 6 + [_I] * 8 + [ctypes.POINTER(_LL), _I, _I, ctypes.c_float, _P, _SZ, _P], _I),
-    "gd_wattn_bwd": ([_P] * 10 + [_I] * 8 + [ctypes.POINTER(_LL), _I, _I, ctypes.c_float, _P, _SZ, _P], _I),
+    "gd_wattn_fwd": ([_P] * 7 + [_I] * 8 + [ctypes.POINTER(_LL), _I, _I, ctypes.c_float, _P, _SZ, _P], _I),
+    "gd_wattn_bwd": ([_P] * 11 + [_I] * 8 + [ctypes.POINTER(_LL), _I, _I, ctypes.c_float, _P, _SZ, _P], _I),
+    "gd_wattn_step_workspace_bytes": ([_I] * 7, _SZ),
+    "gd_wattn_step": ([_P] * 7 + [_I] * 6 + [ctypes.POINTER(_LL), _I, _I, ctypes.c_float, _P, _SZ, _P], _I),
     "gd_rotary": ([_P] * 6 + [_I, _LL, _LL] + [_I] * 7 + [_LL] * 6 + [_I, _I, _P], _I),
 }
 

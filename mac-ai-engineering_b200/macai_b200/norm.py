@@ -15,8 +15,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._call import aligned, launch, recorded
 
 _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 MAX_CHUNKS = 2048  # 16-byte chunks of a row (a width that fills no whole number of them takes two more)
@@ -26,102 +28,71 @@ def supported(x, residual, weight) -> bool:
     """The cases the kernels take: x [..., D] (and the residual, of its shape and dtype) in float32, float16 or
     bfloat16; weight [D] in x's dtype or float32; CUDA tensors; D up to 16,384 at 16 bits (16,375 where it is not a
     multiple of 8) and 8,192 at float32 (8,187 where it is not a multiple of 4)."""
-    ts = (x, weight) if residual is None else (x, residual, weight)
-    if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in ts) or x.dim() == 0 or x.dtype not in _DTYPES:
+    if not (isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor)) or not x.is_cuda or x.dim() == 0:
         return False
-    d = x.shape[-1]
-    e = 4 if x.dtype == torch.float32 else 8
-    chunks = d // e if d % e == 0 else d // e + 2
-    return (0 < d and chunks <= MAX_CHUNKS and weight.dim() == 1 and weight.shape[0] == d
-            and weight.dtype in (x.dtype, torch.float32) and weight.device == x.device
-            and (residual is None or (residual.dtype == x.dtype and residual.shape == x.shape
-                                      and residual.device == x.device)))
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous with a 16-byte aligned start (a copy only when the view is not)."""
-    if not t.is_contiguous():
-        t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _p(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    dt, d, index = x.dtype, x.shape[-1], x.get_device()
+    if dt not in _DTYPES or d == 0:
+        return False
+    e = 4 if dt == torch.float32 else 8
+    if (d // e if d % e == 0 else d // e + 2) > MAX_CHUNKS:
+        return False
+    if weight.shape != (d,) or (weight.dtype != dt and weight.dtype != torch.float32) or weight.get_device() != index:
+        return False
+    return residual is None or (isinstance(residual, torch.Tensor) and residual.dtype == dt
+                                and residual.shape == x.shape and residual.get_device() == index)
 
 
 def _fwd(x, residual, w, eps, zero_centered):
+    """(y, s) on aligned inputs; s is None without a residual."""
     y = torch.empty_like(x)
-    s = torch.empty_like(x) if residual is not None else x.new_empty(0)
+    s = None if residual is None else torch.empty_like(x)
     d = x.shape[-1]
-    with torch.cuda.device(x.device):
-        st = _lib.load().gd_rnorm_fwd(x.data_ptr(), _p(residual), w.data_ptr(),
-                                      s.data_ptr() if residual is not None else None, y.data_ptr(), _DTYPES[x.dtype],
-                                      _DTYPES[w.dtype], zero_centered, x.numel() // d, d, eps,
-                                      torch.cuda.current_stream(x.device).cuda_stream)
-    if st:
-        _lib.check(st, "gd_rnorm_fwd")
+    launch("gd_rnorm_fwd", x.get_device(), x.data_ptr(), None if residual is None else residual.data_ptr(), w.data_ptr(),
+           None if s is None else s.data_ptr(), y.data_ptr(), _DTYPES[x.dtype], _DTYPES[w.dtype], zero_centered,
+           x.numel() // d, d, eps)
     return y, s
 
 
-@torch.library.custom_op("macai_b200::rnorm_fwd", mutates_args=(), device_types="cuda")
-def rnorm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], w: torch.Tensor, eps: float,
-              zero_centered: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """(y, s) in x's dtype and shape; s is empty without a residual."""
-    return _fwd(x, residual, w, eps, zero_centered)
-
-
-@rnorm_fwd.register_fake
-def _(x, residual, w, eps, zero_centered):
-    return torch.empty_like(x), torch.empty_like(x) if residual is not None else x.new_empty(0)
-
-
-@torch.library.custom_op("macai_b200::rnorm_bwd", mutates_args=(), device_types="cuda")
-def rnorm_bwd(s: torch.Tensor, w: torch.Tensor, dy: Optional[torch.Tensor], ds: Optional[torch.Tensor], eps: float,
-              zero_centered: bool, need_dw: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """(dx, dw): dx like s (of x and of the residual), dw an empty tensor unless asked for; a None cotangent is zero."""
-    lib = _lib.load()
+def _bwd(s, w, dy, ds, eps, zero_centered, need_dw):
+    """(dx, dw); dw None unless asked for."""
     d = s.shape[-1]
     rows = s.numel() // d
     dx = torch.empty_like(s)
-    dw = torch.empty_like(w) if need_dw else w.new_empty(0)
-    ws, nbytes = None, 0
+    dw = ws = None
+    nbytes = 0
     if need_dw:
-        nbytes = lib.gd_rnorm_workspace_bytes(rows, d)
+        dw = torch.empty_like(w)
+        nbytes = _lib.load().gd_rnorm_workspace_bytes(rows, d)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
-    with torch.cuda.device(s.device):
-        st = lib.gd_rnorm_bwd(s.data_ptr(), w.data_ptr(), _p(dy), _p(ds), dx.data_ptr(),
-                              dw.data_ptr() if need_dw else None, _DTYPES[s.dtype], _DTYPES[w.dtype], zero_centered,
-                              rows, d, eps, _p(ws), nbytes, torch.cuda.current_stream(s.device).cuda_stream)
-    _lib.check(st, "gd_rnorm_bwd")
+    launch("gd_rnorm_bwd", s.get_device(), s.data_ptr(), w.data_ptr(), None if dy is None else dy.data_ptr(),
+           None if ds is None else ds.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(), _DTYPES[s.dtype],
+           _DTYPES[w.dtype], zero_centered, rows, d, eps, None if ws is None else ws.data_ptr(), nbytes)
     return dx, dw
 
 
-@rnorm_bwd.register_fake
-def _(s, w, dy, ds, eps, zero_centered, need_dw):
-    return torch.empty_like(s), w.new_empty(w.shape[0] if need_dw else 0)
+class AddRMSNorm(torch.autograd.Function):
+    """`AddRMSNorm.apply(x, residual or None, w, eps, zero_centered)` on aligned inputs: (y, s), or y without a residual."""
 
+    @staticmethod
+    def forward(ctx, x, residual, w, eps, zero_centered):
+        y, s = _fwd(x, residual, w, eps, zero_centered)
+        ctx.save_for_backward(x if s is None else s, w)
+        ctx.args = (eps, zero_centered, s is not None)
+        ctx.set_materialize_grads(False)
+        return y if s is None else (y, s)
 
-def _setup_context(ctx, inputs, output):
-    x, residual, w, eps, zero_centered = inputs
-    ctx.save_for_backward(x if residual is None else output[1], w)
-    ctx.eps, ctx.zero_centered, ctx.has_residual = eps, zero_centered, residual is not None
-    ctx.set_materialize_grads(False)
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, w = ctx.saved_tensors
+        eps, zero_centered, has_residual = ctx.args
+        if dy is None and ds is None:
+            return None, None, None, None, None
+        need_dw = ctx.needs_input_grad[2] and dy is not None
+        dx, dw = _bwd(s, w, None if dy is None else aligned(dy), None if ds is None else aligned(ds), eps, zero_centered,
+                      need_dw)
+        return dx, (dx if has_residual else None), dw, None, None
 
-
-def _backward(ctx, dy, ds):
-    s, w = ctx.saved_tensors
-    if not ctx.has_residual:
-        ds = None  # the empty second output
-    if dy is None and ds is None:
-        return None, None, None, None, None
-    need_dw = bool(ctx.needs_input_grad[2]) and dy is not None
-    dy = None if dy is None else _aligned(dy.to(s.dtype))
-    ds = None if ds is None else _aligned(ds.to(s.dtype))
-    dx, dw = rnorm_bwd(s, w, dy, ds, ctx.eps, ctx.zero_centered, need_dw)
-    return dx, (dx if ctx.has_residual else None), (dw if need_dw else None), None, None
-
-
-rnorm_fwd.register_autograd(_backward, setup_context=_setup_context)
 
 _REFUSED = ("x [..., D] and the residual must be CUDA tensors of one float dtype and shape, the weight [D] in x's dtype "
             "or float32, D at most 16,384 (16 bits) or 8,192 (float32); there is no CPU path")
@@ -132,12 +103,13 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     """(y, s) = the RMS norm of s = x + residual, and s. Without a residual s is x itself."""
     if not supported(x, residual, weight):
         raise ValueError("add_rms_norm: " + _REFUSED)
-    x_, w = _aligned(x), _aligned(weight)
-    r = None if residual is None else _aligned(residual)
-    recorded = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                            or (r is not None and r.requires_grad))
-    y, s = (rnorm_fwd if recorded or torch.compiler.is_compiling() else _fwd)(x_, r, w, float(eps), bool(zero_centered))
-    return y, (x if residual is None else s)
+    x_, w = aligned(x), aligned(weight)
+    r = None if residual is None else aligned(residual)
+    if recorded(x, residual, weight):
+        out = AddRMSNorm.apply(x_, r, w, float(eps), bool(zero_centered))
+        return (out, x) if r is None else out
+    y, s = _fwd(x_, r, w, float(eps), bool(zero_centered))
+    return y, (x if r is None else s)
 
 
 def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
@@ -149,19 +121,15 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
         raise ValueError("add_rms_norm_fp8: " + _REFUSED)
     if group is not None and (group <= 0 or group % 8):
         raise ValueError(f"add_rms_norm_fp8: group must be a positive multiple of 8 or None, got {group}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+    if recorded(x, residual, weight):
         raise RuntimeError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad(), or add_rms_norm")
-    x_, w = _aligned(x), _aligned(weight)
-    r = None if residual is None else _aligned(residual)
+    x_, w = aligned(x), aligned(weight)
+    r = None if residual is None else aligned(residual)
     d = x.shape[-1]
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty((*x.shape[:-1], -(-d // group) if group else 1), dtype=torch.float32, device=x.device)
     s = x if r is None else torch.empty_like(x_)
-    with torch.cuda.device(x.device):
-        st = _lib.load().gd_rnorm_fp8(x_.data_ptr(), _p(r), w.data_ptr(), None if r is None else s.data_ptr(),
-                                      q.data_ptr(), scale.data_ptr(), _DTYPES[x.dtype], _DTYPES[w.dtype],
-                                      bool(zero_centered), x.numel() // d, d, group or 0, float(eps),
-                                      torch.cuda.current_stream(x.device).cuda_stream)
-    if st:
-        _lib.check(st, "gd_rnorm_fp8")
+    launch("gd_rnorm_fp8", x.get_device(), x_.data_ptr(), None if r is None else r.data_ptr(), w.data_ptr(),
+           None if r is None else s.data_ptr(), q.data_ptr(), scale.data_ptr(), _DTYPES[x.dtype], _DTYPES[w.dtype],
+           bool(zero_centered), x.numel() // d, d, group or 0, float(eps))
     return q, scale, s

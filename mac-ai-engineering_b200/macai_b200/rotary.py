@@ -15,8 +15,10 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._call import launch, recorded
 
 _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 
@@ -69,65 +71,53 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, scaling: Optio
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
 def _turn(q, k, table, positions, interleaved, inverse):
+    """(q, k) turned, contiguous; None for a k of None."""
+    q = _rows(q)
     B, T, H, D = q.shape
+    qb, qt, qh, _ = q.stride()
     oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if k is None:
-        ok, kp, okp, HK, ks = q.new_empty(0), None, None, 0, (0, 0, 0)
-    else:
+    ok = kp = okp = None
+    HK = kb = kt = kh = 0
+    if k is not None:
+        k = _rows(k)
         ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        kp, okp, HK, ks = k.data_ptr(), ok.data_ptr(), k.shape[2], k.stride()
-    qs = q.stride()
+        kp, okp, HK = k.data_ptr(), ok.data_ptr(), k.shape[2]
+        kb, kt, kh, _ = k.stride()
     pp, p64, pb = None, 0, 0
     if positions is not None:
         pp, p64 = positions.data_ptr(), positions.dtype == torch.int64
         pb = T if positions.dim() == 2 else 0
-    with torch.cuda.device(q.device):
-        st = _lib.load().gd_rotary(q.data_ptr(), kp, oq.data_ptr(), okp, table.data_ptr(), pp, p64, pb, table.shape[0],
-                                   _DTYPES[q.dtype], B, T, H, HK, D, 2 * table.shape[1], qs[0], qs[1], qs[2], ks[0],
-                                   ks[1], ks[2], interleaved, inverse,
-                                   torch.cuda.current_stream(q.device).cuda_stream)
-    if st:
-        _lib.check(st, "gd_rotary")
+    launch("gd_rotary", q.get_device(), q.data_ptr(), kp, oq.data_ptr(), okp, table.data_ptr(), pp, p64, pb,
+           table.shape[0], _DTYPES[q.dtype], B, T, H, HK, D, 2 * table.shape[1], qb, qt, qh, kb, kt, kh, interleaved,
+           inverse)
     return oq, ok
 
 
-@torch.library.custom_op("macai_b200::rotary", mutates_args=(), device_types="cuda")
-def rotary_op(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, positions: Optional[torch.Tensor],
-              interleaved: bool, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """(q, k) turned (contiguous); k's place is an empty tensor without it."""
-    return _turn(_rows(q), None if k is None else _rows(k), table, positions, interleaved, inverse)
+class Rotary(torch.autograd.Function):
+    """`Rotary.apply(q, k or None, table, positions or None, interleaved)`: (q, k), or q without a k."""
 
+    @staticmethod
+    def forward(ctx, q, k, table, positions, interleaved):
+        ctx.save_for_backward(table, positions)
+        ctx.interleaved, ctx.has_k = interleaved, k is not None
+        ctx.set_materialize_grads(False)
+        oq, ok = _turn(q, k, table, positions, interleaved, False)
+        return oq if k is None else (oq, ok)
 
-@rotary_op.register_fake
-def _(q, k, table, positions, interleaved, inverse):
-    return q.new_empty(q.shape), q.new_empty(0 if k is None else k.shape)
-
-
-def _setup_context(ctx, inputs, output):
-    q, k, table, positions, interleaved, inverse = inputs
-    ctx.save_for_backward(table, positions)
-    ctx.flags = (interleaved, inverse, k is not None)
-    ctx.set_materialize_grads(False)
-
-
-def _backward(ctx, dq, dk):
-    table, positions = ctx.saved_tensors
-    interleaved, inverse, has_k = ctx.flags
-    if not has_k:
-        dk = None  # the empty second output
-    if dq is None and dk is None:
-        return None, None, None, None, None, None
-    if dq is None:
-        return None, rotary_op(dk, None, table, positions, interleaved, not inverse)[0], None, None, None, None
-    gq, gk = rotary_op(dq, dk, table, positions, interleaved, not inverse)
-    return gq, (gk if dk is not None else None), None, None, None, None
-
-
-rotary_op.register_autograd(_backward, setup_context=_setup_context)
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        table, positions = ctx.saved_tensors
+        if dq is None and dk is None:
+            return None, None, None, None, None
+        if dq is None:
+            return None, _turn(dk, None, table, positions, ctx.interleaved, True)[0], None, None, None
+        gq, gk = _turn(dq, dk, table, positions, ctx.interleaved, True)
+        return gq, gk, None, None, None
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, positions: Optional[torch.Tensor] = None,
@@ -136,32 +126,30 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, posi
     float dtype, with any strides as long as a head's channels are adjacent (views of a fused projection are read in
     place); table [P, R / 2, 2] from rotary_table; positions int32 or int64 [T] or [B, T] on the device (None: 0 .. T-1).
     A position outside the table is taken as its nearest row."""
-    for name, t in (("q", q), ("k", k)):
-        if t is None and name == "k":
-            continue
-        if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype not in _DTYPES:
-            raise ValueError(f"rotary: {name} must be [B, T, heads, D] in float32, float16 or bfloat16")
-        if not t.is_cuda:
-            raise RuntimeError("rotary: CUDA tensors only (there is no CPU path)")
-    if k is not None and (k.dtype != q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]
-                          or k.device != q.device):
-        raise ValueError("rotary: q and k must agree in dtype, device, batch, tokens and head width")
-    if (not isinstance(table, torch.Tensor) or table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32
-            or table.device != q.device or not table.is_contiguous() or 2 * table.shape[1] > q.shape[3]
-            or table.shape[1] == 0 or table.shape[0] == 0 or table.data_ptr() % 8):
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.dtype not in _DTYPES:
+        raise ValueError("rotary: q must be [B, T, heads, D] in float32, float16 or bfloat16")
+    if not q.is_cuda:
+        raise RuntimeError("rotary: CUDA tensors only (there is no CPU path)")
+    shape, index = q.shape, q.get_device()
+    if k is not None and (not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype != q.dtype
+                          or k.shape[:2] != shape[:2] or k.shape[3] != shape[3] or k.get_device() != index):
+        raise ValueError("rotary: q and k [B, T, heads, D] must agree in dtype, device, batch, tokens and head width")
+    if not isinstance(table, torch.Tensor) or table.dim() != 3 or table.dtype != torch.float32:
+        raise ValueError("rotary: table must be float32 [positions, R / 2, 2]")
+    P, half, two = table.shape
+    if (two != 2 or P == 0 or half == 0 or 2 * half > shape[3] or table.get_device() != index
+            or not table.is_contiguous() or table.data_ptr() % 8):
         raise ValueError("rotary: table must be a contiguous float32 [positions, R / 2, 2] on q's device with R at most "
                          "the head width")
     if positions is not None:
         if (not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64)
-                or positions.device != q.device or tuple(positions.shape) not in ((q.shape[1],), tuple(q.shape[:2]))):
+                or positions.get_device() != index
+                or (positions.shape != shape[:2] and positions.shape != shape[1:2])):
             raise ValueError("rotary: positions must be int32 or int64 [T] or [B, T] on q's device")
         positions = positions.contiguous()
-    elif table.shape[0] < q.shape[1]:
-        raise ValueError(f"rotary: the table has {table.shape[0]} positions, the call {q.shape[1]} tokens")
-    interleaved = bool(interleaved)
-    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) \
-            or torch.compiler.is_compiling():
-        oq, ok = rotary_op(q, k, table, positions, interleaved, False)
-    else:
-        oq, ok = _turn(_rows(q), None if k is None else _rows(k), table, positions, interleaved, False)
-    return oq, (None if k is None else ok)
+    elif P < shape[1]:
+        raise ValueError(f"rotary: the table has {P} positions, the call {shape[1]} tokens")
+    if recorded(q, k):
+        out = Rotary.apply(q, k, table, positions, bool(interleaved))
+        return (out, None) if k is None else out
+    return _turn(q, k, table, positions, bool(interleaved), False)

@@ -15,103 +15,85 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._call import aligned, launch, recorded
 
 _DTYPES = {torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 MAX_D = 256
 
 
-def _p(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+_ERROR_WORD = 64  # gd_wattn_workspace_bytes(..., for_backward=0)
+
+
+def _readable(t: torch.Tensor) -> bool:
+    """Whether the kernels can read t [B, T, heads, D] in place: adjacent channels, 16-byte aligned rows."""
+    if t.data_ptr() % 16:
+        return False
+    if t.is_contiguous():
+        return True
+    b, s, h, d = t.stride()
+    B, T, H, _ = t.shape
+    return (d == 1 and (B <= 1 or (b >= 0 and b % 8 == 0)) and (T <= 1 or (s >= 0 and s % 8 == 0))
+            and (H <= 1 or (h >= 0 and h % 8 == 0)))
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t [B, T, heads, D] if the kernels can read it in place (adjacent channels, 16-byte aligned rows), else a copy."""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(
-        n <= 1 or (s >= 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3]))
-    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+    return t if _readable(t) else aligned(t)
 
 
 def _strides(*ts):
-    return (ctypes.c_longlong * (3 * len(ts)))(*[s for t in ts for s in t.stride()[:3]])
+    out = (ctypes.c_longlong * (3 * len(ts)))()
+    for i, t in enumerate(ts):
+        out[3 * i], out[3 * i + 1], out[3 * i + 2], _ = t.stride()
+    return out
 
 
-def _stream(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _fwd(q, k, v, cu, window, sinks, scale):
-    lib = _lib.load()
-    q, k, v = _rows(q), _rows(k), _rows(v)
+def _fwd(q, k, v, cu, window, sinks, scale, keep):
+    """(o, o_low, lse) on readable inputs; keep: o_low, what o's rounding took away, for the backward (else None)."""
     B, Tq, H, D = q.shape
-    Tk, HK = k.shape[1:3]
-    o = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device)
-    ws = torch.empty(64, dtype=torch.uint8, device=q.device)  # gd_wattn_workspace_bytes(..., for_backward=0)
-    with torch.cuda.device(q.device):
-        st = lib.gd_wattn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _p(cu),
-                              0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], B, Tq, Tk, H, HK, D,
-                              _strides(q, k, v), window, sinks, scale, ws.data_ptr(), 64, _stream(q))
-    _lib.check(st, "gd_wattn_fwd")
-    return o, lse
+    Tk, HK = k.shape[1], k.shape[2]
+    dev = q.device
+    o = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
+    low = torch.empty_like(o) if keep else None
+    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
+    ws = torch.empty(_ERROR_WORD, dtype=torch.uint8, device=dev)
+    launch("gd_wattn_fwd", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+           None if low is None else low.data_ptr(), lse.data_ptr(), None if cu is None else cu.data_ptr(), 0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], B, Tq, Tk, H, HK,
+           D, _strides(q, k, v), window, sinks, scale, ws.data_ptr(), _ERROR_WORD)
+    return o, low, lse
 
 
-@torch.library.custom_op("macai_b200::window_attention_fwd", mutates_args=(), device_types="cuda")
-def window_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor],
-                         window: int, sinks: int, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
-    """(o [B, Tq, H, D], lse [B, H, Tq] float32, the log2-sum of a row's exponentials); window 0: none."""
-    return _fwd(q, k, v, cu_seqlens, window, sinks, scale)
-
-
-@window_attention_fwd.register_fake
-def _(q, k, v, cu_seqlens, window, sinks, scale):
-    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
-
-
-@torch.library.custom_op("macai_b200::window_attention_bwd", mutates_args=(), device_types="cuda")
-def window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
-                         do: torch.Tensor, cu_seqlens: Optional[torch.Tensor], window: int, sinks: int,
-                         scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(dq, dk, dv), contiguous, in the inputs' dtype."""
-    lib = _lib.load()
-    q, k, v, do = _rows(q), _rows(k), _rows(v), _rows(do)
+def _bwd(q, k, v, o, low, lse, do, cu, window, sinks, scale):
+    """(dq, dk, dv), contiguous, on readable inputs."""
     B, Tq, H, D = q.shape
-    Tk, HK = k.shape[1:3]
+    Tk, HK = k.shape[1], k.shape[2]
     dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    n = lib.gd_wattn_workspace_bytes(B, Tq, Tk, H, HK, D, window, sinks, cu_seqlens is not None, 1)
+    n = _lib.load().gd_wattn_workspace_bytes(B, Tq, Tk, H, HK, D, window, sinks, cu is not None, 1)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        st = lib.gd_wattn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), do.data_ptr(),
-                              dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(cu_seqlens),
-                              0 if cu_seqlens is None else cu_seqlens.numel() - 1, _DTYPES[q.dtype], B, Tq, Tk, H, HK, D,
-                              _strides(q, k, v, do), window, sinks, scale, ws.data_ptr(), n, _stream(q))
-    _lib.check(st, "gd_wattn_bwd")
+    launch("gd_wattn_bwd", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), low.data_ptr(),
+           lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None if cu is None else cu.data_ptr(),
+           0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], B, Tq, Tk, H, HK, D, _strides(q, k, v, do), window,
+           sinks, scale, ws.data_ptr(), n)
     return dq, dk, dv
 
 
-@window_attention_bwd.register_fake
-def _(q, k, v, o, lse, do, cu_seqlens, window, sinks, scale):
-    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+class WindowAttention(torch.autograd.Function):
+    """`WindowAttention.apply(q, k, v, cu_seqlens or None, window (0: none), sinks, scale)` on readable inputs."""
 
+    @staticmethod
+    def forward(ctx, q, k, v, cu, window, sinks, scale):
+        o, low, lse = _fwd(q, k, v, cu, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, o, low, lse, cu)
+        ctx.args = (window, sinks, scale)
+        return o
 
-def _setup_context(ctx, inputs, output):
-    q, k, v, cu_seqlens, window, sinks, scale = inputs
-    ctx.save_for_backward(q, k, v, cu_seqlens, *output)
-    ctx.mask = (window, sinks, scale)
-    ctx.set_materialize_grads(False)
-    ctx.mark_non_differentiable(output[1])
-
-
-def _backward(ctx, do, _):
-    if do is None:
-        return None, None, None, None, None, None, None
-    q, k, v, cu_seqlens, o, lse = ctx.saved_tensors
-    dq, dk, dv = window_attention_bwd(q, k, v, o, lse, do.to(q.dtype), cu_seqlens, *ctx.mask)
-    return dq, dk, dv, None, None, None, None
-
-
-window_attention_fwd.register_autograd(_backward, setup_context=_setup_context)
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, low, lse, cu = ctx.saved_tensors
+        return (*_bwd(q, k, v, o, low, lse, _rows(do), cu, *ctx.args), None, None, None, None)
 
 
 def _check_qkv(name, q, k, v):
@@ -120,14 +102,18 @@ def _check_qkv(name, q, k, v):
             raise ValueError(f"{name}: {x} must be [B, T, heads, D]")
         if t.dtype not in _DTYPES:
             raise TypeError(f"{name}: bfloat16 or float16, got {t.dtype} for {x}")
-        if t.dtype != q.dtype or t.device != q.device:
+        if t.dtype != q.dtype or t.get_device() != q.get_device():
             raise ValueError(f"{name}: q, k and v must share one dtype and device")
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+    if not q.is_cuda:
+        raise RuntimeError(f"{name}: CUDA tensors only (there is no CPU path)")
+    B, _, H, D = q.shape
+    kb, _, HK, kd = k.shape
+    if k.shape != v.shape or kb != B or kd != D:
         raise ValueError(f"{name}: k and v [B, T_k, H_k, D] must agree with each other and with q's batch and head width")
-    if q.shape[2] == 0 or k.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError(f"{name}: {q.shape[2]} query heads are no multiple of {k.shape[2]} key heads")
-    if not 0 < q.shape[3] <= MAX_D or q.shape[3] % 8:
-        raise NotImplementedError(f"{name}: head widths are multiples of 8 up to {MAX_D}, got {q.shape[3]}")
+    if H == 0 or HK == 0 or H % HK:
+        raise ValueError(f"{name}: {H} query heads are no multiple of {HK} key heads")
+    if not 0 < D <= MAX_D or D % 8:
+        raise NotImplementedError(f"{name}: head widths are multiples of 8 up to {MAX_D}, got {D}")
 
 
 def _check_mask(name, window, sinks):
@@ -164,9 +150,51 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     _check_qkv("window_attention", q, k, v)
     w, s = _check_mask("window_attention", window, sinks)
     cu = _check_cu(cu_seqlens, q, k)
-    if not q.is_cuda:
-        raise RuntimeError("window_attention: CUDA tensors only (there is no CPU path)")
     scale = float(q.shape[3] ** -0.5 if scale is None else scale)
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-        return window_attention_fwd(q, k, v, cu, w, s, scale)[0]
-    return _fwd(q, k, v, cu, w, s, scale)[0]
+    q_, k_, v_ = _rows(q), _rows(k), _rows(v)
+    if recorded(q, k, v):
+        return WindowAttention.apply(q_, k_, v_, cu, w, s, scale)
+    return _fwd(q_, k_, v_, cu, w, s, scale, False)[0]
+
+
+def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                          v_cache: torch.Tensor, lengths: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
+                          scale: Optional[float] = None) -> torch.Tensor:
+    """One new token for each request: stores its key and value in the caches (in place) and returns its attention
+    o [B, 1, H, D] over the visible positions, its own included. q [B, 1, H, D], k, v [B, 1, H_k, D], k_cache, v_cache
+    [B, S, H_k, D] (any strides with adjacent channels and 16-byte aligned rows), lengths int32 [B] on the device: the
+    tokens in each request's cache before the call, which is the new token's position. The caller adds 1 to lengths after
+    its last layer. A negative length marks an idle request: zeros, nothing stored.
+
+    Position j stands in slot j while j < S, then in slot sinks + (j - sinks) mod (S - sinks): with S >= sinks + window the
+    cache rolls, keeping its first `sinks` tokens, and requests may grow without limit; a smaller cache then shows the last
+    S - sinks positions. No gradient. Nothing waits for the host."""
+    _check_qkv("window_attention_step", q, k, v)
+    w, s = _check_mask("window_attention_step", window, sinks)
+    B, t, H, D = q.shape
+    HK, index = k.shape[2], q.get_device()
+    if t != 1 or k.shape[1] != 1:
+        raise ValueError("window_attention_step: one token a request (q [B, 1, H, D], k and v [B, 1, H_k, D])")
+    if not isinstance(k_cache, torch.Tensor) or not isinstance(v_cache, torch.Tensor) or k_cache.dim() != 4:
+        raise ValueError("window_attention_step: k_cache and v_cache must be [B, S, H_k, D]")
+    S = k_cache.shape[1]
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.shape != (B, S, HK, D) or S == 0 or c.dtype != q.dtype or c.get_device() != index:
+            raise ValueError(f"window_attention_step: {name} must be [B, S, H_k, D] with k's batch, heads, width, dtype and "
+                             "device")
+        if not _readable(c):
+            raise ValueError(f"window_attention_step: {name} needs adjacent channels and 16-byte aligned rows (it is "
+                             "written in place)")
+    if (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or lengths.shape != (B,)
+            or lengths.get_device() != index or not lengths.is_contiguous()):
+        raise ValueError("window_attention_step: lengths must be a contiguous int32 [B] on q's device")
+    if recorded(q, k, v, k_cache, v_cache):
+        raise RuntimeError("window_attention_step has no gradient: call it under torch.no_grad()")
+    q, k, v = aligned(q), aligned(k), aligned(v)
+    o = torch.empty((B, 1, H, D), dtype=q.dtype, device=q.device)
+    n = _lib.load().gd_wattn_step_workspace_bytes(B, S, H, HK, D, w, s)
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    launch("gd_wattn_step", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+           lengths.data_ptr(), o.data_ptr(), _DTYPES[q.dtype], B, S, H, HK, D, _strides(k_cache, v_cache), w, s,
+           float(D ** -0.5 if scale is None else scale), None if ws is None else ws.data_ptr(), n)
+    return o

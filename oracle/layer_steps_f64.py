@@ -87,3 +87,31 @@ def attention(q, k, v, window=None, sinks=0, scale=None, do=None):
                 dk[b, :, c] += dS.T @ Q
                 dv[b, :, c] += P.T @ G
     return o if do is None else (o, dq, dk, dv)
+
+
+def attention_step(q, k, v, k_cache, v_cache, lengths, window=None, sinks=0, scale=None):
+    """(o [B, 1, H, D], k_cache, v_cache) in float64 after one token for each request (copies: nothing in place)."""
+    B, _, H, D = q.shape
+    S, HK = k_cache.shape[1:3]
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    kc, vc = k_cache.double().clone(), v_cache.double().clone()
+    o = torch.zeros(B, 1, H, D, dtype=torch.float64, device=q.device)
+    first = min(sinks, S - 1)
+    ring = S - first
+    for b, p in enumerate(lengths.tolist()):
+        if p < 0:
+            continue
+
+        def slot(j):
+            return j if j < S else first + (j - first) % ring
+        kc[b, slot(p)], vc[b, slot(p)] = k[b, 0].double(), v[b, 0].double()
+        w = p + 1 if window is None else window
+        if p >= S:
+            w = min(w, ring)
+        see = [j for j in range(max(0, p - w + 1))][:min(first, max(0, p - w + 1))] + list(range(max(0, p - w + 1), p + 1))
+        at = torch.tensor([slot(j) for j in see], device=q.device)
+        for h in range(H):
+            c = h * HK // H
+            P = torch.softmax(kc[b, at, c] @ q[b, 0, h].double() * scale, 0)
+            o[b, 0, h] = P @ vc[b, at, c]
+    return o, kc, vc
