@@ -81,10 +81,6 @@ __device__ __forceinline__ T from_f(float x) {
   else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
   else return __float2bfloat16_rn(x);
 }
-template <typename T, int E>
-__device__ __forceinline__ void round_to(float (&f)[E]) {  // to T and back
-  if constexpr (!std::is_same<T, float>::value) Vec<T>::unpack(Vec<T>::pack(f), f);
-}
 
 // A thread's view of its row: chunk j of the thread starts at flat element `at(j)`; elements [lo, hi) are the row's.
 template <typename T, bool FLAT>
@@ -157,12 +153,13 @@ struct Row {
   }
 };
 
-// The sum over a team of TPR threads (a multiple of 32 consecutive threads of the CTA); every thread of the CTA calls.
-// red: one float per warp, its own for each call between two barriers.
+// The sum over a team of TPR threads (a power of two, 4 or more consecutive threads of the CTA); every thread of the CTA
+// calls. red: one float per warp; two buffers in turn, so that one barrier a row is enough.
 __device__ __forceinline__ float team_sum(float v, int tpr, float* red) {
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (tpr == 32) return v;
+  for (int o = 16; o >= 1; o >>= 1)
+    if (o < tpr) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (tpr <= 32) return v;
   const int warp = threadIdx.x >> 5;
   if ((threadIdx.x & 31) == 0) red[warp] = v;
   __syncthreads();
@@ -175,167 +172,155 @@ __device__ __forceinline__ float team_sum(float v, int tpr, float* red) {
 // 1 / sqrt(mean + eps), correctly rounded root and division
 __device__ __forceinline__ float inv_rms(float ss, int D, float eps) { return 1.f / sqrtf(ss / (float)D + eps); }
 
-// s in registers (rounded to T), stored when there is a residual; returns the lane's sum of squares
-template <typename T, int NV, bool FLAT>
-__device__ __forceinline__ float load_stream(const Row<T, FLAT>& row, const T* x, const T* res, T* s,
-                                             float (&v)[NV][Vec<T>::E]) {
+// ---- forward, plain (FP8 = 0) or with the 8-bit output. Persistent CTAs: a team walks the rows, with the next row's
+// loads in flight while this one is reduced and written, and keeps its columns' weights in registers (FLAT: the columns
+// stay its own).
+//
+// 8 bits: group g of a row is channels [g G, (g + 1) G). FP8 = 1: a group is the chunks of `lanes` consecutive lanes (FLAT
+// rows, a power of two of 32 chunks at most) and its maximum a shuffle. FP8 = 2: any G of 8 channels or more, a maximum per
+// group in shared memory (integer maxima of non-negative floats: the order does not matter); a chunk touches two groups at
+// most. A NaN counts in no maximum and comes out as e4m3's NaN.
+template <typename T, int NV, bool FLAT, int FP8, int THREADS>
+__global__ void __launch_bounds__(THREADS) rnorm_fwd(const T* __restrict__ x, const T* __restrict__ res,
+                                                     const void* __restrict__ w, T* __restrict__ s, T* __restrict__ y,
+                                                     uint8_t* __restrict__ q, float* __restrict__ scale, int wdtype,
+                                                     float bias, long long rows, int D, int G, int lanes, int tpr,
+                                                     float eps) {
   constexpr int E = Vec<T>::E;
-  float ss = 0.f;
-  uint4 a[NV], b[NV];  // all of the row's loads in flight before any arithmetic
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    a[j] = row.live(j) ? row.load(x, row.at(j)) : zero;
-    b[j] = res != nullptr && row.live(j) ? row.load(res, row.at(j)) : zero;
-  }
-#pragma unroll
-  for (int j = 0; j < NV; ++j) Vec<T>::unpack(a[j], v[j]);
-  if (res != nullptr) {
+  __shared__ float red[2][32];
+  extern __shared__ unsigned int tops[];  // FP8 = 2: [teams][groups] bit patterns
+  const int teams = blockDim.x / tpr, team = threadIdx.x / tpr, sub = threadIdx.x % tpr;
+  const int groups = FP8 ? (D + G - 1) / G : 0;
+  const long long step = (long long)gridDim.x * teams;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 a[NV], b[NV];
+  auto fetch = [&](long long r) {
+    const Row<T, FLAT> row(r, rows, D, sub, tpr);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!row.live(j)) continue;
-      float f[E];
-      Vec<T>::unpack(b[j], f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[j][e] += f[e];
-      round_to<T>(v[j]);
-      row.store(s, row.at(j), v[j]);
+      a[j] = row.live(j) ? row.load(x, row.at(j)) : zero;
+      b[j] = res != nullptr && row.live(j) ? row.load(res, row.at(j)) : zero;
     }
+  };
+  long long base = (long long)blockIdx.x * teams;
+  fetch(base + team);
+  float wv[NV][E];
+  if constexpr (FLAT) {
+    const Row<T, FLAT> row(0, 1, D, sub, tpr);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (row.live(j)) row.weights(w, wdtype, bias, row.at(j), wv[j]);
   }
+  for (int parity = 0; base < rows; base += step, parity ^= 1) {
+    const long long r0 = base + team;
+    const Row<T, FLAT> row(r0, rows, D, sub, tpr);
+    float v[NV][E];
+    float ss = 0.f;
+    if constexpr (FP8 == 2) {
+      __syncthreads();  // the last row's maxima are read
+      for (int i = threadIdx.x; i < groups * teams; i += blockDim.x) tops[i] = 0u;
+      __syncthreads();
+    }
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      Vec<T>::unpack(a[j], v[j]);
+      if (res != nullptr && row.live(j)) {
+        float f[E];
+        Vec<T>::unpack(b[j], f);
 #pragma unroll
-    for (int e = 0; e < E; ++e) ss = fmaf(v[j][e], v[j][e], ss);
-  return ss;
-}
-
-template <typename T, int NV, bool FLAT>
-__global__ void __launch_bounds__(1024) rnorm_fwd(const T* __restrict__ x, const T* __restrict__ res,
-                                                  const void* __restrict__ w, T* __restrict__ s, T* __restrict__ y,
-                                                  int wdtype, float bias, long long rows, int D, int tpr, float eps) {
-  constexpr int E = Vec<T>::E;
-  __shared__ float red[32];
-  const int team = threadIdx.x / tpr, sub = threadIdx.x % tpr;
-  const Row<T, FLAT> row((long long)blockIdx.x * (blockDim.x / tpr) + team, rows, D, sub, tpr);
-  float v[NV][E];
-  const float ss = load_stream<T, NV, FLAT>(row, x, res, s, v);
-  const float r = inv_rms(team_sum(ss, tpr, red), D, eps);
+        for (int e = 0; e < E; ++e) v[j][e] += f[e];
+        const uint4 packed = Vec<T>::pack(v[j]);
+        Vec<T>::unpack(packed, v[j]);  // rounded to T
+        row.store(s, row.at(j), v[j]);
+      }
+    }
+    if (base + step < rows) fetch(r0 + step);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (!row.live(j)) continue;
-    float wv[E];
-    row.weights(w, wdtype, bias, row.at(j), wv);
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[j][e] = v[j][e] * r * wv[e];
-    row.store(y, row.at(j), v[j]);
-  }
-}
-
-// ---- the 8-bit output. Group g of a row: channels [g G, (g + 1) G). SHUFFLE: a group is the chunks of G / E consecutive
-// lanes (FLAT rows, a power of two of 32 chunks at most) and its maximum a shuffle. Else any G of 8 channels or more, a
-// maximum per group in shared memory (integer maxima of non-negative floats: the order does not matter); a chunk touches
-// two groups at most. A NaN counts in no maximum and comes out as e4m3's NaN.
-template <typename T, int NV, bool FLAT, bool SHUFFLE>
-__global__ void __launch_bounds__(1024) rnorm_fp8(const T* __restrict__ x, const T* __restrict__ res,
-                                                  const void* __restrict__ w, T* __restrict__ s,
-                                                  uint8_t* __restrict__ q, float* __restrict__ scale, int wdtype,
-                                                  float bias, long long rows, int D, int G, int tpr, float eps) {
-  constexpr int E = Vec<T>::E;
-  __shared__ float red[32];
-  extern __shared__ unsigned int tops[];  // [teams][groups] bit patterns (not SHUFFLE)
-  const int team = threadIdx.x / tpr, sub = threadIdx.x % tpr;
-  const int groups = (D + G - 1) / G;
-  const long long r0 = (long long)blockIdx.x * (blockDim.x / tpr) + team;
-  const Row<T, FLAT> row(r0, rows, D, sub, tpr);
-  float v[NV][E];
-  if constexpr (!SHUFFLE) {
-    for (int i = threadIdx.x; i < groups * (blockDim.x / tpr); i += blockDim.x) tops[i] = 0u;
-    __syncthreads();
-  }
-  const float ss = load_stream<T, NV, FLAT>(row, x, res, s, v);
-  const float r = inv_rms(team_sum(ss, tpr, red), D, eps);
-  float top[NV];
+      for (int e = 0; e < E; ++e) ss = fmaf(v[j][e], v[j][e], ss);
+    const float r = inv_rms(team_sum(ss, tpr, red[parity]), D, eps);
+    float top[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    float wv[E];
-    top[j] = 0.f;
-    if (row.live(j)) {
-      row.weights(w, wdtype, bias, row.at(j), wv);
+    for (int j = 0; j < NV; ++j) {
+      top[j] = 0.f;
+      if (!row.live(j)) continue;
+      if constexpr (!FLAT) row.weights(w, wdtype, bias, row.at(j), wv[j]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[j][e] = v[j][e] * r * wv[e];
-      if constexpr (SHUFFLE) {
+      for (int e = 0; e < E; ++e) v[j][e] = v[j][e] * r * wv[j][e];
+      if constexpr (FP8 == 0) row.store(y, row.at(j), v[j]);
+      if constexpr (FP8 == 1) {
 #pragma unroll
         for (int e = 0; e < E; ++e) top[j] = fmaxf(top[j], fabsf(v[j][e]));
-      } else {
+      }
+      if constexpr (FP8 == 2) {
         const int c0 = (int)(row.at(j) - row.lo);  // may be negative: the chunk starts in the row before
         const int g0 = c0 > 0 ? c0 / G : 0, split = (g0 + 1) * G;
-        float a = 0.f, b = 0.f;
+        float f = 0.f, g = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float m = row.mine(row.at(j) + e) ? fabsf(v[j][e]) : 0.f;
-          if (c0 + e < split) a = fmaxf(a, m);
-          else b = fmaxf(b, m);
+          if (c0 + e < split) f = fmaxf(f, m);
+          else g = fmaxf(g, m);
         }
-        atomicMax(&tops[team * groups + g0], __float_as_uint(a));
-        if (b > 0.f) atomicMax(&tops[team * groups + g0 + 1], __float_as_uint(b));
+        atomicMax(&tops[team * groups + g0], __float_as_uint(f));
+        if (g > 0.f) atomicMax(&tops[team * groups + g0 + 1], __float_as_uint(g));
       }
     }
-  }
-  if constexpr (SHUFFLE) {
-    const int lanes = G / E;
+    if constexpr (FP8 != 0) {
+      if constexpr (FP8 == 1) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      for (int o = lanes >> 1; o >= 1; o >>= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
-    }
-  } else {
-    __syncthreads();
-  }
+        for (int j = 0; j < NV; ++j)
+          for (int o = lanes >> 1; o >= 1; o >>= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+      }
+      if constexpr (FP8 == 2) __syncthreads();
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (!row.live(j)) continue;
-    const long long a = row.at(j);
-    const int c0 = (int)(a - row.lo);
-    uint32_t packed[E / 4];
-    float sc = 1.f, sc2 = 1.f;
-    int split = 1 << 30;
-    if constexpr (SHUFFLE) {
-      sc = top[j] > 0.f ? top[j] / kE4m3Max : 1.f;
-      if ((c0 % G) == 0) scale[r0 * groups + c0 / G] = sc;
-    } else {
-      const int g0 = c0 > 0 ? c0 / G : 0;
-      split = (g0 + 1) * G;
-      const float t1 = __uint_as_float(tops[team * groups + g0]);
-      sc = t1 > 0.f ? t1 / kE4m3Max : 1.f;
-      if (g0 + 1 < groups) {
-        const float t2 = __uint_as_float(tops[team * groups + g0 + 1]);
-        sc2 = t2 > 0.f ? t2 / kE4m3Max : 1.f;
+      for (int j = 0; j < NV; ++j) {
+        if (!row.live(j)) continue;
+        const long long at = row.at(j);
+        const int c0 = (int)(at - row.lo);
+        uint32_t packed[E / 4];
+        float sc = 1.f, sc2 = 1.f;  // 1 / scale: the product is within 2 units in the last place of y / scale
+        int split = 1 << 30;
+        if constexpr (FP8 == 1) {
+          sc = top[j] > 0.f ? kE4m3Max / top[j] : 1.f;
+          if ((sub & (lanes - 1)) == 0) scale[r0 * groups + c0 / G] = top[j] > 0.f ? top[j] / kE4m3Max : 1.f;
+        } else {
+          const int g0 = c0 > 0 ? c0 / G : 0;
+          split = (g0 + 1) * G;
+          const float t1 = __uint_as_float(tops[team * groups + g0]);
+          sc = t1 > 0.f ? kE4m3Max / t1 : 1.f;
+          if (g0 + 1 < groups) {
+            const float t2 = __uint_as_float(tops[team * groups + g0 + 1]);
+            sc2 = t2 > 0.f ? kE4m3Max / t2 : 1.f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) {
+          float f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = v[j][4 * i + e] * (FP8 == 1 || c0 + 4 * i + e < split ? sc : sc2);
+          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+          packed[i] = lo | hi << 16;
+        }
+        if (row.whole(at)) {
+          if constexpr (E == 8) *reinterpret_cast<uint2*>(q + at) = make_uint2(packed[0], packed[1]);
+          else *reinterpret_cast<uint32_t*>(q + at) = packed[0];
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (row.mine(at + e)) q[at + e] = (uint8_t)(packed[e / 4] >> (8 * (e % 4)));
+        }
+      }
+      if constexpr (FP8 == 2) {
+        if (r0 < rows)
+          for (int g = sub; g < groups; g += tpr) {
+            const float t = __uint_as_float(tops[team * groups + g]);
+            scale[r0 * groups + g] = t > 0.f ? t / kE4m3Max : 1.f;
+          }
       }
     }
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i) {
-      uint32_t u = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float f = v[j][4 * i + e] / (c0 + 4 * i + e < split ? sc : sc2);
-        u |= (uint32_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3) << (8 * e);
-      }
-      packed[i] = u;
-    }
-    if (row.whole(a)) {
-      if constexpr (E == 8) *reinterpret_cast<uint2*>(q + a) = make_uint2(packed[0], packed[1]);
-      else *reinterpret_cast<uint32_t*>(q + a) = packed[0];
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (row.mine(a + e)) q[a + e] = (uint8_t)(packed[e / 4] >> (8 * (e % 4)));
-    }
-  }
-  if constexpr (!SHUFFLE) {
-    if (r0 < rows)
-      for (int g = sub; g < groups; g += tpr) {
-        const float t = __uint_as_float(tops[team * groups + g]);
-        scale[r0 * groups + g] = t > 0.f ? t / kE4m3Max : 1.f;
-      }
   }
 }
 
@@ -343,16 +328,40 @@ __global__ void __launch_bounds__(1024) rnorm_fp8(const T* __restrict__ x, const
 // FLAT thread keeps its columns' sums in registers (the columns stay its own over the rows) and the CTA's teams are
 // added in team order; without FLAT the columns move with the row, so the sums stand in shared memory, where one thread
 // adds to an element at a time, in the rows' order (one team a CTA).
-template <typename T, int NV, bool FLAT, bool DW>
-__global__ void __launch_bounds__(1024) rnorm_bwd(const T* __restrict__ s, const void* __restrict__ w,
-                                                  const T* __restrict__ dy, const T* __restrict__ ds,
-                                                  T* __restrict__ dx, float* __restrict__ part, int wdtype, float bias,
-                                                  long long rows, int D, int tpr, float eps) {
+template <typename T, int NV, bool FLAT, bool DW, int THREADS>
+__global__ void __launch_bounds__(THREADS) rnorm_bwd(const T* __restrict__ s, const void* __restrict__ w,
+                                                     const T* __restrict__ dy, const T* __restrict__ ds,
+                                                     T* __restrict__ dx, float* __restrict__ part, int wdtype, float bias,
+                                                     long long rows, int D, int tpr, float eps) {
   constexpr int E = Vec<T>::E;
-  __shared__ float red[2][32];
+  __shared__ float red[2][2][32];
   extern __shared__ __align__(16) float sums[];  // DW: [teams][D] (FLAT, at the end), or [D]
   const int teams = blockDim.x / tpr, team = threadIdx.x / tpr, sub = threadIdx.x % tpr;
-  float acc[DW && FLAT ? NV : 1][E];
+  const long long step = (long long)gridDim.x * teams;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 nv[NV], ng[NV], nc[NV];  // the next row's s, dy, ds as they stand in memory
+  auto fetch = [&](long long r) {
+    const Row<T, FLAT> row(r, rows, D, sub, tpr);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const bool live = row.live(j);
+      nv[j] = live ? row.load(s, row.at(j)) : zero;
+      ng[j] = live && dy != nullptr ? row.load(dy, row.at(j)) : zero;
+      nc[j] = live && ds != nullptr ? row.load(ds, row.at(j)) : zero;
+    }
+  };
+  long long base = (long long)blockIdx.x * teams;
+  fetch(base + team);
+  float acc[DW && FLAT ? NV : 1][E], wv[NV][E];
+  if constexpr (FLAT) {
+    const Row<T, FLAT> row(0, 1, D, sub, tpr);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) wv[j][e] = 0.f;
+      if (row.live(j)) row.weights(w, wdtype, bias, row.at(j), wv[j]);
+    }
+  }
   if constexpr (DW) {
     if constexpr (FLAT) {
 #pragma unroll
@@ -361,53 +370,54 @@ __global__ void __launch_bounds__(1024) rnorm_bwd(const T* __restrict__ s, const
         for (int e = 0; e < E; ++e) acc[j][e] = 0.f;
     } else {
       for (int i = threadIdx.x; i < D; i += blockDim.x) sums[i] = 0.f;
+      __syncthreads();
     }
   }
-  for (long long base = (long long)blockIdx.x * teams; base < rows; base += (long long)gridDim.x * teams) {
+  for (int parity = 0; base < rows; base += step, parity ^= 1) {
     const Row<T, FLAT> row(base + team, rows, D, sub, tpr);
-    uint4 v[NV], g[NV], c[NV];  // as they stand in memory: half the registers of their floats
-    float ss = 0.f;
+    uint4 v[NV], g[NV], c[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      v[j] = g[j] = c[j] = make_uint4(0, 0, 0, 0);
-      if (!row.live(j)) continue;
-      v[j] = row.load(s, row.at(j));
-      if (dy != nullptr) g[j] = row.load(dy, row.at(j));
-      if (ds != nullptr) c[j] = row.load(ds, row.at(j));
+      v[j] = nv[j];
+      g[j] = ng[j];
+      c[j] = nc[j];
     }
-    float dot = 0.f;  // sum of h s: the mean of h xh is dot r / D
+    if (base + step < rows) fetch(base + step + team);
+    float ss = 0.f, dot = 0.f;  // sum of s^2, and of h s: the mean of h xh is dot r / D
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (!row.live(j)) continue;
-      float wv[E], vf[E], gf[E];
-      row.weights(w, wdtype, bias, row.at(j), wv);
+      float vf[E], gf[E];
+      if constexpr (!FLAT) row.weights(w, wdtype, bias, row.at(j), wv[j]);
       Vec<T>::unpack(v[j], vf);
       Vec<T>::unpack(g[j], gf);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         ss = fmaf(vf[e], vf[e], ss);
-        dot = fmaf(gf[e] * wv[e], vf[e], dot);
+        dot = fmaf(gf[e] * wv[j][e], vf[e], dot);
       }
     }
-    // two sums at once: their warp parts side by side, one barrier
+    // two sums at once: their warp parts side by side, one barrier a row (two buffers in turn)
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-      ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    }
+    for (int o = 16; o >= 1; o >>= 1)
+      if (o < tpr) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      }
     if (tpr > 32) {
       const int warp = threadIdx.x >> 5, n = tpr >> 5, w0 = warp / n * n;
-      __syncthreads();  // the last row's readers are done with red
       if ((threadIdx.x & 31) == 0) {
-        red[0][warp] = ss;
-        red[1][warp] = dot;
+        red[parity][0][warp] = ss;
+        red[parity][1][warp] = dot;
       }
       __syncthreads();
       ss = dot = 0.f;
       for (int i = 0; i < n; ++i) {
-        ss += red[0][w0 + i];
-        dot += red[1][w0 + i];
+        ss += red[parity][0][w0 + i];
+        dot += red[parity][1][w0 + i];
       }
+    } else if constexpr (DW && !FLAT) {
+      __syncthreads();  // the last row's sums are in place (one team: an element's adders take turns)
     }
     const float r = inv_rms(ss, D, eps);
     const float m = dot * r / (float)D;
@@ -415,15 +425,14 @@ __global__ void __launch_bounds__(1024) rnorm_bwd(const T* __restrict__ s, const
     for (int j = 0; j < NV; ++j) {
       if (!row.live(j)) continue;
       const long long a = row.at(j);
-      float wv[E], vf[E], gf[E], out[E];
-      row.weights(w, wdtype, bias, a, wv);
+      float vf[E], gf[E], out[E];
       Vec<T>::unpack(v[j], vf);
       Vec<T>::unpack(g[j], gf);
       Vec<T>::unpack(c[j], out);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float xh = vf[e] * r;
-        out[e] += r * (gf[e] * wv[e] - xh * m);
+        out[e] += r * (gf[e] * wv[j][e] - xh * m);
         if constexpr (DW) {
           if constexpr (FLAT) acc[j][e] = fmaf(gf[e], xh, acc[j][e]);
           else if (row.mine(a + e)) sums[a - row.lo + e] += gf[e] * xh;
@@ -476,29 +485,31 @@ struct Shape {
   int tpr, nv, threads, teams;
 };
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n > 0 ? n : 148;
-}
+constexpr int kSms = 148;  // of a B200
 
 int chunks_of(int D, int E) { return D % E == 0 ? D / E : D / E + 2; }  // with the two shared with the neighbours
 
-// The team: as few threads as hold the row in `most` chunks each when there are rows to fill the GPU; one chunk a
-// thread when there are not (a few tokens: the shortest chain of loads).
-Shape shape_of(long long rows, int D, int E, bool one_team, int most, int sms) {
+// The team: one chunk a thread (two past 1,024 threads): the next row's loads already double what is in flight. CTAs of
+// 256 threads hold several teams of narrow rows, except where rows are too few to give every SM a CTA so.
+Shape shape_of(long long rows, int D, int E, bool one_team) {
   Shape s;
   s.flat = D % E == 0;
   const int chunks = chunks_of(D, E);
-  const int want = rows < 4ll * sms ? 1 : most;
-  s.tpr = 32;
-  while (s.tpr < 1024 && s.tpr * want < chunks) s.tpr *= 2;
+  s.tpr = 4;
+  while (s.tpr < 1024 && s.tpr < chunks) s.tpr *= 2;
   s.nv = s.tpr < chunks ? 2 : 1;
-  s.threads = one_team || s.tpr > kThreads ? s.tpr : kThreads;
-  if (rows < 4ll * sms && !one_team) s.threads = s.tpr;  // spread over the SMs
+  s.threads = s.tpr > kThreads ? s.tpr : kThreads;
+  if (one_team) s.threads = s.tpr;
+  while (!one_team && s.threads > s.tpr && s.threads > 32 && rows * s.tpr / s.threads < kSms) s.threads /= 2;
+  if (s.threads < 32) s.threads = s.tpr = 32;
   s.teams = s.threads / s.tpr;
   return s;
+}
+// persistent CTAs: as many as are resident at 64 registers a thread
+int grid_of(long long rows, const Shape& s, int most = 1 << 30) {
+  const long long blocks = (rows + s.teams - 1) / s.teams, resident = (long long)kSms * (1024 / s.threads);
+  const long long g = blocks < resident ? blocks : resident;
+  return (int)(g < most ? g : most);
 }
 
 int chunk_elems(int dtype) { return dtype == GD_FLOAT32 ? 4 : 8; }
@@ -514,10 +525,6 @@ int check_common(const void* w, int dtype, int wdtype, long long rows, int D) {
 }
 
 template <typename F>
-int with_nv(int nv, F&& f) {
-  return nv == 1 ? f(std::integral_constant<int, 1>{}) : f(std::integral_constant<int, 2>{});
-}
-template <typename F>
 int with_type(int dtype, F&& f) {
   switch (dtype) {
     case GD_FLOAT32: return f(float{});
@@ -527,12 +534,34 @@ int with_type(int dtype, F&& f) {
 }
 int launched() { return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH); }
 
-int bwd_grid(long long rows, const Shape& s, int sms, bool dw) {
-  const long long blocks = (rows + s.teams - 1) / s.teams;
-  const long long resident = (long long)sms * (1024 / s.threads);
-  long long g = blocks < resident ? blocks : resident;
-  if (dw && g > kMaxPartials) g = kMaxPartials;
-  return (int)(g > 0 ? g : 1);
+
+// f(integral_constant NV, integral_constant THREADS): kernels of up to 256 threads get more registers each
+template <typename F>
+int with_shape(const Shape& s, F&& f) {
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (s.nv == 2) return f(Two{}, std::integral_constant<int, 1024>{});
+  return s.threads <= 256 ? f(One{}, std::integral_constant<int, 256>{}) : f(One{}, std::integral_constant<int, 1024>{});
+}
+
+template <int FP8>
+int forward(const void* x, const void* res, const void* w, void* s, void* y, void* q, float* scale, int dtype, int wdtype,
+            int zero_centered, long long rows, int D, int G, int lanes, const Shape& sh, size_t smem, float eps,
+            void* stream) {
+  const int grid = grid_of(rows, sh);
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    return with_shape(sh, [&](auto nv, auto threads) {
+      constexpr int NV = decltype(nv)::value, TH = decltype(threads)::value;
+      auto k = rnorm_fwd<T, NV, true, FP8, TH>;
+      if constexpr (FP8 != 1)
+        if (!sh.flat) k = rnorm_fwd<T, NV, false, FP8, TH>;
+      k<<<grid, sh.threads, smem, static_cast<cudaStream_t>(stream)>>>(
+          static_cast<const T*>(x), static_cast<const T*>(res), w, static_cast<T*>(s), static_cast<T*>(y),
+          static_cast<uint8_t*>(q), scale, wdtype, zero_centered ? 1.f : 0.f, rows, D, G, lanes, sh.tpr, eps);
+      return launched();
+    });
+  });
 }
 
 }  // namespace
@@ -543,21 +572,8 @@ extern "C" int gd_rnorm_fwd(const void* x, const void* res, const void* w, void*
   if (rows == 0) return GD_OK;
   if (x == nullptr || y == nullptr || (res != nullptr && s == nullptr)) return GD_ERR_ARG;
   if (misaligned(x) || misaligned(res) || misaligned(w) || misaligned(s) || misaligned(y)) return GD_ERR_ALIGN;
-  const Shape sh = shape_of(rows, D, chunk_elems(dtype), false, 2, sm_count());
-  const long long grid = (rows + sh.teams - 1) / sh.teams;
-  if (grid > 0x7fffffffll) return GD_ERR_SHAPE;
-  const float bias = zero_centered ? 1.f : 0.f;
-  return with_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    return with_nv(sh.nv, [&](auto nv) {
-      constexpr int NV = decltype(nv)::value;
-      auto k = sh.flat ? rnorm_fwd<T, NV, true> : rnorm_fwd<T, NV, false>;
-      k<<<(unsigned)grid, sh.threads, 0, static_cast<cudaStream_t>(stream)>>>(
-          static_cast<const T*>(x), static_cast<const T*>(res), w, static_cast<T*>(s), static_cast<T*>(y), wdtype, bias,
-          rows, D, sh.tpr, eps);
-      return launched();
-    });
-  });
+  const Shape sh = shape_of(rows, D, chunk_elems(dtype), false);
+  return forward<0>(x, res, w, s, y, nullptr, nullptr, dtype, wdtype, zero_centered, rows, D, 1, 1, sh, 0, eps, stream);
 }
 
 extern "C" int gd_rnorm_fp8(const void* x, const void* res, const void* w, void* s, void* q, float* scale, int dtype,
@@ -568,25 +584,14 @@ extern "C" int gd_rnorm_fp8(const void* x, const void* res, const void* w, void*
   if (x == nullptr || q == nullptr || scale == nullptr || (res != nullptr && s == nullptr)) return GD_ERR_ARG;
   if (misaligned(x) || misaligned(res) || misaligned(w) || misaligned(s) || misaligned(q)) return GD_ERR_ALIGN;
   const int E = chunk_elems(dtype);
-  const int G = group == 0 ? (D + 7) / 8 * 8 : group;  // 0: the whole row
-  const Shape sh = shape_of(rows, D, E, false, 2, sm_count());
-  const long long grid = (rows + sh.teams - 1) / sh.teams;
-  if (grid > 0x7fffffffll) return GD_ERR_SHAPE;
-  const float bias = zero_centered ? 1.f : 0.f;
-  const int lanes = G / E;
-  const bool shuffle = sh.flat && lanes <= 32 && (lanes & (lanes - 1)) == 0;
-  const size_t smem = shuffle ? 0 : (size_t)sh.teams * ((D + G - 1) / G) * sizeof(unsigned int);
-  return with_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    return with_nv(sh.nv, [&](auto nv) {
-      constexpr int NV = decltype(nv)::value;
-      auto k = !sh.flat ? rnorm_fp8<T, NV, false, false> : shuffle ? rnorm_fp8<T, NV, true, true> : rnorm_fp8<T, NV, true, false>;
-      k<<<(unsigned)grid, sh.threads, smem, static_cast<cudaStream_t>(stream)>>>(
-          static_cast<const T*>(x), static_cast<const T*>(res), w, static_cast<T*>(s), static_cast<uint8_t*>(q), scale,
-          wdtype, bias, rows, D, G, sh.tpr, eps);
-      return launched();
-    });
-  });
+  const int G = group == 0 || group > D ? (D + 7) / 8 * 8 : group;  // 0: the whole row
+  const Shape sh = shape_of(rows, D, E, false);
+  // groups that are the chunks of a power of two of lanes of one warp; a row of one group: of the whole team
+  const int groups = (D + G - 1) / G, lanes = groups == 1 ? sh.tpr : G / E;
+  if (sh.flat && lanes <= 32 && lanes <= sh.tpr && (lanes & (lanes - 1)) == 0)
+    return forward<1>(x, res, w, s, nullptr, q, scale, dtype, wdtype, zero_centered, rows, D, G, lanes, sh, 0, eps, stream);
+  return forward<2>(x, res, w, s, nullptr, q, scale, dtype, wdtype, zero_centered, rows, D, G, 1, sh,
+                    (size_t)sh.teams * groups * sizeof(unsigned int), eps, stream);
 }
 
 extern "C" size_t gd_rnorm_workspace_bytes(long long rows, int D) {
@@ -611,24 +616,23 @@ extern "C" int gd_rnorm_bwd(const void* s, const void* w, const void* dy, const 
     return GD_ERR_ALIGN;
   if (dw != nullptr && (workspace == nullptr || workspace_bytes < gd_rnorm_workspace_bytes(rows, D)))
     return GD_ERR_WORKSPACE;
-  const int E = chunk_elems(dtype), sms = sm_count();
-  const Shape sh = shape_of(rows, D, E, dw != nullptr && D % E != 0, 1, sms);
-  const int grid = bwd_grid(rows, sh, sms, dw != nullptr);
+  const int E = chunk_elems(dtype);
+  const Shape sh = shape_of(rows, D, E, dw != nullptr && D % E != 0);
+  const int grid = grid_of(rows, sh, dw != nullptr ? kMaxPartials : 1 << 30);
   const float bias = zero_centered ? 1.f : 0.f;
   float* part = static_cast<float*>(workspace);
   const size_t smem = dw == nullptr ? 0 : (size_t)(sh.flat ? sh.teams : 1) * D * sizeof(float);
   int st = with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    return with_nv(sh.nv, [&](auto nv) {
-      constexpr int NV = decltype(nv)::value;
-      auto k = dw != nullptr ? (sh.flat ? rnorm_bwd<T, NV, true, true> : rnorm_bwd<T, NV, false, true>)
-                             : (sh.flat ? rnorm_bwd<T, NV, true, false> : rnorm_bwd<T, NV, false, false>);
+    return with_shape(sh, [&](auto nv, auto threads) {
+      constexpr int NV = decltype(nv)::value, TH = decltype(threads)::value;
+      auto k = dw != nullptr ? (sh.flat ? rnorm_bwd<T, NV, true, true, TH> : rnorm_bwd<T, NV, false, true, TH>)
+                             : (sh.flat ? rnorm_bwd<T, NV, true, false, TH> : rnorm_bwd<T, NV, false, false, TH>);
       if (smem > 48 * 1024 &&
           cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return (cudaGetLastError(), GD_ERR_LAUNCH);
-      k<<<grid, sh.threads, smem, cs>>>(static_cast<const T*>(s), w, static_cast<const T*>(dy),
-                                        static_cast<const T*>(ds), static_cast<T*>(dx), part, wdtype, bias, rows, D,
-                                        sh.tpr, eps);
+      k<<<grid, sh.threads, smem, cs>>>(static_cast<const T*>(s), w, static_cast<const T*>(dy), static_cast<const T*>(ds),
+                                        static_cast<T*>(dx), part, wdtype, bias, rows, D, sh.tpr, eps);
       return launched();
     });
   });

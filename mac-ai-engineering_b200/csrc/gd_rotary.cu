@@ -4,8 +4,7 @@
 // with pairs (i, i + R/2) (half layout) or (2 i, 2 i + 1) (interleaved), cos and sin from a table [P, R/2, 2] in fp32
 // indexed by the token's position. The backward is the turn by the opposite angle (sign = -1).
 //
-// Bound by HBM: every channel of q and k is read and written once; a token's R/2 angles serve all its heads (they come
-// from L1 and L2 after the first). q and k may be views of a fused projection (any batch, token and head stride);
+// Bound by HBM: every channel of q and k is read and written once; a token's R/2 angles serve all its heads (through shared memory). q and k may be views of a fused projection (any batch, token and head stride);
 // outputs are contiguous. A unit of work is V channels of a head that pass through or are turned among themselves
 // (interleaved), or the two V-channel halves of V pairs; V is the widest that divides widths, strides and addresses.
 #include <cuda_bf16.h>
@@ -20,7 +19,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kItems = 4;  // units a thread has in flight
+constexpr int kItems = 2;  // units a thread has in flight: with 48 warps an SM, enough; more registers cost more warps
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
@@ -52,93 +51,136 @@ struct Args {
   long long P;
   int B, T, H, HK, D, R;
   float sign;
+  bool table16;           // every row of the table starts on 16 bytes
 };
 
+// n / d for n < 2^16 and d <= 2^16, by m = ceil(2^32 / d): n m is off n 2^32 / d by less than n d <= 2^32
+__device__ __forceinline__ unsigned div16(unsigned n, unsigned m) { return m == 0u ? n : __umulhi(n, m); }
+
+// How a CTA's items are numbered: first the turned units of its tokens, (token, head, unit), then the copied ones, so that
+// a warp does one or the other.
+struct Items {
+  int tokens;                       // of a CTA
+  int turn, copy;                   // units of a head
+  unsigned m_turn, m_copy;          // div16's numbers: of turn, copy
+  unsigned m_hturn, m_hcopy;        // of heads * turn, heads * copy
+};
+
+// A CTA takes `tokens` consecutive tokens of a batch row. A thread's items lie kThreads apart; their loads are in flight
+// before any arithmetic.
 template <typename T, int V, bool IL>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const T* __restrict__ q, const T* __restrict__ k,
-                                                          T* __restrict__ oq, T* __restrict__ ok, const Args a,
-                                                          const int turn_units, const int units, long long items) {
-  constexpr int N = IL && V == 1 ? 2 : V;  // channels of a unit (of each half of its pairs in the half layout)
+__global__ void __launch_bounds__(kThreads, 6) rotary_kernel(const T* __restrict__ q, const T* __restrict__ k,
+                                                             T* __restrict__ oq, T* __restrict__ ok, const Args a,
+                                                             const Items n) {
+  constexpr int N = IL && V == 1 ? 2 : V;  // channels of a turned unit (of each half of its pairs in the half layout)
+  constexpr int L = N / V;                 // packs of it
+  constexpr int A = IL ? N / 2 : V;        // angles of it
   using Pk = Pack<T, V>;
-  const long long first = (long long)blockIdx.x * (kThreads * kItems) + threadIdx.x;
-  const int heads = a.H + a.HK;
+  const unsigned heads = a.H + a.HK;
+  const int b = blockIdx.y, t0 = blockIdx.x * n.tokens, here = a.T - t0 < n.tokens ? a.T - t0 : n.tokens;
+  const unsigned turned = (unsigned)here * heads * n.turn, items = turned + (unsigned)here * heads * n.copy;
+  const bool small = items <= 65536u;  // (a CTA of one token may have more: it divides)
+  for (unsigned first = threadIdx.x; first < items; first += kThreads * kItems) {
+    Pk x[kItems][L], y[kItems];
+    T* dst[kItems];
+    const float2* cs[kItems];  // a turned item's angles
+    bool live[kItems];
 #pragma unroll
-  for (int it = 0; it < kItems; ++it) {
-    const long long item = first + it * kThreads;
-    if (item >= items) return;
-    // item -> (token, head, unit); 32-bit divisions inside the token
-    const int per_token = heads * units;
-    const long long token = item < 0x7fffffff ? (long long)((unsigned)item / (unsigned)per_token) : item / per_token;
-    const unsigned rest = (unsigned)(item - token * per_token);
-    const int hh = rest / units, u = rest - hh * units;
-    const int b = token < 0x7fffffff ? (int)((unsigned)token / (unsigned)a.T) : (int)(token / a.T);
-    const int t = (int)(token - (long long)b * a.T);
-    const bool is_q = hh < a.H;
-    const int h = is_q ? hh : hh - a.H;
-    const T* src = is_q ? q + b * a.q.b + t * a.q.t + h * a.q.h : k + b * a.k.b + t * a.k.t + h * a.k.h;
-    T* dst = is_q ? oq + (token * a.H + h) * a.D : ok + (token * a.HK + h) * a.D;
-    if (u >= turn_units) {  // channels past R
-      const int c = a.R + (u - turn_units) * V;
-      *reinterpret_cast<Pk*>(dst + c) = *reinterpret_cast<const Pk*>(src + c);
-      continue;
+    for (int it = 0; it < kItems; ++it) {
+      unsigned i = first + it * kThreads;
+      live[it] = i < items;
+      cs[it] = nullptr;
+      if (!live[it]) continue;
+      const bool turn = i < turned;
+      if (!turn) i -= turned;
+      const unsigned units = turn ? n.turn : n.copy, per_token = heads * units;
+      const unsigned tt = small ? div16(i, turn ? n.m_hturn : n.m_hcopy) : i / per_token, rest = i - tt * per_token;
+      const unsigned hh = small ? div16(rest, turn ? n.m_turn : n.m_copy) : rest / units, u = rest - hh * units;
+      const int t = t0 + (int)tt;
+      const bool is_q = hh < (unsigned)a.H;
+      const long long h = is_q ? hh : hh - a.H, token = (long long)b * a.T + t;
+      const int c = turn ? (int)u * N : a.R + (int)u * V;
+      const T* src = (is_q ? q + b * a.q.b + t * a.q.t + h * a.q.h : k + b * a.k.b + t * a.k.t + h * a.k.h) + c;
+      dst[it] = (is_q ? oq + (token * a.H + h) * a.D : ok + (token * a.HK + h) * a.D) + c;
+      x[it][0] = *reinterpret_cast<const Pk*>(src);
+      if (turn) {
+#pragma unroll
+        for (int l = 1; l < L; ++l) x[it][l] = *reinterpret_cast<const Pk*>(src + l * V);
+        if (!IL) y[it] = *reinterpret_cast<const Pk*>(src + a.R / 2);
+        long long p = t;
+        if (a.positions != nullptr) {
+          const long long w = b * a.pos_b + t;
+          p = a.pos64 ? __ldg(static_cast<const long long*>(a.positions) + w)
+                      : (long long)__ldg(static_cast<const int*>(a.positions) + w);
+        }
+        p = p < 0 ? 0 : p >= a.P ? a.P - 1 : p;  // never outside the table
+        cs[it] = a.table + p * (a.R / 2) + (IL ? c / 2 : c);
+      }
     }
-    long long p = t;
-    if (a.positions != nullptr) {
-      const long long at = b * a.pos_b + t;
-      p = a.pos64 ? __ldg(static_cast<const long long*>(a.positions) + at)
-                  : (long long)__ldg(static_cast<const int*>(a.positions) + at);
-    }
-    p = p < 0 ? 0 : p >= a.P ? a.P - 1 : p;  // never outside the table
-    const float2* tab = a.table + p * (a.R / 2);
-    if constexpr (IL) {
-      const int c = u * N;
-      T x[N];
 #pragma unroll
-      for (int i = 0; i < N / V; ++i) {
-        const Pk pk = *reinterpret_cast<const Pk*>(src + c + i * V);
+    for (int it = 0; it < kItems; ++it) {
+      if (!live[it]) continue;
+      if (cs[it] != nullptr) {
+        float2 t[A];
+        if constexpr (A % 2 == 0) {  // an even number of angles starts on 16 bytes when the table does
+          if (a.table16) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[i * V + e] = pk.v[e];
+            for (int i = 0; i < A; i += 2) {
+              const float4 v = __ldg(reinterpret_cast<const float4*>(cs[it] + i));
+              t[i] = make_float2(v.x, v.y);
+              t[i + 1] = make_float2(v.z, v.w);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < A; ++i) t[i] = __ldg(cs[it] + i);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < A; ++i) t[i] = __ldg(cs[it] + i);
+        }
+        if constexpr (IL) {
+          T* v = reinterpret_cast<T*>(x[it]);
+#pragma unroll
+          for (int i = 0; i < A; ++i) {
+            const float f = to_f<T>(v[2 * i]), g = to_f<T>(v[2 * i + 1]), sn = t[i].y * a.sign;
+            v[2 * i] = from_f<T>(f * t[i].x - g * sn);
+            v[2 * i + 1] = from_f<T>(g * t[i].x + f * sn);
+          }
+#pragma unroll
+          for (int l = 1; l < L; ++l) *reinterpret_cast<Pk*>(dst[it] + l * V) = x[it][l];
+        } else {
+#pragma unroll
+          for (int e = 0; e < A; ++e) {
+            const float f = to_f<T>(x[it][0].v[e]), g = to_f<T>(y[it].v[e]), sn = t[e].y * a.sign;
+            x[it][0].v[e] = from_f<T>(f * t[e].x - g * sn);
+            y[it].v[e] = from_f<T>(g * t[e].x + f * sn);
+          }
+          *reinterpret_cast<Pk*>(dst[it] + a.R / 2) = y[it];
+        }
       }
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        const float2 cs = __ldg(tab + c / 2 + i);
-        const float sn = cs.y * a.sign, f = to_f<T>(x[2 * i]), g = to_f<T>(x[2 * i + 1]);
-        x[2 * i] = from_f<T>(f * cs.x - g * sn);
-        x[2 * i + 1] = from_f<T>(g * cs.x + f * sn);
-      }
-#pragma unroll
-      for (int i = 0; i < N / V; ++i) {
-        Pk pk;
-#pragma unroll
-        for (int e = 0; e < V; ++e) pk.v[e] = x[i * V + e];
-        *reinterpret_cast<Pk*>(dst + c + i * V) = pk;
-      }
-    } else {
-      const int c = u * V;
-      Pk x = *reinterpret_cast<const Pk*>(src + c), y = *reinterpret_cast<const Pk*>(src + c + a.R / 2);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float2 cs = __ldg(tab + c + e);
-        const float sn = cs.y * a.sign, f = to_f<T>(x.v[e]), g = to_f<T>(y.v[e]);
-        x.v[e] = from_f<T>(f * cs.x - g * sn);
-        y.v[e] = from_f<T>(g * cs.x + f * sn);
-      }
-      *reinterpret_cast<Pk*>(dst + c) = x;
-      *reinterpret_cast<Pk*>(dst + c + a.R / 2) = y;
+      *reinterpret_cast<Pk*>(dst[it]) = x[it][0];
     }
   }
 }
 
+unsigned magic(unsigned d) { return d <= 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d); }
+
 template <typename T, int V, bool IL>
 int launch(const void* q, const void* k, void* oq, void* ok, const Args& a, cudaStream_t stream) {
-  const int turn = IL ? a.R / (V == 1 ? 2 : V) : a.R / 2 / V;
-  const int units = turn + (a.D - a.R) / V;
-  const long long items = (long long)a.B * a.T * (a.H + a.HK) * units;
-  const long long grid = (items + kThreads * kItems - 1) / (kThreads * kItems);
-  if (grid > 0x7fffffffll) return GD_ERR_SHAPE;
-  rotary_kernel<T, V, IL><<<(unsigned)grid, kThreads, 0, stream>>>(static_cast<const T*>(q), static_cast<const T*>(k),
-                                                                  static_cast<T*>(oq), static_cast<T*>(ok), a, turn,
-                                                                  units, items);
+  Items n;
+  n.turn = IL ? a.R / (V == 1 ? 2 : V) : a.R / 2 / V;
+  n.copy = (a.D - a.R) / V;
+  const unsigned heads = (unsigned)(a.H + a.HK), per_token = heads * (unsigned)(n.turn + n.copy);
+  // as many tokens as give each thread twice kItems units; one where a token has more, or where that leaves SMs idle
+  int tokens = (int)(kThreads * 2 * kItems / per_token);
+  while (tokens > 1 && (long long)a.B * ((a.T + tokens - 1) / tokens) < 148) tokens /= 2;
+  if (tokens < 1) tokens = 1;
+  n.tokens = tokens;
+  n.m_turn = magic(n.turn), n.m_copy = magic(n.copy);
+  n.m_hturn = magic(heads * n.turn), n.m_hcopy = magic(heads * n.copy);
+  rotary_kernel<T, V, IL>
+      <<<dim3((unsigned)((a.T + tokens - 1) / tokens), (unsigned)a.B), kThreads, 0, stream>>>(
+          static_cast<const T*>(q), static_cast<const T*>(k), static_cast<T*>(oq), static_cast<T*>(ok), a, n);
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
 }
 
@@ -163,7 +205,7 @@ extern "C" int gd_rotary(const void* q, const void* k, void* oq, void* ok, const
                          long long k_stride_b, long long k_stride_t, long long k_stride_h, int interleaved, int inverse,
                          void* stream) {
   if (dtype != GD_FLOAT32 && dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) return GD_ERR_ARG;
-  if (B < 0 || T < 0 || H < 0 || HK < 0 || D <= 0 || R <= 0 || R % 2 != 0 || R > D || table_rows < 0) return GD_ERR_SHAPE;
+  if (B < 0 || B > 65535 || T < 0 || H < 0 || HK < 0 || D <= 0 || R <= 0 || R % 2 != 0 || R > D || table_rows < 0) return GD_ERR_SHAPE;
   if ((long long)B * T == 0 || H + HK == 0) return GD_OK;
   if (table_rows == 0 || (long long)(H + HK) * D > 0x3fffffff) return GD_ERR_SHAPE;
   if (table == nullptr || (H > 0 && (q == nullptr || oq == nullptr)) || (HK > 0 && (k == nullptr || ok == nullptr)))
@@ -194,6 +236,7 @@ extern "C" int gd_rotary(const void* q, const void* k, void* oq, void* ok, const
   a.P = table_rows;
   a.B = B, a.T = T, a.H = H, a.HK = HK, a.D = D, a.R = R;
   a.sign = inverse ? -1.f : 1.f;
+  a.table16 = reinterpret_cast<uintptr_t>(table) % 16 == 0 && R % 4 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == GD_FLOAT32) return by_layout<float>(interleaved, v, q, k, oq, ok, a, s);
   if (dtype == GD_FLOAT16) return by_layout<__half>(interleaved, v, q, k, oq, ok, a, s);

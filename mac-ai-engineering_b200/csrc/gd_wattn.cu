@@ -21,7 +21,7 @@ int check(const void* q, const void* k, const void* v, const long long* strides,
           int Tq, int Tk, int H, int HK, int D, int window, int sinks, float scale) {
   if (dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) return GD_ERR_ARG;
   if (B < 0 || Tq < 0 || Tk < 0 || B > 65535 || Tq > (1 << 29) || Tk > (1 << 29) || H <= 0 || HK <= 0 || H > 65535 ||
-      H % HK != 0 || D <= 0 || D % 8 != 0 || D > 256 || window < 0 || sinks < 0 || !std::isfinite(scale))
+      H % HK != 0 || (long long)Tq * H >= (1ll << 31) || D <= 0 || D % 8 != 0 || D > 256 || window < 0 || sinks < 0 || !std::isfinite(scale))
     return GD_ERR_SHAPE;
   if (cu != nullptr && (B != 1 || Tq != Tk || N <= 0 || N > (1 << 24))) return GD_ERR_SHAPE;
   if (B == 0 || Tq == 0) return GD_OK;

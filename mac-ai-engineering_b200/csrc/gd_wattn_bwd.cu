@@ -38,26 +38,32 @@ constexpr int kRowsEach = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, const T* __restrict__ low,
                                                     const T* __restrict__ g, long long gb, long long gt, long long gh,
-                                                    float* __restrict__ delta, int B, int Tq, int H, int D, ErrorWord* err) {
+                                                    float* __restrict__ delta, int Tq, int H, int D, ErrorWord* err) {
   const int sub = threadIdx.x & 15;
-  const long long rows = (long long)B * Tq * H, row0 = (long long)blockIdx.x * (16 * kRowsEach) + (threadIdx.x >> 4);
+  const unsigned rows = (unsigned)Tq * (unsigned)H;  // of batch row blockIdx.y
+  const unsigned row0 = blockIdx.x * (16 * kRowsEach) + (threadIdx.x >> 4);
+  o += (long long)blockIdx.y * rows * D;
+  low += (long long)blockIdx.y * rows * D;
+  g += blockIdx.y * gb;
+  delta += (long long)blockIdx.y * rows;
   float s[kRowsEach], top = 0.f;
-  long long to[kRowsEach];
+  unsigned h[kRowsEach], t[kRowsEach];
 #pragma unroll
-  for (int r = 0; r < kRowsEach; ++r) s[r] = 0.f;
+  for (int r = 0; r < kRowsEach; ++r) {
+    s[r] = 0.f;
+    t[r] = (row0 + r * 16) / (unsigned)H;
+    h[r] = row0 + r * 16 - t[r] * (unsigned)H;
+  }
   for (int c = sub * 8; c < D; c += 128) {
     uint4 a[kRowsEach], l[kRowsEach], d[kRowsEach];
 #pragma unroll
     for (int r = 0; r < kRowsEach; ++r) {
-      const long long row = row0 + r * 16;
+      const unsigned row = row0 + r * 16;
       a[r] = l[r] = d[r] = make_uint4(0, 0, 0, 0);
       if (row < rows) {
-        const unsigned h = (unsigned)(row % H);
-        const long long bt = row / H, b = bt / Tq, t = bt - b * Tq;
-        to[r] = (b * H + h) * Tq + t;
-        a[r] = __ldg(reinterpret_cast<const uint4*>(o + row * D + c));
-        l[r] = __ldg(reinterpret_cast<const uint4*>(low + row * D + c));
-        d[r] = __ldg(reinterpret_cast<const uint4*>(g + b * gb + t * gt + h * gh + c));
+        a[r] = __ldg(reinterpret_cast<const uint4*>(o + (long long)row * D + c));
+        l[r] = __ldg(reinterpret_cast<const uint4*>(low + (long long)row * D + c));
+        d[r] = __ldg(reinterpret_cast<const uint4*>(g + t[r] * gt + h[r] * gh + c));
       }
     }
 #pragma unroll
@@ -77,7 +83,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, con
   for (int r = 0; r < kRowsEach; ++r) {
 #pragma unroll
     for (int w = 8; w >= 1; w >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], w);
-    if (row0 + r * 16 < rows && sub == 0) delta[to[r]] = s[r];
+    if (row0 + r * 16 < rows && sub == 0) delta[(long long)h[r] * Tq + t[r]] = s[r];
   }
   if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
@@ -808,10 +814,10 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
       !tile_map(&mv, v, dt, pr.B, pr.Tk, pr.HK, pr.D, st[6], st[7], st[8], kTile) ||
       !tile_map(&mo, g, dt, pr.B, pr.Tq, pr.H, pr.D, st[9], st[10], st[11], kTile))
     return GD_ERR_LAUNCH;
-  const long long rows = (long long)pr.B * pr.Tq * pr.H;
-  delta_kernel<T><<<(unsigned)((rows + 16 * kRowsEach - 1) / (16 * kRowsEach)), 256, 0, stream>>>(
-      static_cast<const T*>(o), static_cast<const T*>(low), static_cast<const T*>(g), st[9], st[10], st[11], delta, pr.B,
-      pr.Tq, pr.H, pr.D, err);
+  const long long rows = (long long)pr.Tq * pr.H;
+  delta_kernel<T><<<dim3((unsigned)((rows + 16 * kRowsEach - 1) / (16 * kRowsEach)), (unsigned)pr.B), 256, 0, stream>>>(
+      static_cast<const T*>(o), static_cast<const T*>(low), static_cast<const T*>(g), st[9], st[10], st[11], delta, pr.Tq,
+      pr.H, pr.D, err);
   static bool done_q[kMaxDevices], done_kv[kMaxDevices];
   auto kq = dq_kernel<T, NS>;
   auto kkv = dkv_kernel<T, NS>;

@@ -27,15 +27,18 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 16;   // keys a warp takes at a time
 constexpr int kRows = 16;   // query heads of a CTA
 constexpr int kMaxClusters = 32;
+constexpr int kSms = 148;   // of a B200
+static_assert(kThreads == 8 * kRows, "the join's factors: eight threads a row");
 
 template <int DP>
 struct Cfg {
   static constexpr int kStages = 3;
   static constexpr int kHalf = kStep * DP * 2;  // a step's keys (or values)
   static constexpr int kWarpBytes = kStages * 2 * kHalf;
-  static constexpr int kQBytes = kRows * DP * 2;
+  static constexpr int kQBytes = kRows * DP * 2 > 2304 ? kRows * DP * 2 : 2304;
   static constexpr size_t kSmem = kQBytes + kWarps * (size_t)kWarpBytes + 2 * kWarps * kRows * sizeof(float);
   static_assert(kWarpBytes >= kRows * DP * 4, "a warp's sums fit in its stages");
+  static_assert(kQBytes >= (8 * kWarps + 2) * kRows * 4, "the join's factors fit in Q's place");
 };
 
 struct StepArgs {
@@ -279,30 +282,50 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const StepArgs a) {
     ls[warp * kRows + r + 8] = l1;
   }
   cluster.sync();
-  // each CTA of the cluster joins its share of the (head, channel) pairs over all its CTAs and warps, in order
-  const int clusters = gridDim.x / cs, rank = (int)cluster.block_rank();
+  // each CTA of the cluster joins its share of the (head, channel) pairs over all its CTAs' warps (the parts), in order.
+  // First the parts' factors exp2(maximum - overall maximum), and the overall sums: Q's place, free by now
+  const int clusters = gridDim.x / cs, rank = (int)cluster.block_rank(), parts = cs * kWarps;
+  float* fac = reinterpret_cast<float*>(smem);  // [part][16]
+  float* tops = fac + 8 * kWarps * kRows;       // [16], then the sums [16]
+  {
+    const int row = threadIdx.x >> 3, x = threadIdx.x & 7;  // eight threads a row, a CTA of the cluster each
+    const float* rm = cluster.map_shared_rank(ms, x < cs ? x : 0);
+    const float* rl = cluster.map_shared_rank(ls, x < cs ? x : 0);
+    float mw[kWarps], lw[kWarps], top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      mw[w] = x < cs ? rm[w * kRows + row] : -INFINITY;
+      lw[w] = x < cs ? rl[w * kRows + row] : 0.f;
+      top = fmaxf(top, mw[w]);
+    }
+#pragma unroll
+    for (int o = 1; o <= 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = mw[w] == -INFINITY ? 0.f : ex2f(mw[w] - top);
+      if (x < cs) fac[(x * kWarps + w) * kRows + row] = f;
+      l = fmaf(lw[w], f, l);
+    }
+#pragma unroll
+    for (int o = 1; o <= 4; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (x == 0) {
+      tops[row] = top;
+      tops[kRows + row] = l;
+    }
+  }
+  __syncthreads();
   for (int i = rank * kThreads + threadIdx.x; i < rows * (a.D / 2); i += cs * kThreads) {
     const int row = i / (a.D / 2), c = i % (a.D / 2) * 2;
-    float top = -INFINITY;
-    for (int x = 0; x < cs; ++x) {
-      const float* rm = cluster.map_shared_rank(ms, x);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, rm[w * kRows + row]);
-    }
-    float l = 0.f, y0 = 0.f, y1 = 0.f;
-    for (int x = 0; x < cs; ++x) {
-      const float* rm = cluster.map_shared_rank(ms, x);
-      const float* rl = cluster.map_shared_rank(ls, x);
-      const float* ra = cluster.map_shared_rank(reinterpret_cast<float*>(smem + C::kQBytes), x);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float mw = rm[w * kRows + row], lw = rl[w * kRows + row];
-        const float f = mw == -INFINITY ? 0.f : ex2f(mw - top);
-        const float2 z = *reinterpret_cast<const float2*>(ra + w * (C::kWarpBytes / 4) + row * DP + c);
-        l = fmaf(lw, f, l);
-        y0 = fmaf(z.x, f, y0);
-        y1 = fmaf(z.y, f, y1);
-      }
+    const float top = tops[row], l = tops[kRows + row];
+    float y0 = 0.f, y1 = 0.f;
+#pragma unroll 8
+    for (int x = 0; x < parts; ++x) {
+      const float* ra = cluster.map_shared_rank(reinterpret_cast<float*>(smem + C::kQBytes), x / kWarps);
+      const float2 z = *reinterpret_cast<const float2*>(ra + x % kWarps * (C::kWarpBytes / 4) + row * DP + c);
+      const float f = fac[x * kRows + row];
+      y0 = fmaf(z.x, f, y0);
+      y1 = fmaf(z.y, f, y1);
     }
     // NaN scores appear in no maximum but in the sums, and stay NaN
     if (clusters > 1) {
@@ -342,20 +365,20 @@ __global__ void __launch_bounds__(256) step_join(const StepArgs a, int clusters)
   }
 }
 
-// CTAs of a cluster and clusters per (request, key head): enough for two CTAs an SM, at least 64 keys (a step for each
-// warp) a CTA at the most that can be visible.
+// CTAs of a cluster and clusters per (request, key head): enough to give every SM a CTA, at least 64 keys (a step for
+// each warp) a CTA at the most that can be visible; a second kernel's launch pays from 512 keys a CTA.
 struct Split {
   int cs, clusters;
 };
 Split split_of(int B, int S, int HK, int groups, int window, int sinks) {
   long long most = window == 0 ? S : (long long)window + sinks;
   if (most > S) most = S;
-  long long want = (2 * 148 + (long long)B * HK * groups - 1) / ((long long)B * HK * groups);
+  long long want = (kSms + (long long)B * HK * groups - 1) / ((long long)B * HK * groups);
   const long long fit = (most + kWarps * kStep - 1) / (kWarps * kStep);
   if (want > fit) want = fit;
   Split s = {1, 1};
   while (s.cs < 8 && s.cs * 2 <= want) s.cs *= 2;
-  if (want > 8) s.clusters = (int)((want + 7) / 8 < kMaxClusters ? (want + 7) / 8 : kMaxClusters);
+  if (want > 8 && most > 8 * 512) s.clusters = (int)((want + 7) / 8 < kMaxClusters ? (want + 7) / 8 : kMaxClusters);
   return s;
 }
 size_t part_bytes(int B, int HK, int groups, int D, const Split& s) {
