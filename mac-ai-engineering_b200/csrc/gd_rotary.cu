@@ -4,9 +4,10 @@
 // with pairs (i, i + R/2) (half layout) or (2 i, 2 i + 1) (interleaved), cos and sin from a table [P, R/2, 2] in fp32
 // indexed by the token's position. The backward is the turn by the opposite angle (sign = -1).
 //
-// Bound by HBM: every channel of q and k is read and written once; a token's R/2 angles serve all its heads (through shared memory). q and k may be views of a fused projection (any batch, token and head stride);
-// outputs are contiguous. A unit of work is V channels of a head that pass through or are turned among themselves
-// (interleaved), or the two V-channel halves of V pairs; V is the widest that divides widths, strides and addresses.
+// Bound by HBM: every channel of q and k is read and written once; a token's R/2 angles serve all its heads (they come
+// from L1 and L2 after the first). q and k may be views of a fused projection (any batch, token and head stride); outputs
+// are contiguous. A unit of work is V channels of a head that pass through or are turned among themselves (interleaved),
+// or the two V-channel halves of V pairs; V is the widest that divides widths, strides and addresses.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -18,8 +19,8 @@
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kItems = 2;  // units a thread has in flight: with 48 warps an SM, enough; more registers cost more warps
+constexpr int kMaxThreads = 512;
+constexpr int kTokens = 4;  // of a CTA
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
@@ -54,133 +55,96 @@ struct Args {
   bool table16;           // every row of the table starts on 16 bytes
 };
 
-// n / d for n < 2^16 and d <= 2^16, by m = ceil(2^32 / d): n m is off n 2^32 / d by less than n d <= 2^32
-__device__ __forceinline__ unsigned div16(unsigned n, unsigned m) { return m == 0u ? n : __umulhi(n, m); }
-
-// How a CTA's items are numbered: first the turned units of its tokens, (token, head, unit), then the copied ones, so that
-// a warp does one or the other.
-struct Items {
-  int tokens;                       // of a CTA
-  int turn, copy;                   // units of a head
-  unsigned m_turn, m_copy;          // div16's numbers: of turn, copy
-  unsigned m_hturn, m_hcopy;        // of heads * turn, heads * copy
-};
-
-// A CTA takes `tokens` consecutive tokens of a batch row. A thread's items lie kThreads apart; their loads are in flight
-// before any arithmetic.
+// A thread has one unit of one head (the turned units first, so that a warp turns or copies) and walks the CTA's tokens:
+// the address arithmetic of an item is done once, not once per token. Warps, not loads per thread, keep memory busy: with
+// one token's loads in flight a thread needs 40 registers, and q, k of 4 x 4096 tokens (16 + 4 heads of 128, 32 turned,
+// bf16, views of a fused projection) take 35 us (4.9 TB/s); with two tokens ahead 49 us, with four 65 us.
 template <typename T, int V, bool IL>
-__global__ void __launch_bounds__(kThreads, 6) rotary_kernel(const T* __restrict__ q, const T* __restrict__ k,
+__global__ void __launch_bounds__(kMaxThreads, 3) rotary_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                              T* __restrict__ oq, T* __restrict__ ok, const Args a,
-                                                             const Items n) {
+                                                             const int turn_units, const int copy_units, const int tokens) {
   constexpr int N = IL && V == 1 ? 2 : V;  // channels of a turned unit (of each half of its pairs in the half layout)
   constexpr int L = N / V;                 // packs of it
   constexpr int A = IL ? N / 2 : V;        // angles of it
   using Pk = Pack<T, V>;
-  const unsigned heads = a.H + a.HK;
-  const int b = blockIdx.y, t0 = blockIdx.x * n.tokens, here = a.T - t0 < n.tokens ? a.T - t0 : n.tokens;
-  const unsigned turned = (unsigned)here * heads * n.turn, items = turned + (unsigned)here * heads * n.copy;
-  const bool small = items <= 65536u;  // (a CTA of one token may have more: it divides)
-  for (unsigned first = threadIdx.x; first < items; first += kThreads * kItems) {
-    Pk x[kItems][L], y[kItems];
-    T* dst[kItems];
-    const float2* cs[kItems];  // a turned item's angles
-    bool live[kItems];
+  const unsigned heads = a.H + a.HK, turned = heads * turn_units;
+  unsigned i = blockIdx.z * blockDim.x + threadIdx.x;
+  if (i >= turned + heads * copy_units) return;
+  const bool turn = i < turned;
+  if (!turn) i -= turned;
+  const unsigned units = turn ? turn_units : copy_units, hh = i / units, u = i - hh * units;
+  const int b = blockIdx.y, t0 = blockIdx.x * tokens, t1 = a.T - t0 < tokens ? a.T : t0 + tokens;
+  const bool is_q = hh < (unsigned)a.H;
+  const Rows in = is_q ? a.q : a.k;
+  const long long h = is_q ? hh : hh - a.H, nh = is_q ? a.H : a.HK;
+  const int c = turn ? (int)u * N : a.R + (int)u * V;
+  const T* src = (is_q ? q : k) + b * in.b + t0 * in.t + h * in.h + c;
+  T* dst = (is_q ? oq : ok) + (((long long)b * a.T + t0) * nh + h) * a.D + c;
+  const long long sstep = in.t, dstep = nh * a.D;
+  if (!turn) {
+    for (int t = t0; t < t1; ++t, src += sstep, dst += dstep) *reinterpret_cast<Pk*>(dst) = *reinterpret_cast<const Pk*>(src);
+    return;
+  }
+  for (int t = t0; t < t1; ++t, src += sstep, dst += dstep) {
+    Pk x[L], y;
+    float2 an[A];
 #pragma unroll
-    for (int it = 0; it < kItems; ++it) {
-      unsigned i = first + it * kThreads;
-      live[it] = i < items;
-      cs[it] = nullptr;
-      if (!live[it]) continue;
-      const bool turn = i < turned;
-      if (!turn) i -= turned;
-      const unsigned units = turn ? n.turn : n.copy, per_token = heads * units;
-      const unsigned tt = small ? div16(i, turn ? n.m_hturn : n.m_hcopy) : i / per_token, rest = i - tt * per_token;
-      const unsigned hh = small ? div16(rest, turn ? n.m_turn : n.m_copy) : rest / units, u = rest - hh * units;
-      const int t = t0 + (int)tt;
-      const bool is_q = hh < (unsigned)a.H;
-      const long long h = is_q ? hh : hh - a.H, token = (long long)b * a.T + t;
-      const int c = turn ? (int)u * N : a.R + (int)u * V;
-      const T* src = (is_q ? q + b * a.q.b + t * a.q.t + h * a.q.h : k + b * a.k.b + t * a.k.t + h * a.k.h) + c;
-      dst[it] = (is_q ? oq + (token * a.H + h) * a.D : ok + (token * a.HK + h) * a.D) + c;
-      x[it][0] = *reinterpret_cast<const Pk*>(src);
-      if (turn) {
+    for (int l = 0; l < L; ++l) x[l] = *reinterpret_cast<const Pk*>(src + l * V);
+    if (!IL) y = *reinterpret_cast<const Pk*>(src + a.R / 2);
+    long long p = t;
+    if (a.positions != nullptr) {
+      const long long w = b * a.pos_b + t;
+      p = a.pos64 ? __ldg(static_cast<const long long*>(a.positions) + w)
+                  : (long long)__ldg(static_cast<const int*>(a.positions) + w);
+    }
+    p = p < 0 ? 0 : p >= a.P ? a.P - 1 : p;  // never outside the table
+    const float2* cs = a.table + p * (a.R / 2) + (IL ? c / 2 : c);
+    if (A % 2 == 0 && a.table16) {  // an even number of angles starts on 16 bytes when the table's rows do
 #pragma unroll
-        for (int l = 1; l < L; ++l) x[it][l] = *reinterpret_cast<const Pk*>(src + l * V);
-        if (!IL) y[it] = *reinterpret_cast<const Pk*>(src + a.R / 2);
-        long long p = t;
-        if (a.positions != nullptr) {
-          const long long w = b * a.pos_b + t;
-          p = a.pos64 ? __ldg(static_cast<const long long*>(a.positions) + w)
-                      : (long long)__ldg(static_cast<const int*>(a.positions) + w);
-        }
-        p = p < 0 ? 0 : p >= a.P ? a.P - 1 : p;  // never outside the table
-        cs[it] = a.table + p * (a.R / 2) + (IL ? c / 2 : c);
+      for (int e = 0; e + 1 < A; e += 2) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(cs + e));
+        an[e] = make_float2(v.x, v.y);
+        an[e + 1] = make_float2(v.z, v.w);
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < A; ++e) an[e] = __ldg(cs + e);
+    }
+    if constexpr (IL) {
+      T* v = reinterpret_cast<T*>(x);
+#pragma unroll
+      for (int e = 0; e < A; ++e) {
+        const float f = to_f<T>(v[2 * e]), g = to_f<T>(v[2 * e + 1]), sn = an[e].y * a.sign;
+        v[2 * e] = from_f<T>(f * an[e].x - g * sn);
+        v[2 * e + 1] = from_f<T>(g * an[e].x + f * sn);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < A; ++e) {
+        const float f = to_f<T>(x[0].v[e]), g = to_f<T>(y.v[e]), sn = an[e].y * a.sign;
+        x[0].v[e] = from_f<T>(f * an[e].x - g * sn);
+        y.v[e] = from_f<T>(g * an[e].x + f * sn);
+      }
+      *reinterpret_cast<Pk*>(dst + a.R / 2) = y;
     }
 #pragma unroll
-    for (int it = 0; it < kItems; ++it) {
-      if (!live[it]) continue;
-      if (cs[it] != nullptr) {
-        float2 t[A];
-        if constexpr (A % 2 == 0) {  // an even number of angles starts on 16 bytes when the table does
-          if (a.table16) {
-#pragma unroll
-            for (int i = 0; i < A; i += 2) {
-              const float4 v = __ldg(reinterpret_cast<const float4*>(cs[it] + i));
-              t[i] = make_float2(v.x, v.y);
-              t[i + 1] = make_float2(v.z, v.w);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < A; ++i) t[i] = __ldg(cs[it] + i);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < A; ++i) t[i] = __ldg(cs[it] + i);
-        }
-        if constexpr (IL) {
-          T* v = reinterpret_cast<T*>(x[it]);
-#pragma unroll
-          for (int i = 0; i < A; ++i) {
-            const float f = to_f<T>(v[2 * i]), g = to_f<T>(v[2 * i + 1]), sn = t[i].y * a.sign;
-            v[2 * i] = from_f<T>(f * t[i].x - g * sn);
-            v[2 * i + 1] = from_f<T>(g * t[i].x + f * sn);
-          }
-#pragma unroll
-          for (int l = 1; l < L; ++l) *reinterpret_cast<Pk*>(dst[it] + l * V) = x[it][l];
-        } else {
-#pragma unroll
-          for (int e = 0; e < A; ++e) {
-            const float f = to_f<T>(x[it][0].v[e]), g = to_f<T>(y[it].v[e]), sn = t[e].y * a.sign;
-            x[it][0].v[e] = from_f<T>(f * t[e].x - g * sn);
-            y[it].v[e] = from_f<T>(g * t[e].x + f * sn);
-          }
-          *reinterpret_cast<Pk*>(dst[it] + a.R / 2) = y[it];
-        }
-      }
-      *reinterpret_cast<Pk*>(dst[it]) = x[it][0];
-    }
+    for (int l = 0; l < L; ++l) *reinterpret_cast<Pk*>(dst + l * V) = x[l];
   }
 }
 
-unsigned magic(unsigned d) { return d <= 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d); }
-
 template <typename T, int V, bool IL>
 int launch(const void* q, const void* k, void* oq, void* ok, const Args& a, cudaStream_t stream) {
-  Items n;
-  n.turn = IL ? a.R / (V == 1 ? 2 : V) : a.R / 2 / V;
-  n.copy = (a.D - a.R) / V;
-  const unsigned heads = (unsigned)(a.H + a.HK), per_token = heads * (unsigned)(n.turn + n.copy);
-  // as many tokens as give each thread twice kItems units; one where a token has more, or where that leaves SMs idle
-  int tokens = (int)(kThreads * 2 * kItems / per_token);
-  while (tokens > 1 && (long long)a.B * ((a.T + tokens - 1) / tokens) < 148) tokens /= 2;
-  if (tokens < 1) tokens = 1;
-  n.tokens = tokens;
-  n.m_turn = magic(n.turn), n.m_copy = magic(n.copy);
-  n.m_hturn = magic(heads * n.turn), n.m_hcopy = magic(heads * n.copy);
-  rotary_kernel<T, V, IL>
-      <<<dim3((unsigned)((a.T + tokens - 1) / tokens), (unsigned)a.B), kThreads, 0, stream>>>(
-          static_cast<const T*>(q), static_cast<const T*>(k), static_cast<T*>(oq), static_cast<T*>(ok), a, n);
+  const int turn = IL ? a.R / (V == 1 ? 2 : V) : a.R / 2 / V, copy = (a.D - a.R) / V;
+  const long long items = (long long)(a.H + a.HK) * (turn + copy);
+  const long long passes = (items + kMaxThreads - 1) / kMaxThreads;
+  if (passes > 65535) return GD_ERR_SHAPE;
+  const int threads = (int)((items + passes * 32 - 1) / (passes * 32)) * 32;
+  // fewer tokens a CTA where that many leave SMs with less than 1,024 threads
+  int tokens = kTokens;
+  while (tokens > 1 && (long long)a.B * ((a.T + tokens - 1) / tokens) * passes * threads < 148 * 1024) tokens /= 2;
+  rotary_kernel<T, V, IL><<<dim3((unsigned)((a.T + tokens - 1) / tokens), (unsigned)a.B, (unsigned)passes), threads, 0,
+                            stream>>>(static_cast<const T*>(q), static_cast<const T*>(k), static_cast<T*>(oq),
+                                      static_cast<T*>(ok), a, turn, copy, tokens);
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
 }
 
