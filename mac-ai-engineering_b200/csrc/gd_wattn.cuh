@@ -171,22 +171,22 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(id), "r"(acc)
       : "memory");
 }
-// D[128 x 128] = X Y^T, both tiles of NS slabs, contracted over their channels
-template <typename T, int NS>
+// D[128 x N] = X Y^T: X 128 rows, Y N rows, of NS slabs, contracted over their channels
+template <typename T, int NS, int N = 128>
 __device__ __forceinline__ void mma_xyt(uint32_t d, uint32_t x, uint32_t y, bool acc = false) {
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      mma_bf16(d, desc_k(x + s * kSlabBytes) + 2 * k, desc_k(y + s * kSlabBytes) + 2 * k, idesc<T>(128, 128, false),
+      mma_bf16(d, desc_k(x + s * kSlabBytes) + 2 * k, desc_k(y + s * kSlabBytes) + 2 * k, idesc<T>(128, N, false),
                acc || s > 0 || k > 0);
 }
-// D[128 x NS 64] (+)= P Y: P in TMEM (128 rows, 128 contracted columns as 64 words), Y's rows contracted. P stands in
+// D[128 x NS 64] (+)= P Y: P in TMEM (128 rows, 16 K contracted columns as 8 K words), Y's rows contracted. P stands in
 // pieces of 32 contracted columns (16 words), `gap` words apart.
-template <typename T, int NS>
+template <typename T, int NS, int K = 8>
 __device__ __forceinline__ void mma_py(uint32_t d, uint32_t p, uint32_t y, bool acc, int gap) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = 0; k < K; ++k)
     mma_ts(d, p + (k & 1) * 8 + (k >> 1) * gap, desc_mn(y) + 128 * k, idesc<T>(128, NS * 64, true), acc || k > 0);
 }
 
@@ -296,6 +296,39 @@ template <typename T>
 __device__ __forceinline__ float2 unpack16(uint32_t u) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&u));
   else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+
+// byte of 16-byte chunk c (8 channels) of a row in a swizzled tile
+__device__ __forceinline__ uint32_t tile_at(int row, int c) {
+  return (c >> 3) * kSlabBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void st_shared16(uint32_t a, const uint32_t (&u)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+}
+// A warp's rows row0 .. row0 + N - 1 of a swizzled tile -> tokens t0 + row of a [T, heads, D] array (`out`: its head's first
+// channel), rows below `live` only; 16-byte pieces, a row's adjacent
+template <typename T, int N = 32>
+__device__ __forceinline__ void store_rows(T* out, uint32_t smem, int row0, int t0, int live, int heads, int D) {
+  const int chunks = D >> 3, lane = threadIdx.x & 31;
+  int r = lane / chunks, c = lane % chunks;
+  const int dr = 32 / chunks, dc = 32 % chunks;
+#pragma unroll 4
+  for (; r < N;) {
+    if (row0 + r < live) {
+      uint4 u;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                   : "r"(smem + tile_at(row0 + r, c))
+                   : "memory");
+      *reinterpret_cast<uint4*>(out + ((long long)(t0 + row0 + r) * heads) * D + c * 8) = u;
+    }
+    r += dr;
+    c += dc;
+    if (c >= chunks) {
+      c -= chunks;
+      ++r;
+    }
+  }
 }
 
 // The entry points' parts (host): strides of q, k, v in elements, (batch, token, head) each; low: what o's rounding took

@@ -3,57 +3,61 @@
 // in one pass over the keys with a running maximum and sum (fp32); O stays in TMEM between key tiles. A query without a
 // visible key gets zeros and L = +inf.
 //
-// One CTA takes 128 queries of a head. Roles: warps 0-7 softmax (TMEM lane = query row; two threads a row, 64 key columns
-// each, which agree on the row's maximum through shared memory when it moves), warp 8 loads (TMA), warp 9 issues the
-// products. Key tiles outside the window and past the first tokens are never loaded.
-//   S (128 x 128 fp32) comes from tcgen05 into TMEM; the softmax writes P over it as 16-bit pairs, where it is the A
-//   operand of P V (no trip through shared memory). P is rounded to the inputs' 16-bit type (the operand type of the
+// One CTA takes 128 queries of a head. Roles: warps 0-3 softmax (a thread owns a query row, TMEM lane = row), warp 4 loads
+// (TMA), warp 5 issues the products. Key tiles (128 keys) outside the window and past the first tokens are never loaded.
+//   S comes from tcgen05 into TMEM in halves of 64 keys; the softmax writes a half's P over it as 16-bit pairs, where it is
+//   the A operand of P V (no trip through shared memory). P is rounded to the inputs' 16-bit type (the operand type of the
 //   matrix instruction); its sum is taken before the rounding, in fp32.
 //   The maximum that P refers to moves only when a row outgrows it by 2^8: O is rescaled in TMEM then (rarely), and P
 //   stays below 2^8, far inside both 16-bit types.
-// D <= 128: two CTAs share an SM (<= 113 KB of shared memory, 256 TMEM columns each), so that one's products run under
-// the other's softmax. D <= 256: one CTA an SM, S double-buffered: the products of the next tile run under the softmax.
+// D <= 128: two CTAs share an SM (<= 100 KB of shared memory, 256 TMEM columns each). While the softmax works on one half,
+// the other half's P V and its next S run, so the softmax warps hardly wait: the exponentials (16 a clock and SM) and the
+// products share the SM's time. S of 64 keys at a time costs the product 1.5 times its shared-memory reads of Q; S of 128
+// keys in one buffer left every step's latency (4,200 clocks a tile and CTA) on the critical path.
+// D <= 256: one CTA an SM, S of 128 keys double-buffered, K and V pass in halves of 128 channels through a ring of five.
 #include "gd_wattn.cuh"
 
 namespace gd {
 namespace wattn {
 namespace {
 
-constexpr int kWarpsSm = 8;                     // softmax: two threads a query row, 64 columns each
+constexpr int kWarpsSm = 4;
 constexpr int kThreads = 32 * (kWarpsSm + 2);   // + loads, + products
-constexpr float kMaxGrowth = 8.f;  // log2
+constexpr float kMaxGrowth = 8.f;               // log2
 
 template <int NS>
 struct Cfg {
-  static constexpr int kBufs = NS == 4 ? 2 : 1;            // S buffers
-  static constexpr int kSlots = NS == 1 ? 4 : 2;           // K / V tiles in shared memory
-  static constexpr int kTileBytes = NS * kSlabBytes;
-  static constexpr int kCols = NS == 4 ? 512 : 256;        // TMEM columns
-  static constexpr int kO = kBufs * 128;                   // O's first column
-  static constexpr int kBarriers = 1 + 2 * kSlots + 2 * kBufs + 2;
-  static constexpr size_t kSmem = 1024 + (size_t)kTileBytes * (1 + kSlots) + 8 * kBarriers + 64 + 8 * kTile;
+  static constexpr bool kWide = NS == 4;
+  static constexpr int kSets = kWide ? 2 : 1;              // buffers of S of 128 keys (two halves each)
+  static constexpr int kUnit = (kWide ? 2 : NS) * kSlabBytes;
+  static constexpr int kSlots = kWide ? 5 : NS == 1 ? 4 : 2;  // K / V units in shared memory
+  static constexpr int kQBytes = NS * kSlabBytes;
+  static constexpr int kCols = kWide ? 512 : 256;          // TMEM columns
+  static constexpr int kO = kSets * 128;                   // O's first column
+  static constexpr int kBarriers = 1 + 2 * kSlots + 4 * kSets + 3;
+  static constexpr size_t kSmem = 1024 + kQBytes + (size_t)kUnit * kSlots + 8 * kBarriers + 64;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 template <typename T, int NS>
 __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                const __grid_constant__ CUtensorMap mv, const Problem pr, T* __restrict__ o, T* __restrict__ o_low,
-               float* __restrict__ lse,
-               ErrorWord* err) {
+               float* __restrict__ lse, ErrorWord* err) {
   using C = Cfg<NS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kTileBytes * (1 + C::kSlots));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kQBytes + C::kUnit * C::kSlots);
   uint64_t* q_full = bars;
   uint64_t* full = bars + 1;
   uint64_t* empty = full + C::kSlots;
-  uint64_t* s_full = empty + C::kSlots;
-  uint64_t* p_full = s_full + C::kBufs;
-  uint64_t* o_done = p_full + C::kBufs;
-  uint64_t* fin = o_done + 1;
+  uint64_t* s_full = empty + C::kSlots;       // of each half
+  uint64_t* p_full = s_full + 2 * C::kSets;
+  uint64_t* o_done = p_full + 2 * C::kSets;   // a phase per half's P V
+  uint64_t* t_done = o_done + 1;              // kWide: a phase per tile's P V
+  uint64_t* fin = o_done + 2;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   int* info = reinterpret_cast<int*>(tslot + 1);  // the packed sequence and tile of this CTA
-  float* xchg = reinterpret_cast<float*>(bars + C::kBarriers) + 16;  // [2][128]: a row's two threads
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -62,11 +66,12 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
     }
-    for (int i = 0; i < C::kBufs; ++i) {
+    for (int i = 0; i < 2 * C::kSets; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, kWarpsSm);
     }
     mbar_init(o_done, 1);
+    mbar_init(t_done, 1);
     mbar_init(fin, 1);
     fence_mbar_init();
   }
@@ -78,14 +83,12 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   const int item = gridDim.x - 1 - blockIdx.x, h = blockIdx.y;
   Seq sq;
   int tile = item;
-  if (pr.cu != nullptr) {
-    if (warp == 0) {
-      tile = find_item(pr.cu, pr.N, pr.Tq, item, [](int n) { return (n + kTile - 1) / kTile; }, sq);
-      if (lane == 0) {
-        info[0] = tile;
-        info[1] = sq.q0;
-        info[2] = sq.Tq;
-      }
+  if (pr.cu != nullptr && warp == 0) {
+    tile = find_item(pr.cu, pr.N, pr.Tq, item, [](int n) { return (n + kTile - 1) / kTile; }, sq);
+    if (lane == 0) {
+      info[0] = tile;
+      info[1] = sq.q0;
+      info[2] = sq.Tq;
     }
   }
   tc_fence_before();
@@ -104,20 +107,22 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   const int i1 = i0 + kTile - 1 < sq.Tq - 1 ? i0 + kTile - 1 : sq.Tq - 1;
   const int p0 = i0 + sq.offset(), p1 = i1 + sq.offset();
   const KeyRange kr(tile < 0 ? -1 : p0, tile < 0 ? -1 : p1, pr.window, pr.sinks);
-  const uint32_t s_q = smem_u32(base), s_kv = s_q + C::kTileBytes;
+  const uint32_t s_q = smem_u32(base), s_kv = s_q + C::kQBytes;
 
   if (warp == kWarpsSm) {
     if (lane == 0 && kr.n > 0) {
       const int hk = h / (pr.H / pr.HK);
-      mbar_arrive_expect_tx(q_full, C::kTileBytes);
+      constexpr int kPer = C::kWide ? 2 : 1;  // units of a tile
+      mbar_arrive_expect_tx(q_full, C::kQBytes);
       load_tile<NS>(s_q, &mq, h, sq.q0 + i0, sq.b, q_full);
       int c = 0;
-      bool ok = true;
-      for (; c < 2 * kr.n; ++c) {
-        const int slot = c % C::kSlots, use = c / C::kSlots;
-        if (use > 0 && !(ok = mbar_wait(empty + slot, (use - 1) & 1, err, 60))) break;
-        mbar_arrive_expect_tx(full + slot, C::kTileBytes);
-        load_tile<NS>(s_kv + slot * C::kTileBytes, (c & 1) ? &mv : &mk, hk, sq.k0 + kr.key(c >> 1), sq.b, full + slot);
+      for (; c < 2 * kPer * kr.n; ++c) {  // K's units, V's units, of tile after tile
+        const int slot = c % C::kSlots, use = c / C::kSlots, j = c / (2 * kPer), x = c % (2 * kPer);
+        if (use > 0 && !mbar_wait(empty + slot, (use - 1) & 1, err, 60)) break;
+        mbar_arrive_expect_tx(full + slot, C::kUnit);
+        const CUtensorMap* m = x < kPer ? &mk : &mv;
+        if constexpr (C::kWide) load_half(s_kv + slot * C::kUnit, m, x & 1, hk, sq.k0 + kr.key(j), sq.b, full + slot);
+        else load_tile<NS>(s_kv + slot * C::kUnit, m, hk, sq.k0 + kr.key(j), sq.b, full + slot);
       }
       // the copies in flight land before the CTA ends, whatever became of their readers
       mbar_wait(q_full, 0, err, 61);
@@ -126,49 +131,91 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   } else if (warp == kWarpsSm + 1) {
     if (lane == 0 && kr.n > 0) {
       bool ok = mbar_wait(q_full, 0, err, 62);
-      auto scores = [&](int j) {  // S of tile j
-        const int c = 2 * j, slot = c % C::kSlots, buf = j % C::kBufs;
-        if (!mbar_wait(full + slot, (c / C::kSlots) & 1, err, 63)) return false;
-        if (j >= C::kBufs && !mbar_wait(o_done, (j - C::kBufs) & 1, err, 64)) return false;  // P of the buffer is read
-        tc_fence_after();
-        mma_xyt<T, NS>(tm + buf * 128, s_q, s_kv + slot * C::kTileBytes);
-        mma_commit(empty + slot);
-        mma_commit(s_full + buf);
-        return true;
-      };
-      for (int j = 0; ok && j < C::kBufs - 1 && j < kr.n; ++j) ok = scores(j);
-      for (int j = 0; ok && j < kr.n; ++j) {
-        if (j + C::kBufs - 1 < kr.n) ok = scores(j + C::kBufs - 1);
-        const int c = 2 * j + 1, slot = c % C::kSlots, buf = j % C::kBufs;
-        ok = ok && mbar_wait(full + slot, (c / C::kSlots) & 1, err, 65) && mbar_wait(p_full + buf, (j / C::kBufs) & 1, err, 66);
-        if (!ok) break;
-        tc_fence_after();
-        mma_py<T, NS>(tm + C::kO, tm + buf * 128, s_kv + slot * C::kTileBytes, j > 0, 32);
-        mma_commit(empty + slot);
-        mma_commit(o_done);
+      auto landed = [&](int c) { return mbar_wait(full + c % C::kSlots, (c / C::kSlots) & 1, err, 63); };
+      if constexpr (!C::kWide) {
+        // units: K(j) = 2 j, V(j) = 2 j + 1; half x of tile j is half-tile 2 j + x
+        auto scores = [&](int j, int x) {
+          const int c = 2 * j;
+          if (x == 0 && !landed(c)) return false;
+          if (j > 0 && !mbar_wait(o_done, (2 * (j - 1) + x) & 1, err, 64)) return false;  // P over these columns is read
+          tc_fence_after();
+          mma_xyt<T, NS, 64>(tm + 64 * x, s_q, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128);
+          mma_commit(s_full + x);
+          if (x == 1) mma_commit(empty + c % C::kSlots);
+          return true;
+        };
+        ok = ok && scores(0, 0) && scores(0, 1);
+        for (int j = 0; ok && j < kr.n; ++j) {
+          const int c = 2 * j + 1;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (x == 0) ok = landed(c);
+            if (!(ok = ok && mbar_wait(p_full + x, j & 1, err, 66))) break;
+            tc_fence_after();
+            mma_py<T, NS, 4>(tm + C::kO, tm + 64 * x, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
+            if (x == 1) mma_commit(empty + c % C::kSlots);
+            mma_commit(o_done);
+            if (j + 1 < kr.n && !(ok = scores(j + 1, x))) break;
+          }
+        }
+      } else {
+        // units: K(j) = 4 j, 4 j + 1 and V(j) = 4 j + 2, 4 j + 3, by halves of the channels
+        auto scores = [&](int j) {
+          if (j >= 2 && !mbar_wait(t_done, j & 1, err, 64)) return false;  // of tile j - 2: P over these columns is read
+          const uint32_t d = tm + (j & 1) * 128;
+          for (int y = 0; y < 2; ++y) {
+            const int c = 4 * j + y;
+            if (!landed(c)) return false;
+            tc_fence_after();
+            mma_xyt<T, 2>(d, s_q + y * 2 * kSlabBytes, s_kv + c % C::kSlots * C::kUnit, y > 0);
+            mma_commit(empty + c % C::kSlots);
+          }
+          mma_commit(s_full + 2 * (j & 1));
+          mma_commit(s_full + 2 * (j & 1) + 1);
+          return true;
+        };
+        ok = ok && scores(0);
+        for (int j = 0; ok && j < kr.n; ++j) {
+          if (j + 1 < kr.n && !(ok = scores(j + 1))) break;
+          const int c = 4 * j + 2, set = j & 1;
+          ok = landed(c) && landed(c + 1);
+          for (int x = 0; ok && x < 2; ++x) {
+            if (!(ok = mbar_wait(p_full + 2 * set + x, (j >> 1) & 1, err, 66))) break;
+            tc_fence_after();
+            for (int y = 0; y < 2; ++y) {
+              const int v = (c + y) % C::kSlots;
+              mma_py<T, 2, 4>(tm + C::kO + y * 128, tm + set * 128 + 64 * x, s_kv + v * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
+              if (x == 1) mma_commit(empty + v);
+            }
+            mma_commit(o_done);
+          }
+          if (ok) mma_commit(t_done);
+        }
       }
       mma_commit(fin);
       mbar_wait(fin, 0, err, 67);
     }
   } else if (tile >= 0) {
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;  // TMEM lane, which 64 columns
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int pair = 1 + (warp & 3);  // named barrier of the two warps that share 32 rows
+    const int row = threadIdx.x;  // TMEM lane
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const int p = p0 + row;
-    float m = -INFINITY;             // the maximum P refers to (log2 units, of scaled scores): the same in both threads
-    F2 l2 = f2(0.f, 0.f);            // this thread's part of the sum
-    bool ok = true;                  // (a failed wait leaves the loop's barriers in step: both warps go on without waiting)
-    for (int j = 0; j < kr.n; ++j) {
-      const int buf = j % C::kBufs;
-      ok = ok && warp_wait(s_full + buf, (j / C::kBufs) & 1, err, 68);
+    float m = -INFINITY;  // the maximum P refers to (log2 units, of scaled scores)
+    F2 l2 = f2(0.f, 0.f);
+    bool ok = true;
+    const F2 sc = f2(pr.scale_log2, pr.scale_log2);
+    for (int t = 0; ok && t < 2 * kr.n; ++t) {  // half-tiles
+      const int j = t >> 1, x = t & 1, b = C::kWide ? t & 3 : x, phase = C::kWide ? j >> 1 : j;
+      if (!(ok = warp_wait(s_full + b, phase & 1, err, 68))) break;
+      // a wait on o_done tells phases t - 1 and t - 3 apart only once t - 2 is over: D <= 128, half-tile t's S was issued
+      // after that; else it is waited for
+      if (C::kWide && t >= 2 && !(ok = warp_wait(o_done, t & 1, err, 71))) break;
       tc_fence_after();
-      const uint32_t ts = tm + lanes + buf * 128 + half * 64;
+      const uint32_t ts = tm + lanes + b * 64;
       float s[64];
       tmem_ld64(ts, s);
-      const int c0 = kr.key(j);
-      if (!all_visible(c0, p0, p1, pr.window, pr.sinks)) {
-        const uint32_t v0 = visible_keys(c0 + half * 64, p, pr.window, pr.sinks);
-        const uint32_t v1 = visible_keys(c0 + half * 64 + 32, p, pr.window, pr.sinks);
+      const int c0 = kr.key(j) + 64 * x;
+      if (!all_visible(kr.key(j), p0, p1, pr.window, pr.sinks)) {
+        const uint32_t v0 = visible_keys(c0, p, pr.window, pr.sinks), v1 = visible_keys(c0 + 32, p, pr.window, pr.sinks);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           s[i] = (v0 >> i) & 1 ? s[i] : -INFINITY;
@@ -183,30 +230,17 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[60 + e]);
-      float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * pr.scale_log2;
-      // does a row of the two warps outgrow its reference (or meet its first visible key)?
-      uint32_t any;
-      asm volatile(
-          "{\n\t.reg .pred a, b;\n\t"
-          "setp.ne.u32 a, %1, 0;\n\t"
-          "barrier.cta.red.or.pred b, %2, 64, a;\n\t"
-          "selp.u32 %0, 1, 0, b;\n\t}\n"
-          : "=r"(any)
-          : "r"((uint32_t)(top > m + kMaxGrowth)), "r"(pair)
-          : "memory");
-      if (any) {
-        xchg[half * 128 + row] = top;
-        asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair) : "memory");
-        top = fmaxf(top, xchg[(half ^ 1) * 128 + row]);
-        const bool grow = top > m + kMaxGrowth;
+      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * pr.scale_log2;
+      const bool grow = top > m + kMaxGrowth;  // also a row's first visible key
+      if (__any_sync(0xffffffffu, grow)) {
         const float next = grow ? top : m;
         const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2(m - next);
         l2 = mul2(l2, f2(f, f));
-        if (j > 0) {  // O of the tiles so far, once their products are done; half of its columns each
-          ok = ok && warp_wait(o_done, (j - 1) & 1, err, 69);
+        if (t > 0) {  // O of the half-tiles so far, once their products are done
+          if (!(ok = warp_wait(o_done, (t - 1) & 1, err, 69))) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = half * NS * 32; c < (half + 1) * NS * 32; c += 16) {
+          for (int c = 0; c < NS * 64; c += 16) {
             float v[16];
             uint32_t u[16];
             tmem_ld16(tm + lanes + C::kO + c, v);
@@ -218,63 +252,69 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
         m = next;
       }
       const float ref = m == -INFINITY ? 0.f : m;
-      const F2 sc = f2(pr.scale_log2, pr.scale_log2), rf = f2(-ref, -ref);
+      const F2 rf = f2(-ref, -ref);
       F2 acc = f2(0.f, 0.f);
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t u[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float a, b;
-          unf2(fma2(f2(s[c + i], s[c + i + 1]), sc, rf), a, b);
+          float a, e;
+          unf2(fma2(f2(s[c + i], s[c + i + 1]), sc, rf), a, e);
           a = ex2(a);
-          b = ex2(b);
-          acc = add2(acc, f2(a, b));
-          u[i / 2] = pack16<T>(a, b);
+          e = ex2(e);
+          acc = add2(acc, f2(a, e));
+          u[i / 2] = pack16<T>(a, e);
         }
-        tmem_st16(ts + c, u);  // over this thread's own columns, a piece of 32 keys every 32 words
+        tmem_st16(ts + c / 2, u);
       }
       l2 = add2(l2, acc);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive_warp(p_full + buf);
+      mbar_arrive_warp(p_full + b);
     }
     if (kr.n > 0) {
-      ok = ok && warp_wait(o_done, (kr.n - 1) & 1, err, 70);
+      ok = ok && warp_wait(o_done, 0, err, 70) && warp_wait(o_done, 1, err, 70);  // half-tiles 2 n - 2, 2 n - 1
       tc_fence_after();
     }
     float l, lb;
     unf2(l2, l, lb);
     l += lb;
-    xchg[half * 128 + row] = l;  // (every row had its exchanges of the loop before the last barrier there)
-    asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair) : "memory");
-    l = xchg[row] + xchg[128 + row];
     const int i = i0 + row;
-    const bool live = i < sq.Tq;
-    const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;  // a wait that gave up leaves NaN
-    if (live && half == 0) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m + log2f(l);
-    const long long at = (((long long)sq.b * pr.Tq + sq.q0 + i) * pr.H + h) * pr.D;
-    const bool none = l == 0.f && ok;  // a row without a visible key: zeros, whatever O's columns hold
+    const bool none = l == 0.f && ok;                 // a row without a visible key: zeros, whatever O's columns hold
+    const float inv = !ok ? NAN : none ? 0.f : 1.f / l;  // a wait that gave up leaves NaN
+    if (i < sq.Tq) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m + log2f(l);
+    // out through shared memory (Q's place; a warp's own 32 rows), so that a row leaves as whole lines; then, for the
+    // backward's delta, what the rounding took away
+    for (int pass = 0; pass < (o_low != nullptr ? 2 : 1); ++pass) {
 #pragma unroll 1
-    for (int c = half * NS * 32; c < (half + 1) * NS * 32; c += 32) {
-      float v[32];
-      if (kr.n > 0) tmem_ld32(tm + lanes + C::kO + c, v);
-      if (!live) continue;
+      for (int c = 0; c < NS * 64; c += 32) {
+        float v[32];
+        if (kr.n > 0) {
+          tmem_ld32(tm + lanes + C::kO + c, v);
+        } else {
 #pragma unroll
-      for (int k = 0; k < 32; k += 8) {
-        if (c + k >= pr.D) break;
-        uint32_t u[4], w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = none ? 0.f : v[k + 2 * e] * inv, b = none ? 0.f : v[k + 2 * e + 1] * inv;
-          u[e] = pack16<T>(a, b);
-          const float2 r = unpack16<T>(u[e]);
-          w[e] = pack16<T>(a - r.x, b - r.y);
+          for (int k = 0; k < 32; ++k) v[k] = 0.f;
         }
-        *reinterpret_cast<uint4*>(o + at + c + k) = make_uint4(u[0], u[1], u[2], u[3]);
-        // what the rounding took away, for the backward's delta
-        if (o_low != nullptr) *reinterpret_cast<uint4*>(o_low + at + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          uint32_t u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = none ? 0.f : v[k + 2 * e] * inv, d = none ? 0.f : v[k + 2 * e + 1] * inv;
+            u[e] = pack16<T>(a, d);
+            if (pass == 1) {
+              const float2 r = unpack16<T>(u[e]);
+              u[e] = pack16<T>(a - r.x, d - r.y);
+            }
+          }
+          st_shared16(s_q + tile_at(row, (c + k) >> 3), u);
+        }
       }
+      __syncwarp();
+      T* out = pass == 0 ? o : o_low;
+      store_rows(out + ((long long)sq.b * pr.Tq * pr.H + h) * pr.D, s_q, warp * 32, sq.q0 + i0, sq.Tq - i0, pr.H, pr.D);
+      __syncwarp();
     }
   }
   tc_fence_before();
