@@ -147,47 +147,79 @@ __device__ __forceinline__ void load_half(uint32_t smem, const CUtensorMap* m, i
         : "memory");
 }
 
-// ---- tcgen05 operands in the 128-byte swizzle (layout type 2)
-// K-major: 8-row groups 1024 bytes apart; 16 channels further = 32 bytes
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// ---- tcgen05 products. The whole warp that issues them runs the same code, one elected lane's instructions take effect
+// (`lead`): warp-uniform addresses and descriptors stay in uniform registers, which the instruction reads. (Issued from a
+// branch of one lane, every product first moved its operands there: 80 to 100 clocks an instruction of 64.)
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t lead;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, e;\n\t}\n"
+      : "=r"(lead));
+  return lead;
 }
-// MN-major: 64-channel groups one slab apart, 8-row groups 1024 bytes apart; 16 rows further = 2048 bytes
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kSlabBytes >> 4) << 16) | (64ull << 32) | (1ull << 46) |
-         (2ull << 61);
-}
+// Shared-memory descriptors in the 128-byte swizzle (layout type 2): the high word is the same for all, 8-row groups 1024
+// bytes apart. Low word, K-major: 16 channels further = 32 bytes; MN-major: 64-channel groups one slab apart, 16 rows
+// further = 2048 bytes.
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | ((uint32_t)(kSlabBytes >> 4) << 16); }
 template <typename T>
 __host__ __device__ constexpr uint32_t idesc(int M, int N, bool b_mn) {
   return (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | ((b_mn ? 1u : 0u) << 16) |
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-// D (+)= A B with A in TMEM (128 lanes, 16-bit pairs in 32-bit columns)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 x, y;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc)
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "mov.b64 x, {%1, %6};\n\t"
+      "mov.b64 y, {%2, %6};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(acc), "r"(lead), "r"(kDescHigh)
+      : "memory");
+}
+// A in TMEM (128 lanes, 16-bit pairs in 32-bit columns)
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 y;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "mov.b64 y, {%2, %6};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(acc), "r"(lead), "r"(kDescHigh)
+      : "memory");
+}
+// `bar` completes when the lead lane's products so far have
+__device__ __forceinline__ void mma_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
       : "memory");
 }
 // D[128 x N] = X Y^T: X 128 rows, Y N rows, of NS slabs, contracted over their channels
 template <typename T, int NS, int N = 128>
-__device__ __forceinline__ void mma_xyt(uint32_t d, uint32_t x, uint32_t y, bool acc = false) {
+__device__ __forceinline__ void mma_xyt(uint32_t lead, uint32_t d, uint32_t x, uint32_t y, bool acc = false) {
+  const uint32_t a = desc_k(x), b = desc_k(y);
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      mma_bf16(d, desc_k(x + s * kSlabBytes) + 2 * k, desc_k(y + s * kSlabBytes) + 2 * k, idesc<T>(128, N, false),
-               acc || s > 0 || k > 0);
+      mma_ss(lead, d, a + s * (kSlabBytes >> 4) + 2 * k, b + s * (kSlabBytes >> 4) + 2 * k, idesc<T>(128, N, false),
+             acc || s > 0 || k > 0);
 }
 // D[128 x NS 64] (+)= P Y: P in TMEM (128 rows, 16 K contracted columns as 8 K words), Y's rows contracted. P stands in
 // pieces of 32 contracted columns (16 words), `gap` words apart.
 template <typename T, int NS, int K = 8>
-__device__ __forceinline__ void mma_py(uint32_t d, uint32_t p, uint32_t y, bool acc, int gap) {
+__device__ __forceinline__ void mma_py(uint32_t lead, uint32_t d, uint32_t p, uint32_t y, bool acc, int gap) {
+  const uint32_t b = desc_mn(y);
 #pragma unroll
   for (int k = 0; k < K; ++k)
-    mma_ts(d, p + (k & 1) * 8 + (k >> 1) * gap, desc_mn(y) + 128 * k, idesc<T>(128, NS * 64, true), acc || k > 0);
+    mma_ts(lead, d, p + (k & 1) * 8 + (k >> 1) * gap, b + 128 * k, idesc<T>(128, NS * 64, true), acc || k > 0);
 }
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -215,9 +247,9 @@ __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one is NaN
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 // bits [from, end) of 32 (any ints)
@@ -236,6 +268,12 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void ex2_pair(F2 x, float& a, float& b) {
+  unf2(x, a, b);
+  a = ex2(a);
+  b = ex2(b);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
   if constexpr (std::is_same<T, __half>::value) {

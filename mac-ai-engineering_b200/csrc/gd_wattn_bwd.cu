@@ -20,7 +20,7 @@ namespace wattn {
 namespace {
 
 constexpr int kWarpsEw = 16;                     // elementwise work: four threads a row, 32 columns each
-constexpr int kThreads = 32 * (kWarpsEw + 2);    // + loads, + products
+constexpr int kThreads = 32 * (kWarpsEw + 2);    // + loads, + products (dK, dV: one more, for L and delta)
 
 // the error word's first spare field holds the bits of the largest |dO| (float16)
 __device__ __forceinline__ float ds_scale(const ErrorWord* err) {
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* fin = s_full + 6;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   int* info = reinterpret_cast<int*>(tslot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
 
   if (threadIdx.x == 0) {
     mbar_init(in_full, 1);
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     sq = {(int)blockIdx.z, 0, pr.Tq, 0, pr.Tk};
   }
-  const uint32_t tm = *tslot;
+  const uint32_t tm = __shfl_sync(0xffffffffu, *tslot, 0);  // uniform
   const int i0 = tile * kTile;
   const int i1 = i0 + kTile - 1 < sq.Tq - 1 ? i0 + kTile - 1 : sq.Tq - 1;
   const int p0 = i0 + sq.offset(), p1 = i1 + sq.offset();
@@ -250,75 +250,76 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_wait(full + C::kKs + l % C::kVs, (l / C::kVs) & 1, err, 83);
     }
   } else if (warp == kWarpsEw + 1) {
-    if (lane == 0 && kr.n > 0) {
-      bool ok = mbar_wait(in_full, 0, err, 84);
+    if (kr.n > 0) {
+      const uint32_t lead = elect();
+      bool ok = warp_wait(in_full, 0, err, 84);
       if constexpr (!C::kHalves) {
         auto first = [&](int j) {  // S and dP of tile j
           const int a = j % C::kKs, b = C::kKs + j % C::kVs;
-          if (!mbar_wait(full + a, (j / C::kKs) & 1, err, 85)) return false;
-          if (j > 0 && !mbar_wait(s_read, (j - 1) & 1, err, 86)) return false;
+          if (!warp_wait(full + a, (j / C::kKs) & 1, err, 85)) return false;
+          if (j > 0 && !warp_wait(s_read, (j - 1) & 1, err, 86)) return false;
           tc_fence_after();
-          mma_xyt<T, NS>(tm, s_q, s_k + a * C::kUnit);
-          mma_commit(s_full);
-          if (!mbar_wait(full + b, (j / C::kVs) & 1, err, 87)) return false;
-          if (j > 0 && !mbar_wait(dp_read, (j - 1) & 1, err, 88)) return false;
+          mma_xyt<T, NS>(lead, tm, s_q, s_k + a * C::kUnit);
+          mma_commit(lead, s_full);
+          if (!warp_wait(full + b, (j / C::kVs) & 1, err, 87)) return false;
+          if (j > 0 && !warp_wait(dp_read, (j - 1) & 1, err, 88)) return false;
           tc_fence_after();
-          mma_xyt<T, NS>(tm + C::kDp, s_o, s_v + (j % C::kVs) * C::kUnit);
-          mma_commit(dp_full);
-          mma_commit(empty + b);
+          mma_xyt<T, NS>(lead, tm + C::kDp, s_o, s_v + (j % C::kVs) * C::kUnit);
+          mma_commit(lead, dp_full);
+          mma_commit(lead, empty + b);
           return true;
         };
         ok = ok && first(0);
         for (int j = 0; ok && j < kr.n; ++j) {
           if (j + 1 < kr.n) ok = first(j + 1);
-          if (!(ok = ok && mbar_wait(ds_full, j & 1, err, 89))) break;
+          if (!(ok = ok && warp_wait(ds_full, j & 1, err, 89))) break;
           tc_fence_after();
-          mma_py<T, NS>(tm + C::kDq, tm + C::kDs, s_k + (j % C::kKs) * C::kUnit, j > 0, 16);
-          mma_commit(empty + j % C::kKs);
-          mma_commit(dq_done);
+          mma_py<T, NS>(lead, tm + C::kDq, tm + C::kDs, s_k + (j % C::kKs) * C::kUnit, j > 0, 16);
+          mma_commit(lead, empty + j % C::kKs);
+          mma_commit(lead, dq_done);
         }
       } else {
         int n = 0;  // units used
         auto pair = [&](uint32_t d, uint32_t x) {  // D = X Y^T over the ring's next two halves
           for (int y = 0; y < 2; ++y, ++n) {
             const int a = n % C::kKs;
-            if (!mbar_wait(full + a, (n / C::kKs) & 1, err, 85)) return false;
+            if (!warp_wait(full + a, (n / C::kKs) & 1, err, 85)) return false;
             tc_fence_after();
-            mma_xyt<T, 2>(d, x + y * 2 * kSlabBytes, s_k + a * C::kUnit, y > 0);
-            mma_commit(empty + a);
+            mma_xyt<T, 2>(lead, d, x + y * 2 * kSlabBytes, s_k + a * C::kUnit, y > 0);
+            mma_commit(lead, empty + a);
           }
           return true;
         };
         ok = ok && pair(tm, s_q);
-        if (ok) mma_commit(s_full);
+        if (ok) mma_commit(lead, s_full);
         ok = ok && pair(tm + C::kDp, s_o);
-        if (ok) mma_commit(dp_full);
+        if (ok) mma_commit(lead, dp_full);
         for (int j = 0; ok && j < kr.n; ++j) {
           if (j + 1 < kr.n) {
-            ok = mbar_wait(s_read, j & 1, err, 86) && pair(tm, s_q);
-            if (ok) mma_commit(s_full);
+            ok = warp_wait(s_read, j & 1, err, 86) && pair(tm, s_q);
+            if (ok) mma_commit(lead, s_full);
           }
-          if (!(ok = ok && mbar_wait(ds_full, j & 1, err, 89))) break;
+          if (!(ok = ok && warp_wait(ds_full, j & 1, err, 89))) break;
           tc_fence_after();
           for (int y = 0; ok && y < 2; ++y, ++n) {
             const int a = n % C::kKs;
-            if (!(ok = mbar_wait(full + a, (n / C::kKs) & 1, err, 85))) break;
+            if (!(ok = warp_wait(full + a, (n / C::kKs) & 1, err, 85))) break;
             tc_fence_after();
-            mma_py<T, 2>(tm + C::kDq + y * 128, tm + C::kDs, s_k + a * C::kUnit, j > 0, 16);
-            mma_commit(empty + a);
+            mma_py<T, 2>(lead, tm + C::kDq + y * 128, tm + C::kDs, s_k + a * C::kUnit, j > 0, 16);
+            mma_commit(lead, empty + a);
           }
           if (!ok) break;
-          mma_commit(dq_done);
+          mma_commit(lead, dq_done);
           if (j + 1 < kr.n) {  // dP over dS, once its products have read it
-            ok = mbar_wait(dq_done, j & 1, err, 88);
+            ok = warp_wait(dq_done, j & 1, err, 88);
             tc_fence_after();
             ok = ok && pair(tm + C::kDp, s_o);
-            if (ok) mma_commit(dp_full);
+            if (ok) mma_commit(lead, dp_full);
           }
         }
       }
-      mma_commit(fin);
-      mbar_wait(fin, 0, err, 90);
+      mma_commit(lead, fin);
+      warp_wait(fin, 0, err, 90);
     }
   } else if (tile >= 0) {
     const int row = (warp & 3) * 32 + lane, part = warp >> 2;  // TMEM lane, which 32 columns
@@ -343,10 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive_warp(s_read);
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
-        float a, b;
-        unf2(fma2(f2(s[c], s[c + 1]), sc, mL), a, b);
-        s[c] = ex2(a);
-        s[c + 1] = ex2(b);
+        ex2_pair(fma2(f2(s[c], s[c + 1]), sc, mL), s[c], s[c + 1]);
       }
       if (!(ok = warp_wait(dp_full, j & 1, err, 92))) break;
       tc_fence_after();
@@ -417,7 +415,7 @@ struct DkvCfg {
   static constexpr int kQs = kHalves ? 3 : 2, kOs = kHalves ? 0 : 2;
   static constexpr int kDp = 128, kDv = 256, kDk = 256 + kAcc;
   static constexpr int kStats = kHalves ? 1 : 2;   // buffers of L and delta of a query tile
-  static constexpr int kBarriers = 1 + 2 * (kQs + kOs) + 8;
+  static constexpr int kBarriers = 1 + 2 * (kQs + kOs) + 7 + kStats;
   static constexpr size_t kSmem =
       1024 + 2 * NS * kSlabBytes + (size_t)kUnit * (kQs + kOs) + 8 * kBarriers + 64 + kStats * 2 * 4 * kTile;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -429,7 +427,7 @@ struct Split {
 };
 
 template <typename T, int NS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads + 32, 1)
     dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo, const Problem pr,
                const Split sp, const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
@@ -449,10 +447,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* dv_done = s_full + 4;
   uint64_t* dk_done = s_full + 5;
   uint64_t* st_full = s_full + 6;
-  uint64_t* fin = s_full + 7;
+  uint64_t* fin = s_full + 6 + C::kStats;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   int* info = reinterpret_cast<int*>(tslot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
 
   if (threadIdx.x == 0) {
     mbar_init(in_full, 1);
@@ -466,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(ds_full, kWarpsEw);
     mbar_init(dv_done, 1);
     mbar_init(dk_done, 1);
-    mbar_init(st_full, kWarpsEw);
+    for (int i = 0; i < C::kStats; ++i) mbar_init(st_full + i, 1);
     mbar_init(fin, 1);
     fence_mbar_init();
   }
@@ -506,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     sq = {(int)blockIdx.z, 0, pr.Tq, 0, pr.Tk};
   }
-  const uint32_t tm = *tslot;
+  const uint32_t tm = __shfl_sync(0xffffffffu, *tslot, 0);  // uniform
   const int c0 = tile * kTile, off = sq.offset();
   // the query tiles that see some of these keys
   int lo = 0, nq = 0;
@@ -525,7 +523,33 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t s_k = smem_u32(base), s_v = s_k + NS * kSlabBytes, s_q = s_v + NS * kSlabBytes,
                  s_o = s_q + C::kQs * C::kUnit;
 
-  if (warp == kWarpsEw) {
+  if (warp == kWarpsEw + 2) {
+    // -L and -delta of each iteration's queries, a step ahead of the elementwise warps; dead queries get -inf and 0
+    const long long at = (long long)sq.b * pr.H * pr.Tq + sq.q0;
+    int h = hk * G + (n > 0 ? it0 / nq : 0), qt = lo + (n > 0 ? it0 % nq : 0);
+    for (int i = 0; i < n; ++i) {
+      float L[4], de[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = qt * kTile + x * 32 + lane;
+        const bool live = t < sq.Tq;
+        L[x] = live ? -__ldg(lse + at + (long long)h * pr.Tq + t) : -INFINITY;
+        de[x] = live ? -__ldg(delta + at + (long long)h * pr.Tq + t) : 0.f;
+      }
+      if (++qt == lo + nq) {
+        qt = lo;
+        ++h;
+      }
+      float* st = stats + (i % C::kStats) * 256;  // free once its last iteration's dS is handed on
+      if (i >= C::kStats && !warp_wait(ds_full, (i - C::kStats) & 1, err, 115)) break;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        st[x * 32 + lane] = L[x];
+        st[128 + x * 32 + lane] = de[x];
+      }
+      mbar_arrive_warp(st_full + i % C::kStats);
+    }
+  } else if (warp == kWarpsEw) {
     if (lane == 0 && n > 0) {
       mbar_arrive_expect_tx(in_full, 2 * NS * kSlabBytes);
       load_tile<NS>(s_k, &mk, hk, sq.k0 + c0, sq.b, in_full);
@@ -574,87 +598,88 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_wait(full + C::kQs + l % C::kOs, (l / C::kOs) & 1, err, 103);
     }
   } else if (warp == kWarpsEw + 1) {
-    if (lane == 0 && n > 0) {
-      bool ok = mbar_wait(in_full, 0, err, 104);
+    if (n > 0) {
+      const uint32_t lead = elect();
+      bool ok = warp_wait(in_full, 0, err, 104);
       if constexpr (!C::kHalves) {
         auto scores = [&](int i) {
           const int a = i % C::kQs;
-          if (!mbar_wait(full + a, (i / C::kQs) & 1, err, 105)) return false;
-          if (i > 0 && !mbar_wait(dv_done, (i - 1) & 1, err, 106)) return false;  // P^T of the columns is read
+          if (!warp_wait(full + a, (i / C::kQs) & 1, err, 105)) return false;
+          if (i > 0 && !warp_wait(dv_done, (i - 1) & 1, err, 106)) return false;  // P^T of the columns is read
           tc_fence_after();
-          mma_xyt<T, NS>(tm, s_k, s_q + a * C::kUnit);
-          mma_commit(s_full);
+          mma_xyt<T, NS>(lead, tm, s_k, s_q + a * C::kUnit);
+          mma_commit(lead, s_full);
           return true;
         };
         auto dps = [&](int i) {
           const int b = i % C::kOs;
-          if (!mbar_wait(full + C::kQs + b, (i / C::kOs) & 1, err, 107)) return false;
-          if (i > 0 && !mbar_wait(dk_done, (i - 1) & 1, err, 108)) return false;  // dS^T of the columns is read
+          if (!warp_wait(full + C::kQs + b, (i / C::kOs) & 1, err, 107)) return false;
+          if (i > 0 && !warp_wait(dk_done, (i - 1) & 1, err, 108)) return false;  // dS^T of the columns is read
           tc_fence_after();
-          mma_xyt<T, NS>(tm + C::kDp, s_v, s_o + b * C::kUnit);
-          mma_commit(dp_full);
+          mma_xyt<T, NS>(lead, tm + C::kDp, s_v, s_o + b * C::kUnit);
+          mma_commit(lead, dp_full);
           return true;
         };
         ok = ok && scores(0) && dps(0);
         for (int i = 0; ok && i < n; ++i) {
-          if (!(ok = mbar_wait(p_full, i & 1, err, 109))) break;
+          if (!(ok = warp_wait(p_full, i & 1, err, 109))) break;
           tc_fence_after();
-          mma_py<T, NS>(tm + C::kDv, tm, s_o + (i % C::kOs) * C::kUnit, i > 0, 32);
-          mma_commit(dv_done);
-          mma_commit(empty + C::kQs + i % C::kOs);
+          mma_py<T, NS>(lead, tm + C::kDv, tm, s_o + (i % C::kOs) * C::kUnit, i > 0, 32);
+          mma_commit(lead, dv_done);
+          mma_commit(lead, empty + C::kQs + i % C::kOs);
           if (i + 1 < n) ok = scores(i + 1);
-          if (!(ok = ok && mbar_wait(ds_full, i & 1, err, 110))) break;
+          if (!(ok = ok && warp_wait(ds_full, i & 1, err, 110))) break;
           tc_fence_after();
-          mma_py<T, NS>(tm + C::kDk, tm + C::kDp, s_q + (i % C::kQs) * C::kUnit, i > 0, 32);
-          mma_commit(dk_done);
-          mma_commit(empty + i % C::kQs);
+          mma_py<T, NS>(lead, tm + C::kDk, tm + C::kDp, s_q + (i % C::kQs) * C::kUnit, i > 0, 32);
+          mma_commit(lead, dk_done);
+          mma_commit(lead, empty + i % C::kQs);
           if (i + 1 < n) ok = dps(i + 1);
         }
       } else {
         int u = 0;  // units used
-        auto next = [&]() { return mbar_wait(full + u % C::kQs, (u / C::kQs) & 1, err, 105); };
+        auto next = [&]() { return warp_wait(full + u % C::kQs, (u / C::kQs) & 1, err, 105); };
         auto pair = [&](uint32_t d, uint32_t x) {
           for (int y = 0; y < 2; ++y, ++u) {
             if (!next()) return false;
             tc_fence_after();
-            mma_xyt<T, 2>(d, x + y * 2 * kSlabBytes, s_q + u % C::kQs * C::kUnit, y > 0);
-            mma_commit(empty + u % C::kQs);
+            mma_xyt<T, 2>(lead, d, x + y * 2 * kSlabBytes, s_q + u % C::kQs * C::kUnit, y > 0);
+            mma_commit(lead, empty + u % C::kQs);
           }
           return true;
         };
         ok = ok && pair(tm, s_k);
-        if (ok) mma_commit(s_full);
+        if (ok) mma_commit(lead, s_full);
         ok = ok && pair(tm + C::kDp, s_v);
-        if (ok) mma_commit(dp_full);
+        if (ok) mma_commit(lead, dp_full);
         for (int i = 0; ok && i < n; ++i) {
-          if (!(ok = mbar_wait(p_full, i & 1, err, 109) && next())) break;
+          if (!(ok = warp_wait(p_full, i & 1, err, 109) && next())) break;
           tc_fence_after();
-          mma_py<T, 2>(tm + C::kDv, tm, s_q + u % C::kQs * C::kUnit, i > 0, 32);
-          mma_commit(empty + u % C::kQs);
-          mma_commit(dv_done);
+          mma_py<T, 2>(lead, tm + C::kDv, tm, s_q + u % C::kQs * C::kUnit, i > 0, 32);
+          mma_commit(lead, empty + u % C::kQs);
+          mma_commit(lead, dv_done);
           ++u;
           if (i + 1 < n) {
-            ok = mbar_wait(dv_done, i & 1, err, 106);
+            ok = warp_wait(dv_done, i & 1, err, 106);
             tc_fence_after();
             ok = ok && pair(tm, s_k);
-            if (ok) mma_commit(s_full);
+            if (ok) mma_commit(lead, s_full);
           }
-          if (!(ok = ok && mbar_wait(ds_full, i & 1, err, 110) && next())) break;
+          if (!(ok = ok && warp_wait(ds_full, i & 1, err, 110) && next())) break;
           tc_fence_after();
-          mma_py<T, 2>(tm + C::kDk, tm + C::kDp, s_q + u % C::kQs * C::kUnit, i > 0, 32);
-          mma_commit(empty + u % C::kQs);
-          mma_commit(dk_done);
+          mma_py<T, 2>(lead, tm + C::kDk, tm + C::kDp, s_q + u % C::kQs * C::kUnit, i > 0, 32);
+          mma_commit(lead, empty + u % C::kQs);
+          mma_commit(lead, dk_done);
           ++u;
           if (i + 1 < n) {
-            ok = mbar_wait(dk_done, i & 1, err, 108);
+            ok = warp_wait(dk_done, i & 1, err, 108);
             tc_fence_after();
             ok = ok && pair(tm + C::kDp, s_v);
-            if (ok) mma_commit(dp_full);
+            if (ok) mma_commit(lead, dp_full);
           }
         }
       }
-      mma_commit(fin);
-      mbar_wait(fin, 0, err, 111);
+      mma_commit(lead, fin);
+      warp_wait(fin, 0, err, 111);
     }
   } else if (tile >= 0) {
     const int row = (warp & 3) * 32 + lane, quarter = warp >> 2;  // TMEM lane, which 32 columns
@@ -664,30 +689,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     float f = 1.f;
     if constexpr (std::is_same<T, __half>::value) f = ds_scale(err);
     bool ok = true;
-    // -L and -delta of the queries of iteration i: thread t < 128 loads L of query t, threads 128 .. 255 delta
-    const float* stat_of = (threadIdx.x < 128 ? lse : delta) + (long long)sq.b * pr.H * pr.Tq + sq.q0;
-    auto stat = [&](int h, int qt) -> float {
-      const int t = qt * kTile + (threadIdx.x & 127);
-      return t < sq.Tq ? -__ldg(stat_of + (long long)h * pr.Tq + t) : threadIdx.x < 128 ? -INFINITY : 0.f;
-    };
-    int h = hk * G + (n > 0 ? it0 / nq : 0), qt = lo + (n > 0 ? it0 % nq : 0);  // of the iteration
-    float ahead = n > 0 && threadIdx.x < 256 ? stat(h, qt) : 0.f;
+    int qt = lo + (n > 0 ? it0 % nq : 0);  // the iteration's query tile
     for (int i = 0; i < n; ++i) {
-      // two buffers: all warps have passed iteration i - 1's barrier, so they are done with iteration i - 2's values; one
-      // buffer: they are done with iteration i - 1's when they have handed on its dS
-      float* st = stats + (i % C::kStats) * 256;
-      if (C::kStats == 1 && i > 0 && !(ok = warp_wait(ds_full, (i - 1) & 1, err, 115))) break;
-      if (threadIdx.x < 256) st[threadIdx.x] = ahead;
-      mbar_arrive_warp(st_full);
-      const int i0 = qt * kTile, q0 = i0 + off;  // the tile's first query and its position
-      if (++qt == lo + nq) {
-        qt = lo;
-        ++h;
-      }
-      if (i + 1 < n && threadIdx.x < 256) ahead = stat(h, qt);
-      if (!(ok = warp_wait(st_full, i & 1, err, 116))) break;
+      const float* st = stats + (i % C::kStats) * 256;  // -L and -delta of the tile's queries
       const ulonglong2* L4 = reinterpret_cast<const ulonglong2*>(st + quarter * 32);
       const ulonglong2* D4 = reinterpret_cast<const ulonglong2*>(st + 128 + quarter * 32);
+      const int i0 = qt * kTile, q0 = i0 + off;  // the tile's first query and its position
       const bool whole = i0 + kTile <= sq.Tq && all_visible(c0, q0, q0 + kTile - 1, pr.window, pr.sinks);
       uint32_t vis = 0xffffffffu;
       if (!whole) {
@@ -697,7 +704,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (to < end) end = (int)to;
         vis = bits(key - q0 - quarter * 32, end);
       }
-      if (!(ok = warp_wait(s_full, i & 1, err, 112))) break;
+      if (++qt == lo + nq) qt = lo;
+      if (!(ok = warp_wait(st_full + i % C::kStats, (i / C::kStats) & 1, err, 116) && warp_wait(s_full, i & 1, err, 112))) break;
       tc_fence_after();
       float s[32], d[32];
       tmem_ld32(tm + lanes + quarter * 32, s);
@@ -705,13 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const ulonglong2 L = L4[c / 4];
-        float a, b;
-        unf2(fma2(f2(s[c], s[c + 1]), sc, L.x), a, b);
-        s[c] = ex2(a);
-        s[c + 1] = ex2(b);
-        unf2(fma2(f2(s[c + 2], s[c + 3]), sc, L.y), a, b);
-        s[c + 2] = ex2(a);
-        s[c + 3] = ex2(b);
+        ex2_pair(fma2(f2(s[c], s[c + 1]), sc, L.x), s[c], s[c + 1]);
+        ex2_pair(fma2(f2(s[c + 2], s[c + 3]), sc, L.y), s[c + 2], s[c + 3]);
       }
       if (!whole) {
 #pragma unroll
@@ -827,7 +830,7 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
   const long long kt = (pr.cu ? (long long)pr.Tk / kTile + pr.N : (pr.Tk + kTile - 1) / kTile) + (long long)sp.heavy * (sp.parts - 1);
   kq<<<dim3((unsigned)qt, (unsigned)pr.H, (unsigned)pr.B), kThreads, DqCfg<NS>::kSmem, stream>>>(
       mq, mk, mv, mo, pr, lse, delta, static_cast<T*>(dq), err);
-  kkv<<<dim3((unsigned)kt, (unsigned)(pr.HK * (NS == 4 ? 2 : 1)), (unsigned)pr.B), kThreads, DkvCfg<NS>::kSmem, stream>>>(
+  kkv<<<dim3((unsigned)kt, (unsigned)(pr.HK * (NS == 4 ? 2 : 1)), (unsigned)pr.B), kThreads + 32, DkvCfg<NS>::kSmem, stream>>>(
       mq, mk, mv, mo, pr, sp, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), err);
   if (sp.parts > 1)
     sum_parts<T><<<dim3((unsigned)((kTile * pr.D / 4 + 255) / 256), (unsigned)(2 * sp.heavy), (unsigned)(pr.B * pr.HK)), 256,

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   uint64_t* fin = o_done + 2;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   int* info = reinterpret_cast<int*>(tslot + 1);  // the packed sequence and tile of this CTA
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   } else {
     sq = {(int)blockIdx.z, 0, pr.Tq, 0, pr.Tk};
   }
-  const uint32_t tm = *tslot;
+  const uint32_t tm = __shfl_sync(0xffffffffu, *tslot, 0);  // uniform
   const int i0 = tile * kTile;
   const int i1 = i0 + kTile - 1 < sq.Tq - 1 ? i0 + kTile - 1 : sq.Tq - 1;
   const int p0 = i0 + sq.offset(), p1 = i1 + sq.offset();
@@ -129,19 +129,20 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       for (int l = c > C::kSlots ? c - C::kSlots : 0; l < c; ++l) mbar_wait(full + l % C::kSlots, (l / C::kSlots) & 1, err, 61);
     }
   } else if (warp == kWarpsSm + 1) {
-    if (lane == 0 && kr.n > 0) {
-      bool ok = mbar_wait(q_full, 0, err, 62);
-      auto landed = [&](int c) { return mbar_wait(full + c % C::kSlots, (c / C::kSlots) & 1, err, 63); };
+    if (kr.n > 0) {
+      const uint32_t lead = elect();
+      bool ok = warp_wait(q_full, 0, err, 62);
+      auto landed = [&](int c) { return warp_wait(full + c % C::kSlots, (c / C::kSlots) & 1, err, 63); };
       if constexpr (!C::kWide) {
         // units: K(j) = 2 j, V(j) = 2 j + 1; half x of tile j is half-tile 2 j + x
         auto scores = [&](int j, int x) {
           const int c = 2 * j;
           if (x == 0 && !landed(c)) return false;
-          if (j > 0 && !mbar_wait(o_done, (2 * (j - 1) + x) & 1, err, 64)) return false;  // P over these columns is read
+          if (j > 0 && !warp_wait(o_done, (2 * (j - 1) + x) & 1, err, 64)) return false;  // P over these columns is read
           tc_fence_after();
-          mma_xyt<T, NS, 64>(tm + 64 * x, s_q, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128);
-          mma_commit(s_full + x);
-          if (x == 1) mma_commit(empty + c % C::kSlots);
+          mma_xyt<T, NS, 64>(lead, tm + 64 * x, s_q, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128);
+          mma_commit(lead, s_full + x);
+          if (x == 1) mma_commit(lead, empty + c % C::kSlots);
           return true;
         };
         ok = ok && scores(0, 0) && scores(0, 1);
@@ -150,28 +151,28 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if (x == 0) ok = landed(c);
-            if (!(ok = ok && mbar_wait(p_full + x, j & 1, err, 66))) break;
+            if (!(ok = ok && warp_wait(p_full + x, j & 1, err, 66))) break;
             tc_fence_after();
-            mma_py<T, NS, 4>(tm + C::kO, tm + 64 * x, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
-            if (x == 1) mma_commit(empty + c % C::kSlots);
-            mma_commit(o_done);
+            mma_py<T, NS, 4>(lead, tm + C::kO, tm + 64 * x, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
+            if (x == 1) mma_commit(lead, empty + c % C::kSlots);
+            mma_commit(lead, o_done);
             if (j + 1 < kr.n && !(ok = scores(j + 1, x))) break;
           }
         }
       } else {
         // units: K(j) = 4 j, 4 j + 1 and V(j) = 4 j + 2, 4 j + 3, by halves of the channels
         auto scores = [&](int j) {
-          if (j >= 2 && !mbar_wait(t_done, j & 1, err, 64)) return false;  // of tile j - 2: P over these columns is read
+          if (j >= 2 && !warp_wait(t_done, j & 1, err, 64)) return false;  // of tile j - 2: P over these columns is read
           const uint32_t d = tm + (j & 1) * 128;
           for (int y = 0; y < 2; ++y) {
             const int c = 4 * j + y;
             if (!landed(c)) return false;
             tc_fence_after();
-            mma_xyt<T, 2>(d, s_q + y * 2 * kSlabBytes, s_kv + c % C::kSlots * C::kUnit, y > 0);
-            mma_commit(empty + c % C::kSlots);
+            mma_xyt<T, 2>(lead, d, s_q + y * 2 * kSlabBytes, s_kv + c % C::kSlots * C::kUnit, y > 0);
+            mma_commit(lead, empty + c % C::kSlots);
           }
-          mma_commit(s_full + 2 * (j & 1));
-          mma_commit(s_full + 2 * (j & 1) + 1);
+          mma_commit(lead, s_full + 2 * (j & 1));
+          mma_commit(lead, s_full + 2 * (j & 1) + 1);
           return true;
         };
         ok = ok && scores(0);
@@ -180,20 +181,20 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
           const int c = 4 * j + 2, set = j & 1;
           ok = landed(c) && landed(c + 1);
           for (int x = 0; ok && x < 2; ++x) {
-            if (!(ok = mbar_wait(p_full + 2 * set + x, (j >> 1) & 1, err, 66))) break;
+            if (!(ok = warp_wait(p_full + 2 * set + x, (j >> 1) & 1, err, 66))) break;
             tc_fence_after();
             for (int y = 0; y < 2; ++y) {
               const int v = (c + y) % C::kSlots;
-              mma_py<T, 2, 4>(tm + C::kO + y * 128, tm + set * 128 + 64 * x, s_kv + v * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
-              if (x == 1) mma_commit(empty + v);
+              mma_py<T, 2, 4>(lead, tm + C::kO + y * 128, tm + set * 128 + 64 * x, s_kv + v * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
+              if (x == 1) mma_commit(lead, empty + v);
             }
-            mma_commit(o_done);
+            mma_commit(lead, o_done);
           }
-          if (ok) mma_commit(t_done);
+          if (ok) mma_commit(lead, t_done);
         }
       }
-      mma_commit(fin);
-      mbar_wait(fin, 0, err, 67);
+      mma_commit(lead, fin);
+      warp_wait(fin, 0, err, 67);
     }
   } else if (tile >= 0) {
     const int row = threadIdx.x;  // TMEM lane
@@ -222,16 +223,14 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
           s[32 + i] = (v1 >> i) & 1 ? s[32 + i] : -INFINITY;
         }
       }
-      float mx[4] = {s[0], s[1], s[2], s[3]};
+      float mx[4] = {s[0], s[1], s[2], s[3]};  // (a NaN score makes the maximum NaN, and with it the row)
 #pragma unroll
       for (int i = 4; i < 60; i += 8) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + 2 * e], s[i + 2 * e + 1]);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[60 + e]);
-      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * pr.scale_log2;
-      const bool grow = top > m + kMaxGrowth;  // also a row's first visible key
+      const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], s[60], s[61]), max3(s[62], s[63], s[62])) * pr.scale_log2;
+      const bool grow = !(top <= m + kMaxGrowth);  // also a row's first visible key, and NaN
       if (__any_sync(0xffffffffu, grow)) {
         const float next = grow ? top : m;
         const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2(m - next);
@@ -260,9 +259,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           float a, e;
-          unf2(fma2(f2(s[c + i], s[c + i + 1]), sc, rf), a, e);
-          a = ex2(a);
-          e = ex2(e);
+          ex2_pair(fma2(f2(s[c + i], s[c + i + 1]), sc, rf), a, e);
           acc = add2(acc, f2(a, e));
           u[i / 2] = pack16<T>(a, e);
         }
