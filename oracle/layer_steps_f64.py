@@ -67,25 +67,19 @@ def attention(q, k, v, window=None, sinks=0, scale=None, do=None):
     Tk, HK = k.shape[1:3]
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     seen = visible(Tq, Tk, window, sinks, q.device)
-    o, dq = torch.zeros(B, Tq, H, D, dtype=torch.float64, device=q.device), torch.zeros(B, Tq, H, D, dtype=torch.float64, device=q.device)
-    dk, dv = torch.zeros(B, Tk, HK, D, dtype=torch.float64, device=q.device), torch.zeros(B, Tk, HK, D, dtype=torch.float64, device=q.device)
-    for b in range(B):
-        for h in range(H):
-            c = h * HK // H
-            Q, K, V = q[b, :, h].double(), k[b, :, c].double(), v[b, :, c].double()
-            s = (Q @ K.T * scale).masked_fill(~seen, -math.inf)
-            m = s.amax(-1, keepdim=True) if Tk else s.new_zeros(Tq, 1)
-            e = torch.exp(s - torch.where(m.isinf(), torch.zeros_like(m), m))
-            z = e.sum(-1, keepdim=True)
-            P = e / torch.where(z > 0, z, torch.ones_like(z))
-            o[b, :, h] = P @ V
-            if do is not None:
-                G = do[b, :, h].double()
-                dP = G @ V.T
-                dS = P * (dP - (P * dP).sum(-1, keepdim=True)) * scale
-                dq[b, :, h] = dS @ K
-                dk[b, :, c] += dS.T @ Q
-                dv[b, :, c] += P.T @ G
+    Q = q.double().transpose(1, 2)                                                     # [B, H, Tq, D]
+    K, V = (t.double().transpose(1, 2).repeat_interleave(H // HK, 1) for t in (k, v))
+    e = torch.exp((Q @ K.transpose(-1, -2) * scale).masked_fill(~seen, -math.inf).sub_(
+        (Q @ K.transpose(-1, -2) * scale).masked_fill(~seen, -1e300).amax(-1, keepdim=True) if Tk else 0.0))
+    z = e.sum(-1, keepdim=True)
+    P = e / torch.where(z > 0, z, torch.ones_like(z))
+    o = (P @ V).transpose(1, 2)
+    if do is not None:
+        G = do.double().transpose(1, 2)
+        dP = G @ V.transpose(-1, -2)
+        dS = P * (dP - (P * dP).sum(-1, keepdim=True)) * scale
+        dq = (dS @ K).transpose(1, 2)
+        dk, dv = ((t.transpose(-1, -2) @ x).unflatten(1, (HK, H // HK)).sum(2).transpose(1, 2) for t, x in ((dS, Q), (P, G)))
     return o if do is None else (o, dq, dk, dv)
 
 
@@ -108,10 +102,9 @@ def attention_step(q, k, v, k_cache, v_cache, lengths, window=None, sinks=0, sca
         w = p + 1 if window is None else window
         if p >= S:
             w = min(w, ring)
-        see = [j for j in range(max(0, p - w + 1))][:min(first, max(0, p - w + 1))] + list(range(max(0, p - w + 1), p + 1))
-        at = torch.tensor([slot(j) for j in see], device=q.device)
-        for h in range(H):
-            c = h * HK // H
-            P = torch.softmax(kc[b, at, c] @ q[b, 0, h].double() * scale, 0)
-            o[b, 0, h] = P @ vc[b, at, c]
+        since = max(0, p - w + 1)
+        at = torch.tensor([slot(j) for j in list(range(min(first, since))) + list(range(since, p + 1))], device=q.device)
+        K, V = kc[b, at].repeat_interleave(H // HK, 1), vc[b, at].repeat_interleave(H // HK, 1)   # [n, H, D]
+        P = torch.softmax((K * q[b, 0].double()).sum(-1) * scale, 0)
+        o[b, 0] = (P[..., None] * V).sum(0)
     return o, kc, vc
