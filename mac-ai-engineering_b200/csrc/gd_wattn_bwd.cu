@@ -402,9 +402,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------------------------------------------------------
 // dK, dV. S^T = K Q^T and dP^T = V dO^T with the keys on the rows. TMEM: S^T | dP^T | dV | dK, P^T over S^T and dS^T over
-// dP^T (each thread's 32 columns over its own). Order of the products, so that each runs under elementwise work:
-// dV(i), S(i + 1) under dS(i); dK(i), dP(i + 1) under P(i + 1). NS = 4: a CTA accumulates one half of the channels
-// (S^T and dP^T over all of them), Q and dO pass through a ring of half tiles in the order of their use.
+// dP^T (each thread's 32 columns over its own). The elementwise warps are two groups of eight, one for each 64 of a tile's
+// queries, with signals of their own; the products alternate between the groups, so that each waits for what the other
+// group's product covers: dV(i) on P^T(i), S^T(i + 1) once dV(i) has read P^T, dK(i) on dS^T(i), dP^T(i + 1) once dK(i) has
+// read dS^T. (One signal for all sixteen warps left the tensor pipe idle for every one of those four latencies: 316 us
+// against 296 us at 1 x 8192 x 16, 4 key heads, D 128, window 2048.) The sums are formed in this order in every run. NS = 4: a
+// CTA accumulates one half of the channels (S^T and dP^T over all of them), Q and dO pass through a ring of half tiles in the
+// order of their use, and the groups stay in step.
 // parts > 1 (the first `heavy` key tiles): the tile's list of (query head, query tile) is cut into `parts` pieces, a CTA
 // each, whose sums go to fp32 partial tiles that sum_parts adds in order.
 template <int NS>
@@ -415,7 +419,7 @@ struct DkvCfg {
   static constexpr int kQs = kHalves ? 3 : 2, kOs = kHalves ? 0 : 2;
   static constexpr int kDp = 128, kDv = 256, kDk = 256 + kAcc;
   static constexpr int kStats = kHalves ? 1 : 2;   // buffers of L and delta of a query tile
-  static constexpr int kBarriers = 1 + 2 * (kQs + kOs) + 7 + kStats;
+  static constexpr int kBarriers = 1 + 2 * (kQs + kOs) + 13 + kStats;
   static constexpr size_t kSmem =
       1024 + 2 * NS * kSlabBytes + (size_t)kUnit * (kQs + kOs) + 8 * kBarriers + 64 + kStats * 2 * 4 * kTile;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -441,13 +445,13 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
   uint64_t* full = bars + 1;  // Q ring, then dO ring
   uint64_t* empty = full + C::kQs + C::kOs;
   uint64_t* s_full = empty + C::kQs + C::kOs;
-  uint64_t* dp_full = s_full + 1;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* ds_full = s_full + 3;
-  uint64_t* dv_done = s_full + 4;
-  uint64_t* dk_done = s_full + 5;
-  uint64_t* st_full = s_full + 6;
-  uint64_t* fin = s_full + 6 + C::kStats;
+  uint64_t* dp_full = s_full + 2;             // of each group, as the next four
+  uint64_t* p_full = s_full + 4;
+  uint64_t* ds_full = s_full + 6;
+  uint64_t* dv_done = s_full + 8;
+  uint64_t* dk_done = s_full + 10;
+  uint64_t* st_full = s_full + 12;
+  uint64_t* fin = s_full + 12 + C::kStats;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   int* info = reinterpret_cast<int*>(tslot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
@@ -456,14 +460,16 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
     mbar_init(in_full, 1);
     for (int i = 0; i < C::kQs + C::kOs; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, 1);
+      mbar_init(empty + i, C::kHalves ? 1 : 2);  // both groups' products have read the tile
     }
-    mbar_init(s_full, 1);
-    mbar_init(dp_full, 1);
-    mbar_init(p_full, kWarpsEw);
-    mbar_init(ds_full, kWarpsEw);
-    mbar_init(dv_done, 1);
-    mbar_init(dk_done, 1);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(s_full + g, 1);
+      mbar_init(dp_full + g, 1);
+      mbar_init(p_full + g, kWarpsEw / 2);
+      mbar_init(ds_full + g, kWarpsEw / 2);
+      mbar_init(dv_done + g, 1);
+      mbar_init(dk_done + g, 1);
+    }
     for (int i = 0; i < C::kStats; ++i) mbar_init(st_full + i, 1);
     mbar_init(fin, 1);
     fence_mbar_init();
@@ -541,7 +547,9 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
         ++h;
       }
       float* st = stats + (i % C::kStats) * 256;  // free once its last iteration's dS is handed on
-      if (i >= C::kStats && !warp_wait(ds_full, (i - C::kStats) & 1, err, 115)) break;
+      if (i >= C::kStats && !(warp_wait(ds_full, (i - C::kStats) & 1, err, 115) &&
+                              warp_wait(ds_full + 1, (i - C::kStats) & 1, err, 115)))
+        break;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         st[x * 32 + lane] = L[x];
@@ -602,38 +610,57 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       const uint32_t lead = elect();
       bool ok = warp_wait(in_full, 0, err, 104);
       if constexpr (!C::kHalves) {
-        auto scores = [&](int i) {
-          const int a = i % C::kQs;
-          if (!warp_wait(full + a, (i / C::kQs) & 1, err, 105)) return false;
-          if (i > 0 && !warp_wait(dv_done, (i - 1) & 1, err, 106)) return false;  // P^T of the columns is read
+        constexpr int kRows64 = 64 * 128;  // bytes of 64 rows of a slab
+        auto scores = [&](int i, int g) {
           tc_fence_after();
-          mma_xyt<T, NS>(lead, tm, s_k, s_q + a * C::kUnit);
-          mma_commit(lead, s_full);
-          return true;
+          mma_xyt<T, NS, 64>(lead, tm + 64 * g, s_k, s_q + i % C::kQs * C::kUnit + g * kRows64);
+          mma_commit(lead, s_full + g);
         };
-        auto dps = [&](int i) {
-          const int b = i % C::kOs;
-          if (!warp_wait(full + C::kQs + b, (i / C::kOs) & 1, err, 107)) return false;
-          if (i > 0 && !warp_wait(dk_done, (i - 1) & 1, err, 108)) return false;  // dS^T of the columns is read
+        auto dps = [&](int i, int g) {
           tc_fence_after();
-          mma_xyt<T, NS>(lead, tm + C::kDp, s_v, s_o + b * C::kUnit);
-          mma_commit(lead, dp_full);
-          return true;
+          mma_xyt<T, NS, 64>(lead, tm + C::kDp + 64 * g, s_v, s_o + i % C::kOs * C::kUnit + g * kRows64);
+          mma_commit(lead, dp_full + g);
         };
-        ok = ok && scores(0) && dps(0);
+        if ((ok = ok && warp_wait(full, 0, err, 105) && warp_wait(full + C::kQs, 0, err, 107))) {
+          scores(0, 0);
+          scores(0, 1);
+          dps(0, 0);
+          dps(0, 1);
+        }
         for (int i = 0; ok && i < n; ++i) {
-          if (!(ok = warp_wait(p_full, i & 1, err, 109))) break;
-          tc_fence_after();
-          mma_py<T, NS>(lead, tm + C::kDv, tm, s_o + (i % C::kOs) * C::kUnit, i > 0, 32);
-          mma_commit(lead, dv_done);
-          mma_commit(lead, empty + C::kQs + i % C::kOs);
-          if (i + 1 < n) ok = scores(i + 1);
-          if (!(ok = ok && warp_wait(ds_full, i & 1, err, 110))) break;
-          tc_fence_after();
-          mma_py<T, NS>(lead, tm + C::kDk, tm + C::kDp, s_q + (i % C::kQs) * C::kUnit, i > 0, 32);
-          mma_commit(lead, dk_done);
-          mma_commit(lead, empty + i % C::kQs);
-          if (i + 1 < n) ok = dps(i + 1);
+          const uint32_t qa = s_q + i % C::kQs * C::kUnit, oa = s_o + i % C::kOs * C::kUnit;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!(ok = ok && warp_wait(p_full + g, i & 1, err, 109))) break;
+            tc_fence_after();
+            mma_py<T, NS, 4>(lead, tm + C::kDv, tm + 64 * g, oa + g * kRows64, i > 0 || g > 0, 32);
+            mma_commit(lead, dv_done + g);
+            mma_commit(lead, empty + C::kQs + i % C::kOs);
+          }
+          if (i + 1 < n) {  // S over P, once that is read
+            ok = ok && warp_wait(full + (i + 1) % C::kQs, ((i + 1) / C::kQs) & 1, err, 105);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (!(ok = ok && warp_wait(dv_done + g, i & 1, err, 106))) break;
+              scores(i + 1, g);
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!(ok = ok && warp_wait(ds_full + g, i & 1, err, 110))) break;
+            tc_fence_after();
+            mma_py<T, NS, 4>(lead, tm + C::kDk, tm + C::kDp + 64 * g, qa + g * kRows64, i > 0 || g > 0, 32);
+            mma_commit(lead, dk_done + g);
+            mma_commit(lead, empty + i % C::kQs);
+          }
+          if (i + 1 < n) {  // dP over dS, once that is read
+            ok = ok && warp_wait(full + C::kQs + (i + 1) % C::kOs, ((i + 1) / C::kOs) & 1, err, 107);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (!(ok = ok && warp_wait(dk_done + g, i & 1, err, 108))) break;
+              dps(i + 1, g);
+            }
+          }
         }
       } else {
         int u = 0;  // units used
@@ -648,11 +675,18 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
           return true;
         };
         ok = ok && pair(tm, s_k);
-        if (ok) mma_commit(lead, s_full);
+        auto both = [&](uint64_t* bar) {
+          mma_commit(lead, bar);
+          mma_commit(lead, bar + 1);
+        };
+        auto wait2 = [&](uint64_t* bar, int i, int where) {
+          return warp_wait(bar, i & 1, err, where) && warp_wait(bar + 1, i & 1, err, where);
+        };
+        if (ok) both(s_full);
         ok = ok && pair(tm + C::kDp, s_v);
-        if (ok) mma_commit(lead, dp_full);
+        if (ok) both(dp_full);
         for (int i = 0; ok && i < n; ++i) {
-          if (!(ok = warp_wait(p_full, i & 1, err, 109) && next())) break;
+          if (!(ok = wait2(p_full, i, 109) && next())) break;
           tc_fence_after();
           mma_py<T, 2>(lead, tm + C::kDv, tm, s_q + u % C::kQs * C::kUnit, i > 0, 32);
           mma_commit(lead, empty + u % C::kQs);
@@ -662,9 +696,9 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
             ok = warp_wait(dv_done, i & 1, err, 106);
             tc_fence_after();
             ok = ok && pair(tm, s_k);
-            if (ok) mma_commit(lead, s_full);
+            if (ok) both(s_full);
           }
-          if (!(ok = ok && warp_wait(ds_full, i & 1, err, 110) && next())) break;
+          if (!(ok = ok && wait2(ds_full, i, 110) && next())) break;
           tc_fence_after();
           mma_py<T, 2>(lead, tm + C::kDk, tm + C::kDp, s_q + u % C::kQs * C::kUnit, i > 0, 32);
           mma_commit(lead, empty + u % C::kQs);
@@ -674,7 +708,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
             ok = warp_wait(dk_done, i & 1, err, 108);
             tc_fence_after();
             ok = ok && pair(tm + C::kDp, s_v);
-            if (ok) mma_commit(lead, dp_full);
+            if (ok) both(dp_full);
           }
         }
       }
@@ -682,7 +716,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       warp_wait(fin, 0, err, 111);
     }
   } else if (tile >= 0) {
-    const int row = (warp & 3) * 32 + lane, quarter = warp >> 2;  // TMEM lane, which 32 columns
+    const int row = (warp & 3) * 32 + lane, quarter = warp >> 2, gr = quarter >> 1;  // TMEM lane, which 32 columns, group
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int key = c0 + row;
     const F2 sc = f2(pr.scale_log2, pr.scale_log2);
@@ -705,7 +739,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
         vis = bits(key - q0 - quarter * 32, end);
       }
       if (++qt == lo + nq) qt = lo;
-      if (!(ok = warp_wait(st_full + i % C::kStats, (i / C::kStats) & 1, err, 116) && warp_wait(s_full, i & 1, err, 112))) break;
+      if (!(ok = warp_wait(st_full + i % C::kStats, (i / C::kStats) & 1, err, 116) &&
+            warp_wait(s_full + gr, i & 1, err, 112))) break;
       tc_fence_after();
       float s[32], d[32];
       tmem_ld32(tm + lanes + quarter * 32, s);
@@ -725,8 +760,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       tmem_st16(tm + lanes + quarter * 32, u);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive_warp(p_full);
-      if (!(ok = warp_wait(dp_full, i & 1, err, 113))) break;
+      mbar_arrive_warp(p_full + gr);
+      if (!(ok = warp_wait(dp_full + gr, i & 1, err, 113))) break;
       tc_fence_after();
       tmem_ld32(tm + lanes + C::kDp + quarter * 32, d);
       if (!whole) {  // nothing of a masked pair reaches dS, infinities and NaN included
@@ -742,10 +777,10 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       tmem_st16(tm + lanes + C::kDp + quarter * 32, u);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive_warp(ds_full);
+      mbar_arrive_warp(ds_full + gr);
     }
     if (ok && n > 0) {
-      ok = warp_wait(dv_done, (n - 1) & 1, err, 114) && warp_wait(dk_done, (n - 1) & 1, err, 114);
+      ok = warp_wait(fin, 0, err, 114);  // all products
       tc_fence_after();
     }
     // quarters 0 and 1 write dK's channels, 2 and 3 dV's; key row each
