@@ -124,6 +124,11 @@ inline bool tile_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, i
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// a contiguous output [B, T, heads, D], stored 32 rows at a time
+inline bool out_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int B, int T, int heads, int D) {
+  return tile_map(m, base, dt, B, T, heads, D, (long long)T * heads * D, (long long)heads * D, D, 32);
+}
+
 // all NS slabs of the tile at token t of head h, row b
 template <int NS>
 __device__ __forceinline__ void load_tile(uint32_t smem, const CUtensorMap* m, int h, int t, int b, uint64_t* bar) {
@@ -343,29 +348,40 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
 __device__ __forceinline__ void st_shared16(uint32_t a, const uint32_t (&u)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
 }
-// A warp's rows row0 .. row0 + N - 1 of a swizzled tile -> tokens t0 + row of a [T, heads, D] array (`out`: its head's first
-// channel), rows below `live` only; 16-byte pieces, a row's adjacent
-template <typename T, int N = 32>
-__device__ __forceinline__ void store_rows(T* out, uint32_t smem, int row0, int t0, int live, int heads, int D) {
-  const int chunks = D >> 3, lane = threadIdx.x & 31;
-  int r = lane / chunks, c = lane % chunks;
-  const int dr = 32 / chunks, dc = 32 % chunks;
-#pragma unroll 4
-  for (; r < N;) {
-    if (row0 + r < live) {
-      uint4 u;
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                   : "r"(smem + tile_at(row0 + r, c))
-                   : "memory");
-      *reinterpret_cast<uint4*>(out + ((long long)(t0 + row0 + r) * heads) * D + c * 8) = u;
+// Rows row0 .. row0 + 31 of a swizzled tile in shared memory -> tokens t0 + row of head h, row b of a [B, T, heads, D] array,
+// rows below `live` only, NS slabs from channel ch on; one whole warp, whose own rows these are (or after a barrier). By TMA (one lane issues it and
+// waits until shared memory is read; the array's end cuts it off) unless rows past `live` belong to someone else.
+template <typename T, int NS>
+__device__ __forceinline__ void store_rows(const CUtensorMap* m, T* out, uint32_t smem, int row0, int b, int t0, int live, int T_,
+                                           int h, int heads, int D, int ch = 0) {
+  if (row0 >= live) return;
+  if (live - row0 >= 32 || t0 + live == T_) {
+    fence_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        if (ch + s * 64 < D)
+          asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                           reinterpret_cast<uint64_t>(m)),
+                       "r"(ch + 64 * s), "r"(h), "r"(t0 + row0), "r"(b), "r"(smem + s * kSlabBytes + row0 * 128)
+                       : "memory");
+      bulk_commit();
+      bulk_wait_read0();
     }
-    r += dr;
-    c += dc;
-    if (c >= chunks) {
-      c -= chunks;
-      ++r;
-    }
+    return;
+  }
+  __syncwarp();
+  const int chunks = (D - ch < NS * 64 ? D - ch : NS * 64) >> 3, lane = threadIdx.x & 31, n = (live - row0) * chunks;
+  out += (((long long)b * T_ + t0 + row0) * heads + h) * D + ch;
+  for (int i = lane; i < n; i += 32) {
+    const int r = i / chunks, c = i - r * chunks;
+    uint4 u;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                 : "r"(smem + tile_at(row0 + r, c))
+                 : "memory");
+    *reinterpret_cast<uint4*>(out + (long long)r * heads * D + c * 8) = u;
   }
 }
 

@@ -92,17 +92,21 @@ __global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, con
   }
 }
 
-// 16 fp32 columns of the accumulator times f -> row `out` (16-bit), channels c .. c + 15 below D
+// 16 fp32 columns (from channel c) of an accumulator times f -> row `row` of a swizzled tile in shared memory, rounded
 template <typename T>
-__device__ __forceinline__ void store16(T* out, int c, int D, const float (&v)[16], float f) {
+__device__ __forceinline__ void stage16(uint32_t smem, int row, int c, const float (&v)[16], float f) {
 #pragma unroll
   for (int k = 0; k < 16; k += 8) {
-    if (c + k >= D) break;
     uint32_t u[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) u[e] = pack16<T>(v[k + 2 * e] * f, v[k + 2 * e + 1] * f);
-    *reinterpret_cast<uint4*>(out + c + k) = make_uint4(u[0], u[1], u[2], u[3]);
+    st_shared16(smem + tile_at(row, (c + k) >> 3), u);
   }
+}
+// between the staging of a tile and its store: the elementwise warps (each gets here in bounded time, failed waits or not)
+__device__ __forceinline__ void staged() {
+  fence_async_smem();
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarpsEw) : "memory");
 }
 
 // dS of two columns: p (dp - delta) f, packed
@@ -134,8 +138,8 @@ struct DqCfg {
 template <typename T, int NS>
 __global__ void __launch_bounds__(kThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-              const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo, const Problem pr,
-              const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dq, ErrorWord* err) {
+              const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo,
+              const __grid_constant__ CUtensorMap mdq, const Problem pr, const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dq, ErrorWord* err) {
   using C = DqCfg<NS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -378,9 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = warp_wait(dq_done, (kr.n - 1) & 1, err, 94);
       tc_fence_after();
     }
-    T* out = dq + (((long long)sq.b * pr.Tq + sq.q0 + i) * pr.H + h) * pr.D;
     const float g = ok ? pr.scale / f : NAN;
-#pragma unroll 1
+#pragma unroll
     for (int c = part * NS * 16; c < (part + 1) * NS * 16; c += 16) {
       float v[16];
       if (kr.n > 0) {
@@ -389,8 +392,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 16; ++k) v[k] = 0.f;
       }
-      if (live) store16(out, c, pr.D, v, g);
+      stage16<T>(s_q, row, c, v, g);  // Q's place
     }
+    staged();
+    if (warp < 4) store_rows<T, NS>(&mdq, dq, s_q, warp * 32, sq.b, sq.q0 + i0, sq.Tq - i0, pr.Tq, h, pr.H, pr.D);
   }
   tc_fence_before();
   __syncthreads();
@@ -419,7 +424,7 @@ struct DkvCfg {
   static constexpr int kQs = kHalves ? 3 : 2, kOs = kHalves ? 0 : 2;
   static constexpr int kDp = 128, kDv = 256, kDk = 256 + kAcc;
   static constexpr int kStats = kHalves ? 1 : 2;   // buffers of L and delta of a query tile
-  static constexpr int kBarriers = 1 + 2 * (kQs + kOs) + 13 + kStats;
+  static constexpr int kBarriers = 1 + 2 * (kQs + kOs) + 13 + 2 * kStats;
   static constexpr size_t kSmem =
       1024 + 2 * NS * kSlabBytes + (size_t)kUnit * (kQs + kOs) + 8 * kBarriers + 64 + kStats * 2 * 4 * kTile;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -433,8 +438,8 @@ struct Split {
 template <typename T, int NS>
 __global__ void __launch_bounds__(kThreads + 32, 1)
     dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-               const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo, const Problem pr,
-               const Split sp, const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
+               const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo,
+               const __grid_constant__ CUtensorMap mdk, const __grid_constant__ CUtensorMap mdv, const Problem pr, const Split sp, const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
                T* __restrict__ dv, ErrorWord* err) {
   using C = DkvCfg<NS>;
   extern __shared__ uint8_t smem_raw[];
@@ -451,7 +456,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
   uint64_t* dv_done = s_full + 8;
   uint64_t* dk_done = s_full + 10;
   uint64_t* st_full = s_full + 12;
-  uint64_t* fin = s_full + 12 + C::kStats;
+  uint64_t* st_empty = st_full + C::kStats;
+  uint64_t* fin = st_empty + C::kStats;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   int* info = reinterpret_cast<int*>(tslot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
@@ -470,7 +476,10 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       mbar_init(dv_done + g, 1);
       mbar_init(dk_done + g, 1);
     }
-    for (int i = 0; i < C::kStats; ++i) mbar_init(st_full + i, 1);
+    for (int i = 0; i < C::kStats; ++i) {
+      mbar_init(st_full + i, 1);
+      mbar_init(st_empty + i, kWarpsEw);
+    }
     mbar_init(fin, 1);
     fence_mbar_init();
   }
@@ -546,10 +555,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
         qt = lo;
         ++h;
       }
-      float* st = stats + (i % C::kStats) * 256;  // free once its last iteration's dS is handed on
-      if (i >= C::kStats && !(warp_wait(ds_full, (i - C::kStats) & 1, err, 115) &&
-                              warp_wait(ds_full + 1, (i - C::kStats) & 1, err, 115)))
-        break;
+      float* st = stats + (i % C::kStats) * 256;
+      if (i >= C::kStats && !warp_wait(st_empty + i % C::kStats, (i / C::kStats - 1) & 1, err, 115)) break;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         st[x * 32 + lane] = L[x];
@@ -778,12 +785,13 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive_warp(ds_full + gr);
+      mbar_arrive_warp(st_empty + i % C::kStats);
     }
     if (ok && n > 0) {
       ok = warp_wait(fin, 0, err, 114);  // all products
       tc_fence_after();
     }
-    // quarters 0 and 1 write dK's channels, 2 and 3 dV's; key row each
+    // quarters 0 and 1 take dK's channels, 2 and 3 dV's; key row each
     const bool is_k = quarter < 2;
     const float g = !ok ? NAN : is_k ? pr.scale / f : 1.f;
     const uint32_t acc = tm + lanes + (is_k ? C::kDk : C::kDv);
@@ -797,17 +805,22 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
 #pragma unroll
         for (int k = 0; k < 16; ++k) v[k] = 0.f;
       }
-      if (key >= sq.Tk) continue;
-      if (parts > 1) {
+      if (parts == 1) {
+        stage16<T>(is_k ? s_k : s_v, row, c, v, g);  // K's and V's places
+      } else if (key < sq.Tk) {
         float* out = sp.part + (((((long long)sq.b * pr.HK + hk) * sp.heavy + tile) * parts + part) * 2 + (is_k ? 0 : 1)) *
                                    kTile * pr.D + (long long)row * pr.D;
 #pragma unroll
         for (int k = 0; k < 16; k += 4)
           if (ch + c + k < pr.D)
             *reinterpret_cast<float4*>(out + ch + c + k) = make_float4(v[k] * g, v[k + 1] * g, v[k + 2] * g, v[k + 3] * g);
-      } else {
-        store16((is_k ? dk : dv) + (((long long)sq.b * pr.Tk + sq.k0 + key) * pr.HK + hk) * pr.D, ch + c, pr.D, v, g);
       }
+    }
+    staged();
+    if (parts == 1 && warp < 8) {
+      const bool kw = warp < 4;
+      store_rows<T, C::kAcc / 64>(kw ? &mdk : &mdv, kw ? dk : dv, kw ? s_k : s_v, (warp & 3) * 32, sq.b, sq.k0 + c0,
+                                  sq.Tk - c0, pr.Tk, hk, pr.HK, pr.D, ch);
     }
   }
   tc_fence_before();
@@ -845,12 +858,14 @@ template <typename T, int NS>
 int launch(const void* q, const void* k, const void* v, const void* o, const void* low, const void* g, const long long* st,
            const Problem& pr, const float* lse, float* delta, void* dq, void* dk, void* dv, Split sp, ErrorWord* err,
            cudaStream_t stream) {
-  CUtensorMap mq, mk, mv, mo;
+  CUtensorMap mq, mk, mv, mo, mdq, mdk, mdv;
   const CUtensorMapDataType dt = map_dtype<T>();
   if (!tile_map(&mq, q, dt, pr.B, pr.Tq, pr.H, pr.D, st[0], st[1], st[2], kTile) ||
       !tile_map(&mk, k, dt, pr.B, pr.Tk, pr.HK, pr.D, st[3], st[4], st[5], kTile) ||
       !tile_map(&mv, v, dt, pr.B, pr.Tk, pr.HK, pr.D, st[6], st[7], st[8], kTile) ||
-      !tile_map(&mo, g, dt, pr.B, pr.Tq, pr.H, pr.D, st[9], st[10], st[11], kTile))
+      !tile_map(&mo, g, dt, pr.B, pr.Tq, pr.H, pr.D, st[9], st[10], st[11], kTile) ||
+      !out_map(&mdq, dq, dt, pr.B, pr.Tq, pr.H, pr.D) || !out_map(&mdk, dk, dt, pr.B, pr.Tk, pr.HK, pr.D) ||
+      !out_map(&mdv, dv, dt, pr.B, pr.Tk, pr.HK, pr.D))
     return GD_ERR_LAUNCH;
   const long long rows = (long long)pr.Tq * pr.H;
   delta_kernel<T><<<dim3((unsigned)((rows + 16 * kRowsEach - 1) / (16 * kRowsEach)), (unsigned)pr.B), 256, 0, stream>>>(
@@ -864,9 +879,9 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
   const long long qt = pr.cu ? (long long)pr.Tq / kTile + pr.N : (pr.Tq + kTile - 1) / kTile;
   const long long kt = (pr.cu ? (long long)pr.Tk / kTile + pr.N : (pr.Tk + kTile - 1) / kTile) + (long long)sp.heavy * (sp.parts - 1);
   kq<<<dim3((unsigned)qt, (unsigned)pr.H, (unsigned)pr.B), kThreads, DqCfg<NS>::kSmem, stream>>>(
-      mq, mk, mv, mo, pr, lse, delta, static_cast<T*>(dq), err);
+      mq, mk, mv, mo, mdq, pr, lse, delta, static_cast<T*>(dq), err);
   kkv<<<dim3((unsigned)kt, (unsigned)(pr.HK * (NS == 4 ? 2 : 1)), (unsigned)pr.B), kThreads + 32, DkvCfg<NS>::kSmem, stream>>>(
-      mq, mk, mv, mo, pr, sp, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), err);
+      mq, mk, mv, mo, mdk, mdv, pr, sp, lse, delta, static_cast<T*>(dk), static_cast<T*>(dv), err);
   if (sp.parts > 1)
     sum_parts<T><<<dim3((unsigned)((kTile * pr.D / 4 + 255) / 256), (unsigned)(2 * sp.heavy), (unsigned)(pr.B * pr.HK)), 256,
                    0, stream>>>(sp.part, static_cast<T*>(dk), static_cast<T*>(dv), pr.Tk, pr.HK, pr.D, sp.heavy, sp.parts);

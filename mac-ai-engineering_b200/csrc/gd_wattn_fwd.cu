@@ -42,7 +42,8 @@ struct Cfg {
 template <typename T, int NS>
 __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-               const __grid_constant__ CUtensorMap mv, const Problem pr, T* __restrict__ o, T* __restrict__ o_low,
+               const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo,
+               const __grid_constant__ CUtensorMap ml, const Problem pr, T* __restrict__ o, T* __restrict__ o_low,
                float* __restrict__ lse, ErrorWord* err) {
   using C = Cfg<NS>;
   extern __shared__ uint8_t smem_raw[];
@@ -53,8 +54,9 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   uint64_t* empty = full + C::kSlots;
   uint64_t* s_full = empty + C::kSlots;       // of each half
   uint64_t* p_full = s_full + 2 * C::kSets;
-  uint64_t* o_done = p_full + 2 * C::kSets;   // a phase per half's P V
-  uint64_t* t_done = o_done + 1;              // kWide: a phase per tile's P V
+  // P V of half x: a phase a tile. Whoever waits on a phase is also needed for the next one of that barrier (a wait by
+  // parity tells neighbouring phases apart, no more), hence a barrier for each half and one of its own for the end.
+  uint64_t* o_done = p_full + 2 * C::kSets;
   uint64_t* fin = o_done + 2;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   int* info = reinterpret_cast<int*>(tslot + 1);  // the packed sequence and tile of this CTA
@@ -71,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       mbar_init(p_full + i, kWarpsSm);
     }
     mbar_init(o_done, 1);
-    mbar_init(t_done, 1);
+    mbar_init(o_done + 1, 1);
     mbar_init(fin, 1);
     fence_mbar_init();
   }
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
         auto scores = [&](int j, int x) {
           const int c = 2 * j;
           if (x == 0 && !landed(c)) return false;
-          if (j > 0 && !warp_wait(o_done, (2 * (j - 1) + x) & 1, err, 64)) return false;  // P over these columns is read
+          if (j > 0 && !warp_wait(o_done + x, (j - 1) & 1, err, 64)) return false;  // P over these columns is read
           tc_fence_after();
           mma_xyt<T, NS, 64>(lead, tm + 64 * x, s_q, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128);
           mma_commit(lead, s_full + x);
@@ -155,14 +157,14 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
             tc_fence_after();
             mma_py<T, NS, 4>(lead, tm + C::kO, tm + 64 * x, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
             if (x == 1) mma_commit(lead, empty + c % C::kSlots);
-            mma_commit(lead, o_done);
+            mma_commit(lead, o_done + x);
             if (j + 1 < kr.n && !(ok = scores(j + 1, x))) break;
           }
         }
       } else {
         // units: K(j) = 4 j, 4 j + 1 and V(j) = 4 j + 2, 4 j + 3, by halves of the channels
         auto scores = [&](int j) {
-          if (j >= 2 && !warp_wait(t_done, j & 1, err, 64)) return false;  // of tile j - 2: P over these columns is read
+          if (j >= 2 && !warp_wait(o_done + 1, j & 1, err, 64)) return false;  // of tile j - 2: P over these columns is read
           const uint32_t d = tm + (j & 1) * 128;
           for (int y = 0; y < 2; ++y) {
             const int c = 4 * j + y;
@@ -188,9 +190,8 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
               mma_py<T, 2, 4>(lead, tm + C::kO + y * 128, tm + set * 128 + 64 * x, s_kv + v * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
               if (x == 1) mma_commit(lead, empty + v);
             }
-            mma_commit(lead, o_done);
+            mma_commit(lead, o_done + x);
           }
-          if (ok) mma_commit(lead, t_done);
         }
       }
       mma_commit(lead, fin);
@@ -207,9 +208,9 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     for (int t = 0; ok && t < 2 * kr.n; ++t) {  // half-tiles
       const int j = t >> 1, x = t & 1, b = C::kWide ? t & 3 : x, phase = C::kWide ? j >> 1 : j;
       if (!(ok = warp_wait(s_full + b, phase & 1, err, 68))) break;
-      // a wait on o_done tells phases t - 1 and t - 3 apart only once t - 2 is over: D <= 128, half-tile t's S was issued
-      // after that; else it is waited for
-      if (C::kWide && t >= 2 && !(ok = warp_wait(o_done, t & 1, err, 71))) break;
+      // half-tile t - 2 is over (D <= 128: its S was issued after that), so that the wait below cannot take an older phase
+      // for its own
+      if (C::kWide && j > 0 && !(ok = warp_wait(o_done + x, (j - 1) & 1, err, 71))) break;
       tc_fence_after();
       const uint32_t ts = tm + lanes + b * 64;
       float s[64];
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
         const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2(m - next);
         l2 = mul2(l2, f2(f, f));
         if (t > 0) {  // O of the half-tiles so far, once their products are done
-          if (!(ok = warp_wait(o_done, (t - 1) & 1, err, 69))) break;
+          if (!(ok = warp_wait(o_done + (x ^ 1), (x == 0 ? j - 1 : j) & 1, err, 69))) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < NS * 64; c += 16) {
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       mbar_arrive_warp(p_full + b);
     }
     if (kr.n > 0) {
-      ok = ok && warp_wait(o_done, 0, err, 70) && warp_wait(o_done, 1, err, 70);  // half-tiles 2 n - 2, 2 n - 1
+      ok = ok && warp_wait(fin, 0, err, 70);  // all products
       tc_fence_after();
     }
     float l, lb;
@@ -281,38 +282,35 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     const bool none = l == 0.f && ok;                 // a row without a visible key: zeros, whatever O's columns hold
     const float inv = !ok ? NAN : none ? 0.f : 1.f / l;  // a wait that gave up leaves NaN
     if (i < sq.Tq) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m + log2f(l);
-    // out through shared memory (Q's place; a warp's own 32 rows), so that a row leaves as whole lines; then, for the
-    // backward's delta, what the rounding took away
-    for (int pass = 0; pass < (o_low != nullptr ? 2 : 1); ++pass) {
-#pragma unroll 1
-      for (int c = 0; c < NS * 64; c += 32) {
-        float v[32];
-        if (kr.n > 0) {
-          tmem_ld32(tm + lanes + C::kO + c, v);
-        } else {
+    // out through shared memory (Q's place and the first key unit's; a warp's own 32 rows), so that rows leave as whole lines
+    // (16-byte stores a thread and row took 5 us a CTA); o_low: what the rounding took away, for the backward's delta
+    const bool low = o_low != nullptr;
+#pragma unroll 2
+    for (int c = 0; c < NS * 64; c += 32) {
+      float v[32];
+      if (kr.n > 0) {
+        tmem_ld32(tm + lanes + C::kO + c, v);
+      } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          uint32_t u[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a = none ? 0.f : v[k + 2 * e] * inv, d = none ? 0.f : v[k + 2 * e + 1] * inv;
-            u[e] = pack16<T>(a, d);
-            if (pass == 1) {
-              const float2 r = unpack16<T>(u[e]);
-              u[e] = pack16<T>(a - r.x, d - r.y);
-            }
-          }
-          st_shared16(s_q + tile_at(row, (c + k) >> 3), u);
-        }
+        for (int k = 0; k < 32; ++k) v[k] = 0.f;
       }
-      __syncwarp();
-      T* out = pass == 0 ? o : o_low;
-      store_rows(out + ((long long)sq.b * pr.Tq * pr.H + h) * pr.D, s_q, warp * 32, sq.q0 + i0, sq.Tq - i0, pr.H, pr.D);
-      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 32; k += 8) {
+        uint32_t u[4], w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = none ? 0.f : v[k + 2 * e] * inv, d = none ? 0.f : v[k + 2 * e + 1] * inv;
+          u[e] = pack16<T>(a, d);
+          const float2 r = unpack16<T>(u[e]);
+          w[e] = pack16<T>(a - r.x, d - r.y);
+        }
+        const uint32_t at = tile_at(row, (c + k) >> 3);
+        st_shared16(s_q + at, u);
+        if (low) st_shared16(s_kv + at, w);
+      }
     }
+    store_rows<T, NS>(&mo, o, s_q, warp * 32, sq.b, sq.q0 + i0, sq.Tq - i0, pr.Tq, h, pr.H, pr.D);
+    if (low) store_rows<T, NS>(&ml, o_low, s_kv, warp * 32, sq.b, sq.q0 + i0, sq.Tq - i0, pr.Tq, h, pr.H, pr.D);
   }
   tc_fence_before();
   __syncthreads();
@@ -325,17 +323,19 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
 template <typename T, int NS>
 int launch(const void* q, const void* k, const void* v, const long long* st, const Problem& pr, void* o, void* low, float* lse,
            ErrorWord* err, cudaStream_t stream) {
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo, ml;
   if (!tile_map(&mq, q, map_dtype<T>(), pr.B, pr.Tq, pr.H, pr.D, st[0], st[1], st[2], kTile) ||
       !tile_map(&mk, k, map_dtype<T>(), pr.B, pr.Tk, pr.HK, pr.D, st[3], st[4], st[5], kTile) ||
-      !tile_map(&mv, v, map_dtype<T>(), pr.B, pr.Tk, pr.HK, pr.D, st[6], st[7], st[8], kTile))
+      !tile_map(&mv, v, map_dtype<T>(), pr.B, pr.Tk, pr.HK, pr.D, st[6], st[7], st[8], kTile) ||
+      !out_map(&mo, o, map_dtype<T>(), pr.B, pr.Tq, pr.H, pr.D) ||
+      !out_map(&ml, low != nullptr ? low : o, map_dtype<T>(), pr.B, pr.Tq, pr.H, pr.D))
     return GD_ERR_LAUNCH;
   static bool done[kMaxDevices];
   auto kern = fwd_kernel<T, NS>;
   if (set_smem_once(kern, Cfg<NS>::kSmem, done) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const long long tiles = pr.cu ? (long long)pr.Tq / kTile + pr.N : (pr.Tq + kTile - 1) / kTile;
   const dim3 grid((unsigned)tiles, (unsigned)pr.H, (unsigned)pr.B);
-  kern<<<grid, kThreads, Cfg<NS>::kSmem, stream>>>(mq, mk, mv, pr, static_cast<T*>(o), static_cast<T*>(low), lse, err);
+  kern<<<grid, kThreads, Cfg<NS>::kSmem, stream>>>(mq, mk, mv, mo, ml, pr, static_cast<T*>(o), static_cast<T*>(low), lse, err);
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
 }
 
