@@ -301,13 +301,16 @@ int gd_rotary(const void* q, const void* k, void* oq, void* ok, const float* tab
  * channels adjacent); o, dq [B, Tq, H, D] and dk, dv [B, Tk, HK, D] contiguous; every pointer 16-byte aligned. lse
  * [B, H, Tq] fp32: log2 of the sum of the exponentials, for the backward. cu_seqlens (device int32 [N + 1], or NULL):
  * packed rows, B = 1 and Tq = Tk, each sequence on its own; boundaries outside [0, Tq] or falling are clamped.
- * The workspace starts with an error word (gd_read_error). A wait that gives up leaves NaN in the rows it was for. */
+ * The workspace starts with an error word (gd_read_error); the forward's is nothing else and may be NULL. A wait that gives
+ * up leaves NaN in the rows it was for, word or no word. A finite result row needs finite values in its tile of 128 keys and
+ * 128 queries: masked scores are never used, but a masked key's infinity or NaN in v (or in k, q, d_o for the gradients)
+ * meets a weight of 0 in the products, as it would in a matrix product of the formula. */
 
 /* Bytes of workspace gd_wattn_fwd (for_backward 0) or gd_wattn_bwd need (0 for invalid sizes); packed: with cu_seqlens. */
 size_t gd_wattn_workspace_bytes(int B, int Tq, int Tk, int H, int HK, int D, int window, int sinks, int packed,
                                 int for_backward);
 
-/* o_low (for the backward; NULL otherwise): what o's rounding took away, in `dtype`, with o's shape. */
+/* o_low and lse are for the backward (NULL otherwise). o_low: what o's rounding took away, in `dtype`, with o's shape. */
 int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, const int* cu_seqlens,
                  int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D, const long long* strides, int window, int sinks, float scale,
                  void* workspace, size_t workspace_bytes, void* stream);

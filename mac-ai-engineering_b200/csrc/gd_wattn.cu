@@ -17,6 +17,13 @@ bool strides_ok(const long long* s, int B, int T, int heads) {
   return ok(s[0], B) && ok(s[1], T) && ok(s[2], heads);
 }
 
+// Tensor maps are encoded by the driver, which wants the device's context bound to the calling thread; a thread whose first
+// call this is (autograd's) has none until the runtime binds it.
+bool bind_context() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
+
 int check(const void* q, const void* k, const void* v, const long long* strides, const int* cu, int N, int dtype, int B,
           int Tq, int Tk, int H, int HK, int D, int window, int sinks, float scale) {
   if (dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) return GD_ERR_ARG;
@@ -101,17 +108,19 @@ extern "C" int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o
                             int window, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int st = check(q, k, v, strides, cu_seqlens, N, dtype, B, Tq, Tk, H, HK, D, window, sinks, scale)) return st;
   if (B == 0 || Tq == 0) return GD_OK;
-  if (o == nullptr || lse == nullptr) return GD_ERR_ARG;
+  if (o == nullptr || (lse == nullptr && o_low != nullptr)) return GD_ERR_ARG;
   if (!aligned16(o) || !aligned16(o_low) || !aligned16(workspace)) return GD_ERR_ALIGN;
-  if (workspace == nullptr || workspace_bytes < sizeof(ErrorWord)) return GD_ERR_WORKSPACE;
+  if (workspace != nullptr && workspace_bytes < sizeof(ErrorWord)) return GD_ERR_WORKSPACE;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if (cudaMemsetAsync(workspace, 0, sizeof(ErrorWord), cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
+  if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
+  if (workspace != nullptr && cudaMemsetAsync(workspace, 0, sizeof(ErrorWord), cs) != cudaSuccess)
+    return (cudaGetLastError(), GD_ERR_LAUNCH);
   const Problem p = problem(cu_seqlens, N, B, Tq, Tk, H, HK, D, window, sinks, scale);
   if (Tk == 0) {  // no keys at all: zeros
     const size_t n = (size_t)B * Tq * H * D * 2;
     if (cudaMemsetAsync(o, 0, n, cs) != cudaSuccess ||
         (o_low != nullptr && cudaMemsetAsync(o_low, 0, n, cs) != cudaSuccess) ||
-        cudaMemsetAsync(lse, 0x7f, (size_t)B * H * Tq * sizeof(float), cs) != cudaSuccess)  // 3.4e38: as good as +inf
+        (lse != nullptr && cudaMemsetAsync(lse, 0x7f, (size_t)B * H * Tq * sizeof(float), cs) != cudaSuccess))  // 3.4e38: as good as +inf
       return (cudaGetLastError(), GD_ERR_LAUNCH);
     return GD_OK;
   }
@@ -124,6 +133,7 @@ extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const v
                             void* workspace, size_t workspace_bytes, void* stream) {
   if (const int st = check(q, k, v, strides, cu_seqlens, N, dtype, B, Tq, Tk, H, HK, D, window, sinks, scale)) return st;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
   if (B == 0 || Tq == 0 || Tk == 0) {  // no pair: zero gradients
     const size_t nq = (size_t)B * Tq * H * D * 2, nk = (size_t)B * Tk * HK * D * 2;
     if ((nq > 0 && dq == nullptr) || (nk > 0 && (dk == nullptr || dv == nullptr))) return GD_ERR_ARG;
@@ -139,7 +149,9 @@ extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const v
   if (workspace == nullptr ||
       workspace_bytes < gd_wattn_workspace_bytes(B, Tq, Tk, H, HK, D, window, sinks, cu_seqlens != nullptr, 1))
     return GD_ERR_WORKSPACE;
-  if (cudaMemsetAsync(workspace, 0, sizeof(ErrorWord), cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
+  // the error word, with float16's largest |dO| in it; bfloat16's first kernel clears it
+  if (dtype == GD_FLOAT16 && cudaMemsetAsync(workspace, 0, sizeof(ErrorWord), cs) != cudaSuccess)
+    return (cudaGetLastError(), GD_ERR_LAUNCH);
   const Problem p = problem(cu_seqlens, N, B, Tq, Tk, H, HK, D, window, sinks, scale);
   const Cut c = cu_seqlens != nullptr ? Cut{0, 1} : cut_of(B, Tq, Tk, H, HK, D, p.window, p.sinks);
   char* ws = static_cast<char*>(workspace);

@@ -22,6 +22,11 @@ def launch(name: str, index: int, *args) -> None:
         _lib.check(st, name)
 
 
+def like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape, dtype and device."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def aligned(t: torch.Tensor) -> torch.Tensor:
     """Contiguous with a 16-byte aligned start (a copy only when the view is not)."""
     if not t.is_contiguous():

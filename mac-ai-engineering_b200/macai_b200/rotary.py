@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import launch, recorded
+from ._call import launch, like, recorded
 
 _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 
@@ -79,12 +79,12 @@ def _turn(q, k, table, positions, interleaved, inverse):
     q = _rows(q)
     B, T, H, D = q.shape
     qb, qt, qh, _ = q.stride()
-    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    oq = like(q)
     ok = kp = okp = None
     HK = kb = kt = kh = 0
     if k is not None:
         k = _rows(k)
-        ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        ok = like(k)
         kp, okp, HK = k.data_ptr(), ok.data_ptr(), k.shape[2]
         kb, kt, kh, _ = k.stride()
     pp, p64, pb = None, 0, 0

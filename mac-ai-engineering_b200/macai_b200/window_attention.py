@@ -12,19 +12,29 @@ only.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import aligned, launch, recorded
+from ._call import aligned, launch, like, recorded
 
 _DTYPES = {torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 MAX_D = 256
 
 
-_ERROR_WORD = 64  # gd_wattn_workspace_bytes(..., for_backward=0)
+
+
+@functools.lru_cache(maxsize=1024)
+def _bwd_bytes(*sizes) -> int:
+    return _lib.load().gd_wattn_workspace_bytes(*sizes, 1)
+
+
+@functools.lru_cache(maxsize=1024)
+def _step_bytes(*sizes) -> int:
+    return _lib.load().gd_wattn_step_workspace_bytes(*sizes)
 
 
 def _readable(t: torch.Tensor) -> bool:
@@ -44,24 +54,20 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _strides(*ts):
-    out = (ctypes.c_longlong * (3 * len(ts)))()
-    for i, t in enumerate(ts):
-        out[3 * i], out[3 * i + 1], out[3 * i + 2], _ = t.stride()
-    return out
+    return (ctypes.c_longlong * (3 * len(ts)))(*[s for t in ts for s in t.stride()[:3]])
 
 
 def _fwd(q, k, v, cu, window, sinks, scale, keep):
-    """(o, o_low, lse) on readable inputs; keep: o_low, what o's rounding took away, for the backward (else None)."""
+    """(o, o_low, lse) on readable inputs; keep: for the backward, o_low, what o's rounding took away, and lse (else None)."""
     B, Tq, H, D = q.shape
     Tk, HK = k.shape[1], k.shape[2]
-    dev = q.device
-    o = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
-    low = torch.empty_like(o) if keep else None
-    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
-    ws = torch.empty(_ERROR_WORD, dtype=torch.uint8, device=dev)
+    o = like(q)
+    low = lse = None
+    if keep:
+        low, lse = like(q), torch.empty((B, H, Tq), dtype=torch.float32, device=q.device)
     launch("gd_wattn_fwd", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-           None if low is None else low.data_ptr(), lse.data_ptr(), None if cu is None else cu.data_ptr(), 0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], B, Tq, Tk, H, HK,
-           D, _strides(q, k, v), window, sinks, scale, ws.data_ptr(), _ERROR_WORD)
+           None if low is None else low.data_ptr(), None if lse is None else lse.data_ptr(), None if cu is None else cu.data_ptr(), 0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], B, Tq, Tk, H, HK,
+           D, _strides(q, k, v), window, sinks, scale, None, 0)
     return o, low, lse
 
 
@@ -69,8 +75,8 @@ def _bwd(q, k, v, o, low, lse, do, cu, window, sinks, scale):
     """(dq, dk, dv), contiguous, on readable inputs."""
     B, Tq, H, D = q.shape
     Tk, HK = k.shape[1], k.shape[2]
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    n = _lib.load().gd_wattn_workspace_bytes(B, Tq, Tk, H, HK, D, window, sinks, cu is not None, 1)
+    dq, dk, dv = like(q), like(k), like(v)
+    n = _bwd_bytes(B, Tq, Tk, H, HK, D, window, sinks, cu is not None)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device)
     launch("gd_wattn_bwd", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), low.data_ptr(),
            lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None if cu is None else cu.data_ptr(),
@@ -191,8 +197,8 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     if recorded(q, k, v, k_cache, v_cache):
         raise RuntimeError("window_attention_step has no gradient: call it under torch.no_grad()")
     q, k, v = aligned(q), aligned(k), aligned(v)
-    o = torch.empty((B, 1, H, D), dtype=q.dtype, device=q.device)
-    n = _lib.load().gd_wattn_step_workspace_bytes(B, S, H, HK, D, w, s)
+    o = torch.empty_like(q)
+    n = _step_bytes(B, S, H, HK, D, w, s)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     launch("gd_wattn_step", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
            lengths.data_ptr(), o.data_ptr(), _DTYPES[q.dtype], B, S, H, HK, D, _strides(k_cache, v_cache), w, s,
