@@ -4,6 +4,7 @@ current)."""
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -32,6 +33,16 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
     if not t.is_contiguous():
         return t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def first_order(backward):
+    """once_differentiable for an autograd function's backward, without its cost (a grad-mode switch) where no graph of the
+    gradient is asked for."""
+    guarded = once_differentiable(backward)
+
+    def wrapper(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return wrapper
 
 
 def recorded(*ts) -> bool:

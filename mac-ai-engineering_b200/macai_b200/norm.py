@@ -15,10 +15,9 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import aligned, launch, recorded
+from ._call import aligned, first_order, launch, recorded
 
 _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 MAX_CHUNKS = 2048  # 16-byte chunks of a row (a width that fills no whole number of them takes two more)
@@ -82,7 +81,7 @@ class AddRMSNorm(torch.autograd.Function):
         return y if s is None else (y, s)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dy, ds=None):
         s, w = ctx.saved_tensors
         eps, zero_centered, has_residual = ctx.args

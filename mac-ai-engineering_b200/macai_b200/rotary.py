@@ -15,10 +15,9 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import launch, like, recorded
+from ._call import first_order, launch, like, recorded
 
 _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 
@@ -109,7 +108,7 @@ class Rotary(torch.autograd.Function):
         return oq if k is None else (oq, ok)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dq, dk=None):
         table, positions = ctx.saved_tensors
         if dq is None and dk is None:

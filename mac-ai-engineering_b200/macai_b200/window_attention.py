@@ -16,10 +16,9 @@ import functools
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import aligned, launch, like, recorded
+from ._call import aligned, first_order, launch, like, recorded
 
 _DTYPES = {torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 MAX_D = 256
@@ -96,7 +95,7 @@ class WindowAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, do):
         q, k, v, o, low, lse, cu = ctx.saved_tensors
         return (*_bwd(q, k, v, o, low, lse, _rows(do), cu, *ctx.args), None, None, None, None)
