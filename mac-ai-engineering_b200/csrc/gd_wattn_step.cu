@@ -159,8 +159,28 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const StepArgs a) {
   const uint32_t stages = sq + C::kQBytes + warp * C::kWarpBytes;
   auto load = [&](int s, int stage) {  // step s of the visible positions; rows past the last are zeros
     const uint32_t dst = stages + stage * 2 * C::kHalf;
-    if (s < s1) {
+    const int first = s * kStep, at0 = seen.slot(first);
+    if (s >= s1) {
+    } else if (first + kStep < seen.n && (first >= seen.head || first + kStep <= seen.head) &&
+               seen.slot(first + kStep - 1) == at0 + kStep - 1) {
+      // adjacent slots, none of them the new token's: a lane keeps its channels and walks the rows (the general way below
+      // takes twice the instructions of everything else in the step)
+      constexpr int kRowsAtOnce = 32 / kChunks > 0 ? 32 / kChunks : 1;
+      const int r0 = lane / kChunks, c = lane % kChunks;
+      const bool live = c * 8 < a.D;
+      const T* pk = kc + (long long)(at0 + r0) * a.ks + (live ? c * 8 : 0);
+      const T* pv = vc + (long long)(at0 + r0) * a.vs + (live ? c * 8 : 0);
 #pragma unroll
+      for (int r = 0; r < kStep; r += kRowsAtOnce) {
+        const int row = r + r0;
+        const uint32_t d = dst + row * DP * 2 + ((c ^ (row & 7)) << 4);
+        cp16(d, pk, live);
+        cp16(d + C::kHalf, pv, live);
+        pk += kRowsAtOnce * a.ks;
+        pv += kRowsAtOnce * a.vs;
+      }
+    } else {
+#pragma unroll 1
       for (int i = lane; i < kStep * kChunks; i += 32) {
         const int r = i / kChunks, c = i % kChunks, at = s * kStep + r;
         const bool live = at < seen.n && c * 8 < a.D;
@@ -186,6 +206,18 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const StepArgs a) {
   for (int i = 0; i < C::kStages - 1; ++i) load(s0 + warp + i * kWarps, i);
   asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");  // Q, of all threads
   __syncthreads();
+  // Q's fragments: in registers up to 128 channels
+  constexpr bool kQRegs = DP <= 128;
+  uint32_t qf[kQRegs ? DP / 16 : 1][4];
+  const int r8 = lane & 7, mat = lane >> 3;
+  auto q_at = [&](int k) {
+    const int qr = r8 + (mat & 1) * 8, qc = 2 * k + (mat >> 1);
+    return sq + qr * DP * 2 + ((qc ^ (qr & 7)) << 4);
+  };
+  if constexpr (kQRegs) {
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) ldsm4(qf[k], q_at(k));
+  }
   int stage = 0;
   for (int s = s0 + warp; s < s1; s += kWarps) {
     __syncwarp();  // every lane is done with the stage that is loaded next
@@ -196,12 +228,15 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const StepArgs a) {
     stage = stage + 1 == C::kStages ? 0 : stage + 1;
     // S [16 heads x 16 keys]
     float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    const int r8 = lane & 7, mat = lane >> 3;
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
       uint32_t qa[4], kb[4];
-      const int qr = r8 + (mat & 1) * 8, qc = 2 * k + (mat >> 1);
-      ldsm4(qa, sq + qr * DP * 2 + ((qc ^ (qr & 7)) << 4));
+      if constexpr (kQRegs) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qa[e] = qf[k][e];
+      } else {
+        ldsm4(qa, q_at(k));
+      }
       const int kr = r8 + (mat >> 1) * 8, kcn = 2 * k + (mat & 1);
       ldsm4(kb, sk + kr * DP * 2 + ((kcn ^ (kr & 7)) << 4));
       mma16816<T>(c[0], qa, kb[0], kb[1]);
