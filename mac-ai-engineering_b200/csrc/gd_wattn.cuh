@@ -348,6 +348,25 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
 __device__ __forceinline__ void st_shared16(uint32_t a, const uint32_t (&u)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
 }
+// A tile that has landed, NS slabs: rows from .. to - 1 set to 0, thread `id` of `n`. For rows past the end of a packed
+// sequence: they are the next one's, whose infinities and NaN would meet weights of 0 in the product that sums over them.
+// That product is issued after a barrier that every one of these threads arrives at.
+template <int NS>
+__device__ __forceinline__ void zero_rows(uint32_t smem, int from, int to, int id, int n) {
+  const uint32_t zero[4] = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int s = 0; s < NS; ++s)
+#pragma unroll 1
+    for (int a = from * 128 + id * 16; a < to * 128; a += n * 16) st_shared16(smem + s * kSlabBytes + a, zero);
+  fence_async_smem();
+}
+// the same by the warp that issues the product
+template <int NS>
+__device__ __forceinline__ void zero_rows(uint32_t smem, int from) {
+  if (from >= kTile) return;
+  zero_rows<NS>(smem, from, kTile, threadIdx.x & 31, 32);
+  __syncwarp();
+}
 // Rows row0 .. row0 + 31 of a swizzled tile in shared memory -> tokens t0 + row of head h, row b of a [B, T, heads, D] array,
 // rows below `live` only, NS slabs from channel ch on; one whole warp, whose own rows these are (or after a barrier). By TMA (one lane issues it and
 // waits until shared memory is read; the array's end cuts it off) unless rows past `live` belong to someone else.

@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int y = 0; ok && y < 2; ++y, ++n) {
             const int a = n % C::kKs;
             if (!(ok = warp_wait(full + a, (n / C::kKs) & 1, err, 85))) break;
+            if (pr.cu != nullptr) zero_rows<2>(s_k + a * C::kUnit, sq.Tk - kr.key(j));
             tc_fence_after();
             mma_py<T, 2>(lead, tm + C::kDq + y * 128, tm + C::kDs, s_k + a * C::kUnit, j > 0, 16);
             mma_commit(lead, empty + a);
@@ -345,6 +346,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float s[32], d[32];
       if (!(ok = warp_wait(s_full, j & 1, err, 91))) break;
       tc_fence_after();
+      if (!C::kHalves && pr.cu != nullptr && kr.key(j) + kTile > sq.Tk)  // K's rows past the sequence (S has read them)
+        zero_rows<NS>(s_k + j % C::kKs * C::kUnit, sq.Tk - kr.key(j), kTile, threadIdx.x, 32 * kWarpsEw);
       tmem_ld32(tm + lanes + part * 32, s);
       tc_fence_before();
       mbar_arrive_warp(s_read);
@@ -684,6 +687,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
           return true;
         };
         ok = ok && pair(tm, s_k);
+        auto live = [&](int i) { return sq.Tq - (lo + (it0 + i) % nq) * kTile; };  // rows of the iteration's tile
         auto both = [&](uint64_t* bar) {
           mma_commit(lead, bar);
           mma_commit(lead, bar + 1);
@@ -696,6 +700,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
         if (ok) both(dp_full);
         for (int i = 0; ok && i < n; ++i) {
           if (!(ok = wait2(p_full, i, 109) && next())) break;
+          if (pr.cu != nullptr) zero_rows<2>(s_q + u % C::kQs * C::kUnit, live(i));
           tc_fence_after();
           mma_py<T, 2>(lead, tm + C::kDv, tm, s_q + u % C::kQs * C::kUnit, i > 0, 32);
           mma_commit(lead, empty + u % C::kQs);
@@ -708,6 +713,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
             if (ok) both(s_full);
           }
           if (!(ok = ok && wait2(ds_full, i, 110) && next())) break;
+          if (pr.cu != nullptr) zero_rows<2>(s_q + u % C::kQs * C::kUnit, live(i));
           tc_fence_after();
           mma_py<T, 2>(lead, tm + C::kDk, tm + C::kDp, s_q + u % C::kQs * C::kUnit, i > 0, 32);
           mma_commit(lead, empty + u % C::kQs);
@@ -750,6 +756,16 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       if (++qt == lo + nq) qt = lo;
       if (!(ok = warp_wait(st_full + i % C::kStats, (i / C::kStats) & 1, err, 116) &&
             warp_wait(s_full + gr, i & 1, err, 112))) break;
+      if constexpr (!C::kHalves) {
+        if (pr.cu != nullptr && i0 + (gr + 1) * 64 > sq.Tq) {
+          // rows past the sequence of the group's 64 of Q and dO, once S and dP have read them (the warp that issues the
+          // products, doing this, took 10 us more of 45 at 4,093 packed rows of seven sequences, 12 heads of 96)
+          if (!(ok = warp_wait(dp_full + gr, i & 1, err, 113))) break;
+          const int from = sq.Tq - i0 > gr * 64 ? sq.Tq - i0 : gr * 64, id = threadIdx.x & 255;
+          zero_rows<NS>(s_q + i % C::kQs * C::kUnit, from, (gr + 1) * 64, id, 256);
+          zero_rows<NS>(s_o + i % C::kOs * C::kUnit, from, (gr + 1) * 64, id, 256);
+        }
+      }
       tc_fence_after();
       float s[32], d[32];
       tmem_ld32(tm + lanes + quarter * 32, s);

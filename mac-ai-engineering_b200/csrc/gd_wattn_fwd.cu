@@ -135,6 +135,11 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       const uint32_t lead = elect();
       bool ok = warp_wait(q_full, 0, err, 62);
       auto landed = [&](int c) { return warp_wait(full + c % C::kSlots, (c / C::kSlots) & 1, err, 63); };
+      auto values = [&](int c, int j) {  // the same for a unit of tile j's values
+        if (!landed(c)) return false;
+        if (pr.cu != nullptr) zero_rows<C::kUnit / kSlabBytes>(s_kv + c % C::kSlots * C::kUnit, sq.Tk - kr.key(j));
+        return true;
+      };
       if constexpr (!C::kWide) {
         // units: K(j) = 2 j, V(j) = 2 j + 1; half x of tile j is half-tile 2 j + x
         auto scores = [&](int j, int x) {
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
           const int c = 2 * j + 1;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (x == 0) ok = landed(c);
+            if (x == 0) ok = values(c, j);
             if (!(ok = ok && warp_wait(p_full + x, j & 1, err, 66))) break;
             tc_fence_after();
             mma_py<T, NS, 4>(lead, tm + C::kO, tm + 64 * x, s_kv + c % C::kSlots * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
@@ -181,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
         for (int j = 0; ok && j < kr.n; ++j) {
           if (j + 1 < kr.n && !(ok = scores(j + 1))) break;
           const int c = 4 * j + 2, set = j & 1;
-          ok = landed(c) && landed(c + 1);
+          ok = values(c, j) && values(c + 1, j);
           for (int x = 0; ok && x < 2; ++x) {
             if (!(ok = warp_wait(p_full + 2 * set + x, (j >> 1) & 1, err, 66))) break;
             tc_fence_after();

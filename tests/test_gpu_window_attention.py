@@ -124,6 +124,24 @@ def test_packed_rows(cu, D, w, s, dt):
 
 
 @gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_packed_sequences_do_not_reach_each_other(D):
+    """Infinities and NaN of a sequence stay in it, in tiles that hold rows of both too."""
+    cu, T = [0, 150, 300, 427, 700], 700
+    seqs = torch.tensor(cu, dtype=torch.int32)
+    q, k, v, do = _inputs(1, T, T, 4, 2, D, BF, 11)
+    want = _run(q, k, v, do, window=90, sinks=3, cu_seqlens=seqs)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        w = [t.clone() for t in (q, k, v, do)]
+        for t in w:
+            t[:, 150:300] = bad
+            t[:, 427:430] = bad
+        got = _run(*w, window=90, sinks=3, cu_seqlens=seqs)
+        for a, b in ((0, 150), (300, 427)):
+            assert all(torch.equal(x[:, a:b], y[:, a:b]) for x, y in zip(want, got)), (bad, a)
+
+
+@gpu
 def test_many_packed_sequences():
     """More sequences than a warp's scan step holds (256)."""
     lens = [(7 * i) % 5 for i in range(700)]
