@@ -1,5 +1,5 @@
 """A small hybrid decoder on the package's operators: a gated-delta-rule layer and a sliding-window attention layer, trained
-for some steps on a copying task, then served token by token. Run it on a B200 (the package built first):
+for some steps on a counting task, then served token by token. Run it on a B200 (the package built first):
 
     python examples/hybrid_decoder.py
 
