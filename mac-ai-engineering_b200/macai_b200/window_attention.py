@@ -6,6 +6,8 @@ alternate with the gated delta rule's, on B200 (C ABI gd_wattn_* in libgated_del
 Query i of T_q stands at position p = i + T_k - T_q (the queries are the last T_q positions) and sees key j when j <= p and
 (j > p - window or j < sinks); a query that sees no key gets zeros. `window_attention` trains and prefills (tcgen05
 products, probabilities rounded to the inputs' 16-bit type as the matrix instruction's operand, everything else float32);
+Masked scores are never used; a masked value's infinity or NaN still meets a weight of 0 in the products of its tile, as
+in the formula's matrix product, except across packed sequences, which stay apart.
 `window_attention_step` is the single-token form over a cache. bfloat16 and float16. There is no CPU path: CUDA tensors
 only.
 """
