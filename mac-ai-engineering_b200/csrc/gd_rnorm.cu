@@ -8,8 +8,8 @@
 //   8 bits:   a = max |y| over a group of channels, scale = a / 448 (1 where a = 0), q = e4m3(y / scale), from the
 //             fp32 y: the only rounding is the one to e4m3
 //
-// Bound by HBM: the forward moves 4 elements per channel (x, res in; s, y out), the backward 4 (s, dy, ds in; dx out),
-// the 8-bit form 3 and a byte. So a row is read once: a team of TPR threads holds it in registers as 16-byte chunks.
+// Bound by HBM, the backward and the 8-bit form nearly as much by issue slots: the forward moves 4 elements per channel
+// (x, res in; s, y out), the backward 4 (s, dy, ds in; dx out), the 8-bit form 3 and a byte. So a row is read once: a team of TPR threads holds it in registers as 16-byte chunks.
 // Chunks are those of the flat [rows * D] array, which start on 16-byte boundaries whatever D is; where D is not a
 // multiple of the chunk a row's first and last chunk are shared with its neighbours: their foreign
 // elements are read with them, count as zero, and are not written. So odd widths run on 16-byte loads too.

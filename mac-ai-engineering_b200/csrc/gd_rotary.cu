@@ -58,7 +58,7 @@ struct Args {
 // A thread has one unit of one head (the turned units first, so that a warp turns or copies) and walks the CTA's tokens:
 // the address arithmetic of an item is done once, not once per token. Warps, not loads per thread, keep memory busy: with
 // one token's loads in flight a thread needs 40 registers, and q, k of 4 x 4096 tokens (16 + 4 heads of 128, 32 turned,
-// bf16, views of a fused projection) take 35 us (4.9 TB/s); with two tokens ahead 49 us, with four 65 us.
+// bf16, views of a fused projection) take 33 us (5.1 TB/s); with two tokens ahead 49 us, with four 65 us.
 template <typename T, int V, bool IL>
 __global__ void __launch_bounds__(kMaxThreads, 3) rotary_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                              T* __restrict__ oq, T* __restrict__ ok, const Args a,

@@ -17,7 +17,7 @@
 // D <= 256: one CTA an SM, S of 128 keys double-buffered, K and V pass in halves of 128 channels through a ring of five.
 // Measured (bf16, operations of visible pairs): 1 x 8192 x 16 heads (4 key heads), D 128, window 2048 139 us (870 TFLOP/s);
 // 1 x 16384 x 16 causal D 128 1,150, D 256 1,010 TFLOP/s; D 64 with window 4096 395 us (615 TFLOP/s), where an exponential
-// comes with half the operations of D 128 and the special-function and issue slots bound it. cuBLAS: 1,641 TFLOP/s.
+// comes with half the operations of D 128 (special-function pipe 62 % busy, tensor pipe 31 %). cuBLAS: 1,641 TFLOP/s.
 #include "gd_wattn.cuh"
 
 namespace gd {
