@@ -30,8 +30,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[dict] 
                           fastest keeps its speed
       "yarn"              pairs that turn more than "fast" (32) times within "original_length" positions keep their
                           speed, those that turn less than "slow" (1) times are slowed by "factor", in between a linear
-                          ramp over the pair's index; cos and sin are multiplied by "attention_factor"
-                          (default 0.1 ln factor + 1)"""
+                          ramp over the pair's index (which may end past the last pair); cos and sin are multiplied
+                          by "attention_factor" (default 0.1 ln factor + 1)"""
     if dim <= 0 or dim % 2:
         raise ValueError(f"rotary_frequencies: dim must be positive and even, got {dim}")
     i = torch.arange(0, dim, 2, dtype=torch.float64)
@@ -53,7 +53,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[dict] 
         def pair(turns):  # the (fractional) pair that turns so often within the original length
             return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
         low = max(math.floor(pair(float(scaling.get("fast", 32.0)))), 0)
-        high = min(math.ceil(pair(float(scaling.get("slow", 1.0)))), dim // 2 - 1)
+        # bounded by dim - 1 as published: a ramp that ends past the last pair keeps its slope
+        high = min(math.ceil(pair(float(scaling.get("slow", 1.0)))), dim - 1)
         slowed = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
         return freq * (1 - slowed) + freq / factor * slowed, float(
             scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
