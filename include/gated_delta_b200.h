@@ -305,7 +305,8 @@ int gd_rotary(const void* q, const void* k, void* oq, void* ok, const float* tab
  * up leaves NaN in the rows it was for, word or no word. A finite result row needs finite values in its tile of 128 keys and
  * 128 queries: masked scores are never used, but a masked key's infinity or NaN in v (or in k, q, d_o for the gradients)
  * meets a weight of 0 in the products, as it would in a matrix product of the formula. (A packed sequence's infinities
- * and NaN stay in it; float16's gradients share one power-of-two scale, from the call's largest |d_o|.) */
+ * and NaN stay in it; float16's dS has one power-of-two scale for the call, from the largest
+ * norms of d_o's and v's rows: it does not overflow, and keeps float16's 11 bits down to 2^-29 of its bound.) */
 
 /* Bytes of workspace gd_wattn_fwd (for_backward 0) or gd_wattn_bwd need (0 for invalid sizes); packed: with cu_seqlens. */
 size_t gd_wattn_workspace_bytes(int B, int Tq, int Tk, int H, int HK, int D, int window, int sinks, int packed,

@@ -150,7 +150,7 @@ extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const v
       workspace_bytes < gd_wattn_workspace_bytes(B, Tq, Tk, H, HK, D, window, sinks, cu_seqlens != nullptr, 1))
     return GD_ERR_WORKSPACE;
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  // the error word, with float16's largest |dO| in it; bfloat16's first kernel clears it
+  // the error word, with float16's largest norms in it; bfloat16's first kernel clears it
   if (dtype == GD_FLOAT16 && cudaMemsetAsync(workspace, 0, sizeof(ErrorWord), cs) != cudaSuccess)
     return (cudaGetLastError(), GD_ERR_LAUNCH);
   const Problem p = problem(cu_seqlens, N, B, Tq, Tk, H, HK, D, window, sinks, scale);

@@ -6,7 +6,7 @@
 // bf16: delta 21 us (4.7 TB/s), dq 171 us, dk dv 300 us (1,060 and 810 TFLOP/s of 6 and 8 D operations a visible pair); at
 // 2 x 2048 x 8 (2), D 256, causal: 10, 73 and 145 us.
 // Three kernels, none of which waits on another CTA and none with atomics on results (the same bits every run):
-//   delta_kernel  delta, and for float16 the largest |dO| (the scale below)
+//   delta_kernel  delta, and for float16 the largest ||dO|| and ||v|| (the scale below)
 //   dq_kernel     one CTA per 128 queries of a head, over the key tiles they see
 //   dkv_kernel    one CTA per 128 keys of a key head, over the group's query heads and the query tiles that see them
 // S and dP are formed twice (7 products of 128 x 128 x D a tile pair instead of 5): with the queries on the rows in the
@@ -14,8 +14,12 @@
 // dS, P are the A operands of the products that follow straight from TMEM; nothing is exchanged between CTAs.
 //
 // P and dS are rounded to the inputs' 16-bit type (the operand type of the matrix instruction); exponentials, sums and
-// accumulators are fp32. float16: dS is scaled by a power of two that brings the largest |dO| into [1, 2) before its
-// rounding, and dQ, dK are scaled back: gradients of any size keep float16's 11 bits.
+// accumulators are fp32. float16 has normal numbers from 2^-14 to 2^16 only, so both are scaled by powers of two before their
+// rounding and the results scaled back:
+//   P by 2^15 (P <= 1): all 11 bits down to P = 2^-29, as rows of millions of keys have
+//   dS by F = 2^e, one for the call, with 2 F max ||dO|| max ||v|| in [2^14, 2^15]. That bounds F |dS| (dP is a product of two
+//   rows, delta an average of dP), so nothing overflows whatever the sizes of dO and v, and |dS| keeps 11 bits down to 2^-29
+//   of its bound; below, it is off by 2^-40 of the bound at most.
 #include "gd_wattn.cuh"
 
 namespace gd {
@@ -25,37 +29,87 @@ namespace {
 constexpr int kWarpsEw = 16;                     // elementwise work: four threads a row, 32 columns each
 constexpr int kThreads = 32 * (kWarpsEw + 2);    // + loads, + products (dK, dV: one more, for L and delta)
 
-// the error word's first spare field holds the bits of the largest |dO| (float16)
+constexpr float kPScale = 32768.f, kPLog2 = 15.f;  // float16's P in dV and dK
+
+// F. The error word's first spare fields hold the bits of the largest ||dO||^2 and ||v||^2 (float16; 0 or 2^-48 .. 2^41 each).
 __device__ __forceinline__ float ds_scale(const ErrorWord* err) {
-  const float a = __int_as_float(*reinterpret_cast<const volatile int*>(&err->pad[0]));
-  if (!(a > 0.f) || a > 3e38f) return 1.f;
-  const int e = 127 - ((__float_as_int(a) >> 23) & 0xff);  // a 2^e in [1, 2); subnormal a: e = 127
-  return __int_as_float((127 + (e > 100 ? 100 : e)) << 23);
+  const volatile int* p = &err->pad[0];
+  const float c = __int_as_float(p[0]) * __int_as_float(p[1]);
+  if (!(c > 0.f)) return 1.f;  // dS is 0
+  const int e = ((__float_as_int(c) >> 23) & 0xff) - 127;  // sqrt(c) in [2^(k - 1), 2^k] with k = (e + 2) >> 1
+  return __int_as_float((127 + 14 - ((e + 2) >> 1)) << 23);
 }
 
 // ---- delta = rowsum(dO O), O as its 16-bit value and what its rounding took away (delta and dP nearly cancel in rows
 // that see few keys: O's rounding alone would cost dS half a bit there). 16 lanes a row of [B, Tq, H], kRowsEach rows in
-// flight. HBM-bound: three reads of [B, Tq, H, D].
+// flight. HBM-bound: three reads of [B, Tq, H, D]. float16: also the largest ||dO||^2, and in the CTAs from `first_v` on the
+// largest ||v||^2 (a row with an infinity or NaN does not count: what it reaches is infinite or NaN under any scale).
 constexpr int kRowsEach = 4;
+
+struct ValueRows {  // v [B, Tk, HK, D], strides in elements
+  const void* v;
+  long long b, t, h, rows;  // rows: Tk HK
+  int HK;
+  unsigned first;           // the CTAs from here on
+};
+
+// the largest of the warp's non-negative values, infinities and NaN aside -> word `to` (a maximum: any order)
+__device__ __forceinline__ void put_max(float top, int* to) {
+#pragma unroll
+  for (int w = 16; w >= 1; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(to, __float_as_int(top));
+}
+__device__ __forceinline__ float finite_or_0(float x) { return x <= 3e38f ? x : 0.f; }
 
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, const T* __restrict__ low,
                                                     const T* __restrict__ g, long long gb, long long gt, long long gh,
-                                                    float* __restrict__ delta, int Tq, int H, int D, ErrorWord* err) {
+                                                    float* __restrict__ delta, int Tq, int H, int D, const ValueRows vr,
+                                                    ErrorWord* err) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   const int sub = threadIdx.x & 15;
+  if constexpr (kHalf) {
+    if (blockIdx.x >= vr.first) {
+      const long long row0 = (long long)(blockIdx.x - vr.first) * (16 * kRowsEach) + (threadIdx.x >> 4);
+      float top = 0.f;
+#pragma unroll
+      for (int r = 0; r < kRowsEach; ++r) {
+        const long long row = row0 + r * 16, t = row / vr.HK;
+        float n = 0.f;
+        if (row < vr.rows) {
+          const T* v = static_cast<const T*>(vr.v) + blockIdx.y * vr.b + t * vr.t + (row - t * vr.HK) * vr.h;
+          for (int c = sub * 8; c < D; c += 128) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(v + c));
+            const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 y = unpack16<T>(uu[i]);
+              n = fmaf(y.x, y.x, n);
+              n = fmaf(y.y, y.y, n);
+            }
+          }
+        }
+#pragma unroll
+        for (int w = 8; w >= 1; w >>= 1) n += __shfl_xor_sync(0xffffffffu, n, w);
+        top = fmaxf(top, finite_or_0(n));
+      }
+      put_max(top, &err->pad[1]);
+      return;
+    }
+  }
   const unsigned rows = (unsigned)Tq * (unsigned)H;  // of batch row blockIdx.y
-  if (!std::is_same<T, __half>::value && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < sizeof(ErrorWord) / 4)
+  if (!kHalf && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < sizeof(ErrorWord) / 4)
     reinterpret_cast<int*>(err)[threadIdx.x] = 0;  // (this kernel waits for nothing; the next ones record)
   const unsigned row0 = blockIdx.x * (16 * kRowsEach) + (threadIdx.x >> 4);
   o += (long long)blockIdx.y * rows * D;
   low += (long long)blockIdx.y * rows * D;
   g += blockIdx.y * gb;
   delta += (long long)blockIdx.y * rows;
-  float s[kRowsEach], top = 0.f;
+  float s[kRowsEach], n[kRowsEach];  // n: ||dO||^2
   unsigned h[kRowsEach], t[kRowsEach];
 #pragma unroll
   for (int r = 0; r < kRowsEach; ++r) {
-    s[r] = 0.f;
+    s[r] = n[r] = 0.f;
     t[r] = (row0 + r * 16) / (unsigned)H;
     h[r] = row0 + r * 16 - t[r] * (unsigned)H;
   }
@@ -78,23 +132,24 @@ __global__ void __launch_bounds__(256) delta_kernel(const T* __restrict__ o, con
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 x = unpack16<T>(ua[i]), z = unpack16<T>(ul[i]), y = unpack16<T>(ud[i]);
-        if constexpr (std::is_same<T, __half>::value) top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+        if constexpr (kHalf) n[r] = fmaf(y.x, y.x, fmaf(y.y, y.y, n[r]));
         s[r] = fmaf(x.x + z.x, y.x, s[r]);
         s[r] = fmaf(x.y + z.y, y.y, s[r]);
       }
     }
   }
+  float top = 0.f;
 #pragma unroll
   for (int r = 0; r < kRowsEach; ++r) {
 #pragma unroll
-    for (int w = 8; w >= 1; w >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], w);
+    for (int w = 8; w >= 1; w >>= 1) {
+      s[r] += __shfl_xor_sync(0xffffffffu, s[r], w);
+      if constexpr (kHalf) n[r] += __shfl_xor_sync(0xffffffffu, n[r], w);
+    }
     if (row0 + r * 16 < rows && sub == 0) delta[(long long)h[r] * Tq + t[r]] = s[r];
+    top = fmaxf(top, finite_or_0(n[r]));
   }
-  if constexpr (std::is_same<T, __half>::value) {
-#pragma unroll
-    for (int w = 16; w >= 1; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&err->pad[0], __float_as_int(top));  // a maximum: any order
-  }
+  if constexpr (kHalf) put_max(top, &err->pad[0]);
 }
 
 // 16 fp32 columns (from channel c) of an accumulator times f -> row `row` of a swizzled tile in shared memory, rounded
@@ -547,7 +602,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
                  s_o = s_q + C::kQs * C::kUnit;
 
   if (warp == kWarpsEw + 2) {
-    // -L and -delta of each iteration's queries, a step ahead of the elementwise warps; dead queries get -inf and 0
+    // -L (float16: + 15, P's scale) and -delta of each iteration's queries, a step ahead of the elementwise warps; dead queries get -inf and 0
     const long long at = (long long)sq.b * pr.H * pr.Tq + sq.q0;
     int h = hk * G + (n > 0 ? it0 / nq : 0), qt = lo + (n > 0 ? it0 % nq : 0);
     for (int i = 0; i < n; ++i) {
@@ -556,7 +611,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       for (int x = 0; x < 4; ++x) {
         const int t = qt * kTile + x * 32 + lane;
         const bool live = t < sq.Tq;
-        L[x] = live ? -__ldg(lse + at + (long long)h * pr.Tq + t) : -INFINITY;
+        L[x] = live ? (std::is_same<T, __half>::value ? kPLog2 : 0.f) - __ldg(lse + at + (long long)h * pr.Tq + t) : -INFINITY;
         de[x] = live ? -__ldg(delta + at + (long long)h * pr.Tq + t) : 0.f;
       }
       if (++qt == lo + nq) {
@@ -738,8 +793,10 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int key = c0 + row;
     const F2 sc = f2(pr.scale_log2, pr.scale_log2);
+    constexpr bool kHalf = std::is_same<T, __half>::value;
     float f = 1.f;
-    if constexpr (std::is_same<T, __half>::value) f = ds_scale(err);
+    if constexpr (kHalf) f = ds_scale(err);
+    const float fp = kHalf ? f / kPScale : f;  // dS from a P that carries 2^15
     bool ok = true;
     int qt = lo + (n > 0 ? it0 % nq : 0);  // the iteration's query tile
     for (int i = 0; i < n; ++i) {
@@ -799,8 +856,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const ulonglong2 e = D4[c / 4];
-        u[c / 2] = ds2<T>(f2(s[c], s[c + 1]), f2(d[c], d[c + 1]), e.x, f);
-        u[c / 2 + 1] = ds2<T>(f2(s[c + 2], s[c + 3]), f2(d[c + 2], d[c + 3]), e.y, f);
+        u[c / 2] = ds2<T>(f2(s[c], s[c + 1]), f2(d[c], d[c + 1]), e.x, fp);
+        u[c / 2 + 1] = ds2<T>(f2(s[c + 2], s[c + 3]), f2(d[c + 2], d[c + 3]), e.y, fp);
       }
       tmem_st16(tm + lanes + C::kDp + quarter * 32, u);
       tmem_st_wait();
@@ -814,7 +871,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
     }
     // quarters 0 and 1 take dK's channels, 2 and 3 dV's; key row each
     const bool is_k = quarter < 2;
-    const float g = !ok ? NAN : is_k ? pr.scale / f : 1.f;
+    const float g = !ok ? NAN : is_k ? pr.scale / f : kHalf ? 1.f / kPScale : 1.f;
     const uint32_t acc = tm + lanes + (is_k ? C::kDk : C::kDv);
     const int ch = xh * 128;  // the first channel accumulated
 #pragma unroll 1
@@ -888,10 +945,12 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
       !out_map(&mdq, dq, dt, pr.B, pr.Tq, pr.H, pr.D) || !out_map(&mdk, dk, dt, pr.B, pr.Tk, pr.HK, pr.D) ||
       !out_map(&mdv, dv, dt, pr.B, pr.Tk, pr.HK, pr.D))
     return GD_ERR_LAUNCH;
-  const long long rows = (long long)pr.Tq * pr.H;
-  delta_kernel<T><<<dim3((unsigned)((rows + 16 * kRowsEach - 1) / (16 * kRowsEach)), (unsigned)pr.B), 256, 0, stream>>>(
+  auto ctas = [](long long rows) { return (unsigned)((rows + 16 * kRowsEach - 1) / (16 * kRowsEach)); };
+  const ValueRows vr = {v, st[6], st[7], st[8], (long long)pr.Tk * pr.HK, pr.HK, ctas((long long)pr.Tq * pr.H)};
+  const unsigned blocks = vr.first + (std::is_same<T, __half>::value ? ctas(vr.rows) : 0);
+  delta_kernel<T><<<dim3(blocks, (unsigned)pr.B), 256, 0, stream>>>(
       static_cast<const T*>(o), static_cast<const T*>(low), static_cast<const T*>(g), st[9], st[10], st[11], delta, pr.Tq,
-      pr.H, pr.D, err);
+      pr.H, pr.D, vr, err);
   static bool done_q[kMaxDevices], done_kv[kMaxDevices];
   auto kq = dq_kernel<T, NS>;
   auto kkv = dkv_kernel<T, NS>;
