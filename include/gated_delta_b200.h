@@ -295,7 +295,7 @@ int gd_rotary(const void* q, const void* k, void* oq, void* ok, const float* tab
 /* ---- causal softmax attention with a sliding window and first tokens that stay visible ----
  * The mixer of the layers that alternate with the rule's. Query i of Tq stands at position p = i + Tk - Tq and sees key j
  * when j <= p and (j > p - window or j < sinks); window 0: no window. o = softmax(scale q k^T) v over the visible keys,
- * zeros for a query that sees none. q [B, Tq, H, D], k, v [B, Tk, HK, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), H a
+ * zeros for a query that sees none; scale: any finite number. q [B, Tq, H, D], k, v [B, Tk, HK, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), H a
  * multiple of HK (each key head serves H / HK consecutive query heads), D a multiple of 8 up to 256, read through
  * `strides` (host array, elements: batch, token and head stride of q, k, v, and for the backward of d_o; multiples of 8,
  * channels adjacent); o, dq [B, Tq, H, D] and dk, dv [B, Tk, HK, D] contiguous; every pointer 16-byte aligned. lse

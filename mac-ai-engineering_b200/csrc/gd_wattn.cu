@@ -46,6 +46,7 @@ Problem problem(const int* cu, int N, int B, int Tq, int Tk, int H, int HK, int 
   p.sinks = sinks < Tk ? sinks : Tk;
   p.scale = scale;
   p.scale_log2 = scale * gd::wattn::kLog2e;
+  p.negate = false;
   p.cu = cu;
   p.N = N;
   return p;
@@ -116,7 +117,10 @@ extern "C" int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
   if (workspace != nullptr && cudaMemsetAsync(workspace, 0, sizeof(ErrorWord), cs) != cudaSuccess)
     return (cudaGetLastError(), GD_ERR_LAUNCH);
-  const Problem p = problem(cu_seqlens, N, B, Tq, Tk, H, HK, D, window, sinks, scale);
+  Problem p = problem(cu_seqlens, N, B, Tq, Tk, H, HK, D, window, sinks, scale);
+  // a scale of 0 as a tiny one: finite scores vanish beside 1, and a masked one stays -inf
+  p.scale_log2 = scale == 0.f ? 1e-30f : std::fabs(p.scale_log2);
+  p.negate = scale < 0.f;
   if (Tk == 0) {  // no keys at all: zeros
     const size_t n = (size_t)B * Tq * H * D * 2;
     if (cudaMemsetAsync(o, 0, n, cs) != cudaSuccess ||

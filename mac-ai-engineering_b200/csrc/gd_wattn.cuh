@@ -21,7 +21,10 @@ struct Problem {
   int B, Tq, Tk, H, HK;    // packed rows: B = 1, Tq = Tk = all rows
   int D;
   int window, sinks;       // key j is visible to position p: j <= p and (j > p - window or j < sinks)
-  float scale, scale_log2;  // scale, and scale * log2(e)
+  // scale, and scale * log2(e). The forward, whose mask and maximum come before its scale, takes a positive scale_log2 and
+  // the scale's sign apart.
+  float scale, scale_log2;
+  bool negate;
   const int* cu;           // packed rows' boundaries [N + 1], or NULL
   int N;
 };

@@ -223,6 +223,10 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       const uint32_t ts = tm + lanes + b * 64;
       float s[64];
       tmem_ld64(ts, s);
+      if (pr.negate) {  // from here on the scale is positive
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s[i] = -s[i];
+      }
       const int c0 = kr.key(j) + 64 * x;
       if (!all_visible(kr.key(j), p0, p1, pr.window, pr.sinks)) {
         const uint32_t v0 = visible_keys(c0, p, pr.window, pr.sinks), v1 = visible_keys(c0 + 32, p, pr.window, pr.sinks);
