@@ -300,7 +300,9 @@ int gd_rotary(const void* q, const void* k, void* oq, void* ok, const float* tab
  * `strides` (host array, elements: batch, token and head stride of q, k, v, and for the backward of d_o; multiples of 8,
  * channels adjacent); o, dq [B, Tq, H, D] and dk, dv [B, Tk, HK, D] contiguous; every pointer 16-byte aligned. lse
  * [B, H, Tq] fp32: log2 of the sum of the exponentials, for the backward. cu_seqlens (device int32 [N + 1], or NULL):
- * packed rows, B = 1 and Tq = Tk, each sequence on its own; boundaries outside [0, Tq] or falling are clamped.
+ * packed rows, B = 1 and Tq = Tk, each sequence on its own; rows before the first and behind the last
+ * (padding) give zeros, in o and in the gradients. Boundaries are clamped into [0, Tq]; one below an earlier one counts as that
+ * one.
  * The workspace starts with an error word (gd_read_error); the forward's is nothing else and may be NULL. A wait that gives
  * up leaves NaN in the rows it was for, word or no word. A finite result row needs finite values in its tile of 128 keys and
  * 128 queries: masked scores are never used, but a masked key's infinity or NaN in v (or in k, q, d_o for the gradients)

@@ -37,20 +37,38 @@ struct Seq {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
-// The packed sequence that owns work item `item`, when a sequence of n rows has count(n) items; returns its index within
-// the sequence, or -1 past the last. One whole warp; boundaries are clamped into [0, rows], so no input leaves the arrays.
+// The packed sequence that owns work item `item`, when a run of n rows has count(n) items; returns its index within the
+// sequence, or -1 past the last. After the sequences' items come those of the rows before the first and behind the last, which
+// belong to none: `gap` is set (their results are zeros). One whole warp. Boundaries are clamped into [0, rows], and one below
+// an earlier one counts as that one: whatever cu holds, every row has exactly one owner.
 template <typename Count>
-__device__ __forceinline__ int find_item(const int* cu, int N, int rows, int item, Count count, Seq& s) {
+__device__ __forceinline__ int find_item(const int* cu, int N, int rows, int item, Count count, Seq& s, bool& gap) {
   constexpr int kPer = 8;
   const int lane = threadIdx.x & 31;
-  int before = 0;
+  int before = 0, top = 0;  // items and the highest boundary so far
+  gap = false;
   for (int base = 0; base < N; base += 32 * kPer) {
-    int first[kPer], len[kPer], sum = 0;
+    int first[kPer], len[kPer], high = 0, sum = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int n = base + lane * kPer + i;
-      first[i] = n < N ? clampi(__ldg(cu + n), 0, rows) : 0;
-      len[i] = n < N ? clampi(__ldg(cu + n + 1), first[i], rows) - first[i] : 0;
+      first[i] = high = max(high, n < N ? clampi(__ldg(cu + n), 0, rows) : 0);  // the lane's highest so far
+    }
+    int upto = high;  // of the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto = max(upto, y);
+    }
+    int below = __shfl_up_sync(0xffffffffu, upto, 1);
+    below = lane > 0 ? max(below, top) : top;
+    int end = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int n = base + lane * kPer + i;
+      first[i] = max(first[i], below);
+      len[i] = n < N ? max(clampi(__ldg(cu + n + 1), 0, rows) - first[i], 0) : 0;
+      end = max(end, first[i] + len[i]);
       sum += count(len[i]);
     }
     int incl = sum;
@@ -80,9 +98,22 @@ __device__ __forceinline__ int find_item(const int* cu, int N, int rows, int ite
       return __shfl_sync(0xffffffffu, found, src);
     }
     before += total;
+    top = __reduce_max_sync(0xffffffffu, end);
   }
-  return -1;
+  gap = true;
+  const int head = clampi(__ldg(cu), 0, rows);
+  int i = item - before;
+  s.b = 0;
+  s.q0 = s.k0 = 0;
+  s.Tq = s.Tk = head;
+  if (i < count(head)) return i;
+  i -= count(head);
+  s.q0 = s.k0 = top;
+  s.Tq = s.Tk = rows - top;
+  return i < count(rows - top) ? i : -1;
 }
+// The items of N packed sequences of `rows` rows in all, in tiles of kTile, with the two runs of rows that belong to none
+inline long long packed_items(int rows, int N) { return (long long)rows / kTile + N + 2; }
 
 // The key tiles that queries [i0, i1] (positions p0 .. p1) of a sequence see: the first `head` tiles, then tiles
 // lo .. lo + n - head - 1.

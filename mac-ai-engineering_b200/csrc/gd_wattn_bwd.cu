@@ -240,12 +240,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int item = gridDim.x - 1 - blockIdx.x, h = blockIdx.y;  // later tiles see more keys: first
   Seq sq;
   int tile = item;
+  bool gap = false;
   if (pr.cu != nullptr && warp == 0) {
-    tile = find_item(pr.cu, pr.N, pr.Tq, item, [](int n) { return (n + kTile - 1) / kTile; }, sq);
+    tile = find_item(pr.cu, pr.N, pr.Tq, item, [](int n) { return (n + kTile - 1) / kTile; }, sq, gap);
     if (lane == 0) {
       info[0] = tile;
       info[1] = sq.q0;
       info[2] = sq.Tq;
+      info[3] = gap;
     }
   }
   tc_fence_before();
@@ -256,6 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     sq.b = 0;
     sq.q0 = sq.k0 = info[1];
     sq.Tq = sq.Tk = info[2];
+    gap = info[3] != 0;
   } else {
     sq = {(int)blockIdx.z, 0, pr.Tq, 0, pr.Tk};
   }
@@ -263,7 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int i0 = tile * kTile;
   const int i1 = i0 + kTile - 1 < sq.Tq - 1 ? i0 + kTile - 1 : sq.Tq - 1;
   const int p0 = i0 + sq.offset(), p1 = i1 + sq.offset();
-  const KeyRange kr(tile < 0 ? -1 : p0, tile < 0 ? -1 : p1, pr.window, pr.sinks);
+  const bool idle = tile < 0 || gap;
+  const KeyRange kr(idle ? -1 : p0, idle ? -1 : p1, pr.window, pr.sinks);
   const uint32_t s_q = smem_u32(base), s_o = s_q + NS * kSlabBytes, s_k = s_o + NS * kSlabBytes,
                  s_v = s_k + C::kKs * C::kUnit;
 
@@ -556,6 +560,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
   Seq sq;
   // the first key tiles are seen by most queries: they start first, cut into parts where that pays
   int tile = blockIdx.x, part = 0, parts = 1;
+  bool gap = false;
   if (tile < sp.heavy * sp.parts) {
     parts = sp.parts;
     part = tile % parts;
@@ -564,11 +569,12 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
     tile -= sp.heavy * (sp.parts - 1);
   }
   if (pr.cu != nullptr && warp == 0) {
-    tile = find_item(pr.cu, pr.N, pr.Tk, blockIdx.x, [](int n) { return (n + kTile - 1) / kTile; }, sq);
+    tile = find_item(pr.cu, pr.N, pr.Tk, blockIdx.x, [](int n) { return (n + kTile - 1) / kTile; }, sq, gap);
     if (lane == 0) {
       info[0] = tile;
       info[1] = sq.q0;
       info[2] = sq.Tq;
+      info[3] = gap;
     }
   }
   tc_fence_before();
@@ -579,6 +585,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
     sq.b = 0;
     sq.q0 = sq.k0 = info[1];
     sq.Tq = sq.Tk = info[2];
+    gap = info[3] != 0;
   } else {
     sq = {(int)blockIdx.z, 0, pr.Tq, 0, pr.Tk};
   }
@@ -586,7 +593,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
   const int c0 = tile * kTile, off = sq.offset();
   // the query tiles that see some of these keys
   int lo = 0, nq = 0;
-  if (tile >= 0) {
+  if (tile >= 0 && !gap) {
     const int from = c0 - off > 0 ? c0 - off : 0;
     int last = sq.Tq - 1;
     if (c0 >= pr.sinks && pr.window < kNoWindow) {
@@ -956,8 +963,8 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
   auto kkv = dkv_kernel<T, NS>;
   if (set_smem_once(kq, DqCfg<NS>::kSmem, done_q) != cudaSuccess || set_smem_once(kkv, DkvCfg<NS>::kSmem, done_kv) != cudaSuccess)
     return (cudaGetLastError(), GD_ERR_LAUNCH);
-  const long long qt = pr.cu ? (long long)pr.Tq / kTile + pr.N : (pr.Tq + kTile - 1) / kTile;
-  const long long kt = (pr.cu ? (long long)pr.Tk / kTile + pr.N : (pr.Tk + kTile - 1) / kTile) + (long long)sp.heavy * (sp.parts - 1);
+  const long long qt = pr.cu ? packed_items(pr.Tq, pr.N) : (pr.Tq + kTile - 1) / kTile;
+  const long long kt = (pr.cu ? packed_items(pr.Tk, pr.N) : (pr.Tk + kTile - 1) / kTile) + (long long)sp.heavy * (sp.parts - 1);
   kq<<<dim3((unsigned)qt, (unsigned)pr.H, (unsigned)pr.B), kThreads, DqCfg<NS>::kSmem, stream>>>(
       mq, mk, mv, mo, mdq, pr, lse, delta, static_cast<T*>(dq), err);
   kkv<<<dim3((unsigned)kt, (unsigned)(pr.HK * (NS == 4 ? 2 : 1)), (unsigned)pr.B), kThreads + 32, DkvCfg<NS>::kSmem, stream>>>(

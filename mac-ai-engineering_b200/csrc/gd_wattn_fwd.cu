@@ -88,12 +88,14 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   const int item = gridDim.x - 1 - blockIdx.x, h = blockIdx.y;
   Seq sq;
   int tile = item;
+  bool gap = false;
   if (pr.cu != nullptr && warp == 0) {
-    tile = find_item(pr.cu, pr.N, pr.Tq, item, [](int n) { return (n + kTile - 1) / kTile; }, sq);
+    tile = find_item(pr.cu, pr.N, pr.Tq, item, [](int n) { return (n + kTile - 1) / kTile; }, sq, gap);
     if (lane == 0) {
       info[0] = tile;
       info[1] = sq.q0;
       info[2] = sq.Tq;
+      info[3] = gap;
     }
   }
   tc_fence_before();
@@ -104,6 +106,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     sq.b = 0;
     sq.q0 = sq.k0 = info[1];
     sq.Tq = sq.Tk = info[2];
+    gap = info[3] != 0;
   } else {
     sq = {(int)blockIdx.z, 0, pr.Tq, 0, pr.Tk};
   }
@@ -111,7 +114,8 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
   const int i0 = tile * kTile;
   const int i1 = i0 + kTile - 1 < sq.Tq - 1 ? i0 + kTile - 1 : sq.Tq - 1;
   const int p0 = i0 + sq.offset(), p1 = i1 + sq.offset();
-  const KeyRange kr(tile < 0 ? -1 : p0, tile < 0 ? -1 : p1, pr.window, pr.sinks);
+  const bool idle = tile < 0 || gap;
+  const KeyRange kr(idle ? -1 : p0, idle ? -1 : p1, pr.window, pr.sinks);
   const uint32_t s_q = smem_u32(base), s_kv = s_q + C::kQBytes;
 
   if (warp == kWarpsSm) {
@@ -345,7 +349,7 @@ int launch(const void* q, const void* k, const void* v, const long long* st, con
   static bool done[kMaxDevices];
   auto kern = fwd_kernel<T, NS>;
   if (set_smem_once(kern, Cfg<NS>::kSmem, done) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  const long long tiles = pr.cu ? (long long)pr.Tq / kTile + pr.N : (pr.Tq + kTile - 1) / kTile;
+  const long long tiles = pr.cu ? packed_items(pr.Tq, pr.N) : (pr.Tq + kTile - 1) / kTile;
   const dim3 grid((unsigned)tiles, (unsigned)pr.H, (unsigned)pr.B);
   kern<<<grid, kThreads, Cfg<NS>::kSmem, stream>>>(mq, mk, mv, mo, ml, pr, static_cast<T*>(o), static_cast<T*>(low), lse, err);
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);

@@ -150,10 +150,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
                      scale: Optional[float] = None, cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
     """o [B, T_q, H, D] for q [B, T_q, H, D] and k, v [B, T_k, H_k, D] (H a multiple of H_k: each key head serves
     H / H_k consecutive query heads), bfloat16 or float16, D a multiple of 8 up to 256. Each query sees its own position
-    and those before it, of which the last `window` (None: all) and the first `sinks`. scale: of the scores, any
-    finite number, default D^-0.5. cu_seqlens: int [N + 1], the boundaries of N sequences packed along the tokens of one batch row, each on its
-    own (positions count from its first token, also for `sinks`). Inputs may be strided views; gradients are the same
-    bits every run."""
+    and those before it, of which the last `window` (None: all) and the first `sinks`. scale: of the scores, any finite
+    number, default D^-0.5. cu_seqlens: int [N + 1], the boundaries of N sequences packed along the tokens of one batch
+    row, each on its own (positions count from its first token, also for `sinks`). A list on the host must rise from 0 to
+    T; one on the device is not looked at by the host: rows before its first and behind its last boundary give zeros, in o
+    and in the gradients, and a boundary below an earlier one counts as that one. Inputs may be strided views; gradients are
+    the same bits every run."""
     _check_qkv("window_attention", q, k, v)
     w, s = _check_mask("window_attention", window, sinks)
     cu = _check_cu(cu_seqlens, q, k)
