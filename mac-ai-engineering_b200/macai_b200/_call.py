@@ -4,6 +4,7 @@ current)."""
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -45,10 +46,18 @@ def first_order(backward):
     return wrapper
 
 
+def has_tangent(*ts) -> bool:
+    """Whether one of these inputs (None allowed) carries a forward-mode tangent (torch.autograd.forward_ad)."""
+    if forward_ad._current_level < 0:  # no dual level is open
+        return False
+    return any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
 def recorded(*ts) -> bool:
-    """Whether autograd records a call with these inputs (None allowed)."""
+    """Whether autograd has a part in a call with these inputs (None allowed): a gradient to record, or a tangent, which
+    the autograd functions refuse (they have no forward-mode derivative)."""
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
                 return True
-    return False
+    return has_tangent(*ts)
