@@ -264,7 +264,8 @@ int gd_rnorm_fwd(const void* x, const void* res, const void* w, void* s, void* y
                  int zero_centered, long long rows, int D, float eps, void* stream);
 
 /* The same with y in 8 bits: q [rows, D] e4m3 and scale [rows, ceil(D / group)] fp32, y = q scale. Each `group`
- * channels (a multiple of 8; 0: the whole row) share scale = max |y| / 448, or 1 where they are all zero. */
+ * channels (a multiple of 8; 0: the whole row) share scale = max |y| / 448, at least 2^-126, or 1 where
+ * they are all zero. */
 int gd_rnorm_fp8(const void* x, const void* res, const void* w, void* s, void* q, float* scale, int dtype, int wdtype,
                  int zero_centered, long long rows, int D, int group, float eps, void* stream);
 

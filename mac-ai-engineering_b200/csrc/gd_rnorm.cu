@@ -5,8 +5,8 @@
 //   y = (xh w').to(T)                           w' = w, or 1 + w for a zero-centred weight; one rounding
 //   backward: h = dy w',  dx = (ds + r (h - xh mean(h xh))).to(T)  (the gradient of x and of res),
 //             dw = sum over rows of dy xh       (only when asked: fixed-order partial rows, then a sum)
-//   8 bits:   a = max |y| over a group of channels, scale = a / 448 (1 where a = 0), q = e4m3(y / scale), from the
-//             fp32 y: the only rounding is the one to e4m3
+//   8 bits:   a = max |y| over a group of channels, scale = max(a / 448, 2^-126) (1 where a = 0), q = e4m3(y / scale),
+//             from the fp32 y: the only rounding is the one to e4m3
 //
 // Bound by HBM, the backward and the 8-bit form nearly as much by issue slots: the forward moves 4 elements per channel
 // (x, res in; s, y out), the backward 4 (s, dy, ds in; dx out), the 8-bit form 3 and a byte. So a row is read once: a team of TPR threads holds it in registers as 16-byte chunks.
@@ -32,6 +32,7 @@ constexpr int kMaxD = kMaxChunks * 8;
 constexpr int kThreads = 256;       // a CTA, unless a row needs more
 constexpr int kMaxPartials = 1024;  // CTAs of the backward with dw (its fixed-order partial rows)
 constexpr float kE4m3Max = 448.f;
+constexpr float kLeastTop = kE4m3Max * 1.17549435e-38f;  // of a group: its scale is the smallest normal number
 
 // Resident CTAs of an SM, which the register limits are set for. The backward holds more of a row: 80 registers a thread at
 // one chunk (three CTAs of 256; at four its sums spill and it takes 160 us instead of 111 us for 32,771 rows of 2,048, bf16),
@@ -258,6 +259,14 @@ __device__ __forceinline__ float team_sum(float v, int tpr, const Parts& p, floa
 // 1 / sqrt(mean + eps): the approximate reciprocal root is within 2 units in the last place
 __device__ __forceinline__ float inv_rms(float ss, float inv_D, float eps) { return rsqrtf(fmaf(ss, inv_D, eps)); }
 
+// The scale of a group whose largest |y| is `top`, and 1 / scale to 2 units in the last place (any number where all are
+// zero). Below kLeastTop the scale stays 2^-126: a smaller one would have lost bits (or be 0), and its reciprocal would
+// overflow. The eighths keep the divisor inside __fdividef's range, up to 2^126.
+__device__ __forceinline__ float group_scale(float top) { return top > 0.f ? fmaxf(top, kLeastTop) / kE4m3Max : 1.f; }
+__device__ __forceinline__ float group_factor(float top) {
+  return __fdividef(0.125f * kE4m3Max, 0.125f * fmaxf(top, kLeastTop));
+}
+
 // ---- forward, plain (FP8 = 0) or with the 8-bit output. Persistent CTAs: a team walks the rows, with the next row's
 // loads in flight while this one is reduced and written, and keeps its columns' weights in registers.
 //
@@ -365,9 +374,9 @@ __global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false)) rnorm_fwd
         if (!live || col[j] < 0) continue;
         const int g = col[j] / G;
         if constexpr (FP8 == 2) top[j] = __uint_as_float(tops[team * groups + g]);
-        const float sc = top[j] > 0.f ? __fdividef(kE4m3Max, top[j]) : 1.f;  // 1 / scale to 2 units in the last place
+        const float sc = group_factor(top[j]);
         if (FP8 == 1 ? (sub & (lanes - 1)) == 0 : col[j] == g * G)
-          scale[r0 * groups + g] = top[j] > 0.f ? top[j] / kE4m3Max : 1.f;
+          scale[r0 * groups + g] = group_scale(top[j]);
         uint32_t packed[E / 4];
 #pragma unroll
         for (int i = 0; i < E / 4; ++i) {
@@ -476,8 +485,7 @@ __global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false)) rnorm_fwd
         uint32_t packed[E / 4];
         const float t1 = __uint_as_float(tops[team * groups + g0]);
         const float t2 = g0 + 1 < groups ? __uint_as_float(tops[team * groups + g0 + 1]) : 0.f;
-        // 1 / scale: the product is within 2 units in the last place of y / scale
-        const float sc = t1 > 0.f ? kE4m3Max / t1 : 1.f, sc2 = t2 > 0.f ? kE4m3Max / t2 : 1.f;
+        const float sc = group_factor(t1), sc2 = group_factor(t2);
 #pragma unroll
         for (int i = 0; i < E / 4; ++i) {
           float f[4];
@@ -499,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false)) rnorm_fwd
       if (r0 < rows)
         for (int g = sub; g < groups; g += tpr) {
           const float t = __uint_as_float(tops[team * groups + g]);
-          scale[r0 * groups + g] = t > 0.f ? t / kE4m3Max : 1.f;
+          scale[r0 * groups + g] = group_scale(t);
         }
     }
   }

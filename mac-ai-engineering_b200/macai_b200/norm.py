@@ -114,8 +114,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
 def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
                      group: Optional[int] = 128, zero_centered: bool = False):
     """(q, scale, s): q [..., D] float8_e4m3fn and scale [..., ceil(D / group)] float32 with y = q * scale, one scale for
-    each `group` channels (a multiple of 8; None: for the whole row), scale = max |y| / 448 over them, or 1 where y is
-    all zero; s as add_rms_norm's. No gradient."""
+    each `group` channels (a multiple of 8; None: for the whole row), scale = max |y| / 448 over them, at least the
+    smallest normal number 2^-126, or 1 where y is all zero; s as add_rms_norm's. No gradient."""
     if not supported(x, residual, weight):
         raise ValueError("add_rms_norm_fp8: " + _REFUSED)
     if group is not None and (group <= 0 or group % 8):
