@@ -298,8 +298,8 @@ int gd_rotary(const void* q, const void* k, void* oq, void* ok, const float* tab
  * when j <= p and (j > p - window or j < sinks); window 0: no window. o = softmax(scale q k^T) v over the visible keys,
  * zeros for a query that sees none; scale: any finite number. q [B, Tq, H, D], k, v [B, Tk, HK, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), H a
  * multiple of HK (each key head serves H / HK consecutive query heads), D a multiple of 8 up to 256, read through
- * `strides` (host array, elements: batch, token and head stride of q, k, v, and for the backward of d_o; multiples of 8,
- * channels adjacent); o, dq [B, Tq, H, D] and dk, dv [B, Tk, HK, D] contiguous; every pointer 16-byte aligned. lse
+ * `strides` (host array, elements: batch, token and head stride of q, k, v, and for the backward of d_o; positive multiples of
+ * 8, channels adjacent); o, dq [B, Tq, H, D] and dk, dv [B, Tk, HK, D] contiguous; every pointer 16-byte aligned. lse
  * [B, H, Tq] fp32: log2 of the sum of the exponentials, for the backward. cu_seqlens (device int32 [N + 1], or NULL):
  * packed rows, B = 1 and Tq = Tk, each sequence on its own; rows before the first and behind the last
  * (padding) give zeros, in o and in the gradients. Boundaries are clamped into [0, Tq]; one below an earlier one counts as that
@@ -329,7 +329,7 @@ int gd_wattn_bwd(const void* q, const void* k, const void* v, const void* o, con
 
 /* The single-token form over a cache: request b's new token stands at position p = lengths[b] (device int32; negative:
  * idle, zeros, nothing stored). Stores its key and value rows k, v [B, HK, D] in their slot of k_cache, v_cache
- * [B, S, HK, D] (strides: host array, elements, batch, slot and head stride of both) and writes o [B, H, D] = the
+ * [B, S, HK, D] (strides: host array, elements, batch, slot and head stride of both; no two rows share memory) and writes o [B, H, D] = the
  * attention of q [B, H, D] over the visible positions, the new one included. Position j stands in slot j while j < S, then
  * in slot sinks + (j - sinks) mod (S - sinks), so the cache may roll; once p >= S the last S - sinks positions at most are
  * visible besides the first tokens. The workspace (gd_wattn_step_workspace_bytes(), 0 for most sizes) need not be

@@ -11,9 +11,9 @@ using gd::wattn::Problem;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// strides: every (batch, token, head) stride a multiple of 8 elements (TMA's 16 bytes) where the dimension has one
+// strides: every (batch, token, head) stride a positive multiple of 8 elements (TMA's 16 bytes) where the dimension has one
 bool strides_ok(const long long* s, int B, int T, int heads) {
-  auto ok = [](long long x, int n) { return n <= 1 || (x >= 0 && x % 8 == 0 && x < (1ll << 38)); };
+  auto ok = [](long long x, int n) { return n <= 1 || (x > 0 && x % 8 == 0 && x < (1ll << 38)); };
   return ok(s[0], B) && ok(s[1], T) && ok(s[2], heads);
 }
 

@@ -454,6 +454,25 @@ bool sizes_ok(int B, int S, int H, int HK, int D, int window, int sinks) {
   return B >= 0 && B <= 65535 && S > 0 && H > 0 && HK > 0 && H % HK == 0 && H <= 65535 && D > 0 && D % 8 == 0 && D <= 256 &&
          window >= 0 && sinks >= 0;
 }
+// Whether no two rows of D elements of a cache [B, S, HK] share memory: each stride passes what the smaller ones span (the
+// kernel's CTAs write rows of their own at the same time).
+bool rows_apart(const long long* st, int B, int S, int HK, int D) {
+  long long x[3] = {st[0], st[1], st[2]}, n[3] = {B, S, HK};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (x[j] > x[j + 1]) {
+        const long long a = x[j], b = n[j];
+        x[j] = x[j + 1], n[j] = n[j + 1];
+        x[j + 1] = a, n[j + 1] = b;
+      }
+  long long span = D;
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] <= 1) continue;
+    if (x[i] < span || x[i] >= (1ll << 40)) return false;
+    span += (n[i] - 1) * x[i];
+  }
+  return true;
+}
 int groups_of(int H, int HK) { return (H / HK + kRows - 1) / kRows; }
 
 }  // namespace
@@ -480,11 +499,9 @@ extern "C" int gd_wattn_step(const void* q, const void* k, const void* v, void* 
                   reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(workspace);
   for (int i = 0; i < 6; ++i) {
     const int n = i % 3 == 0 ? B : i % 3 == 1 ? S : HK;
-    if (n > 1) {
-      if (strides[i] < 0) return GD_ERR_ALIGN;
-      all |= (uintptr_t)strides[i] * 2;
-    }
+    if (n > 1) all |= (uintptr_t)strides[i] * 2;
   }
+  if (!rows_apart(strides, B, S, HK, D) || !rows_apart(strides + 3, B, S, HK, D)) return GD_ERR_ALIGN;
   if ((all & 15) != 0 || (reinterpret_cast<uintptr_t>(lengths) & 3) != 0) return GD_ERR_ALIGN;
   const int groups = groups_of(H, HK);
   const Split s = split_of(B, S, HK, groups, window, sinks);

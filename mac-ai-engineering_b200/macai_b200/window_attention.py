@@ -39,15 +39,16 @@ def _step_bytes(*sizes) -> int:
 
 
 def _readable(t: torch.Tensor) -> bool:
-    """Whether the kernels can read t [B, T, heads, D] in place: adjacent channels, 16-byte aligned rows."""
+    """Whether the kernels can read t [B, T, heads, D] in place: adjacent channels, 16-byte aligned rows of their own (an
+    expanded dimension has the stride 0, which the tensor maps are not documented to take)."""
     if t.data_ptr() % 16:
         return False
     if t.is_contiguous():
         return True
     b, s, h, d = t.stride()
     B, T, H, _ = t.shape
-    return (d == 1 and (B <= 1 or (b >= 0 and b % 8 == 0)) and (T <= 1 or (s >= 0 and s % 8 == 0))
-            and (H <= 1 or (h >= 0 and h % 8 == 0)))
+    return (d == 1 and (B <= 1 or (b > 0 and b % 8 == 0)) and (T <= 1 or (s > 0 and s % 8 == 0))
+            and (H <= 1 or (h > 0 and h % 8 == 0)))
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -154,8 +155,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     number, default D^-0.5. cu_seqlens: int [N + 1], the boundaries of N sequences packed along the tokens of one batch
     row, each on its own (positions count from its first token, also for `sinks`). A list on the host must rise from 0 to
     T; one on the device is not looked at by the host: rows before its first and behind its last boundary give zeros, in o
-    and in the gradients, and a boundary below an earlier one counts as that one. Inputs may be strided views; gradients are
-    the same bits every run."""
+    and in the gradients, and a boundary below an earlier one counts as that one. Inputs may be strided views
+    (expanded ones are copied); gradients are the same bits every run."""
     _check_qkv("window_attention", q, k, v)
     w, s = _check_mask("window_attention", window, sinks)
     cu = _check_cu(cu_seqlens, q, k)
@@ -171,9 +172,9 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
                           scale: Optional[float] = None) -> torch.Tensor:
     """One new token for each request: stores its key and value in the caches (in place) and returns its attention
     o [B, 1, H, D] over the visible positions, its own included. q [B, 1, H, D], k, v [B, 1, H_k, D], k_cache, v_cache
-    [B, S, H_k, D] (any strides with adjacent channels and 16-byte aligned rows), lengths int32 [B] on the device: the
-    tokens in each request's cache before the call, which is the new token's position. The caller adds 1 to lengths after
-    its last layer. A negative length marks an idle request: zeros, nothing stored.
+    [B, S, H_k, D] (any strides with adjacent channels and 16-byte aligned rows that share no memory), lengths int32 [B] on
+    the device: the tokens in each request's cache before the call, which is the new token's position. The caller adds 1 to
+    lengths after its last layer. A negative length marks an idle request: zeros, nothing stored.
 
     Position j stands in slot j while j < S, then in slot sinks + (j - sinks) mod (S - sinks): with S >= sinks + window the
     cache rolls, keeping its first `sinks` tokens, and requests may grow without limit; a smaller cache then shows the last
@@ -192,8 +193,8 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
             raise ValueError(f"window_attention_step: {name} must be [B, S, H_k, D] with k's batch, heads, width, dtype and "
                              "device")
         if not _readable(c):
-            raise ValueError(f"window_attention_step: {name} needs adjacent channels and 16-byte aligned rows (it is "
-                             "written in place)")
+            raise ValueError(f"window_attention_step: {name} needs adjacent channels and 16-byte aligned rows, each "
+                             "with memory of its own (it is written in place)")
     if (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or lengths.shape != (B,)
             or lengths.get_device() != index or not lengths.is_contiguous()):
         raise ValueError("window_attention_step: lengths must be a contiguous int32 [B] on q's device")
