@@ -18,6 +18,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._call import aligned, first_order, launch, like, recorded
@@ -207,4 +208,5 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     launch("gd_wattn_step", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
            lengths.data_ptr(), o.data_ptr(), _DTYPES[q.dtype], B, S, H, HK, D, _strides(k_cache, v_cache), w, s,
            float(D ** -0.5 if scale is None else scale), None if ws is None else ws.data_ptr(), n)
+    increment_version((k_cache, v_cache))  # written through their pointers: autograd sees that saved ones have changed
     return o
