@@ -125,7 +125,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, posi
     """(q, k) with their first 2 * table.shape[1] channels turned. q [B, T, H, D], k [B, T, H_k, D] (or None) in one
     float dtype, with any strides as long as a head's channels are adjacent (views of a fused projection are read in
     place); table [P, R / 2, 2] from rotary_table; positions int32 or int64 [T] or [B, T] on the device (None: 0 .. T-1).
-    A position outside the table is taken as its nearest row."""
+    A position outside the table is taken as its nearest row. The gradients are q's and k's; the table has none."""
     if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.dtype not in _DTYPES:
         raise ValueError("rotary: q must be [B, T, heads, D] in float32, float16 or bfloat16")
     if not q.is_cuda:
@@ -149,6 +149,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, posi
         positions = positions.contiguous()
     elif P < shape[1]:
         raise ValueError(f"rotary: the table has {P} positions, the call {shape[1]} tokens")
+    if recorded(table):
+        raise RuntimeError("rotary: the table has no gradient: pass table.detach()")
     if recorded(q, k):
         out = Rotary.apply(q, k, table, positions, bool(interleaved))
         return (out, None) if k is None else out
