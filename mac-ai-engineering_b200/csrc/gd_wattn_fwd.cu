@@ -9,7 +9,8 @@
 //   the A operand of P V (no trip through shared memory). P is rounded to the inputs' 16-bit type (the operand type of the
 //   matrix instruction); its sum is taken before the rounding, in fp32.
 //   The maximum that P refers to moves only when a row outgrows it by 2^8: O is rescaled in TMEM then (rarely), and P
-//   stays below 2^8, far inside both 16-bit types.
+//   stays below 2^8. float16's P carries 2^7 more, up to the end of its range: it keeps its 11 bits down to 2^-21 of the
+//   maximum's weight and is off by 2^-32 of it at most (many keys of 2^-25 beside one that outweighs them were lost together).
 // D <= 128: two CTAs share an SM (<= 100 KB of shared memory, 256 TMEM columns each). While the softmax works on one half,
 // the other half's P V and its next S run, so the softmax warps hardly wait: the exponentials (16 a clock and SM) and the
 // products share the SM's time. S of 64 keys at a time costs the product 1.5 times its shared-memory reads of Q; S of 128
@@ -27,6 +28,8 @@ namespace {
 constexpr int kWarpsSm = 4;
 constexpr int kThreads = 32 * (kWarpsSm + 2);   // + loads, + products
 constexpr float kMaxGrowth = 8.f;               // log2
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;  // log2 of what P carries
 
 template <int NS>
 struct Cfg {
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
         }
         m = next;
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = m == -INFINITY ? 0.f : m - kLift<T>;
       const F2 rf = f2(-ref, -ref);
       F2 acc = f2(0.f, 0.f);
 #pragma unroll
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     const int i = i0 + row;
     const bool none = l == 0.f && ok;                 // a row without a visible key: zeros, whatever O's columns hold
     const float inv = !ok ? NAN : none ? 0.f : 1.f / l;  // a wait that gave up leaves NaN
-    if (i < sq.Tq && lse != nullptr) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m + log2f(l);
+    if (i < sq.Tq && lse != nullptr) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m - kLift<T> + log2f(l);
     // out through shared memory (Q's place and the first key unit's; a warp's own 32 rows), so that rows leave as whole lines
     // (16-byte stores a thread and row took 5 us a CTA); o_low: what the rounding took away, for the backward's delta
     const bool low = o_low != nullptr;
