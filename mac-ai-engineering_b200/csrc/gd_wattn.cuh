@@ -22,7 +22,7 @@ struct Problem {
   int D;
   int window, sinks;       // key j is visible to position p: j <= p and (j > p - window or j < sinks)
   // scale, and scale * log2(e). The forward, whose mask and maximum come before its scale, takes a positive scale_log2 and
-  // the scale's sign apart.
+  // the scale's sign apart (Q takes it).
   float scale, scale_log2;
   bool negate;
   const int* cu;           // packed rows' boundaries [N + 1], or NULL
@@ -399,6 +399,23 @@ template <int NS>
 __device__ __forceinline__ void zero_rows(uint32_t smem, int from) {
   if (from >= kTile) return;
   zero_rows<NS>(smem, from, kTile, threadIdx.x & 31, 32);
+  __syncwarp();
+}
+// A tile of 16-bit values that has landed, NS slabs, times -1; by the warp that issues the products that read it.
+template <int NS>
+__device__ __forceinline__ void negate_tile(uint32_t smem) {
+#pragma unroll 1
+  for (int a = (threadIdx.x & 31) * 16; a < NS * kSlabBytes; a += 32 * 16) {
+    uint32_t u[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+                 : "r"(smem + a)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] ^= 0x80008000u;
+    st_shared16(smem + a, u);
+  }
+  fence_async_smem();
   __syncwarp();
 }
 // Rows row0 .. row0 + 31 of a swizzled tile in shared memory -> tokens t0 + row of head h, row b of a [B, T, heads, D] array,

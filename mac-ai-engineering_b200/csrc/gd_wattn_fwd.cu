@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     if (kr.n > 0) {
       const uint32_t lead = elect();
       bool ok = warp_wait(q_full, 0, err, 62);
+      if (pr.negate) negate_tile<NS>(s_q);  // from here on the scale is positive
       auto landed = [&](int c) { return warp_wait(full + c % C::kSlots, (c / C::kSlots) & 1, err, 63); };
       auto values = [&](int c, int j) {  // the same for a unit of tile j's values
         if (!landed(c)) return false;
@@ -230,10 +231,6 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
       const uint32_t ts = tm + lanes + b * 64;
       float s[64];
       tmem_ld64(ts, s);
-      if (pr.negate) {  // from here on the scale is positive
-#pragma unroll
-        for (int i = 0; i < 64; ++i) s[i] = -s[i];
-      }
       const int c0 = kr.key(j) + 64 * x;
       if (!all_visible(kr.key(j), p0, p1, pr.window, pr.sinks)) {
         const uint32_t v0 = visible_keys(c0, p, pr.window, pr.sinks), v1 = visible_keys(c0 + 32, p, pr.window, pr.sinks);
