@@ -29,6 +29,10 @@ constexpr int kStep = 16;   // keys a warp takes at a time
 constexpr int kRows = 16;   // query heads of a CTA
 constexpr int kMaxClusters = 32;
 constexpr int kSms = 148;   // of a B200
+// log2 of what P carries before its rounding: float16's, at most 1 otherwise, would lose the keys that weigh less than 2^-14
+// of the maximum (all 11 bits now down to 2^-29); the sums carry it too, and o is their quotient
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
 static_assert(kThreads == 8 * kRows, "the join's factors: eight threads a row");
 
 template <int DP>
@@ -274,7 +278,7 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const StepArgs a) {
       m0 = n0;
       m1 = n1;
     }
-    const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+    const float r0 = m0 == -INFINITY ? 0.f : m0 - kLift<T>, r1 = m1 == -INFINITY ? 0.f : m1 - kLift<T>;
     uint32_t pa[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
