@@ -53,6 +53,12 @@ def has_tangent(*ts) -> bool:
     return any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
+def refuse_tangents(name: str, *ts) -> None:
+    """Raises where one of these inputs carries a forward-mode tangent: the custom ops would drop it in silence."""
+    if has_tangent(*ts):
+        raise NotImplementedError(f"{name}: no forward-mode derivative")
+
+
 def recorded(*ts) -> bool:
     """Whether autograd has a part in a call with these inputs (None allowed): a gradient to record, or a tangent, which
     the autograd functions refuse (they have no forward-mode derivative)."""

@@ -20,6 +20,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from ._call import refuse_tangents
 
 K = 4
 _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
@@ -133,6 +134,7 @@ class ConvQKV:
 
     @staticmethod
     def apply(x, weight, kd, dk, rep, dv):
+        refuse_tangents("conv_qkv", x, weight)
         if not supported(x, weight, kd, dk, rep, dv):
             raise ValueError("conv_qkv: x must be a CUDA [B, T, C] tensor with C = 2 kd + vd and the head widths "
                              "dividing it (multiples of 8 channels at 16 bits, 4 at float32); weight C x 4 in x's "

@@ -15,6 +15,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
+from .._call import refuse_tangents
 
 # The chunk length of every kernel (tokens). The drop-in accepts `chunk_size` for signature compatibility and, like the
 # reference (op.py:268-269), runs its own chunking; 64 is also the value every caller passes.
@@ -513,6 +514,7 @@ class GatedDeltaRule:
 
     @staticmethod
     def apply(q, k, v, g, beta, s0, save: bool = True):
+        refuse_tangents("GatedDeltaRule", q, k, v, g, beta, s0)
         dt = q.dtype
         check_dtype(dt)
         k, v = k.to(dt), v.to(dt)
@@ -537,6 +539,7 @@ def chunk_gated_delta_rule(query, key, value, g, beta, chunk_size: int = 64, ini
     64 tokens), as in the reference (op.py:264-269). cu_seqlens (packed rows: batch size 1, N sequences along the
     tokens, initial_state and the final state [N, H, DK, DV]) runs every sequence as its own row, with fla's
     semantics; the reference refuses it (op.py:270-273)."""
+    refuse_tangents("chunk_gated_delta_rule", query, key, value, g, beta, initial_state)
     cu_seqlens = kwargs.get("cu_seqlens")
     dt = query.dtype
     check_dtype(dt)

@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from ._call import refuse_tangents
 
 _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 MAX_D = 1024
@@ -113,6 +114,7 @@ class GatedRMSNorm:
 
     @staticmethod
     def apply(x, z, w, eps):
+        refuse_tangents("gated_rms_norm", x, z, w)
         if not supported(x, z, w):
             raise ValueError("gated_rms_norm: x and z must be CUDA tensors of one float dtype and shape [..., D] with "
                              "D % 4 == 0 and D <= 1024; w [D] in x's dtype or float32")

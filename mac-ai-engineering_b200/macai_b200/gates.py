@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from ._call import refuse_tangents
 
 _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 
@@ -111,6 +112,7 @@ class Gates:
 
     @staticmethod
     def apply(b, a, A_log, dt_bias):
+        refuse_tangents("gates", b, a, A_log, dt_bias)
         if not supported(b, a, A_log, dt_bias):
             raise ValueError("gates: b and a must be CUDA tensors of one float dtype and shape [..., H]; A_log and "
                              "dt_bias [H] of one float dtype")
