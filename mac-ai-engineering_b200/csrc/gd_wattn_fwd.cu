@@ -295,9 +295,11 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     unf2(l2, l, lb);
     l += lb;
     const int i = i0 + row;
-    const bool none = l == 0.f && ok;                 // a row without a visible key: zeros, whatever O's columns hold
+    // A row without a visible key (its own is visible from position 0 on): zeros, whatever O's columns hold. A row whose
+    // visible scores are all -inf has a sum of 0 and comes out as NaN.
+    const bool none = ok && (kr.n == 0 || p < 0);
     const float inv = !ok ? NAN : none ? 0.f : 1.f / l;  // a wait that gave up leaves NaN
-    if (i < sq.Tq && lse != nullptr) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = l == 0.f ? INFINITY : m - kLift<T> + log2f(l);
+    if (i < sq.Tq && lse != nullptr) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = none ? INFINITY : m - kLift<T> + log2f(l);
     // out through shared memory (Q's place and the first key unit's; a warp's own 32 rows), so that rows leave as whole lines
     // (16-byte stores a thread and row took 5 us a CTA); o_low: what the rounding took away, for the backward's delta
     const bool low = o_low != nullptr;

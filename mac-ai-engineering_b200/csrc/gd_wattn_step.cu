@@ -377,9 +377,9 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const StepArgs a) {
       out[2 + c] = y0;
       out[3 + c] = y1;
     } else {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = 1.f / l;  // a sum of 0 over visible keys (scores of -inf) gives NaN; an idle request zeros
       uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + ((long long)b * a.H + hk * G + g0 + row) * a.D + c);
-      *out = l == 0.f ? 0u : pack<T>(y0 * inv, y1 * inv);
+      *out = seen.n == 0 ? 0u : pack<T>(y0 * inv, y1 * inv);
     }
   }
   cluster.sync();  // no CTA ends while another reads its shared memory
@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(256) step_join(const StepArgs a, int clusters)
   const int hk = blockIdx.x / a.groups, g0 = blockIdx.x % a.groups * kRows, b = blockIdx.y;
   const int G = a.H / a.HK, rows = G - g0 < kRows ? G - g0 : kRows;
   const float* part = a.part + ((long long)b * gridDim.x + blockIdx.x) * clusters * kRows * (2 + a.D);
+  const bool idle = __ldg(a.lengths + b) < 0;
   for (int i = threadIdx.x; i < rows * a.D; i += 256) {
     const int row = i / a.D, c = i % a.D;
     float top = -INFINITY, l = 0.f, y = 0.f;
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(256) step_join(const StepArgs a, int clusters)
       l = fmaf(p[1], f, l);
       y = fmaf(p[2 + c], f, y);
     }
-    static_cast<T*>(a.o)[((long long)b * a.H + hk * G + g0 + row) * a.D + c] = to16<T>(l == 0.f ? 0.f : y / l);
+    static_cast<T*>(a.o)[((long long)b * a.H + hk * G + g0 + row) * a.D + c] = to16<T>(idle ? 0.f : y / l);
   }
 }
 
