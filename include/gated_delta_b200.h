@@ -296,20 +296,20 @@ int gd_rotary(const void* q, const void* k, void* oq, void* ok, const float* tab
 /* ---- causal softmax attention with a sliding window and first tokens that stay visible ----
  * The mixer of the layers that alternate with the rule's. Query i of Tq stands at position p = i + Tk - Tq and sees key j
  * when j <= p and (j > p - window or j < sinks); window 0: no window. o = softmax(scale q k^T) v over the visible keys,
- * zeros for a query that sees none; scale: any finite number. q [B, Tq, H, D], k, v [B, Tk, HK, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), H a
- * multiple of HK (each key head serves H / HK consecutive query heads), D a multiple of 8 up to 256, read through
- * `strides` (host array, elements: batch, token and head stride of q, k, v, and for the backward of d_o; positive multiples of
- * 8, channels adjacent); o, dq [B, Tq, H, D] and dk, dv [B, Tk, HK, D] contiguous; every pointer 16-byte aligned. lse
- * [B, H, Tq] fp32: log2 of the sum of the exponentials, for the backward. cu_seqlens (device int32 [N + 1], or NULL):
- * packed rows, B = 1 and Tq = Tk, each sequence on its own; rows before the first and behind the last
- * (padding) give zeros, in o and in the gradients. Boundaries are clamped into [0, Tq]; one below an earlier one counts as that
- * one.
+ * zeros for a query that sees none (NaN for one whose visible scores are all -inf); scale: any finite number.
+ * q [B, Tq, H, D], k, v [B, Tk, HK, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), H a multiple of HK (each key head serves
+ * H / HK consecutive query heads), D a multiple of 8 up to 256, read through `strides` (host array, elements: batch, token
+ * and head stride of q, k, v, and for the backward of d_o; positive multiples of 8, channels adjacent); o, dq [B, Tq, H, D]
+ * and dk, dv [B, Tk, HK, D] contiguous; every pointer 16-byte aligned. lse [B, H, Tq] fp32: log2 of the sum of the
+ * exponentials, for the backward. cu_seqlens (device int32 [N + 1], or NULL): packed rows, B = 1 and Tq = Tk, each sequence
+ * on its own; rows before the first and behind the last (padding) give zeros, in o and in the gradients. Boundaries are
+ * clamped into [0, Tq]; one below an earlier one counts as that one.
  * The workspace starts with an error word (gd_read_error); the forward's is nothing else and may be NULL. A wait that gives
  * up leaves NaN in the rows it was for, word or no word. A finite result row needs finite values in its tile of 128 keys and
  * 128 queries: masked scores are never used, but a masked key's infinity or NaN in v (or in k, q, d_o for the gradients)
  * meets a weight of 0 in the products, as it would in a matrix product of the formula. (A packed sequence's infinities
- * and NaN stay in it; float16's dS has one power-of-two scale for the call, from the largest
- * norms of d_o's and v's rows: it does not overflow, and keeps float16's 11 bits down to 2^-29 of its bound.) */
+ * and NaN stay in it; float16's dS has one power-of-two scale for the call, from the largest norms of d_o's and v's rows: it
+ * does not overflow, and keeps float16's 11 bits down to 2^-29 of its bound.) */
 
 /* Bytes of workspace gd_wattn_fwd (for_backward 0) or gd_wattn_bwd need (0 for invalid sizes); packed: with cu_seqlens. */
 size_t gd_wattn_workspace_bytes(int B, int Tq, int Tk, int H, int HK, int D, int window, int sinks, int packed,
@@ -317,20 +317,20 @@ size_t gd_wattn_workspace_bytes(int B, int Tq, int Tk, int H, int HK, int D, int
 
 /* o_low and lse are for the backward (NULL otherwise). o_low: what o's rounding took away, in `dtype`, with o's shape. */
 int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, const int* cu_seqlens,
-                 int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D, const long long* strides, int window, int sinks, float scale,
-                 void* workspace, size_t workspace_bytes, void* stream);
+                 int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D, const long long* strides, int window,
+                 int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
-/* dq, dk, dv from the forward's inputs, o, o_low and lse, and d_o. dk and dv are summed over the query heads of a key head in a
- * fixed order (no atomics: the same bits every run). */
+/* dq, dk, dv from the forward's inputs, o, o_low and lse, and d_o. dk and dv are summed over the query heads of a key head
+ * in a fixed order (no atomics: the same bits every run). */
 int gd_wattn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse,
-                 const void* d_o, void* dq, void* dk, void* dv, const int* cu_seqlens, int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D,
-                 const long long* strides, int window, int sinks, float scale, void* workspace, size_t workspace_bytes,
-                 void* stream);
+                 const void* d_o, void* dq, void* dk, void* dv, const int* cu_seqlens, int N, int dtype, int B, int Tq,
+                 int Tk, int H, int HK, int D, const long long* strides, int window, int sinks, float scale,
+                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* The single-token form over a cache: request b's new token stands at position p = lengths[b] (device int32; negative:
  * idle, zeros, nothing stored). Stores its key and value rows k, v [B, HK, D] in their slot of k_cache, v_cache
- * [B, S, HK, D] (strides: host array, elements, batch, slot and head stride of both; no two rows share memory) and writes o [B, H, D] = the
- * attention of q [B, H, D] over the visible positions, the new one included. Position j stands in slot j while j < S, then
+ * [B, S, HK, D] (strides: host array, elements, batch, slot and head stride of both; no two rows share memory) and writes
+ * o [B, H, D] = the attention of q [B, H, D] over the visible positions, the new one included. Position j stands in slot j while j < S, then
  * in slot sinks + (j - sinks) mod (S - sinks), so the cache may roll; once p >= S the last S - sinks positions at most are
  * visible besides the first tokens. The workspace (gd_wattn_step_workspace_bytes(), 0 for most sizes) need not be
  * initialised. */

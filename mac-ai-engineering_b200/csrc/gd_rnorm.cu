@@ -9,12 +9,13 @@
 //             from the fp32 y: the only rounding is the one to e4m3
 //
 // Bound by HBM, the backward and the 8-bit form nearly as much by issue slots: the forward moves 4 elements per channel
-// (x, res in; s, y out), the backward 4 (s, dy, ds in; dx out), the 8-bit form 3 and a byte. So a row is read once: a team of TPR threads holds it in registers as 16-byte chunks.
+// (x, res in; s, y out), the backward 4 (s, dy, ds in; dx out), the 8-bit form 3 and a byte. So a row is read once: a team
+// of TPR threads holds it in registers as 16-byte chunks.
 // Chunks are those of the flat [rows * D] array, which start on 16-byte boundaries whatever D is; where D is not a
 // multiple of the chunk a row's first and last chunk are shared with its neighbours: their foreign
 // elements are read with them, count as zero, and are not written. So odd widths run on 16-byte loads too.
 // Measured (bf16): 32,771 rows of 2,048 forward 83.6 us (6.4 TB/s), backward with dw 102.3 + 3.5 us (5.2 TB/s); 16,384
-// rows of 4,096 to e4m3 in groups of 128 91.9 us (5.1 TB/s). A plain copy runs at 6.5 TB/s.
+// rows of 4,096 to e4m3 in groups of 128 90.5 us (5.2 TB/s). A plain copy runs at 6.5 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -277,11 +278,12 @@ __device__ __forceinline__ float group_factor(float top) {
 //
 // The widths that are whole chunks (the others below):
 template <typename T, int NV, int FP8, int THREADS>
-__global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false)) rnorm_fwd_flat(const T* __restrict__ x, const T* __restrict__ res,
-                                                          const void* __restrict__ w, T* __restrict__ s, T* __restrict__ y,
-                                                          uint8_t* __restrict__ q, float* __restrict__ scale, int wdtype,
-                                                          float bias, long long rows, int D, int G, int lanes, int tpr,
-                                                          float eps) {
+__global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false))
+    rnorm_fwd_flat(const T* __restrict__ x, const T* __restrict__ res,
+                   const void* __restrict__ w, T* __restrict__ s, T* __restrict__ y,
+                   uint8_t* __restrict__ q, float* __restrict__ scale, int wdtype,
+                   float bias, long long rows, int D, int G, int lanes, int tpr,
+                   float eps) {
   constexpr int E = Vec<T>::E, H = E / 2;
   __shared__ __align__(16) float red[2][32];
   const Parts parts(tpr);
@@ -396,10 +398,11 @@ __global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false)) rnorm_fwd
 
 // Widths that are no whole number of chunks (FP8 = 0 or 2): the same walk, a row's chunks cut out of the flat array.
 template <typename T, int NV, int FP8, int THREADS>
-__global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false)) rnorm_fwd_odd(const T* __restrict__ x, const T* __restrict__ res,
-                                                     const void* __restrict__ w, T* __restrict__ s, T* __restrict__ y,
-                                                     uint8_t* __restrict__ q, float* __restrict__ scale, int wdtype,
-                                                     float bias, long long rows, int D, int G, int tpr, float eps) {
+__global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false))
+    rnorm_fwd_odd(const T* __restrict__ x, const T* __restrict__ res,
+                  const void* __restrict__ w, T* __restrict__ s, T* __restrict__ y,
+                  uint8_t* __restrict__ q, float* __restrict__ scale, int wdtype,
+                  float bias, long long rows, int D, int G, int tpr, float eps) {
   constexpr int E = Vec<T>::E;
   __shared__ __align__(16) float red[2][32];
   const Parts parts(tpr);
@@ -518,10 +521,11 @@ __global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, false)) rnorm_fwd
 // its own over the rows) and the CTA's teams are added in team order; else the columns move with the row, so the sums stand
 // in shared memory, where one thread adds to an element at a time, in the rows' order (one team a CTA).
 template <typename T, int NV, bool DW, int THREADS>
-__global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, true)) rnorm_bwd_flat(const T* __restrict__ s, const void* __restrict__ w,
-                                                          const T* __restrict__ dy, const T* __restrict__ ds,
-                                                          T* __restrict__ dx, float* __restrict__ part, int wdtype,
-                                                          float bias, long long rows, int D, int tpr, float eps) {
+__global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, true))
+    rnorm_bwd_flat(const T* __restrict__ s, const void* __restrict__ w,
+                   const T* __restrict__ dy, const T* __restrict__ ds,
+                   T* __restrict__ dx, float* __restrict__ part, int wdtype,
+                   float bias, long long rows, int D, int tpr, float eps) {
   constexpr int E = Vec<T>::E, H = E / 2;
   __shared__ __align__(16) float red[2][2][32];
   const Parts parts(tpr);
@@ -628,10 +632,11 @@ __global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, true)) rnorm_bwd_
 
 // Widths that are no whole number of chunks, or more than 1,024 of them.
 template <typename T, int NV, bool DW, int THREADS>
-__global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, true)) rnorm_bwd_odd(const T* __restrict__ s, const void* __restrict__ w,
-                                                     const T* __restrict__ dy, const T* __restrict__ ds,
-                                                     T* __restrict__ dx, float* __restrict__ part, int wdtype, float bias,
-                                                     long long rows, int D, int tpr, float eps) {
+__global__ void __launch_bounds__(THREADS, per_sm(THREADS, NV, true))
+    rnorm_bwd_odd(const T* __restrict__ s, const void* __restrict__ w,
+                  const T* __restrict__ dy, const T* __restrict__ ds,
+                  T* __restrict__ dx, float* __restrict__ part, int wdtype, float bias,
+                  long long rows, int D, int tpr, float eps) {
   constexpr int E = Vec<T>::E;
   __shared__ __align__(16) float red[2][2][32];
   const Parts parts(tpr);

@@ -169,7 +169,8 @@ extern "C" int gd_rotary(const void* q, const void* k, void* oq, void* ok, const
                          long long k_stride_b, long long k_stride_t, long long k_stride_h, int interleaved, int inverse,
                          void* stream) {
   if (dtype != GD_FLOAT32 && dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) return GD_ERR_ARG;
-  if (B < 0 || B > 65535 || T < 0 || H < 0 || HK < 0 || D <= 0 || R <= 0 || R % 2 != 0 || R > D || table_rows < 0) return GD_ERR_SHAPE;
+  if (B < 0 || B > 65535 || T < 0 || H < 0 || HK < 0 || D <= 0 || R <= 0 || R % 2 != 0 || R > D || table_rows < 0)
+    return GD_ERR_SHAPE;
   if ((long long)B * T == 0 || H + HK == 0) return GD_OK;
   if (table_rows == 0 || (long long)(H + HK) * D > 0x3fffffff) return GD_ERR_SHAPE;
   if (table == nullptr || (H > 0 && (q == nullptr || oq == nullptr)) || (HK > 0 && (k == nullptr || ok == nullptr)))

@@ -28,7 +28,8 @@ int check(const void* q, const void* k, const void* v, const long long* strides,
           int Tq, int Tk, int H, int HK, int D, int window, int sinks, float scale) {
   if (dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) return GD_ERR_ARG;
   if (B < 0 || Tq < 0 || Tk < 0 || B > 65535 || Tq > (1 << 29) || Tk > (1 << 29) || H <= 0 || HK <= 0 || H > 65535 ||
-      H % HK != 0 || (long long)Tq * H >= (1ll << 31) || D <= 0 || D % 8 != 0 || D > 256 || window < 0 || sinks < 0 || !std::isfinite(scale))
+      H % HK != 0 || (long long)Tq * H >= (1ll << 31) || D <= 0 || D % 8 != 0 || D > 256 || window < 0 || sinks < 0 ||
+      !std::isfinite(scale))
     return GD_ERR_SHAPE;
   if (cu != nullptr && (B != 1 || Tq != Tk || N <= 0 || N > (1 << 24))) return GD_ERR_SHAPE;
   if (B == 0 || Tq == 0) return GD_OK;
@@ -106,8 +107,9 @@ extern "C" size_t gd_wattn_workspace_bytes(int B, int Tq, int Tk, int H, int HK,
 }
 
 extern "C" int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse,
-                            const int* cu_seqlens, int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D, const long long* strides,
-                            int window, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+                            const int* cu_seqlens, int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D,
+                            const long long* strides, int window, int sinks, float scale, void* workspace,
+                            size_t workspace_bytes, void* stream) {
   if (const int st = check(q, k, v, strides, cu_seqlens, N, dtype, B, Tq, Tk, H, HK, D, window, sinks, scale)) return st;
   if (B == 0 || Tq == 0) return GD_OK;
   if (o == nullptr || (lse == nullptr && o_low != nullptr)) return GD_ERR_ARG;
@@ -125,7 +127,8 @@ extern "C" int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o
     const size_t n = (size_t)B * Tq * H * D * 2;
     if (cudaMemsetAsync(o, 0, n, cs) != cudaSuccess ||
         (o_low != nullptr && cudaMemsetAsync(o_low, 0, n, cs) != cudaSuccess) ||
-        (lse != nullptr && cudaMemsetAsync(lse, 0x7f, (size_t)B * H * Tq * sizeof(float), cs) != cudaSuccess))  // 3.4e38: as good as +inf
+        // 3.4e38: as good as +inf
+        (lse != nullptr && cudaMemsetAsync(lse, 0x7f, (size_t)B * H * Tq * sizeof(float), cs) != cudaSuccess))
       return (cudaGetLastError(), GD_ERR_LAUNCH);
     return GD_OK;
   }
@@ -133,21 +136,25 @@ extern "C" int gd_wattn_fwd(const void* q, const void* k, const void* v, void* o
 }
 
 extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low,
-                            const float* lse, const void* d_o, void* dq, void* dk, void* dv, const int* cu_seqlens, int N, int dtype, int B, int Tq, int Tk,
-                            int H, int HK, int D, const long long* strides, int window, int sinks, float scale,
-                            void* workspace, size_t workspace_bytes, void* stream) {
+                            const float* lse, const void* d_o, void* dq, void* dk, void* dv, const int* cu_seqlens,
+                            int N, int dtype, int B, int Tq, int Tk, int H, int HK, int D, const long long* strides,
+                            int window, int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int st = check(q, k, v, strides, cu_seqlens, N, dtype, B, Tq, Tk, H, HK, D, window, sinks, scale)) return st;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   if (B == 0 || Tq == 0 || Tk == 0) {  // no pair: zero gradients
     const size_t nq = (size_t)B * Tq * H * D * 2, nk = (size_t)B * Tk * HK * D * 2;
     if ((nq > 0 && dq == nullptr) || (nk > 0 && (dk == nullptr || dv == nullptr))) return GD_ERR_ARG;
-    if ((nq > 0 && cudaMemsetAsync(dq, 0, nq, cs) != cudaSuccess) || (nk > 0 && cudaMemsetAsync(dk, 0, nk, cs) != cudaSuccess) ||
+    if ((nq > 0 && cudaMemsetAsync(dq, 0, nq, cs) != cudaSuccess) ||
+        (nk > 0 && cudaMemsetAsync(dk, 0, nk, cs) != cudaSuccess) ||
         (nk > 0 && cudaMemsetAsync(dv, 0, nk, cs) != cudaSuccess))
       return (cudaGetLastError(), GD_ERR_LAUNCH);
     return GD_OK;
   }
-  if (o == nullptr || o_low == nullptr || lse == nullptr || d_o == nullptr || dq == nullptr || dk == nullptr || dv == nullptr) return GD_ERR_ARG;
-  if (!aligned16(o) || !aligned16(o_low) || !aligned16(d_o) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(workspace))
+  if (o == nullptr || o_low == nullptr || lse == nullptr || d_o == nullptr || dq == nullptr || dk == nullptr ||
+      dv == nullptr)
+    return GD_ERR_ARG;
+  if (!aligned16(o) || !aligned16(o_low) || !aligned16(d_o) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
+      !aligned16(workspace))
     return GD_ERR_ALIGN;
   if (!strides_ok(strides + 9, B, Tq, H)) return GD_ERR_ALIGN;
   if (workspace == nullptr ||
@@ -158,9 +165,11 @@ extern "C" int gd_wattn_bwd(const void* q, const void* k, const void* v, const v
   if (dtype == GD_FLOAT16 && cudaMemsetAsync(workspace, 0, sizeof(ErrorWord), cs) != cudaSuccess)
     return (cudaGetLastError(), GD_ERR_LAUNCH);
   const Problem p = problem(cu_seqlens, N, B, Tq, Tk, H, HK, D, window, sinks, scale);
+  // packed rows are not cut: where their sequences end, and so which tiles are heavy, is known on the device only
   const Cut c = cu_seqlens != nullptr ? Cut{0, 1} : cut_of(B, Tq, Tk, H, HK, D, p.window, p.sinks);
   char* ws = static_cast<char*>(workspace);
-  return gd::wattn::backward(q, k, v, o, o_low, d_o, strides, p, dtype, lse, reinterpret_cast<float*>(ws + delta_at()), dq, dk, dv,
-                             c.heavy, c.parts, reinterpret_cast<float*>(ws + delta_at() + delta_bytes(B, Tq, H)),
+  return gd::wattn::backward(q, k, v, o, o_low, d_o, strides, p, dtype, lse, reinterpret_cast<float*>(ws + delta_at()),
+                             dq, dk, dv, c.heavy, c.parts,
+                             reinterpret_cast<float*>(ws + delta_at() + delta_bytes(B, Tq, H)),
                              static_cast<ErrorWord*>(workspace), cs);
 }

@@ -419,11 +419,12 @@ __device__ __forceinline__ void negate_tile(uint32_t smem) {
   __syncwarp();
 }
 // Rows row0 .. row0 + 31 of a swizzled tile in shared memory -> tokens t0 + row of head h, row b of a [B, T, heads, D] array,
-// rows below `live` only, NS slabs from channel ch on; one whole warp, whose own rows these are (or after a barrier). By TMA (one lane issues it and
-// waits until shared memory is read; the array's end cuts it off) unless rows past `live` belong to someone else.
+// rows below `live` only, NS slabs from channel ch on; one whole warp, whose own rows these are (or after a barrier). By
+// TMA (one lane issues it and waits until shared memory is read; the array's end cuts it off) unless rows past `live` belong
+// to someone else.
 template <typename T, int NS>
-__device__ __forceinline__ void store_rows(const CUtensorMap* m, T* out, uint32_t smem, int row0, int b, int t0, int live, int T_,
-                                           int h, int heads, int D, int ch = 0) {
+__device__ __forceinline__ void store_rows(const CUtensorMap* m, T* out, uint32_t smem, int row0, int b, int t0, int live,
+                                           int T_, int h, int heads, int D, int ch = 0) {
   if (row0 >= live) return;
   if (live - row0 >= 32 || t0 + live == T_) {
     fence_async_smem();
@@ -460,8 +461,8 @@ __device__ __forceinline__ void store_rows(const CUtensorMap* m, T* out, uint32_
 int forward(const void* q, const void* k, const void* v, const long long* strides, const Problem& pr, int dtype, void* o,
             void* low, float* lse, ErrorWord* err, cudaStream_t stream);
 // (and of dO: strides[9 .. 11]); the first `heavy` key tiles are cut into `parts` CTAs with fp32 partial tiles at `part`
-int backward(const void* q, const void* k, const void* v, const void* o, const void* low, const void* g, const long long* strides,
-             const Problem& pr, int dtype, const float* lse, float* delta, void* dq, void* dk, void* dv, int heavy,
+int backward(const void* q, const void* k, const void* v, const void* o, const void* low, const void* g,
+             const long long* strides, const Problem& pr, int dtype, const float* lse, float* delta, void* dq, void* dk, void* dv, int heavy,
              int parts, float* part, ErrorWord* err, cudaStream_t stream);
 
 }  // namespace wattn

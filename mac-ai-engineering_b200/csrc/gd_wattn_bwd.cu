@@ -2,8 +2,8 @@
 // L the forward's log2-sum and delta = rowsum(dO O):
 //   P = exp2(scale log2(e) S - L),  dP = dO V^T,  dS = P (dP - delta)
 //   dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q       (dK, dV summed over the query heads of a key head)
-// Bound by the chain product, elementwise work, product within a tile (tensor pipe 60 % busy). Measured at 1 x 8192 x 16 heads (4 key heads), D 128, window 2048,
-// bf16: delta 21 us (4.7 TB/s), dq 171 us, dk dv 300 us (1,060 and 810 TFLOP/s of 6 and 8 D operations a visible pair); at
+// Bound by the chain product, elementwise work, product within a tile (tensor pipe 60 % busy). Measured at 1 x 8192 x 16
+// heads (4 key heads), D 128, window 2048, bf16: delta 21 us (4.7 TB/s), dq 171 us, dk dv 300 us (1,060 and 810 TFLOP/s of 6 and 8 D operations a visible pair); at
 // 2 x 2048 x 8 (2), D 256, causal: 10, 73 and 145 us.
 // Three kernels, none of which waits on another CTA and none with atomics on results (the same bits every run):
 //   delta_kernel  delta, and for float16 the largest ||dO|| and ||v|| (the scale below)
@@ -199,7 +199,8 @@ template <typename T, int NS>
 __global__ void __launch_bounds__(kThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
               const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo,
-              const __grid_constant__ CUtensorMap mdq, const Problem pr, const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dq, ErrorWord* err) {
+              const __grid_constant__ CUtensorMap mdq, const Problem pr, const float* __restrict__ lse,
+              const float* __restrict__ delta, T* __restrict__ dq, ErrorWord* err) {
   using C = DqCfg<NS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -506,12 +507,14 @@ template <typename T, int NS>
 __global__ void __launch_bounds__(kThreads + 32, 1)
     dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo,
-               const __grid_constant__ CUtensorMap mdk, const __grid_constant__ CUtensorMap mdv, const Problem pr, const Split sp, const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
+               const __grid_constant__ CUtensorMap mdk, const __grid_constant__ CUtensorMap mdv, const Problem pr,
+               const Split sp, const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
                T* __restrict__ dv, ErrorWord* err) {
   using C = DkvCfg<NS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* stats = reinterpret_cast<float*>(base + 2 * NS * kSlabBytes + C::kUnit * (C::kQs + C::kOs));  // [kStats][L, delta][128]
+  // [kStats][L, delta][128]
+  float* stats = reinterpret_cast<float*>(base + 2 * NS * kSlabBytes + C::kUnit * (C::kQs + C::kOs));
   uint64_t* bars = reinterpret_cast<uint64_t*>(stats + C::kStats * 2 * kTile);
   uint64_t* in_full = bars;   // K and V
   uint64_t* full = bars + 1;  // Q ring, then dO ring
@@ -609,7 +612,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
                  s_o = s_q + C::kQs * C::kUnit;
 
   if (warp == kWarpsEw + 2) {
-    // -L (float16: + 15, P's scale) and -delta of each iteration's queries, a step ahead of the elementwise warps; dead queries get -inf and 0
+    // -L (float16: + 15, P's scale) and -delta of each iteration's queries, a step ahead of the elementwise warps; dead
+    // queries get -inf and 0
     const long long at = (long long)sq.b * pr.H * pr.Tq + sq.q0;
     int h = hk * G + (n > 0 ? it0 / nq : 0), qt = lo + (n > 0 ? it0 % nq : 0);
     for (int i = 0; i < n; ++i) {
@@ -618,7 +622,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1)
       for (int x = 0; x < 4; ++x) {
         const int t = qt * kTile + x * 32 + lane;
         const bool live = t < sq.Tq;
-        L[x] = live ? (std::is_same<T, __half>::value ? kPLog2 : 0.f) - __ldg(lse + at + (long long)h * pr.Tq + t) : -INFINITY;
+        constexpr float up = std::is_same<T, __half>::value ? kPLog2 : 0.f;
+        L[x] = live ? up - __ldg(lse + at + (long long)h * pr.Tq + t) : -INFINITY;
         de[x] = live ? -__ldg(delta + at + (long long)h * pr.Tq + t) : 0.f;
       }
       if (++qt == lo + nq) {
@@ -961,7 +966,8 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
   static bool done_q[kMaxDevices], done_kv[kMaxDevices];
   auto kq = dq_kernel<T, NS>;
   auto kkv = dkv_kernel<T, NS>;
-  if (set_smem_once(kq, DqCfg<NS>::kSmem, done_q) != cudaSuccess || set_smem_once(kkv, DkvCfg<NS>::kSmem, done_kv) != cudaSuccess)
+  if (set_smem_once(kq, DqCfg<NS>::kSmem, done_q) != cudaSuccess ||
+      set_smem_once(kkv, DkvCfg<NS>::kSmem, done_kv) != cudaSuccess)
     return (cudaGetLastError(), GD_ERR_LAUNCH);
   const long long qt = pr.cu ? packed_items(pr.Tq, pr.N) : (pr.Tq + kTile - 1) / kTile;
   const long long kt = (pr.cu ? packed_items(pr.Tk, pr.N) : (pr.Tk + kTile - 1) / kTile) + (long long)sp.heavy * (sp.parts - 1);
@@ -977,8 +983,8 @@ int launch(const void* q, const void* k, const void* v, const void* o, const voi
 
 }  // namespace
 
-int backward(const void* q, const void* k, const void* v, const void* o, const void* low, const void* g, const long long* strides,
-             const Problem& pr, int dtype, const float* lse, float* delta, void* dq, void* dk, void* dv, int heavy,
+int backward(const void* q, const void* k, const void* v, const void* o, const void* low, const void* g,
+             const long long* strides, const Problem& pr, int dtype, const float* lse, float* delta, void* dq, void* dk, void* dv, int heavy,
              int parts, float* part, ErrorWord* err, cudaStream_t stream) {
   const Split sp = {heavy, parts, part};
   auto run = [&](auto t, auto ns) {

@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
             tc_fence_after();
             for (int y = 0; y < 2; ++y) {
               const int v = (c + y) % C::kSlots;
-              mma_py<T, 2, 4>(lead, tm + C::kO + y * 128, tm + set * 128 + 64 * x, s_kv + v * C::kUnit + x * 64 * 128, j > 0 || x > 0, 16);
+              mma_py<T, 2, 4>(lead, tm + C::kO + y * 128, tm + set * 128 + 64 * x, s_kv + v * C::kUnit + x * 64 * 128,
+                              j > 0 || x > 0, 16);
               if (x == 1) mma_commit(lead, empty + v);
             }
             mma_commit(lead, o_done + x);
@@ -299,7 +300,8 @@ __global__ void __launch_bounds__(kThreads, NS == 4 ? 1 : 2)
     // visible scores are all -inf has a sum of 0 and comes out as NaN.
     const bool none = ok && (kr.n == 0 || p < 0);
     const float inv = !ok ? NAN : none ? 0.f : 1.f / l;  // a wait that gave up leaves NaN
-    if (i < sq.Tq && lse != nullptr) lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = none ? INFINITY : m - kLift<T> + log2f(l);
+    if (i < sq.Tq && lse != nullptr)
+      lse[((long long)sq.b * pr.H + h) * pr.Tq + sq.q0 + i] = none ? INFINITY : m - kLift<T> + log2f(l);
     // out through shared memory (Q's place and the first key unit's; a warp's own 32 rows), so that rows leave as whole lines
     // (16-byte stores a thread and row took 5 us a CTA); o_low: what the rounding took away, for the backward's delta
     const bool low = o_low != nullptr;

@@ -4,10 +4,10 @@ alternate with the gated delta rule's, on B200 (C ABI gd_wattn_* in libgated_del
     o = softmax(scale q k^T over the visible keys) v
 
 Query i of T_q stands at position p = i + T_k - T_q (the queries are the last T_q positions) and sees key j when j <= p and
-(j > p - window or j < sinks); a query that sees no key gets zeros. `window_attention` trains and prefills (tcgen05
-products, probabilities rounded to the inputs' 16-bit type as the matrix instruction's operand, everything else float32);
-Masked scores are never used; a masked value's infinity or NaN still meets a weight of 0 in the products of its tile, as
-in the formula's matrix product, except across packed sequences, which stay apart.
+(j > p - window or j < sinks); a query that sees no key gets zeros. `window_attention` trains and prefills: tcgen05
+products; the probabilities and the scores' gradients are rounded to the inputs' 16-bit type as the matrix instruction's
+operands, everything else is float32. Masked scores are never used; a masked value's infinity or NaN still meets a weight of
+0 in the products of its tile, as in the formula's matrix product, except across packed sequences, which stay apart.
 `window_attention_step` is the single-token form over a cache. bfloat16 and float16. There is no CPU path: CUDA tensors
 only.
 """
@@ -25,8 +25,6 @@ from ._call import aligned, first_order, launch, like, recorded
 
 _DTYPES = {torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 MAX_D = 256
-
-
 
 
 @functools.lru_cache(maxsize=1024)
@@ -69,8 +67,9 @@ def _fwd(q, k, v, cu, window, sinks, scale, keep):
     if keep:
         low, lse = like(q), torch.empty((B, H, Tq), dtype=torch.float32, device=q.device)
     launch("gd_wattn_fwd", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-           None if low is None else low.data_ptr(), None if lse is None else lse.data_ptr(), None if cu is None else cu.data_ptr(), 0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], B, Tq, Tk, H, HK,
-           D, _strides(q, k, v), window, sinks, scale, None, 0)
+           None if low is None else low.data_ptr(), None if lse is None else lse.data_ptr(),
+           None if cu is None else cu.data_ptr(), 0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], B, Tq, Tk, H, HK, D,
+           _strides(q, k, v), window, sinks, scale, None, 0)
     return o, low, lse
 
 
