@@ -339,6 +339,22 @@ int gd_wattn_step(const void* q, const void* k, const void* v, void* k_cache, vo
                   int dtype, int B, int S, int H, int HK, int D, const long long* strides, int window, int sinks,
                   float scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- the rule's recurrent form (single tokens and short runs over kept states) ----
+ * For each request b and value head h, token after token: S <- exp(g) S, d = beta (v - S^T k), S <- S + k d^T, o = S^T q, with
+ * q scaled by DK^-1/2 (and q, k l2-normalised first with GD_L2NORM, the only flag), everything in float32. q, k
+ * [B, T, HK, DK] and o [B, T, H, DV] in `dtype` (any of the three), v [B, T, H, DV] in `vdtype` (dtype or GD_FLOAT32), g, beta
+ * [B, T, H] float32. States are float32 [n_slots, H, DK, DV]: request b starts from s_in's slot slots[b] (s_in NULL: from
+ * zeros) and leaves its state in s_out's slot out_slots[b] (s_out NULL: nowhere); slots and out_slots, int32 [B] on the device,
+ * are both given or both NULL (slot b, n_slots >= B). s_in and s_out may be one pool. Other slots are neither read nor written.
+ * A negative slot marks an idle request: its o is zeros. A request with a slot >= n_slots, or whose written slot another
+ * request of the call reads or writes, gets o = NaN. Neither of them changes a state. DK, DV: multiples of 32 up to 256.
+ * No allocation, no atomics, asynchronous on `stream`.
+ * Replaces: the token-serial kernels gdr_fwd* (src/macai/gated_delta/_metal.py:37-77, :202-243) for decoding, with the
+ * arguments of transformers' torch_recurrent_gated_delta_rule. */
+int gd_rule_step(const void* q, const void* k, const void* v, const float* g, const float* beta, const float* s_in,
+                 float* s_out, const int* slots, const int* out_slots, void* o, int dtype, int vdtype, int B, int T,
+                 int H, int HK, int DK, int DV, int n_slots, int flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
