@@ -355,6 +355,47 @@ int gd_rule_step(const void* q, const void* k, const void* v, const float* g, co
                  float* s_out, const int* slots, const int* out_slots, void* o, int dtype, int vdtype, int B, int T,
                  int H, int HK, int DK, int DV, int n_slots, int flags, void* stream);
 
+/* ---- the gated feed-forward block ----
+ * g = x w_gate^T, u = x w_up^T, h = silu(g) u, y = h w_down^T: x [rows, D], w_gate, w_up [F, D], w_down [O, F], y [rows, O], all
+ * in `dtype` (GD_FLOAT16 or GD_BFLOAT16); D, F, O multiples of 8. Products of 16-bit operands, sums in float32; h (and g, u,
+ * which the backward keeps) are rounded to `dtype`. ld: elements from row to row of x, w_gate, w_up, w_down (and dy in the
+ * backward), multiples of 8; g, u, y and the gradients are contiguous. All pointers 16-byte aligned. Asynchronous on `stream`,
+ * no atomics whose order changes results.
+ * Replaces: the SwiGLU part and the three projections around it (src/macai/layer/_swiglu.py:41-45). */
+size_t gd_ff_workspace_bytes(long long rows, int D, int F, int O, int for_backward);
+
+/* g, u [rows, F]: kept for the backward, or both NULL. bounds (GD_FLOAT16 with g and u; 16 bytes): max |g| and max |u|, kept
+ * for the backward, else NULL. */
+int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* g, void* u,
+              unsigned int* bounds, void* y, int dtype, long long rows, int D, int F, int O, const long long* ld,
+              void* workspace, size_t workspace_bytes, void* stream);
+
+/* dx, dw_gate, dw_up, dw_down from dy [rows, O]; each may be NULL (not formed). The gradients of g and u are rounded to `dtype`
+ * as operands of the products that follow; in GD_FLOAT16 they carry one power of two for the call that keeps them in range. */
+int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* g, const void* u,
+              const unsigned int* bounds, const void* dy, void* dx, void* dw_gate, void* dw_up, void* dw_down, int dtype,
+              long long rows, int D, int F, int O, const long long* ld, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- softmax cross entropy of a vocabulary projection, without the logits ----
+ * loss_i = logsumexp_v(x_i . w_v) - x_i . w_label(i): x [rows, D], w [V, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), ldx and ldw
+ * elements from row to row (multiples of 8), D a multiple of 8, any V up to 2^24; labels [rows] int32, or int64 with label64.
+ * A row whose label is `ignore` has loss 0 and no gradient, whatever its values are; any other label outside [0, V) gives NaN.
+ * reduction 0: loss [rows]; 1: the mean over the rows that are not ignored (none: NaN); 2: their sum; float32.
+ * The workspace of the forward holds 8 bytes a row and 128 columns; that of the backward a piece of the vocabulary's gradients
+ * of the logits in `dtype` (at most 256 MiB, or 256 columns) and, with more than one piece, dx in float32. Asynchronous on
+ * `stream`; the same bits every run. No counterpart in the reference. */
+size_t gd_xent_workspace_bytes(long long rows, int D, int V, int for_backward);
+
+/* lse2 [rows]: the logsumexp in log2 units, kept for the backward, or NULL. */
+int gd_xent_fwd(const void* x, const void* w, const void* labels, int label64, float* loss, float* lse2, int reduction,
+                long long ignore, int dtype, long long rows, int D, int V, long long ldx, long long ldw, void* workspace,
+                size_t workspace_bytes, void* stream);
+
+/* dx [rows, D], dw [V, D] (each may be NULL) from dloss: float32 [rows] for reduction 0, else one value. */
+int gd_xent_bwd(const void* x, const void* w, const void* labels, int label64, const float* lse2, const float* dloss,
+                void* dx, void* dw, int reduction, long long ignore, int dtype, long long rows, int D, int V, long long ldx,
+                long long ldw, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,626 @@
+// Matrix products on tcgen05 with an epilogue each, the core of the gated feed-forward block (gd_ff.cu) and of the vocabulary
+// projection's cross entropy (gd_xent.cu):  C[M, N] = sum over k of A[m, k] B[n, k],  16-bit operands, fp32 accumulators.
+//
+// Each operand is read where the caller has it: rows of k (K-major: a matrix whose rows are m or n) or rows of m or n
+// (MN-major: a matrix whose rows are k); the tensor core takes both from the same 128-byte swizzled tiles, only descriptor and
+// tensor map differ. TMA fills what lies past a matrix with zeros, so no size has to fill a tile.
+//
+// A pair of CTAs (cluster of two, tcgen05 cta_group::2) computes 256 x 256: each CTA holds its 128 rows of A and 128 of the 256
+// rows of B, so that a product of 64 k reads 32 KB of shared memory an SM where a lone CTA's 128 x 256 would read 48 KB. Roles:
+// warp 0 loads (TMA, a ring of stages), warp 1 of the first CTA issues the products, warps 4 - 11 are the epilogue (a thread
+// owns a row and half of the tile's columns; TMEM lane = row). The accumulator is double-buffered (2 x 256 TMEM columns), so a
+// tile's epilogue runs under the next one's products. The CTAs are persistent and walk the tiles of up to kMaxOps problems.
+#pragma once
+
+#include "gd_wattn.cuh"
+
+namespace gd {
+namespace gemm {
+
+using wattn::elect;
+using wattn::ex2;
+using wattn::pack16;
+using wattn::st_shared16;
+using wattn::unpack16;
+using wattn::warp_wait;
+
+constexpr int kBlockK = 64;            // k of a stage: one 128-byte row of the swizzle
+constexpr int kHalf = 128;             // rows of A, and of B, that a CTA holds
+constexpr int kTileM = 256, kTileN = 256;
+constexpr int kOperand = kHalf * 128;  // bytes of a CTA's part of an operand's stage
+constexpr int kStage = 2 * kOperand;
+constexpr int kSlab = 32 * 128;        // a warp's 32 rows of 64 16-bit columns, on their way in or out
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (4 + kEpiWarps);
+constexpr int kMaxOps = 4;
+constexpr int kGroupM = 8;             // row tiles that are walked together, column tile after column tile (L2)
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum Epilogue {
+  kStore,    // C, times a factor, in 16 bits; or summed over calls in fp32 (see Op::sum)
+  kSwiglu,   // B's two halves are the gate's and the up projection's rows: h = silu(g) u (and g, u where kept)
+  kDSwiglu,  // C = dh: dg, du (and h again) from the kept g, u
+  kLse,      // each row's maximum and sum of exponentials over the tile's columns, and its label's logit
+  kDLogit    // (softmax - onehot) times the row's factor, in 16 bits
+};
+
+// One product. a[s], b[s]: the operands of contraction segment s (kSwiglu: b[0] gate, b[1] up, one segment).
+struct Op {
+  CUtensorMap a[2], b[2], c;
+  int tiles_m, tiles_n, first;  // first: its first tile's index
+  int kb[2];                    // stages of each segment
+  bool a_mn, b_mn;
+  int M, N;
+  // kStore: 0 = C in 16 bits; 1 = C into `sum`; 2 = added to `sum`; 3 = `sum` + C in 16 bits. The sums lie as the threads
+  // hold them: [tile][CTA][column][row].
+  int sum_mode;
+  float* sum;
+  const float* factor;  // NULL: 1
+  bool unscale;         // C is divided by what dg and du carry (Params::bounds)
+};
+
+struct Params {
+  Op op[kMaxOps];
+  int ops, tiles;
+  CUtensorMap x[3];         // kSwiglu: g, u (both or neither kept: keep); kDSwiglu: g, u, h
+  CUtensorMap y;            // kDSwiglu: du (Op::c is dg)
+  bool keep;                // kSwiglu: store g, u; kDSwiglu: store h
+  // float16's feed-forward block: the bits of max |g|, max |u| (kSwiglu collects them), max ||dy row||_1, max |w_down|
+  uint32_t* bounds;
+  // kLse, kDLogit
+  const void* labels;
+  int label64;
+  long long ignore;
+  int v0;                   // the first column's place in the vocabulary
+  float2* part;             // [2 tiles_n][M]: maximum (log2 units), sum
+  float* target;            // [M]: the label's logit
+  const float* lse2;        // [M], log2 units
+  const float* row_scale;   // [M]
+  ErrorWord* err;
+};
+
+template <int E>
+struct Cfg {
+  static constexpr int kSlabs = E == kDSwiglu ? 2 : 1;  // a warp's
+  static constexpr int kStages = E == kDSwiglu ? 5 : 6;
+  static constexpr int kBarriers = 2 * kStages + 4 + 1 + kEpiWarps;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kEpiWarps * kSlabs * kSlab + 8 * kBarriers + 16;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// ---- host: a [rows, cols] matrix of 16-bit values, `ld` elements from row to row, as boxes of 64 columns x box_rows
+inline bool matrix_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, long long rows, long long cols, long long ld,
+                       int box_rows) {
+  EncodeTiled enc = encode_tiled();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld : (cols + 7) / 8 * 8) * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// an operand: K-major [m or n, k], or MN-major [k, m or n]
+inline bool operand_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, long long rows, long long cols, long long ld,
+                        bool mn) {
+  return matrix_map(m, base, dt, rows, cols, ld, mn ? kBlockK : kHalf);
+}
+// what a warp stores or loads: 32 rows
+inline bool slab_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, long long rows, long long cols, long long ld) {
+  return matrix_map(m, base, dt, rows, cols, ld, 32);
+}
+inline int blocks_of(long long n, int b) { return (int)((n + b - 1) / b); }
+
+// ---- device: clusters, pairs of CTAs
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_first_cta(const void* p) {  // the same place in the cluster's first CTA
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(0));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Waits (the whole warp, one answer) for a phase that threads of the other CTA arrive at, too.
+__device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, ErrorWord* err, int where) {
+  const long long t0 = clock64();
+  bool ok = false;
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    ok = done != 0;
+    if (ok) break;
+    if (clock64() - t0 > kWaitCycles) {
+      report(err, GD_ERR_TIMEOUT, where);
+      break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+// A box into this CTA's shared memory, counted on a barrier of the pair's first CTA.
+__device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void load_slab(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void store_slab(const CUtensorMap* m, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 x, y;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "mov.b64 x, {%1, %6};\n\t"
+      "mov.b64 y, {%2, %6};\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(acc), "r"(lead), "r"(wattn::kDescHigh)
+      : "memory");
+}
+// both CTAs' barriers at this place complete when the products so far have
+__device__ __forceinline__ void commit_pair(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}\n" ::"r"(
+          smem_u32(bar)),
+      "r"(lead), "h"((uint16_t)3)
+      : "memory");
+}
+
+struct Where {
+  int op, m, n;  // the problem, the tile's first row and column
+};
+template <int E>
+__device__ __forceinline__ Where locate(const Params& p, int tile) {
+  Where w;
+  w.op = 0;
+  if (E == kStore)
+    while (w.op + 1 < p.ops && tile >= p.op[w.op + 1].first) ++w.op;
+  const Op& o = p.op[w.op];
+  const int t = tile - o.first, band = kGroupM * o.tiles_n, g = t / band, r = t - g * band;
+  const int high = o.tiles_m - g * kGroupM < kGroupM ? o.tiles_m - g * kGroupM : kGroupM;
+  w.m = (g * kGroupM + r % high) * kTileM;
+  w.n = (r / high) * (E == kSwiglu ? kHalf : kTileN);
+  return w;
+}
+
+__device__ __forceinline__ uint32_t slab_at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+// 64 packed columns of the thread's row into its warp's slab
+__device__ __forceinline__ void put_row(uint32_t slab, int lane, const uint32_t (&u)[32]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const uint32_t v[4] = {u[4 * c], u[4 * c + 1], u[4 * c + 2], u[4 * c + 3]};
+    st_shared16(slab + slab_at(lane, c), v);
+  }
+}
+__device__ __forceinline__ void get_row(uint32_t slab, int lane, uint32_t (&u)[32]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(u[4 * c]), "=r"(u[4 * c + 1]), "=r"(u[4 * c + 2]), "=r"(u[4 * c + 3])
+                 : "r"(slab + slab_at(lane, c))
+                 : "memory");
+}
+// The warp's slab of 32 x 64 values leaves for rows m0 .. of matrix m, columns n0 ..; what lies past the matrix is cut off.
+// `u`: the thread's row. Waits until the slab's previous content is read.
+__device__ __forceinline__ void send_row(const CUtensorMap* m, uint32_t slab, int lane, int n0, int m0, const uint32_t (&u)[32]) {
+  if (lane == 0) bulk_wait_read0();
+  __syncwarp();
+  put_row(slab, lane, u);
+  fence_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    store_slab(m, n0, m0, slab);
+    bulk_commit();
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float fits(float x) {  // a finite value stays finite in T
+  if constexpr (std::is_same<T, __half>::value)
+    return fabsf(x) > 65504.f && fabsf(x) < INFINITY ? copysignf(65504.f, x) : x;
+  return x;
+}
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + ex2(-kLog2e * x)); }
+
+// The power of two that dg and du carry in float16, the same for a whole call: |dh| <= ||dy row||_1 max |w_down|, |silu'| < 1.1
+// and |silu(g)| <= |g| bound both by B, and 2^15 is the largest power of two in range. Without a bound above 0: 1.
+__device__ __forceinline__ float carried(const uint32_t* b) {
+  if (b == nullptr) return 1.f;
+  const float g = __uint_as_float(b[0]), u = __uint_as_float(b[1]);
+  const float most = __uint_as_float(b[2]) * __uint_as_float(b[3]) * fmaxf(g, 1.1f * u);
+  if (!(most > 0.f && most < INFINITY)) return 1.f;
+  const int e = 14 - ilogbf(most);
+  return ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e);
+}
+
+__device__ __forceinline__ long long label_of(const Params& p, int row) {
+  return p.label64 ? __ldg(static_cast<const long long*>(p.labels) + row) : __ldg(static_cast<const int*>(p.labels) + row);
+}
+
+template <typename T, int E>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<E>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* slabs = base + C::kStages * kStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(slabs + kEpiWarps * C::kSlabs * kSlab);
+  uint64_t* full = bars;                 // of the pair: the first CTA's are used
+  uint64_t* empty = full + C::kStages;   // each CTA's own
+  uint64_t* acc_full = empty + C::kStages;
+  uint64_t* acc_empty = acc_full + 2;    // of the pair: the first CTA's are used
+  uint64_t* fin = acc_empty + 2;
+  uint64_t* aux = fin + 1;               // each epilogue warp's own loads
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, 2 * kEpiWarps);
+    }
+    mbar_init(fin, 1);
+    for (int i = 0; i < kEpiWarps; ++i) mbar_init(aux + i, 1);
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tm = __shfl_sync(0xffffffffu, *tslot, 0);
+  const uint32_t s_base = smem_u32(base);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int slot = 0, laps = 0, issued = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
+        const Where w = locate<E>(p, tile);
+        const Op& op = p.op[w.op];
+        const int am = w.m + (int)rank * kHalf, bn = E == kSwiglu ? w.n : w.n + (int)rank * kHalf;
+        for (int s = 0; ok && s < 2; ++s) {
+          const CUtensorMap* ma = &op.a[s];
+          const CUtensorMap* mb = E == kSwiglu ? &op.b[rank] : &op.b[s];
+          for (int kb = 0; kb < op.kb[s]; ++kb) {
+            if (laps > 0 && !mbar_wait(empty + slot, (laps - 1) & 1, p.err, 80)) {
+              ok = false;
+              break;
+            }
+            if (rank == 0) mbar_arrive_expect_tx(full + slot, 2 * kStage);
+            const uint32_t bar = in_first_cta(full + slot), a = s_base + slot * kStage, b = a + kOperand;
+            if (op.a_mn) {
+              load_pair(a, ma, am, kb * kBlockK, bar);
+              load_pair(a + kOperand / 2, ma, am + 64, kb * kBlockK, bar);
+            } else {
+              load_pair(a, ma, kb * kBlockK, am, bar);
+            }
+            if (op.b_mn) {
+              load_pair(b, mb, bn, kb * kBlockK, bar);
+              load_pair(b + kOperand / 2, mb, bn + 64, kb * kBlockK, bar);
+            } else {
+              load_pair(b, mb, kb * kBlockK, bn, bar);
+            }
+            ++issued;
+            if (++slot == C::kStages) {
+              slot = 0;
+              ++laps;
+            }
+          }
+        }
+      }
+      // The copies in flight land before the CTAs end, whatever became of their readers (they are counted on the first CTA's
+      // barriers; the pair ends together).
+      if (rank == 0)
+        for (int i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
+          mbar_wait(full + i % C::kStages, (i / C::kStages) & 1, p.err, 81);
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t lead = elect();
+      int slot = 0, laps = 0, it = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < p.tiles; tile += pairs, ++it) {
+        const Where w = locate<E>(p, tile);
+        const Op& op = p.op[w.op];
+        const int buf = it & 1;
+        if (it >= 2 && !(ok = cluster_wait(acc_empty + buf, ((it >> 1) - 1) & 1, p.err, 82))) break;
+        tc_fence_after();
+        const uint32_t id = wattn::idesc<T>(256, 256, false) | (op.a_mn ? 1u << 15 : 0u) | (op.b_mn ? 1u << 16 : 0u);
+        const uint32_t a_hi = op.a_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16, b_hi = op.b_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16;
+        const uint32_t a_step = op.a_mn ? 128 : 2, b_step = op.b_mn ? 128 : 2;  // 16 k further, in 16 bytes
+        const uint32_t d = tm + buf * kTileN;
+        const int n = op.kb[0] + op.kb[1];
+        for (int kb = 0; kb < n; ++kb) {
+          if (!(ok = cluster_wait(full + slot, laps & 1, p.err, 83))) break;
+          tc_fence_after();
+          const uint32_t a = ((s_base + slot * kStage) >> 4) | a_hi, b = ((s_base + slot * kStage + kOperand) >> 4) | b_hi;
+#pragma unroll
+          for (int k = 0; k < kBlockK / 16; ++k) mma_pair(lead, d, a + k * a_step, b + k * b_step, id, kb > 0 || k > 0);
+          commit_pair(lead, empty + slot);
+          if (++slot == C::kStages) {
+            slot = 0;
+            ++laps;
+          }
+        }
+        if (ok) commit_pair(lead, acc_full + buf);
+      }
+      commit_pair(lead, fin);  // (a pair whose waits gave up ends with no product in flight)
+      warp_wait(fin, 0, p.err, 84);
+    }
+  } else if (warp >= 4) {
+    const int ew = warp - 4, quad = warp & 3, half = ew >> 2;  // a warp reads the TMEM lanes of its quarter
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t slab = smem_u32(slabs) + ew * C::kSlabs * kSlab;
+    bool ok = true;
+    int it = 0, loads = 0;
+    for (int tile = pair; tile < p.tiles; tile += pairs, ++it) {
+      const Where w = locate<E>(p, tile);
+      const Op& op = p.op[w.op];
+      const int buf = it & 1, m0 = w.m + (int)rank * kHalf + quad * 32, row = m0 + lane;
+      const uint32_t t0 = tm + lanes + buf * kTileN;
+      const bool live = m0 < op.M;  // the warp has rows of the matrix
+      auto fetch = [&](int n0) {    // kDSwiglu: g and u of 64 columns, into the warp's slabs
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          bulk_wait_read0();
+          mbar_arrive_expect_tx(aux + ew, 2 * kSlab);
+          load_slab(slab, &p.x[0], n0, m0, aux + ew);
+          load_slab(slab + kSlab, &p.x[1], n0, m0, aux + ew);
+        }
+      };
+      auto has = [&](int n0) { return live && n0 < op.N; };
+      if (E == kDSwiglu && has(w.n + half * 128)) fetch(w.n + half * 128);
+      ok = ok && warp_wait(acc_full + buf, (it >> 1) & 1, p.err, 85);
+      tc_fence_after();
+      const float bad = ok ? 0.f : NAN;  // a wait that gave up leaves NaN
+      auto release = [&] {               // the accumulator is read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(in_first_cta(acc_empty + buf));
+      };
+
+      if constexpr (E == kStore) {
+        const float f = (op.factor != nullptr ? __ldg(op.factor) : op.unscale ? 1.f / carried(p.bounds) : 1.f) + bad;
+        float* sum = op.sum_mode == 0 ? nullptr
+                                      : op.sum + (((long long)(tile - op.first) * 2 + rank) * kTileN + half * 128) * kHalf +
+                                            quad * 32 + lane;
+#pragma unroll 1
+        for (int s = 0; s < 2; ++s) {
+          const int c = half * 128 + s * 64, n0 = w.n + c;
+          float v[64];
+          wattn::tmem_ld64(t0 + c, v);
+          if (s == 1) release();
+          if (!has(n0)) continue;
+          if (op.sum_mode != 0) {
+            float* at = sum + (long long)s * 64 * kHalf;
+            if (op.sum_mode != 1) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) v[i] += at[(long long)i * kHalf];
+            }
+            if (op.sum_mode != 3) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) at[(long long)i * kHalf] = v[i] + bad;
+              continue;
+            }
+          }
+          uint32_t u[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) u[i] = pack16<T>(v[2 * i] * f, v[2 * i + 1] * f);
+          send_row(&op.c, slab, lane, n0, m0, u);
+        }
+      } else if constexpr (E == kSwiglu) {
+        const int n0 = w.n + half * 64;
+        uint32_t hp[32], gp[32], up[32];
+        float top_g = 0.f, top_u = 0.f;
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          float g[32], u[32];
+          tmem_ld32(t0 + half * 64 + c, g);
+          tmem_ld32(t0 + kHalf + half * 64 + c, u);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float a = g[i] * sigmoid(g[i]) * u[i] + bad, b = g[i + 1] * sigmoid(g[i + 1]) * u[i + 1] + bad;
+            hp[(c + i) / 2] = pack16<T>(a, b);
+            gp[(c + i) / 2] = pack16<T>(fits<T>(g[i]), fits<T>(g[i + 1]));
+            up[(c + i) / 2] = pack16<T>(fits<T>(u[i]), fits<T>(u[i + 1]));
+            if constexpr (std::is_same<T, __half>::value) {
+              top_g = wattn::max3(top_g, fabsf(g[i]), fabsf(g[i + 1]));
+              top_u = wattn::max3(top_u, fabsf(u[i]), fabsf(u[i + 1]));
+            }
+          }
+        }
+        release();
+        if (has(n0)) {
+          send_row(&op.c, slab, lane, n0, m0, hp);
+          if (p.keep) {
+            if constexpr (std::is_same<T, __half>::value) {  // (zeros past the matrix)
+              top_g = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_g)));
+              top_u = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_u)));
+              if (lane == 0) {
+                atomicMax(p.bounds, __float_as_uint(top_g));
+                atomicMax(p.bounds + 1, __float_as_uint(top_u));
+              }
+            }
+            send_row(&p.x[0], slab, lane, n0, m0, gp);
+            send_row(&p.x[1], slab, lane, n0, m0, up);
+          }
+        }
+      } else if constexpr (E == kDSwiglu) {
+        const float f = carried(p.bounds) + bad;
+#pragma unroll 1
+        for (int s = 0; s < 2; ++s) {
+          const int c = half * 128 + s * 64, n0 = w.n + c;
+          if (!has(n0)) {
+            if (s == 1) release();
+            continue;
+          }
+          if (s == 1) fetch(n0);
+          uint32_t gp[32], up[32], hp[32];
+          warp_wait(aux + ew, loads & 1, p.err, 86);
+          ++loads;
+          get_row(slab, lane, gp);
+          get_row(slab + kSlab, lane, up);
+#pragma unroll
+          for (int x = 0; x < 64; x += 32) {
+            float d[32];
+            tmem_ld32(t0 + c + x, d);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const int j = (x + i) / 2;
+              const float2 g = unpack16<T>(gp[j]), u = unpack16<T>(up[j]);
+              const float s0 = sigmoid(g.x), s1 = sigmoid(g.y), a0 = g.x * s0, a1 = g.y * s1;
+              const float d0 = d[i] * f, d1 = d[i + 1] * f;
+              hp[j] = pack16<T>(a0 * u.x, a1 * u.y);
+              gp[j] = pack16<T>(d0 * u.x * (s0 + a0 * (1.f - s0)), d1 * u.y * (s1 + a1 * (1.f - s1)));
+              up[j] = pack16<T>(d0 * a0, d1 * a1);
+            }
+          }
+          if (s == 1) release();
+          __syncwarp();  // g and u are read
+          put_row(slab, lane, gp);
+          put_row(slab + kSlab, lane, up);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            store_slab(&op.c, n0, m0, slab);
+            store_slab(&p.y, n0, m0, slab + kSlab);
+            bulk_commit();
+          }
+          if (p.keep) send_row(&p.x[2], slab, lane, n0, m0, hp);
+        }
+      } else if constexpr (E == kLse) {
+        const long long lab = row < op.M ? label_of(p, row) - p.v0 : -1;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+        for (int s = 0; s < 2; ++s) {
+          const int c = half * 128 + s * 64, n0 = w.n + c;
+          float v[64];
+          wattn::tmem_ld64(t0 + c, v);
+          if (s == 1) release();
+          if (n0 >= op.N) continue;
+          const bool here = row < op.M && lab >= n0 && lab < n0 + 64 && lab < op.N;
+          if (__any_sync(0xffffffffu, here)) {
+            float x = 0.f;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) x = lab == n0 + i ? v[i] : x;
+            if (here) p.target[row] = x + bad;
+          }
+          if (n0 + 64 > op.N) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) v[i] = n0 + i < op.N ? v[i] : -INFINITY;
+          }
+          float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int i = 4; i < 60; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = wattn::max3(mx[e], v[i + 2 * e], v[i + 2 * e + 1]);
+          }
+          const float high = wattn::max3(wattn::max3(mx[0], mx[1], mx[2]), wattn::max3(mx[3], v[60], v[61]),
+                                         wattn::max3(v[62], v[63], v[62])) * kLog2e;
+          const float next = wattn::max3(top, high, high), ref = next == -INFINITY ? 0.f : next;
+          float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 64; ++i) a[i & 3] += ex2(fmaf(v[i], kLog2e, -ref));
+          sum = sum * ex2(top - ref) + ((a[0] + a[1]) + (a[2] + a[3]));
+          top = next;
+        }
+        if (row < op.M && w.n + half * 128 < op.N)
+          p.part[(long long)(w.n / kTileN * 2 + half) * op.M + row] = make_float2(top, sum + bad);
+      } else {  // kDLogit
+        const long long lab = row < op.M ? label_of(p, row) : p.ignore;
+        const bool kept = lab != p.ignore;
+        const long long at = kept ? lab - p.v0 : -1;
+        const float l2 = kept ? __ldg(p.lse2 + row) : 0.f, f = kept ? __ldg(p.row_scale + row) + bad : 0.f;
+#pragma unroll 1
+        for (int s = 0; s < 2; ++s) {
+          const int c = half * 128 + s * 64, n0 = w.n + c;
+          float v[64];
+          wattn::tmem_ld64(t0 + c, v);
+          if (s == 1) release();
+          if (!has(n0)) continue;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -l2));
+          if (__any_sync(0xffffffffu, at >= n0 && at < n0 + 64)) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) v[i] -= at == n0 + i ? 1.f : 0.f;
+          }
+          uint32_t u[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const uint32_t x = pack16<T>(v[2 * i] * f, v[2 * i + 1] * f);
+            u[i] = kept ? x : 0u;  // an ignored row's logits may be anything
+          }
+          send_row(&op.c, slab, lane, n0, m0, u);
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_read0();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
+}
+
+// Problems in order: each one's first tile is set here. Persistent pairs: as many as SMs allow.
+template <typename T, int E>
+int launch(Params& p, cudaStream_t stream) {
+  int tiles = 0;
+  for (int i = 0; i < p.ops; ++i) {
+    p.op[i].first = tiles;
+    tiles += p.op[i].tiles_m * p.op[i].tiles_n;
+  }
+  p.tiles = tiles;
+  if (tiles == 0) return GD_OK;
+  static bool done[kMaxDevices];
+  auto kern = gemm_kernel<T, E>;
+  if (set_smem_once(kern, Cfg<E>::kSmem, done) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return (cudaGetLastError(), GD_ERR_LAUNCH);
+  const int pairs = tiles < sms / 2 ? tiles : sms / 2;
+  kern<<<2 * pairs, kThreads, Cfg<E>::kSmem, stream>>>(p);
+  return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
+}
+
+}  // namespace gemm
+}  // namespace gd

@@ -1,0 +1,110 @@
+"""The gated feed-forward block of a decoder layer on B200 (C ABI gd_ff_* in libgated_delta_b200.so), the half of the layer
+after its mixer:
+
+    g = x w_gate^T,   u = x w_up^T,   h = silu(g) * u,   y = h w_down^T
+
+`gated_feed_forward` trains, prefills, and takes the few tokens of a decoding step. tcgen05 products with float32 sums; the
+activation and its gradient are taken in float32 as the products leave the tensor core, so neither g nor u is read again in
+the forward, and the gradient of h never leaves the chip. h, and for the backward g, u and their gradients, are rounded to the
+inputs' 16-bit type (the matrix instruction's operands). bfloat16 and float16. There is no CPU path: CUDA tensors only.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+
+import torch
+
+from . import _lib
+from ._call import first_order, launch, matrix, pitch, recorded
+
+_DTYPES = {torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
+
+
+@functools.lru_cache(maxsize=1024)
+def _bytes(*sizes) -> int:
+    n = _lib.load().gd_ff_workspace_bytes(*sizes)
+    if n == 0:
+        raise NotImplementedError(f"gated_feed_forward: sizes (rows, D, F, O) = {sizes[:4]} are too large")
+    return n
+
+
+def _pitches(*ms):
+    return (ctypes.c_longlong * len(ms))(*[pitch(m) for m in ms])
+
+
+def _sizes(x, wg, wd):
+    return x.shape[0], x.shape[1], wg.shape[0], wd.shape[0]
+
+
+def _fwd(x, wg, wu, wd, keep):
+    """(y, g, u, bounds) on matrices; keep: g, u (and float16's bounds) for the backward, else None."""
+    n, D, F, O = _sizes(x, wg, wd)
+    y = torch.empty((n, O), dtype=x.dtype, device=x.device)
+    g = u = bounds = None
+    if keep:
+        g, u = (torch.empty((n, F), dtype=x.dtype, device=x.device) for _ in range(2))
+        if x.dtype == torch.float16:
+            bounds = torch.empty(4, dtype=torch.int32, device=x.device)
+    size = _bytes(n, D, F, O, 0)
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    launch("gd_ff_fwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), p(g), p(u), p(bounds),
+           y.data_ptr(), _DTYPES[x.dtype], n, D, F, O, _pitches(x, wg, wu, wd), ws.data_ptr(), size)
+    return y, g, u, bounds
+
+
+def _bwd(x, wg, wu, wd, g, u, bounds, dy, need):
+    """(dx, dw_gate, dw_up, dw_down), contiguous, each None unless needed."""
+    n, D, F, O = _sizes(x, wg, wd)
+    make = lambda yes, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if yes else None  # noqa: E731
+    out = (make(need[0], n, D), make(need[1], F, D), make(need[2], F, D), make(need[3], O, F))
+    size = _bytes(n, D, F, O, 1)
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    launch("gd_ff_bwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), g.data_ptr(), u.data_ptr(),
+           None if bounds is None else bounds.data_ptr(), dy.data_ptr(), *(None if t is None else t.data_ptr() for t in out),
+           _DTYPES[x.dtype], n, D, F, O, _pitches(x, wg, wu, wd, dy), ws.data_ptr(), size)
+    return out
+
+
+class GatedFeedForward(torch.autograd.Function):
+    """`GatedFeedForward.apply(x, w_gate, w_up, w_down)` on matrices (adjacent columns, aligned rows)."""
+
+    @staticmethod
+    def forward(ctx, x, wg, wu, wd):
+        y, g, u, bounds = _fwd(x, wg, wu, wd, True)
+        ctx.save_for_backward(x, wg, wu, wd, g, u, bounds)
+        return y
+
+    @staticmethod
+    @first_order
+    def backward(ctx, dy):
+        return _bwd(*ctx.saved_tensors, matrix(dy), ctx.needs_input_grad)
+
+
+def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
+    """y [..., O] for x [..., D], w_gate and w_up [F, D] (as nn.Linear keeps them; halves of one [2 F, D] weight are read in
+    place) and w_down [O, F], all bfloat16 or all float16, D, F and O multiples of 8. Gradients of all four come in their
+    type, the same bits every run; those of frozen inputs are not formed. Views with adjacent columns and 16-byte aligned
+    rows are read in place, others are copied."""
+    name = "gated_feed_forward"
+    for n, t, d in (("x", x, 1), ("w_gate", w_gate, 2), ("w_up", w_up, 2), ("w_down", w_down, 2)):
+        if not isinstance(t, torch.Tensor) or t.dim() < d or (d == 2 and t.dim() != 2):
+            raise ValueError(f"{name}: {n} must be {'[..., D]' if d == 1 else 'a matrix'}")
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"{name}: bfloat16 or float16, got {t.dtype} for {n}")
+        if t.dtype != x.dtype or t.get_device() != x.get_device():
+            raise ValueError(f"{name}: x and the weights must share one dtype and device")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name}: CUDA tensors only (there is no CPU path)")
+    D, (F, d2), O = x.shape[-1], w_gate.shape, w_down.shape[0]
+    if d2 != D or w_up.shape != w_gate.shape or w_down.shape[1] != F:
+        raise ValueError(f"{name}: w_gate and w_up [F, D] and w_down [O, F] must agree with x [..., D]; got {tuple(x.shape)}, "
+                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
+    if min(D, F, O) == 0 or D % 8 or F % 8 or O % 8:
+        raise NotImplementedError(f"{name}: D, F and O are multiples of 8, got {D}, {F}, {O}")
+    if recorded(x, w_gate, w_up, w_down):
+        y = GatedFeedForward.apply(matrix(x), matrix(w_gate), matrix(w_up), matrix(w_down))
+    else:
+        y = _fwd(matrix(x), matrix(w_gate), matrix(w_up), matrix(w_down), False)[0]
+    return y.view(*x.shape[:-1], O)
