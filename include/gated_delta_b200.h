@@ -357,22 +357,23 @@ int gd_rule_step(const void* q, const void* k, const void* v, const float* g, co
 
 /* ---- the gated feed-forward block ----
  * g = x w_gate^T, u = x w_up^T, h = silu(g) u, y = h w_down^T: x [rows, D], w_gate, w_up [F, D], w_down [O, F], y [rows, O], all
- * in `dtype` (GD_FLOAT16 or GD_BFLOAT16); D, F, O multiples of 8. Products of 16-bit operands, sums in float32; h (and g, u,
- * which the backward keeps) are rounded to `dtype`. ld: elements from row to row of x, w_gate, w_up, w_down (and dy in the
- * backward), multiples of 8; g, u, y and the gradients are contiguous. All pointers 16-byte aligned. Asynchronous on `stream`,
+ * in `dtype` (GD_FLOAT16 or GD_BFLOAT16); D, F, O multiples of 8. Products of 16-bit operands, sums in float32; h is rounded to
+ * `dtype`. ld: elements from row to row of x, w_gate, w_up, w_down (and dy in the
+ * backward), multiples of 8; y and the gradients are contiguous. All pointers 16-byte aligned. Asynchronous on `stream`,
  * no atomics whose order changes results.
  * Replaces: the SwiGLU part and the three projections around it (src/macai/layer/_swiglu.py:41-45). */
 size_t gd_ff_workspace_bytes(long long rows, int D, int F, int O, int for_backward);
 
-/* g, u [rows, F]: kept for the backward, or both NULL. bounds (GD_FLOAT16 with g and u; 16 bytes): max |g| and max |u|, kept
- * for the backward, else NULL. */
-int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* g, void* u,
-              unsigned int* bounds, void* y, int dtype, long long rows, int D, int F, int O, const long long* ld,
+/* kept [3, rows, F] 16-bit words: the upper 24 bits of g's and u's float32 values (the upper halves of g's, of u's, the next
+ * byte of both), for the backward; or NULL. bounds (GD_FLOAT16 with kept; 16 bytes): max |g| and max |u|, for the backward;
+ * else NULL. */
+int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* kept, unsigned int* bounds,
+              void* y, int dtype, long long rows, int D, int F, int O, const long long* ld,
               void* workspace, size_t workspace_bytes, void* stream);
 
 /* dx, dw_gate, dw_up, dw_down from dy [rows, O]; each may be NULL (not formed). The gradients of g and u are rounded to `dtype`
  * as operands of the products that follow; in GD_FLOAT16 they carry one power of two for the call that keeps them in range. */
-int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* g, const void* u,
+int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* kept,
               const unsigned int* bounds, const void* dy, void* dx, void* dw_gate, void* dw_up, void* dw_down, int dtype,
               long long rows, int D, int F, int O, const long long* ld, void* workspace, size_t workspace_bytes, void* stream);
 

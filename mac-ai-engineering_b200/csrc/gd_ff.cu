@@ -52,18 +52,18 @@ void shape(Op& op, long long M, long long N, int tile_n = gemm::kTileN) {
 }
 
 template <typename T>
-int forward(const Problem& q, void* g, void* u, void* h, void* y, uint32_t* bounds, ErrorWord* err, cudaStream_t stream) {
+int forward(const Problem& q, void* const* kept, void* h, void* y, uint32_t* bounds, ErrorWord* err, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const long long n = q.rows;
   Params p = {};
-  p.ops = 1, p.err = err, p.keep = g != nullptr, p.bounds = bounds;
+  p.ops = 1, p.err = err, p.keep = kept[0] != nullptr, p.bounds = bounds;
   Op& o = p.op[0];
   shape(o, n, q.F, gemm::kHalf);
   o.kb[0] = gemm::blocks_of(q.D, gemm::kBlockK);
   bool ok = gemm::operand_map(&o.a[0], q.x, dt, n, q.D, q.ldx, false) &&
             gemm::operand_map(&o.b[0], q.wg, dt, q.F, q.D, q.ldg, false) &&
-            gemm::operand_map(&o.b[1], q.wu, dt, q.F, q.D, q.ldu, false) && gemm::slab_map(&o.c, h, dt, n, q.F, q.F);
-  if (p.keep) ok = ok && gemm::slab_map(&p.x[0], g, dt, n, q.F, q.F) && gemm::slab_map(&p.x[1], u, dt, n, q.F, q.F);
+            gemm::operand_map(&o.b[1], q.wu, dt, q.F, q.D, q.ldu, false) && gemm::strip_map(&o.c, h, dt, n, q.F, q.F);
+  for (int i = 0; p.keep && i < 3; ++i) ok = ok && gemm::strip_map(&p.x[i], kept[i], dt, n, q.F, q.F);
   if (!ok) return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kSwiglu>(p, stream)) return st;
   Params r = {};
@@ -82,7 +82,7 @@ struct Grads {
 };
 
 template <typename T>
-int backward(const Problem& q, const void* g, const void* u, const void* dy, long long ldy, const Grads& out, void* dg, void* du,
+int backward(const Problem& q, const void* const* kept, const void* dy, long long ldy, const Grads& out, void* dg, void* du,
              void* h, uint32_t* bounds, ErrorWord* err, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const long long n = q.rows;
@@ -99,10 +99,11 @@ int backward(const Problem& q, const void* g, const void* u, const void* dy, lon
   o.kb[0] = gemm::blocks_of(q.O, gemm::kBlockK);
   o.b_mn = true;
   if (!gemm::operand_map(&o.a[0], dy, dt, n, q.O, ldy, false) || !gemm::operand_map(&o.b[0], q.wd, dt, q.O, q.F, q.ldd, true) ||
-      !gemm::slab_map(&o.c, dg, dt, n, q.F, q.F) || !gemm::slab_map(&p.y, du, dt, n, q.F, q.F) ||
-      !gemm::slab_map(&p.x[0], g, dt, n, q.F, q.F) || !gemm::slab_map(&p.x[1], u, dt, n, q.F, q.F) ||
-      (p.keep && !gemm::slab_map(&p.x[2], h, dt, n, q.F, q.F)))
+      !gemm::strip_map(&o.c, dg, dt, n, q.F, q.F) || !gemm::strip_map(&p.y[0], du, dt, n, q.F, q.F) ||
+      (p.keep && !gemm::strip_map(&p.y[1], h, dt, n, q.F, q.F)))
     return GD_ERR_LAUNCH;
+  for (int i = 0; i < 3; ++i)
+    if (!gemm::strip_map(&p.x[i], kept[i], dt, n, q.F, q.F)) return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kDSwiglu>(p, stream)) return st;
   Params r = {};
   r.err = err, r.bounds = bounds;
@@ -169,17 +170,16 @@ extern "C" size_t gd_ff_workspace_bytes(long long rows, int D, int F, int O, int
   return gd::ff::kHead + (for_backward ? 3 : 1) * gd::ff::matrix_bytes(rows, F);
 }
 
-extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* g, void* u,
+extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* kept,
                          unsigned int* bounds, void* y, int dtype, long long rows, int D, int F, int O, const long long* ld,
                          void* workspace, size_t workspace_bytes, void* stream) {
   using namespace gd::ff;
   if (const int st = check(dtype, rows, D, F, O, ld, 4)) return st;
   if (rows == 0) return GD_OK;
-  if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr || y == nullptr || (g == nullptr) != (u == nullptr) ||
-      (dtype == GD_FLOAT16 && (g == nullptr) != (bounds == nullptr)))
+  if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr || y == nullptr ||
+      (dtype == GD_FLOAT16 && (kept == nullptr) != (bounds == nullptr)))
     return GD_ERR_ARG;
-  for (const void* t : {x, w_gate, w_up, w_down, (const void*)g, (const void*)u, (const void*)y, (const void*)workspace,
-                        (const void*)bounds})
+  for (const void* t : {x, w_gate, w_up, w_down, (const void*)kept, (const void*)y, (const void*)workspace, (const void*)bounds})
     if (!aligned16(t)) return GD_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < gd_ff_workspace_bytes(rows, D, F, O, 0)) return GD_ERR_WORKSPACE;
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
@@ -190,11 +190,13 @@ extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, co
     return (cudaGetLastError(), GD_ERR_LAUNCH);
   const Problem q = {x, w_gate, w_up, w_down, ld[0], ld[1], ld[2], ld[3], (int)rows, D, F, O};
   void* h = static_cast<char*>(workspace) + kHead;
-  return dtype == GD_FLOAT16 ? forward<__half>(q, g, u, h, y, bounds, err, cs)
-                             : forward<__nv_bfloat16>(q, g, u, h, y, nullptr, err, cs);
+  void* planes[3];
+  for (int i = 0; i < 3; ++i) planes[i] = kept == nullptr ? nullptr : static_cast<char*>(kept) + i * (size_t)rows * F * 2;
+  return dtype == GD_FLOAT16 ? forward<__half>(q, planes, h, y, bounds, err, cs)
+                             : forward<__nv_bfloat16>(q, planes, h, y, nullptr, err, cs);
 }
 
-extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* g, const void* u,
+extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* kept,
                          const unsigned int* bounds, const void* dy, void* dx, void* dw_gate, void* dw_up, void* dw_down,
                          int dtype, long long rows, int D, int F, int O, const long long* ld, void* workspace,
                          size_t workspace_bytes, void* stream) {
@@ -209,10 +211,10 @@ extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, co
       return (cudaGetLastError(), GD_ERR_LAUNCH);
     return GD_OK;
   }
-  if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr || g == nullptr || u == nullptr || dy == nullptr ||
+  if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr || kept == nullptr || dy == nullptr ||
       (dtype == GD_FLOAT16 && bounds == nullptr))
     return GD_ERR_ARG;
-  for (const void* t : {x, w_gate, w_up, w_down, g, u, dy, (const void*)dx, (const void*)dw_gate, (const void*)dw_up,
+  for (const void* t : {x, w_gate, w_up, w_down, kept, dy, (const void*)dx, (const void*)dw_gate, (const void*)dw_up,
                         (const void*)dw_down, (const void*)workspace, (const void*)bounds})
     if (!aligned16(t)) return GD_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < gd_ff_workspace_bytes(rows, D, F, O, 1)) return GD_ERR_WORKSPACE;
@@ -229,6 +231,8 @@ extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, co
   const Grads out = {dx, dw_gate, dw_up, dw_down};
   const size_t m = matrix_bytes(rows, F);
   void *dg = at + kHead, *du = at + kHead + m, *h = at + kHead + 2 * m;
-  return dtype == GD_FLOAT16 ? backward<__half>(q, g, u, dy, ld[4], out, dg, du, h, own, err, cs)
-                             : backward<__nv_bfloat16>(q, g, u, dy, ld[4], out, dg, du, h, nullptr, err, cs);
+  const void* planes[3];
+  for (int i = 0; i < 3; ++i) planes[i] = static_cast<const char*>(kept) + i * (size_t)rows * F * 2;
+  return dtype == GD_FLOAT16 ? backward<__half>(q, planes, dy, ld[4], out, dg, du, h, own, err, cs)
+                             : backward<__nv_bfloat16>(q, planes, dy, ld[4], out, dg, du, h, nullptr, err, cs);
 }

@@ -21,7 +21,6 @@ using wattn::elect;
 using wattn::ex2;
 using wattn::pack16;
 using wattn::st_shared16;
-using wattn::unpack16;
 using wattn::warp_wait;
 
 constexpr int kBlockK = 64;            // k of a stage: one 128-byte row of the swizzle
@@ -29,7 +28,8 @@ constexpr int kHalf = 128;             // rows of A, and of B, that a CTA holds
 constexpr int kTileM = 256, kTileN = 256;
 constexpr int kOperand = kHalf * 128;  // bytes of a CTA's part of an operand's stage
 constexpr int kStage = 2 * kOperand;
-constexpr int kSlab = 32 * 128;        // a warp's 32 rows of 64 16-bit columns, on their way in or out
+constexpr int kSlab = 32 * 128;        // a warp's 32 rows of 64 16-bit columns, on their way out
+constexpr int kStrip = 32 * 64;        // the same of 32 columns, in or out (64-byte swizzle)
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (4 + kEpiWarps);
 constexpr int kMaxOps = 4;
@@ -62,8 +62,8 @@ struct Op {
 struct Params {
   Op op[kMaxOps];
   int ops, tiles;
-  CUtensorMap x[3];         // kSwiglu: g, u (both or neither kept: keep); kDSwiglu: g, u, h
-  CUtensorMap y;            // kDSwiglu: du (Op::c is dg)
+  CUtensorMap x[3];         // g and u as they are kept: the upper halves of their float32 bits, and the bytes below them
+  CUtensorMap y[2];         // kDSwiglu: du (Op::c is dg), h
   bool keep;                // kSwiglu: store g, u; kDSwiglu: store h
   // float16's feed-forward block: the bits of max |g|, max |u| (kSwiglu collects them), max ||dy row||_1, max |w_down|
   uint32_t* bounds;
@@ -81,31 +81,35 @@ struct Params {
 
 template <int E>
 struct Cfg {
-  static constexpr int kSlabs = E == kDSwiglu ? 2 : 1;  // a warp's
-  static constexpr int kStages = E == kDSwiglu ? 5 : 6;
-  static constexpr int kBarriers = 2 * kStages + 4 + 1 + kEpiWarps;
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kEpiWarps * kSlabs * kSlab + 8 * kBarriers + 16;
+  static constexpr int kOut = E == kDSwiglu ? 6 * kStrip : E == kSwiglu ? 4 * kStrip : kSlab;  // a warp's
+  static constexpr int kStages = E == kDSwiglu ? 4 : E == kSwiglu ? 5 : 6;
+  static constexpr int kBarriers = 2 * kStages + 4 + 1 + 2 * kEpiWarps;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kEpiWarps * kOut + 8 * kBarriers + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// ---- host: a [rows, cols] matrix of 16-bit values, `ld` elements from row to row, as boxes of 64 columns x box_rows
+// ---- host: a [rows, cols] matrix of 16-bit values, `ld` elements from row to row, as boxes of box_cols (64 or 32) x box_rows
 inline bool matrix_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, long long rows, long long cols, long long ld,
-                       int box_rows) {
+                       int box_rows, int box_cols = 64) {
   EncodeTiled enc = encode_tiled();
   if (enc == nullptr) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld : (cols + 7) / 8 * 8) * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return enc(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+             box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // an operand: K-major [m or n, k], or MN-major [k, m or n]
 inline bool operand_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, long long rows, long long cols, long long ld,
                         bool mn) {
   return matrix_map(m, base, dt, rows, cols, ld, mn ? kBlockK : kHalf);
 }
-// what a warp stores or loads: 32 rows
+// what a warp stores or loads: 32 rows of 64 columns, or of 32 (kSwiglu, kDSwiglu)
+inline bool strip_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, long long rows, long long cols, long long ld) {
+  return matrix_map(m, base, dt, rows, cols, ld, 32, 32);
+}
 inline bool slab_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, long long rows, long long cols, long long ld) {
   return matrix_map(m, base, dt, rows, cols, ld, 32);
 }
@@ -130,9 +134,9 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 }
 // Waits (the whole warp, one answer) for a phase that threads of the other CTA arrive at, too.
 __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, ErrorWord* err, int where) {
-  const long long t0 = clock64();
+  long long t0 = 0;
   bool ok = false;
-  for (;;) {
+  for (int turn = 0;; ++turn) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -143,6 +147,7 @@ __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, Err
         : "memory");
     ok = done != 0;
     if (ok) break;
+    if (turn == 0) t0 = clock64();
     if (clock64() - t0 > kWaitCycles) {
       report(err, GD_ERR_TIMEOUT, where);
       break;
@@ -151,11 +156,13 @@ __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, Err
   return __all_sync(0xffffffffu, ok);
 }
 // A box into this CTA's shared memory, counted on a barrier of the pair's first CTA.
-__device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void load_pair(uint32_t lead, uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
-      "[%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(bar)
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(bar), "r"(lead)
       : "memory");
 }
 __device__ __forceinline__ void load_slab(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
@@ -210,6 +217,14 @@ __device__ __forceinline__ Where locate(const Params& p, int tile) {
 }
 
 __device__ __forceinline__ uint32_t slab_at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+__device__ __forceinline__ uint32_t strip_at(int row, int chunk) { return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4); }
+__device__ __forceinline__ void put_strip(uint32_t strip, int lane, const uint32_t (&u)[16]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t v[4] = {u[4 * c], u[4 * c + 1], u[4 * c + 2], u[4 * c + 3]};
+    st_shared16(strip + strip_at(lane, c), v);
+  }
+}
 // 64 packed columns of the thread's row into its warp's slab
 __device__ __forceinline__ void put_row(uint32_t slab, int lane, const uint32_t (&u)[32]) {
 #pragma unroll
@@ -218,13 +233,11 @@ __device__ __forceinline__ void put_row(uint32_t slab, int lane, const uint32_t 
     st_shared16(slab + slab_at(lane, c), v);
   }
 }
-__device__ __forceinline__ void get_row(uint32_t slab, int lane, uint32_t (&u)[32]) {
-#pragma unroll
-  for (int c = 0; c < 8; ++c)
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(u[4 * c]), "=r"(u[4 * c + 1]), "=r"(u[4 * c + 2]), "=r"(u[4 * c + 3])
-                 : "r"(slab + slab_at(lane, c))
-                 : "memory");
+__device__ __forceinline__ void ld_shared16(uint32_t a, uint32_t (&u)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+               : "r"(a)
+               : "memory");
 }
 // The warp's slab of 32 x 64 values leaves for rows m0 .. of matrix m, columns n0 ..; what lies past the matrix is cut off.
 // `u`: the thread's row. Waits until the slab's previous content is read.
@@ -240,11 +253,22 @@ __device__ __forceinline__ void send_row(const CUtensorMap* m, uint32_t slab, in
   }
 }
 
-template <typename T>
-__device__ __forceinline__ float fits(float x) {  // a finite value stays finite in T
-  if constexpr (std::is_same<T, __half>::value)
-    return fabsf(x) > 65504.f && fabsf(x) < INFINITY ? copysignf(65504.f, x) : x;
-  return x;
+// g and u are kept as the upper 24 of their 32 bits, in three matrices of 16-bit words: the upper halves of g's, of u's, and the
+// next byte of both (g's first). Rounded to 16 bits they would add two roundings to the weights' gradients, which have one of
+// their own and one of dg or du: 1.8 times the error of a float32 form rounded at its end, with 24 bits 1.4 times.
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) {
+  return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+}
+__device__ __forceinline__ uint32_t next_bytes(float g0, float u0, float g1, float u1) {
+  return __byte_perm(__byte_perm(__float_as_uint(g0), __float_as_uint(u0), 0x0051),
+                     __byte_perm(__float_as_uint(g1), __float_as_uint(u1), 0x0051), 0x5410);
+}
+// and back (the byte once more below itself: half of what the cut took away, and an infinity stays one)
+__device__ __forceinline__ void kept_values(uint32_t g, uint32_t u, uint32_t low, float& g0, float& g1, float& u0, float& u1) {
+  g0 = __uint_as_float(__byte_perm(g, low, 0x1044));
+  g1 = __uint_as_float(__byte_perm(g, low, 0x3266));
+  u0 = __uint_as_float(__byte_perm(u, low, 0x1055));
+  u1 = __uint_as_float(__byte_perm(u, low, 0x3277));
 }
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + ex2(-kLog2e * x)); }
 
@@ -269,13 +293,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* slabs = base + C::kStages * kStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(slabs + kEpiWarps * C::kSlabs * kSlab);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(slabs + kEpiWarps * C::kOut);
   uint64_t* full = bars;                 // of the pair: the first CTA's are used
   uint64_t* empty = full + C::kStages;   // each CTA's own
   uint64_t* acc_full = empty + C::kStages;
   uint64_t* acc_empty = acc_full + 2;    // of the pair: the first CTA's are used
   uint64_t* fin = acc_empty + 2;
-  uint64_t* aux = fin + 1;               // each epilogue warp's own loads
+  uint64_t* aux = fin + 1;               // each epilogue warp's own loads, two in turn
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + C::kBarriers);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
@@ -291,7 +315,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       mbar_init(acc_empty + i, 2 * kEpiWarps);
     }
     mbar_init(fin, 1);
-    for (int i = 0; i < kEpiWarps; ++i) mbar_init(aux + i, 1);
+    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(aux + i, 1);
     fence_mbar_init();
   }
   if (warp == 2) {
@@ -307,49 +331,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   const uint32_t s_base = smem_u32(base);
 
   if (warp == 0) {
-    if (lane == 0) {
-      int slot = 0, laps = 0, issued = 0;
-      bool ok = true;
-      for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
-        const Where w = locate<E>(p, tile);
-        const Op& op = p.op[w.op];
-        const int am = w.m + (int)rank * kHalf, bn = E == kSwiglu ? w.n : w.n + (int)rank * kHalf;
-        for (int s = 0; ok && s < 2; ++s) {
-          const CUtensorMap* ma = &op.a[s];
-          const CUtensorMap* mb = E == kSwiglu ? &op.b[rank] : &op.b[s];
-          for (int kb = 0; kb < op.kb[s]; ++kb) {
-            if (laps > 0 && !mbar_wait(empty + slot, (laps - 1) & 1, p.err, 80)) {
-              ok = false;
-              break;
-            }
-            if (rank == 0) mbar_arrive_expect_tx(full + slot, 2 * kStage);
-            const uint32_t bar = in_first_cta(full + slot), a = s_base + slot * kStage, b = a + kOperand;
-            if (op.a_mn) {
-              load_pair(a, ma, am, kb * kBlockK, bar);
-              load_pair(a + kOperand / 2, ma, am + 64, kb * kBlockK, bar);
-            } else {
-              load_pair(a, ma, kb * kBlockK, am, bar);
-            }
-            if (op.b_mn) {
-              load_pair(b, mb, bn, kb * kBlockK, bar);
-              load_pair(b + kOperand / 2, mb, bn + 64, kb * kBlockK, bar);
-            } else {
-              load_pair(b, mb, kb * kBlockK, bn, bar);
-            }
-            ++issued;
-            if (++slot == C::kStages) {
-              slot = 0;
-              ++laps;
-            }
+    // (the whole warp runs this, one elected lane's instructions take effect: addresses and coordinates in uniform registers)
+    const uint32_t lead = elect();
+    int slot = 0, laps = 0, issued = 0;
+    bool ok = true;
+    for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
+      Where w = locate<E>(p, tile);
+      w.op = __shfl_sync(0xffffffffu, w.op, 0);
+      const Op& op = p.op[w.op];
+      const int am = __shfl_sync(0xffffffffu, w.m + (int)rank * kHalf, 0);
+      const int bn = __shfl_sync(0xffffffffu, E == kSwiglu ? w.n : w.n + (int)rank * kHalf, 0);
+      auto segment = [&](auto a_mn, auto b_mn, const CUtensorMap* ma, const CUtensorMap* mb, int n) {
+        for (int kb = 0; kb < n; ++kb) {
+          if (laps > 0 && !(ok = warp_wait(empty + slot, (laps - 1) & 1, p.err, 80))) return;
+          if (rank == 0 && lead) mbar_arrive_expect_tx(full + slot, 2 * kStage);
+          const uint32_t bar = in_first_cta(full + slot), a = s_base + slot * kStage, b = a + kOperand;
+          if (a_mn) {
+            load_pair(lead, a, ma, am, kb * kBlockK, bar);
+            load_pair(lead, a + kOperand / 2, ma, am + 64, kb * kBlockK, bar);
+          } else {
+            load_pair(lead, a, ma, kb * kBlockK, am, bar);
+          }
+          if (b_mn) {
+            load_pair(lead, b, mb, bn, kb * kBlockK, bar);
+            load_pair(lead, b + kOperand / 2, mb, bn + 64, kb * kBlockK, bar);
+          } else {
+            load_pair(lead, b, mb, kb * kBlockK, bn, bar);
+          }
+          ++issued;
+          if (++slot == C::kStages) {
+            slot = 0;
+            ++laps;
           }
         }
+      };
+      using Yes = std::true_type;
+      using No = std::false_type;
+      for (int s = 0; ok && s < 2; ++s) {
+        const CUtensorMap *ma = &op.a[s], *mb = E == kSwiglu ? &op.b[rank] : &op.b[s];
+        const int n = __shfl_sync(0xffffffffu, op.kb[s], 0);
+        if constexpr (E == kStore) {
+          const int layout = __shfl_sync(0xffffffffu, (op.a_mn ? 2 : 0) + (op.b_mn ? 1 : 0), 0);
+          if (layout == 0) segment(No{}, No{}, ma, mb, n);
+          else if (layout == 1) segment(No{}, Yes{}, ma, mb, n);
+          else segment(Yes{}, Yes{}, ma, mb, n);
+        } else {
+          segment(No{}, std::integral_constant<bool, E == kDSwiglu>{}, ma, mb, n);
+        }
       }
-      // The copies in flight land before the CTAs end, whatever became of their readers (they are counted on the first CTA's
-      // barriers; the pair ends together).
-      if (rank == 0)
-        for (int i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
-          mbar_wait(full + i % C::kStages, (i / C::kStages) & 1, p.err, 81);
     }
+    // The copies in flight land before the CTAs end, whatever became of their readers (they are counted on the first CTA's
+    // barriers; the pair ends together).
+    if (rank == 0)
+      for (int i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
+        warp_wait(full + i % C::kStages, (i / C::kStages) & 1, p.err, 81);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t lead = elect();
@@ -361,22 +396,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const int buf = it & 1;
         if (it >= 2 && !(ok = cluster_wait(acc_empty + buf, ((it >> 1) - 1) & 1, p.err, 82))) break;
         tc_fence_after();
-        const uint32_t id = wattn::idesc<T>(256, 256, false) | (op.a_mn ? 1u << 15 : 0u) | (op.b_mn ? 1u << 16 : 0u);
-        const uint32_t a_hi = op.a_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16, b_hi = op.b_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16;
-        const uint32_t a_step = op.a_mn ? 128 : 2, b_step = op.b_mn ? 128 : 2;  // 16 k further, in 16 bytes
+        const int n = __shfl_sync(0xffffffffu, op.kb[0] + op.kb[1], 0);
         const uint32_t d = tm + buf * kTileN;
-        const int n = op.kb[0] + op.kb[1];
-        for (int kb = 0; kb < n; ++kb) {
-          if (!(ok = cluster_wait(full + slot, laps & 1, p.err, 83))) break;
-          tc_fence_after();
-          const uint32_t a = ((s_base + slot * kStage) >> 4) | a_hi, b = ((s_base + slot * kStage + kOperand) >> 4) | b_hi;
+        // The layouts are constants of each loop: descriptors and steps then stay in uniform registers, which the instruction
+        // reads (as variables of the problem they were moved there for every product: 1,250 instead of 1,600 TFLOP/s).
+        auto products = [&](auto a_mn, auto b_mn) {
+          constexpr uint32_t id = wattn::idesc<T>(256, 256, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+          constexpr uint32_t a_hi = a_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16, b_hi = b_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16;
+          constexpr uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;  // 16 k further, in 16 bytes
+          for (int kb = 0; kb < n; ++kb) {
+            if (!(ok = cluster_wait(full + slot, laps & 1, p.err, 83))) break;
+            tc_fence_after();
+            const uint32_t a = ((s_base + slot * kStage) >> 4) | a_hi, b = ((s_base + slot * kStage + kOperand) >> 4) | b_hi;
 #pragma unroll
-          for (int k = 0; k < kBlockK / 16; ++k) mma_pair(lead, d, a + k * a_step, b + k * b_step, id, kb > 0 || k > 0);
-          commit_pair(lead, empty + slot);
-          if (++slot == C::kStages) {
-            slot = 0;
-            ++laps;
+            for (int k = 0; k < kBlockK / 16; ++k) mma_pair(lead, d, a + k * a_step, b + k * b_step, id, kb > 0 || k > 0);
+            commit_pair(lead, empty + slot);
+            if (++slot == C::kStages) {
+              slot = 0;
+              ++laps;
+            }
           }
+        };
+        using Yes = std::true_type;
+        using No = std::false_type;
+        if constexpr (E == kStore) {
+          const int layout = __shfl_sync(0xffffffffu, (op.a_mn ? 2 : 0) + (op.b_mn ? 1 : 0), 0);
+          if (layout == 0) products(No{}, No{});
+          else if (layout == 1) products(No{}, Yes{});
+          else products(Yes{}, Yes{});
+        } else {
+          products(No{}, std::integral_constant<bool, E == kDSwiglu>{});
         }
         if (ok) commit_pair(lead, acc_full + buf);
       }
@@ -386,27 +435,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   } else if (warp >= 4) {
     const int ew = warp - 4, quad = warp & 3, half = ew >> 2;  // a warp reads the TMEM lanes of its quarter
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t slab = smem_u32(slabs) + ew * C::kSlabs * kSlab;
+    const uint32_t slab = smem_u32(slabs) + ew * C::kOut;
     bool ok = true;
-    int it = 0, loads = 0;
+    int it = 0;
+    // kDSwiglu: the kept g and u of 32 columns, a step of four to a tile, into one of two sets of strips, a step ahead of its use
+    int step = 0;
+    auto fetch = [&](int at, const Where& w) {  // step `at` is step at & 3 of w's tile
+      const int n0 = w.n + half * 128 + (at & 3) * 32, m0 = w.m + (int)rank * kHalf + quad * 32;
+      if (m0 >= p.op[0].M || n0 >= p.op[0].N) return;
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t to = slab + (at & 1) * 3 * kStrip;
+        bulk_wait_read0();  // the step before the one that calls this stored from these strips
+        mbar_arrive_expect_tx(aux + 2 * ew + (at & 1), 3 * kStrip);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) load_slab(to + i * kStrip, &p.x[i], n0, m0, aux + 2 * ew + (at & 1));
+      }
+    };
+    if (E == kDSwiglu && pair < p.tiles) fetch(0, locate<E>(p, pair));
+    uint32_t landed = 0;  // kDSwiglu: the phase of each set's barrier (a step past the matrix loads nothing)
     for (int tile = pair; tile < p.tiles; tile += pairs, ++it) {
       const Where w = locate<E>(p, tile);
       const Op& op = p.op[w.op];
       const int buf = it & 1, m0 = w.m + (int)rank * kHalf + quad * 32, row = m0 + lane;
       const uint32_t t0 = tm + lanes + buf * kTileN;
       const bool live = m0 < op.M;  // the warp has rows of the matrix
-      auto fetch = [&](int n0) {    // kDSwiglu: g and u of 64 columns, into the warp's slabs
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          bulk_wait_read0();
-          mbar_arrive_expect_tx(aux + ew, 2 * kSlab);
-          load_slab(slab, &p.x[0], n0, m0, aux + ew);
-          load_slab(slab + kSlab, &p.x[1], n0, m0, aux + ew);
-        }
-      };
       auto has = [&](int n0) { return live && n0 < op.N; };
-      if (E == kDSwiglu && has(w.n + half * 128)) fetch(w.n + half * 128);
       ok = ok && warp_wait(acc_full + buf, (it >> 1) & 1, p.err, 85);
       tc_fence_after();
       const float bad = ok ? 0.f : NAN;  // a wait that gave up leaves NaN
@@ -446,84 +501,102 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           send_row(&op.c, slab, lane, n0, m0, u);
         }
       } else if constexpr (E == kSwiglu) {
-        const int n0 = w.n + half * 64;
-        uint32_t hp[32], gp[32], up[32];
         float top_g = 0.f, top_u = 0.f;
-#pragma unroll
-        for (int c = 0; c < 64; c += 32) {
+#pragma unroll 1
+        for (int s = 0; s < 2; ++s) {
+          const int c = half * 64 + s * 32, n0 = w.n + c;
           float g[32], u[32];
-          tmem_ld32(t0 + half * 64 + c, g);
-          tmem_ld32(t0 + kHalf + half * 64 + c, u);
+          tmem_ld32(t0 + c, g);
+          tmem_ld32(t0 + kHalf + c, u);
+          if (s == 1) release();
+          if (!has(n0)) continue;
+          uint32_t h[16], gh[16], uh[16], low[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float a = g[i] * sigmoid(g[i]) * u[i] + bad, b = g[i + 1] * sigmoid(g[i + 1]) * u[i + 1] + bad;
-            hp[(c + i) / 2] = pack16<T>(a, b);
-            gp[(c + i) / 2] = pack16<T>(fits<T>(g[i]), fits<T>(g[i + 1]));
-            up[(c + i) / 2] = pack16<T>(fits<T>(u[i]), fits<T>(u[i + 1]));
-            if constexpr (std::is_same<T, __half>::value) {
+            h[i / 2] = pack16<T>(g[i] * sigmoid(g[i]) * u[i] + bad, g[i + 1] * sigmoid(g[i + 1]) * u[i + 1] + bad);
+            gh[i / 2] = upper_halves(g[i], g[i + 1]);
+            uh[i / 2] = upper_halves(u[i], u[i + 1]);
+            low[i / 2] = next_bytes(g[i], u[i], g[i + 1], u[i + 1]);
+            if constexpr (std::is_same<T, __half>::value) {  // (zeros past the matrix)
               top_g = wattn::max3(top_g, fabsf(g[i]), fabsf(g[i + 1]));
               top_u = wattn::max3(top_u, fabsf(u[i]), fabsf(u[i + 1]));
             }
           }
-        }
-        release();
-        if (has(n0)) {
-          send_row(&op.c, slab, lane, n0, m0, hp);
+          if (lane == 0) bulk_wait_read0();
+          __syncwarp();
+          put_strip(slab, lane, h);
           if (p.keep) {
-            if constexpr (std::is_same<T, __half>::value) {  // (zeros past the matrix)
-              top_g = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_g)));
-              top_u = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_u)));
-              if (lane == 0) {
-                atomicMax(p.bounds, __float_as_uint(top_g));
-                atomicMax(p.bounds + 1, __float_as_uint(top_u));
-              }
+            put_strip(slab + kStrip, lane, gh);
+            put_strip(slab + 2 * kStrip, lane, uh);
+            put_strip(slab + 3 * kStrip, lane, low);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            store_slab(&op.c, n0, m0, slab);
+            if (p.keep) {
+#pragma unroll
+              for (int i = 0; i < 3; ++i) store_slab(&p.x[i], n0, m0, slab + (i + 1) * kStrip);
             }
-            send_row(&p.x[0], slab, lane, n0, m0, gp);
-            send_row(&p.x[1], slab, lane, n0, m0, up);
+            bulk_commit();
+          }
+        }
+        if constexpr (std::is_same<T, __half>::value) {
+          if (p.keep) {
+            top_g = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_g)));
+            top_u = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_u)));
+            if (lane == 0) {
+              atomicMax(p.bounds, __float_as_uint(top_g));
+              atomicMax(p.bounds + 1, __float_as_uint(top_u));
+            }
           }
         }
       } else if constexpr (E == kDSwiglu) {
         const float f = carried(p.bounds) + bad;
 #pragma unroll 1
-        for (int s = 0; s < 2; ++s) {
-          const int c = half * 128 + s * 64, n0 = w.n + c;
-          if (!has(n0)) {
-            if (s == 1) release();
-            continue;
+        for (int s = 0; s < 4; ++s, ++step) {
+          const int c = half * 128 + s * 32, n0 = w.n + c, set = step & 1;
+          float d[32];
+          tmem_ld32(t0 + c, d);
+          if (s == 3) release();
+          const bool here = has(n0);
+          if (here) {
+            warp_wait(aux + 2 * ew + set, (landed >> set) & 1, p.err, 86);
+            landed ^= 1u << set;
           }
-          if (s == 1) fetch(n0);
-          uint32_t gp[32], up[32], hp[32];
-          warp_wait(aux + ew, loads & 1, p.err, 86);
-          ++loads;
-          get_row(slab, lane, gp);
-          get_row(slab + kSlab, lane, up);
+          if (s < 3) fetch(step + 1, w);
+          else if (tile + pairs < p.tiles) fetch(step + 1, locate<E>(p, tile + pairs));
+          if (!here) continue;
+          const uint32_t strips = slab + set * 3 * kStrip;
 #pragma unroll
-          for (int x = 0; x < 64; x += 32) {
-            float d[32];
-            tmem_ld32(t0 + c + x, d);
+          for (int i = 0; i < 32; i += 8) {  // a chunk of 8 columns of the thread's row, in place
+            const uint32_t at = strips + strip_at(lane, i / 8);
+            uint32_t g[4], u[4], h[4];
+            ld_shared16(at, g);
+            ld_shared16(at + kStrip, u);
+            ld_shared16(at + 2 * kStrip, h);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const int j = (x + i) / 2;
-              const float2 g = unpack16<T>(gp[j]), u = unpack16<T>(up[j]);
-              const float s0 = sigmoid(g.x), s1 = sigmoid(g.y), a0 = g.x * s0, a1 = g.y * s1;
-              const float d0 = d[i] * f, d1 = d[i + 1] * f;
-              hp[j] = pack16<T>(a0 * u.x, a1 * u.y);
-              gp[j] = pack16<T>(d0 * u.x * (s0 + a0 * (1.f - s0)), d1 * u.y * (s1 + a1 * (1.f - s1)));
-              up[j] = pack16<T>(d0 * a0, d1 * a1);
+            for (int j = 0; j < 4; ++j) {
+              float g0, g1, u0, u1;
+              kept_values(g[j], u[j], h[j], g0, g1, u0, u1);
+              const float s0 = sigmoid(g0), s1 = sigmoid(g1), a0 = g0 * s0, a1 = g1 * s1;
+              const float d0 = d[i + 2 * j] * f, d1 = d[i + 2 * j + 1] * f;
+              h[j] = pack16<T>(a0 * u0, a1 * u1);
+              g[j] = pack16<T>(d0 * u0 * (s0 + a0 * (1.f - s0)), d1 * u1 * (s1 + a1 * (1.f - s1)));
+              u[j] = pack16<T>(d0 * a0, d1 * a1);
             }
+            st_shared16(at, g);
+            st_shared16(at + kStrip, u);
+            st_shared16(at + 2 * kStrip, h);
           }
-          if (s == 1) release();
-          __syncwarp();  // g and u are read
-          put_row(slab, lane, gp);
-          put_row(slab + kSlab, lane, up);
           fence_async_smem();
           __syncwarp();
           if (lane == 0) {
-            store_slab(&op.c, n0, m0, slab);
-            store_slab(&p.y, n0, m0, slab + kSlab);
+            store_slab(&op.c, n0, m0, strips);
+            store_slab(&p.y[0], n0, m0, strips + kStrip);
+            if (p.keep) store_slab(&p.y[1], n0, m0, strips + 2 * kStrip);
             bulk_commit();
           }
-          if (p.keep) send_row(&p.x[2], slab, lane, n0, m0, hp);
         }
       } else if constexpr (E == kLse) {
         const long long lab = row < op.M ? label_of(p, row) - p.v0 : -1;

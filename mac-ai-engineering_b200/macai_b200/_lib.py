@@ -73,8 +73,8 @@ _SIGS = {
     "gd_wattn_step_workspace_bytes": ([_I] * 7, _SZ),
     "gd_wattn_step": ([_P] * 7 + [_I] * 6 + [ctypes.POINTER(_LL), _I, _I, ctypes.c_float, _P, _SZ, _P], _I),
     "gd_ff_workspace_bytes": ([_LL] + [_I] * 4, _SZ),
-    "gd_ff_fwd": ([_P] * 8 + [_I, _LL, _I, _I, _I, ctypes.POINTER(_LL), _P, _SZ, _P], _I),
-    "gd_ff_bwd": ([_P] * 12 + [_I, _LL, _I, _I, _I, ctypes.POINTER(_LL), _P, _SZ, _P], _I),
+    "gd_ff_fwd": ([_P] * 7 + [_I, _LL, _I, _I, _I, ctypes.POINTER(_LL), _P, _SZ, _P], _I),
+    "gd_ff_bwd": ([_P] * 11 + [_I, _LL, _I, _I, _I, ctypes.POINTER(_LL), _P, _SZ, _P], _I),
     "gd_xent_workspace_bytes": ([_LL] + [_I] * 3, _SZ),
     "gd_xent_fwd": ([_P] * 3 + [_I, _P, _P, _I, _LL, _I, _LL, _I, _I, _LL, _LL, _P, _SZ, _P], _I),
     "gd_xent_bwd": ([_P] * 3 + [_I] + [_P] * 4 + [_I, _LL, _I, _LL, _I, _I, _LL, _LL, _P, _SZ, _P], _I),

@@ -5,8 +5,8 @@ after its mixer:
 
 `gated_feed_forward` trains, prefills, and takes the few tokens of a decoding step. tcgen05 products with float32 sums; the
 activation and its gradient are taken in float32 as the products leave the tensor core, so neither g nor u is read again in
-the forward, and the gradient of h never leaves the chip. h, and for the backward g, u and their gradients, are rounded to the
-inputs' 16-bit type (the matrix instruction's operands). bfloat16 and float16. There is no CPU path: CUDA tensors only.
+the forward, and the gradient of h never leaves the chip. h and the gradients of g and u are rounded to the inputs' 16-bit type
+(the matrix instruction's operands); g and u are kept for the backward in 24 bits. bfloat16 and float16. There is no CPU path: CUDA tensors only.
 """
 from __future__ import annotations
 
@@ -38,30 +38,30 @@ def _sizes(x, wg, wd):
 
 
 def _fwd(x, wg, wu, wd, keep):
-    """(y, g, u, bounds) on matrices; keep: g, u (and float16's bounds) for the backward, else None."""
+    """(y, kept, bounds) on matrices; keep: 24 bits of g and u (and float16's bounds) for the backward, else None."""
     n, D, F, O = _sizes(x, wg, wd)
     y = torch.empty((n, O), dtype=x.dtype, device=x.device)
-    g = u = bounds = None
+    kept = bounds = None
     if keep:
-        g, u = (torch.empty((n, F), dtype=x.dtype, device=x.device) for _ in range(2))
+        kept = torch.empty((3, n, F), dtype=torch.int16, device=x.device)
         if x.dtype == torch.float16:
             bounds = torch.empty(4, dtype=torch.int32, device=x.device)
     size = _bytes(n, D, F, O, 0)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    launch("gd_ff_fwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), p(g), p(u), p(bounds),
+    launch("gd_ff_fwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), p(kept), p(bounds),
            y.data_ptr(), _DTYPES[x.dtype], n, D, F, O, _pitches(x, wg, wu, wd), ws.data_ptr(), size)
-    return y, g, u, bounds
+    return y, kept, bounds
 
 
-def _bwd(x, wg, wu, wd, g, u, bounds, dy, need):
+def _bwd(x, wg, wu, wd, kept, bounds, dy, need):
     """(dx, dw_gate, dw_up, dw_down), contiguous, each None unless needed."""
     n, D, F, O = _sizes(x, wg, wd)
     make = lambda yes, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if yes else None  # noqa: E731
     out = (make(need[0], n, D), make(need[1], F, D), make(need[2], F, D), make(need[3], O, F))
     size = _bytes(n, D, F, O, 1)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    launch("gd_ff_bwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), g.data_ptr(), u.data_ptr(),
+    launch("gd_ff_bwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), kept.data_ptr(),
            None if bounds is None else bounds.data_ptr(), dy.data_ptr(), *(None if t is None else t.data_ptr() for t in out),
            _DTYPES[x.dtype], n, D, F, O, _pitches(x, wg, wu, wd, dy), ws.data_ptr(), size)
     return out
@@ -72,8 +72,8 @@ class GatedFeedForward(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, wg, wu, wd):
-        y, g, u, bounds = _fwd(x, wg, wu, wd, True)
-        ctx.save_for_backward(x, wg, wu, wd, g, u, bounds)
+        y, kept, bounds = _fwd(x, wg, wu, wd, True)
+        ctx.save_for_backward(x, wg, wu, wd, kept, bounds)
         return y
 
     @staticmethod
