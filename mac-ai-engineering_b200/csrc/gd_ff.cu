@@ -1,6 +1,7 @@
 // The gated feed-forward block:  h = silu(x Wg^T) * (x Wu^T),  y = h Wd^T,  and its gradients.
 #include <cstdint>
 
+#include "gd_ff.cuh"
 #include "gd_gemm.cuh"
 
 namespace gd {
@@ -9,12 +10,6 @@ namespace {
 
 using gemm::Op;
 using gemm::Params;
-
-struct Problem {
-  const void *x, *wg, *wu, *wd;
-  long long ldx, ldg, ldu, ldd;
-  int rows, D, F, O;
-};
 
 // max over dy's rows of the sum of absolute values, max |w_down|, as float bits (float16 only; both 8 columns at a time)
 __global__ void __launch_bounds__(256) bounds_kernel(const __half* __restrict__ dy, long long ldy, int rows, int O,
@@ -185,11 +180,12 @@ extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, co
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   gd::ErrorWord* err = static_cast<gd::ErrorWord*>(workspace);
+  const Problem q = {x, w_gate, w_up, w_down, ld[0], ld[1], ld[2], ld[3], (int)rows, D, F, O};
+  void* h = static_cast<char*>(workspace) + kHead;
+  if (kept == nullptr && rows <= kFew) return forward_few(q, dtype, h, y, cs);
   if (cudaMemsetAsync(err, 0, sizeof(*err), cs) != cudaSuccess ||
       (dtype == GD_FLOAT16 && bounds != nullptr && cudaMemsetAsync(bounds, 0, 16, cs) != cudaSuccess))
     return (cudaGetLastError(), GD_ERR_LAUNCH);
-  const Problem q = {x, w_gate, w_up, w_down, ld[0], ld[1], ld[2], ld[3], (int)rows, D, F, O};
-  void* h = static_cast<char*>(workspace) + kHead;
   void* planes[3];
   for (int i = 0; i < 3; ++i) planes[i] = kept == nullptr ? nullptr : static_cast<char*>(kept) + i * (size_t)rows * F * 2;
   return dtype == GD_FLOAT16 ? forward<__half>(q, planes, h, y, bounds, err, cs)

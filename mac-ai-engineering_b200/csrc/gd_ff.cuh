@@ -1,0 +1,20 @@
+// The gated feed-forward block's sizes and parts (host).
+#pragma once
+
+#include <cuda_runtime.h>
+
+namespace gd {
+namespace ff {
+
+struct Problem {
+  const void *x, *wg, *wu, *wd;
+  long long ldx, ldg, ldu, ldd;  // elements from row to row
+  int rows, D, F, O;
+};
+
+// y for at most kFew rows, h [rows, F] on the way (gd_ff_few.cu)
+constexpr int kFew = 128;
+int forward_few(const Problem& q, int dtype, void* h, void* y, cudaStream_t stream);
+
+}  // namespace ff
+}  // namespace gd
