@@ -2,7 +2,7 @@
 //   first kernel:  h = silu(x Wg^T) * (x Wu^T)        second:  y = h Wd^T
 // Bound by the weights' bytes, 6 D F for a call. The weights are the M side of the products (a tile of 128 of their rows; in the
 // first kernel 64 of w_gate's and the same 64 of w_up's), the tokens the N side (16 to 128, zeros past the last), so a tile's
-// weights pass through a CTA once, by TMA through a ring of stages that keeps 64 to 100 KB a CTA on the way. The contraction is
+// weights pass through a CTA once, by TMA through a ring of stages, three CTAs an SM. The contraction is
 // split over a cluster of CTAs: few tiles still put bytes in flight on every SM, and all CTAs run at once, where memory, not their
 // share of the SMs, decides when they end. Their partial products are added in shared memory of the cluster, in a fixed order.
 // The second kernel starts while the first one ends (programmatic launch): its ring fills with weights before h is waited for.
@@ -26,10 +26,12 @@ struct FewParams {
 template <int N>
 struct FewCfg {
   static constexpr int kW = kRowsM * 128, kT = N * 128;  // bytes of a stage: weights, tokens
-  static constexpr int kStages = N <= 32 ? 5 : N == 64 ? 4 : 3;
+  // three CTAs an SM: at 16 tokens, 4,096 x 12,288 four stages take 53 us, five (two CTAs an SM) 58 us, three 55 us
+  static constexpr int kStages = N == 16 ? 4 : N <= 64 ? 3 : 2;
   static constexpr int kRing = kStages * (kW + kT);
   static constexpr int kPart = N * kRowsM * 4;           // a CTA's partial products (in the ring's place)
   static_assert(kPart <= kRing, "partial products");
+  static_assert(3 * (kRing + 2304) <= 227 * 1024, "three CTAs an SM");
   static constexpr size_t kSmem = 1024 + kRing + 8 * (2 * kStages + 1) + 16;
   static constexpr int kCols = N < 32 ? 32 : N;          // TMEM columns
 };
@@ -168,11 +170,14 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ F
   gemm::cluster_sync();  // the parts are read
 }
 
-// CTAs of a cluster: enough for about two CTAs an SM, none with less than two stages.
+// CTAs of a cluster: as many as still run all at once, three on each of 148 SMs (memory then works at its rate whatever the
+// SMs' shares are), none with less than four stages. At 4 tokens, 2,048 x 6,144 that is four (20 us; a fifth, and with it a
+// second turn of CTAs: 23 us; one CTA an SM: 23 us), at 64 tokens, 4,096 x 12,288 two (60 us; one: 66, four: 69 us); at
+// 1 token, 1,024 x 2,816 the least length holds (9.6 us; two stages: 11 us).
 int split_of(int tiles, int blocks) {
-  int s = (2 * 148 + tiles / 2) / tiles;
+  int s = 3 * 148 / tiles;
   if (s > 8) s = 8;
-  if (s > blocks / 2) s = blocks / 2;
+  if (s > blocks / 4) s = blocks / 4;
   return s < 1 ? 1 : s;
 }
 

@@ -22,47 +22,57 @@ _DTYPES = {torch.float32: _lib.GD_FLOAT32, torch.float16: _lib.GD_FLOAT16, torch
 MAX_WIDTH = 256
 
 
-def _inputs(name, q, k, v, g, beta):
-    """(q, k, v, g, beta, sizes) as the kernel reads them; raises for what it does not take."""
+def _refuse(name, q, k, v, g, beta):
+    """The error for inputs that `_inputs` does not take."""
     for x, t in (("query", q), ("key", k), ("value", v)):
         if not isinstance(t, torch.Tensor) or t.dim() != 4:
-            raise ValueError(f"{name}: {x} must be [B, T, heads, width]")
+            return ValueError(f"{name}: {x} must be [B, T, heads, width]")
     if q.dtype not in _DTYPES:
-        raise TypeError(f"{name}: float32, float16 or bfloat16, got {q.dtype}")
+        return TypeError(f"{name}: float32, float16 or bfloat16, got {q.dtype}")
     if not q.is_cuda:
-        raise RuntimeError(f"{name}: CUDA tensors only (there is no CPU path)")
+        return RuntimeError(f"{name}: CUDA tensors only (there is no CPU path)")
     B, T, HK, DK = q.shape
     H, DV = v.shape[2], v.shape[3]
     if k.shape != q.shape or v.shape[:2] != q.shape[:2]:
-        raise ValueError(f"{name}: query and key [B, T, HK, DK] and value [B, T, H, DV] must agree; got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+        return ValueError(f"{name}: query and key [B, T, HK, DK] and value [B, T, H, DV] must agree; got {tuple(q.shape)}, "
+                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     if H == 0 or HK == 0 or H % HK:
-        raise ValueError(f"{name}: value heads ({H}) must be a multiple of key heads ({HK})")
+        return ValueError(f"{name}: value heads ({H}) must be a multiple of key heads ({HK})")
     if DK == 0 or DV == 0 or DK % 32 or DV % 32:
-        raise ValueError(f"{name}: head widths must be multiples of 32; got DK={DK}, DV={DV}")
+        return ValueError(f"{name}: head widths must be multiples of 32; got DK={DK}, DV={DV}")
     if DK > MAX_WIDTH or DV > MAX_WIDTH:
-        raise NotImplementedError(f"{name}: head widths go up to {MAX_WIDTH}; got DK={DK}, DV={DV}")
+        return NotImplementedError(f"{name}: head widths go up to {MAX_WIDTH}; got DK={DK}, DV={DV}")
     if B > 65535:
-        raise NotImplementedError(f"{name}: at most 65,535 requests a call, got {B}")
+        return NotImplementedError(f"{name}: at most 65,535 requests a call, got {B}")
     for x, t in (("g", g), ("beta", beta)):
         if not isinstance(t, torch.Tensor) or t.shape != (B, T, H):
-            raise ValueError(f"{name}: {x} must be [B, T, H] = {(B, T, H)}")
-    if any(t.get_device() != q.get_device() for t in (k, v, g, beta)):
-        raise ValueError(f"{name}: the inputs must be on one device")
-    if v.dtype not in (q.dtype, torch.float32):
-        v = v.to(q.dtype)
-    return (q.contiguous(), k.to(q.dtype).contiguous(), v.contiguous(), g.float().contiguous(), beta.float().contiguous(),
-            (B, T, H, HK, DK, DV))
+            return ValueError(f"{name}: {x} must be [B, T, H] = {(B, T, H)}")
+    return ValueError(f"{name}: the inputs must be on one device")
 
 
-def _run(q, k, v, g, beta, sizes, s_in, s_out, slots, out_slots, n_slots, l2norm):
-    B, T, H, _, _, DV = sizes
-    o = torch.empty((B, T, H, DV), dtype=q.dtype, device=q.device)
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    launch("gd_rule_step", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), p(s_in),
-           p(s_out), p(slots), p(out_slots), o.data_ptr(), _DTYPES[q.dtype], _DTYPES[v.dtype], *sizes, n_slots,
-           _lib.GD_L2NORM if l2norm else 0)
-    return o
+def _inputs(name, q, k, v, g, beta):
+    """(q, k, v, g, beta, B, T, H, HK, DK, DV) as the kernel reads them; raises for what it does not take."""
+    try:
+        B, T, HK, DK = q.shape
+        _, _, H, DV = v.shape
+        row, index, dt = (B, T, H), q.get_device(), q.dtype
+        ok = (q.is_cuda and dt in _DTYPES and k.shape == q.shape and v.shape[:2] == q.shape[:2] and g.shape == row
+              and beta.shape == row and HK > 0 and H > 0 and H % HK == 0 and 0 < DK <= MAX_WIDTH and 0 < DV <= MAX_WIDTH
+              and DK % 32 == 0 and DV % 32 == 0 and B <= 65535 and k.get_device() == index and v.get_device() == index
+              and g.get_device() == index and beta.get_device() == index)
+    except (AttributeError, ValueError):
+        ok = False
+    if not ok:
+        raise _refuse(name, q, k, v, g, beta)
+    if k.dtype != dt:
+        k = k.to(dt)
+    if v.dtype != dt and v.dtype != torch.float32:
+        v = v.to(dt)
+    if g.dtype != torch.float32:
+        g = g.float()
+    if beta.dtype != torch.float32:
+        beta = beta.float()
+    return aligned(q), aligned(k), aligned(v), g.contiguous(), beta.contiguous(), B, T, H, HK, DK, DV
 
 
 def gated_delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -79,8 +89,7 @@ def gated_delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     not have, or whose written slot another request of the call reads or writes, gets NaN. Neither of them changes a state.
     No gradient. Nothing waits for the host."""
     name = "gated_delta_step"
-    q, k, v, g_, beta_, sizes = _inputs(name, query, key, value, g, beta)
-    B, _, H, _, DK, DV = sizes
+    q, k, v, g_, beta_, B, T, H, HK, DK, DV = _inputs(name, query, key, value, g, beta)
     index = q.get_device()
     if not isinstance(state, torch.Tensor) or state.dim() != 4 or state.shape[1:] != (H, DK, DV):
         raise ValueError(f"{name}: state must be [S, H, DK, DV] with (H, DK, DV) = {(H, DK, DV)}")
@@ -89,16 +98,19 @@ def gated_delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
                          "written in place)")
     if slots is None and out_slots is not None:
         raise ValueError(f"{name}: out_slots needs slots")
-    for x, t in (("slots", slots), ("out_slots", out_slots)):
+    for t in (slots, out_slots):
         if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != (B,)
                               or t.get_device() != index or not t.is_contiguous()):
-            raise ValueError(f"{name}: {x} must be a contiguous int32 [B] on the query's device")
+            raise ValueError(f"{name}: slots and out_slots must be contiguous int32 [B] on the query's device")
     if slots is None and state.shape[0] < B:
         raise ValueError(f"{name}: {B} requests need as many slots, the pool has {state.shape[0]}")
     if recorded(query, key, value, g, beta, state):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train with chunk_gated_delta_rule")
-    o = _run(q, k, v, g_, beta_, sizes, state, state, slots, slots if out_slots is None else out_slots, state.shape[0],
-             use_qk_l2norm_in_kernel)
+    o = torch.empty((B, T, H, DV), dtype=q.dtype, device=q.device)
+    pool, at = state.data_ptr(), None if slots is None else slots.data_ptr()
+    launch("gd_rule_step", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), g_.data_ptr(), beta_.data_ptr(), pool, pool, at,
+           at if out_slots is None else out_slots.data_ptr(), o.data_ptr(), _DTYPES[q.dtype], _DTYPES[v.dtype], B, T, H, HK,
+           DK, DV, state.shape[0], _lib.GD_L2NORM if use_qk_l2norm_in_kernel else 0)
     increment_version(state)  # written through its pointer: autograd sees that a saved one has changed
     return o
 
@@ -111,8 +123,7 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, o
     name = "recurrent_gated_delta_rule"
     if kwargs.get("cu_seqlens") is not None:
         raise NotImplementedError(f"{name}: packed rows run through chunk_gated_delta_rule")
-    q, k, v, g_, beta_, sizes = _inputs(name, query, key, value, g, beta)
-    B, _, H, _, DK, DV = sizes
+    q, k, v, g_, beta_, B, T, H, HK, DK, DV = _inputs(name, query, key, value, g, beta)
     if recorded(query, key, value, g, beta, initial_state):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train with chunk_gated_delta_rule")
     s0 = None
@@ -121,4 +132,8 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, o
             raise ValueError(f"{name}: initial_state must be [B, H, DK, DV] = {(B, H, DK, DV)} on the query's device")
         s0 = aligned(initial_state.float())
     sT = torch.empty((B, H, DK, DV), dtype=torch.float32, device=q.device) if output_final_state else None
-    return _run(q, k, v, g_, beta_, sizes, s0, sT, None, None, B, use_qk_l2norm_in_kernel), sT
+    o = torch.empty((B, T, H, DV), dtype=q.dtype, device=q.device)
+    launch("gd_rule_step", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), g_.data_ptr(), beta_.data_ptr(),
+           None if s0 is None else s0.data_ptr(), None if sT is None else sT.data_ptr(), None, None, o.data_ptr(),
+           _DTYPES[q.dtype], _DTYPES[v.dtype], B, T, H, HK, DK, DV, B, _lib.GD_L2NORM if use_qk_l2norm_in_kernel else 0)
+    return o, sT
