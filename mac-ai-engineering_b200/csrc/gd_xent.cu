@@ -103,10 +103,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __r
   }
 }
 
-// Each row's factor g_i F and 1 / F. F is the power of two that brings float16's largest |g_i| to 2^14 .. 2^15, so that D keeps
-// its 11 bits over 28 binades below its largest value; 1 for bfloat16. One CTA.
+// What each row's softmax - onehot is multiplied by before it is rounded, and what the products are multiplied by: g_i over the
+// largest |g| of the call, and that. A row that knows nothing of its label then has -1 exactly where it would have the rounded
+// -g_i, an error all rows of a mean share (up to 2^-8 of both gradients). float16 carries 2^15 more, so that D keeps its 11 bits
+// over 28 binades below its largest value. One CTA.
 __global__ void __launch_bounds__(1024) factors_kernel(const float* __restrict__ g, Labels lab, int n, int reduction, bool half,
-                                                       float* __restrict__ row_scale, float* __restrict__ inv) {
+                                                       float* __restrict__ row_scale, float* __restrict__ factor) {
   __shared__ float sh[32];
   __shared__ float share;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -123,39 +125,31 @@ __global__ void __launch_bounds__(1024) factors_kernel(const float* __restrict__
     __syncthreads();
     return share;
   };
-  float one = 0.f;
+  float one = 0.f, top = 0.f;
   if (reduction != kNone) {
-    one = g[0];
-    if (reduction == kMean) {
-      float c = 0.f;  // (whole numbers up to 2^24: exact)
-      for (int i = threadIdx.x; i < n; i += 1024) c += lab.of(i) != lab.ignore ? 1.f : 0.f;
-      one = one / all(c, true);
-    }
-  }
-  float F = 1.f;
-  if (half) {
-    float top = 0.f;
-    if (reduction != kNone) top = fabsf(one);
-    else
-      for (int i = threadIdx.x; i < n; i += 1024)
-        if (lab.of(i) != lab.ignore) top = wattn::max3(top, fabsf(g[i]), top);
+    float c = 0.f;  // (whole numbers up to 2^24: exact)
+    for (int i = threadIdx.x; i < n; i += 1024) c += lab.of(i) != lab.ignore ? 1.f : 0.f;
+    c = all(c, true);
+    one = reduction == kMean ? g[0] / c : g[0];
+    top = c > 0.f ? fabsf(one) : 0.f;
+  } else {
+    for (int i = threadIdx.x; i < n; i += 1024)
+      if (lab.of(i) != lab.ignore) top = wattn::max3(top, fabsf(g[i]), top);
     top = all(top, false);
-    if (top > 0.f && top < INFINITY) {
-      const int e = 14 - ilogbf(top);
-      F = ldexpf(1.f, e > 120 ? 120 : e < -120 ? -120 : e);
-    }
   }
-  if (threadIdx.x == 0) *inv = 1.f / F;
+  const float lift = half ? 32768.f : 1.f;
+  const bool plain = !(top < INFINITY);  // an infinity or NaN goes the way it came
+  if (threadIdx.x == 0) *factor = plain ? 1.f : top / lift;
   for (int i = threadIdx.x; i < n; i += 1024) {
     const long long l = lab.of(i);
-    const float x = (reduction == kNone ? g[i] : one) * F;
-    row_scale[i] = l == lab.ignore ? 0.f : l < 0 || l >= lab.V ? NAN : x;
+    const float x = reduction == kNone ? g[i] : one;
+    row_scale[i] = l == lab.ignore ? 0.f : l < 0 || l >= lab.V ? NAN : plain ? x : top > 0.f ? x / top * lift : 0.f;
   }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-constexpr size_t kHead = 256;  // the error word, the join's counter (at 64), 1 / F (at 128)
+constexpr size_t kHead = 256;  // the error word, the join's counter (at 64), the products' factor (at 128)
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 struct FwdPlan {
@@ -240,8 +234,8 @@ int backward(const Problem& q, const float* lse2, const float* dloss, void* dx, 
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const BwdPlan b = bwd_plan(q.n, q.D, q.V);
   float* const row_scale = reinterpret_cast<float*>(ws + b.rows);
-  float* const inv = reinterpret_cast<float*>(ws + 128);
-  factors_kernel<<<1, 1024, 0, stream>>>(dloss, q.lab, q.n, q.reduction, std::is_same<T, __half>::value, row_scale, inv);
+  float* const factor = reinterpret_cast<float*>(ws + 128);
+  factors_kernel<<<1, 1024, 0, stream>>>(dloss, q.lab, q.n, q.reduction, std::is_same<T, __half>::value, row_scale, factor);
   if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   void* const d = ws + b.d;
   const int kd = gemm::blocks_of(q.D, gemm::kBlockK);
@@ -270,7 +264,7 @@ int backward(const Problem& q, const float* lse2, const float* dloss, void* dx, 
       g.b_mn = true;
       g.sum_mode = b.pieces == 1 ? 0 : i == 0 ? 1 : i + 1 < b.pieces ? 2 : 3;
       g.sum = reinterpret_cast<float*>(ws + b.sum);
-      g.factor = inv;
+      g.factor = factor;
       ok = ok && gemm::operand_map(&g.a[0], d, dt, q.n, cols, b.ldd, false) &&
            gemm::operand_map(&g.b[0], w, dt, cols, q.D, q.ldw, true) && gemm::slab_map(&g.c, dx, dt, q.n, q.D, q.D);
     }
@@ -279,7 +273,7 @@ int backward(const Problem& q, const float* lse2, const float* dloss, void* dx, 
       shape(g, cols, q.D);
       g.kb[0] = gemm::blocks_of(q.n, gemm::kBlockK);
       g.a_mn = g.b_mn = true;
-      g.factor = inv;
+      g.factor = factor;
       ok = ok && gemm::operand_map(&g.a[0], d, dt, q.n, cols, b.ldd, true) &&
            gemm::operand_map(&g.b[0], q.x, dt, q.n, q.D, q.ldx, true) &&
            gemm::slab_map(&g.c, static_cast<char*>(dw) + v0 * q.D * 2, dt, cols, q.D, q.D);
