@@ -364,7 +364,7 @@ int gd_rule_step(const void* q, const void* k, const void* v, const float* g, co
  * Replaces: the SwiGLU part and the three projections around it (src/macai/layer/_swiglu.py:41-45). */
 size_t gd_ff_workspace_bytes(long long rows, int D, int F, int O, int for_backward);
 
-/* kept [3, rows, F] 16-bit words: the upper 24 bits of g's and u's float32 values (the upper halves of g's, of u's, the next
+/* kept [3, rows, F rounded up to a multiple of 64] 16-bit words: the upper 24 bits of g's and u's float32 values (the upper halves of g's, of u's, the next
  * byte of both), for the backward; or NULL. bounds (GD_FLOAT16 with kept; 16 bytes): max |g| and max |u|, for the backward;
  * else NULL. */
 int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* kept, unsigned int* bounds,

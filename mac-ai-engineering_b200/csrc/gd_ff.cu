@@ -57,8 +57,8 @@ int forward(const Problem& q, void* const* kept, void* h, void* y, uint32_t* bou
   o.kb[0] = gemm::blocks_of(q.D, gemm::kBlockK);
   bool ok = gemm::operand_map(&o.a[0], q.x, dt, n, q.D, q.ldx, false) &&
             gemm::operand_map(&o.b[0], q.wg, dt, q.F, q.D, q.ldg, false) &&
-            gemm::operand_map(&o.b[1], q.wu, dt, q.F, q.D, q.ldu, false) && gemm::strip_map(&o.c, h, dt, n, q.F, q.F);
-  for (int i = 0; p.keep && i < 3; ++i) ok = ok && gemm::strip_map(&p.x[i], kept[i], dt, n, q.F, q.F);
+            gemm::operand_map(&o.b[1], q.wu, dt, q.F, q.D, q.ldu, false) && gemm::strip_map(&o.c, h, dt, n, q.F, pitch(q.F));
+  for (int i = 0; p.keep && i < 3; ++i) ok = ok && gemm::strip_map(&p.x[i], kept[i], dt, n, q.F, pitch(q.F));
   if (!ok) return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kSwiglu>(p, stream)) return st;
   Params r = {};
@@ -66,7 +66,7 @@ int forward(const Problem& q, void* const* kept, void* h, void* y, uint32_t* bou
   Op& d = r.op[0];
   shape(d, n, q.O);
   d.kb[0] = gemm::blocks_of(q.F, gemm::kBlockK);
-  if (!gemm::operand_map(&d.a[0], h, dt, n, q.F, q.F, false) || !gemm::operand_map(&d.b[0], q.wd, dt, q.O, q.F, q.ldd, false) ||
+  if (!gemm::operand_map(&d.a[0], h, dt, n, q.F, pitch(q.F), false) || !gemm::operand_map(&d.b[0], q.wd, dt, q.O, q.F, q.ldd, false) ||
       !gemm::slab_map(&d.c, y, dt, n, q.O, q.O))
     return GD_ERR_LAUNCH;
   return gemm::launch<T, gemm::kStore>(r, stream);
@@ -80,7 +80,7 @@ template <typename T>
 int backward(const Problem& q, const void* const* kept, const void* dy, long long ldy, const Grads& out, void* dg, void* du,
              void* h, uint32_t* bounds, ErrorWord* err, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
-  const long long n = q.rows;
+  const long long n = q.rows, lf = pitch(q.F);
   if (bounds != nullptr) {
     const int rows = q.rows + q.O;
     bounds_kernel<<<rows < 8 * 592 ? (rows + 7) / 8 : 592, 256, 0, stream>>>(
@@ -94,11 +94,11 @@ int backward(const Problem& q, const void* const* kept, const void* dy, long lon
   o.kb[0] = gemm::blocks_of(q.O, gemm::kBlockK);
   o.b_mn = true;
   if (!gemm::operand_map(&o.a[0], dy, dt, n, q.O, ldy, false) || !gemm::operand_map(&o.b[0], q.wd, dt, q.O, q.F, q.ldd, true) ||
-      !gemm::strip_map(&o.c, dg, dt, n, q.F, q.F) || !gemm::strip_map(&p.y[0], du, dt, n, q.F, q.F) ||
-      (p.keep && !gemm::strip_map(&p.y[1], h, dt, n, q.F, q.F)))
+      !gemm::strip_map(&o.c, dg, dt, n, q.F, lf) || !gemm::strip_map(&p.y[0], du, dt, n, q.F, lf) ||
+      (p.keep && !gemm::strip_map(&p.y[1], h, dt, n, q.F, lf)))
     return GD_ERR_LAUNCH;
   for (int i = 0; i < 3; ++i)
-    if (!gemm::strip_map(&p.x[i], kept[i], dt, n, q.F, q.F)) return GD_ERR_LAUNCH;
+    if (!gemm::strip_map(&p.x[i], kept[i], dt, n, q.F, lf)) return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kDSwiglu>(p, stream)) return st;
   Params r = {};
   r.err = err, r.bounds = bounds;
@@ -112,15 +112,15 @@ int backward(const Problem& q, const void* const* kept, const void* dy, long lon
     ok = ok && gemm::operand_map(&w.a[0], a, dt, n, M, lda, true) && gemm::operand_map(&w.b[0], b, dt, n, N, ldb, true) &&
          gemm::slab_map(&w.c, dw, dt, M, N, N);
   };
-  weight(out.dwg, dg, q.F, q.F, q.x, q.ldx, q.D, true);
-  weight(out.dwu, du, q.F, q.F, q.x, q.ldx, q.D, true);
-  weight(out.dwd, dy, ldy, q.O, h, q.F, q.F, false);
+  weight(out.dwg, dg, lf, q.F, q.x, q.ldx, q.D, true);
+  weight(out.dwu, du, lf, q.F, q.x, q.ldx, q.D, true);
+  weight(out.dwd, dy, ldy, q.O, h, lf, q.F, false);
   if (out.dx != nullptr) {
     Op& w = r.op[r.ops++];
     shape(w, n, q.D);  // dx = dg Wg + du Wu
     w.kb[0] = w.kb[1] = gemm::blocks_of(q.F, gemm::kBlockK);
     w.b_mn = true, w.unscale = true;
-    ok = ok && gemm::operand_map(&w.a[0], dg, dt, n, q.F, q.F, false) && gemm::operand_map(&w.a[1], du, dt, n, q.F, q.F, false) &&
+    ok = ok && gemm::operand_map(&w.a[0], dg, dt, n, q.F, lf, false) && gemm::operand_map(&w.a[1], du, dt, n, q.F, lf, false) &&
          gemm::operand_map(&w.b[0], q.wg, dt, q.F, q.D, q.ldg, true) &&
          gemm::operand_map(&w.b[1], q.wu, dt, q.F, q.D, q.ldu, true) && gemm::slab_map(&w.c, out.dx, dt, n, q.D, q.D);
   }
@@ -130,7 +130,7 @@ int backward(const Problem& q, const void* const* kept, const void* dy, long lon
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 constexpr size_t kHead = 256;  // the error word
-size_t matrix_bytes(long long rows, int F) { return ((size_t)rows * F * 2 + 255) / 256 * 256; }
+size_t matrix_bytes(long long rows, int F) { return ((size_t)rows * pitch(F) * 2 + 255) / 256 * 256; }
 
 int check(int dtype, long long rows, int D, int F, int O, const long long* ld, int n_ld) {
   if (dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) return GD_ERR_ARG;
@@ -187,7 +187,7 @@ extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, co
       (dtype == GD_FLOAT16 && bounds != nullptr && cudaMemsetAsync(bounds, 0, 16, cs) != cudaSuccess))
     return (cudaGetLastError(), GD_ERR_LAUNCH);
   void* planes[3];
-  for (int i = 0; i < 3; ++i) planes[i] = kept == nullptr ? nullptr : static_cast<char*>(kept) + i * (size_t)rows * F * 2;
+  for (int i = 0; i < 3; ++i) planes[i] = kept == nullptr ? nullptr : static_cast<char*>(kept) + i * (size_t)rows * pitch(F) * 2;
   return dtype == GD_FLOAT16 ? forward<__half>(q, planes, h, y, bounds, err, cs)
                              : forward<__nv_bfloat16>(q, planes, h, y, nullptr, err, cs);
 }
@@ -228,7 +228,7 @@ extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, co
   const size_t m = matrix_bytes(rows, F);
   void *dg = at + kHead, *du = at + kHead + m, *h = at + kHead + 2 * m;
   const void* planes[3];
-  for (int i = 0; i < 3; ++i) planes[i] = static_cast<const char*>(kept) + i * (size_t)rows * F * 2;
+  for (int i = 0; i < 3; ++i) planes[i] = static_cast<const char*>(kept) + i * (size_t)rows * pitch(F) * 2;
   return dtype == GD_FLOAT16 ? backward<__half>(q, planes, dy, ld[4], out, dg, du, h, own, err, cs)
                              : backward<__nv_bfloat16>(q, planes, dy, ld[4], out, dg, du, h, nullptr, err, cs);
 }

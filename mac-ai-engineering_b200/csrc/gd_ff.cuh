@@ -12,6 +12,10 @@ struct Problem {
   int rows, D, F, O;
 };
 
+// Elements from row to row of h, dg, du and what is kept of g and u: whole 128-byte lines (with 2,728 columns, 16-byte steps,
+// the kernels that write them took LINES)
+inline long long pitch(int F) { return (F + 63) / 64 * 64; }
+
 // y for at most kFew rows, h [rows, F] on the way (gd_ff_few.cu)
 constexpr int kFew = 128;
 int forward_few(const Problem& q, int dtype, void* h, void* y, cudaStream_t stream);

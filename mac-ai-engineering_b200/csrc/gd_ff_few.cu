@@ -20,6 +20,7 @@ constexpr int kThreads = 32 * 6; // warps 0 - 3: epilogue, 4: loads, 5: products
 struct FewParams {
   CUtensorMap w[2], t;  // weights (the second kernel: w[0] alone), tokens
   int n, cols, blocks;  // tokens; the output's columns; stages of the whole contraction
+  long long ld;         // elements from row to row of the output
   void* out;            // [n, cols]
 };
 
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ F
       a += ld_cluster(there);
       if (GATED) b += ld_cluster(there + kRowsM / 2 * 4);
     }
-    if (f0 + f < p.cols) out[(long long)t * p.cols + f0 + f] = cvt_out<T>(GATED ? a * gemm::sigmoid(a) * b : a);
+    if (f0 + f < p.cols) out[t * p.ld + f0 + f] = cvt_out<T>(GATED ? a * gemm::sigmoid(a) * b : a);
   }
   if (warp == 5) tmem_dealloc(tm, C::kCols);
   gemm::cluster_sync();  // the parts are read
@@ -202,13 +203,13 @@ template <typename T, int N>
 int run(const Problem& q, void* h, void* y, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   FewParams p = {};
-  p.n = q.rows, p.cols = q.F, p.blocks = gemm::blocks_of(q.D, kBlockK), p.out = h;
+  p.n = q.rows, p.cols = q.F, p.blocks = gemm::blocks_of(q.D, kBlockK), p.out = h, p.ld = pitch(q.F);
   if (!gemm::matrix_map(&p.w[0], q.wg, dt, q.F, q.D, q.ldg, 64) || !gemm::matrix_map(&p.w[1], q.wu, dt, q.F, q.D, q.ldu, 64) ||
       !gemm::matrix_map(&p.t, q.x, dt, q.rows, q.D, q.ldx, N))
     return GD_ERR_LAUNCH;
   if (const int st = launch<T, N, true>(p, gemm::blocks_of(q.F, kRowsM / 2), false, stream)) return st;
-  p.cols = q.O, p.blocks = gemm::blocks_of(q.F, kBlockK), p.out = y;
-  if (!gemm::matrix_map(&p.w[0], q.wd, dt, q.O, q.F, q.ldd, 64) || !gemm::matrix_map(&p.t, h, dt, q.rows, q.F, q.F, N))
+  p.cols = q.O, p.blocks = gemm::blocks_of(q.F, kBlockK), p.out = y, p.ld = q.O;
+  if (!gemm::matrix_map(&p.w[0], q.wd, dt, q.O, q.F, q.ldd, 64) || !gemm::matrix_map(&p.t, h, dt, q.rows, q.F, pitch(q.F), N))
     return GD_ERR_LAUNCH;
   return launch<T, N, false>(p, gemm::blocks_of(q.O, kRowsM), true, stream);
 }

@@ -43,7 +43,7 @@ def _fwd(x, wg, wu, wd, keep):
     y = torch.empty((n, O), dtype=x.dtype, device=x.device)
     kept = bounds = None
     if keep:
-        kept = torch.empty((3, n, F), dtype=torch.int16, device=x.device)
+        kept = torch.empty((3, n, -(-F // 64) * 64), dtype=torch.int16, device=x.device)
         if x.dtype == torch.float16:
             bounds = torch.empty(4, dtype=torch.int32, device=x.device)
     size = _bytes(n, D, F, O, 0)
