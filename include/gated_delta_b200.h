@@ -380,20 +380,22 @@ int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w
 /* ---- softmax cross entropy of a vocabulary projection, without the logits ----
  * loss_i = logsumexp_v(x_i . w_v) - x_i . w_label(i): x [rows, D], w [V, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), ldx and ldw
  * elements from row to row (multiples of 8), D a multiple of 8, any V up to 2^24; labels [rows] int32, or int64 with label64.
- * A row whose label is `ignore` has loss 0 and no gradient, whatever its values are; any other label outside [0, V) gives NaN.
+ * A row whose label is `ignore` has loss 0 and a zero row in dx, whatever it holds (in dw its infinities and NaN meet a weight
+ * of 0, as in the formula's product); any other label outside [0, V) gives NaN.
  * reduction 0: loss [rows]; 1: the mean over the rows that are not ignored (none: NaN); 2: their sum; float32.
  * The workspace of the forward holds 8 bytes a row and 128 columns; that of the backward a piece of the vocabulary's gradients
  * of the logits in `dtype` (at most 256 MiB, or 256 columns) and, with more than one piece, dx in float32. Asynchronous on
  * `stream`; the same bits every run. No counterpart in the reference. */
 size_t gd_xent_workspace_bytes(long long rows, int D, int V, int for_backward);
 
-/* lse2 [rows]: the logsumexp in log2 units, kept for the backward, or NULL. */
-int gd_xent_fwd(const void* x, const void* w, const void* labels, int label64, float* loss, float* lse2, int reduction,
+/* lse [rows, 2]: each row's largest logit and the base-2 logarithm of its sum of exponentials below it, for the backward, or
+ * NULL. */
+int gd_xent_fwd(const void* x, const void* w, const void* labels, int label64, float* loss, float* lse, int reduction,
                 long long ignore, int dtype, long long rows, int D, int V, long long ldx, long long ldw, void* workspace,
                 size_t workspace_bytes, void* stream);
 
 /* dx [rows, D], dw [V, D] (each may be NULL) from dloss: float32 [rows] for reduction 0, else one value. */
-int gd_xent_bwd(const void* x, const void* w, const void* labels, int label64, const float* lse2, const float* dloss,
+int gd_xent_bwd(const void* x, const void* w, const void* labels, int label64, const float* lse, const float* dloss,
                 void* dx, void* dw, int reduction, long long ignore, int dtype, long long rows, int D, int V, long long ldx,
                 long long ldw, void* workspace, size_t workspace_bytes, void* stream);
 

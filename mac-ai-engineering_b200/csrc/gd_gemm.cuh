@@ -72,9 +72,9 @@ struct Params {
   int label64;
   long long ignore;
   int v0;                   // the first column's place in the vocabulary
-  float2* part;             // [2 tiles_n][M]: maximum (log2 units), sum
+  float2* part;             // [2 tiles_n][M]: maximum, sum of the exponentials of what is below it
   float* target;            // [M]: the label's logit
-  const float* lse2;        // [M], log2 units
+  const float2* lse;        // [M]: the row's maximum, log2 of its sum
   const float* row_scale;   // [M]
   ErrorWord* err;
 };
@@ -626,12 +626,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
             for (int e = 0; e < 4; ++e) mx[e] = wattn::max3(mx[e], v[i + 2 * e], v[i + 2 * e + 1]);
           }
           const float high = wattn::max3(wattn::max3(mx[0], mx[1], mx[2]), wattn::max3(mx[3], v[60], v[61]),
-                                         wattn::max3(v[62], v[63], v[62])) * kLog2e;
+                                         wattn::max3(v[62], v[63], v[62]));
           const float next = wattn::max3(top, high, high), ref = next == -INFINITY ? 0.f : next;
           float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 64; ++i) a[i & 3] += ex2(fmaf(v[i], kLog2e, -ref));
-          sum = sum * ex2(top - ref) + ((a[0] + a[1]) + (a[2] + a[3]));
+          for (int i = 0; i < 64; ++i) a[i & 3] += ex2((v[i] - ref) * kLog2e);  // (1 at the maximum)
+          sum = sum * ex2((top - ref) * kLog2e) + ((a[0] + a[1]) + (a[2] + a[3]));
           top = next;
         }
         if (row < op.M && w.n + half * 128 < op.N)
@@ -640,7 +640,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const long long lab = row < op.M ? label_of(p, row) : p.ignore;
         const bool kept = lab != p.ignore;
         const long long at = kept ? lab - p.v0 : -1;
-        const float l2 = kept ? __ldg(p.lse2 + row) : 0.f, f = kept ? __ldg(p.row_scale + row) + bad : 0.f;
+        const float2 lse = kept ? __ldg(p.lse + row) : make_float2(0.f, 0.f);
+        const float f = kept ? __ldg(p.row_scale + row) + bad : 0.f;
 #pragma unroll 1
         for (int s = 0; s < 2; ++s) {
           const int c = half * 128 + s * 64, n0 = w.n + c;
@@ -649,7 +650,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           if (s == 1) release();
           if (!has(n0)) continue;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -l2));
+          for (int i = 0; i < 64; ++i) v[i] = ex2(fmaf(v[i] - lse.x, kLog2e, -lse.y));
           if (__any_sync(0xffffffffu, at >= n0 && at < n0 + 64)) {
 #pragma unroll
             for (int i = 0; i < 64; ++i) v[i] -= at == n0 + i ? 1.f : 0.f;

@@ -31,10 +31,10 @@ struct Labels {
   }
 };
 
-// Joins each row's parts: lse (log2 units), loss; for a mean or sum the last CTA adds the CTAs' sums in their order.
+// Joins each row's parts: its maximum and the logarithm of its sum, its loss (at least 0: a sure row's sum is 1 and more); for a mean or sum the last CTA adds the CTAs' sums in their order.
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __restrict__ part, const float* __restrict__ target,
                                                                int parts, int n, Labels lab, int reduction,
-                                                               float* __restrict__ lse2, float* __restrict__ loss,
+                                                               float2* __restrict__ lse, float* __restrict__ loss,
                                                                float2* sums, unsigned int* counter) {
   __shared__ float2 sh[kJoinWarps][kRows];
   __shared__ bool last;
@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __r
   float m = -INFINITY, s = 0.f;
   auto add = [&](float2 v) {  // (a NaN sum stays)
     const float next = wattn::max3(m, v.x, v.x), ref = next == -INFINITY ? 0.f : next;
-    s = s * wattn::ex2(m - ref) + v.y * wattn::ex2(v.x - ref);
+    s = s * wattn::ex2((m - ref) * gemm::kLog2e) + v.y * wattn::ex2((v.x - ref) * gemm::kLog2e);
     m = next;
   };
   if (row < n) {
@@ -67,9 +67,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __r
       const float rest = log2f(s);
       if (l != lab.ignore) {
         kept = 1.f;
-        x = l < 0 || l >= lab.V ? NAN : kLn2 * ((m - target[row] * gemm::kLog2e) + rest);
+        x = l < 0 || l >= lab.V ? NAN : (m - target[row]) + kLn2 * rest;
       }
-      if (lse2 != nullptr) lse2[row] = m + rest;
+      if (lse != nullptr) lse[row] = make_float2(m, rest);
       if (reduction == kNone) loss[row] = x;
     }
     if (reduction != kNone) {
@@ -209,7 +209,7 @@ void shape(Op& op, long long M, long long N) {
 }
 
 template <typename T>
-int forward(const Problem& q, float* loss, float* lse2, char* ws, cudaStream_t stream) {
+int forward(const Problem& q, float* loss, float2* lse, char* ws, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const FwdPlan f = fwd_plan(q.n, q.V);
   Params p = {};
@@ -223,14 +223,14 @@ int forward(const Problem& q, float* loss, float* lse2, char* ws, cudaStream_t s
   if (!gemm::operand_map(&o.a[0], q.x, dt, q.n, q.D, q.ldx, false) || !gemm::operand_map(&o.b[0], q.w, dt, q.V, q.D, q.ldw, false))
     return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kLse>(p, stream)) return st;
-  join_kernel<<<f.ctas, 32 * kJoinWarps, 0, stream>>>(p.part, p.target, f.parts, q.n, q.lab, q.reduction, lse2, loss,
+  join_kernel<<<f.ctas, 32 * kJoinWarps, 0, stream>>>(p.part, p.target, f.parts, q.n, q.lab, q.reduction, lse, loss,
                                                      reinterpret_cast<float2*>(ws + f.sums),
                                                      reinterpret_cast<unsigned int*>(ws + 64));
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
 }
 
 template <typename T>
-int backward(const Problem& q, const float* lse2, const float* dloss, void* dx, void* dw, char* ws, cudaStream_t stream) {
+int backward(const Problem& q, const float2* lse, const float* dloss, void* dx, void* dw, char* ws, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const BwdPlan b = bwd_plan(q.n, q.D, q.V);
   float* const row_scale = reinterpret_cast<float*>(ws + b.rows);
@@ -246,7 +246,7 @@ int backward(const Problem& q, const float* lse2, const float* dloss, void* dx, 
     Params p = {};
     p.ops = 1;
     label_params(p, q, reinterpret_cast<ErrorWord*>(ws));
-    p.v0 = (int)v0, p.lse2 = lse2, p.row_scale = row_scale;
+    p.v0 = (int)v0, p.lse = lse, p.row_scale = row_scale;
     Op& o = p.op[0];
     shape(o, q.n, cols);
     o.kb[0] = kd;
@@ -307,24 +307,25 @@ extern "C" size_t gd_xent_workspace_bytes(long long rows, int D, int V, int for_
   return for_backward ? bwd_plan(rows, D, V).total : fwd_plan(rows, V).total;
 }
 
-extern "C" int gd_xent_fwd(const void* x, const void* w, const void* labels, int label64, float* loss, float* lse2,
+extern "C" int gd_xent_fwd(const void* x, const void* w, const void* labels, int label64, float* loss, float* lse,
                            int reduction, long long ignore, int dtype, long long rows, int D, int V, long long ldx,
                            long long ldw, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace gd::xent;
   if (const int st = check(dtype, reduction, rows, D, V, ldx, ldw)) return st;
   if (rows == 0) return GD_OK;
   if (x == nullptr || w == nullptr || labels == nullptr || loss == nullptr) return GD_ERR_ARG;
-  if (!aligned16(x) || !aligned16(w) || !aligned16(workspace)) return GD_ERR_ALIGN;
+  if (!aligned16(x) || !aligned16(w) || !aligned16(lse) || !aligned16(workspace)) return GD_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < gd_xent_workspace_bytes(rows, D, V, 0)) return GD_ERR_WORKSPACE;
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   if (cudaMemsetAsync(workspace, 0, kHead, cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const Problem q = {x, w, ldx, ldw, (int)rows, D, V, {labels, label64, ignore, V}, reduction};
   char* ws = static_cast<char*>(workspace);
-  return dtype == GD_FLOAT16 ? forward<__half>(q, loss, lse2, ws, cs) : forward<__nv_bfloat16>(q, loss, lse2, ws, cs);
+  float2* const kept = reinterpret_cast<float2*>(lse);
+  return dtype == GD_FLOAT16 ? forward<__half>(q, loss, kept, ws, cs) : forward<__nv_bfloat16>(q, loss, kept, ws, cs);
 }
 
-extern "C" int gd_xent_bwd(const void* x, const void* w, const void* labels, int label64, const float* lse2, const float* dloss,
+extern "C" int gd_xent_bwd(const void* x, const void* w, const void* labels, int label64, const float* lse, const float* dloss,
                            void* dx, void* dw, int reduction, long long ignore, int dtype, long long rows, int D, int V,
                            long long ldx, long long ldw, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace gd::xent;
@@ -333,14 +334,16 @@ extern "C" int gd_xent_bwd(const void* x, const void* w, const void* labels, int
   if (rows == 0)
     return dw == nullptr || cudaMemsetAsync(dw, 0, (size_t)V * D * 2, cs) == cudaSuccess ? GD_OK
                                                                                          : (cudaGetLastError(), GD_ERR_LAUNCH);
-  if (x == nullptr || w == nullptr || labels == nullptr || lse2 == nullptr || dloss == nullptr) return GD_ERR_ARG;
-  if (!aligned16(x) || !aligned16(w) || !aligned16(dx) || !aligned16(dw) || !aligned16(workspace)) return GD_ERR_ALIGN;
+  if (x == nullptr || w == nullptr || labels == nullptr || lse == nullptr || dloss == nullptr) return GD_ERR_ARG;
+  if (!aligned16(x) || !aligned16(w) || !aligned16(dx) || !aligned16(dw) || !aligned16(lse) || !aligned16(workspace))
+    return GD_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < gd_xent_workspace_bytes(rows, D, V, 1)) return GD_ERR_WORKSPACE;
   if (dx == nullptr && dw == nullptr) return GD_OK;
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
   if (cudaMemsetAsync(workspace, 0, kHead, cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const Problem q = {x, w, ldx, ldw, (int)rows, D, V, {labels, label64, ignore, V}, reduction};
   char* ws = static_cast<char*>(workspace);
-  return dtype == GD_FLOAT16 ? backward<__half>(q, lse2, dloss, dx, dw, ws, cs)
-                             : backward<__nv_bfloat16>(q, lse2, dloss, dx, dw, ws, cs);
+  const float2* const kept = reinterpret_cast<const float2*>(lse);
+  return dtype == GD_FLOAT16 ? backward<__half>(q, kept, dloss, dx, dw, ws, cs)
+                             : backward<__nv_bfloat16>(q, kept, dloss, dx, dw, ws, cs);
 }

@@ -30,21 +30,21 @@ def _bytes(*sizes) -> int:
 
 
 def _fwd(x, w, labels, ignore, reduction, keep):
-    """(loss, lse2): lse2, the rows' logsumexp in log2 units, for the backward (else None)."""
+    """(loss, lse): lse, the rows' maxima and sums (as logarithms), for the backward (else None)."""
     n, D = x.shape
     loss = torch.empty(n if reduction == 0 else (), dtype=torch.float32, device=x.device)
-    lse2 = torch.empty(n, dtype=torch.float32, device=x.device) if keep else None
+    lse = torch.empty((n, 2), dtype=torch.float32, device=x.device) if keep else None
     if n == 0:  # no row: torch's own results, a mean over nothing among them
-        return loss.fill_(float("nan") if reduction == 1 else 0.0), lse2
+        return loss.fill_(float("nan") if reduction == 1 else 0.0), lse
     size = _bytes(n, D, w.shape[0], 0)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     launch("gd_xent_fwd", x.get_device(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.dtype == torch.int64,
-           loss.data_ptr(), None if lse2 is None else lse2.data_ptr(), reduction, ignore, _DTYPES[x.dtype], n, D, w.shape[0],
+           loss.data_ptr(), None if lse is None else lse.data_ptr(), reduction, ignore, _DTYPES[x.dtype], n, D, w.shape[0],
            pitch(x), pitch(w), ws.data_ptr(), size)
-    return loss, lse2
+    return loss, lse
 
 
-def _bwd(x, w, labels, lse2, dloss, ignore, reduction, need):
+def _bwd(x, w, labels, lse, dloss, ignore, reduction, need):
     """(dx, dw), contiguous, each None unless needed."""
     n, D = x.shape
     V = w.shape[0]
@@ -54,7 +54,7 @@ def _bwd(x, w, labels, lse2, dloss, ignore, reduction, need):
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if n else None
     p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     launch("gd_xent_bwd", x.get_device(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.dtype == torch.int64,
-           lse2.data_ptr(), dloss.data_ptr(), p(dx), p(dw), reduction, ignore, _DTYPES[x.dtype], n, D, V, pitch(x), pitch(w),
+           lse.data_ptr(), dloss.data_ptr(), p(dx), p(dw), reduction, ignore, _DTYPES[x.dtype], n, D, V, pitch(x), pitch(w),
            p(ws), size)
     return dx, dw
 
@@ -64,16 +64,16 @@ class LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, labels, ignore, reduction):
-        loss, lse2 = _fwd(x, w, labels, ignore, reduction, True)
-        ctx.save_for_backward(x, w, labels, lse2)
+        loss, lse = _fwd(x, w, labels, ignore, reduction, True)
+        ctx.save_for_backward(x, w, labels, lse)
         ctx.args = (ignore, reduction)
         return loss
 
     @staticmethod
     @first_order
     def backward(ctx, dloss):
-        x, w, labels, lse2 = ctx.saved_tensors
-        dx, dw = _bwd(x, w, labels, lse2, dloss.float().contiguous(), *ctx.args, ctx.needs_input_grad)
+        x, w, labels, lse = ctx.saved_tensors
+        dx, dw = _bwd(x, w, labels, lse, dloss.float().contiguous(), *ctx.args, ctx.needs_input_grad)
         return dx, dw, None, None, None
 
 
@@ -82,8 +82,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     """The cross entropy of the logits x weight^T, in float32: x [..., D] and weight [V, D] (as nn.Linear keeps it) both
     bfloat16 or both float16, D a multiple of 8, V any size; labels [...] int64 or int32. reduction "none": one loss for each
     row, in the labels' shape; "mean": over the rows that are not ignored (NaN if all are); "sum". A row with the label
-    ignore_index has loss 0 and no gradient, whatever it holds; any other label outside [0, V) gives NaN (nothing waits for
-    the host to look). Gradients of x and weight come in their type, the same bits every run; a frozen one's is not formed.
+    ignore_index has loss 0 and a zero row in x's gradient, whatever it holds (in the weight's, its infinities and NaN meet a
+    weight of 0, as in the formula's product); any other label outside [0, V) gives NaN (nothing waits for the host to look). Gradients of x and weight come in their type, the same bits every run; a frozen one's is not formed.
 
     The logits are never kept: beside the gradients a call holds 8 bytes for each row and 128 columns, the backward at most
     256 MiB (or 256 columns) of the logits' gradients and, with more than one such piece, x's gradient in float32."""
