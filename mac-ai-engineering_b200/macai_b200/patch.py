@@ -14,42 +14,51 @@ transformers 5.x binds the rule in two ways, and both are covered:
     macai_b200.patch.install(model=model)      # and the layers of an already-built model
     with macai_b200.patch.installed():         # or only inside a block
         ...
+    macai_b200.patch.install(recurrent=True)   # the models' single-token form of the rule, too (their decoding steps)
 """
 from __future__ import annotations
 
 import contextlib
 import importlib
 
-from .gated_delta import chunk_gated_delta_rule
+from .gated_delta import chunk_gated_delta_rule, recurrent_gated_delta_rule
 
 MODULES = ("transformers.models.qwen3_5.modeling_qwen3_5", "transformers.models.qwen3_5_moe.modeling_qwen3_5_moe",
            "transformers.models.qwen3_next.modeling_qwen3_next")
 NAMES = ("torch_chunk_gated_delta_rule", "chunk_gated_delta_rule")
 ATTR = "chunk_gated_delta_rule"       # the per-layer binding
+# the recurrent form's: transformers binds `fused_recurrent_gated_delta_rule or torch_recurrent_gated_delta_rule`
+RECURRENT_NAMES = ("torch_recurrent_gated_delta_rule", "fused_recurrent_gated_delta_rule")
+RECURRENT_ATTR = "recurrent_gated_delta_rule"
 _saved: dict = {}                     # (module path, name) -> original
-_rebound: list = []                   # (layer, original bound function)
+_rebound: list = []                   # (layer, attribute, original bound function)
 
 
-def install(model=None) -> list:
+def install(model=None, recurrent: bool = False) -> list:
     """Swap the rule in every modeling module that has it; returns the (module, name) pairs patched. With model, also
-    rebind the rule of every layer of that model that holds one."""
+    rebind the rule of every layer of that model that holds one. recurrent: the single-token form as well."""
+    swaps = [(NAMES, ATTR, chunk_gated_delta_rule)]
+    if recurrent:
+        swaps.append((RECURRENT_NAMES, RECURRENT_ATTR, recurrent_gated_delta_rule))
     done = []
     for path in MODULES:
         try:
             mod = importlib.import_module(path)
         except ImportError:
             continue
-        for name in NAMES:
-            if hasattr(mod, name) and getattr(mod, name) is not chunk_gated_delta_rule:
-                _saved[(path, name)] = getattr(mod, name)
-                setattr(mod, name, chunk_gated_delta_rule)
-                done.append((path, name))
+        for names, _, rule in swaps:
+            for name in names:
+                if hasattr(mod, name) and getattr(mod, name) is not rule:
+                    _saved[(path, name)] = getattr(mod, name)
+                    setattr(mod, name, rule)
+                    done.append((path, name))
     if model is not None:
         for layer in model.modules():
-            fn = getattr(layer, ATTR, None)
-            if callable(fn) and fn is not chunk_gated_delta_rule and not isinstance(fn, type):
-                _rebound.append((layer, fn))
-                setattr(layer, ATTR, chunk_gated_delta_rule)
+            for _, attr, rule in swaps:
+                fn = getattr(layer, attr, None)
+                if callable(fn) and fn is not rule and not isinstance(fn, type):
+                    _rebound.append((layer, attr, fn))
+                    setattr(layer, attr, rule)
     return done
 
 
@@ -58,8 +67,8 @@ def uninstall() -> None:
         setattr(importlib.import_module(path), name, fn)
         del _saved[(path, name)]
     while _rebound:
-        layer, fn = _rebound.pop()
-        setattr(layer, ATTR, fn)
+        layer, attr, fn = _rebound.pop()
+        setattr(layer, attr, fn)
 
 
 def patched() -> list:
@@ -68,8 +77,8 @@ def patched() -> list:
 
 
 @contextlib.contextmanager
-def installed(model=None):
-    install(model=model)
+def installed(model=None, recurrent: bool = False):
+    install(model=model, recurrent=recurrent)
     try:
         yield
     finally:
