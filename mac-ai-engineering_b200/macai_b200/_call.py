@@ -37,18 +37,21 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 def matrix(t: torch.Tensor) -> torch.Tensor:
-    """t [..., D] as rows [N, D] that a tensor map of 16-bit values can read in place: adjacent columns, rows 16-byte aligned
-    and apart (a copy only when the view is not)."""
+    """t [..., D], D a multiple of 8, as rows [N, D] that a tensor map of 16-bit values can read in place: adjacent columns, rows
+    16-byte aligned and apart (a copy only when the view is not)."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t if t.dim() == 2 else t.view(-1, t.shape[-1])
     m = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
     n, d = m.shape
-    if m.data_ptr() % 16 == 0 and (d == 1 or m.stride(1) == 1) and (n <= 1 or (m.stride(0) >= d and m.stride(0) % 8 == 0)):
+    if m.data_ptr() % 16 == 0 and m.stride(1) == 1 and (n <= 1 or (m.stride(0) >= d and m.stride(0) % 8 == 0)):
         return m
     return aligned(m.contiguous())
 
 
 def pitch(m: torch.Tensor) -> int:
     """Elements from row to row of a `matrix`."""
-    return m.stride(0) if m.shape[0] > 1 else -(-m.shape[1] // 8) * 8
+    n, d = m.shape
+    return m.stride(0) if n > 1 else d
 
 
 def first_order(backward):

@@ -29,8 +29,9 @@ def _bytes(*sizes) -> int:
     return n
 
 
-def _pitches(*ms):
-    return (ctypes.c_longlong * len(ms))(*[pitch(m) for m in ms])
+@functools.lru_cache(maxsize=1024)
+def _longs(*x):
+    return (ctypes.c_longlong * len(x))(*x)
 
 
 def _sizes(x, wg, wd):
@@ -48,9 +49,9 @@ def _fwd(x, wg, wu, wd, keep):
             bounds = torch.empty(4, dtype=torch.int32, device=x.device)
     size = _bytes(n, D, F, O, 0)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    launch("gd_ff_fwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), p(kept), p(bounds),
-           y.data_ptr(), _DTYPES[x.dtype], n, D, F, O, _pitches(x, wg, wu, wd), ws.data_ptr(), size)
+    launch("gd_ff_fwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(),
+           None if kept is None else kept.data_ptr(), None if bounds is None else bounds.data_ptr(), y.data_ptr(), _DTYPES[x.dtype], n, D, F, O, _longs(pitch(x), pitch(wg), pitch(wu), pitch(wd)),
+           ws.data_ptr(), size)
     return y, kept, bounds
 
 
@@ -63,7 +64,7 @@ def _bwd(x, wg, wu, wd, kept, bounds, dy, need):
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     launch("gd_ff_bwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), kept.data_ptr(),
            None if bounds is None else bounds.data_ptr(), dy.data_ptr(), *(None if t is None else t.data_ptr() for t in out),
-           _DTYPES[x.dtype], n, D, F, O, _pitches(x, wg, wu, wd, dy), ws.data_ptr(), size)
+           _DTYPES[x.dtype], n, D, F, O, _longs(pitch(x), pitch(wg), pitch(wu), pitch(wd), pitch(dy)), ws.data_ptr(), size)
     return out
 
 
@@ -82,29 +83,43 @@ class GatedFeedForward(torch.autograd.Function):
         return _bwd(*ctx.saved_tensors, matrix(dy), ctx.needs_input_grad)
 
 
+def _refuse(name, x, w_gate, w_up, w_down):
+    """The error for inputs that the block does not take."""
+    for n, t, d in (("x", x, 1), ("w_gate", w_gate, 2), ("w_up", w_up, 2), ("w_down", w_down, 2)):
+        if not isinstance(t, torch.Tensor) or t.dim() < d or (d == 2 and t.dim() != 2):
+            return ValueError(f"{name}: {n} must be {'[..., D]' if d == 1 else 'a matrix'}")
+        if t.dtype not in _DTYPES:
+            return TypeError(f"{name}: bfloat16 or float16, got {t.dtype} for {n}")
+        if t.dtype != x.dtype or t.get_device() != x.get_device():
+            return ValueError(f"{name}: x and the weights must share one dtype and device")
+    if not x.is_cuda:
+        return RuntimeError(f"{name}: CUDA tensors only (there is no CPU path)")
+    D, (F, d2), O = x.shape[-1], w_gate.shape, w_down.shape[0]
+    if d2 != D or w_up.shape != w_gate.shape or w_down.shape[1] != F:
+        return ValueError(f"{name}: w_gate and w_up [F, D] and w_down [O, F] must agree with x [..., D]; got {tuple(x.shape)}, "
+                          f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
+    return NotImplementedError(f"{name}: D, F and O are multiples of 8, got {D}, {F}, {O}")
+
+
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
     """y [..., O] for x [..., D], w_gate and w_up [F, D] (as nn.Linear keeps them; halves of one [2 F, D] weight are read in
     place) and w_down [O, F], all bfloat16 or all float16, D, F and O multiples of 8. Gradients of all four come in their
     type, the same bits every run; those of frozen inputs are not formed. Views with adjacent columns and 16-byte aligned
     rows are read in place, others are copied."""
     name = "gated_feed_forward"
-    for n, t, d in (("x", x, 1), ("w_gate", w_gate, 2), ("w_up", w_up, 2), ("w_down", w_down, 2)):
-        if not isinstance(t, torch.Tensor) or t.dim() < d or (d == 2 and t.dim() != 2):
-            raise ValueError(f"{name}: {n} must be {'[..., D]' if d == 1 else 'a matrix'}")
-        if t.dtype not in _DTYPES:
-            raise TypeError(f"{name}: bfloat16 or float16, got {t.dtype} for {n}")
-        if t.dtype != x.dtype or t.get_device() != x.get_device():
-            raise ValueError(f"{name}: x and the weights must share one dtype and device")
-    if not x.is_cuda:
-        raise RuntimeError(f"{name}: CUDA tensors only (there is no CPU path)")
-    D, (F, d2), O = x.shape[-1], w_gate.shape, w_down.shape[0]
-    if d2 != D or w_up.shape != w_gate.shape or w_down.shape[1] != F:
-        raise ValueError(f"{name}: w_gate and w_up [F, D] and w_down [O, F] must agree with x [..., D]; got {tuple(x.shape)}, "
-                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
-    if min(D, F, O) == 0 or D % 8 or F % 8 or O % 8:
-        raise NotImplementedError(f"{name}: D, F and O are multiples of 8, got {D}, {F}, {O}")
+    try:
+        dt, D, index = x.dtype, x.shape[-1], x.get_device()
+        F, d2 = w_gate.shape
+        O, f2 = w_down.shape
+        ok = (x.is_cuda and dt in _DTYPES and w_gate.dtype == dt and w_up.dtype == dt and w_down.dtype == dt and d2 == D
+              and w_up.shape == w_gate.shape and f2 == F and D > 0 and F > 0 and O > 0 and D % 8 == 0 and F % 8 == 0
+              and O % 8 == 0 and w_gate.get_device() == index and w_up.get_device() == index and w_down.get_device() == index)
+    except (AttributeError, IndexError, ValueError):
+        ok = False
+    if not ok:
+        raise _refuse(name, x, w_gate, w_up, w_down)
     if recorded(x, w_gate, w_up, w_down):
         y = GatedFeedForward.apply(matrix(x), matrix(w_gate), matrix(w_up), matrix(w_down))
     else:
         y = _fwd(matrix(x), matrix(w_gate), matrix(w_up), matrix(w_down), False)[0]
-    return y.view(*x.shape[:-1], O)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], O)

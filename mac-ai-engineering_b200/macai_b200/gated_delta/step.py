@@ -91,9 +91,10 @@ def gated_delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     name = "gated_delta_step"
     q, k, v, g_, beta_, B, T, H, HK, DK, DV = _inputs(name, query, key, value, g, beta)
     index = q.get_device()
-    if not isinstance(state, torch.Tensor) or state.dim() != 4 or state.shape[1:] != (H, DK, DV):
+    if not isinstance(state, torch.Tensor) or state.dim() != 4 or state.shape != (state.shape[0], H, DK, DV):
         raise ValueError(f"{name}: state must be [S, H, DK, DV] with (H, DK, DV) = {(H, DK, DV)}")
-    if state.dtype != torch.float32 or state.get_device() != index or not state.is_contiguous() or state.data_ptr() % 16:
+    pool = state.data_ptr()
+    if state.dtype != torch.float32 or state.get_device() != index or not state.is_contiguous() or pool % 16:
         raise ValueError(f"{name}: state must be float32, contiguous and 16-byte aligned on the query's device (it is "
                          "written in place)")
     if slots is None and out_slots is not None:
@@ -107,7 +108,7 @@ def gated_delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if recorded(query, key, value, g, beta, state):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train with chunk_gated_delta_rule")
     o = torch.empty((B, T, H, DV), dtype=q.dtype, device=q.device)
-    pool, at = state.data_ptr(), None if slots is None else slots.data_ptr()
+    at = None if slots is None else slots.data_ptr()
     launch("gd_rule_step", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), g_.data_ptr(), beta_.data_ptr(), pool, pool, at,
            at if out_slots is None else out_slots.data_ptr(), o.data_ptr(), _DTYPES[q.dtype], _DTYPES[v.dtype], B, T, H, HK,
            DK, DV, state.shape[0], _lib.GD_L2NORM if use_qk_l2norm_in_kernel else 0)
