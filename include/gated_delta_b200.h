@@ -383,21 +383,23 @@ int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w
  * A row whose label is `ignore` has loss 0 and a zero row in dx, whatever it holds (in dw its infinities and NaN meet a weight
  * of 0, as in the formula's product); any other label outside [0, V) gives NaN.
  * reduction 0: loss [rows]; 1: the mean over the rows that are not ignored (none: NaN); 2: their sum; float32.
- * The workspace of the forward holds 8 bytes a row and 128 columns; that of the backward a piece of the vocabulary's gradients
- * of the logits in `dtype` (at most 256 MiB, or 256 columns) and, with more than one piece, dx in float32. Asynchronous on
+ * Ignored rows cost no products: the others are gathered. The workspace of the forward holds their x and 8 bytes a row and 128
+ * columns; that of the backward their x and dx, a piece of the vocabulary's gradients of the logits in `dtype` (at most 256 MiB, or
+ * 256 columns) and float32 sums of dx (with more than one piece: one for each value; else at most 64 MiB). Asynchronous on
  * `stream`; the same bits every run. No counterpart in the reference. */
 size_t gd_xent_workspace_bytes(long long rows, int D, int V, int for_backward);
 
-/* lse [rows, 2]: each row's largest logit and the base-2 logarithm of its sum of exponentials below it, for the backward, or
- * NULL. */
-int gd_xent_fwd(const void* x, const void* w, const void* labels, int label64, float* loss, float* lse, int reduction,
-                long long ignore, int dtype, long long rows, int D, int V, long long ldx, long long ldw, void* workspace,
-                size_t workspace_bytes, void* stream);
+/* For the backward (or NULL, both): lse [rows, 2], the live rows' largest logits and the base-2 logarithms of their sums of
+ * exponentials below them; plan, 4 + 2 rows ints: the number of live rows (whose labels are not ignored), each row's place among
+ * them, their labels. */
+int gd_xent_fwd(const void* x, const void* w, const void* labels, int label64, float* loss, float* lse, int* plan,
+                int reduction, long long ignore, int dtype, long long rows, int D, int V, long long ldx, long long ldw,
+                void* workspace, size_t workspace_bytes, void* stream);
 
 /* dx [rows, D], dw [V, D] (each may be NULL) from dloss: float32 [rows] for reduction 0, else one value. */
-int gd_xent_bwd(const void* x, const void* w, const void* labels, int label64, const float* lse, const float* dloss,
-                void* dx, void* dw, int reduction, long long ignore, int dtype, long long rows, int D, int V, long long ldx,
-                long long ldw, void* workspace, size_t workspace_bytes, void* stream);
+int gd_xent_bwd(const void* x, const void* w, const float* lse, const int* plan, const float* dloss, void* dx, void* dw,
+                int reduction, int dtype, long long rows, int D, int V, long long ldx, long long ldw, void* workspace,
+                size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -47,12 +47,14 @@ enum Epilogue {
 // One product. a[s], b[s]: the operands of contraction segment s (kSwiglu: b[0] gate, b[1] up, one segment).
 struct Op {
   CUtensorMap a[2], b[2], c;
-  int tiles_m, tiles_n, first;  // first: its first tile's index
-  int kb[2];                    // stages of each segment
+  int tiles_m, tiles_n;
+  int kb[2];            // stages of each segment
+  int slices, per;      // (kStore) the contraction in `slices` parts of `per` stages, each a tile of its own
   bool a_mn, b_mn;
+  bool m_live, k_live;  // only the first *Params::live rows of C, or of the contraction, count
   int M, N;
   // kStore: 0 = C in 16 bits; 1 = C into `sum`; 2 = added to `sum`; 3 = `sum` + C in 16 bits. The sums lie as the threads
-  // hold them: [tile][CTA][column][row].
+  // hold them: [slice][tile][CTA][column][row].
   int sum_mode;
   float* sum;
   const float* factor;  // NULL: 1
@@ -61,16 +63,15 @@ struct Op {
 
 struct Params {
   Op op[kMaxOps];
-  int ops, tiles;
+  int ops;
+  const int* live;          // NULL: all
   CUtensorMap x[3];         // g and u as they are kept: the upper halves of their float32 bits, and the bytes below them
   CUtensorMap y[2];         // kDSwiglu: du (Op::c is dg), h
   bool keep;                // kSwiglu: store g, u; kDSwiglu: store h
   // float16's feed-forward block: the bits of max |g|, max |u| (kSwiglu collects them), max ||dy row||_1, max |w_down|
   uint32_t* bounds;
   // kLse, kDLogit
-  const void* labels;
-  int label64;
-  long long ignore;
+  const int* labels;        // of the live rows (-1: none in the vocabulary)
   int v0;                   // the first column's place in the vocabulary
   float2* part;             // [2 tiles_n][M]: maximum, sum of the exponentials of what is below it
   float* target;            // [M]: the label's logit
@@ -199,21 +200,47 @@ __device__ __forceinline__ void commit_pair(uint32_t lead, uint64_t* bar) {
       : "memory");
 }
 
+// The rows that count are known on the device only: sizes that depend on them are computed where they are used.
+__device__ __forceinline__ int row_tiles(const Op& o, int live) { return o.m_live ? (live + kTileM - 1) / kTileM : o.tiles_m; }
+__device__ __forceinline__ int tiles_of(const Op& o, int live) { return row_tiles(o, live) * o.tiles_n * o.slices; }
+template <int E>
+__device__ __forceinline__ int all_tiles(const Params& p, int live) {
+  int n = 0;
+  for (int i = 0; i < (E == kStore ? p.ops : 1); ++i) n += tiles_of(p.op[i], live);
+  return n;
+}
 struct Where {
-  int op, m, n;  // the problem, the tile's first row and column
+  int op, at, slice, m, n;  // the problem, the tile in it, its slice, the tile's first row and column
 };
 template <int E>
-__device__ __forceinline__ Where locate(const Params& p, int tile) {
+__device__ __forceinline__ Where locate(const Params& p, int tile, int live) {
   Where w;
-  w.op = 0;
+  w.op = w.slice = 0;
+  w.at = tile;
   if (E == kStore)
-    while (w.op + 1 < p.ops && tile >= p.op[w.op + 1].first) ++w.op;
+    for (; w.op + 1 < p.ops; ++w.op) {
+      const int c = tiles_of(p.op[w.op], live);
+      if (w.at < c) break;
+      w.at -= c;
+    }
   const Op& o = p.op[w.op];
-  const int t = tile - o.first, band = kGroupM * o.tiles_n, g = t / band, r = t - g * band;
-  const int high = o.tiles_m - g * kGroupM < kGroupM ? o.tiles_m - g * kGroupM : kGroupM;
+  const int rows = row_tiles(o, live);
+  int t = w.at;
+  if (E == kStore && o.slices > 1) {
+    w.slice = t / (rows * o.tiles_n);
+    t -= w.slice * rows * o.tiles_n;
+  }
+  const int band = kGroupM * o.tiles_n, g = t / band, r = t - g * band;
+  const int high = rows - g * kGroupM < kGroupM ? rows - g * kGroupM : kGroupM;
   w.m = (g * kGroupM + r % high) * kTileM;
   w.n = (r / high) * (E == kSwiglu ? kHalf : kTileN);
   return w;
+}
+// the tile's stages of segment s, and the first of them
+__device__ __forceinline__ int stages_of(const Op& o, const Where& w, int s, int live, int& from) {
+  const int n = s == 0 && o.k_live ? (live + kBlockK - 1) / kBlockK : o.kb[s];
+  from = w.slice * o.per;
+  return o.slices == 1 ? n : n - from < o.per ? (n > from ? n - from : 0) : o.per;
 }
 
 __device__ __forceinline__ uint32_t slab_at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
@@ -283,10 +310,6 @@ __device__ __forceinline__ float carried(const uint32_t* b) {
   return ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e);
 }
 
-__device__ __forceinline__ long long label_of(const Params& p, int row) {
-  return p.label64 ? __ldg(static_cast<const long long*>(p.labels) + row) : __ldg(static_cast<const int*>(p.labels) + row);
-}
-
 template <typename T, int E>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Params p) {
   using C = Cfg<E>;
@@ -304,6 +327,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int live = p.live == nullptr ? 0 : __ldg(p.live), tiles = all_tiles<E>(p, live);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
@@ -335,14 +359,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     const uint32_t lead = elect();
     int slot = 0, laps = 0, issued = 0;
     bool ok = true;
-    for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
-      Where w = locate<E>(p, tile);
+    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+      Where w = locate<E>(p, tile, live);
       w.op = __shfl_sync(0xffffffffu, w.op, 0);
       const Op& op = p.op[w.op];
       const int am = __shfl_sync(0xffffffffu, w.m + (int)rank * kHalf, 0);
       const int bn = __shfl_sync(0xffffffffu, E == kSwiglu ? w.n : w.n + (int)rank * kHalf, 0);
-      auto segment = [&](auto a_mn, auto b_mn, const CUtensorMap* ma, const CUtensorMap* mb, int n) {
-        for (int kb = 0; kb < n; ++kb) {
+      auto segment = [&](auto a_mn, auto b_mn, const CUtensorMap* ma, const CUtensorMap* mb, int from, int n) {
+        for (int kb = from; kb < from + n; ++kb) {
           if (laps > 0 && !(ok = warp_wait(empty + slot, (laps - 1) & 1, p.err, 80))) return;
           if (rank == 0 && lead) mbar_arrive_expect_tx(full + slot, 2 * kStage);
           const uint32_t bar = in_first_cta(full + slot), a = s_base + slot * kStage, b = a + kOperand;
@@ -369,14 +393,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       using No = std::false_type;
       for (int s = 0; ok && s < 2; ++s) {
         const CUtensorMap *ma = &op.a[s], *mb = E == kSwiglu ? &op.b[rank] : &op.b[s];
-        const int n = __shfl_sync(0xffffffffu, op.kb[s], 0);
+        int from;
+        int n = stages_of(op, w, s, live, from);
+        n = __shfl_sync(0xffffffffu, n, 0);
+        from = __shfl_sync(0xffffffffu, from, 0);
         if constexpr (E == kStore) {
           const int layout = __shfl_sync(0xffffffffu, (op.a_mn ? 2 : 0) + (op.b_mn ? 1 : 0), 0);
-          if (layout == 0) segment(No{}, No{}, ma, mb, n);
-          else if (layout == 1) segment(No{}, Yes{}, ma, mb, n);
-          else segment(Yes{}, Yes{}, ma, mb, n);
+          if (layout == 0) segment(No{}, No{}, ma, mb, from, n);
+          else if (layout == 1) segment(No{}, Yes{}, ma, mb, from, n);
+          else segment(Yes{}, Yes{}, ma, mb, from, n);
         } else {
-          segment(No{}, std::integral_constant<bool, E == kDSwiglu>{}, ma, mb, n);
+          segment(No{}, std::integral_constant<bool, E == kDSwiglu>{}, ma, mb, from, n);
         }
       }
     }
@@ -390,13 +417,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       const uint32_t lead = elect();
       int slot = 0, laps = 0, it = 0;
       bool ok = true;
-      for (int tile = pair; ok && tile < p.tiles; tile += pairs, ++it) {
-        const Where w = locate<E>(p, tile);
+      for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
+        const Where w = locate<E>(p, tile, live);
         const Op& op = p.op[w.op];
         const int buf = it & 1;
         if (it >= 2 && !(ok = cluster_wait(acc_empty + buf, ((it >> 1) - 1) & 1, p.err, 82))) break;
         tc_fence_after();
-        const int n = __shfl_sync(0xffffffffu, op.kb[0] + op.kb[1], 0);
+        int from;
+        const int n = __shfl_sync(0xffffffffu, stages_of(op, w, 0, live, from) + stages_of(op, w, 1, live, from), 0);
         const uint32_t d = tm + buf * kTileN;
         // The layouts are constants of each loop: descriptors and steps then stay in uniform registers, which the instruction
         // reads (as variables of the problem they were moved there for every product: 1,250 instead of 1,600 TFLOP/s).
@@ -453,15 +481,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         for (int i = 0; i < 3; ++i) load_slab(to + i * kStrip, &p.x[i], n0, m0, aux + 2 * ew + (at & 1));
       }
     };
-    if (E == kDSwiglu && pair < p.tiles) fetch(0, locate<E>(p, pair));
+    if (E == kDSwiglu && pair < tiles) fetch(0, locate<E>(p, pair, live));
     uint32_t landed = 0;  // kDSwiglu: the phase of each set's barrier (a step past the matrix loads nothing)
-    for (int tile = pair; tile < p.tiles; tile += pairs, ++it) {
-      const Where w = locate<E>(p, tile);
+    for (int tile = pair; tile < tiles; tile += pairs, ++it) {
+      const Where w = locate<E>(p, tile, live);
       const Op& op = p.op[w.op];
       const int buf = it & 1, m0 = w.m + (int)rank * kHalf + quad * 32, row = m0 + lane;
       const uint32_t t0 = tm + lanes + buf * kTileN;
-      const bool live = m0 < op.M;  // the warp has rows of the matrix
-      auto has = [&](int n0) { return live && n0 < op.N; };
+      const int rows = op.m_live ? live : op.M;  // (kDLogit: zeros in the rows past them)
+      auto has = [&](int n0) { return m0 < (E == kDLogit ? op.M : rows) && n0 < op.N; };
       ok = ok && warp_wait(acc_full + buf, (it >> 1) & 1, p.err, 85);
       tc_fence_after();
       const float bad = ok ? 0.f : NAN;  // a wait that gave up leaves NaN
@@ -474,8 +502,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       if constexpr (E == kStore) {
         const float f = (op.factor != nullptr ? __ldg(op.factor) : op.unscale ? 1.f / carried(p.bounds) : 1.f) + bad;
         float* sum = op.sum_mode == 0 ? nullptr
-                                      : op.sum + (((long long)(tile - op.first) * 2 + rank) * kTileN + half * 128) * kHalf +
+                                      : op.sum + (((long long)w.at * 2 + rank) * kTileN + half * 128) * kHalf +
                                             quad * 32 + lane;
+        int from;
+        const bool none = stages_of(op, w, 0, live, from) + stages_of(op, w, 1, live, from) == 0;  // a sum over nothing
 #pragma unroll 1
         for (int s = 0; s < 2; ++s) {
           const int c = half * 128 + s * 64, n0 = w.n + c;
@@ -483,6 +513,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           wattn::tmem_ld64(t0 + c, v);
           if (s == 1) release();
           if (!has(n0)) continue;
+          if (none) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) v[i] = 0.f;
+          }
           if (op.sum_mode != 0) {
             float* at = sum + (long long)s * 64 * kHalf;
             if (op.sum_mode != 1) {
@@ -565,7 +599,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
             landed ^= 1u << set;
           }
           if (s < 3) fetch(step + 1, w);
-          else if (tile + pairs < p.tiles) fetch(step + 1, locate<E>(p, tile + pairs));
+          else if (tile + pairs < tiles) fetch(step + 1, locate<E>(p, tile + pairs, live));
           if (!here) continue;
           const uint32_t strips = slab + set * 3 * kStrip;
 #pragma unroll
@@ -599,7 +633,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           }
         }
       } else if constexpr (E == kLse) {
-        const long long lab = row < op.M ? label_of(p, row) - p.v0 : -1;
+        const int lab = row < rows ? __ldg(p.labels + row) : -1;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
         for (int s = 0; s < 2; ++s) {
@@ -608,7 +642,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           wattn::tmem_ld64(t0 + c, v);
           if (s == 1) release();
           if (n0 >= op.N) continue;
-          const bool here = row < op.M && lab >= n0 && lab < n0 + 64 && lab < op.N;
+          const bool here = lab >= n0 && lab < n0 + 64;
           if (__any_sync(0xffffffffu, here)) {
             float x = 0.f;
 #pragma unroll
@@ -634,12 +668,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           sum = sum * ex2((top - ref) * kLog2e) + ((a[0] + a[1]) + (a[2] + a[3]));
           top = next;
         }
-        if (row < op.M && w.n + half * 128 < op.N)
+        if (row < rows && w.n + half * 128 < op.N)
           p.part[(long long)(w.n / kTileN * 2 + half) * op.M + row] = make_float2(top, sum + bad);
       } else {  // kDLogit
-        const long long lab = row < op.M ? label_of(p, row) : p.ignore;
-        const bool kept = lab != p.ignore;
-        const long long at = kept ? lab - p.v0 : -1;
+        const bool kept = row < rows;
+        const int at = kept ? __ldg(p.labels + row) - p.v0 : -1;
         const float2 lse = kept ? __ldg(p.lse + row) : make_float2(0.f, 0.f);
         const float f = kept ? __ldg(p.row_scale + row) + bad : 0.f;
 #pragma unroll 1
@@ -659,7 +692,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const uint32_t x = pack16<T>(v[2 * i] * f, v[2 * i + 1] * f);
-            u[i] = kept ? x : 0u;  // an ignored row's logits may be anything
+            u[i] = kept ? x : 0u;
           }
           send_row(&op.c, slab, lane, n0, m0, u);
         }
@@ -675,15 +708,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
 }
 
-// Problems in order: each one's first tile is set here. Persistent pairs: as many as SMs allow.
+// Persistent pairs: as many as SMs allow.
 template <typename T, int E>
 int launch(Params& p, cudaStream_t stream) {
   int tiles = 0;
   for (int i = 0; i < p.ops; ++i) {
-    p.op[i].first = tiles;
-    tiles += p.op[i].tiles_m * p.op[i].tiles_n;
+    if (p.op[i].slices < 1) p.op[i].slices = 1;
+    tiles += p.op[i].tiles_m * p.op[i].tiles_n * p.op[i].slices;
   }
-  p.tiles = tiles;
   if (tiles == 0) return GD_OK;
   static bool done[kMaxDevices];
   auto kern = gemm_kernel<T, E>;

@@ -1,9 +1,11 @@
 // Softmax cross entropy of a vocabulary projection that never keeps the logits:
 //   l = x W^T,   lse_i = log sum_v exp(l_iv),   loss_i = lse_i - l_i,label(i)
 //   D_iv = (exp(l_iv - lse_i) - [v = label(i)]) g_i,   dx = D W,   dW = D^T x
-// Forward: one product whose epilogue keeps a maximum and a sum for each row and 128 columns, then their join. Backward: the
-// vocabulary in pieces; a piece's logits are formed again and leave as D in 16 bits (the matrix instruction's operand type), then
-// one launch of both gradients' products. dW's rows of a piece are final; dx is summed over the pieces in fp32.
+// Rows whose label is ignored take no part: the others' x is gathered first (packed rows of x, `live` of them, a number that only
+// the device knows; the products' tiles are counted there). Forward: one product whose epilogue keeps a maximum and a sum for each
+// row and 128 columns, then their join. Backward: the vocabulary in pieces; a piece's logits are formed again and leave as D in 16
+// bits (the matrix instruction's operand type), then one launch of both gradients' products. dW's rows of a piece are final; dx is
+// summed over the pieces in fp32, and spread over its rows at the end.
 #include <cstdint>
 
 #include "gd_gemm.cuh"
@@ -26,33 +28,150 @@ struct Labels {
   int is64;
   long long ignore;
   int V;
-  __device__ __forceinline__ long long of(int row) const {
+  __device__ __forceinline__ long long of(long long row) const {
     return is64 ? __ldg(static_cast<const long long*>(at) + row) : __ldg(static_cast<const int*>(at) + row);
   }
 };
 
-// Joins each row's parts: its maximum and the logarithm of its sum, its loss (at least 0: a sure row's sum is 1 and more); for a mean or sum the last CTA adds the CTAs' sums in their order.
+// What the forward finds out about the labels and the backward needs again, int32: the number of live rows, (three unused,)
+// each row's place among them (-1: ignored) [n], each live row's label (-1: not in the vocabulary) [n].
+struct Plan {
+  int *live, *place, *label;
+  __host__ __device__ static Plan of(int* at, int n) { return {at, at + 4, at + 4 + n}; }
+};
+constexpr int kPlanInts(int n) { return 4 + 2 * n; }
+
+// The sum over the CTA's threads (every thread gets it).
+template <int WARPS>
+__device__ __forceinline__ int cta_sum(int v, int* sh) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) s += sh[w];
+  return s;
+}
+
+// The plan of the rows [r0, r1) of each CTA: it counts the live rows before its own by itself (a CTA's reading of up to 8 n bytes
+// of labels, 592 CTAs at most), so that one launch numbers them all. CTA 0 clears the workspace's head and writes the total.
+constexpr int kPlanThreads = 256;
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(Labels lab, int n, int step, Plan plan, int* head) {
+  __shared__ int sh[kPlanThreads / 32];
+  __shared__ int before[kPlanThreads / 32];
+  const int r0 = (int)min((long long)blockIdx.x * step, (long long)n), r1 = (int)min((long long)r0 + step, (long long)n);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stop = blockIdx.x == 0 ? n : r0;
+  int c = 0;
+  for (int i = threadIdx.x; i < stop; i += kPlanThreads) c += lab.of(i) != lab.ignore;
+  int base = cta_sum<kPlanThreads / 32>(c, sh);
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *plan.live = base;
+    if (threadIdx.x < 64) head[threadIdx.x] = 0;
+    base = 0;
+  }
+  for (int r = r0; r < r1; r += kPlanThreads) {
+    const int i = r + threadIdx.x;
+    const long long l = i < r1 ? lab.of(i) : lab.ignore;
+    const bool keep = l != lab.ignore;
+    const unsigned mask = __ballot_sync(0xffffffffu, keep);
+    __syncthreads();
+    if (lane == 0) before[warp] = __popc(mask);
+    __syncthreads();
+    int at = base, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) at += before[w];
+      all += before[w];
+    }
+    at += __popc(mask & ((1u << lane) - 1u));
+    if (i < r1) plan.place[i] = keep ? at : -1;
+    if (keep) plan.label[at] = l < 0 || l >= lab.V ? -1 : (int)l;
+    base += all;
+  }
+}
+
+// The live rows of x, packed, `ld` elements from row to row; zeros in what is left of their last tile of the contraction (dW sums
+// over the rows of whole stages). A warp a row. HEAD: also clears the workspace's head (the backward's first kernel).
+__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* __restrict__ x, long long ldx, int n, int D,
+                                                     const int* __restrict__ live, const int* __restrict__ place,
+                                                     uint16_t* __restrict__ out, long long ld, int* head) {
+  const int warps = gridDim.x * 8, w0 = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (head != nullptr && blockIdx.x == 0 && threadIdx.x < 64) head[threadIdx.x] = 0;
+  for (int i = w0; i < n; i += warps) {
+    const int r = __ldg(place + i);
+    if (r < 0) continue;
+    for (int c = lane * 8; c < D; c += 256)
+      *reinterpret_cast<uint4*>(out + r * ld + c) = __ldg(reinterpret_cast<const uint4*>(x + i * ldx + c));
+  }
+  const int m = __ldg(live), end = min(n, (m + gemm::kBlockK - 1) / gemm::kBlockK * gemm::kBlockK);
+  for (int r = m + w0; r < end; r += warps)
+    for (int c = lane * 8; c < D; c += 256) *reinterpret_cast<uint4*>(out + r * ld + c) = make_uint4(0, 0, 0, 0);
+}
+
+// Every row of dx: its live row's, or zeros. A warp a row.
+__global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict__ in, long long ld, int n, int D,
+                                                     const int* __restrict__ place, uint16_t* __restrict__ dx) {
+  const int warps = gridDim.x * 8, lane = threadIdx.x & 31;
+  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += warps) {
+    const int r = __ldg(place + i);
+    for (int c = lane * 8; c < D; c += 256)
+      *reinterpret_cast<uint4*>(dx + (long long)i * D + c) =
+          r < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(in + r * ld + c);
+  }
+}
+// The same from the slices' sums (gemm's Op::sum, in their order): a thread has 8 columns of a row, a warp 32 rows.
+template <typename T>
+__global__ void __launch_bounds__(256) spread_sums_kernel(const float* __restrict__ sum, int slices, int tiles_n, int n, int D,
+                                                          const int* __restrict__ live, const int* __restrict__ place,
+                                                          const float* __restrict__ factor, T* __restrict__ dx) {
+  const int i = blockIdx.x * 32 + (threadIdx.x & 31), c = (blockIdx.y * 8 + (threadIdx.x >> 5)) * 8;
+  if (i >= n || c >= D) return;
+  const int r = __ldg(place + i), rows = (__ldg(live) + gemm::kTileM - 1) / gemm::kTileM;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (r >= 0) {
+    // the tile's index as the products' kernel counts them
+    const int tm = r / gemm::kTileM, tn = c / gemm::kTileN, g = tm / gemm::kGroupM;
+    const int high = min(rows - g * gemm::kGroupM, gemm::kGroupM);
+    const int tile = g * gemm::kGroupM * tiles_n + tn * high + tm % gemm::kGroupM;
+    const float f = __ldg(factor);
+    for (int s = 0; s < slices; ++s) {
+      const long long t = (long long)s * rows * tiles_n + tile;
+      const float* at = sum + ((t * 2 + r % gemm::kTileM / gemm::kHalf) * gemm::kTileN + c % gemm::kTileN) * gemm::kHalf + r % gemm::kHalf;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += at[j * gemm::kHalf];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= f;
+  }
+  store8<T>(dx + (long long)i * D + c, v);
+}
+
+// Joins each row's parts: its maximum and the logarithm of its sum, its loss (at least 0: a sure row's sum is 1 and more); for a
+// mean or sum the last CTA adds the CTAs' sums in their order. Parts and targets lie by live rows, losses by rows.
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __restrict__ part, const float* __restrict__ target,
-                                                               int parts, int n, Labels lab, int reduction,
+                                                               int parts, int n, Plan plan, int reduction,
                                                                float2* __restrict__ lse, float* __restrict__ loss,
                                                                float2* sums, unsigned int* counter) {
   __shared__ float2 sh[kJoinWarps][kRows];
   __shared__ bool last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * kRows + lane;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = blockIdx.x * kRows + lane;
+  const int row = i < n ? __ldg(plan.place + i) : -1;
   float m = -INFINITY, s = 0.f;
   auto add = [&](float2 v) {  // (a NaN sum stays)
     const float next = wattn::max3(m, v.x, v.x), ref = next == -INFINITY ? 0.f : next;
     s = s * wattn::ex2((m - ref) * gemm::kLog2e) + v.y * wattn::ex2((v.x - ref) * gemm::kLog2e);
     m = next;
   };
-  if (row < n) {
+  if (row >= 0) {
     int p = warp;
     for (; p + 3 * kJoinWarps < parts; p += 4 * kJoinWarps) {
       float2 v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __ldcs(part + (long long)(p + i * kJoinWarps) * n + row);
+      for (int j = 0; j < 4; ++j) v[j] = __ldcs(part + (long long)(p + j * kJoinWarps) * n + row);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) add(v[i]);
+      for (int j = 0; j < 4; ++j) add(v[j]);
     }
     for (; p < parts; p += kJoinWarps) add(__ldcs(part + (long long)p * n + row));
   }
@@ -61,22 +180,18 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __r
   if (warp == 0) {
     m = -INFINITY, s = 0.f;
     for (int w = 0; w < kJoinWarps; ++w) add(sh[w][lane]);
-    float x = 0.f, kept = 0.f;
-    if (row < n) {
-      const long long l = lab.of(row);
+    float x = 0.f;
+    if (row >= 0) {
       const float rest = log2f(s);
-      if (l != lab.ignore) {
-        kept = 1.f;
-        x = l < 0 || l >= lab.V ? NAN : (m - target[row]) + kLn2 * rest;
-      }
+      x = __ldg(plan.label + row) < 0 ? NAN : (m - target[row]) + kLn2 * rest;
       if (lse != nullptr) lse[row] = make_float2(m, rest);
-      if (reduction == kNone) loss[row] = x;
     }
-    if (reduction != kNone) {
+    if (reduction == kNone) {
+      if (i < n) loss[i] = x;
+    } else {
       x = warp_sum(x);
-      kept = warp_sum(kept);
       if (lane == 0) {
-        sums[blockIdx.x] = make_float2(x, kept);
+        sums[blockIdx.x] = make_float2(x, 0.f);
         __threadfence();
         last = atomicAdd(counter, 1u) + 1u == gridDim.x;
       }
@@ -86,64 +201,46 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __r
   __syncthreads();
   if (!last) return;
   __threadfence();
-  float x = 0.f, kept = 0.f;  // (a thread's CTAs in order, then the threads': the same sum every run)
-  for (unsigned int i = threadIdx.x; i < gridDim.x; i += 32 * kJoinWarps) {
-    const float2 v = __ldcg(sums + i);
-    x += v.x;
-    kept += v.y;
-  }
+  float x = 0.f;  // (a thread's CTAs in order, then the threads': the same sum every run)
+  for (unsigned int j = threadIdx.x; j < gridDim.x; j += 32 * kJoinWarps) x += __ldcg(sums + j).x;
   x = warp_sum(x);
-  kept = warp_sum(kept);
-  if (lane == 0) sh[warp][0] = make_float2(x, kept);
+  if (lane == 0) sh[warp][0].x = x;
   __syncthreads();
   if (threadIdx.x == 0) {
-    x = kept = 0.f;
-    for (int w = 0; w < kJoinWarps; ++w) x += sh[w][0].x, kept += sh[w][0].y;
-    loss[0] = reduction == kMean ? x / kept : x;  // (no row: NaN)
+    x = 0.f;
+    for (int w = 0; w < kJoinWarps; ++w) x += sh[w][0].x;
+    loss[0] = reduction == kMean ? x / (float)*plan.live : x;  // (no row: NaN)
   }
 }
 
-// What each row's softmax - onehot is multiplied by before it is rounded, and what the products are multiplied by: g_i over the
-// largest |g| of the call, and that. A row that knows nothing of its label then has -1 exactly where it would have the rounded
+// What each live row's softmax - onehot is multiplied by before it is rounded, and what the products are multiplied by: g_i over
+// the largest |g| of the call, and that. A row that knows nothing of its label then has -1 exactly where it would have the rounded
 // -g_i, an error all rows of a mean share (up to 2^-8 of both gradients). float16 carries 2^15 more, so that D keeps its 11 bits
 // over 28 binades below its largest value. One CTA.
-__global__ void __launch_bounds__(1024) factors_kernel(const float* __restrict__ g, Labels lab, int n, int reduction, bool half,
+__global__ void __launch_bounds__(1024) factors_kernel(const float* __restrict__ g, Plan plan, int n, int reduction, bool half,
                                                        float* __restrict__ row_scale, float* __restrict__ factor) {
   __shared__ float sh[32];
-  __shared__ float share;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto all = [&](float v, bool add) {  // the sum or the maximum over the CTA
-    v = add ? warp_sum(v) : __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
-    __syncthreads();
-    if (lane == 0) sh[warp] = v;
-    __syncthreads();
-    if (warp == 0) {
-      v = sh[lane];
-      v = add ? warp_sum(v) : __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
-      if (lane == 0) share = v;
-    }
-    __syncthreads();
-    return share;
-  };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, live = *plan.live;
   float one = 0.f, top = 0.f;
   if (reduction != kNone) {
-    float c = 0.f;  // (whole numbers up to 2^24: exact)
-    for (int i = threadIdx.x; i < n; i += 1024) c += lab.of(i) != lab.ignore ? 1.f : 0.f;
-    c = all(c, true);
-    one = reduction == kMean ? g[0] / c : g[0];
-    top = c > 0.f ? fabsf(one) : 0.f;
+    one = reduction == kMean ? g[0] / (float)live : g[0];
+    top = live > 0 ? fabsf(one) : 0.f;
   } else {
     for (int i = threadIdx.x; i < n; i += 1024)
-      if (lab.of(i) != lab.ignore) top = wattn::max3(top, fabsf(g[i]), top);
-    top = all(top, false);
+      if (__ldg(plan.place + i) >= 0) top = wattn::max3(top, fabsf(g[i]), top);
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if (lane == 0) sh[warp] = top;
+    __syncthreads();
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(sh[lane])));
   }
   const float lift = half ? 32768.f : 1.f;
   const bool plain = !(top < INFINITY);  // an infinity or NaN goes the way it came
   if (threadIdx.x == 0) *factor = plain ? 1.f : top / lift;
   for (int i = threadIdx.x; i < n; i += 1024) {
-    const long long l = lab.of(i);
+    const int r = __ldg(plan.place + i);
+    if (r < 0) continue;
     const float x = reduction == kNone ? g[i] : one;
-    row_scale[i] = l == lab.ignore ? 0.f : l < 0 || l >= lab.V ? NAN : plain ? x : top > 0.f ? x / top * lift : 0.f;
+    row_scale[r] = __ldg(plan.label + r) < 0 ? NAN : plain ? x : top > 0.f ? x / top * lift : 0.f;
   }
 }
 
@@ -151,16 +248,20 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 constexpr size_t kHead = 256;  // the error word, the join's counter (at 64), the products' factor (at 128)
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
+long long pitch(int D) { return (D + 63) / 64 * 64; }  // of the packed rows: whole 128-byte lines
+int grid_of(long long rows) { return (int)(rows < 8 * 592 ? (rows + 7) / 8 : 592); }
 
 struct FwdPlan {
   int parts, ctas;
-  size_t part, target, sums, total;
+  size_t plan, rows, part, target, sums, total;
 };
-FwdPlan fwd_plan(long long n, int V) {
+FwdPlan fwd_plan(long long n, int D, int V) {
   FwdPlan f;
   f.parts = gemm::blocks_of(V, kPart);
   f.ctas = gemm::blocks_of(n, kRows);
-  f.part = kHead;
+  f.plan = kHead;
+  f.rows = f.plan + up((size_t)kPlanInts((int)n) * 4);
+  f.part = f.rows + up((size_t)n * pitch(D) * 2);
   f.target = f.part + up((size_t)f.parts * n * sizeof(float2));
   f.sums = f.target + up((size_t)n * sizeof(float));
   f.total = f.sums + up((size_t)f.ctas * sizeof(float2));
@@ -168,11 +269,14 @@ FwdPlan fwd_plan(long long n, int V) {
 }
 
 // The pieces of the vocabulary: D of one piece takes at most kPieceBytes (a multiple of a tile's columns, at least one tile).
+// One piece and few tiles of dx: its contraction over the vocabulary, far longer than a tile of dW's over the rows, is cut into
+// slices of about half of a pair's share of the whole, with fp32 sums of their own. At 1,500 rows (half of them live), 768 wide, a
+// vocabulary of 32,003: SLICES.
 constexpr size_t kPieceBytes = (size_t)256 << 20;
 struct BwdPlan {
-  int pieces, cols;  // cols: of every piece but the last
+  int pieces, cols, slices, per;  // cols: of every piece but the last; per: stages of a slice
   long long ldd;
-  size_t rows, d, sum, total;
+  size_t scale, rows, dx, d, sum, total;
 };
 BwdPlan bwd_plan(long long n, int D, int V) {
   BwdPlan b;
@@ -182,12 +286,26 @@ BwdPlan bwd_plan(long long n, int D, int V) {
   b.cols = gemm::blocks_of(gemm::blocks_of(V, b.pieces), gemm::kTileN) * gemm::kTileN;
   b.pieces = gemm::blocks_of(V, b.cols);
   b.ldd = b.pieces > 1 ? b.cols : (V + 63ll) / 64 * 64;
-  b.rows = kHead;
-  b.d = b.rows + up((size_t)n * sizeof(float));
+  const long long tiles_m = gemm::blocks_of(n, gemm::kTileM), tiles_n = gemm::blocks_of(D, gemm::kTileN);
+  b.slices = 1, b.per = gemm::blocks_of(V, gemm::kBlockK);
+  if (b.pieces == 1) {
+    const long long kv = b.per, kn = gemm::blocks_of(n, gemm::kBlockK), tiles = tiles_m * tiles_n;
+    long long share = (tiles * kv + gemm::blocks_of(V, gemm::kTileM) * tiles_n * kn) / 74 / 2;
+    if (share < 16) share = 16;
+    if (kv > share) {
+      b.slices = gemm::blocks_of(kv, (int)share);
+      const long long room = (64ll << 20) / (tiles * gemm::kTileM * gemm::kTileN * 4);  // 64 MiB of sums
+      if (b.slices > room) b.slices = room < 1 ? 1 : (int)room;
+      b.per = gemm::blocks_of(kv, b.slices);
+      b.slices = gemm::blocks_of(kv, b.per);
+    }
+  }
+  b.scale = kHead;
+  b.rows = b.scale + up((size_t)n * sizeof(float));
+  b.dx = b.rows + up((size_t)n * pitch(D) * 2);
+  b.d = b.dx + up((size_t)n * pitch(D) * 2);
   b.sum = b.d + up((size_t)n * b.ldd * 2);
-  b.total = b.sum + (b.pieces > 1 ? (size_t)gemm::blocks_of(n, gemm::kTileM) * gemm::blocks_of(D, gemm::kTileN) *
-                                        (gemm::kTileM * gemm::kTileN * sizeof(float))
-                                  : 0);
+  b.total = b.sum + (b.pieces > 1 || b.slices > 1 ? (size_t)b.slices * tiles_m * tiles_n * (gemm::kTileM * gemm::kTileN * sizeof(float)) : 0);
   return b;
 }
 
@@ -195,35 +313,43 @@ struct Problem {
   const void *x, *w;
   long long ldx, ldw;
   int n, D, V;
-  Labels lab;
+  Plan plan;
   int reduction;
 };
-
-void label_params(Params& p, const Problem& q, ErrorWord* err) {
-  p.labels = q.lab.at, p.label64 = q.lab.is64, p.ignore = q.lab.ignore, p.err = err;
-}
 
 void shape(Op& op, long long M, long long N) {
   op.M = (int)M, op.N = (int)N;
   op.tiles_m = gemm::blocks_of(M, gemm::kTileM), op.tiles_n = gemm::blocks_of(N, gemm::kTileN);
 }
 
+int gather(const Problem& q, void* rows, char* ws, bool head, cudaStream_t stream) {
+  gather_kernel<<<grid_of(q.n), 256, 0, stream>>>(static_cast<const uint16_t*>(q.x), q.ldx, q.n, q.D, q.plan.live, q.plan.place,
+                                                  static_cast<uint16_t*>(rows), pitch(q.D),
+                                                  head ? reinterpret_cast<int*>(ws) : nullptr);
+  return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
+}
+
 template <typename T>
-int forward(const Problem& q, float* loss, float2* lse, char* ws, cudaStream_t stream) {
+int forward(const Problem& q, const Labels& lab, float* loss, float2* lse, char* ws, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
-  const FwdPlan f = fwd_plan(q.n, q.V);
+  const FwdPlan f = fwd_plan(q.n, q.D, q.V);
+  const int step = gemm::blocks_of(q.n, 592) < 32 ? 32 : gemm::blocks_of(q.n, 592);
+  plan_kernel<<<gemm::blocks_of(q.n, step), kPlanThreads, 0, stream>>>(lab, q.n, step, q.plan, reinterpret_cast<int*>(ws));
+  if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
+  if (const int st = gather(q, ws + f.rows, ws, false, stream)) return st;
   Params p = {};
-  p.ops = 1;
-  label_params(p, q, reinterpret_cast<ErrorWord*>(ws));
+  p.ops = 1, p.err = reinterpret_cast<ErrorWord*>(ws), p.live = q.plan.live, p.labels = q.plan.label;
   p.part = reinterpret_cast<float2*>(ws + f.part);
   p.target = reinterpret_cast<float*>(ws + f.target);
   Op& o = p.op[0];
   shape(o, q.n, q.V);
+  o.m_live = true;
   o.kb[0] = gemm::blocks_of(q.D, gemm::kBlockK);
-  if (!gemm::operand_map(&o.a[0], q.x, dt, q.n, q.D, q.ldx, false) || !gemm::operand_map(&o.b[0], q.w, dt, q.V, q.D, q.ldw, false))
+  if (!gemm::operand_map(&o.a[0], ws + f.rows, dt, q.n, q.D, pitch(q.D), false) ||
+      !gemm::operand_map(&o.b[0], q.w, dt, q.V, q.D, q.ldw, false))
     return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kLse>(p, stream)) return st;
-  join_kernel<<<f.ctas, 32 * kJoinWarps, 0, stream>>>(p.part, p.target, f.parts, q.n, q.lab, q.reduction, lse, loss,
+  join_kernel<<<f.ctas, 32 * kJoinWarps, 0, stream>>>(p.part, p.target, f.parts, q.n, q.plan, q.reduction, lse, loss,
                                                      reinterpret_cast<float2*>(ws + f.sums),
                                                      reinterpret_cast<unsigned int*>(ws + 64));
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
@@ -233,53 +359,70 @@ template <typename T>
 int backward(const Problem& q, const float2* lse, const float* dloss, void* dx, void* dw, char* ws, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const BwdPlan b = bwd_plan(q.n, q.D, q.V);
-  float* const row_scale = reinterpret_cast<float*>(ws + b.rows);
+  const long long ld = pitch(q.D);
+  void *const rows = ws + b.rows, *const dxc = ws + b.dx, *const d = ws + b.d;
+  float* const row_scale = reinterpret_cast<float*>(ws + b.scale);
   float* const factor = reinterpret_cast<float*>(ws + 128);
-  factors_kernel<<<1, 1024, 0, stream>>>(dloss, q.lab, q.n, q.reduction, std::is_same<T, __half>::value, row_scale, factor);
+  if (const int st = gather(q, rows, ws, true, stream)) return st;
+  factors_kernel<<<1, 1024, 0, stream>>>(dloss, q.plan, q.n, q.reduction, std::is_same<T, __half>::value, row_scale, factor);
   if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  void* const d = ws + b.d;
   const int kd = gemm::blocks_of(q.D, gemm::kBlockK);
   for (int i = 0; i < b.pieces; ++i) {
     const long long v0 = (long long)i * b.cols;
     const int cols = (int)(q.V - v0 < b.cols ? q.V - v0 : b.cols);
     const char* w = static_cast<const char*>(q.w) + v0 * q.ldw * 2;
     Params p = {};
-    p.ops = 1;
-    label_params(p, q, reinterpret_cast<ErrorWord*>(ws));
+    p.ops = 1, p.err = reinterpret_cast<ErrorWord*>(ws), p.live = q.plan.live, p.labels = q.plan.label;
     p.v0 = (int)v0, p.lse = lse, p.row_scale = row_scale;
     Op& o = p.op[0];
     shape(o, q.n, cols);
+    o.m_live = true;
     o.kb[0] = kd;
-    if (!gemm::operand_map(&o.a[0], q.x, dt, q.n, q.D, q.ldx, false) || !gemm::operand_map(&o.b[0], w, dt, cols, q.D, q.ldw, false) ||
+    if (!gemm::operand_map(&o.a[0], rows, dt, q.n, q.D, ld, false) || !gemm::operand_map(&o.b[0], w, dt, cols, q.D, q.ldw, false) ||
         !gemm::slab_map(&o.c, d, dt, q.n, cols, b.ldd))
       return GD_ERR_LAUNCH;
     if (const int st = gemm::launch<T, gemm::kDLogit>(p, stream)) return st;
     Params r = {};
-    r.err = p.err;
+    r.err = p.err, r.live = q.plan.live;
     bool ok = true;
     if (dx != nullptr) {  // dx += D W
       Op& g = r.op[r.ops++];
       shape(g, q.n, q.D);
+      g.m_live = true;
       g.kb[0] = gemm::blocks_of(cols, gemm::kBlockK);
       g.b_mn = true;
-      g.sum_mode = b.pieces == 1 ? 0 : i == 0 ? 1 : i + 1 < b.pieces ? 2 : 3;
+      g.slices = b.slices, g.per = b.per;
+      g.sum_mode = b.slices > 1 ? 1 : b.pieces == 1 ? 0 : i == 0 ? 1 : i + 1 < b.pieces ? 2 : 3;
       g.sum = reinterpret_cast<float*>(ws + b.sum);
       g.factor = factor;
       ok = ok && gemm::operand_map(&g.a[0], d, dt, q.n, cols, b.ldd, false) &&
-           gemm::operand_map(&g.b[0], w, dt, cols, q.D, q.ldw, true) && gemm::slab_map(&g.c, dx, dt, q.n, q.D, q.D);
+           gemm::operand_map(&g.b[0], w, dt, cols, q.D, q.ldw, true) && gemm::slab_map(&g.c, dxc, dt, q.n, q.D, ld);
     }
     if (dw != nullptr) {  // dW = D^T x
       Op& g = r.op[r.ops++];
       shape(g, cols, q.D);
+      g.k_live = true;
       g.kb[0] = gemm::blocks_of(q.n, gemm::kBlockK);
       g.a_mn = g.b_mn = true;
       g.factor = factor;
       ok = ok && gemm::operand_map(&g.a[0], d, dt, q.n, cols, b.ldd, true) &&
-           gemm::operand_map(&g.b[0], q.x, dt, q.n, q.D, q.ldx, true) &&
+           gemm::operand_map(&g.b[0], rows, dt, q.n, q.D, ld, true) &&
            gemm::slab_map(&g.c, static_cast<char*>(dw) + v0 * q.D * 2, dt, cols, q.D, q.D);
     }
     if (!ok) return GD_ERR_LAUNCH;
     if (const int st = gemm::launch<T, gemm::kStore>(r, stream)) return st;
+  }
+  if (dx != nullptr) {
+    if (b.slices > 1) {
+      const dim3 grid((unsigned)gemm::blocks_of(q.n, 32), (unsigned)gemm::blocks_of(q.D, 64));
+      spread_sums_kernel<T><<<grid, 256, 0, stream>>>(reinterpret_cast<const float*>(ws + b.sum), b.slices,
+                                                      gemm::blocks_of(q.D, gemm::kTileN), q.n, q.D, q.plan.live, q.plan.place, factor,
+                                                      static_cast<T*>(dx));
+    } else {
+      spread_kernel<<<grid_of(q.n), 256, 0, stream>>>(static_cast<const uint16_t*>(dxc), ld, q.n, q.D, q.plan.place,
+                                                      static_cast<uint16_t*>(dx));
+    }
+    if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   }
   return GD_OK;
 }
@@ -304,11 +447,11 @@ bool bind_context() {
 extern "C" size_t gd_xent_workspace_bytes(long long rows, int D, int V, int for_backward) {
   using namespace gd::xent;
   if (check(GD_BFLOAT16, kNone, rows, D, V, D, D) != GD_OK || rows == 0) return 0;
-  return for_backward ? bwd_plan(rows, D, V).total : fwd_plan(rows, V).total;
+  return for_backward ? bwd_plan(rows, D, V).total : fwd_plan(rows, D, V).total;
 }
 
 extern "C" int gd_xent_fwd(const void* x, const void* w, const void* labels, int label64, float* loss, float* lse,
-                           int reduction, long long ignore, int dtype, long long rows, int D, int V, long long ldx,
+                           int* plan, int reduction, long long ignore, int dtype, long long rows, int D, int V, long long ldx,
                            long long ldw, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace gd::xent;
   if (const int st = check(dtype, reduction, rows, D, V, ldx, ldw)) return st;
@@ -318,30 +461,30 @@ extern "C" int gd_xent_fwd(const void* x, const void* w, const void* labels, int
   if (workspace == nullptr || workspace_bytes < gd_xent_workspace_bytes(rows, D, V, 0)) return GD_ERR_WORKSPACE;
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  if (cudaMemsetAsync(workspace, 0, kHead, cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  const Problem q = {x, w, ldx, ldw, (int)rows, D, V, {labels, label64, ignore, V}, reduction};
   char* ws = static_cast<char*>(workspace);
+  int* const at = plan != nullptr ? plan : reinterpret_cast<int*>(ws + fwd_plan(rows, D, V).plan);
+  const Problem q = {x, w, ldx, ldw, (int)rows, D, V, Plan::of(at, (int)rows), reduction};
+  const Labels lab = {labels, label64, ignore, V};
   float2* const kept = reinterpret_cast<float2*>(lse);
-  return dtype == GD_FLOAT16 ? forward<__half>(q, loss, kept, ws, cs) : forward<__nv_bfloat16>(q, loss, kept, ws, cs);
+  return dtype == GD_FLOAT16 ? forward<__half>(q, lab, loss, kept, ws, cs) : forward<__nv_bfloat16>(q, lab, loss, kept, ws, cs);
 }
 
-extern "C" int gd_xent_bwd(const void* x, const void* w, const void* labels, int label64, const float* lse, const float* dloss,
-                           void* dx, void* dw, int reduction, long long ignore, int dtype, long long rows, int D, int V,
-                           long long ldx, long long ldw, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int gd_xent_bwd(const void* x, const void* w, const float* lse, const int* plan, const float* dloss, void* dx, void* dw,
+                           int reduction, int dtype, long long rows, int D, int V, long long ldx, long long ldw, void* workspace,
+                           size_t workspace_bytes, void* stream) {
   using namespace gd::xent;
   if (const int st = check(dtype, reduction, rows, D, V, ldx, ldw)) return st;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   if (rows == 0)
     return dw == nullptr || cudaMemsetAsync(dw, 0, (size_t)V * D * 2, cs) == cudaSuccess ? GD_OK
                                                                                          : (cudaGetLastError(), GD_ERR_LAUNCH);
-  if (x == nullptr || w == nullptr || labels == nullptr || lse == nullptr || dloss == nullptr) return GD_ERR_ARG;
+  if (x == nullptr || w == nullptr || lse == nullptr || plan == nullptr || dloss == nullptr) return GD_ERR_ARG;
   if (!aligned16(x) || !aligned16(w) || !aligned16(dx) || !aligned16(dw) || !aligned16(lse) || !aligned16(workspace))
     return GD_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < gd_xent_workspace_bytes(rows, D, V, 1)) return GD_ERR_WORKSPACE;
   if (dx == nullptr && dw == nullptr) return GD_OK;
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  if (cudaMemsetAsync(workspace, 0, kHead, cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  const Problem q = {x, w, ldx, ldw, (int)rows, D, V, {labels, label64, ignore, V}, reduction};
+  const Problem q = {x, w, ldx, ldw, (int)rows, D, V, Plan::of(const_cast<int*>(plan), (int)rows), reduction};
   char* ws = static_cast<char*>(workspace);
   const float2* const kept = reinterpret_cast<const float2*>(lse);
   return dtype == GD_FLOAT16 ? backward<__half>(q, kept, dloss, dx, dw, ws, cs)

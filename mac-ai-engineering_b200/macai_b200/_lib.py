@@ -76,8 +76,8 @@ _SIGS = {
     "gd_ff_fwd": ([_P] * 7 + [_I, _LL, _I, _I, _I, ctypes.POINTER(_LL), _P, _SZ, _P], _I),
     "gd_ff_bwd": ([_P] * 11 + [_I, _LL, _I, _I, _I, ctypes.POINTER(_LL), _P, _SZ, _P], _I),
     "gd_xent_workspace_bytes": ([_LL] + [_I] * 3, _SZ),
-    "gd_xent_fwd": ([_P] * 3 + [_I, _P, _P, _I, _LL, _I, _LL, _I, _I, _LL, _LL, _P, _SZ, _P], _I),
-    "gd_xent_bwd": ([_P] * 3 + [_I] + [_P] * 4 + [_I, _LL, _I, _LL, _I, _I, _LL, _LL, _P, _SZ, _P], _I),
+    "gd_xent_fwd": ([_P] * 3 + [_I, _P, _P, _P, _I, _LL, _I, _LL, _I, _I, _LL, _LL, _P, _SZ, _P], _I),
+    "gd_xent_bwd": ([_P] * 7 + [_I, _I, _LL, _I, _I, _LL, _LL, _P, _SZ, _P], _I),
     "gd_rule_step": ([_P] * 10 + [_I] * 10 + [_P], _I),
     "gd_rotary": ([_P] * 6 + [_I, _LL, _LL] + [_I] * 7 + [_LL] * 6 + [_I, _I, _P], _I),
 }

@@ -30,21 +30,25 @@ def _bytes(*sizes) -> int:
 
 
 def _fwd(x, w, labels, ignore, reduction, keep):
-    """(loss, lse): lse, the rows' maxima and sums (as logarithms), for the backward (else None)."""
+    """(loss, lse, plan): lse, the live rows' maxima and sums (as logarithms), and plan, which rows those are, for the
+    backward (else None)."""
     n, D = x.shape
     loss = torch.empty(n if reduction == 0 else (), dtype=torch.float32, device=x.device)
-    lse = torch.empty((n, 2), dtype=torch.float32, device=x.device) if keep else None
+    lse = plan = None
+    if keep:
+        lse = torch.empty((n, 2), dtype=torch.float32, device=x.device)
+        plan = torch.empty(4 + 2 * n, dtype=torch.int32, device=x.device)
     if n == 0:  # no row: torch's own results, a mean over nothing among them
-        return loss.fill_(float("nan") if reduction == 1 else 0.0), lse
+        return loss.fill_(float("nan") if reduction == 1 else 0.0), lse, plan
     size = _bytes(n, D, w.shape[0], 0)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     launch("gd_xent_fwd", x.get_device(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.dtype == torch.int64,
-           loss.data_ptr(), None if lse is None else lse.data_ptr(), reduction, ignore, _DTYPES[x.dtype], n, D, w.shape[0],
+           loss.data_ptr(), None if lse is None else lse.data_ptr(), None if plan is None else plan.data_ptr(), reduction, ignore, _DTYPES[x.dtype], n, D, w.shape[0],
            pitch(x), pitch(w), ws.data_ptr(), size)
-    return loss, lse
+    return loss, lse, plan
 
 
-def _bwd(x, w, labels, lse, dloss, ignore, reduction, need):
+def _bwd(x, w, lse, plan, dloss, reduction, need):
     """(dx, dw), contiguous, each None unless needed."""
     n, D = x.shape
     V = w.shape[0]
@@ -53,9 +57,8 @@ def _bwd(x, w, labels, lse, dloss, ignore, reduction, need):
     size = _bytes(n, D, V, 1) if n else 0
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if n else None
     p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    launch("gd_xent_bwd", x.get_device(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.dtype == torch.int64,
-           lse.data_ptr(), dloss.data_ptr(), p(dx), p(dw), reduction, ignore, _DTYPES[x.dtype], n, D, V, pitch(x), pitch(w),
-           p(ws), size)
+    launch("gd_xent_bwd", x.get_device(), x.data_ptr(), w.data_ptr(), lse.data_ptr(), plan.data_ptr(), dloss.data_ptr(), p(dx),
+           p(dw), reduction, _DTYPES[x.dtype], n, D, V, pitch(x), pitch(w), p(ws), size)
     return dx, dw
 
 
@@ -64,16 +67,15 @@ class LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, labels, ignore, reduction):
-        loss, lse = _fwd(x, w, labels, ignore, reduction, True)
-        ctx.save_for_backward(x, w, labels, lse)
-        ctx.args = (ignore, reduction)
+        loss, lse, plan = _fwd(x, w, labels, ignore, reduction, True)
+        ctx.save_for_backward(x, w, lse, plan)
+        ctx.reduction = reduction
         return loss
 
     @staticmethod
     @first_order
     def backward(ctx, dloss):
-        x, w, labels, lse = ctx.saved_tensors
-        dx, dw = _bwd(x, w, labels, lse, dloss.float().contiguous(), *ctx.args, ctx.needs_input_grad)
+        dx, dw = _bwd(*ctx.saved_tensors, dloss.float().contiguous(), ctx.reduction, ctx.needs_input_grad)
         return dx, dw, None, None, None
 
 
@@ -85,8 +87,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     ignore_index has loss 0 and a zero row in x's gradient, whatever it holds (in the weight's, its infinities and NaN meet a
     weight of 0, as in the formula's product); any other label outside [0, V) gives NaN (nothing waits for the host to look). Gradients of x and weight come in their type, the same bits every run; a frozen one's is not formed.
 
-    The logits are never kept: beside the gradients a call holds 8 bytes for each row and 128 columns, the backward at most
-    256 MiB (or 256 columns) of the logits' gradients and, with more than one such piece, x's gradient in float32."""
+    Ignored rows cost no products. The logits are never kept: beside the gradients a call holds the other rows of x and 8 bytes
+    for each row and 128 columns; the backward at most 256 MiB (or 256 columns) of the logits' gradients, x's gradient once
+    more, and float32 sums of it (with several pieces of 256 MiB one for each value, else at most 64 MiB)."""
     name = "linear_cross_entropy"
     if reduction not in _REDUCTIONS:
         raise ValueError(f"{name}: reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
