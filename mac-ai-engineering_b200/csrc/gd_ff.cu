@@ -21,6 +21,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __half* __restrict__ 
     const __half* p = is_dy ? dy + r * ldy : wd + (r - rows) * ldd;
     const int n = is_dy ? O : F;
     float sum = 0.f, m = 0.f;
+#pragma unroll 4
     for (int c = lane * 8; c < n; c += 256) {
       float v[8];
       load8<__half>(p + c, v);
@@ -33,10 +34,14 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __half* __restrict__ 
     if (is_dy) top_sum = wattn::max3(top_sum, warp_sum(sum), top_sum);
     else top = wattn::max3(top, m, top);
   }
-  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-  if (lane == 0) {
-    atomicMax(bounds, __float_as_uint(top_sum));
-    atomicMax(bounds + 1, __float_as_uint(top));
+  __shared__ uint32_t sh[2][8];
+  const uint32_t high = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if (lane == 0) sh[0][threadIdx.x >> 5] = __float_as_uint(top_sum), sh[1][threadIdx.x >> 5] = high;
+  __syncthreads();
+  if (threadIdx.x < 2) {  // (one atomic a CTA and maximum)
+    uint32_t m = 0;
+    for (int i = 0; i < 8; ++i) m = max(m, sh[threadIdx.x][i]);
+    atomicMax(bounds + threadIdx.x, m);
   }
 }
 
@@ -78,17 +83,17 @@ struct Grads {
 
 template <typename T>
 int backward(const Problem& q, const void* const* kept, const void* dy, long long ldy, const Grads& out, void* dg, void* du,
-             void* h, uint32_t* bounds, ErrorWord* err, cudaStream_t stream) {
+             void* h, const uint32_t* bounds, uint32_t* own, ErrorWord* err, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const long long n = q.rows, lf = pitch(q.F);
   if (bounds != nullptr) {
     const int rows = q.rows + q.O;
     bounds_kernel<<<rows < 8 * 592 ? (rows + 7) / 8 : 592, 256, 0, stream>>>(
-        static_cast<const __half*>(dy), ldy, q.rows, q.O, static_cast<const __half*>(q.wd), q.ldd, q.F, bounds + 2);
+        static_cast<const __half*>(dy), ldy, q.rows, q.O, static_cast<const __half*>(q.wd), q.ldd, q.F, own);
     if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   }
   Params p = {};
-  p.ops = 1, p.err = err, p.keep = out.dwd != nullptr, p.bounds = bounds;
+  p.ops = 1, p.err = err, p.keep = out.dwd != nullptr, p.bounds = const_cast<uint32_t*>(bounds), p.more = own;
   Op& o = p.op[0];
   shape(o, n, q.F);  // dh = dy Wd
   o.kb[0] = gemm::blocks_of(q.O, gemm::kBlockK);
@@ -101,7 +106,7 @@ int backward(const Problem& q, const void* const* kept, const void* dy, long lon
     if (!gemm::strip_map(&p.x[i], kept[i], dt, n, q.F, lf)) return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kDSwiglu>(p, stream)) return st;
   Params r = {};
-  r.err = err, r.bounds = bounds;
+  r.err = err, r.bounds = const_cast<uint32_t*>(bounds), r.more = own;
   bool ok = true;
   const int kn = gemm::blocks_of(n, gemm::kBlockK);
   auto weight = [&](void* dw, const void* a, long long lda, long long M, const void* b, long long ldb, long long N, bool scaled) {
@@ -136,7 +141,8 @@ int check(int dtype, long long rows, int D, int F, int O, const long long* ld, i
   if (dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) return GD_ERR_ARG;
   constexpr int kMost = 1 << 24;
   if (rows < 0 || rows > (1ll << 30) || D <= 0 || F <= 0 || O <= 0 || D % 8 || F % 8 || O % 8 || D > kMost || F > kMost ||
-      O > kMost)
+      O > kMost || !gemm::countable(rows, F) || !gemm::countable(rows, D) || !gemm::countable(rows, O) || !gemm::countable(F, D) ||
+      !gemm::countable(F, O))
     return GD_ERR_SHAPE;
   if (ld == nullptr) return GD_ERR_ARG;
   const long long least[5] = {D, D, D, F, O};
@@ -217,18 +223,14 @@ extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, co
   if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
   gd::ErrorWord* err = static_cast<gd::ErrorWord*>(workspace);
   char* const at = static_cast<char*>(workspace);
-  uint32_t* own = nullptr;
   if (cudaMemsetAsync(workspace, 0, kHead, cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  if (dtype == GD_FLOAT16) {  // the forward's two maxima, and room for this call's
-    own = reinterpret_cast<uint32_t*>(at + 128);
-    if (cudaMemcpyAsync(own, bounds, 8, cudaMemcpyDeviceToDevice, cs) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  }
+  uint32_t* const own = reinterpret_cast<uint32_t*>(at + 128);  // float16's two maxima of this call
   const Problem q = {x, w_gate, w_up, w_down, ld[0], ld[1], ld[2], ld[3], (int)rows, D, F, O};
   const Grads out = {dx, dw_gate, dw_up, dw_down};
   const size_t m = matrix_bytes(rows, F);
   void *dg = at + kHead, *du = at + kHead + m, *h = at + kHead + 2 * m;
   const void* planes[3];
   for (int i = 0; i < 3; ++i) planes[i] = static_cast<const char*>(kept) + i * (size_t)rows * pitch(F) * 2;
-  return dtype == GD_FLOAT16 ? backward<__half>(q, planes, dy, ld[4], out, dg, du, h, own, err, cs)
-                             : backward<__nv_bfloat16>(q, planes, dy, ld[4], out, dg, du, h, nullptr, err, cs);
+  return dtype == GD_FLOAT16 ? backward<__half>(q, planes, dy, ld[4], out, dg, du, h, bounds, own, err, cs)
+                             : backward<__nv_bfloat16>(q, planes, dy, ld[4], out, dg, du, h, nullptr, nullptr, err, cs);
 }

@@ -12,6 +12,8 @@
 // tile's epilogue runs under the next one's products. The CTAs are persistent and walk the tiles of up to kMaxOps problems.
 #pragma once
 
+#include <algorithm>
+
 #include "gd_wattn.cuh"
 
 namespace gd {
@@ -68,8 +70,8 @@ struct Params {
   CUtensorMap x[3];         // g and u as they are kept: the upper halves of their float32 bits, and the bytes below them
   CUtensorMap y[2];         // kDSwiglu: du (Op::c is dg), h
   bool keep;                // kSwiglu: store g, u; kDSwiglu: store h
-  // float16's feed-forward block: the bits of max |g|, max |u| (kSwiglu collects them), max ||dy row||_1, max |w_down|
-  uint32_t* bounds;
+  // float16's feed-forward block: the bits of max |g|, max |u| (kSwiglu collects them); max ||dy row||_1, max |w_down|
+  uint32_t *bounds, *more;
   // kLse, kDLogit
   const int* labels;        // of the live rows (-1: none in the vocabulary)
   int v0;                   // the first column's place in the vocabulary
@@ -209,6 +211,22 @@ __device__ __forceinline__ int all_tiles(const Params& p, int live) {
   for (int i = 0; i < (E == kStore ? p.ops : 1); ++i) n += tiles_of(p.op[i], live);
   return n;
 }
+// The tiles that a pair takes: the first problem's in turn; then, where some pairs have one tile of it more, the others make up for
+// that with later problems' (shorter) tiles before all take turns again. (7,370 live rows, 2,048 wide, 16,128 words: three or four
+// tiles of dx of 252 stages for each pair and 504 tiles of dW of 116: WALK)
+struct Walk {
+  int pair, pairs, tiles, first, mine, behind, extra;  // first: the first problem's tiles; behind: pairs with one less of them
+  template <int E>
+  __device__ __forceinline__ static Walk of(const Params& p, int live, int pair, int pairs);
+  __device__ __forceinline__ int operator()(int i) const {  // the pair's i-th tile, or -1
+    if (i < mine) return pair + i * pairs;
+    i -= mine;
+    const bool late = pair >= pairs - behind;
+    if (late && i < extra) return first + pair - (pairs - behind) + i * behind;
+    const int t = first + extra * behind + pair + (late ? i - extra : i) * pairs;
+    return t < tiles ? t : -1;
+  }
+};
 struct Where {
   int op, at, slice, m, n;  // the problem, the tile in it, its slice, the tile's first row and column
 };
@@ -241,6 +259,21 @@ __device__ __forceinline__ int stages_of(const Op& o, const Where& w, int s, int
   const int n = s == 0 && o.k_live ? (live + kBlockK - 1) / kBlockK : o.kb[s];
   from = w.slice * o.per;
   return o.slices == 1 ? n : n - from < o.per ? (n > from ? n - from : 0) : o.per;
+}
+
+template <int E>
+__device__ __forceinline__ Walk Walk::of(const Params& p, int live, int pair, int pairs) {
+  Walk w;
+  w.pair = pair, w.pairs = pairs, w.tiles = all_tiles<E>(p, live), w.first = tiles_of(p.op[0], live);
+  w.mine = w.first > pair ? (w.first - pair + pairs - 1) / pairs : 0;
+  w.behind = pairs - w.first % pairs, w.extra = 0;
+  if (E == kStore && p.ops > 1 && w.behind < pairs) {
+    auto length = [&](const Op& o) { return o.slices > 1 ? o.per : (o.k_live ? (live + kBlockK - 1) / kBlockK : o.kb[0]) + o.kb[1]; };
+    const int next = length(p.op[1]);
+    if (next > 0) w.extra = length(p.op[0]) / next;
+    if (w.extra > (w.tiles - w.first) / w.behind) w.extra = (w.tiles - w.first) / w.behind;
+  }
+  return w;
 }
 
 __device__ __forceinline__ uint32_t slab_at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
@@ -301,10 +334,10 @@ __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f +
 
 // The power of two that dg and du carry in float16, the same for a whole call: |dh| <= ||dy row||_1 max |w_down|, |silu'| < 1.1
 // and |silu(g)| <= |g| bound both by B, and 2^15 is the largest power of two in range. Without a bound above 0: 1.
-__device__ __forceinline__ float carried(const uint32_t* b) {
+__device__ __forceinline__ float carried(const uint32_t* b, const uint32_t* more) {
   if (b == nullptr) return 1.f;
   const float g = __uint_as_float(b[0]), u = __uint_as_float(b[1]);
-  const float most = __uint_as_float(b[2]) * __uint_as_float(b[3]) * fmaxf(g, 1.1f * u);
+  const float most = __uint_as_float(more[0]) * __uint_as_float(more[1]) * fmaxf(g, 1.1f * u);
   if (!(most > 0.f && most < INFINITY)) return 1.f;
   const int e = 14 - ilogbf(most);
   return ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e);
@@ -327,7 +360,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = __shfl_sync(0xffffffffu, cluster_rank(), 0);
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int live = p.live == nullptr ? 0 : __ldg(p.live), tiles = all_tiles<E>(p, live);
+  const int live = p.live == nullptr ? 0 : __ldg(p.live);
+  const Walk walk = Walk::of<E>(p, live, pair, pairs);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
@@ -359,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     const uint32_t lead = elect();
     int slot = 0, laps = 0, issued = 0;
     bool ok = true;
-    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+    for (int i = 0, tile; ok && (tile = walk(i)) >= 0; ++i) {
       Where w = locate<E>(p, tile, live);
       w.op = __shfl_sync(0xffffffffu, w.op, 0);
       const Op& op = p.op[w.op];
@@ -417,7 +451,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       const uint32_t lead = elect();
       int slot = 0, laps = 0, it = 0;
       bool ok = true;
-      for (int tile = pair; ok && tile < tiles; tile += pairs, ++it) {
+      for (int tile; ok && (tile = walk(it)) >= 0; ++it) {
         const Where w = locate<E>(p, tile, live);
         const Op& op = p.op[w.op];
         const int buf = it & 1;
@@ -481,9 +515,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         for (int i = 0; i < 3; ++i) load_slab(to + i * kStrip, &p.x[i], n0, m0, aux + 2 * ew + (at & 1));
       }
     };
-    if (E == kDSwiglu && pair < tiles) fetch(0, locate<E>(p, pair, live));
+    if (E == kDSwiglu && walk(0) >= 0) fetch(0, locate<E>(p, walk(0), live));
     uint32_t landed = 0;  // kDSwiglu: the phase of each set's barrier (a step past the matrix loads nothing)
-    for (int tile = pair; tile < tiles; tile += pairs, ++it) {
+    for (int tile; (tile = walk(it)) >= 0; ++it) {
       const Where w = locate<E>(p, tile, live);
       const Op& op = p.op[w.op];
       const int buf = it & 1, m0 = w.m + (int)rank * kHalf + quad * 32, row = m0 + lane;
@@ -500,7 +534,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       };
 
       if constexpr (E == kStore) {
-        const float f = (op.factor != nullptr ? __ldg(op.factor) : op.unscale ? 1.f / carried(p.bounds) : 1.f) + bad;
+        const float f = (op.factor != nullptr ? __ldg(op.factor) : op.unscale ? 1.f / carried(p.bounds, p.more) : 1.f) + bad;
         float* sum = op.sum_mode == 0 ? nullptr
                                       : op.sum + (((long long)w.at * 2 + rank) * kTileN + half * 128) * kHalf +
                                             quad * 32 + lane;
@@ -586,7 +620,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           }
         }
       } else if constexpr (E == kDSwiglu) {
-        const float f = carried(p.bounds) + bad;
+        const float f = carried(p.bounds, p.more) + bad;
 #pragma unroll 1
         for (int s = 0; s < 4; ++s, ++step) {
           const int c = half * 128 + s * 32, n0 = w.n + c, set = step & 1;
@@ -599,7 +633,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
             landed ^= 1u << set;
           }
           if (s < 3) fetch(step + 1, w);
-          else if (tile + pairs < tiles) fetch(step + 1, locate<E>(p, tile + pairs, live));
+          else if (walk(it + 1) >= 0) fetch(step + 1, locate<E>(p, walk(it + 1), live));
           if (!here) continue;
           const uint32_t strips = slab + set * 3 * kStrip;
 #pragma unroll
@@ -708,9 +742,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
 }
 
-// Persistent pairs: as many as SMs allow.
+// Whether C's tiles can be counted (they are ints, several problems' together).
+inline bool countable(long long M, long long N) { return (M + 127) / 128 * ((N + 127) / 128) < (1ll << 28); }
+
+// Persistent pairs: as many as SMs allow. They take the tiles in turn, the problems' with the longest contractions first (4,093
+// rows, 1,000 x 2,728, float16, the block's four gradients: 111 us, with the longest last 120).
 template <typename T, int E>
 int launch(Params& p, cudaStream_t stream) {
+  auto length = [](const Op& o) { return o.slices > 1 ? o.per : o.kb[0] + o.kb[1]; };
+  std::stable_sort(p.op, p.op + p.ops, [&](const Op& a, const Op& b) { return length(a) > length(b); });
   int tiles = 0;
   for (int i = 0; i < p.ops; ++i) {
     if (p.op[i].slices < 1) p.op[i].slices = 1;

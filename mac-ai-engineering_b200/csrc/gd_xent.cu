@@ -18,8 +18,8 @@ using gemm::Op;
 using gemm::Params;
 
 constexpr int kPart = 128;          // columns of one (maximum, sum)
-constexpr int kRows = 32;           // rows of a join CTA
-constexpr int kJoinWarps = 16;
+constexpr int kRows = 8;            // rows of a join CTA
+constexpr int kJoinThreads = 256, kJoinGroups = kJoinThreads / kRows;
 constexpr float kLn2 = 0.6931471805599453f;
 enum Reduction { kNone, kMean, kSum };
 
@@ -54,23 +54,39 @@ __device__ __forceinline__ int cta_sum(int v, int* sh) {
   return s;
 }
 
-// The plan of the rows [r0, r1) of each CTA: it counts the live rows before its own by itself (a CTA's reading of up to 8 n bytes
-// of labels, 592 CTAs at most), so that one launch numbers them all. CTA 0 clears the workspace's head and writes the total.
+__device__ __forceinline__ void copy_row(const uint16_t* from, uint16_t* to, int D, int lane) {
+  int c = lane * 8;
+  for (; c + 768 < D; c += 1024) {  // (four loads on their way)
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(from + c + 256 * i));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(to + c + 256 * i) = v[i];
+  }
+  for (; c < D; c += 256) *reinterpret_cast<uint4*>(to + c) = __ldg(reinterpret_cast<const uint4*>(from + c));
+}
+// zeros in what is left of the live rows' last tile of the contraction (dW sums over the rows of whole stages)
+__device__ __forceinline__ void clear_rows(uint16_t* out, long long ld, int live, int n, int D, int w0, int warps, int lane) {
+  const int end = min(n, (live + gemm::kBlockK - 1) / gemm::kBlockK * gemm::kBlockK);
+  for (int r = live + w0; r < end; r += warps)
+    for (int c = lane * 8; c < D; c += 256) *reinterpret_cast<uint4*>(out + r * ld + c) = make_uint4(0, 0, 0, 0);
+}
+
+// The plan of the rows [r0, r1) of each CTA, and their x, the live ones packed, `ld` elements from row to row. A CTA counts the live
+// rows before its own by itself (reading up to 8 n bytes of labels, 592 CTAs at most), so that one launch numbers and moves them all.
+// The first CTA clears the workspace's head, the last writes the total.
 constexpr int kPlanThreads = 256;
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(Labels lab, int n, int step, Plan plan, int* head) {
-  __shared__ int sh[kPlanThreads / 32];
-  __shared__ int before[kPlanThreads / 32];
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(Labels lab, const uint16_t* __restrict__ x, long long ldx, int n, int D,
+                                                            int step, Plan plan, uint16_t* __restrict__ out, long long ld, int* head) {
+  constexpr int kWarps = kPlanThreads / 32;
+  __shared__ int sh[kWarps], before[kWarps];
   const int r0 = (int)min((long long)blockIdx.x * step, (long long)n), r1 = (int)min((long long)r0 + step, (long long)n);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int stop = blockIdx.x == 0 ? n : r0;
+  if (blockIdx.x == 0 && threadIdx.x < 64) head[threadIdx.x] = 0;
   int c = 0;
-  for (int i = threadIdx.x; i < stop; i += kPlanThreads) c += lab.of(i) != lab.ignore;
-  int base = cta_sum<kPlanThreads / 32>(c, sh);
-  if (blockIdx.x == 0) {
-    if (threadIdx.x == 0) *plan.live = base;
-    if (threadIdx.x < 64) head[threadIdx.x] = 0;
-    base = 0;
-  }
+#pragma unroll 4
+  for (int i = threadIdx.x; i < r0; i += kPlanThreads) c += lab.of(i) != lab.ignore;
+  int base = cta_sum<kWarps>(c, sh);
   for (int r = r0; r < r1; r += kPlanThreads) {
     const int i = r + threadIdx.x;
     const long long l = i < r1 ? lab.of(i) : lab.ignore;
@@ -81,7 +97,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Labels lab, int n, i
     __syncthreads();
     int at = base, all = 0;
 #pragma unroll
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) at += before[w];
       all += before[w];
     }
@@ -90,24 +106,27 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Labels lab, int n, i
     if (keep) plan.label[at] = l < 0 || l >= lab.V ? -1 : (int)l;
     base += all;
   }
+  __syncthreads();  // the CTA's places
+  for (int i = r0 + warp; i < r1; i += kWarps) {
+    const int r = plan.place[i];
+    if (r >= 0) copy_row(x + i * ldx, out + r * ld, D, lane);
+  }
+  if (r1 == n) {  // (the last CTA)
+    if (threadIdx.x == 0) *plan.live = base;
+    clear_rows(out, ld, base, n, D, warp, kWarps, lane);
+  }
 }
 
-// The live rows of x, packed, `ld` elements from row to row; zeros in what is left of their last tile of the contraction (dW sums
-// over the rows of whole stages). A warp a row. HEAD: also clears the workspace's head (the backward's first kernel).
-__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* __restrict__ x, long long ldx, int n, int D,
-                                                     const int* __restrict__ live, const int* __restrict__ place,
+// The same rows again, for the backward; also clears its workspace's head. A warp a row.
+__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* __restrict__ x, long long ldx, int n, int D, Plan plan,
                                                      uint16_t* __restrict__ out, long long ld, int* head) {
   const int warps = gridDim.x * 8, w0 = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (head != nullptr && blockIdx.x == 0 && threadIdx.x < 64) head[threadIdx.x] = 0;
+  if (blockIdx.x == 0 && threadIdx.x < 64) head[threadIdx.x] = 0;
   for (int i = w0; i < n; i += warps) {
-    const int r = __ldg(place + i);
-    if (r < 0) continue;
-    for (int c = lane * 8; c < D; c += 256)
-      *reinterpret_cast<uint4*>(out + r * ld + c) = __ldg(reinterpret_cast<const uint4*>(x + i * ldx + c));
+    const int r = __ldg(plan.place + i);
+    if (r >= 0) copy_row(x + i * ldx, out + r * ld, D, lane);
   }
-  const int m = __ldg(live), end = min(n, (m + gemm::kBlockK - 1) / gemm::kBlockK * gemm::kBlockK);
-  for (int r = m + w0; r < end; r += warps)
-    for (int c = lane * 8; c < D; c += 256) *reinterpret_cast<uint4*>(out + r * ld + c) = make_uint4(0, 0, 0, 0);
+  clear_rows(out, ld, __ldg(plan.live), n, D, w0, warps, lane);
 }
 
 // Every row of dx: its live row's, or zeros. A warp a row.
@@ -149,14 +168,15 @@ __global__ void __launch_bounds__(256) spread_sums_kernel(const float* __restric
 }
 
 // Joins each row's parts: its maximum and the logarithm of its sum, its loss (at least 0: a sure row's sum is 1 and more); for a
-// mean or sum the last CTA adds the CTAs' sums in their order. Parts and targets lie by live rows, losses by rows.
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __restrict__ part, const float* __restrict__ target,
-                                                               int parts, int n, Plan plan, int reduction,
-                                                               float2* __restrict__ lse, float* __restrict__ loss,
-                                                               float2* sums, unsigned int* counter) {
-  __shared__ float2 sh[kJoinWarps][kRows];
+// mean or sum the last CTA adds the CTAs' sums in their order. Parts and targets lie by live rows, losses by rows. A thread takes
+// every 32nd part of a row. (8 rows a CTA: 777 rows of 393 parts JOIN)
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* __restrict__ part, const float* __restrict__ target,
+                                                            int parts, int n, Plan plan, int reduction, float2* __restrict__ lse,
+                                                            float* __restrict__ loss, float* sums, unsigned int* counter) {
+  __shared__ float2 sh[kJoinGroups][kRows];
+  __shared__ float warps[kJoinThreads / 32];
   __shared__ bool last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = blockIdx.x * kRows + lane;
+  const int group = threadIdx.x / kRows, at = threadIdx.x % kRows, i = blockIdx.x * kRows + at;
   const int row = i < n ? __ldg(plan.place + i) : -1;
   float m = -INFINITY, s = 0.f;
   auto add = [&](float2 v) {  // (a NaN sum stays)
@@ -165,33 +185,34 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __r
     m = next;
   };
   if (row >= 0) {
-    int p = warp;
-    for (; p + 3 * kJoinWarps < parts; p += 4 * kJoinWarps) {
+    int p = group;
+    for (; p + 3 * kJoinGroups < parts; p += 4 * kJoinGroups) {
       float2 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = __ldcs(part + (long long)(p + j * kJoinWarps) * n + row);
+      for (int j = 0; j < 4; ++j) v[j] = __ldcs(part + (long long)(p + j * kJoinGroups) * n + row);
 #pragma unroll
       for (int j = 0; j < 4; ++j) add(v[j]);
     }
-    for (; p < parts; p += kJoinWarps) add(__ldcs(part + (long long)p * n + row));
+    for (; p < parts; p += kJoinGroups) add(__ldcs(part + (long long)p * n + row));
   }
-  sh[warp][lane] = make_float2(m, s);
+  sh[group][at] = make_float2(m, s);
   __syncthreads();
-  if (warp == 0) {
-    m = -INFINITY, s = 0.f;
-    for (int w = 0; w < kJoinWarps; ++w) add(sh[w][lane]);
+  if (threadIdx.x < 32) {
     float x = 0.f;
-    if (row >= 0) {
-      const float rest = log2f(s);
-      x = __ldg(plan.label + row) < 0 ? NAN : (m - target[row]) + kLn2 * rest;
-      if (lse != nullptr) lse[row] = make_float2(m, rest);
+    if (threadIdx.x < kRows) {
+      m = -INFINITY, s = 0.f;
+      for (int g = 0; g < kJoinGroups; ++g) add(sh[g][at]);
+      if (row >= 0) {
+        const float rest = log2f(s);
+        x = __ldg(plan.label + row) < 0 ? NAN : (m - target[row]) + kLn2 * rest;
+        if (lse != nullptr) lse[row] = make_float2(m, rest);
+      }
+      if (reduction == kNone && i < n) loss[i] = x;
     }
-    if (reduction == kNone) {
-      if (i < n) loss[i] = x;
-    } else {
+    if (reduction != kNone) {
       x = warp_sum(x);
-      if (lane == 0) {
-        sums[blockIdx.x] = make_float2(x, 0.f);
+      if (threadIdx.x == 0) {
+        sums[blockIdx.x] = x;
         __threadfence();
         last = atomicAdd(counter, 1u) + 1u == gridDim.x;
       }
@@ -202,13 +223,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const float2* __r
   if (!last) return;
   __threadfence();
   float x = 0.f;  // (a thread's CTAs in order, then the threads': the same sum every run)
-  for (unsigned int j = threadIdx.x; j < gridDim.x; j += 32 * kJoinWarps) x += __ldcg(sums + j).x;
+  for (unsigned int j = threadIdx.x; j < gridDim.x; j += kJoinThreads) x += __ldcg(sums + j);
   x = warp_sum(x);
-  if (lane == 0) sh[warp][0].x = x;
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = x;
   __syncthreads();
   if (threadIdx.x == 0) {
     x = 0.f;
-    for (int w = 0; w < kJoinWarps; ++w) x += sh[w][0].x;
+    for (int w = 0; w < kJoinThreads / 32; ++w) x += warps[w];
     loss[0] = reduction == kMean ? x / (float)*plan.live : x;  // (no row: NaN)
   }
 }
@@ -264,7 +285,7 @@ FwdPlan fwd_plan(long long n, int D, int V) {
   f.part = f.rows + up((size_t)n * pitch(D) * 2);
   f.target = f.part + up((size_t)f.parts * n * sizeof(float2));
   f.sums = f.target + up((size_t)n * sizeof(float));
-  f.total = f.sums + up((size_t)f.ctas * sizeof(float2));
+  f.total = f.sums + up((size_t)f.ctas * sizeof(float));
   return f;
 }
 
@@ -288,7 +309,7 @@ BwdPlan bwd_plan(long long n, int D, int V) {
   b.ldd = b.pieces > 1 ? b.cols : (V + 63ll) / 64 * 64;
   const long long tiles_m = gemm::blocks_of(n, gemm::kTileM), tiles_n = gemm::blocks_of(D, gemm::kTileN);
   b.slices = 1, b.per = gemm::blocks_of(V, gemm::kBlockK);
-  if (b.pieces == 1) {
+  if (b.pieces == 1 && tiles_n < 16384) {  // (spread_sums_kernel's grid)
     const long long kv = b.per, kn = gemm::blocks_of(n, gemm::kBlockK), tiles = tiles_m * tiles_n;
     long long share = (tiles * kv + gemm::blocks_of(V, gemm::kTileM) * tiles_n * kn) / 74 / 2;
     if (share < 16) share = 16;
@@ -322,21 +343,15 @@ void shape(Op& op, long long M, long long N) {
   op.tiles_m = gemm::blocks_of(M, gemm::kTileM), op.tiles_n = gemm::blocks_of(N, gemm::kTileN);
 }
 
-int gather(const Problem& q, void* rows, char* ws, bool head, cudaStream_t stream) {
-  gather_kernel<<<grid_of(q.n), 256, 0, stream>>>(static_cast<const uint16_t*>(q.x), q.ldx, q.n, q.D, q.plan.live, q.plan.place,
-                                                  static_cast<uint16_t*>(rows), pitch(q.D),
-                                                  head ? reinterpret_cast<int*>(ws) : nullptr);
-  return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
-}
-
 template <typename T>
 int forward(const Problem& q, const Labels& lab, float* loss, float2* lse, char* ws, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const FwdPlan f = fwd_plan(q.n, q.D, q.V);
-  const int step = gemm::blocks_of(q.n, 592) < 32 ? 32 : gemm::blocks_of(q.n, 592);
-  plan_kernel<<<gemm::blocks_of(q.n, step), kPlanThreads, 0, stream>>>(lab, q.n, step, q.plan, reinterpret_cast<int*>(ws));
+  const int step = gemm::blocks_of(q.n, 592) < 8 ? 8 : gemm::blocks_of(q.n, 592);  // (a row a warp)
+  plan_kernel<<<gemm::blocks_of(q.n, step), kPlanThreads, 0, stream>>>(lab, static_cast<const uint16_t*>(q.x), q.ldx, q.n, q.D, step,
+                                                                      q.plan, reinterpret_cast<uint16_t*>(ws + f.rows), pitch(q.D),
+                                                                      reinterpret_cast<int*>(ws));
   if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  if (const int st = gather(q, ws + f.rows, ws, false, stream)) return st;
   Params p = {};
   p.ops = 1, p.err = reinterpret_cast<ErrorWord*>(ws), p.live = q.plan.live, p.labels = q.plan.label;
   p.part = reinterpret_cast<float2*>(ws + f.part);
@@ -349,8 +364,8 @@ int forward(const Problem& q, const Labels& lab, float* loss, float2* lse, char*
       !gemm::operand_map(&o.b[0], q.w, dt, q.V, q.D, q.ldw, false))
     return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kLse>(p, stream)) return st;
-  join_kernel<<<f.ctas, 32 * kJoinWarps, 0, stream>>>(p.part, p.target, f.parts, q.n, q.plan, q.reduction, lse, loss,
-                                                     reinterpret_cast<float2*>(ws + f.sums),
+  join_kernel<<<f.ctas, kJoinThreads, 0, stream>>>(p.part, p.target, f.parts, q.n, q.plan, q.reduction, lse, loss,
+                                                     reinterpret_cast<float*>(ws + f.sums),
                                                      reinterpret_cast<unsigned int*>(ws + 64));
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
 }
@@ -363,7 +378,9 @@ int backward(const Problem& q, const float2* lse, const float* dloss, void* dx, 
   void *const rows = ws + b.rows, *const dxc = ws + b.dx, *const d = ws + b.d;
   float* const row_scale = reinterpret_cast<float*>(ws + b.scale);
   float* const factor = reinterpret_cast<float*>(ws + 128);
-  if (const int st = gather(q, rows, ws, true, stream)) return st;
+  gather_kernel<<<grid_of(q.n), 256, 0, stream>>>(static_cast<const uint16_t*>(q.x), q.ldx, q.n, q.D, q.plan,
+                                                  static_cast<uint16_t*>(rows), ld, reinterpret_cast<int*>(ws));
+  if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   factors_kernel<<<1, 1024, 0, stream>>>(dloss, q.plan, q.n, q.reduction, std::is_same<T, __half>::value, row_scale, factor);
   if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   const int kd = gemm::blocks_of(q.D, gemm::kBlockK);
@@ -430,7 +447,7 @@ int backward(const Problem& q, const float2* lse, const float* dloss, void* dx, 
 int check(int dtype, int reduction, long long rows, int D, int V, long long ldx, long long ldw) {
   if ((dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) || reduction < kNone || reduction > kSum) return GD_ERR_ARG;
   if (rows < 0 || rows > (1ll << 24) || D <= 0 || D % 8 || D > (1 << 24) || V <= 0 || V > (1 << 24) || ldx < D || ldw < D ||
-      ldx >= (1ll << 38) || ldw >= (1ll << 38))
+      ldx >= (1ll << 38) || ldw >= (1ll << 38) || !gemm::countable(rows, V) || !gemm::countable(rows, D) || !gemm::countable(V, D))
     return GD_ERR_SHAPE;
   return ldx % 8 || ldw % 8 ? GD_ERR_ALIGN : GD_OK;
 }
