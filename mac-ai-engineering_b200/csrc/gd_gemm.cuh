@@ -10,6 +10,13 @@
 // warp 0 loads (TMA, a ring of stages), warp 1 of the first CTA issues the products, warps 4 - 11 are the epilogue (a thread
 // owns a row and half of the tile's columns; TMEM lane = row). The accumulator is double-buffered (2 x 256 TMEM columns), so a
 // tile's epilogue runs under the next one's products. The CTAs are persistent and walk the tiles of up to kMaxOps problems.
+//
+// Bound by the tensor pipe (97 % busy under four gradients at once) at the clock that the power limit leaves (1.45 to 1.6 GHz).
+// bf16, 16,384 rows, 2,048 x 6,144: the second product 268 us (1,540 TFLOP/s; cuBLAS 264), gate and up 524 us (1,575), the four
+// gradients 1,385 us (1,490). With g and u kept gate and up take 578 us, and dh 413 us (1,000): their epilogues' 0.8 and 1.2 GB cross
+// between the SMs and L2 beside the operands' (dh without its loads 350 us, without its stores 333, without both 281; neither TMA nor
+// the warps' own accesses, 8 or 16 epilogue warps, 4 or 5 stages changed that by more than 3 %). Cross entropy, 7,370 rows, 2,048 x
+// 128,000: logits 2.44 to 2.85 ms (1,360 to 1,580), with their gradients stored 2.53 to 2.97 ms, its two gradients 5.4 to 6.1 ms.
 #pragma once
 
 #include <algorithm>
@@ -212,8 +219,8 @@ __device__ __forceinline__ int all_tiles(const Params& p, int live) {
   return n;
 }
 // The tiles that a pair takes: the first problem's in turn; then, where some pairs have one tile of it more, the others make up for
-// that with later problems' (shorter) tiles before all take turns again. (7,370 live rows, 2,048 wide, 16,128 words: three or four
-// tiles of dx of 252 stages for each pair and 504 tiles of dW of 116: WALK)
+// that with later problems' (shorter) tiles before all take turns again. (1,500 rows, half of them
+// live, 768 wide, 32,003 words: dx's slices and dW 83 us instead of 96 at one clock)
 struct Walk {
   int pair, pairs, tiles, first, mine, behind, extra;  // first: the first problem's tiles; behind: pairs with one less of them
   template <int E>
@@ -389,7 +396,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   const uint32_t s_base = smem_u32(base);
 
   if (warp == 0) {
-    // (the whole warp runs this, one elected lane's instructions take effect: addresses and coordinates in uniform registers)
+    // The whole warp runs this, one elected lane's instructions take effect: addresses and coordinates stay in uniform registers.
+    // (Issued from a branch of one lane, a stage's loads took longer than its products where a launch holds several problems:
+    // 1,215 instead of 1,540 TFLOP/s.)
     const uint32_t lead = elect();
     int slot = 0, laps = 0, issued = 0;
     bool ok = true;
@@ -460,8 +469,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         int from;
         const int n = __shfl_sync(0xffffffffu, stages_of(op, w, 0, live, from) + stages_of(op, w, 1, live, from), 0);
         const uint32_t d = tm + buf * kTileN;
-        // The layouts are constants of each loop: descriptors and steps then stay in uniform registers, which the instruction
-        // reads (as variables of the problem they were moved there for every product: 1,250 instead of 1,600 TFLOP/s).
+        // (the layouts are constants of each loop: descriptors and steps stay in uniform registers, which the instruction reads)
         auto products = [&](auto a_mn, auto b_mn) {
           constexpr uint32_t id = wattn::idesc<T>(256, 256, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
           constexpr uint32_t a_hi = a_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16, b_hi = b_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16;
@@ -746,7 +754,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
 inline bool countable(long long M, long long N) { return (M + 127) / 128 * ((N + 127) / 128) < (1ll << 28); }
 
 // Persistent pairs: as many as SMs allow. They take the tiles in turn, the problems' with the longest contractions first (4,093
-// rows, 1,000 x 2,728, float16, the block's four gradients: 111 us, with the longest last 120).
+// rows, 1,000 x 2,728, float16, the block's four gradients and its second product: 111 us, with the longest last 120).
 template <typename T, int E>
 int launch(Params& p, cudaStream_t stream) {
   auto length = [](const Op& o) { return o.slices > 1 ? o.per : o.kb[0] + o.kb[1]; };
