@@ -51,8 +51,22 @@ void shape(Op& op, long long M, long long N, int tile_n = gemm::kTileN) {
   op.kb[1] = 0;
 }
 
+// Few tiles of y, or of dx beside the weights' gradients, have their contraction cut (gemm::cut_of; as if all gradients were asked
+// for, so that each has the same bits whichever are). 129 rows, 4,096 x 12,288: a call takes 101 us, uncut 116.
+gemm::Cut cut_y(long long n, int F, int O) {
+  return gemm::cut_of((long long)gemm::blocks_of(n, gemm::kTileM) * gemm::blocks_of(O, gemm::kTileN), gemm::blocks_of(F, gemm::kBlockK), 0, O);
+}
+gemm::Cut cut_dx(long long n, int D, int F, int O) {
+  auto tiles = [](long long M, long long N) { return (long long)gemm::blocks_of(M, gemm::kTileM) * gemm::blocks_of(N, gemm::kTileN); };
+  return gemm::cut_of(tiles(n, D), 2ll * gemm::blocks_of(F, gemm::kBlockK),
+                      (2 * tiles(F, D) + tiles(O, F)) * gemm::blocks_of(n, gemm::kBlockK), D);
+}
+size_t sum_bytes(const gemm::Cut& c, long long n, int D) {
+  return gemm::cut_bytes(c, (long long)gemm::blocks_of(n, gemm::kTileM) * gemm::blocks_of(D, gemm::kTileN));
+}
+
 template <typename T>
-int forward(const Problem& q, void* const* kept, void* h, void* y, uint32_t* bounds, ErrorWord* err, cudaStream_t stream) {
+int forward(const Problem& q, void* const* kept, void* h, float* sum, void* y, uint32_t* bounds, ErrorWord* err, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const long long n = q.rows;
   Params p = {};
@@ -74,7 +88,10 @@ int forward(const Problem& q, void* const* kept, void* h, void* y, uint32_t* bou
   if (!gemm::operand_map(&d.a[0], h, dt, n, q.F, pitch(q.F), false) || !gemm::operand_map(&d.b[0], q.wd, dt, q.O, q.F, q.ldd, false) ||
       !gemm::slab_map(&d.c, y, dt, n, q.O, q.O))
     return GD_ERR_LAUNCH;
-  return gemm::launch<T, gemm::kStore>(r, stream);
+  const gemm::Cut c = cut_y(n, q.F, q.O);
+  d.slices = c.slices, d.per = c.per, d.sum_mode = c.slices > 1 ? 1 : 0, d.sum = sum;
+  if (const int st = gemm::launch<T, gemm::kStore>(r, stream)) return st;
+  return c.slices > 1 ? gemm::sum_slices<T>(sum, d, (int)n, q.O, nullptr, nullptr, nullptr, nullptr, y, stream) : GD_OK;
 }
 
 struct Grads {
@@ -83,7 +100,7 @@ struct Grads {
 
 template <typename T>
 int backward(const Problem& q, const void* const* kept, const void* dy, long long ldy, const Grads& out, void* dg, void* du,
-             void* h, const uint32_t* bounds, uint32_t* own, ErrorWord* err, cudaStream_t stream) {
+             void* h, float* sum, const uint32_t* bounds, uint32_t* own, ErrorWord* err, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const long long n = q.rows, lf = pitch(q.F);
   if (bounds != nullptr) {
@@ -120,16 +137,23 @@ int backward(const Problem& q, const void* const* kept, const void* dy, long lon
   weight(out.dwg, dg, lf, q.F, q.x, q.ldx, q.D, true);
   weight(out.dwu, du, lf, q.F, q.x, q.ldx, q.D, true);
   weight(out.dwd, dy, ldy, q.O, h, lf, q.F, false);
+  const gemm::Cut c = cut_dx(n, q.D, q.F, q.O);
+  Op dx = {};
   if (out.dx != nullptr) {
     Op& w = r.op[r.ops++];
     shape(w, n, q.D);  // dx = dg Wg + du Wu
     w.kb[0] = w.kb[1] = gemm::blocks_of(q.F, gemm::kBlockK);
     w.b_mn = true, w.unscale = true;
+    w.slices = c.slices, w.per = c.per, w.sum_mode = c.slices > 1 ? 1 : 0, w.sum = sum;
+    dx = w;
     ok = ok && gemm::operand_map(&w.a[0], dg, dt, n, q.F, lf, false) && gemm::operand_map(&w.a[1], du, dt, n, q.F, lf, false) &&
          gemm::operand_map(&w.b[0], q.wg, dt, q.F, q.D, q.ldg, true) &&
          gemm::operand_map(&w.b[1], q.wu, dt, q.F, q.D, q.ldu, true) && gemm::slab_map(&w.c, out.dx, dt, n, q.D, q.D);
   }
-  return ok ? gemm::launch<T, gemm::kStore>(r, stream) : GD_ERR_LAUNCH;
+  if (!ok) return GD_ERR_LAUNCH;
+  if (const int st = gemm::launch<T, gemm::kStore>(r, stream)) return st;
+  if (out.dx == nullptr || c.slices == 1) return GD_OK;
+  return gemm::sum_slices<T>(sum, dx, (int)n, q.D, nullptr, nullptr, bounds, own, out.dx, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -167,8 +191,10 @@ bool bind_context() {
 
 extern "C" size_t gd_ff_workspace_bytes(long long rows, int D, int F, int O, int for_backward) {
   const long long ld[5] = {D, D, D, F, O};
-  if (gd::ff::check(GD_BFLOAT16, rows, D, F, O, ld, 5) != GD_OK) return 0;
-  return gd::ff::kHead + (for_backward ? 3 : 1) * gd::ff::matrix_bytes(rows, F);
+  if (gd::ff::check(GD_BFLOAT16, rows, D, F, O, ld, 5) != GD_OK || rows == 0) return 0;
+  using namespace gd::ff;
+  return kHead + (for_backward ? 3 * matrix_bytes(rows, F) + sum_bytes(cut_dx(rows, D, F, O), rows, D)
+                               : matrix_bytes(rows, F) + sum_bytes(cut_y(rows, F, O), rows, O));
 }
 
 extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* kept,
@@ -192,10 +218,11 @@ extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, co
   if (cudaMemsetAsync(err, 0, sizeof(*err), cs) != cudaSuccess ||
       (dtype == GD_FLOAT16 && bounds != nullptr && cudaMemsetAsync(bounds, 0, 16, cs) != cudaSuccess))
     return (cudaGetLastError(), GD_ERR_LAUNCH);
+  float* const sum = reinterpret_cast<float*>(static_cast<char*>(h) + matrix_bytes(rows, F));
   void* planes[3];
   for (int i = 0; i < 3; ++i) planes[i] = kept == nullptr ? nullptr : static_cast<char*>(kept) + i * (size_t)rows * pitch(F) * 2;
-  return dtype == GD_FLOAT16 ? forward<__half>(q, planes, h, y, bounds, err, cs)
-                             : forward<__nv_bfloat16>(q, planes, h, y, nullptr, err, cs);
+  return dtype == GD_FLOAT16 ? forward<__half>(q, planes, h, sum, y, bounds, err, cs)
+                             : forward<__nv_bfloat16>(q, planes, h, sum, y, nullptr, err, cs);
 }
 
 extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* kept,
@@ -229,8 +256,9 @@ extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, co
   const Grads out = {dx, dw_gate, dw_up, dw_down};
   const size_t m = matrix_bytes(rows, F);
   void *dg = at + kHead, *du = at + kHead + m, *h = at + kHead + 2 * m;
+  float* const sum = reinterpret_cast<float*>(at + kHead + 3 * m);
   const void* planes[3];
   for (int i = 0; i < 3; ++i) planes[i] = static_cast<const char*>(kept) + i * (size_t)rows * pitch(F) * 2;
-  return dtype == GD_FLOAT16 ? backward<__half>(q, planes, dy, ld[4], out, dg, du, h, bounds, own, err, cs)
-                             : backward<__nv_bfloat16>(q, planes, dy, ld[4], out, dg, du, h, nullptr, nullptr, err, cs);
+  return dtype == GD_FLOAT16 ? backward<__half>(q, planes, dy, ld[4], out, dg, du, h, sum, bounds, own, err, cs)
+                             : backward<__nv_bfloat16>(q, planes, dy, ld[4], out, dg, du, h, sum, nullptr, nullptr, err, cs);
 }

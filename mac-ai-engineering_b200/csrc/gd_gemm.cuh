@@ -261,9 +261,10 @@ __device__ __forceinline__ Where locate(const Params& p, int tile, int live) {
   w.n = (r / high) * (E == kSwiglu ? kHalf : kTileN);
   return w;
 }
-// the tile's stages of segment s, and the first of them
-__device__ __forceinline__ int stages_of(const Op& o, const Where& w, int s, int live, int& from) {
-  const int n = s == 0 && o.k_live ? (live + kBlockK - 1) / kBlockK : o.kb[s];
+// the tile's stages, of both segments one after the other, and the first of them
+__device__ __forceinline__ int first_segment(const Op& o, int live) { return o.k_live ? (live + kBlockK - 1) / kBlockK : o.kb[0]; }
+__device__ __forceinline__ int stages_of(const Op& o, const Where& w, int live, int& from) {
+  const int n = first_segment(o, live) + o.kb[1];
   from = w.slice * o.per;
   return o.slices == 1 ? n : n - from < o.per ? (n > from ? n - from : 0) : o.per;
 }
@@ -275,7 +276,7 @@ __device__ __forceinline__ Walk Walk::of(const Params& p, int live, int pair, in
   w.mine = w.first > pair ? (w.first - pair + pairs - 1) / pairs : 0;
   w.behind = pairs - w.first % pairs, w.extra = 0;
   if (E == kStore && p.ops > 1 && w.behind < pairs) {
-    auto length = [&](const Op& o) { return o.slices > 1 ? o.per : (o.k_live ? (live + kBlockK - 1) / kBlockK : o.kb[0]) + o.kb[1]; };
+    auto length = [&](const Op& o) { return o.slices > 1 ? o.per : first_segment(o, live) + o.kb[1]; };
     const int next = length(p.op[1]);
     if (next > 0) w.extra = length(p.op[0]) / next;
     if (w.extra > (w.tiles - w.first) / w.behind) w.extra = (w.tiles - w.first) / w.behind;
@@ -436,8 +437,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       using No = std::false_type;
       for (int s = 0; ok && s < 2; ++s) {
         const CUtensorMap *ma = &op.a[s], *mb = E == kSwiglu ? &op.b[rank] : &op.b[s];
-        int from;
-        int n = stages_of(op, w, s, live, from);
+        // the tile's stages in this segment
+        int first;
+        const int all = stages_of(op, w, live, first), here = s == 0 ? 0 : first_segment(op, live), size = s == 0 ? first_segment(op, live) : op.kb[1];
+        int from = first > here ? first - here : 0, n = (first + all - here < size ? first + all - here : size) - from;
         n = __shfl_sync(0xffffffffu, n, 0);
         from = __shfl_sync(0xffffffffu, from, 0);
         if constexpr (E == kStore) {
@@ -467,7 +470,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         if (it >= 2 && !(ok = cluster_wait(acc_empty + buf, ((it >> 1) - 1) & 1, p.err, 82))) break;
         tc_fence_after();
         int from;
-        const int n = __shfl_sync(0xffffffffu, stages_of(op, w, 0, live, from) + stages_of(op, w, 1, live, from), 0);
+        const int n = __shfl_sync(0xffffffffu, stages_of(op, w, live, from), 0);
         const uint32_t d = tm + buf * kTileN;
         // (the layouts are constants of each loop: descriptors and steps stay in uniform registers, which the instruction reads)
         auto products = [&](auto a_mn, auto b_mn) {
@@ -547,7 +550,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
                                       : op.sum + (((long long)w.at * 2 + rank) * kTileN + half * 128) * kHalf +
                                             quad * 32 + lane;
         int from;
-        const bool none = stages_of(op, w, 0, live, from) + stages_of(op, w, 1, live, from) == 0;  // a sum over nothing
+        const bool none = stages_of(op, w, live, from) == 0;  // a sum over nothing
 #pragma unroll 1
         for (int s = 0; s < 2; ++s) {
           const int c = half * 128 + s * 64, n0 = w.n + c;
@@ -749,6 +752,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   if (warp == 2)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
 }
+
+// The sums of slices, in their order, in 16 bits: row i of out [n, D] is row place[i] of C (NULL: i; -1: zeros). A thread has 8
+// columns of a row, a warp 32 rows.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_slices_kernel(const float* __restrict__ sum, int slices, int tiles_n, int n, int D,
+                                                         const int* __restrict__ live, const int* __restrict__ place,
+                                                         const float* __restrict__ factor, const uint32_t* bounds,
+                                                         const uint32_t* more, T* __restrict__ out) {
+  const int i = blockIdx.x * 32 + (threadIdx.x & 31), c = (blockIdx.y * 8 + (threadIdx.x >> 5)) * 8;
+  if (i >= n || c >= D) return;
+  const int r = place == nullptr ? i : __ldg(place + i), rows = ((live == nullptr ? n : __ldg(live)) + kTileM - 1) / kTileM;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (r >= 0) {
+    // the tile's index as the products' kernel counts them
+    const int tm = r / kTileM, tn = c / kTileN, g = tm / kGroupM, high = min(rows - g * kGroupM, kGroupM);
+    const int tile = g * kGroupM * tiles_n + tn * high + tm % kGroupM;
+    const float f = factor != nullptr ? __ldg(factor) : 1.f / carried(bounds, more);
+    for (int s = 0; s < slices; ++s) {
+      const long long t = (long long)s * rows * tiles_n + tile;
+      const float* at = sum + ((t * 2 + r % kTileM / kHalf) * kTileN + c % kTileN) * kHalf + r % kHalf;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += at[j * kHalf];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= f;
+  }
+  store8<T>(out + (long long)i * D + c, v);
+}
+template <typename T>
+int sum_slices(const float* sum, const Op& o, int n, int D, const int* live, const int* place, const uint32_t* bounds,
+               const uint32_t* more, void* out, cudaStream_t stream) {
+  const dim3 grid((unsigned)blocks_of(n, 32), (unsigned)blocks_of(D, 64));
+  sum_slices_kernel<T><<<grid, 256, 0, stream>>>(sum, o.slices, o.tiles_n, n, D, live, place, o.factor, bounds, more,
+                                                 static_cast<T*>(out));
+  return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
+}
+// How a contraction of `stages` for `tiles` tiles is cut where others of `rest` stages in all run beside it: a tile's length into
+// about half of a pair's share of the whole, at least 16 stages; 64 MiB of sums at most. {slices, stages of one}
+struct Cut {
+  int slices, per;
+};
+inline Cut cut_of(long long tiles, long long stages, long long rest, int D) {
+  Cut c = {1, (int)stages};
+  long long share = (tiles * stages + rest) / 74 / (rest > 0 ? 2 : 1);
+  if (share < 16) share = 16;
+  if (stages <= share + share / 2 || blocks_of(D, 64) > 65535) return c;
+  c.slices = blocks_of(stages, (int)share);
+  const long long room = (64ll << 20) / (tiles * kTileM * kTileN * 4);
+  if (c.slices > room) c.slices = room < 1 ? 1 : (int)room;
+  c.per = blocks_of(stages, c.slices);
+  c.slices = blocks_of(stages, c.per);
+  return c;
+}
+inline size_t cut_bytes(const Cut& c, long long tiles) { return c.slices > 1 ? (size_t)c.slices * tiles * kTileM * kTileN * 4 : 0; }
 
 // Whether C's tiles can be counted (they are ints, several problems' together).
 inline bool countable(long long M, long long N) { return (M + 127) / 128 * ((N + 127) / 128) < (1ll << 28); }

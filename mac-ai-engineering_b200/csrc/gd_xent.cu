@@ -140,33 +140,6 @@ __global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict_
           r < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(in + r * ld + c);
   }
 }
-// The same from the slices' sums (gemm's Op::sum, in their order): a thread has 8 columns of a row, a warp 32 rows.
-template <typename T>
-__global__ void __launch_bounds__(256) spread_sums_kernel(const float* __restrict__ sum, int slices, int tiles_n, int n, int D,
-                                                          const int* __restrict__ live, const int* __restrict__ place,
-                                                          const float* __restrict__ factor, T* __restrict__ dx) {
-  const int i = blockIdx.x * 32 + (threadIdx.x & 31), c = (blockIdx.y * 8 + (threadIdx.x >> 5)) * 8;
-  if (i >= n || c >= D) return;
-  const int r = __ldg(place + i), rows = (__ldg(live) + gemm::kTileM - 1) / gemm::kTileM;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (r >= 0) {
-    // the tile's index as the products' kernel counts them
-    const int tm = r / gemm::kTileM, tn = c / gemm::kTileN, g = tm / gemm::kGroupM;
-    const int high = min(rows - g * gemm::kGroupM, gemm::kGroupM);
-    const int tile = g * gemm::kGroupM * tiles_n + tn * high + tm % gemm::kGroupM;
-    const float f = __ldg(factor);
-    for (int s = 0; s < slices; ++s) {
-      const long long t = (long long)s * rows * tiles_n + tile;
-      const float* at = sum + ((t * 2 + r % gemm::kTileM / gemm::kHalf) * gemm::kTileN + c % gemm::kTileN) * gemm::kHalf + r % gemm::kHalf;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += at[j * gemm::kHalf];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= f;
-  }
-  store8<T>(dx + (long long)i * D + c, v);
-}
-
 // Joins each row's parts: its maximum and the logarithm of its sum, its loss (at least 0: a sure row's sum is 1 and more); for a
 // mean or sum the last CTA adds the CTAs' sums in their order. Parts and targets lie by live rows, losses by rows. A thread takes
 // every 32nd part of a row. (777 rows of 393 parts: 6 us, with 32 rows a CTA 8 us; 7,370 of 1,000: 20 us, 26 us)
@@ -291,11 +264,12 @@ FwdPlan fwd_plan(long long n, int D, int V) {
 
 // The pieces of the vocabulary: D of one piece takes at most kPieceBytes (a multiple of a tile's columns, at least one tile).
 // One piece and few tiles of dx: its contraction over the vocabulary, far longer than a tile of dW's over the rows, is cut into
-// slices of about half of a pair's share of the whole, with fp32 sums of their own. At 1,500 rows (half of them live), 768 wide, a
-// vocabulary of 32,003, both gradients' products take 89 us, without slices 250 us (at one clock).
+// slices with fp32 sums of their own. At 1,500 rows (half of them live), 768 wide, a
+// vocabulary of 32,003, both gradients' products take 54 us; uncut, the longest tile alone takes 250 us.
 constexpr size_t kPieceBytes = (size_t)256 << 20;
 struct BwdPlan {
-  int pieces, cols, slices, per;  // cols: of every piece but the last; per: stages of a slice
+  int pieces, cols;  // cols: of every piece but the last
+  gemm::Cut cut;     // of dx's contraction
   long long ldd;
   size_t scale, rows, dx, d, sum, total;
 };
@@ -308,25 +282,16 @@ BwdPlan bwd_plan(long long n, int D, int V) {
   b.pieces = gemm::blocks_of(V, b.cols);
   b.ldd = b.pieces > 1 ? b.cols : (V + 63ll) / 64 * 64;
   const long long tiles_m = gemm::blocks_of(n, gemm::kTileM), tiles_n = gemm::blocks_of(D, gemm::kTileN);
-  b.slices = 1, b.per = gemm::blocks_of(V, gemm::kBlockK);
-  if (b.pieces == 1 && tiles_n < 16384) {  // (spread_sums_kernel's grid)
-    const long long kv = b.per, kn = gemm::blocks_of(n, gemm::kBlockK), tiles = tiles_m * tiles_n;
-    long long share = (tiles * kv + gemm::blocks_of(V, gemm::kTileM) * tiles_n * kn) / 74 / 2;
-    if (share < 16) share = 16;
-    if (kv > share) {
-      b.slices = gemm::blocks_of(kv, (int)share);
-      const long long room = (64ll << 20) / (tiles * gemm::kTileM * gemm::kTileN * 4);  // 64 MiB of sums
-      if (b.slices > room) b.slices = room < 1 ? 1 : (int)room;
-      b.per = gemm::blocks_of(kv, b.slices);
-      b.slices = gemm::blocks_of(kv, b.per);
-    }
-  }
+  const long long kn = gemm::blocks_of(n, gemm::kBlockK);
+  b.cut = {1, 0};
+  if (b.pieces == 1)
+    b.cut = gemm::cut_of(tiles_m * tiles_n, gemm::blocks_of(V, gemm::kBlockK), gemm::blocks_of(V, gemm::kTileM) * tiles_n * kn, D);
   b.scale = kHead;
   b.rows = b.scale + up((size_t)n * sizeof(float));
   b.dx = b.rows + up((size_t)n * pitch(D) * 2);
   b.d = b.dx + up((size_t)n * pitch(D) * 2);
   b.sum = b.d + up((size_t)n * b.ldd * 2);
-  b.total = b.sum + (b.pieces > 1 || b.slices > 1 ? (size_t)b.slices * tiles_m * tiles_n * (gemm::kTileM * gemm::kTileN * sizeof(float)) : 0);
+  b.total = b.sum + (b.pieces > 1 ? (size_t)tiles_m * tiles_n * gemm::kTileM * gemm::kTileN * 4 : gemm::cut_bytes(b.cut, tiles_m * tiles_n));
   return b;
 }
 
@@ -408,8 +373,8 @@ int backward(const Problem& q, const float2* lse, const float* dloss, void* dx, 
       g.m_live = true;
       g.kb[0] = gemm::blocks_of(cols, gemm::kBlockK);
       g.b_mn = true;
-      g.slices = b.slices, g.per = b.per;
-      g.sum_mode = b.slices > 1 ? 1 : b.pieces == 1 ? 0 : i == 0 ? 1 : i + 1 < b.pieces ? 2 : 3;
+      g.slices = b.cut.slices, g.per = b.cut.per;
+      g.sum_mode = b.cut.slices > 1 ? 1 : b.pieces == 1 ? 0 : i == 0 ? 1 : i + 1 < b.pieces ? 2 : 3;
       g.sum = reinterpret_cast<float*>(ws + b.sum);
       g.factor = factor;
       ok = ok && gemm::operand_map(&g.a[0], d, dt, q.n, cols, b.ldd, false) &&
@@ -430,16 +395,18 @@ int backward(const Problem& q, const float2* lse, const float* dloss, void* dx, 
     if (const int st = gemm::launch<T, gemm::kStore>(r, stream)) return st;
   }
   if (dx != nullptr) {
-    if (b.slices > 1) {
-      const dim3 grid((unsigned)gemm::blocks_of(q.n, 32), (unsigned)gemm::blocks_of(q.D, 64));
-      spread_sums_kernel<T><<<grid, 256, 0, stream>>>(reinterpret_cast<const float*>(ws + b.sum), b.slices,
-                                                      gemm::blocks_of(q.D, gemm::kTileN), q.n, q.D, q.plan.live, q.plan.place, factor,
-                                                      static_cast<T*>(dx));
+    if (b.cut.slices > 1) {
+      Op g = {};
+      shape(g, q.n, q.D);
+      g.slices = b.cut.slices, g.factor = factor;
+      if (const int st = gemm::sum_slices<T>(reinterpret_cast<const float*>(ws + b.sum), g, q.n, q.D, q.plan.live, q.plan.place, nullptr,
+                                             nullptr, dx, stream))
+        return st;
     } else {
       spread_kernel<<<grid_of(q.n), 256, 0, stream>>>(static_cast<const uint16_t*>(dxc), ld, q.n, q.D, q.plan.place,
                                                       static_cast<uint16_t*>(dx));
+      if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
     }
-    if (cudaPeekAtLastError() != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   }
   return GD_OK;
 }

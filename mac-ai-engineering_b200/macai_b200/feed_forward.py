@@ -42,6 +42,8 @@ def _fwd(x, wg, wu, wd, keep):
     """(y, kept, bounds) on matrices; keep: 24 bits of g and u (and float16's bounds) for the backward, else None."""
     n, D, F, O = _sizes(x, wg, wd)
     y = torch.empty((n, O), dtype=x.dtype, device=x.device)
+    if n == 0:
+        return y, None, None
     kept = bounds = None
     if keep:
         kept = torch.empty((3, n, -(-F // 64) * 64), dtype=torch.int16, device=x.device)
@@ -60,6 +62,8 @@ def _bwd(x, wg, wu, wd, kept, bounds, dy, need):
     n, D, F, O = _sizes(x, wg, wd)
     make = lambda yes, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if yes else None  # noqa: E731
     out = (make(need[0], n, D), make(need[1], F, D), make(need[2], F, D), make(need[3], O, F))
+    if n == 0:
+        return tuple(None if t is None else t.zero_() for t in out)
     size = _bytes(n, D, F, O, 1)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     launch("gd_ff_bwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), kept.data_ptr(),
