@@ -478,7 +478,7 @@ int launch(const Args& a, cudaStream_t stream) {
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return (cudaGetLastError(), GD_ERR_LAUNCH);
   const long long heads = (long long)a.B * a.H;
-  if (a.T == 1 && heads > sms) {  // (up to here every SM has work in run_kernel at once)
+  if (a.T == 1 && heads > sms && a.slots > 0) {  // (up to as many heads run_kernel has work for every SM at once)
     return a.DK <= 64    ? launch_token<T, TV, 64, 32>(a, sms, stream)
            : a.DK <= 128 ? launch_token<T, TV, 128, 16>(a, sms, stream)
                          : launch_token<T, TV, 256, 16>(a, sms, stream);

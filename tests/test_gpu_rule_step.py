@@ -46,6 +46,26 @@ def test_recurrence(B, T, HK, H, DK, DV, dt, vdt):
     assert torch.equal(got2, got) and torch.equal(sT, state) and torch.equal(s0, kept)
 
 
+@pytest.mark.parametrize("B,HK,H,DK,DV", [(38, 4, 4, 32, 32), (75, 1, 2, 64, 96), (50, 1, 3, 96, 128), (19, 4, 8, 128, 128),
+                                          (160, 1, 1, 160, 64), (38, 2, 4, 256, 256), (300, 2, 4, 128, 32)])
+@pytest.mark.parametrize("dt,vdt", [(torch.bfloat16, None), (torch.bfloat16, torch.float32), (torch.float16, None),
+                                    (torch.float16, torch.float32), (torch.float32, None)])
+def test_tokens_of_many_heads(B, HK, H, DK, DV, dt, vdt):
+    """One token of more heads than the GPU has SMs (another kernel), with a state, without one, and without keeping it."""
+    q, k, v, g, beta, s0 = _inputs(B, 1, HK, H, DK, DV, dt, vdt, seed=DK)
+    for norm in (True, False):
+        o, s, eo, es = steps.rule_step(q, k, v, g, beta, s0, l2norm=norm)
+        got, sT = recurrent_gated_delta_rule(q, k, v, g, beta, s0, True, norm)
+        _near(got, o, eo, dt)
+        _near(sT, s, es)
+        only, none = recurrent_gated_delta_rule(q, k, v, g, beta, s0, False, norm)
+        assert none is None and torch.equal(only, got)
+    o, s, eo, es = steps.rule_step(q, k, v, g, beta, torch.zeros_like(s0), l2norm=True)
+    got, sT = recurrent_gated_delta_rule(q, k, v, g, beta, None, True, True)
+    _near(got, o, eo, dt)
+    _near(sT, s, es)
+
+
 def test_without_norm_and_without_a_state():
     q, k, v, g, beta, s0 = _inputs(2, 5, 2, 4, 64, 64, torch.float32, seed=3)
     k = k * 0.1
@@ -118,6 +138,29 @@ def test_slots_that_cannot_be():
     a = pool.clone()
     o = gated_delta_step(q, k, v, g, beta, a, i32(5, 5, 5, 5, 5), i32(0, 1, 2, 3, 4))
     assert bool(o.isfinite().all()) and torch.equal(a[5], pool[5])
+
+
+@pytest.mark.parametrize("B", [2, 100])
+def test_many_heads_and_an_empty_pool(B):
+    """The same refusals where heads outnumber the SMs (another kernel), and a pool without a slot."""
+    q, k, v, g, beta, _ = _inputs(B, 1, 2, 4, 64, 64, torch.bfloat16, seed=12)
+    pool = torch.randn(B + 3, 4, 64, 64, device="cuda")
+    slots = torch.arange(B, dtype=torch.int32, device="cuda")
+    slots[1] = B + 3
+    if B > 2:
+        slots[7], slots[40], slots[50] = -5, 41, 1 << 30
+    live = [i for i in range(B) if i not in (1, 7, 40, 41, 50)]
+    o, s, eo, es = steps.rule_step(q[live], k[live], v[live], g[live], beta[live], pool[live], l2norm=True)
+    a = pool.clone()
+    got = gated_delta_step(q, k, v, g, beta, a, slots, use_qk_l2norm_in_kernel=True)
+    _near(got[live], o, eo, torch.bfloat16)
+    _near(a[live], s, es)
+    rest = [i for i in range(B + 3) if i not in live]
+    assert torch.equal(a[rest], pool[rest]) and bool(got[1].isnan().all())
+    if B > 2:
+        assert not got[7].any() and bool(got[[40, 41, 50]].isnan().all())
+    none = gated_delta_step(q, k, v, g, beta, pool[:0], slots)
+    assert bool(none[[i for i in range(B) if B == 2 or i != 7]].isnan().all())
 
 
 def test_a_run_equals_its_tokens():
