@@ -358,15 +358,16 @@ int gd_rule_step(const void* q, const void* k, const void* v, const float* g, co
 /* ---- the gated feed-forward block ----
  * g = x w_gate^T, u = x w_up^T, h = silu(g) u, y = h w_down^T: x [rows, D], w_gate, w_up [F, D], w_down [O, F], y [rows, O], all
  * in `dtype` (GD_FLOAT16 or GD_BFLOAT16); D, F, O multiples of 8. Products of 16-bit operands, sums in float32; h is rounded to
- * `dtype`. ld: elements from row to row of x, w_gate, w_up, w_down (and dy in the
- * backward), multiples of 8; y and the gradients are contiguous. All pointers 16-byte aligned. Asynchronous on `stream`,
- * no atomics whose order changes results.
+ * `dtype`. ld: elements from row to row of x, w_gate, w_up, w_down (and dy in the backward), multiples of 8; y and the gradients
+ * are contiguous. All pointers 16-byte aligned. A device wait that gives up leaves NaN in what it could not compute and its code
+ * in the workspace's first word (up to 128 rows without `kept`: NaN alone). Asynchronous on `stream`, no atomics whose order
+ * changes results.
  * Replaces: the SwiGLU part and the three projections around it (src/macai/layer/_swiglu.py:41-45). */
 size_t gd_ff_workspace_bytes(long long rows, int D, int F, int O, int for_backward);
 
-/* kept [3, rows, F rounded up to a multiple of 64] 16-bit words: the upper 24 bits of g's and u's float32 values (the upper halves of g's, of u's, the next
- * byte of both), for the backward; or NULL. bounds (GD_FLOAT16 with kept; 16 bytes): max |g| and max |u|, for the backward;
- * else NULL. */
+/* kept [3, rows, F rounded up to a multiple of 64] 16-bit words: the upper 24 bits of g's and u's float32 values (the upper
+ * halves of g's, of u's, the next byte of both), for the backward; or NULL. bounds (GD_FLOAT16 with kept; 16 bytes): max |g| and
+ * max |u|, for the backward; else NULL. */
 int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, void* kept, unsigned int* bounds,
               void* y, int dtype, long long rows, int D, int F, int O, const long long* ld,
               void* workspace, size_t workspace_bytes, void* stream);
@@ -380,13 +381,14 @@ int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w
 /* ---- softmax cross entropy of a vocabulary projection, without the logits ----
  * loss_i = logsumexp_v(x_i . w_v) - x_i . w_label(i): x [rows, D], w [V, D] in `dtype` (GD_FLOAT16 or GD_BFLOAT16), ldx and ldw
  * elements from row to row (multiples of 8), D a multiple of 8, any V up to 2^24; labels [rows] int32, or int64 with label64.
- * A row whose label is `ignore` has loss 0 and a zero row in dx, whatever it holds (in dw its infinities and NaN meet a weight
- * of 0, as in the formula's product); any other label outside [0, V) gives NaN.
+ * A row whose label is `ignore` has loss 0, a zero row in dx and no part in dw, whatever it holds; any other label outside
+ * [0, V) gives NaN.
  * reduction 0: loss [rows]; 1: the mean over the rows that are not ignored (none: NaN); 2: their sum; float32.
  * Ignored rows cost no products: the others are gathered. The workspace of the forward holds their x and 8 bytes a row and 128
- * columns; that of the backward their x and dx, a piece of the vocabulary's gradients of the logits in `dtype` (at most 256 MiB, or
- * 256 columns) and float32 sums of dx (with more than one piece: one for each value; else at most 64 MiB). Asynchronous on
- * `stream`; the same bits every run. No counterpart in the reference. */
+ * columns; that of the backward their x and dx, a piece of the vocabulary's gradients of the logits in `dtype` (at most 256 MiB,
+ * or 256 columns) and float32 sums of dx (with more than one piece: one for each value; else at most 64 MiB). A device wait that
+ * gives up leaves its code in the workspace's first word and NaN in what it could not compute. Asynchronous on `stream`; the same
+ * bits every run. No counterpart in the reference. */
 size_t gd_xent_workspace_bytes(long long rows, int D, int V, int for_backward);
 
 /* For the backward (or NULL, both): lse [rows, 2], the live rows' largest logits and the base-2 logarithms of their sums of

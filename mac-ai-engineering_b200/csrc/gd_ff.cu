@@ -54,10 +54,13 @@ void shape(Op& op, long long M, long long N, int tile_n = gemm::kTileN) {
 // Few tiles of y, or of dx beside the weights' gradients, have their contraction cut (gemm::cut_of; as if all gradients were asked
 // for, so that each has the same bits whichever are). 129 rows, 4,096 x 12,288: a call takes 101 us, uncut 116.
 gemm::Cut cut_y(long long n, int F, int O) {
-  return gemm::cut_of((long long)gemm::blocks_of(n, gemm::kTileM) * gemm::blocks_of(O, gemm::kTileN), gemm::blocks_of(F, gemm::kBlockK), 0, O);
+  const long long tiles = (long long)gemm::blocks_of(n, gemm::kTileM) * gemm::blocks_of(O, gemm::kTileN);
+  return gemm::cut_of(tiles, gemm::blocks_of(F, gemm::kBlockK), 0, O);
 }
 gemm::Cut cut_dx(long long n, int D, int F, int O) {
-  auto tiles = [](long long M, long long N) { return (long long)gemm::blocks_of(M, gemm::kTileM) * gemm::blocks_of(N, gemm::kTileN); };
+  auto tiles = [](long long M, long long N) {
+    return (long long)gemm::blocks_of(M, gemm::kTileM) * gemm::blocks_of(N, gemm::kTileN);
+  };
   return gemm::cut_of(tiles(n, D), 2ll * gemm::blocks_of(F, gemm::kBlockK),
                       (2 * tiles(F, D) + tiles(O, F)) * gemm::blocks_of(n, gemm::kBlockK), D);
 }
@@ -66,7 +69,8 @@ size_t sum_bytes(const gemm::Cut& c, long long n, int D) {
 }
 
 template <typename T>
-int forward(const Problem& q, void* const* kept, void* h, float* sum, void* y, uint32_t* bounds, ErrorWord* err, cudaStream_t stream) {
+int forward(const Problem& q, void* const* kept, void* h, float* sum, void* y, uint32_t* bounds, ErrorWord* err,
+            cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const long long n = q.rows;
   Params p = {};
@@ -85,8 +89,8 @@ int forward(const Problem& q, void* const* kept, void* h, float* sum, void* y, u
   Op& d = r.op[0];
   shape(d, n, q.O);
   d.kb[0] = gemm::blocks_of(q.F, gemm::kBlockK);
-  if (!gemm::operand_map(&d.a[0], h, dt, n, q.F, pitch(q.F), false) || !gemm::operand_map(&d.b[0], q.wd, dt, q.O, q.F, q.ldd, false) ||
-      !gemm::slab_map(&d.c, y, dt, n, q.O, q.O))
+  if (!gemm::operand_map(&d.a[0], h, dt, n, q.F, pitch(q.F), false) ||
+      !gemm::operand_map(&d.b[0], q.wd, dt, q.O, q.F, q.ldd, false) || !gemm::slab_map(&d.c, y, dt, n, q.O, q.O))
     return GD_ERR_LAUNCH;
   const gemm::Cut c = cut_y(n, q.F, q.O);
   d.slices = c.slices, d.per = c.per, d.sum_mode = c.slices > 1 ? 1 : 0, d.sum = sum;

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ F
   // (the first kernel's inputs may come from the kernel before it in the stream, which need not know of this)
   if (GATED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  bool fed = true;  // (the products' warp) no wait for a stage gave up
   if (warp == 4) {
     const uint32_t lead = wattn::elect();
     const int total = to - from;
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ F
     constexpr uint32_t id = wattn::idesc<T>(kRowsM, N, false);
     for (int i = 0; i < total; ++i) {
       const int slot = i % C::kStages;
-      if (!gemm::warp_wait(full + slot, (i / C::kStages) & 1, nullptr, 0)) break;
+      if (!(fed = gemm::warp_wait(full + slot, (i / C::kStages) & 1, nullptr, 0))) break;
       tc_fence_after();
       const uint32_t a = wattn::desc_k(s_base + slot * (C::kW + C::kT)), b = wattn::desc_k(s_base + slot * (C::kW + C::kT) + C::kW);
 #pragma unroll
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ F
     wattn::mma_commit(lead, done);
     gemm::warp_wait(done, 0, nullptr, 0);
   }
-  const bool ok = __syncthreads_and(warp >= 4 || gemm::warp_wait(done, 0, nullptr, 0)) != 0;
+  const bool ok = __syncthreads_and(warp >= 4 ? fed : gemm::warp_wait(done, 0, nullptr, 0)) != 0;
   float* const part = reinterpret_cast<float*>(base);  // [token][row of the tile]; the ring is read and its copies have landed
   if (warp < 4) {
     tc_fence_after();

@@ -19,7 +19,7 @@
 // 128,000: logits 2.44 to 2.85 ms (1,360 to 1,580), with their gradients stored 2.53 to 2.97 ms, its two gradients 5.4 to 6.1 ms.
 #pragma once
 
-#include <algorithm>
+#include <utility>
 
 #include "gd_wattn.cuh"
 
@@ -262,7 +262,9 @@ __device__ __forceinline__ Where locate(const Params& p, int tile, int live) {
   return w;
 }
 // the tile's stages, of both segments one after the other, and the first of them
-__device__ __forceinline__ int first_segment(const Op& o, int live) { return o.k_live ? (live + kBlockK - 1) / kBlockK : o.kb[0]; }
+__device__ __forceinline__ int first_segment(const Op& o, int live) {
+  return o.k_live ? (live + kBlockK - 1) / kBlockK : o.kb[0];
+}
 __device__ __forceinline__ int stages_of(const Op& o, const Where& w, int live, int& from) {
   const int n = first_segment(o, live) + o.kb[1];
   from = w.slice * o.per;
@@ -439,7 +441,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const CUtensorMap *ma = &op.a[s], *mb = E == kSwiglu ? &op.b[rank] : &op.b[s];
         // the tile's stages in this segment
         int first;
-        const int all = stages_of(op, w, live, first), here = s == 0 ? 0 : first_segment(op, live), size = s == 0 ? first_segment(op, live) : op.kb[1];
+        const int all = stages_of(op, w, live, first), one = first_segment(op, live);
+        const int here = s == 0 ? 0 : one, size = s == 0 ? one : op.kb[1];
         int from = first > here ? first - here : 0, n = (first + all - here < size ? first + all - here : size) - from;
         n = __shfl_sync(0xffffffffu, n, 0);
         from = __shfl_sync(0xffffffffu, from, 0);
@@ -631,7 +634,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           }
         }
       } else if constexpr (E == kDSwiglu) {
-        const float f = carried(p.bounds, p.more) + bad;
+        float f = carried(p.bounds, p.more) + bad;
 #pragma unroll 1
         for (int s = 0; s < 4; ++s, ++step) {
           const int c = half * 128 + s * 32, n0 = w.n + c, set = step & 1;
@@ -640,7 +643,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           if (s == 3) release();
           const bool here = has(n0);
           if (here) {
-            warp_wait(aux + 2 * ew + set, (landed >> set) & 1, p.err, 86);
+            if (!warp_wait(aux + 2 * ew + set, (landed >> set) & 1, p.err, 86)) f = NAN;
             landed ^= 1u << set;
           }
           if (s < 3) fetch(step + 1, w);
@@ -805,7 +808,9 @@ inline Cut cut_of(long long tiles, long long stages, long long rest, int D) {
   c.slices = blocks_of(stages, c.per);
   return c;
 }
-inline size_t cut_bytes(const Cut& c, long long tiles) { return c.slices > 1 ? (size_t)c.slices * tiles * kTileM * kTileN * 4 : 0; }
+inline size_t cut_bytes(const Cut& c, long long tiles) {
+  return c.slices > 1 ? (size_t)c.slices * tiles * kTileM * kTileN * 4 : 0;
+}
 
 // Whether C's tiles can be counted (they are ints, several problems' together).
 inline bool countable(long long M, long long N) { return (M + 127) / 128 * ((N + 127) / 128) < (1ll << 28); }
@@ -815,7 +820,8 @@ inline bool countable(long long M, long long N) { return (M + 127) / 128 * ((N +
 template <typename T, int E>
 int launch(Params& p, cudaStream_t stream) {
   auto length = [](const Op& o) { return o.slices > 1 ? o.per : o.kb[0] + o.kb[1]; };
-  std::stable_sort(p.op, p.op + p.ops, [&](const Op& a, const Op& b) { return length(a) > length(b); });
+  for (int i = 1; i < p.ops; ++i)
+    for (int j = i; j > 0 && length(p.op[j]) > length(p.op[j - 1]); --j) std::swap(p.op[j], p.op[j - 1]);
   int tiles = 0;
   for (int i = 0; i < p.ops; ++i) {
     if (p.op[i].slices < 1) p.op[i].slices = 1;

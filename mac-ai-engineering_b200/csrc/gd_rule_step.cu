@@ -508,9 +508,9 @@ extern "C" int gd_rule_step(const void* q, const void* k, const void* v, const f
   if ((dtype != GD_FLOAT32 && dtype != GD_FLOAT16 && dtype != GD_BFLOAT16) || (vdtype != dtype && vdtype != GD_FLOAT32) ||
       (flags & ~GD_L2NORM))
     return GD_ERR_ARG;
-  if (B < 0 || B > 65535 || T < 0 || H <= 0 || HK <= 0 || H % HK != 0 || H > (1 << 24) || (long long)n_slots * H >= (1ll << 31) || DK <= 0 || DK % 32 != 0 ||
-      DK > kMaxWidth || DV <= 0 || DV % 32 != 0 || DV > kMaxWidth || n_slots < 0 ||
-      (slots == nullptr && n_slots < B))
+  if (B < 0 || B > 65535 || T < 0 || H <= 0 || HK <= 0 || H % HK != 0 || H > (1 << 24) || n_slots < 0 ||
+      (long long)n_slots * H >= (1ll << 31) || DK <= 0 || DK % 32 != 0 || DK > kMaxWidth || DV <= 0 || DV % 32 != 0 ||
+      DV > kMaxWidth || (slots == nullptr && n_slots < B))
     return GD_ERR_SHAPE;
   if (B == 0) return GD_OK;
   if ((slots == nullptr) != (out_slots == nullptr)) return GD_ERR_ARG;

@@ -285,13 +285,15 @@ BwdPlan bwd_plan(long long n, int D, int V) {
   const long long kn = gemm::blocks_of(n, gemm::kBlockK);
   b.cut = {1, 0};
   if (b.pieces == 1)
-    b.cut = gemm::cut_of(tiles_m * tiles_n, gemm::blocks_of(V, gemm::kBlockK), gemm::blocks_of(V, gemm::kTileM) * tiles_n * kn, D);
+    b.cut = gemm::cut_of(tiles_m * tiles_n, gemm::blocks_of(V, gemm::kBlockK),
+                         gemm::blocks_of(V, gemm::kTileM) * tiles_n * kn, D);
   b.scale = kHead;
   b.rows = b.scale + up((size_t)n * sizeof(float));
   b.dx = b.rows + up((size_t)n * pitch(D) * 2);
   b.d = b.dx + up((size_t)n * pitch(D) * 2);
   b.sum = b.d + up((size_t)n * b.ldd * 2);
-  b.total = b.sum + (b.pieces > 1 ? (size_t)tiles_m * tiles_n * gemm::kTileM * gemm::kTileN * 4 : gemm::cut_bytes(b.cut, tiles_m * tiles_n));
+  b.total = b.sum + (b.pieces > 1 ? (size_t)tiles_m * tiles_n * gemm::kTileM * gemm::kTileN * 4
+                                  : gemm::cut_bytes(b.cut, tiles_m * tiles_n));
   return b;
 }
 
@@ -399,8 +401,8 @@ int backward(const Problem& q, const float2* lse, const float* dloss, void* dx, 
       Op g = {};
       shape(g, q.n, q.D);
       g.slices = b.cut.slices, g.factor = factor;
-      if (const int st = gemm::sum_slices<T>(reinterpret_cast<const float*>(ws + b.sum), g, q.n, q.D, q.plan.live, q.plan.place, nullptr,
-                                             nullptr, dx, stream))
+      if (const int st = gemm::sum_slices<T>(reinterpret_cast<const float*>(ws + b.sum), g, q.n, q.D, q.plan.live,
+                                             q.plan.place, nullptr, nullptr, dx, stream))
         return st;
     } else {
       spread_kernel<<<grid_of(q.n), 256, 0, stream>>>(static_cast<const uint16_t*>(dxc), ld, q.n, q.D, q.plan.place,
