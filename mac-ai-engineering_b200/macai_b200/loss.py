@@ -43,8 +43,8 @@ def _fwd(x, w, labels, ignore, reduction, keep):
     size = _bytes(n, D, w.shape[0], 0)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     launch("gd_xent_fwd", x.get_device(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.dtype == torch.int64,
-           loss.data_ptr(), None if lse is None else lse.data_ptr(), None if plan is None else plan.data_ptr(), reduction, ignore, _DTYPES[x.dtype], n, D, w.shape[0],
-           pitch(x), pitch(w), ws.data_ptr(), size)
+           loss.data_ptr(), None if lse is None else lse.data_ptr(), None if plan is None else plan.data_ptr(), reduction,
+           ignore, _DTYPES[x.dtype], n, D, w.shape[0], pitch(x), pitch(w), ws.data_ptr(), size)
     return loss, lse, plan
 
 
@@ -84,8 +84,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     """The cross entropy of the logits x weight^T, in float32: x [..., D] and weight [V, D] (as nn.Linear keeps it) both
     bfloat16 or both float16, D a multiple of 8, V any size; labels [...] int64 or int32. reduction "none": one loss for each
     row, in the labels' shape; "mean": over the rows that are not ignored (NaN if all are); "sum". A row with the label
-    ignore_index has loss 0 and a zero row in x's gradient, whatever it holds (in the weight's, its infinities and NaN meet a
-    weight of 0, as in the formula's product); any other label outside [0, V) gives NaN (nothing waits for the host to look). Gradients of x and weight come in their type, the same bits every run; a frozen one's is not formed.
+    ignore_index has loss 0, a zero row in x's gradient and no part in the weight's, whatever it holds; any other label outside
+    [0, V) gives NaN (nothing waits for the host to look). Gradients of x and weight come in their type, the same bits every
+    run; a frozen one's is not formed.
 
     Ignored rows cost no products. The logits are never kept: beside the gradients a call holds the other rows of x and 8 bytes
     for each row and 128 columns; the backward at most 256 MiB (or 256 columns) of the logits' gradients, x's gradient once

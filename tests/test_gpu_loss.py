@@ -280,3 +280,16 @@ def test_refusals():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises((NotImplementedError, RuntimeError)):
             linear_cross_entropy(dual, w, lab)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("n,D,V", [(300, 64, 500), (65, 200, 70)])
+def test_ignored_rows_may_hold_anything(n, D, V, value):
+    """Their infinities and NaN reach no loss and neither gradient, the weight's included: they are not gathered."""
+    x, w, lab = _inputs(n, D, V, BF, seed=21, ignored=0.4)
+    g = torch.tensor(1.0, device="cuda")
+    want = _run(x, w, lab, "mean", g)
+    y = x.clone()
+    y[lab < 0] = value
+    got = _run(y, w, lab, "mean", g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and bool(got[2].isfinite().all())
