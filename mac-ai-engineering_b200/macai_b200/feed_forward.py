@@ -6,7 +6,8 @@ after its mixer:
 `gated_feed_forward` trains, prefills, and takes the few tokens of a decoding step. tcgen05 products with float32 sums; the
 activation and its gradient are taken in float32 as the products leave the tensor core, so neither g nor u is read again in
 the forward, and the gradient of h never leaves the chip. h and the gradients of g and u are rounded to the inputs' 16-bit type
-(the matrix instruction's operands); g and u are kept for the backward in 24 bits. bfloat16 and float16. There is no CPU path: CUDA tensors only.
+(the matrix instruction's operands); g and u are kept for the backward in 24 bits. bfloat16 and float16. There is no CPU path:
+CUDA tensors only.
 """
 from __future__ import annotations
 
@@ -41,7 +42,7 @@ def _sizes(x, wg, wd):
 def _fwd(x, wg, wu, wd, keep):
     """(y, kept, bounds) on matrices; keep: 24 bits of g and u (and float16's bounds) for the backward, else None."""
     n, D, F, O = _sizes(x, wg, wd)
-    y = torch.empty((n, O), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, O))
     if n == 0:
         return y, None, None
     kept = bounds = None
@@ -49,11 +50,11 @@ def _fwd(x, wg, wu, wd, keep):
         kept = torch.empty((3, n, -(-F // 64) * 64), dtype=torch.int16, device=x.device)
         if x.dtype == torch.float16:
             bounds = torch.empty(4, dtype=torch.int32, device=x.device)
-    size = _bytes(n, D, F, O, 0)
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    size = _bytes(n, D, F, O, 0)  # (a multiple of 256)
+    ws = x.new_empty(size // 2)
     launch("gd_ff_fwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(),
-           None if kept is None else kept.data_ptr(), None if bounds is None else bounds.data_ptr(), y.data_ptr(), _DTYPES[x.dtype], n, D, F, O, _longs(pitch(x), pitch(wg), pitch(wu), pitch(wd)),
-           ws.data_ptr(), size)
+           None if kept is None else kept.data_ptr(), None if bounds is None else bounds.data_ptr(), y.data_ptr(),
+           _DTYPES[x.dtype], n, D, F, O, _longs(pitch(x), pitch(wg), pitch(wu), pitch(wd)), ws.data_ptr(), size)
     return y, kept, bounds
 
 

@@ -107,7 +107,7 @@ def gated_delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         raise ValueError(f"{name}: {B} requests need as many slots, the pool has {state.shape[0]}")
     if recorded(query, key, value, g, beta, state):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train with chunk_gated_delta_rule")
-    o = torch.empty((B, T, H, DV), dtype=q.dtype, device=q.device)
+    o = torch.empty_like(v) if v.dtype == q.dtype else q.new_empty((B, T, H, DV))
     at = None if slots is None else slots.data_ptr()
     launch("gd_rule_step", index, q.data_ptr(), k.data_ptr(), v.data_ptr(), g_.data_ptr(), beta_.data_ptr(), pool, pool, at,
            at if out_slots is None else out_slots.data_ptr(), o.data_ptr(), _DTYPES[q.dtype], _DTYPES[v.dtype], B, T, H, HK,
@@ -133,7 +133,7 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, o
             raise ValueError(f"{name}: initial_state must be [B, H, DK, DV] = {(B, H, DK, DV)} on the query's device")
         s0 = aligned(initial_state.float())
     sT = torch.empty((B, H, DK, DV), dtype=torch.float32, device=q.device) if output_final_state else None
-    o = torch.empty((B, T, H, DV), dtype=q.dtype, device=q.device)
+    o = torch.empty_like(v) if v.dtype == q.dtype else q.new_empty((B, T, H, DV))
     launch("gd_rule_step", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), g_.data_ptr(), beta_.data_ptr(),
            None if s0 is None else s0.data_ptr(), None if sT is None else sT.data_ptr(), None, None, o.data_ptr(),
            _DTYPES[q.dtype], _DTYPES[v.dtype], B, T, H, HK, DK, DV, B, _lib.GD_L2NORM if use_qk_l2norm_in_kernel else 0)
