@@ -67,7 +67,7 @@ def _inputs(name, q, k, v, g, beta):
     if k.dtype != dt:
         k = k.to(dt)
     if v.dtype != dt and v.dtype != torch.float32:
-        v = v.to(dt)
+        v = v.float()  # (exact for any other type of 16 bits)
     if g.dtype != torch.float32:
         g = g.float()
     if beta.dtype != torch.float32:

@@ -243,3 +243,38 @@ def test_forward_mode_is_refused():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises((NotImplementedError, RuntimeError)):
             gated_feed_forward(dual, wg, wu, wd)
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+def test_a_kept_graph_and_a_shared_weight(dt):
+    """The backward twice over one graph has the same bits; a weight given twice gets the sum of its two gradients."""
+    x, wg, wu, wd, dy = _inputs(150, 64, 136, 72, dt, seed=30)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = gated_feed_forward(*leaves)
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    torch.autograd.grad(y, leaves, 3 * dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    one, two = wg.clone().requires_grad_(True), wg.clone().requires_grad_(True)
+    both = torch.autograd.grad(gated_feed_forward(x, one, two, wd), [one, two], dy)
+    same = torch.autograd.grad(gated_feed_forward(x, one, one, wd), [one], dy)[0]
+    assert torch.equal(same, both[0] + both[1])
+
+
+def test_checkpointed_block():
+    """Formed again in the backward: the same gradients, in both of torch's forms of it."""
+    from torch.utils.checkpoint import checkpoint
+    x, wg, wu, wd, dy = _inputs(140, 64, 128, 64, BF, seed=31)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    want = torch.autograd.grad(gated_feed_forward(*leaves), leaves, dy)
+    for reentrant in (False, True):
+        copies = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+        checkpoint(gated_feed_forward, *copies, use_reentrant=reentrant).backward(dy)
+        assert all(torch.equal(t.grad, v) for t, v in zip(copies, want))
+
+
+def test_inference_mode():
+    x, wg, wu, wd, _ = _inputs(5, 64, 128, 64, BF, seed=32)
+    want = gated_feed_forward(x, wg, wu, wd)
+    with torch.inference_mode():
+        assert torch.equal(gated_feed_forward(x.clone(), wg, wu, wd), want)

@@ -293,3 +293,30 @@ def test_ignored_rows_may_hold_anything(n, D, V, value):
     y[lab < 0] = value
     got = _run(y, w, lab, "mean", g)
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and bool(got[2].isfinite().all())
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+def test_a_kept_graph_and_changed_labels(dt):
+    """The backward twice over one graph has the same bits, whatever became of the labels after the forward."""
+    x, w, lab = _inputs(150, 64, 200, dt, seed=22)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    g = torch.rand(150, device="cuda")
+    loss = linear_cross_entropy(*leaves, lab, reduction="none")
+    first = torch.autograd.grad(loss, leaves, g, retain_graph=True)
+    lab.fill_(-100)
+    torch.autograd.grad(loss, leaves, 2 * g, retain_graph=True)
+    again = torch.autograd.grad(loss, leaves, g)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_a_tied_weight():
+    """x made from the weight itself, as with tied embeddings: both gradients arrive in it."""
+    w = _inputs(4, 64, 90, BF, seed=23)[1].requires_grad_(True)
+    tokens, lab = torch.tensor([3, 70, 3, 89, 0], device="cuda"), torch.tensor([70, 3, 89, 0, -100], device="cuda")
+    got = torch.autograd.grad(linear_cross_entropy(w[tokens], w, lab), w)[0]
+    x = w.detach()[tokens].requires_grad_(True)
+    dx, dw = torch.autograd.grad(linear_cross_entropy(x, w, lab), [x, w])
+    e = w.detach().clone().requires_grad_(True)
+    want = dw.double() + torch.autograd.grad(e[tokens], e, dx)[0].double()
+    # one rounding of the sum of two gradients in bf16
+    assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-30).all())

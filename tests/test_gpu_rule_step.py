@@ -244,3 +244,15 @@ def test_refusals():
             gated_delta_step(q, k, v, g, beta, s0, **kw)
     with pytest.raises(ValueError, match="initial_state"):
         recurrent_gated_delta_rule(q, k, v, g, beta, s0[:1])
+
+
+def test_a_value_of_another_type():
+    """A float16 value beside bfloat16 queries is not rounded to their type; inference mode's tensors are taken."""
+    q, k, v, g, beta, s0 = _inputs(2, 3, 2, 2, 64, 64, torch.bfloat16, torch.float16, seed=40)
+    a, sa = recurrent_gated_delta_rule(q, k, v, g, beta, s0, True, True)
+    b, sb = recurrent_gated_delta_rule(q, k, v.float(), g, beta, s0, True, True)
+    assert torch.equal(a, b) and torch.equal(sa, sb)
+    with torch.inference_mode():
+        pool = s0.clone()
+        c = gated_delta_step(q, k, v, g, beta, pool, use_qk_l2norm_in_kernel=True)
+    assert torch.equal(a, c) and torch.equal(sa, pool)
