@@ -48,6 +48,11 @@ def matrix(t: torch.Tensor) -> torch.Tensor:
     return aligned(m.contiguous())
 
 
+def room(m: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor like the `matrix` m."""
+    return torch.empty_like(m) if m.is_contiguous() else m.new_empty(m.shape)
+
+
 def pitch(m: torch.Tensor) -> int:
     """Elements from row to row of a `matrix`."""
     n, d = m.shape

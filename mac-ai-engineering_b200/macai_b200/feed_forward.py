@@ -17,7 +17,7 @@ import functools
 import torch
 
 from . import _lib
-from ._call import first_order, launch, matrix, pitch, recorded
+from ._call import first_order, launch, matrix, pitch, recorded, room
 
 _DTYPES = {torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 
@@ -40,37 +40,38 @@ def _sizes(x, wg, wd):
 
 
 def _fwd(x, wg, wu, wd, keep):
-    """(y, kept, bounds) on matrices; keep: 24 bits of g and u (and float16's bounds) for the backward, else None."""
+    """(y, kept) on matrices; keep: 24 bits of g and u, and behind them float16's two bounds, for the backward, else None."""
     n, D, F, O = _sizes(x, wg, wd)
     y = x.new_empty((n, O))
     if n == 0:
-        return y, None, None
-    kept = bounds = None
+        return y, None
+    kept = at = bounds = None
     if keep:
-        kept = torch.empty((3, n, -(-F // 64) * 64), dtype=torch.int16, device=x.device)
-        if x.dtype == torch.float16:
-            bounds = torch.empty(4, dtype=torch.int32, device=x.device)
+        words = 3 * n * (-(-F // 64) * 64)
+        kept = x.new_empty(words + 8)
+        at = kept.data_ptr()
+        bounds = at + 2 * words if x.dtype == torch.float16 else None
     size = _bytes(n, D, F, O, 0)  # (a multiple of 256)
     ws = x.new_empty(size // 2)
-    launch("gd_ff_fwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(),
-           None if kept is None else kept.data_ptr(), None if bounds is None else bounds.data_ptr(), y.data_ptr(),
+    launch("gd_ff_fwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), at, bounds, y.data_ptr(),
            _DTYPES[x.dtype], n, D, F, O, _longs(pitch(x), pitch(wg), pitch(wu), pitch(wd)), ws.data_ptr(), size)
-    return y, kept, bounds
+    return y, kept
 
 
-def _bwd(x, wg, wu, wd, kept, bounds, dy, need):
+def _bwd(x, wg, wu, wd, kept, dy, need):
     """(dx, dw_gate, dw_up, dw_down), contiguous, each None unless needed."""
     n, D, F, O = _sizes(x, wg, wd)
-    make = lambda yes, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if yes else None  # noqa: E731
-    out = (make(need[0], n, D), make(need[1], F, D), make(need[2], F, D), make(need[3], O, F))
+    out = [room(t) if yes else None for t, yes in zip((x, wg, wu, wd), need)]
     if n == 0:
         return tuple(None if t is None else t.zero_() for t in out)
+    at = kept.data_ptr()
     size = _bytes(n, D, F, O, 1)
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    launch("gd_ff_bwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), kept.data_ptr(),
-           None if bounds is None else bounds.data_ptr(), dy.data_ptr(), *(None if t is None else t.data_ptr() for t in out),
-           _DTYPES[x.dtype], n, D, F, O, _longs(pitch(x), pitch(wg), pitch(wu), pitch(wd), pitch(dy)), ws.data_ptr(), size)
-    return out
+    ws = x.new_empty(size // 2)
+    launch("gd_ff_bwd", x.get_device(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), at,
+           at + 2 * (kept.numel() - 8) if x.dtype == torch.float16 else None, dy.data_ptr(),
+           *[None if t is None else t.data_ptr() for t in out], _DTYPES[x.dtype], n, D, F, O,
+           _longs(pitch(x), pitch(wg), pitch(wu), pitch(wd), pitch(dy)), ws.data_ptr(), size)
+    return tuple(out)
 
 
 class GatedFeedForward(torch.autograd.Function):
@@ -78,8 +79,8 @@ class GatedFeedForward(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, wg, wu, wd):
-        y, kept, bounds = _fwd(x, wg, wu, wd, True)
-        ctx.save_for_backward(x, wg, wu, wd, kept, bounds)
+        y, kept = _fwd(x, wg, wu, wd, True)
+        ctx.save_for_backward(x, wg, wu, wd, kept)
         return y
 
     @staticmethod

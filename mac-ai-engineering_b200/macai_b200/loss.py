@@ -15,7 +15,7 @@ import functools
 import torch
 
 from . import _lib
-from ._call import first_order, launch, matrix, pitch, recorded
+from ._call import first_order, launch, matrix, pitch, recorded, room
 
 _DTYPES = {torch.float16: _lib.GD_FLOAT16, torch.bfloat16: _lib.GD_BFLOAT16}
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -30,35 +30,38 @@ def _bytes(*sizes) -> int:
 
 
 def _fwd(x, w, labels, ignore, reduction, keep):
-    """(loss, lse, plan): lse, the live rows' maxima and sums (as logarithms), and plan, which rows those are, for the
-    backward (else None)."""
+    """(loss, kept): kept, int32 for the backward (else None): the live rows' maxima and sums (as logarithms), 2 n, and which
+    rows those are, 4 + 2 n."""
     n, D = x.shape
     loss = torch.empty(n if reduction == 0 else (), dtype=torch.float32, device=x.device)
-    lse = plan = None
-    if keep:
-        lse = torch.empty((n, 2), dtype=torch.float32, device=x.device)
-        plan = torch.empty(4 + 2 * n, dtype=torch.int32, device=x.device)
+    kept = lse = plan = None
     if n == 0:  # no row: torch's own results, a mean over nothing among them
-        return loss.fill_(float("nan") if reduction == 1 else 0.0), lse, plan
-    size = _bytes(n, D, w.shape[0], 0)
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        return loss.fill_(float("nan") if reduction == 1 else 0.0), kept
+    if keep:
+        kept = torch.empty(4 + 4 * n, dtype=torch.int32, device=x.device)
+        lse = kept.data_ptr()
+        plan = lse + 8 * n
+    size = _bytes(n, D, w.shape[0], 0)  # (even)
+    ws = x.new_empty(size // 2)
     launch("gd_xent_fwd", x.get_device(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.dtype == torch.int64,
-           loss.data_ptr(), None if lse is None else lse.data_ptr(), None if plan is None else plan.data_ptr(), reduction,
-           ignore, _DTYPES[x.dtype], n, D, w.shape[0], pitch(x), pitch(w), ws.data_ptr(), size)
-    return loss, lse, plan
+           loss.data_ptr(), lse, plan, reduction, ignore, _DTYPES[x.dtype], n, D, w.shape[0], pitch(x), pitch(w), ws.data_ptr(),
+           size)
+    return loss, kept
 
 
-def _bwd(x, w, lse, plan, dloss, reduction, need):
+def _bwd(x, w, kept, dloss, reduction, need):
     """(dx, dw), contiguous, each None unless needed."""
     n, D = x.shape
     V = w.shape[0]
-    dx = torch.empty((n, D), dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty((V, D), dtype=x.dtype, device=x.device) if need[1] else None
-    size = _bytes(n, D, V, 1) if n else 0
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if n else None
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    launch("gd_xent_bwd", x.get_device(), x.data_ptr(), w.data_ptr(), lse.data_ptr(), plan.data_ptr(), dloss.data_ptr(), p(dx),
-           p(dw), reduction, _DTYPES[x.dtype], n, D, V, pitch(x), pitch(w), p(ws), size)
+    dx, dw = room(x) if need[0] else None, room(w) if need[1] else None
+    if n == 0:
+        return dx, None if dw is None else dw.zero_()
+    size = _bytes(n, D, V, 1)
+    ws = x.new_empty(size // 2)
+    lse = kept.data_ptr()
+    launch("gd_xent_bwd", x.get_device(), x.data_ptr(), w.data_ptr(), lse, lse + 8 * n, dloss.data_ptr(),
+           None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), reduction, _DTYPES[x.dtype], n, D, V,
+           pitch(x), pitch(w), ws.data_ptr(), size)
     return dx, dw
 
 
@@ -67,8 +70,8 @@ class LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, labels, ignore, reduction):
-        loss, lse, plan = _fwd(x, w, labels, ignore, reduction, True)
-        ctx.save_for_backward(x, w, lse, plan)
+        loss, kept = _fwd(x, w, labels, ignore, reduction, True)
+        ctx.save_for_backward(x, w, kept)
         ctx.reduction = reduction
         return loss
 
