@@ -6,17 +6,19 @@
 // so a token costs one pass over S in registers and one join over the rows.
 //
 // Bound by memory: 8 DK DV bytes of a head's state for about 7 DK DV operations a token. The state is read once into registers,
-// run through all tokens of the call, and written once. The recurrence never mixes value columns, so a warp has COLS columns of a
-// head with all their rows (a lane four adjacent columns of every 128 / COLS-th row), and its sums need no other warp. Two kernels:
-//   run_kernel: runs of tokens, and few heads. The four warps of a CTA prepare the tokens' q and k together, up to eight at a time,
-// while the state is on its way; the token loop has no barrier. 24 requests x 16 heads of 128 x 128, 6 tokens: 22 us (bound by the
-// packed multiply-adds and their operands from shared memory: about 2 us a token, after 10 us of memory); 1 request x 32 heads, 1
-// token: 4.2 us with 8 columns a warp (16: 4.8, 32: 6.9), latency.
-//   token_kernel: one token of many heads. Persistent warps walk the (request, head, columns) items; while a warp works on one in
-// registers, TMA brings the next one's columns into the warp's stage of shared memory, and its rows of q, k, v into registers.
-// 125 live of 128 requests x 32 heads of 128 x 128: 99 us, 5.3 TB/s (run_kernel: 122 us; a plain copy of the states: 83 us; this
-// kernel without its arithmetic: 96 us, so that the memory's order of reads and writes is what is left). 8 requests: 10.3 us
-// (run_kernel 11.6).
+// run through all tokens of the call, and written once. The recurrence never mixes value columns, so a warp has 2,048 / ROWS
+// columns of a head with all their rows (ROWS: 64, 128 or 256, at least DK; a lane four adjacent columns of every RG-th row, 16 in
+// all), and its sums need no other warp. The order of the sums goes by DK alone: a token has the same bits in a run or alone,
+// whatever the other requests are. What decides is how many bytes are on their way, that is, how many warps with 64 registers of
+// state an SM holds: 16 of up to 128 registers. The compiler would keep the k of all rows from the sums for the update (16 registers
+// more; with spills a single token of 128 requests took 91 to 125 us); read again through a volatile pointer they cost nothing.
+// Square heads have their strides as constants (128 requests: 83 us, else 87; 64 requests x 32 heads, 4 tokens: 64, else 71).
+//   token_kernel: single tokens. 125 live of 128 requests x 32 heads of 128 x 128: 83 us, 6.35 TB/s (a plain copy of the states:
+// 81 us); 8 requests: 7.5 us; 1 request: 3.4 us. (Persistent warps with the next states on their way by TMA took 99 us: 96 KB an SM
+// under way where this one has 128; a persistent form of this one took 91, five CTAs an SM, which spill, 86.)
+//   run_kernel: runs of tokens. The four warps of a CTA prepare the tokens' q and k together, up to eight at a time, while the state
+// is on its way; the token loop has no barrier. 24 requests x 16 heads of 128 x 128, 6 tokens: 19 us: 10 us of memory, then the
+// packed multiply-adds, about 1.5 us a token; 768 CTAs are 1.3 turns of the 592 that run at once.
 #include <cstdint>
 
 #include "gd_common.cuh"
@@ -27,15 +29,15 @@ namespace rule_step {
 namespace {
 
 using wattn::F2;
-using wattn::add2;
 using wattn::f2;
 using wattn::fma2;
 using wattn::mul2;
 using wattn::unf2;
 
 constexpr int kMaxWidth = 256;  // DK, DV
-constexpr int kRunWarps = 4;
-constexpr int kRunThreads = 32 * kRunWarps;
+constexpr int kWarps = 4;       // of a CTA, at most
+constexpr int kThreads = 32 * kWarps;
+constexpr int kCtas = 4;        // an SM
 constexpr int kRun = 8;         // tokens prepared at a time
 
 struct Args {
@@ -75,26 +77,24 @@ __device__ __forceinline__ void put4(T* p, float a, float b, float c, float d) {
   else *reinterpret_cast<uint2*>(p) = make_uint2(wattn::pack16<T>(a, b), wattn::pack16<T>(c, d));
 }
 
-// ROWS: 64, 128 or 256, at least DK; COLS: columns of a warp.
-template <typename T, typename TV, int ROWS, int COLS>
-__global__ void __launch_bounds__(kRunThreads, ROWS > 128 ? 2 : 3) run_kernel(const Args a) {
-  constexpr int LC = COLS / 4, RG = 32 / LC, R = ROWS / RG;  // lanes across the columns, row groups, rows a lane has
-  constexpr int kParts = (ROWS + 127) / 128;                 // of a row of q or k, 128 values each
+template <typename T, typename TV, int ROWS, bool SQUARE>
+__global__ void __launch_bounds__(kThreads, kCtas) run_kernel(const Args a) {
+  constexpr int COLS = 2048 / ROWS, LC = COLS / 4, RG = 32 / LC, R = 16;  // a warp's columns, lanes across them, row groups, rows a lane
+  constexpr int kParts = (ROWS + 127) / 128;                              // of a row of q or k, 128 values each
   // a token's k and q, normalised, each twice (operands of the packed arithmetic), and its decay, beta, q k
   __shared__ __align__(16) float4 kq[kRun][ROWS];
   __shared__ float scalars[kRun][4];
-  const int slices = (a.DV + kRunWarps * COLS - 1) / (kRunWarps * COLS);
-  const int b = blockIdx.y, h = blockIdx.x / slices;
+  const int DK = SQUARE ? ROWS : a.DK, DV = SQUARE ? ROWS : a.DV;
+  const int warps = SQUARE ? (ROWS / COLS < kWarps ? ROWS / COLS : kWarps) : blockDim.x >> 5;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cl = lane % LC, rg = lane / LC;
-  const int c0 = ((blockIdx.x - h * slices) * kRunWarps + warp) * COLS, col = c0 + cl * 4;
-  const bool mine = c0 < a.DV;  // (DV is a multiple of 32)
+  const int per = DV / (COLS * warps), b = blockIdx.y, h = blockIdx.x / per;
+  const int col = ((blockIdx.x - h * per) * warps + warp) * COLS + cl * 4;
   const int hk = h / (a.H / a.HK);
   const int from = a.in == nullptr ? b : __ldg(a.in + b), to = a.out == nullptr ? b : __ldg(a.out + b);
-  T* const o = static_cast<T*>(a.o) + ((long long)b * a.T * a.H + h) * a.DV + col;
-  const long long o_step = (long long)a.H * a.DV;
+  T* const o = static_cast<T*>(a.o) + ((long long)b * a.T * a.H + h) * DV + col;
+  const long long o_step = (long long)a.H * DV;
   auto fill = [&](float x) {
-    if (mine)
-      for (int t = rg; t < a.T; t += RG) put4<T>(o + t * o_step, x, x, x, x);
+    for (int t = rg; t < a.T; t += RG) put4<T>(o + t * o_step, x, x, x, x);
   };
   // an idle request gives zeros; one whose slot does not exist, or that another request writes or reads, gives NaN; neither
   // touches the states
@@ -102,36 +102,37 @@ __global__ void __launch_bounds__(kRunThreads, ROWS > 128 ? 2 : 3) run_kernel(co
   if (from >= a.slots || to >= a.slots) return fill(NAN);
 
   F2 s[R][2];
-  const long long head = ((long long)a.H * from + h) * a.DK;
+  const long long step = (long long)RG * DV;
+  const float* src = a.s_in + (((long long)a.H * from + h) * DK + rg) * DV + col;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int r = i * RG + rg;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (a.s_in != nullptr && mine && r < a.DK) x = __ldcs(reinterpret_cast<const float4*>(a.s_in + (head + r) * a.DV + col));
+    if (a.s_in != nullptr && (SQUARE || i * RG + rg < DK)) x = __ldcs(reinterpret_cast<const float4*>(src));
+    src += step;
     s[i][0] = f2(x.x, x.y);
     s[i][1] = f2(x.z, x.w);
   }
   // (while the state is on its way) does another request read or write the slot that this one writes?
   bool hit = false;
   if (a.out != nullptr)
-    for (int j = threadIdx.x; j < a.B; j += kRunThreads)
+    for (int j = threadIdx.x; j < a.B; j += blockDim.x)
       if (j != b) {
         const int x = __ldg(a.in + j), y = __ldg(a.out + j);
         hit |= x >= 0 && y >= 0 && (x == to || y == to);  // (an idle request does neither)
       }
 
-  const float scale = rsqrtf((float)a.DK);
+  const float scale = rsqrtf((float)DK);
   for (int t0 = 0; t0 < a.T; t0 += kRun) {
     const int n = a.T - t0 < kRun ? a.T - t0 : kRun;
     if (t0 > 0) __syncthreads();  // the tokens before are read
-    for (int j = warp; j < n; j += kRunWarps) {
-      const long long row = (long long)b * a.T + t0 + j, key = (row * a.HK + hk) * a.DK + lane * 4;
+    for (int j = warp; j < n; j += warps) {
+      const long long row = (long long)b * a.T + t0 + j, key = (row * a.HK + hk) * DK + lane * 4;
       float q[kParts][4], k[kParts][4], kk = 0.f, qq = 0.f, qk = 0.f;
 #pragma unroll
       for (int x = 0; x < kParts; ++x) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[x][i] = k[x][i] = 0.f;
-        if (lane * 4 + 128 * x < a.DK) {
+        if (lane * 4 + 128 * x < DK) {
           Four<T>(static_cast<const T*>(a.q) + key + 128 * x).get(q[x]);
           Four<T>(static_cast<const T*>(a.k) + key + 128 * x).get(k[x]);
         }
@@ -160,11 +161,9 @@ __global__ void __launch_bounds__(kRunThreads, ROWS > 128 ? 2 : 3) run_kernel(co
         scalars[j][2] = qk * fk * fq;
       }
     }
-    const TV* const vp = static_cast<const TV*>(a.v) + (((long long)b * a.T + t0) * a.H + h) * a.DV + col;
-    Four<TV> v_next;
-    if (mine) v_next.load(vp);
+    const TV* const vp = static_cast<const TV*>(a.v) + (((long long)b * a.T + t0) * a.H + h) * DV + col;
+    Four<TV> v_next(vp);
     if (__syncthreads_or(hit)) return fill(NAN);
-    if (!mine) continue;
     for (int j = 0; j < n; ++j) {
       float v[4];
       v_next.get(v);
@@ -203,296 +202,161 @@ __global__ void __launch_bounds__(kRunThreads, ROWS > 128 ? 2 : 3) run_kernel(co
       const F2 d0 = f2(d[0], d[1]), d1 = f2(d[2], d[3]), e = f2(decay, decay);
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const F2 w = *reinterpret_cast<const F2*>(&kq[j][i * RG + rg]);
+        const F2 w = *reinterpret_cast<const volatile F2*>(&kq[j][i * RG + rg]);
         s[i][0] = fma2(w, d0, mul2(e, s[i][0]));
         s[i][1] = fma2(w, d1, mul2(e, s[i][1]));
       }
     }
   }
   if (a.T == 0 && __syncthreads_or(hit)) return;
-  if (a.s_out == nullptr || !mine) return;
-  float* const dst = a.s_out + (((long long)a.H * to + h) * a.DK + rg) * a.DV + col;
+  if (a.s_out == nullptr) return;
+  float* dst = a.s_out + (((long long)a.H * to + h) * DK + rg) * DV + col;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     float4 x;
     unf2(s[i][0], x.x, x.y);
     unf2(s[i][1], x.z, x.w);
-    if (i * RG + rg < a.DK) __stcs(reinterpret_cast<float4*>(dst + (long long)i * RG * a.DV), x);
+    if (SQUARE || i * RG + rg < DK) __stcs(reinterpret_cast<float4*>(dst), x);
+    dst += step;
   }
 }
 
-// ROWS: 64, 128 or 256, at least DK; COLS: columns of an item.
-template <int ROWS, int COLS>
-struct Cfg {
-  static constexpr int LC = COLS / 4, RG = 32 / LC, R = ROWS / RG;  // lanes across the columns, row groups, rows a lane has
-  static constexpr int kParts = (ROWS + 127) / 128;                 // of a row of q or k, 128 values each
-  static constexpr int kStage = ROWS * COLS * 4, kWarp = kStage + ROWS * 8;
-  static constexpr int kFit = 220 * 1024 / kWarp, kMost = R <= 16 ? 12 : 8, kWarps = kFit > kMost ? kMost : kFit;
-  static constexpr size_t kSmem = 128 + (size_t)kWarps * kWarp;
-};
-
-enum Kind { kLive, kIdle, kBad };
-struct Item {
-  int b, h, c0, from, to, kind;
-};
-
-template <typename T, typename TV, int ROWS, int COLS>
-__global__ void __launch_bounds__(32 * Cfg<ROWS, COLS>::kWarps, 1)
-    token_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
-  using C = Cfg<ROWS, COLS>;
-  constexpr int LC = C::LC, RG = C::RG, R = C::R, kWarps = C::kWarps;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[kWarps];
+template <typename T, typename TV, int ROWS, bool SQUARE>
+__global__ void __launch_bounds__(kThreads, kCtas) token_kernel(const Args a) {
+  constexpr int COLS = 2048 / ROWS, LC = COLS / 4, RG = 32 / LC, R = 16;
+  constexpr int kParts = (ROWS + 127) / 128;
+  __shared__ __align__(16) float2 kq[ROWS];                               // the token's k and q, normalised
+  const int DK = SQUARE ? ROWS : a.DK, DV = SQUARE ? ROWS : a.DV;
+  const int warps = SQUARE ? (ROWS / COLS < kWarps ? ROWS / COLS : kWarps) : blockDim.x >> 5;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cl = lane % LC, rg = lane / LC;
-  uint8_t* const own =
-      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127)) + warp * C::kWarp;
-  float4* const stage = reinterpret_cast<float4*>(own) + rg * LC + cl;  // the lane's first row
-  float2* const kq = reinterpret_cast<float2*>(own + C::kStage);        // a token's k and q, normalised
-  uint64_t* const bar = bars + warp;
-  if (lane == 0) {
-    mbar_init(bar, 1);
-    fence_mbar_init();
+  const int per = DV / (COLS * warps), b = blockIdx.y, h = blockIdx.x / per;
+  const int col = ((blockIdx.x - h * per) * warps + warp) * COLS + cl * 4;
+  const int from = a.in == nullptr ? b : __ldg(a.in + b), to = a.out == nullptr ? b : __ldg(a.out + b);
+  const long long row = (long long)b * a.H + h, step = (long long)RG * DV;
+  T* const o = static_cast<T*>(a.o) + row * DV + col;
+  // an idle request gives zeros; one whose slot does not exist, or that another request writes or reads, gives NaN
+  if (from < 0 || to < 0 || from >= a.slots || to >= a.slots) {
+    const float x = from < 0 || to < 0 ? 0.f : NAN;
+    if (rg == 0) put4<T>(o, x, x, x, x);
+    return;
   }
-  for (int i = lane; i < ROWS * COLS / 4; i += 32) reinterpret_cast<float4*>(own)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = lane; i < ROWS; i += 32) kq[i] = make_float2(0.f, 0.f);
-  __syncwarp();
-
-  const int slices = a.DV / COLS;
-  const long long items = (long long)a.B * a.H * slices;
-  // a CTA's items lie together and its warps take them in turn: neighbours read and write the same rows at about the same time
-  const long long end = items * (blockIdx.x + 1) / gridDim.x;
-  long long at = items * blockIdx.x / gridDim.x + warp;
-  if (at >= end) return;
-
-  int checked = -1, from = 0, to = 0, kind = kLive;  // the request whose slots these are
-  auto plan = [&](long long i) {
-    const long long r = i / slices;
-    Item it;
-    it.c0 = (int)(i - r * slices) * COLS;
-    it.b = (int)(r / a.H);
-    it.h = (int)(r - (long long)it.b * a.H);
-    if (it.b != checked) {
-      checked = it.b;
-      from = a.in == nullptr ? it.b : __ldg(a.in + it.b);
-      to = a.out == nullptr ? it.b : __ldg(a.out + it.b);
-      kind = from < 0 || to < 0 ? kIdle : from >= a.slots || to >= a.slots ? kBad : kLive;
-      if (kind == kLive && a.out != nullptr) {  // does another request read or write the slot that this one writes?
-        bool hit = false;
-        for (int j = lane; j < a.B; j += 32)
-          if (j != it.b) {
-            const int x = __ldg(a.in + j), y = __ldg(a.out + j);
-            hit |= x >= 0 && y >= 0 && (x == to || y == to);  // (an idle request does neither)
-          }
-        if (__any_sync(0xffffffffu, hit)) kind = kBad;
-      }
+  float4 s[R];
+  const float* src = a.s_in + (((long long)a.H * from + h) * DK + rg) * DV + col;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.s_in != nullptr && (SQUARE || i * RG + rg < DK)) s[i] = __ldcs(reinterpret_cast<const float4*>(src));
+    src += step;
+  }
+  // (while the state is on its way)
+  const long long key = ((long long)b * a.HK + h / (a.H / a.HK)) * DK + lane * 4;
+  float q[kParts][4], k[kParts][4], kk = 0.f, qq = 0.f, qk = 0.f;
+#pragma unroll
+  for (int x = 0; x < kParts; ++x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[x][i] = k[x][i] = 0.f;
+    if (lane * 4 + 128 * x < DK) {
+      Four<T>(static_cast<const T*>(a.q) + key + 128 * x).get(q[x]);
+      Four<T>(static_cast<const T*>(a.k) + key + 128 * x).get(k[x]);
     }
-    it.from = from, it.to = to, it.kind = kind;
-    return it;
-  };
-  const bool reads = a.s_in != nullptr, writes = a.s_out != nullptr;
-  auto fetch = [&](const Item& it) {  // when the stage is read
-    if (it.kind != kLive || !reads) return;
-    fence_async_smem();
-    __syncwarp();
-    if (lane != 0) return;
-    mbar_arrive_expect_tx(bar, a.DK * COLS * 4);
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-            smem_u32(own)),
-        "l"(reinterpret_cast<uint64_t>(&map)), "r"(it.c0), "r"(0), "r"(it.from * a.H + it.h), "r"(smem_u32(bar))
-        : "memory");
-  };
-  // the next item's rows: values of q and k a lane, v for the lane's columns
-  Four<T> q4[C::kParts], k4[C::kParts];
-  Four<TV> v4;
-  float g1 = 0.f, b1 = 0.f;
-  auto rows = [&](const Item& it) {
-    const long long row = it.b, key = (row * a.HK + it.h / (a.H / a.HK)) * a.DK + lane * 4;
 #pragma unroll
-    for (int j = 0; j < C::kParts; ++j)
-      if (lane * 4 + 128 * j < a.DK) {
-        q4[j].load(static_cast<const T*>(a.q) + key + 128 * j);
-        k4[j].load(static_cast<const T*>(a.k) + key + 128 * j);
-      }
-    v4.load(static_cast<const TV*>(a.v) + (row * a.H + it.h) * a.DV + it.c0 + cl * 4);
-    g1 = __ldg(a.g + row * a.H + it.h);
-    b1 = __ldg(a.beta + row * a.H + it.h);
-  };
-
-  const float scale = rsqrtf((float)a.DK);
-  uint32_t phase = 0;
-  Item next = plan(at);
-  fetch(next);
-  rows(next);
-  for (; at < end; at += kWarps) {
-    const Item it = next;
-    const bool more = at + kWarps < end;
-    if (more) next = plan(at + kWarps);
-    T* const o = static_cast<T*>(a.o) + ((long long)it.b * a.H + it.h) * a.DV + it.c0 + cl * 4;
-    if (it.kind != kLive) {
-      // an idle request gives zeros; one whose slot does not exist, or that another request writes or reads, gives NaN
-      const float x = it.kind == kIdle ? 0.f : NAN;
-      if (rg == 0) put4<T>(o, x, x, x, x);
-      if (more) fetch(next);
-      if (more) rows(next);
-    } else {
-      F2 s[R][2];
-#pragma unroll
-      for (int i = 0; i < R; ++i) s[i][0] = s[i][1] = f2(0.f, 0.f);
-      if (reads) {
-        const bool ok = mbar_wait(bar, phase, nullptr, 0);
-        phase ^= 1;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {  // (zeros past DK)
-          const float4 x = stage[i * RG * LC];
-          s[i][0] = f2(x.x, x.y);
-          s[i][1] = f2(x.z, x.w);
-        }
-        if (!ok) s[0][0] = s[0][1] = f2(NAN, NAN);  // a wait that gave up leaves NaN
-      }
-      if (more) fetch(next);
-      float q[C::kParts][4], k[C::kParts][4], v[4];
-      float kk = 0.f, qq = 0.f, qk = 0.f;
-#pragma unroll
-      for (int j = 0; j < C::kParts; ++j) {
-        q4[j].get(q[j]);
-        k4[j].get(k[j]);
-        const bool in = lane * 4 + 128 * j < a.DK;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          k[j][i] = in ? k[j][i] : 0.f;
-          q[j][i] = in ? q[j][i] : 0.f;
-          kk = fmaf(k[j][i], k[j][i], kk);
-          qq = fmaf(q[j][i], q[j][i], qq);
-          qk = fmaf(q[j][i], k[j][i], qk);
-        }
-      }
-      v4.get(v);
-      const float decay = expf(g1), beta = b1;
-      if (more) rows(next);
-      qk = warp_sum(qk);
-      float fk = 1.f, fq = scale;
-      if (a.l2norm) {
-        fk = rsqrtf(warp_sum(kk) + 1e-6f);
-        fq *= rsqrtf(warp_sum(qq) + 1e-6f);
-      }
-      __syncwarp();  // the rows of the item before are read
-#pragma unroll
-      for (int j = 0; j < C::kParts; ++j)
-        if (lane * 4 + 128 * j < a.DK) {
-#pragma unroll
-          for (int i = 0; i < 4; i += 2)
-            *reinterpret_cast<float4*>(kq + lane * 4 + 128 * j + i) =
-                make_float4(k[j][i] * fk, q[j][i] * fq, k[j][i + 1] * fk, q[j][i + 1] * fq);
-        }
-      __syncwarp();
-      F2 pk0 = f2(0.f, 0.f), pk1 = pk0, pq0 = pk0, pq1 = pk0;
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const float2 w = kq[i * RG + rg];
-        const F2 kx = f2(w.x, w.x), qx = f2(w.y, w.y);
-        pk0 = fma2(kx, s[i][0], pk0);
-        pk1 = fma2(kx, s[i][1], pk1);
-        pq0 = fma2(qx, s[i][0], pq0);
-        pq1 = fma2(qx, s[i][1], pq1);
-      }
-      float pk[4], pq[4];
-      unf2(pk0, pk[0], pk[1]);
-      unf2(pk1, pk[2], pk[3]);
-      unf2(pq0, pq[0], pq[1]);
-      unf2(pq1, pq[2], pq[3]);
-#pragma unroll
-      for (int m = LC; m < 32; m *= 2) {  // the row groups
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pk[i] += __shfl_xor_sync(0xffffffffu, pk[i], m);
-          pq[i] += __shfl_xor_sync(0xffffffffu, pq[i], m);
-        }
-      }
-      float d[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = beta * (v[i] - decay * pk[i]);
-      if (rg == 0) {
-        const float f = qk * fq * fk;
-        put4<T>(o, fmaf(f, d[0], decay * pq[0]), fmaf(f, d[1], decay * pq[1]), fmaf(f, d[2], decay * pq[2]),
-                fmaf(f, d[3], decay * pq[3]));
-      }
-      const F2 d0 = f2(d[0], d[1]), d1 = f2(d[2], d[3]), e = f2(decay, decay);
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const float w = kq[i * RG + rg].x;
-        const F2 kx = f2(w, w);
-        s[i][0] = fma2(kx, d0, mul2(e, s[i][0]));
-        s[i][1] = fma2(kx, d1, mul2(e, s[i][1]));
-      }
-      if (writes) {
-        float* const dst = a.s_out + (((long long)it.to * a.H + it.h) * a.DK + rg) * a.DV + it.c0 + cl * 4;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          float4 x;
-          unf2(s[i][0], x.x, x.y);
-          unf2(s[i][1], x.z, x.w);
-          if (i * RG + rg < a.DK) __stcs(reinterpret_cast<float4*>(dst + (long long)i * RG * a.DV), x);
-        }
-      }
+    for (int i = 0; i < 4; ++i) {
+      kk = fmaf(k[x][i], k[x][i], kk);
+      qq = fmaf(q[x][i], q[x][i], qq);
+      qk = fmaf(q[x][i], k[x][i], qk);
     }
+  }
+  const Four<TV> v4(static_cast<const TV*>(a.v) + row * DV + col);
+  const float decay = expf(__ldg(a.g + row)), beta = __ldg(a.beta + row);
+  qk = warp_sum(qk);
+  float fk = 1.f, fq = rsqrtf((float)DK);
+  if (a.l2norm) {
+    fk = rsqrtf(warp_sum(kk) + 1e-6f);
+    fq *= rsqrtf(warp_sum(qq) + 1e-6f);
+  }
+  // (all warps have the sums; each writes its share of the lanes)
+#pragma unroll
+  for (int x = 0; x < kParts; ++x)
+    if (lane % warps == warp && lane * 4 + 128 * x < ROWS) {
+#pragma unroll
+      for (int i = 0; i < 4; i += 2)
+        *reinterpret_cast<float4*>(kq + lane * 4 + 128 * x + i) =
+            make_float4(k[x][i] * fk, q[x][i] * fq, k[x][i + 1] * fk, q[x][i + 1] * fq);
+    }
+  bool hit = false;  // does another request read or write the slot that this one writes?
+  if (a.out != nullptr)
+    for (int j = threadIdx.x; j < a.B; j += blockDim.x)
+      if (j != b) {
+        const int x = __ldg(a.in + j), y = __ldg(a.out + j);
+        hit |= x >= 0 && y >= 0 && (x == to || y == to);  // (an idle request does neither)
+      }
+  if (__syncthreads_or(hit)) {
+    if (rg == 0) put4<T>(o, NAN, NAN, NAN, NAN);
+    return;
+  }
+  float pk[4] = {0.f, 0.f, 0.f, 0.f}, pq[4] = {0.f, 0.f, 0.f, 0.f}, v[4], d[4];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {  // (zeros past DK)
+    const float2 w = kq[i * RG + rg];
+    const float x[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      pk[c] = fmaf(w.x, x[c], pk[c]);
+      pq[c] = fmaf(w.y, x[c], pq[c]);
+    }
+  }
+#pragma unroll
+  for (int m = LC; m < 32; m *= 2) {  // the row groups
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pk[i] += __shfl_xor_sync(0xffffffffu, pk[i], m);
+      pq[i] += __shfl_xor_sync(0xffffffffu, pq[i], m);
+    }
+  }
+  v4.get(v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = beta * (v[i] - decay * pk[i]);
+  if (rg == 0) {
+    const float f = qk * fk * fq;
+    put4<T>(o, fmaf(f, d[0], decay * pq[0]), fmaf(f, d[1], decay * pq[1]), fmaf(f, d[2], decay * pq[2]),
+            fmaf(f, d[3], decay * pq[3]));
+  }
+  if (a.s_out == nullptr) return;
+  float* dst = a.s_out + (((long long)a.H * to + h) * DK + rg) * DV + col;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    // (read again: kept from above, the k of all rows would cost 16 registers, and a CTA an SM)
+    const float w = *const_cast<const volatile float*>(&kq[i * RG + rg].x);
+    if (SQUARE || i * RG + rg < DK)
+      __stcs(reinterpret_cast<float4*>(dst),
+             make_float4(fmaf(w, d[0], decay * s[i].x), fmaf(w, d[1], decay * s[i].y), fmaf(w, d[2], decay * s[i].z),
+                         fmaf(w, d[3], decay * s[i].w)));
+    dst += step;
   }
 }
 
-// [slots * H, DK, DV] float32 as boxes of `cols` columns x DK rows
-bool state_map(CUtensorMap* m, const Args& a, int cols) {
-  EncodeTiled enc = encode_tiled();
-  if (enc == nullptr) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)a.DV, (cuuint64_t)a.DK, (cuuint64_t)a.slots * a.H};
-  const cuuint64_t strides[2] = {(cuuint64_t)a.DV * 4, (cuuint64_t)a.DK * a.DV * 4};
-  const cuuint32_t box[3] = {(cuuint32_t)cols, (cuuint32_t)a.DK, 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(a.s_in), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <typename T, typename TV, int ROWS, int COLS>
-int launch_run(const Args& a, cudaStream_t stream) {
-  const int slices = (a.DV + kRunWarps * COLS - 1) / (kRunWarps * COLS);
-  run_kernel<T, TV, ROWS, COLS><<<dim3((unsigned)(a.H * slices), (unsigned)a.B), kRunThreads, 0, stream>>>(a);
-  return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
-}
-
-template <typename T, typename TV, int ROWS, int COLS>
-int launch_token(const Args& a, int sms, cudaStream_t stream) {
-  using C = Cfg<ROWS, COLS>;
-  CUtensorMap m = {};
-  if (a.s_in != nullptr && !state_map(&m, a, COLS)) return GD_ERR_LAUNCH;
-  static bool done[kMaxDevices];
-  auto kern = token_kernel<T, TV, ROWS, COLS>;
-  if (set_smem_once(kern, C::kSmem, done) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
-  const long long items = (long long)a.B * a.H * (a.DV / COLS);
-  kern<<<(unsigned)(items < sms ? items : sms), 32 * C::kWarps, C::kSmem, stream>>>(m, a);
+template <typename T, typename TV, int ROWS>
+int launch_rows(const Args& a, cudaStream_t stream) {
+  const int parts = a.DV * ROWS / 2048;  // a head's warps; its CTAs, all of one size
+  int ctas = (parts + kWarps - 1) / kWarps;
+  while (parts % ctas) ++ctas;
+  const dim3 grid((unsigned)(a.H * ctas), (unsigned)a.B);
+  const int threads = 32 * (parts / ctas);
+  const bool square = a.DK == ROWS && a.DV == ROWS;
+  if (a.T == 1)
+    square ? token_kernel<T, TV, ROWS, true><<<grid, threads, 0, stream>>>(a)
+           : token_kernel<T, TV, ROWS, false><<<grid, threads, 0, stream>>>(a);
+  else
+    square ? run_kernel<T, TV, ROWS, true><<<grid, threads, 0, stream>>>(a)
+           : run_kernel<T, TV, ROWS, false><<<grid, threads, 0, stream>>>(a);
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
 }
 
 template <typename T, typename TV>
 int launch(const Args& a, cudaStream_t stream) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return (cudaGetLastError(), GD_ERR_LAUNCH);
-  const long long heads = (long long)a.B * a.H;
-  if (a.T == 1 && heads > sms && a.slots > 0) {  // (up to as many heads run_kernel has work for every SM at once)
-    return a.DK <= 64    ? launch_token<T, TV, 64, 32>(a, sms, stream)
-           : a.DK <= 128 ? launch_token<T, TV, 128, 16>(a, sms, stream)
-                         : launch_token<T, TV, 256, 16>(a, sms, stream);
-  }
-  return a.DK > 128       ? launch_run<T, TV, 256, 16>(a, stream)
-         : a.DK <= 64     ? launch_run<T, TV, 64, 32>(a, stream)
-         : heads * 2 <= sms ? launch_run<T, TV, 128, 8>(a, stream)
-                          : launch_run<T, TV, 128, 16>(a, stream);
-}
-
-// Tensor maps are encoded by the driver, which wants the device's context bound to the calling thread.
-bool bind_context() {
-  int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+  return a.DK <= 64    ? launch_rows<T, TV, 64>(a, stream)
+         : a.DK <= 128 ? launch_rows<T, TV, 128>(a, stream)
+                       : launch_rows<T, TV, 256>(a, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -518,7 +382,6 @@ extern "C" int gd_rule_step(const void* q, const void* k, const void* v, const f
     return GD_ERR_ARG;
   for (const void* p : {q, k, v, (const void*)s_in, (const void*)s_out, (const void*)o})
     if (!aligned16(p)) return GD_ERR_ALIGN;
-  if (!bind_context()) return (cudaGetLastError(), GD_ERR_LAUNCH);
   Args a;
   a.q = q, a.k = k, a.v = v, a.g = g, a.beta = beta, a.s_in = s_in, a.s_out = s_out, a.in = slots, a.out = out_slots;
   a.o = o, a.B = B, a.T = T, a.H = H, a.HK = HK, a.DK = DK, a.DV = DV, a.slots = n_slots;

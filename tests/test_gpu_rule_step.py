@@ -256,3 +256,20 @@ def test_a_value_of_another_type():
         pool = s0.clone()
         c = gated_delta_step(q, k, v, g, beta, pool, use_qk_l2norm_in_kernel=True)
     assert torch.equal(a, c) and torch.equal(sa, pool)
+
+
+@pytest.mark.parametrize("HK,H,DK,DV", [(2, 4, 128, 128), (1, 3, 64, 96), (2, 2, 96, 160), (1, 2, 256, 64), (4, 8, 32, 32)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_same_bits_in_any_company(HK, H, DK, DV, dt):
+    """Tokens one at a time of one request at a time, and a run of all requests: the same bits."""
+    q, k, v, g, beta, s0 = _inputs(40, 11, HK, H, DK, DV, dt, seed=41)
+    o, state = recurrent_gated_delta_rule(q, k, v, g, beta, s0, True, True)
+    for b in (0, 7, 39):
+        pool = s0[b:b + 1].clone()
+        for t in range(11):
+            at = slice(b, b + 1), slice(t, t + 1)
+            assert torch.equal(gated_delta_step(q[at], k[at], v[at], g[at], beta[at], pool, use_qk_l2norm_in_kernel=True), o[at])
+        assert torch.equal(pool[0], state[b])
+    pool, at = s0.clone(), slice(0, 1)
+    assert torch.equal(gated_delta_step(q[:, at], k[:, at], v[:, at], g[:, at], beta[:, at], pool, use_qk_l2norm_in_kernel=True),
+                       o[:, at])
