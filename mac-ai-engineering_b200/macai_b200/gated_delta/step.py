@@ -5,8 +5,8 @@ and short runs over kept states, token after token, everything in float32:
 
 `gated_delta_step` works on a pool of states in place, as a server keeps it; `recurrent_gated_delta_rule` is the drop-in for
 transformers' torch_recurrent_gated_delta_rule (the reference's token-serial kernels, src/macai/gated_delta/_metal.py:37-77).
-A call reads and writes each state once, however many tokens it runs; long rows belong to `chunk_gated_delta_rule`. No
-gradient, and no CPU path: CUDA tensors only.
+A call reads and writes each state once, however many tokens it runs, and a token has the same bits alone, in a run, and in any
+batch; long rows belong to `chunk_gated_delta_rule`. No gradient, and no CPU path: CUDA tensors only.
 """
 from __future__ import annotations
 
