@@ -62,7 +62,7 @@ gemm::Cut cut_dx(long long n, int D, int F, int O) {
     return (long long)gemm::blocks_of(M, gemm::kTileM) * gemm::blocks_of(N, gemm::kTileN);
   };
   return gemm::cut_of(tiles(n, D), 2ll * gemm::blocks_of(F, gemm::kBlockK),
-                      (2 * tiles(F, D) + tiles(O, F)) * gemm::blocks_of(n, gemm::kBlockK), D);
+                      (2 * tiles(F, D) + tiles(O, F)) * gemm::length_of(gemm::blocks_of(n, gemm::kBlockK)), D);
 }
 size_t sum_bytes(const gemm::Cut& c, long long n, int D) {
   return gemm::cut_bytes(c, (long long)gemm::blocks_of(n, gemm::kTileM) * gemm::blocks_of(D, gemm::kTileN));

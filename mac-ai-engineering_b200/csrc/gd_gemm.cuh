@@ -44,6 +44,9 @@ constexpr int kThreads = 32 * (4 + kEpiWarps);
 constexpr int kMaxOps = 4;
 constexpr int kGroupM = 8;             // row tiles that are walked together, column tile after column tile (L2)
 constexpr float kLog2e = 1.4426950408889634f;
+// Stages whose time a tile's way out takes, where its contraction is shorter (64 rows, 2,048 wide, 128,000 words, both gradients'
+// products, one stage a tile of dW: 222 us; counted as 4 stages 251, 12 227, as it is 390)
+constexpr int kLeast = 8;
 
 enum Epilogue {
   kStore,    // C, times a factor, in 16 bits; or summed over calls in fp32 (see Op::sum)
@@ -278,9 +281,11 @@ __device__ __forceinline__ Walk Walk::of(const Params& p, int live, int pair, in
   w.mine = w.first > pair ? (w.first - pair + pairs - 1) / pairs : 0;
   w.behind = pairs - w.first % pairs, w.extra = 0;
   if (E == kStore && p.ops > 1 && w.behind < pairs) {
-    auto length = [&](const Op& o) { return o.slices > 1 ? o.per : first_segment(o, live) + o.kb[1]; };
-    const int next = length(p.op[1]);
-    if (next > 0) w.extra = length(p.op[0]) / next;
+    auto length = [&](const Op& o) {  // (a tile's way out takes as long as kLeast stages)
+      const int n = o.slices > 1 ? o.per : first_segment(o, live) + o.kb[1];
+      return n < kLeast ? kLeast : n;
+    };
+    w.extra = length(p.op[0]) / length(p.op[1]);
     if (w.extra > (w.tiles - w.first) / w.behind) w.extra = (w.tiles - w.first) / w.behind;
   }
   return w;
@@ -796,6 +801,7 @@ int sum_slices(const float* sum, const Op& o, int n, int D, const int* live, con
 struct Cut {
   int slices, per;
 };
+inline long long length_of(long long stages) { return stages < kLeast ? kLeast : stages; }  // as Walk counts them
 inline Cut cut_of(long long tiles, long long stages, long long rest, int D) {
   Cut c = {1, (int)stages};
   long long share = (tiles * stages + rest) / 74 / (rest > 0 ? 2 : 1);

@@ -286,7 +286,7 @@ BwdPlan bwd_plan(long long n, int D, int V) {
   b.cut = {1, 0};
   if (b.pieces == 1)
     b.cut = gemm::cut_of(tiles_m * tiles_n, gemm::blocks_of(V, gemm::kBlockK),
-                         gemm::blocks_of(V, gemm::kTileM) * tiles_n * kn, D);
+                         gemm::blocks_of(V, gemm::kTileM) * tiles_n * gemm::length_of(kn), D);
   b.scale = kHead;
   b.rows = b.scale + up((size_t)n * sizeof(float));
   b.dx = b.rows + up((size_t)n * pitch(D) * 2);
