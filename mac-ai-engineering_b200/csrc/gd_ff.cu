@@ -52,7 +52,7 @@ void shape(Op& op, long long M, long long N, int tile_n = gemm::kTileN) {
 }
 
 // Few tiles of y, or of dx beside the weights' gradients, have their contraction cut (gemm::cut_of; as if all gradients were asked
-// for, so that each has the same bits whichever are). 129 rows, 4,096 x 12,288: a call takes 101 us, uncut 116.
+// for, so that each has the same bits whichever are). 129 rows, 4,096 x 12,288: a call takes 88 us, uncut 116.
 gemm::Cut cut_y(long long n, int F, int O) {
   const long long tiles = (long long)gemm::blocks_of(n, gemm::kTileM) * gemm::blocks_of(O, gemm::kTileN);
   return gemm::cut_of(tiles, gemm::blocks_of(F, gemm::kBlockK), 0, O);

@@ -796,19 +796,31 @@ int sum_slices(const float* sum, const Op& o, int n, int D, const int* live, con
                                                  static_cast<T*>(out));
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
 }
-// How a contraction of `stages` for `tiles` tiles is cut where others of `rest` stages in all run beside it: a tile's length into
-// about half of a pair's share of the whole, at least 16 stages; 64 MiB of sums at most. {slices, stages of one}
+// How a contraction of `stages` for `tiles` tiles is cut, with 64 MiB of sums at most. {slices, stages of one} Where others
+// of `rest` stages in all run beside it: a tile's length into about half of a pair's share of the whole, 16 stages or more. Alone:
+// into what takes the fewest stages' times, the turns that 74 pairs take, each as long as a slice and its way out, and the joining.
+// (256 rows, 4,096 x 12,288, the block's second product: four slices, 64 tiles in one turn; five would be 80 in two.)
 struct Cut {
   int slices, per;
 };
 inline long long length_of(long long stages) { return stages < kLeast ? kLeast : stages; }  // as Walk counts them
 inline Cut cut_of(long long tiles, long long stages, long long rest, int D) {
   Cut c = {1, (int)stages};
-  long long share = (tiles * stages + rest) / 74 / (rest > 0 ? 2 : 1);
-  if (share < 16) share = 16;
-  if (stages <= share + share / 2 || blocks_of(D, 64) > 65535) return c;
-  c.slices = blocks_of(stages, (int)share);
+  if (blocks_of(D, 64) > 65535) return c;
   const long long room = (64ll << 20) / (tiles * kTileM * kTileN * 4);
+  if (rest == 0) {
+    long long least = (tiles + 73) / 74 * (stages + kLeast);
+    for (int s = 2; s <= room && s <= stages / 12; ++s) {
+      const int per = blocks_of(stages, s), slices = blocks_of(stages, per);
+      const long long time = (tiles * slices + 73) / 74 * (per + kLeast) + 10 + tiles * slices / 8;
+      if (time < least) least = time, c = {slices, per};
+    }
+    return c;
+  }
+  long long share = (tiles * stages + rest) / 74 / 2;
+  if (share < 16) share = 16;
+  if (stages <= share + share / 2) return c;
+  c.slices = blocks_of(stages, (int)share);
   if (c.slices > room) c.slices = room < 1 ? 1 : (int)room;
   c.per = blocks_of(stages, c.slices);
   c.slices = blocks_of(stages, c.per);
