@@ -89,6 +89,7 @@ struct Params {
   float* target;            // [M]: the label's logit
   const float2* lse;        // [M]: the row's maximum, log2 of its sum
   const float* row_scale;   // [M]
+  float log2e;              // log2(e), times what the logits are stretched by
   ErrorWord* err;
 };
 
@@ -717,8 +718,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           const float next = wattn::max3(top, high, high), ref = next == -INFINITY ? 0.f : next;
           float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 64; ++i) a[i & 3] += ex2((v[i] - ref) * kLog2e);  // (1 at the maximum)
-          sum = sum * ex2((top - ref) * kLog2e) + ((a[0] + a[1]) + (a[2] + a[3]));
+          for (int i = 0; i < 64; ++i) a[i & 3] += ex2((v[i] - ref) * p.log2e);  // (1 at the maximum)
+          sum = sum * ex2((top - ref) * p.log2e) + ((a[0] + a[1]) + (a[2] + a[3]));
           top = next;
         }
         if (row < rows && w.n + half * 128 < op.N)
@@ -736,7 +737,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           if (s == 1) release();
           if (!has(n0)) continue;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) v[i] = ex2(fmaf(v[i] - lse.x, kLog2e, -lse.y));
+          for (int i = 0; i < 64; ++i) v[i] = ex2(fmaf(v[i] - lse.x, p.log2e, -lse.y));
           if (__any_sync(0xffffffffu, at >= n0 && at < n0 + 64)) {
 #pragma unroll
             for (int i = 0; i < 64; ++i) v[i] -= at == n0 + i ? 1.f : 0.f;

@@ -3,10 +3,10 @@ libgated_delta_b200.so):
 
     loss_i = logsumexp_v(x_i . w_v) - x_i . w_label(i)
 
-tcgen05 products of 16-bit operands with float32 sums; the logits leave the tensor core as float32 and stay on the chip: the
-forward keeps a maximum and a sum of exponentials for every 128 of them, the backward forms them again, a piece of the
-vocabulary at a time, and rounds their gradient to the inputs' 16-bit type (the matrix instruction's operand). bfloat16 and
-float16. There is no CPU path: CUDA tensors only.
+tcgen05 products of 16-bit operands with float32 sums (the mean of what the tensor core's adder cuts off is put back); the
+logits leave the tensor core as float32 and stay on the chip: the forward keeps a maximum and a sum of exponentials for every 128
+of them, the backward forms them again, a piece of the vocabulary at a time, and rounds their gradient to the inputs' 16-bit type
+(the matrix instruction's operand). bfloat16 and float16. There is no CPU path: CUDA tensors only.
 """
 from __future__ import annotations
 

@@ -320,3 +320,23 @@ def test_a_tied_weight():
     want = dw.double() + torch.autograd.grad(e[tokens], e, dx)[0].double()
     # one rounding of the sum of two gradients in bf16
     assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-30).all())
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+@pytest.mark.parametrize("D", [512, 2048, 4096])
+def test_the_adders_cut_is_taken_back(D, dt):
+    """Losses of long sums are not shifted towards the smaller logits. A sum of D products in fp32 whose D / 16 steps are each cut
+    by up to 2^-23 of it would be off by up to D / 16 x 2^-23 of a logit, always towards zero; half of that is the mean of such
+    cuts. What is left on average is held to a fifth of it (the logits' own size: the difference of the label's and the mean one)."""
+    n, V = 600, 1500
+    gen = torch.Generator().manual_seed(D)
+    w = (torch.randn(V, D, generator=gen) * 1.5 * D ** -0.5).to(dt)
+    lab = torch.randint(0, V, (n,), generator=gen)
+    x = (torch.randn(n, D, generator=gen) + 4 * torch.rand(n, 1, generator=gen) * w[lab].float()).to(dt)
+    x, w, lab = x.cuda(), w.cuda(), lab.cuda()
+    loss = linear_cross_entropy(x, w, lab, reduction="none").double()
+    logits = x.double() @ w.double().t()
+    at = logits.gather(1, lab[:, None])[:, 0]
+    size = at - (logits.softmax(1) * logits).sum(1)
+    off = loss - (logits.logsumexp(1) - at)
+    assert abs(float((off * size).sum() / (size * size).sum())) <= D / 16 * 2.0 ** -24 / 5
