@@ -464,9 +464,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     }
     // The copies in flight land before the CTAs end, whatever became of their readers (they are counted on the first CTA's
     // barriers; the pair ends together).
+    const int left = issued > C::kStages ? issued - C::kStages : 0;
     if (rank == 0)
-      for (int i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
-        warp_wait(full + i % C::kStages, (i / C::kStages) & 1, p.err, 81);
+      for (int i = left; i < issued; ++i) warp_wait(full + i % C::kStages, (i / C::kStages) & 1, p.err, 81);
+    // So do the arrivals of the last products, which the first CTA's tensor core sends to both: a CTA that ended before them would
+    // be written to when its shared memory is another's.
+    for (int i = left; ok && i < issued; ++i) ok = warp_wait(empty + i % C::kStages, (i / C::kStages) & 1, p.err, 87);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t lead = elect();
@@ -512,8 +515,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         if (ok) commit_pair(lead, acc_full + buf);
       }
       commit_pair(lead, fin);  // (a pair whose waits gave up ends with no product in flight)
-      warp_wait(fin, 0, p.err, 84);
     }
+    warp_wait(fin, 0, p.err, 84);  // (both: it arrives in both, also where the pair has no tile and nothing else to wait for)
   } else if (warp >= 4) {
     const int ew = warp - 4, quad = warp & 3, half = ew >> 2;  // a warp reads the TMEM lanes of its quarter
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
