@@ -72,10 +72,14 @@ class DeltaMixer(nn.Module):
         return self.close(o, x)
 
     def prefill(self, x):
-        """The output and what single tokens go on from: the convolution's last three inputs and the states."""
+        """The output and what single tokens go on from: the convolution's last three inputs (zeros where the prompt has fewer,
+        as the convolution has before a row's first token) and the states."""
         qkv = self.qkv(x)
         o, state = chunk_gated_delta_rule(*self.rows(qkv, x), output_final_state=True, use_qk_l2norm_in_kernel=True)
-        return self.close(o, x), qkv[:, -3:].clone(), state
+        before = qkv.new_zeros(qkv.shape[0], 3, qkv.shape[2])
+        n = min(3, qkv.shape[1])
+        before[:, 3 - n:] = qkv[:, qkv.shape[1] - n:]
+        return self.close(o, x), before, state
 
     def step(self, x, before, state):
         """One token a request: x [B, 1, DIM]; carries on `before` and the states in place."""
