@@ -65,7 +65,8 @@ extern "C" {
  * signals, with a ~1 ms budget. The wait expires, the kernel records GD_ERR_TIMEOUT at stage 28 in the error word,
  * every role of the CTA gives up in its own bounded wait (~2 s) with no product or copy left in flight, and the CTA
  * frees its TMEM and returns: gd_read_error then reports (GD_ERR_TIMEOUT, 28), and the context stays usable. The
- * high-level entry points (gd_forward, gd_backward, ...) do not pass it on. */
+ * high-level entry points (gd_forward, gd_backward, ...) do not pass it on.
+ * Added to gd_ff_fwd's dtype (with `kept`): its first product's waits end as ever and then count as given up (stage 85). */
 #define GD_TEST_WAIT_EXPIRES 0x40000000
 
 /* Text for a status code. */

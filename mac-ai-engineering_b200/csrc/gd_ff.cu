@@ -69,12 +69,12 @@ size_t sum_bytes(const gemm::Cut& c, long long n, int D) {
 }
 
 template <typename T>
-int forward(const Problem& q, void* const* kept, void* h, float* sum, void* y, uint32_t* bounds, ErrorWord* err,
+int forward(const Problem& q, void* const* kept, void* h, float* sum, void* y, uint32_t* bounds, ErrorWord* err, bool expire,
             cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const long long n = q.rows;
   Params p = {};
-  p.ops = 1, p.err = err, p.keep = kept[0] != nullptr, p.bounds = bounds;
+  p.ops = 1, p.err = err, p.keep = kept[0] != nullptr, p.bounds = bounds, p.expire = expire ? 85 : 0;
   Op& o = p.op[0];
   shape(o, n, q.F, gemm::kHalf);
   o.kb[0] = gemm::blocks_of(q.D, gemm::kBlockK);
@@ -205,6 +205,9 @@ extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, co
                          unsigned int* bounds, void* y, int dtype, long long rows, int D, int F, int O, const long long* ld,
                          void* workspace, size_t workspace_bytes, void* stream) {
   using namespace gd::ff;
+  const bool expire = dtype & GD_TEST_WAIT_EXPIRES;
+  dtype &= ~GD_TEST_WAIT_EXPIRES;
+  if (expire && kept == nullptr) return GD_ERR_ARG;
   if (const int st = check(dtype, rows, D, F, O, ld, 4)) return st;
   if (rows == 0) return GD_OK;
   if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr || y == nullptr ||
@@ -225,8 +228,8 @@ extern "C" int gd_ff_fwd(const void* x, const void* w_gate, const void* w_up, co
   float* const sum = reinterpret_cast<float*>(static_cast<char*>(h) + matrix_bytes(rows, F));
   void* planes[3];
   for (int i = 0; i < 3; ++i) planes[i] = kept == nullptr ? nullptr : static_cast<char*>(kept) + i * (size_t)rows * pitch(F) * 2;
-  return dtype == GD_FLOAT16 ? forward<__half>(q, planes, h, sum, y, bounds, err, cs)
-                             : forward<__nv_bfloat16>(q, planes, h, sum, y, nullptr, err, cs);
+  return dtype == GD_FLOAT16 ? forward<__half>(q, planes, h, sum, y, bounds, err, expire, cs)
+                             : forward<__nv_bfloat16>(q, planes, h, sum, y, nullptr, err, expire, cs);
 }
 
 extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* kept,

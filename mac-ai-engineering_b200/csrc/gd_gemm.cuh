@@ -91,6 +91,7 @@ struct Params {
   const float* row_scale;   // [M]
   float log2e;              // log2(e), times what the logits are stretched by
   ErrorWord* err;
+  int expire;               // (tests) the epilogue's wait that counts as given up
 };
 
 template <int E>
@@ -168,6 +169,12 @@ __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, Err
     }
   }
   return __all_sync(0xffffffffu, ok);
+}
+// (tests) Whether the wait `where`, though it ended well, counts as given up.
+__device__ __forceinline__ bool expires(const Params& p, int where) {
+  if (p.expire != where) return false;
+  report(p.err, GD_ERR_TIMEOUT, where);
+  return true;
 }
 // A box into this CTA's shared memory, counted on a barrier of the pair's first CTA.
 __device__ __forceinline__ void load_pair(uint32_t lead, uint32_t dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
@@ -547,7 +554,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       const uint32_t t0 = tm + lanes + buf * kTileN;
       const int rows = op.m_live ? live : op.M;  // (kDLogit: zeros in the rows past them)
       auto has = [&](int n0) { return m0 < (E == kDLogit ? op.M : rows) && n0 < op.N; };
-      ok = ok && warp_wait(acc_full + buf, (it >> 1) & 1, p.err, 85);
+      ok = ok && warp_wait(acc_full + buf, (it >> 1) & 1, p.err, 85) && !expires(p, 85);
       tc_fence_after();
       const float bad = ok ? 0.f : NAN;  // a wait that gave up leaves NaN
       auto release = [&] {               // the accumulator is read
@@ -601,10 +608,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           tmem_ld32(t0 + kHalf + c, u);
           if (s == 1) release();
           if (!has(n0)) continue;
+          if (!ok) {  // (NaN in what is kept, too)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) g[i] = u[i] = NAN;
+          }
           uint32_t h[16], gh[16], uh[16], low[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            h[i / 2] = pack16<T>(g[i] * sigmoid(g[i]) * u[i] + bad, g[i + 1] * sigmoid(g[i + 1]) * u[i + 1] + bad);
+            h[i / 2] = pack16<T>(g[i] * sigmoid(g[i]) * u[i], g[i + 1] * sigmoid(g[i + 1]) * u[i + 1]);
             gh[i / 2] = upper_halves(g[i], g[i + 1]);
             uh[i / 2] = upper_halves(u[i], u[i + 1]);
             low[i / 2] = next_bytes(g[i], u[i], g[i + 1], u[i + 1]);
