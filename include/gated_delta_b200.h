@@ -66,7 +66,8 @@ extern "C" {
  * every role of the CTA gives up in its own bounded wait (~2 s) with no product or copy left in flight, and the CTA
  * frees its TMEM and returns: gd_read_error then reports (GD_ERR_TIMEOUT, 28), and the context stays usable. The
  * high-level entry points (gd_forward, gd_backward, ...) do not pass it on.
- * Added to gd_ff_fwd's dtype (with `kept`): its first product's waits end as ever and then count as given up (stage 85). */
+ * Added to gd_ff_fwd's dtype (with `kept`): its first product's waits end as ever and then count as given up (stage 85);
+ * to gd_ff_bwd's: the first product's waits for what is kept do (stage 86). */
 #define GD_TEST_WAIT_EXPIRES 0x40000000
 
 /* Text for a status code. */

@@ -104,7 +104,7 @@ struct Grads {
 
 template <typename T>
 int backward(const Problem& q, const void* const* kept, const void* dy, long long ldy, const Grads& out, void* dg, void* du,
-             void* h, float* sum, const uint32_t* bounds, uint32_t* own, ErrorWord* err, cudaStream_t stream) {
+             void* h, float* sum, const uint32_t* bounds, uint32_t* own, ErrorWord* err, bool expire, cudaStream_t stream) {
   constexpr CUtensorMapDataType dt = map_dtype<T>();
   const long long n = q.rows, lf = pitch(q.F);
   if (bounds != nullptr) {
@@ -115,6 +115,7 @@ int backward(const Problem& q, const void* const* kept, const void* dy, long lon
   }
   Params p = {};
   p.ops = 1, p.err = err, p.keep = out.dwd != nullptr, p.bounds = const_cast<uint32_t*>(bounds), p.more = own;
+  p.expire = expire ? 86 : 0;
   Op& o = p.op[0];
   shape(o, n, q.F);  // dh = dy Wd
   o.kb[0] = gemm::blocks_of(q.O, gemm::kBlockK);
@@ -237,6 +238,8 @@ extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, co
                          int dtype, long long rows, int D, int F, int O, const long long* ld, void* workspace,
                          size_t workspace_bytes, void* stream) {
   using namespace gd::ff;
+  const bool expire = dtype & GD_TEST_WAIT_EXPIRES;
+  dtype &= ~GD_TEST_WAIT_EXPIRES;
   if (const int st = check(dtype, rows, D, F, O, ld, 5)) return st;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   if (rows == 0) {
@@ -266,6 +269,7 @@ extern "C" int gd_ff_bwd(const void* x, const void* w_gate, const void* w_up, co
   float* const sum = reinterpret_cast<float*>(at + kHead + 3 * m);
   const void* planes[3];
   for (int i = 0; i < 3; ++i) planes[i] = static_cast<const char*>(kept) + i * (size_t)rows * pitch(F) * 2;
-  return dtype == GD_FLOAT16 ? backward<__half>(q, planes, dy, ld[4], out, dg, du, h, sum, bounds, own, err, cs)
-                             : backward<__nv_bfloat16>(q, planes, dy, ld[4], out, dg, du, h, sum, nullptr, nullptr, err, cs);
+  return dtype == GD_FLOAT16
+             ? backward<__half>(q, planes, dy, ld[4], out, dg, du, h, sum, bounds, own, err, expire, cs)
+             : backward<__nv_bfloat16>(q, planes, dy, ld[4], out, dg, du, h, sum, nullptr, nullptr, err, expire, cs);
 }

@@ -545,8 +545,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         for (int i = 0; i < 3; ++i) load_slab(to + i * kStrip, &p.x[i], n0, m0, aux + 2 * ew + (at & 1));
       }
     };
+    auto send_strips = [&](const Op& op, uint32_t strips, int n0, int m0) {  // dg, du and h
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        store_slab(&op.c, n0, m0, strips);
+        store_slab(&p.y[0], n0, m0, strips + kStrip);
+        if (p.keep) store_slab(&p.y[1], n0, m0, strips + 2 * kStrip);
+        bulk_commit();
+      }
+    };
     if (E == kDSwiglu && walk(0) >= 0) fetch(0, locate<E>(p, walk(0), live));
     uint32_t landed = 0;  // kDSwiglu: the phase of each set's barrier (a step past the matrix loads nothing)
+    int late = -1;        // kDSwiglu: the set whose wait gave up: what it waited for may still come, so the other set sends NaN
     for (int tile; (tile = walk(it)) >= 0; ++it) {
       const Where w = locate<E>(p, tile, live);
       const Op& op = p.op[w.op];
@@ -654,7 +665,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           }
         }
       } else if constexpr (E == kDSwiglu) {
-        float f = carried(p.bounds, p.more) + bad;
+        const float f = carried(p.bounds, p.more) + bad;
 #pragma unroll 1
         for (int s = 0; s < 4; ++s, ++step) {
           const int c = half * 128 + s * 32, n0 = w.n + c, set = step & 1;
@@ -662,13 +673,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           tmem_ld32(t0 + c, d);
           if (s == 3) release();
           const bool here = has(n0);
-          if (here) {
-            if (!warp_wait(aux + 2 * ew + set, (landed >> set) & 1, p.err, 86)) f = NAN;
-            landed ^= 1u << set;
+          if (here && late < 0) {
+            if (warp_wait(aux + 2 * ew + set, (landed >> set) & 1, p.err, 86) && !expires(p, 86)) landed ^= 1u << set;
+            else late = set;
           }
-          if (s < 3) fetch(step + 1, w);
-          else if (walk(it + 1) >= 0) fetch(step + 1, locate<E>(p, walk(it + 1), live));
+          if (late < 0) {
+            if (s < 3) fetch(step + 1, w);
+            else if (walk(it + 1) >= 0) fetch(step + 1, locate<E>(p, walk(it + 1), live));
+          }
           if (!here) continue;
+          if (late >= 0) {  // NaN from here on (0x7fff in both types), nothing more is loaded
+            const uint32_t nan[4] = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+            const uint32_t strips = slab + (late ^ 1) * 3 * kStrip;
+            if (lane == 0) bulk_wait_read0();
+            __syncwarp();
+#pragma unroll 1
+            for (int i = 0; i < 12; ++i) st_shared16(strips + (i / 4) * kStrip + strip_at(lane, i & 3), nan);
+            send_strips(op, strips, n0, m0);
+            continue;
+          }
           const uint32_t strips = slab + set * 3 * kStrip;
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {  // a chunk of 8 columns of the thread's row, in place
@@ -691,14 +714,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
             st_shared16(at + kStrip, u);
             st_shared16(at + 2 * kStrip, h);
           }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            store_slab(&op.c, n0, m0, strips);
-            store_slab(&p.y[0], n0, m0, strips + kStrip);
-            if (p.keep) store_slab(&p.y[1], n0, m0, strips + 2 * kStrip);
-            bulk_commit();
-          }
+          send_strips(op, strips, n0, m0);
         }
       } else if constexpr (E == kLse) {
         const int lab = row < rows ? __ldg(p.labels + row) : -1;
@@ -766,6 +782,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         }
       }
     }
+    if (late >= 0) warp_wait(aux + 2 * ew + late, (landed >> late) & 1, p.err, 86);  // its copies land before the CTA ends
     if (lane == 0) bulk_wait_read0();
   }
   tc_fence_before();

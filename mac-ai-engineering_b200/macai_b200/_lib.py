@@ -23,7 +23,7 @@ def GD_KEY_WIDTH(dk: int) -> int:
 
 
 GD_WIDE_STATE_PASS = 16  # gd_fwd_state: always two CTAs per (head, row) (the default picks four when they fit)
-GD_TEST_WAIT_EXPIRES = 0x40000000  # test only: a wait of gd_fwd_state's or gd_ff_fwd's expires (the failure path's tests)
+GD_TEST_WAIT_EXPIRES = 0x40000000  # test only: a wait of gd_fwd_state, gd_ff_fwd or gd_ff_bwd expires (the failure path's tests)
 
 # every entry point declared in include/gated_delta_b200.h
 EXPORTS = ("gd_status_string", "gd_workspace_bytes", "gd_prep", "gd_fwd_state", "gd_bwd_state", "gd_bwd_chunk",

@@ -44,15 +44,15 @@ def _forward(x, wg, wu, wd, extra=0):
     return y, kept, bounds, _error(ws)
 
 
-def _backward(x, wg, wu, wd, dy, kept, bounds, extra=0):
+def _backward(x, wg, wu, wd, dy, kept, bounds, extra=0, need=(0, 1, 2, 3)):
     lib, half = _lib.load(), x.dtype == torch.float16
-    out = [torch.zeros_like(t) for t in (x, wg, wu, wd)]
+    out = [torch.zeros_like(t) if i in need else None for i, t in enumerate((x, wg, wu, wd))]
     n = lib.gd_ff_workspace_bytes(N, D, F, O, 1)
     ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
     ld = (ctypes.c_longlong * 5)(D, D, D, F, O)
     _lib.check(lib.gd_ff_bwd(_at(x), _at(wg), _at(wu), _at(wd), _at(kept), _at(bounds), _at(dy), *(_at(t) for t in out),
                              (_lib.GD_FLOAT16 if half else _lib.GD_BFLOAT16) | extra, N, D, F, O, ld, _at(ws), n, _stream()), "gd_ff_bwd")
-    return out, _error(ws)
+    return [t for t in out if t is not None], _error(ws)
 
 
 def _planes(kept):
@@ -79,3 +79,17 @@ def test_forward(dt):
     assert error[0] == _lib.GD_OK and all(bool(t.isnan().all()) for t in grads)
     again = _forward(x, wg, wu, wd)
     assert again[3][0] == _lib.GD_OK and all(torch.equal(a, b) for a, b in zip(again[:2], clean[:2]))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("need", [(0, 1, 2, 3), (3,), (0,)])
+def test_backward(dt, need):
+    """A backward that could not wait for what was kept: no gradient is made of numbers that did not arrive."""
+    x, wg, wu, wd, dy = _block(dt, seed=1)
+    _, kept, bounds, _ = _forward(x, wg, wu, wd)
+    clean, error = _backward(x, wg, wu, wd, dy, kept, bounds, need=need)
+    assert error[0] == _lib.GD_OK and all(bool(t.isfinite().all()) for t in clean)
+    grads, error = _backward(x, wg, wu, wd, dy, kept, bounds, _lib.GD_TEST_WAIT_EXPIRES, need)
+    assert error == (_lib.GD_ERR_TIMEOUT, 86) and all(bool(t.isnan().all()) for t in grads)
+    again, error = _backward(x, wg, wu, wd, dy, kept, bounds, need=need)
+    assert error[0] == _lib.GD_OK and all(torch.equal(a, b) for a, b in zip(again, clean))
