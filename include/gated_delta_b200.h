@@ -349,7 +349,8 @@ int gd_wattn_step(const void* q, const void* k, const void* v, void* k_cache, vo
  * zeros) and leaves its state in s_out's slot out_slots[b] (s_out NULL: nowhere); slots and out_slots, int32 [B] on the device,
  * are both given or both NULL (slot b, n_slots >= B). s_in and s_out may be one pool. Other slots are neither read nor written.
  * A negative slot marks an idle request: its o is zeros. A request with a slot >= n_slots, or whose written slot another
- * request of the call reads or writes, gets o = NaN. Neither of them changes a state. DK, DV: multiples of 32 up to 256.
+ * request of the call reads or writes (idle ones and those without a slot do neither), gets o = NaN. Neither of them changes a
+ * state. DK, DV: multiples of 32 up to 256.
  * q, k, v, o and the states 16-byte aligned. No allocation, no atomics, asynchronous on `stream`.
  * Replaces: the token-serial kernels gdr_fwd* (src/macai/gated_delta/_metal.py:37-77, :202-243) for decoding, with the
  * arguments of transformers' torch_recurrent_gated_delta_rule. */

@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) run_kernel(const Args a) {
     for (int j = threadIdx.x; j < a.B; j += blockDim.x)
       if (j != b) {
         const int x = __ldg(a.in + j), y = __ldg(a.out + j);
-        hit |= x >= 0 && y >= 0 && (x == to || y == to);  // (an idle request does neither)
+        // (an idle request does neither, nor does one whose slot does not exist)
+        hit |= (unsigned)x < (unsigned)a.slots && (unsigned)y < (unsigned)a.slots && (x == to || y == to);
       }
 
   const float scale = rsqrtf((float)DK);
@@ -288,7 +289,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_kernel(const Args a) {
     for (int j = threadIdx.x; j < a.B; j += blockDim.x)
       if (j != b) {
         const int x = __ldg(a.in + j), y = __ldg(a.out + j);
-        hit |= x >= 0 && y >= 0 && (x == to || y == to);  // (an idle request does neither)
+        // (an idle request does neither, nor does one whose slot does not exist)
+        hit |= (unsigned)x < (unsigned)a.slots && (unsigned)y < (unsigned)a.slots && (x == to || y == to);
       }
   if (__syncthreads_or(hit)) {
     if (rg == 0) put4<T>(o, NAN, NAN, NAN, NAN);

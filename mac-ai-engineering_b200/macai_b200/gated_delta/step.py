@@ -86,7 +86,8 @@ def gated_delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     slots (int32 [B] on the device, default: request b has slot b): the slot whose state each request starts from, and,
     unless out_slots names others, the one that it leaves its state in. out_slots lets the state before the tokens stay,
     as drafted tokens need. A negative slot marks an idle request: its output is zeros. A request whose slot the pool does
-    not have, or whose written slot another request of the call reads or writes, gets NaN. Neither of them changes a state.
+    not have, or whose written slot another request of the call reads or writes, gets NaN. Neither of them changes a state;
+    idle requests and those without a slot contest none.
     No gradient. Nothing waits for the host."""
     name = "gated_delta_step"
     q, k, v, g_, beta_, B, T, H, HK, DK, DV = _inputs(name, query, key, value, g, beta)
