@@ -118,12 +118,12 @@ def gated_delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
 
 
 def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, output_final_state: bool = False,
-                               use_qk_l2norm_in_kernel: bool = False, **kwargs):
+                               use_qk_l2norm_in_kernel: bool = False, cu_seqlens=None):
     """Drop-in for transformers' torch_recurrent_gated_delta_rule: arguments as `chunk_gated_delta_rule`'s, any of the three
     float types; returns the output [B, T, H, DV] in the query's dtype and the final state (float32, a new tensor) when
-    output_final_state, else None. No gradient."""
+    output_final_state, else None. cu_seqlens only None. No gradient."""
     name = "recurrent_gated_delta_rule"
-    if kwargs.get("cu_seqlens") is not None:
+    if cu_seqlens is not None:
         raise NotImplementedError(f"{name}: packed rows run through chunk_gated_delta_rule")
     q, k, v, g_, beta_, B, T, H, HK, DK, DV = _inputs(name, query, key, value, g, beta)
     if recorded(query, key, value, g, beta, initial_state):
