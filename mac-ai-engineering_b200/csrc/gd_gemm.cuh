@@ -47,6 +47,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Stages whose time a tile's way out takes, where its contraction is shorter (64 rows, 2,048 wide, 128,000 words, both gradients'
 // products, one stage a tile of dW: 222 us; counted as 4 stages 251, 12 227, as it is 390)
 constexpr int kLeast = 8;
+constexpr int kRun = 12;  // stages of a logit's run, at most (see sums_in_runs)
 
 enum Epilogue {
   kStore,    // C, times a factor, in 16 bits; or summed over calls in fp32 (see Op::sum)
@@ -55,6 +56,23 @@ enum Epilogue {
   kLse,      // each row's maximum and sum of exponentials over the tile's columns, and its label's logit
   kDLogit    // (softmax - onehot) times the row's factor, in 16 bits
 };
+
+// The tensor core's adder cuts off what lies below its accumulator, always towards zero: a sum of D products in one go loses about
+// a quarter of D / 16 x 2^-24 to 2^-23 of itself (2e-6 at 2,048 terms; twice that and more where all terms have one sign). Logits are
+// therefore summed in runs of at most 768 terms (two runs at least, from two stages on), a run an accumulator, and the runs added
+// in float32 registers by the epilogue's threads, which hold their 128 columns: what is lost does not grow with D. Losses of 777
+// rows, 5,000 words, bf16, are off by 3.4e-7 of their norm at D = 2,048 (a float32 product's: 3.4e-7), 3.5e-7 at 8,192 (7.5e-7); with
+// one sign 3.5e-7 (3.2e-6) and 7.3e-7 (1.4e-5). Reading an accumulator takes about 2,000 clocks beside the products, which two
+// accumulators hide where a run is long enough: 777 rows, 2,048 wide, 50,257 words take 149.6 us, in one go 147.9, in runs of 512
+// terms 156 (2.5e-7), of 256 terms 185 (1.2e-7). 1,500 rows of 768 (two runs of six stages): the logits' kernels 5 to 8 % more.
+// 128 sums a thread want more registers than twelve warps share evenly: the first four warps give some away.
+constexpr bool sums_in_runs(int E) { return E == kLse || E == kDLogit; }
+constexpr int kFewRegs = 80, kManyRegs = 208;
+__host__ __device__ inline int run_stages(int stages) {  // of every run but the last
+  int runs = (stages + kRun - 1) / kRun;
+  if (runs < 2) runs = 2;
+  return (stages + runs - 1) / runs;
+}
 
 // One product. a[s], b[s]: the operands of contraction segment s (kSwiglu: b[0] gate, b[1] up, one segment).
 struct Op {
@@ -89,7 +107,6 @@ struct Params {
   float* target;            // [M]: the label's logit
   const float2* lse;        // [M]: the row's maximum, log2 of its sum
   const float* row_scale;   // [M]
-  float log2e;              // log2(e), times what the logits are stretched by
   ErrorWord* err;
   int expire;               // (tests) the epilogue's wait that counts as given up
 };
@@ -410,99 +427,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   tc_fence_after();
   const uint32_t tm = __shfl_sync(0xffffffffu, *tslot, 0);
   const uint32_t s_base = smem_u32(base);
-
-  if (warp == 0) {
-    // The whole warp runs this, one elected lane's instructions take effect: addresses and coordinates stay in uniform registers.
-    // (Issued from a branch of one lane, a stage's loads took longer than its products where a launch holds several problems:
-    // 1,215 instead of 1,540 TFLOP/s.)
-    const uint32_t lead = elect();
-    int slot = 0, laps = 0, issued = 0;
-    bool ok = true;
-    for (int i = 0, tile; ok && (tile = walk(i)) >= 0; ++i) {
-      Where w = locate<E>(p, tile, live);
-      w.op = __shfl_sync(0xffffffffu, w.op, 0);
-      const Op& op = p.op[w.op];
-      const int am = __shfl_sync(0xffffffffu, w.m + (int)rank * kHalf, 0);
-      const int bn = __shfl_sync(0xffffffffu, E == kSwiglu ? w.n : w.n + (int)rank * kHalf, 0);
-      auto segment = [&](auto a_mn, auto b_mn, const CUtensorMap* ma, const CUtensorMap* mb, int from, int n) {
-        for (int kb = from; kb < from + n; ++kb) {
-          if (laps > 0 && !(ok = warp_wait(empty + slot, (laps - 1) & 1, p.err, 80))) return;
-          if (rank == 0 && lead) mbar_arrive_expect_tx(full + slot, 2 * kStage);
-          const uint32_t bar = in_first_cta(full + slot), a = s_base + slot * kStage, b = a + kOperand;
-          if (a_mn) {
-            load_pair(lead, a, ma, am, kb * kBlockK, bar);
-            load_pair(lead, a + kOperand / 2, ma, am + 64, kb * kBlockK, bar);
-          } else {
-            load_pair(lead, a, ma, kb * kBlockK, am, bar);
-          }
-          if (b_mn) {
-            load_pair(lead, b, mb, bn, kb * kBlockK, bar);
-            load_pair(lead, b + kOperand / 2, mb, bn + 64, kb * kBlockK, bar);
-          } else {
-            load_pair(lead, b, mb, kb * kBlockK, bn, bar);
-          }
-          ++issued;
-          if (++slot == C::kStages) {
-            slot = 0;
-            ++laps;
-          }
-        }
-      };
-      using Yes = std::true_type;
-      using No = std::false_type;
-      for (int s = 0; ok && s < 2; ++s) {
-        const CUtensorMap *ma = &op.a[s], *mb = E == kSwiglu ? &op.b[rank] : &op.b[s];
-        // the tile's stages in this segment
-        int first;
-        const int all = stages_of(op, w, live, first), one = first_segment(op, live);
-        const int here = s == 0 ? 0 : one, size = s == 0 ? one : op.kb[1];
-        int from = first > here ? first - here : 0, n = (first + all - here < size ? first + all - here : size) - from;
-        n = __shfl_sync(0xffffffffu, n, 0);
-        from = __shfl_sync(0xffffffffu, from, 0);
-        if constexpr (E == kStore) {
-          const int layout = __shfl_sync(0xffffffffu, (op.a_mn ? 2 : 0) + (op.b_mn ? 1 : 0), 0);
-          if (layout == 0) segment(No{}, No{}, ma, mb, from, n);
-          else if (layout == 1) segment(No{}, Yes{}, ma, mb, from, n);
-          else segment(Yes{}, Yes{}, ma, mb, from, n);
-        } else {
-          segment(No{}, std::integral_constant<bool, E == kDSwiglu>{}, ma, mb, from, n);
-        }
-      }
-    }
-    // The copies in flight land before the CTAs end, whatever became of their readers (they are counted on the first CTA's
-    // barriers; the pair ends together).
-    const int left = issued > C::kStages ? issued - C::kStages : 0;
-    if (rank == 0)
-      for (int i = left; i < issued; ++i) warp_wait(full + i % C::kStages, (i / C::kStages) & 1, p.err, 81);
-    // So do the arrivals of the last products, which the first CTA's tensor core sends to both: a CTA that ended before them would
-    // be written to when its shared memory is another's.
-    for (int i = left; ok && i < issued; ++i) ok = warp_wait(empty + i % C::kStages, (i / C::kStages) & 1, p.err, 87);
-  } else if (warp == 1) {
-    if (rank == 0) {
+  if (warp < 4) {
+    if constexpr (sums_in_runs(E)) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+    if (warp == 0) {
+      // The whole warp runs this, one elected lane's instructions take effect: addresses and coordinates stay in uniform registers.
+      // (Issued from a branch of one lane, a stage's loads took longer than its products where a launch holds several problems:
+      // 1,215 instead of 1,540 TFLOP/s.)
       const uint32_t lead = elect();
-      int slot = 0, laps = 0, it = 0;
+      int slot = 0, laps = 0, issued = 0;
       bool ok = true;
-      for (int tile; ok && (tile = walk(it)) >= 0; ++it) {
-        const Where w = locate<E>(p, tile, live);
+      for (int i = 0, tile; ok && (tile = walk(i)) >= 0; ++i) {
+        Where w = locate<E>(p, tile, live);
+        w.op = __shfl_sync(0xffffffffu, w.op, 0);
         const Op& op = p.op[w.op];
-        const int buf = it & 1;
-        if (it >= 2 && !(ok = cluster_wait(acc_empty + buf, ((it >> 1) - 1) & 1, p.err, 82))) break;
-        tc_fence_after();
-        int from;
-        const int n = __shfl_sync(0xffffffffu, stages_of(op, w, live, from), 0);
-        const uint32_t d = tm + buf * kTileN;
-        // (the layouts are constants of each loop: descriptors and steps stay in uniform registers, which the instruction reads)
-        auto products = [&](auto a_mn, auto b_mn) {
-          constexpr uint32_t id = wattn::idesc<T>(256, 256, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
-          constexpr uint32_t a_hi = a_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16, b_hi = b_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16;
-          constexpr uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;  // 16 k further, in 16 bytes
-          for (int kb = 0; kb < n; ++kb) {
-            if (!(ok = cluster_wait(full + slot, laps & 1, p.err, 83))) break;
-            tc_fence_after();
-            const uint32_t a = ((s_base + slot * kStage) >> 4) | a_hi, b = ((s_base + slot * kStage + kOperand) >> 4) | b_hi;
-#pragma unroll
-            for (int k = 0; k < kBlockK / 16; ++k) mma_pair(lead, d, a + k * a_step, b + k * b_step, id, kb > 0 || k > 0);
-            commit_pair(lead, empty + slot);
+        const int am = __shfl_sync(0xffffffffu, w.m + (int)rank * kHalf, 0);
+        const int bn = __shfl_sync(0xffffffffu, E == kSwiglu ? w.n : w.n + (int)rank * kHalf, 0);
+        auto segment = [&](auto a_mn, auto b_mn, const CUtensorMap* ma, const CUtensorMap* mb, int from, int n) {
+          for (int kb = from; kb < from + n; ++kb) {
+            if (laps > 0 && !(ok = warp_wait(empty + slot, (laps - 1) & 1, p.err, 80))) return;
+            if (rank == 0 && lead) mbar_arrive_expect_tx(full + slot, 2 * kStage);
+            const uint32_t bar = in_first_cta(full + slot), a = s_base + slot * kStage, b = a + kOperand;
+            if (a_mn) {
+              load_pair(lead, a, ma, am, kb * kBlockK, bar);
+              load_pair(lead, a + kOperand / 2, ma, am + 64, kb * kBlockK, bar);
+            } else {
+              load_pair(lead, a, ma, kb * kBlockK, am, bar);
+            }
+            if (b_mn) {
+              load_pair(lead, b, mb, bn, kb * kBlockK, bar);
+              load_pair(lead, b + kOperand / 2, mb, bn + 64, kb * kBlockK, bar);
+            } else {
+              load_pair(lead, b, mb, kb * kBlockK, bn, bar);
+            }
+            ++issued;
             if (++slot == C::kStages) {
               slot = 0;
               ++laps;
@@ -511,25 +468,105 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         };
         using Yes = std::true_type;
         using No = std::false_type;
-        if constexpr (E == kStore) {
-          const int layout = __shfl_sync(0xffffffffu, (op.a_mn ? 2 : 0) + (op.b_mn ? 1 : 0), 0);
-          if (layout == 0) products(No{}, No{});
-          else if (layout == 1) products(No{}, Yes{});
-          else products(Yes{}, Yes{});
-        } else {
-          products(No{}, std::integral_constant<bool, E == kDSwiglu>{});
+        for (int s = 0; ok && s < 2; ++s) {
+          const CUtensorMap *ma = &op.a[s], *mb = E == kSwiglu ? &op.b[rank] : &op.b[s];
+          // the tile's stages in this segment
+          int first;
+          const int all = stages_of(op, w, live, first), one = first_segment(op, live);
+          const int here = s == 0 ? 0 : one, size = s == 0 ? one : op.kb[1];
+          int from = first > here ? first - here : 0, n = (first + all - here < size ? first + all - here : size) - from;
+          n = __shfl_sync(0xffffffffu, n, 0);
+          from = __shfl_sync(0xffffffffu, from, 0);
+          if constexpr (E == kStore) {
+            const int layout = __shfl_sync(0xffffffffu, (op.a_mn ? 2 : 0) + (op.b_mn ? 1 : 0), 0);
+            if (layout == 0) segment(No{}, No{}, ma, mb, from, n);
+            else if (layout == 1) segment(No{}, Yes{}, ma, mb, from, n);
+            else segment(Yes{}, Yes{}, ma, mb, from, n);
+          } else {
+            segment(No{}, std::integral_constant<bool, E == kDSwiglu>{}, ma, mb, from, n);
+          }
         }
-        if (ok) commit_pair(lead, acc_full + buf);
       }
-      commit_pair(lead, fin);  // (a pair whose waits gave up ends with no product in flight)
+      // The copies in flight land before the CTAs end, whatever became of their readers (they are counted on the first CTA's
+      // barriers; the pair ends together).
+      const int left = issued > C::kStages ? issued - C::kStages : 0;
+      if (rank == 0)
+        for (int i = left; i < issued; ++i) warp_wait(full + i % C::kStages, (i / C::kStages) & 1, p.err, 81);
+      // So do the arrivals of the last products, which the first CTA's tensor core sends to both: a CTA that ended before them
+      // would be written to when its shared memory is another's.
+      for (int i = left; ok && i < issued; ++i) ok = warp_wait(empty + i % C::kStages, (i / C::kStages) & 1, p.err, 87);
+    } else if (warp == 1) {
+      if (rank == 0) {
+        const uint32_t lead = elect();
+        int slot = 0, laps = 0, turn = 0;  // turn: of the accumulators
+        bool ok = true;
+        for (int it = 0, tile; ok && (tile = walk(it)) >= 0; ++it) {
+          const Where w = locate<E>(p, tile, live);
+          const Op& op = p.op[w.op];
+          int from;
+          const int n = __shfl_sync(0xffffffffu, stages_of(op, w, live, from), 0);
+          const int run = sums_in_runs(E) ? run_stages(n) : 0;
+          // (the layouts are constants of each loop: descriptors and steps stay in uniform registers, which the instruction reads)
+          auto products = [&](auto a_mn, auto b_mn) {
+            constexpr uint32_t id = wattn::idesc<T>(256, 256, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+            constexpr uint32_t a_hi = a_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16;
+            constexpr uint32_t b_hi = b_mn ? (kOperand / 2 >> 4) << 16 : 1u << 16;
+            constexpr uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;  // 16 k further, in 16 bytes
+            uint32_t d = 0;
+            auto begin = [&] {  // an accumulator whose last content is read
+              const int buf = turn & 1;
+              if (turn >= 2 && !(ok = cluster_wait(acc_empty + buf, ((turn >> 1) - 1) & 1, p.err, 82))) return;
+              tc_fence_after();
+              d = tm + buf * kTileN;
+            };
+            auto end = [&] { commit_pair(lead, acc_full + (turn++ & 1)); };
+            begin();
+            int at = 0;  // the stage in its run
+            for (int kb = 0; ok && kb < n; ++kb) {
+              if constexpr (sums_in_runs(E)) {
+                if (at == run) {
+                  end();
+                  begin();
+                  if (!ok) break;
+                  at = 0;
+                }
+              }
+              if (!(ok = cluster_wait(full + slot, laps & 1, p.err, 83))) break;
+              tc_fence_after();
+              const uint32_t a = ((s_base + slot * kStage) >> 4) | a_hi, b = ((s_base + slot * kStage + kOperand) >> 4) | b_hi;
+  #pragma unroll
+              for (int k = 0; k < kBlockK / 16; ++k) mma_pair(lead, d, a + k * a_step, b + k * b_step, id, at > 0 || k > 0);
+              commit_pair(lead, empty + slot);
+              ++at;
+              if (++slot == C::kStages) {
+                slot = 0;
+                ++laps;
+              }
+            }
+            if (ok) end();
+          };
+          using Yes = std::true_type;
+          using No = std::false_type;
+          if constexpr (E == kStore) {
+            const int layout = __shfl_sync(0xffffffffu, (op.a_mn ? 2 : 0) + (op.b_mn ? 1 : 0), 0);
+            if (layout == 0) products(No{}, No{});
+            else if (layout == 1) products(No{}, Yes{});
+            else products(Yes{}, Yes{});
+          } else {
+            products(No{}, std::integral_constant<bool, E == kDSwiglu>{});
+          }
+        }
+        commit_pair(lead, fin);  // (a pair whose waits gave up ends with no product in flight)
+      }
+      warp_wait(fin, 0, p.err, 84);  // (both: it arrives in both, also where the pair has no tile and nothing else to wait for)
     }
-    warp_wait(fin, 0, p.err, 84);  // (both: it arrives in both, also where the pair has no tile and nothing else to wait for)
-  } else if (warp >= 4) {
+  } else {
+    if constexpr (sums_in_runs(E)) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
     const int ew = warp - 4, quad = warp & 3, half = ew >> 2;  // a warp reads the TMEM lanes of its quarter
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t slab = smem_u32(slabs) + ew * C::kOut;
     bool ok = true;
-    int it = 0;
+    int it = 0, turn = 0;  // (of the accumulators)
     // kDSwiglu: the kept g and u of 32 columns, a step of four to a tile, into one of two sets of strips, a step ahead of its use
     int step = 0;
     auto fetch = [&](int at, const Where& w) {  // step `at` is step at & 3 of w's tile
@@ -561,18 +598,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     for (int tile; (tile = walk(it)) >= 0; ++it) {
       const Where w = locate<E>(p, tile, live);
       const Op& op = p.op[w.op];
-      const int buf = it & 1, m0 = w.m + (int)rank * kHalf + quad * 32, row = m0 + lane;
-      const uint32_t t0 = tm + lanes + buf * kTileN;
+      const int m0 = w.m + (int)rank * kHalf + quad * 32, row = m0 + lane;
       const int rows = op.m_live ? live : op.M;  // (kDLogit: zeros in the rows past them)
       auto has = [&](int n0) { return m0 < (E == kDLogit ? op.M : rows) && n0 < op.N; };
-      ok = ok && warp_wait(acc_full + buf, (it >> 1) & 1, p.err, 85) && !expires(p, 85);
-      tc_fence_after();
-      const float bad = ok ? 0.f : NAN;  // a wait that gave up leaves NaN
-      auto release = [&] {               // the accumulator is read
+      auto acquire = [&] {  // an accumulator is formed: its columns
+        ok = ok && warp_wait(acc_full + (turn & 1), (turn >> 1) & 1, p.err, 85) && !expires(p, 85);
+        tc_fence_after();
+        return tm + lanes + (turn & 1) * kTileN;
+      };
+      auto release = [&] {  // it is read
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_cluster(in_first_cta(acc_empty + buf));
+        if (lane == 0) arrive_cluster(in_first_cta(acc_empty + (turn & 1)));
+        ++turn;
       };
+      uint32_t t0 = 0;
+      float logit[2][sums_in_runs(E) ? 64 : 1];  // the row's 128 sums
+      if constexpr (sums_in_runs(E)) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) logit[0][i] = logit[1][i] = 0.f;
+        int from;
+        const int n = stages_of(op, w, live, from), run = run_stages(n);
+#pragma unroll 1
+        for (int k = 0; k < n; k += run) {
+          const uint32_t t = acquire() + half * 128;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float v[32];
+            tmem_ld32(t + c * 32, v);
+            if (c == 3) release();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) logit[c >> 1][(c & 1) * 32 + i] += v[i];
+          }
+        }
+      } else {
+        t0 = acquire();
+      }
+      const float bad = ok ? 0.f : NAN;  // a wait that gave up leaves NaN
 
       if constexpr (E == kStore) {
         const float f = (op.factor != nullptr ? __ldg(op.factor) : op.unscale ? 1.f / carried(p.bounds, p.more) : 1.f) + bad;
@@ -719,12 +781,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       } else if constexpr (E == kLse) {
         const int lab = row < rows ? __ldg(p.labels + row) : -1;
         float top = -INFINITY, sum = 0.f;
-#pragma unroll 1
+#pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const int c = half * 128 + s * 64, n0 = w.n + c;
-          float v[64];
-          wattn::tmem_ld64(t0 + c, v);
-          if (s == 1) release();
+          const int n0 = w.n + half * 128 + s * 64;
+          float(&v)[64] = logit[s];
           if (n0 >= op.N) continue;
           const bool here = lab >= n0 && lab < n0 + 64;
           if (__any_sync(0xffffffffu, here)) {
@@ -748,8 +808,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
           const float next = wattn::max3(top, high, high), ref = next == -INFINITY ? 0.f : next;
           float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 64; ++i) a[i & 3] += ex2((v[i] - ref) * p.log2e);  // (1 at the maximum)
-          sum = sum * ex2((top - ref) * p.log2e) + ((a[0] + a[1]) + (a[2] + a[3]));
+          for (int i = 0; i < 64; ++i) a[i & 3] += ex2((v[i] - ref) * kLog2e);  // (1 at the maximum)
+          sum = sum * ex2((top - ref) * kLog2e) + ((a[0] + a[1]) + (a[2] + a[3]));
           top = next;
         }
         if (row < rows && w.n + half * 128 < op.N)
@@ -759,15 +819,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const int at = kept ? __ldg(p.labels + row) - p.v0 : -1;
         const float2 lse = kept ? __ldg(p.lse + row) : make_float2(0.f, 0.f);
         const float f = kept ? __ldg(p.row_scale + row) + bad : 0.f;
-#pragma unroll 1
+#pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const int c = half * 128 + s * 64, n0 = w.n + c;
-          float v[64];
-          wattn::tmem_ld64(t0 + c, v);
-          if (s == 1) release();
+          const int n0 = w.n + half * 128 + s * 64;
+          float(&v)[64] = logit[s];
           if (!has(n0)) continue;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) v[i] = ex2(fmaf(v[i] - lse.x, p.log2e, -lse.y));
+          for (int i = 0; i < 64; ++i) v[i] = ex2(fmaf(v[i] - lse.x, kLog2e, -lse.y));
           if (__any_sync(0xffffffffu, at >= n0 && at < n0 + 64)) {
 #pragma unroll
             for (int i = 0; i < 64; ++i) v[i] -= at == n0 + i ? 1.f : 0.f;
@@ -881,6 +939,13 @@ int launch(Params& p, cudaStream_t stream) {
   static bool done[kMaxDevices];
   auto kern = gemm_kernel<T, E>;
   if (set_smem_once(kern, Cfg<E>::kSmem, done) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
+  if constexpr (sums_in_runs(E)) {  // the launch has the warps' shares (else the epilogue would wait for registers for good)
+    static const bool fits = [&] {
+      cudaFuncAttributes a;
+      return cudaFuncGetAttributes(&a, kern) == cudaSuccess && a.numRegs * kThreads >= 128 * kFewRegs + 32 * kEpiWarps * kManyRegs;
+    }();
+    if (!fits) return (cudaGetLastError(), GD_ERR_LAUNCH);
+  }
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return (cudaGetLastError(), GD_ERR_LAUNCH);

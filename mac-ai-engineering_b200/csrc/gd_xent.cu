@@ -21,14 +21,6 @@ constexpr int kPart = 128;          // columns of one (maximum, sum)
 constexpr int kRows = 8;            // rows of a join CTA
 constexpr int kJoinThreads = 256, kJoinGroups = kJoinThreads / kRows;
 constexpr float kLn2 = 0.6931471805599453f;
-// The tensor core's adder cuts off what lies below its accumulator: a logit of D terms comes out 0.27 (bfloat16; float16 0.30) times
-// 2^-24 D / 16 of itself too near to zero (measured on largest logits and by the losses' errors, D from 256 to 8,192, four kinds of
-// inputs; terms that all have one sign lose more). The exponents and the difference to the label's logit are stretched by that much:
-// at D = 2,048 losses are 3.5e-7 off instead of 1.1e-6 (a float32 product's: 3e-7). Maxima and differences of 0 stay as they are.
-template <typename T>
-float stretch(int D) {
-  return (float)(1.0 + (std::is_same<T, __half>::value ? 0.30 : 0.27) * ((D + 15) / 16) / 16777216.0);
-}
 enum Reduction { kNone, kMean, kSum };
 
 struct Labels {
@@ -155,7 +147,7 @@ __global__ void __launch_bounds__(256) spread_kernel(const uint16_t* __restrict_
 // mean or sum the last CTA adds the CTAs' sums in their order. Parts and targets lie by live rows, losses by rows. A thread takes
 // every 32nd part of a row. (777 rows of 393 parts: 6 us, with 32 rows a CTA 8 us; 7,370 of 1,000: 20 us, 26 us)
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* __restrict__ part, const float* __restrict__ target,
-                                                            int parts, int n, Plan plan, int reduction, float stretched,
+                                                            int parts, int n, Plan plan, int reduction,
                                                             float2* __restrict__ lse, float* __restrict__ loss, float* sums,
                                                             unsigned int* counter) {
   __shared__ float2 sh[kJoinGroups][kRows];
@@ -163,11 +155,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* __rest
   __shared__ bool last;
   const int group = threadIdx.x / kRows, at = threadIdx.x % kRows, i = blockIdx.x * kRows + at;
   const int row = i < n ? __ldg(plan.place + i) : -1;
-  const float log2e = gemm::kLog2e * stretched;
   float m = -INFINITY, s = 0.f;
   auto add = [&](float2 v) {  // (a NaN sum stays)
     const float next = wattn::max3(m, v.x, v.x), ref = next == -INFINITY ? 0.f : next;
-    s = s * wattn::ex2((m - ref) * log2e) + v.y * wattn::ex2((v.x - ref) * log2e);
+    s = s * wattn::ex2((m - ref) * gemm::kLog2e) + v.y * wattn::ex2((v.x - ref) * gemm::kLog2e);
     m = next;
   };
   if (row >= 0) {
@@ -190,7 +181,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float2* __rest
       for (int g = 0; g < kJoinGroups; ++g) add(sh[g][at]);
       if (row >= 0) {
         const float rest = log2f(s);
-        x = __ldg(plan.label + row) < 0 ? NAN : fmaf(m - target[row], stretched, kLn2 * rest);
+        x = __ldg(plan.label + row) < 0 ? NAN : fmaf(kLn2, rest, m - target[row]);
         if (lse != nullptr) lse[row] = make_float2(m, rest);
       }
       if (reduction == kNone && i < n) loss[i] = x;
@@ -340,12 +331,11 @@ int forward(const Problem& q, const Labels& lab, float* loss, float2* lse, char*
   shape(o, q.n, q.V);
   o.m_live = true;
   o.kb[0] = gemm::blocks_of(q.D, gemm::kBlockK);
-  p.log2e = gemm::kLog2e * stretch<T>(q.D);
   if (!gemm::operand_map(&o.a[0], ws + f.rows, dt, packed_rows(q.n), q.D, pitch(q.D), false) ||
       !gemm::operand_map(&o.b[0], q.w, dt, q.V, q.D, q.ldw, false))
     return GD_ERR_LAUNCH;
   if (const int st = gemm::launch<T, gemm::kLse>(p, stream)) return st;
-  join_kernel<<<f.ctas, kJoinThreads, 0, stream>>>(p.part, p.target, f.parts, q.n, q.plan, q.reduction, stretch<T>(q.D), lse, loss,
+  join_kernel<<<f.ctas, kJoinThreads, 0, stream>>>(p.part, p.target, f.parts, q.n, q.plan, q.reduction, lse, loss,
                                                      reinterpret_cast<float*>(ws + f.sums),
                                                      reinterpret_cast<unsigned int*>(ws + 64));
   return cudaPeekAtLastError() == cudaSuccess ? GD_OK : (cudaGetLastError(), GD_ERR_LAUNCH);
@@ -371,7 +361,7 @@ int backward(const Problem& q, const float2* lse, const float* dloss, void* dx, 
     const char* w = static_cast<const char*>(q.w) + v0 * q.ldw * 2;
     Params p = {};
     p.ops = 1, p.err = reinterpret_cast<ErrorWord*>(ws), p.live = q.plan.live, p.labels = q.plan.label;
-    p.v0 = (int)v0, p.lse = lse, p.row_scale = row_scale, p.log2e = gemm::kLog2e * stretch<T>(q.D);
+    p.v0 = (int)v0, p.lse = lse, p.row_scale = row_scale;
     Op& o = p.op[0];
     shape(o, q.n, cols);
     o.m_live = true;
