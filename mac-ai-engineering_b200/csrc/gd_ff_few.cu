@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const __grid_constant__ F
 }
 
 // CTAs of a cluster: as many as still run all at once, three on each of 148 SMs (memory then works at its rate whatever the
-// SMs' shares are), none with less than four stages. At 4 tokens, 2,048 x 6,144 that is four (20 us; a fifth, and with it a
+// SMs' shares are), but eight at most (the second product of a block 2,048 wide has 16 tiles, and so 128 CTAs of the 444 that
+// fit; 4,096 wide 256), and none with less than four stages. At 4 tokens, 2,048 x 6,144 that is four (20 us; a fifth, and with it a
 // second turn of CTAs: 23 us; one CTA an SM: 23 us), at 64 tokens, 4,096 x 12,288 two (60 us; one: 66, four: 69 us); at
 // 1 token, 1,024 x 2,816 the least length holds (9.6 us; two stages: 11 us).
 int split_of(int tiles, int blocks) {

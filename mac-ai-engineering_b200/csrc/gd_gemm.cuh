@@ -13,10 +13,12 @@
 //
 // Bound by the tensor pipe (97 % busy under four gradients at once) at the clock that the power limit leaves (1.45 to 1.6 GHz).
 // bf16, 16,384 rows, 2,048 x 6,144: the second product 268 us (1,540 TFLOP/s; cuBLAS 264), gate and up 524 us (1,575), the four
-// gradients 1,385 us (1,490). With g and u kept gate and up take 578 us, and dh 413 us (1,000): their epilogues' 0.8 and 1.2 GB cross
-// between the SMs and L2 beside the operands' (dh without its loads 350 us, without its stores 333, without both 281; neither TMA nor
-// the warps' own accesses, 8 or 16 epilogue warps, 4 or 5 stages changed that by more than 3 %). Cross entropy, 7,370 rows, 2,048 x
-// 128,000: logits 2.44 to 2.85 ms (1,360 to 1,580), with their gradients stored 2.53 to 2.97 ms, its two gradients 5.4 to 6.1 ms.
+// gradients 1,385 us (1,490). With g and u kept gate and up take 578 us, and dh 413 us (1,000): their epilogues' 0.8 and 1.2 GB
+// cross between the SMs and L2 beside the operands' (dh without its loads 350 us, without its stores 333, without both 281;
+// neither TMA nor the warps' own accesses, 8 or 16 epilogue warps, 4 or 5 stages changed that by more than 3 %). Cross entropy,
+// 7,370 rows, 2,048 x 128,000: logits 2.87 to 3.15 ms (1,230 to 1,350), with their gradients stored 2.96 to 3.28 ms, its two
+// gradients 5.9 to 6.65 ms, all at the clocks of a long run (1.3 to 1.45 GHz). 777 rows, 50,257 words: the logits 128 us at 1.54
+// GHz, 93 % of the tensor pipe.
 #pragma once
 
 #include <utility>
@@ -58,14 +60,15 @@ enum Epilogue {
 };
 
 // The tensor core's adder cuts off what lies below its accumulator, always towards zero: a sum of D products in one go loses about
-// a quarter of D / 16 x 2^-24 to 2^-23 of itself (2e-6 at 2,048 terms; twice that and more where all terms have one sign). Logits are
-// therefore summed in runs of at most 768 terms (two runs at least, from two stages on), a run an accumulator, and the runs added
-// in float32 registers by the epilogue's threads, which hold their 128 columns: what is lost does not grow with D. Losses of 777
-// rows, 5,000 words, bf16, are off by 3.4e-7 of their norm at D = 2,048 (a float32 product's: 3.4e-7), 3.5e-7 at 8,192 (7.5e-7); with
-// one sign 3.5e-7 (3.2e-6) and 7.3e-7 (1.4e-5). Reading an accumulator takes about 2,000 clocks beside the products, which two
-// accumulators hide where a run is long enough: 777 rows, 2,048 wide, 50,257 words take 149.6 us, in one go 147.9, in runs of 512
-// terms 156 (2.5e-7), of 256 terms 185 (1.2e-7). 1,500 rows of 768 (two runs of six stages): the logits' kernels 5 to 8 % more.
-// 128 sums a thread want more registers than twelve warps share evenly: the first four warps give some away.
+// a quarter of D / 16 x 2^-24 of itself (2e-6 at 2,048 terms; twice that and more where all terms have one sign). Logits
+// are therefore summed in runs of at most 768 terms (two runs at least, from two stages on), a run an accumulator, and the runs
+// added in float32 registers by the epilogue's threads, which hold their 128 columns: what is lost does not grow with D. Losses of
+// 777 rows, 5,000 words, bf16, are off by 3.4e-7 of their norm at D = 2,048 (a float32 product's: 3.4e-7), 3.5e-7 at 8,192
+// (7.5e-7); with one sign 3.5e-7 (3.2e-6) and 7.3e-7 (1.4e-5). Reading an accumulator takes about 2,000 clocks beside the
+// products, which two accumulators hide where a run is long enough: 777 rows, 2,048 wide, 50,257 words take 149.6 us, in one go
+// 147.9, in runs of 512 terms 156 (2.5e-7), of 256 terms 185 (1.2e-7). 750 rows of 768 terms (two runs of six stages), 32,003
+// words, float16: the logits 38 us instead of 32.5, with their gradients stored 40 instead of 35. 128 sums a thread want more
+// registers than twelve warps share evenly: the first four warps give some away.
 constexpr bool sums_in_runs(int E) { return E == kLse || E == kDLogit; }
 constexpr int kFewRegs = 80, kManyRegs = 208;
 __host__ __device__ inline int run_stages(int stages) {  // of every run but the last

@@ -110,7 +110,8 @@ def _refuse(name, x, w_gate, w_up, w_down):
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
     """y [..., O] for x [..., D], w_gate and w_up [F, D] (as nn.Linear keeps them; halves of one [2 F, D] weight are read in
     place) and w_down [O, F], all bfloat16 or all float16, D, F and O multiples of 8. Gradients of all four come in their
-    type, the same bits every run; those of frozen inputs are not formed. Views with adjacent columns and 16-byte aligned
+    type, the same bits every run; those of frozen inputs are not formed. Up to 128 rows a call that records no gradient takes
+    another kernel than one that does, and its last bits may differ. Views with adjacent columns and 16-byte aligned
     rows are read in place, others are copied."""
     name = "gated_feed_forward"
     try:

@@ -3,10 +3,11 @@ libgated_delta_b200.so):
 
     loss_i = logsumexp_v(x_i . w_v) - x_i . w_label(i)
 
-tcgen05 products of 16-bit operands with float32 sums, in runs of at most 768 terms that are added outside the tensor core (whose
-adder cuts off instead of rounding: long sums would be shifted towards zero). The logits stay on the chip as float32: the forward
-keeps a maximum and a sum of exponentials for every 128 of them, the backward forms them again, a piece of the vocabulary at a time, and rounds their gradient to the inputs' 16-bit type
-(the matrix instruction's operand). bfloat16 and float16. There is no CPU path: CUDA tensors only.
+tcgen05 products of 16-bit operands with float32 sums, in runs of at most 768 terms that are added outside the tensor core
+(whose adder cuts off instead of rounding: long sums would be shifted towards zero). The logits stay on the chip as float32:
+the forward keeps a maximum and a sum of exponentials for every 128 of them, the backward forms them again, a piece of the
+vocabulary at a time, and rounds their gradient to the inputs' 16-bit type (the matrix instruction's operand). bfloat16 and
+float16. There is no CPU path: CUDA tensors only.
 """
 from __future__ import annotations
 
