@@ -17,7 +17,11 @@ def _layer(dt, value_heads):
                               num_attention_heads=2, num_key_value_heads=1, head_dim=64, linear_key_head_dim=64,
                               linear_value_head_dim=64, linear_num_key_heads=2, linear_num_value_heads=value_heads)
     torch.manual_seed(0)
-    layer = M.Qwen3_5GatedDeltaNet(cfg, 0).to("cuda", dt).eval()
+    layer = M.Qwen3_5GatedDeltaNet(cfg, 0)
+    # transformers' own forms, also where another library's kernels were found
+    layer.chunk_gated_delta_rule, layer.recurrent_gated_delta_rule = M.torch_chunk_gated_delta_rule, M.torch_recurrent_gated_delta_rule
+    layer.norm = M.Qwen3_5RMSNormGated(64, eps=cfg.rms_norm_eps)
+    layer = layer.to("cuda", dt).eval()
     return layer, M.DynamicCache(config=cfg)
 
 
