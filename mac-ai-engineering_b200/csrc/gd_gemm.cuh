@@ -943,11 +943,11 @@ int launch(Params& p, cudaStream_t stream) {
   auto kern = gemm_kernel<T, E>;
   if (set_smem_once(kern, Cfg<E>::kSmem, done) != cudaSuccess) return (cudaGetLastError(), GD_ERR_LAUNCH);
   if constexpr (sums_in_runs(E)) {  // the launch has the warps' shares (else the epilogue would wait for registers for good)
-    static const bool fits = [&] {
-      cudaFuncAttributes a;
-      return cudaFuncGetAttributes(&a, kern) == cudaSuccess && a.numRegs * kThreads >= 128 * kFewRegs + 32 * kEpiWarps * kManyRegs;
-    }();
-    if (!fits) return (cudaGetLastError(), GD_ERR_LAUNCH);
+    static bool fits = false;
+    cudaFuncAttributes at;
+    if (!fits && (cudaFuncGetAttributes(&at, kern) != cudaSuccess ||
+                  !(fits = at.numRegs * kThreads >= 128 * kFewRegs + 32 * kEpiWarps * kManyRegs)))
+      return (cudaGetLastError(), GD_ERR_LAUNCH);
   }
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
